@@ -235,6 +235,7 @@ kvd_decode_desc paged_as_dense(const kvd_paged_desc& p, PagedView* pv) {
     pv->kv_sblk = p.kv_stride_block;
     pv->kv_st = p.kv_stride_t;
     pv->sc_sblk = p.sc_stride_block;
+    pv->per_head = false;
     return d;
 }
 
@@ -281,6 +282,37 @@ extern "C" cudaError_t kvd_paged_decode_launch(const kvd_paged_desc* desc, const
         return launch_gqa_tc(d, Q, K_pool, V_pool, k_scale_pool, v_scale_pool, out, workspace, workspace_bytes,
                              stream, &tl_launches, &pv);
     if (desc->flags & KVD_FLAG_QK_INT8) return cudaErrorNotSupported;
+    return launch_generic(d, Q, K_pool, V_pool, k_scale_pool, v_scale_pool, out, workspace, workspace_bytes, stream,
+                          &tl_launches, &pv);
+}
+
+extern "C" size_t kvd_sparse_workspace_size(const kvd_paged_desc* desc) {
+    if (check_paged(desc) != cudaSuccess) return 0;
+    PagedView pv;
+    const kvd_decode_desc d = paged_as_dense(*desc, &pv);
+    const size_t gen = generic_workspace_size(d);
+    const size_t gqa = paged_tc_shape(*desc, d) ? gqa_workspace_size(d, true) : 0;
+    return gen > gqa ? gen : gqa;
+}
+
+extern "C" cudaError_t kvd_sparse_decode_launch(const kvd_paged_desc* desc, const void* Q, const int8_t* K_pool,
+                                                const int8_t* V_pool, const float* k_scale_pool,
+                                                const float* v_scale_pool, void* out, void* workspace,
+                                                size_t workspace_bytes, cudaStream_t stream) {
+    tl_launches = 0;
+    const cudaError_t e = check_paged(desc);
+    if (e != cudaSuccess) return e;
+    if (!Q || !K_pool || !V_pool || !k_scale_pool || !v_scale_pool || !out) return cudaErrorInvalidValue;
+    if (desc->flags & KVD_FLAG_QK_INT8) return cudaErrorNotSupported;
+    if ((desc->flags & KVD_FLAG_PARTIAL_OUT) && desc->num_q_heads > 1 && desc->o_stride_h < desc->head_dim + 4)
+        return cudaErrorInvalidValue;
+    if (!workspace) workspace_bytes = 0;
+    PagedView pv;
+    const kvd_decode_desc d = paged_as_dense(*desc, &pv);
+    pv.per_head = true;
+    if (paged_tc_ok(*desc, d, Q, K_pool, V_pool, k_scale_pool, v_scale_pool))
+        return launch_gqa_tc(d, Q, K_pool, V_pool, k_scale_pool, v_scale_pool, out, workspace, workspace_bytes,
+                             stream, &tl_launches, &pv);
     return launch_generic(d, Q, K_pool, V_pool, k_scale_pool, v_scale_pool, out, workspace, workspace_bytes, stream,
                           &tl_launches, &pv);
 }

@@ -1,0 +1,962 @@
+// kvd_blocks.cu -- the paged serving step around the attention kernels: block
+// tables and slot maps from request lengths, quantised writes and reads by
+// slot, and the selection of blocks that a decode attends to.
+//
+// No reference counterpart (the reference's caches are dense and complete,
+// kv_cache/new_kvint8.cu:83-84). This file must not be built with fast-math:
+// the quantiser's divisions are IEEE.
+#include <cooperative_groups.h>
+
+#include "kvd_common.cuh"
+#include "kvd_decode.cuh"
+#include "kvd_quant.cuh"
+
+namespace kvd {
+namespace {
+
+namespace cg = cooperative_groups;
+
+template <class... A, class... B>
+cudaError_t launch_after(void (*kern)(A...), unsigned grid, unsigned block, size_t smem, unsigned cluster,
+                         cudaStream_t st, B... args) {
+    // Programmatic dependent of the kernel before it; every kernel here waits
+    // (griddepcontrol.wait) before its first global access.
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(grid, 1, 1);
+    cfg.blockDim = dim3(block, 1, 1);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = st;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = cluster;
+    attr[1].val.clusterDim.y = 1;
+    attr[1].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = cluster > 1 ? 2 : 1;
+    return cudaLaunchKernelEx(&cfg, kern, args...);
+}
+
+// ----------------------------------------------------------------------- plan
+// Prefix sums over the requests (new tokens, blocks needed, blocks given back)
+// place every slot, table entry and free-list entry independently, so after
+// the sums all writes run in parallel. Every CTA makes the sums itself
+// (24 bytes a request from L2) and writes its share; the CTA that ends last
+// writes the lengths and the count, which may alias the inputs.
+constexpr int kPlanMaxBatch = 8192;
+
+struct PlanParams {
+    kvd_paged_plan_desc d;
+    const int32_t* seq_lens;
+    const int32_t* new_lens;
+    int32_t* table;
+    int32_t* free_blocks;
+    const int32_t* free_count;
+    int64_t* slots;
+    int32_t* starts;
+    int32_t* lens_out;
+    int32_t* count_out;
+    unsigned int* ticket;
+};
+
+// Sums saturate at 2^31 - 1: lengths no pool can hold are refused, not wrapped.
+__device__ __forceinline__ uint32_t sat_add(uint32_t a, uint32_t b) { return min(a + b, 0x7fffffffu); }
+
+// Inclusive prefix sum of one value per thread over the block, plus `carry`.
+__device__ __forceinline__ uint32_t block_scan(uint32_t x, uint32_t carry, uint32_t* warp_sums) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, nw = blockDim.x >> 5;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const uint32_t y = __shfl_up_sync(0xffffffffu, x, o);
+        if (lane >= o) x = sat_add(x, y);
+    }
+    __syncthreads();  // the sums of the scan before are no longer read
+    if (lane == 31) warp_sums[warp] = x;
+    __syncthreads();
+    uint32_t s = lane < nw ? warp_sums[lane] : 0u;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const uint32_t y = __shfl_up_sync(0xffffffffu, s, o);
+        if (lane >= o) s = sat_add(s, y);
+    }
+    const uint32_t before = __shfl_sync(0xffffffffu, s, (warp - 1) & 31);
+    return sat_add(x, warp > 0 ? sat_add(carry, before) : carry);
+}
+
+// First index in [0, n) whose inclusive sum is above v (n when there is none).
+__device__ __forceinline__ int first_above(const uint32_t* sums, int n, uint32_t v) {
+    int lo = 0, hi = n;
+    while (lo < hi) {
+        const int mid = (lo + hi) >> 1;
+        if (sums[mid] > v) hi = mid;
+        else lo = mid + 1;
+    }
+    return lo;
+}
+
+__global__ void __launch_bounds__(1024) plan_kernel(const PlanParams p) {
+    extern __shared__ uint32_t plan_smem[];
+    __shared__ uint32_t warp_sums[32];
+    __shared__ uint32_t s_popped;
+    __shared__ int s_last;
+    grid_dependency_wait();
+    allow_dependents();
+    const int B = p.d.batch, bs = p.d.block_size, MB = p.d.max_blocks_per_seq, NB = p.d.num_blocks;
+    const int64_t cap = static_cast<int64_t>(MB) * bs;
+    uint32_t* tok = plan_smem;   // [B] tokens up to and with request b
+    uint32_t* need = tok + B;    // [B] blocks needed up to and with request b
+    uint32_t* back = need + B;   // [B] blocks given back up to and with request b
+    uint8_t* okay = reinterpret_cast<uint8_t*>(back + B);  // [B] served
+    const bool writer = blockIdx.x == 0;
+    auto length = [&](int b) { return static_cast<int>(min(static_cast<int64_t>(max(0, p.seq_lens[b])), cap)); };
+    auto blocks_of = [&](int64_t tokens) { return static_cast<int>((tokens + bs - 1) / bs); };
+    uint32_t carry_t = 0, carry_n = 0, carry_b = 0;
+    if (threadIdx.x == 0) s_popped = 0;
+    int status = 0;
+    for (int b0 = 0; b0 < B; b0 += blockDim.x) {
+        const int b = b0 + threadIdx.x;
+        const bool in = b < B;
+        const int n = in ? p.new_lens[b] : 0;
+        const int len = in ? length(b) : 0;
+        const uint32_t stop = block_scan(n > 0 ? n : 0, carry_t, warp_sums);
+        const bool over = n > 0 && (len + static_cast<int64_t>(n) > cap || stop > static_cast<uint32_t>(p.d.num_slots));
+        const int held = blocks_of(len);
+        const uint32_t nd = n > 0 && !over ? blocks_of(len + static_cast<int64_t>(n)) - held : 0;
+        const uint32_t nstop = block_scan(nd, carry_n, warp_sums);
+        const uint32_t bstop = block_scan(n < 0 ? held : 0, carry_b, warp_sums);
+        if (in) {
+            tok[b] = stop;
+            need[b] = nstop;
+            back[b] = bstop;
+            okay[b] = over ? 0 : nd > 0 ? 2 : 1;  // 2: served if the blocks suffice
+            if (over) status |= KVD_STATUS_CACHE_FULL;
+        }
+        __syncthreads();
+        const int last = min(B, b0 + static_cast<int>(blockDim.x)) - 1;
+        carry_t = tok[last];
+        carry_n = need[last];
+        carry_b = back[last];
+    }
+    const uint32_t fc = static_cast<uint32_t>(min(max(0, *p.free_count), NB));
+    const uint32_t total = sat_add(fc, carry_b);  // stack height with the ended requests' blocks on top
+    for (int b = threadIdx.x; b < B; b += blockDim.x) {
+        if (okay[b] != 2) continue;
+        if (need[b] <= total) {
+            atomicMax(&s_popped, need[b]);
+        } else {
+            okay[b] = 0;
+            status |= KVD_STATUS_NO_BLOCKS;
+        }
+    }
+    __syncthreads();
+    const uint32_t popped = s_popped, left = total - popped;
+    // Entry i of the stack.
+    auto stack = [&](uint32_t i) -> int {
+        if (i < fc) return p.free_blocks[i];
+        const int b = first_above(back, B, i - fc);
+        const uint32_t before = b > 0 ? back[b - 1] : 0u;
+        return p.table[b * p.d.block_table_stride + (i - fc - before)];
+    };
+    const uint32_t stride = gridDim.x * blockDim.x, me = blockIdx.x * blockDim.x + threadIdx.x;
+    // table entries of the new blocks
+    for (uint32_t k = me; k < popped; k += stride) {
+        const int b = first_above(need, B, k);
+        const uint32_t before = b > 0 ? need[b - 1] : 0u;
+        p.table[b * p.d.block_table_stride + blocks_of(length(b)) + (k - before)] = stack(total - 1 - k);
+    }
+    // ended requests' blocks that stay on the stack
+    for (uint32_t i = fc + me; i < left; i += stride) {
+        if (i < static_cast<uint32_t>(NB)) p.free_blocks[i] = stack(i);
+        else status |= KVD_STATUS_BAD_BLOCK;  // more blocks than the pool has: some were given back twice
+    }
+    // slots
+    const uint32_t tokens = min(tok[B - 1], static_cast<uint32_t>(p.d.num_slots));
+    for (uint32_t t = me; t < static_cast<uint32_t>(p.d.num_slots); t += stride) {
+        int64_t slot = -1;
+        if (t < tokens) {
+            const int b = first_above(tok, B, t);
+            if (okay[b]) {
+                const int len = length(b), held = blocks_of(len);
+                const uint32_t pos = len + (t - (b > 0 ? tok[b - 1] : 0u));
+                const int j = static_cast<int>(pos) / bs;
+                const int id = j < held ? p.table[b * p.d.block_table_stride + j]
+                                        : stack(total - 1 - ((b > 0 ? need[b - 1] : 0u) + (j - held)));
+                if (id >= 0 && id < NB) slot = static_cast<int64_t>(id) * bs + (pos - static_cast<uint32_t>(j) * bs);
+                else status |= KVD_STATUS_BAD_BLOCK;
+            }
+        }
+        p.slots[t] = slot;
+    }
+    if (writer)
+        for (int b = threadIdx.x; b <= B; b += blockDim.x)
+            p.starts[b] = b > 0 ? min(tok[b - 1], static_cast<uint32_t>(p.d.num_slots)) : 0;
+    if (status && writer) record_status(status);
+    else if (status & KVD_STATUS_BAD_BLOCK) record_status(KVD_STATUS_BAD_BLOCK);
+    // lengths and count: after every CTA has read them
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        __threadfence();
+        s_last = gridDim.x == 1 || atomicInc(p.ticket, gridDim.x - 1) == gridDim.x - 1;
+    }
+    __syncthreads();
+    if (!s_last) return;
+    __threadfence();
+    for (int b = threadIdx.x; b < B; b += blockDim.x) {
+        const int n = p.new_lens[b], len = length(b);
+        p.lens_out[b] = n < 0 ? 0 : okay[b] ? len + n : len;
+    }
+    if (threadIdx.x == 0) *p.count_out = static_cast<int32_t>(min(left, static_cast<uint32_t>(NB)));
+}
+
+// ------------------------------------------------------------- rows by slot
+template <class T>
+__device__ __forceinline__ float widen(T x);
+template <>
+__device__ __forceinline__ float widen(float x) { return x; }
+template <>
+__device__ __forceinline__ float widen(__nv_bfloat16 x) { return __bfloat162float(x); }
+template <>
+__device__ __forceinline__ float widen(__half x) { return __half2float(x); }
+template <class T>
+__device__ __forceinline__ T narrow(float x);
+template <>
+__device__ __forceinline__ float narrow(float x) { return x; }
+template <>
+__device__ __forceinline__ __nv_bfloat16 narrow(float x) { return __float2bfloat16_rn(x); }
+template <>
+__device__ __forceinline__ __half narrow(float x) { return __float2half_rn(x); }
+
+struct RowsParams {
+    kvd_paged_rows_desc d;
+    const void* k_rows;
+    const void* v_rows;
+    void* k_out;
+    void* v_out;
+    const int64_t* slots;
+    int8_t* K;
+    int8_t* V;
+    float* ks;
+    float* vs;
+    int8_t* bounds;      // or nullptr
+    float* bound_scale;
+    int tile;            // tokens whose runs one CTA writes
+};
+
+// A lane's share of a row of D values: E = D / 32 neighbours (VEC: one load of
+// E elements), or, for other D, every 32nd value (E = 16 covers D <= 512).
+template <int E, bool VEC>
+struct Lane {
+    static __device__ __forceinline__ int at(int lane, int j) { return VEC ? lane * E + j : lane + 32 * j; }
+    static __device__ __forceinline__ bool in(int lane, int j, int D) { return VEC || lane + 32 * j < D; }
+    template <class T>
+    static __device__ __forceinline__ void load(const T* row, int lane, int D, float (&x)[E]) {
+        if constexpr (VEC) {
+            struct alignas(sizeof(T) * E < 16 ? sizeof(T) * E : 16) Pack { T v[E]; };
+            const Pack q = *reinterpret_cast<const Pack*>(row + lane * E);
+#pragma unroll
+            for (int j = 0; j < E; ++j) x[j] = widen<T>(q.v[j]);
+        } else {
+#pragma unroll
+            for (int j = 0; j < E; ++j) x[j] = in(lane, j, D) ? widen<T>(row[at(lane, j)]) : 0.f;
+        }
+    }
+    static __device__ __forceinline__ void load_codes(const int8_t* row, int lane, int D, float (&x)[E]) {
+        if constexpr (VEC) {
+            struct alignas(E < 16 ? E : 16) Pack { int8_t v[E]; };
+            const Pack q = *reinterpret_cast<const Pack*>(row + lane * E);
+#pragma unroll
+            for (int j = 0; j < E; ++j) x[j] = static_cast<float>(q.v[j]);
+        } else {
+#pragma unroll
+            for (int j = 0; j < E; ++j) x[j] = in(lane, j, D) ? static_cast<float>(row[at(lane, j)]) : 0.f;
+        }
+    }
+    template <class T>
+    static __device__ __forceinline__ void store(T* row, int lane, int D, const T (&x)[E]) {
+        if constexpr (VEC) {
+            struct alignas(sizeof(T) * E < 16 ? sizeof(T) * E : 16) Pack { T v[E]; };
+            Pack q;
+#pragma unroll
+            for (int j = 0; j < E; ++j) q.v[j] = x[j];
+            *reinterpret_cast<Pack*>(row + lane * E) = q;
+        } else {
+#pragma unroll
+            for (int j = 0; j < E; ++j)
+                if (in(lane, j, D)) row[at(lane, j)] = x[j];
+        }
+    }
+};
+
+__device__ __forceinline__ float warp_amax(float a) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) a = fmaxf(a, __shfl_xor_sync(0xffffffffu, a, o));
+    return a;
+}
+
+// Quantises a row held across a warp with the rule of kvd_quant.cuh; codes as
+// floats in x. Returns the scale.
+template <int E>
+__device__ __forceinline__ float quantise_lanes(float (&x)[E]) {
+    float a = 0.f;
+#pragma unroll
+    for (int j = 0; j < E; ++j) a = fmaxf(a, fabsf(x[j]));
+    a = warp_amax(a);
+    const float s = a == 0.f ? 0.f : a / 127.0f;
+#pragma unroll
+    for (int j = 0; j < E; ++j) x[j] = a == 0.f ? 0.f : fminf(fmaxf(rintf(x[j] / s), -127.0f), 127.0f);
+    return s;
+}
+
+constexpr int kRowWarps = 4;
+
+// Writes: a run is a maximal stretch of tokens in one block, skipped tokens
+// (slot -1) aside. One CTA per (tile of tokens, KV head) takes the runs that start in its tile, one
+// after the other, its warps the rows of a run in turn. A run's key bounds
+// are then the maximum and minimum over values that the CTA holds in
+// registers (and the block's earlier tokens, read from the pool), so the
+// bounds cost no second pass and no exchange between CTAs. Bound: HBM.
+template <class T, int E, bool VEC>
+__global__ void __launch_bounds__(32 * kRowWarps) write_kernel(const RowsParams p) {
+    using L = Lane<E, VEC>;
+    extern __shared__ float write_smem[];  // [kRowWarps][2][D] bounds of each warp
+    __shared__ int s_end, s_before;
+    __shared__ int s_odd[kRowWarps];
+    grid_dependency_wait();
+    allow_dependents();
+    const kvd_paged_rows_desc& d = p.d;
+    const int D = d.head_dim, bs = d.block_size, nt = d.num_tokens;
+    const int tiles = (nt + p.tile - 1) / p.tile;
+    const int h = blockIdx.x / tiles;
+    const int t0 = (blockIdx.x - h * tiles) * p.tile, t1 = min(nt, t0 + p.tile);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int64_t n_slots = static_cast<int64_t>(d.num_blocks) * bs;
+    auto block_at = [&](int t) -> int {  // block of token t, -1 for none
+        const int64_t s = p.slots[t];
+        return s >= 0 && s < n_slots ? static_cast<int>(s / bs) : -1;
+    };
+    auto odd_slot = [&](int t) {  // a skipped slot that is not -1
+        if (h == 0 && p.slots[t] != -1) record_status(KVD_STATUS_BAD_BLOCK);
+    };
+    bool fresh = false;  // the next token with a slot is known to start a run
+    int t = t0;
+    while (t < t1) {
+        const int blk = block_at(t);
+        if (blk < 0) {
+            if (threadIdx.x == 0) odd_slot(t);
+            ++t;
+            continue;
+        }
+        // end of the run: the first later token of another block
+        if (threadIdx.x == 0) { s_end = nt; s_before = -1; }
+        __syncthreads();
+        for (int u = t + 1;; u += blockDim.x) {
+            const int v = u + static_cast<int>(threadIdx.x);
+            const int at = v < nt ? block_at(v) : -2;
+            const bool other = at != blk && at != -1;
+            if (other) atomicMin(&s_end, v);
+            if (__syncthreads_or(other)) break;
+        }
+        const int end = min(s_end, nt);
+        if (!fresh) {  // the token with a slot before t: a run that started in an earlier tile is its CTA's
+            for (int u = t - 1;; u -= blockDim.x) {
+                const int v = u - static_cast<int>(threadIdx.x);
+                const bool found = v < 0 || block_at(v) >= 0;
+                if (found && v >= 0) atomicMax(&s_before, v);
+                if (__syncthreads_or(found)) break;
+            }
+            fresh = true;
+            if (s_before >= 0 && block_at(s_before) == blk) {
+                t = end;
+                __syncthreads();
+                continue;
+            }
+        }
+        float hi[E], lo[E];
+        bool odd = false;  // a token scale that is not finite
+#pragma unroll
+        for (int j = 0; j < E; ++j) { hi[j] = -INFINITY; lo[j] = INFINITY; }
+        const int64_t kv0 = blk * d.kv_stride_block + h * d.kv_stride_h;
+        const int64_t sc0 = blk * d.sc_stride_block + h * d.sc_stride_h;
+        auto place = [&](int i) { return static_cast<int>(p.slots[i] - static_cast<int64_t>(blk) * bs); };
+        auto earlier = [&](int o) {  // bounds take in a token that an earlier call wrote
+            float c[E];
+            L::load_codes(p.K + kv0 + o * d.kv_stride_t, lane, D, c);
+            const float s = p.ks[sc0 + o];
+            odd |= !isfinite(s);
+#pragma unroll
+            for (int j = 0; j < E; ++j) { hi[j] = fmaxf(hi[j], c[j] * s); lo[j] = fminf(lo[j], c[j] * s); }
+        };
+        if (p.bounds)
+            for (int o = warp, first = place(t); o < first; o += kRowWarps) earlier(o);
+        for (int i = t + warp; i < end; i += kRowWarps) {
+            if (block_at(i) < 0) {
+                if (lane == 0) odd_slot(i);
+                continue;
+            }
+            const int o = place(i);
+            const int64_t row = i * d.row_stride_t + h * d.row_stride_h;
+            float xk[E], xv[E];
+            L::load(static_cast<const T*>(p.k_rows) + row, lane, D, xk);
+            L::load(static_cast<const T*>(p.v_rows) + row, lane, D, xv);
+            const float sk = quantise_lanes<E>(xk), sv = quantise_lanes<E>(xv);
+            int8_t ck[E], cv[E];
+#pragma unroll
+            for (int j = 0; j < E; ++j) { ck[j] = static_cast<int8_t>(xk[j]); cv[j] = static_cast<int8_t>(xv[j]); }
+            L::store(p.K + kv0 + o * d.kv_stride_t, lane, D, ck);
+            L::store(p.V + kv0 + o * d.kv_stride_t, lane, D, cv);
+            if (lane == 0) { p.ks[sc0 + o] = sk; p.vs[sc0 + o] = sv; }
+            if (!p.bounds) continue;
+            odd |= !isfinite(sk);
+#pragma unroll
+            for (int j = 0; j < E; ++j) { hi[j] = fmaxf(hi[j], xk[j] * sk); lo[j] = fminf(lo[j], xk[j] * sk); }
+            int next = i + 1;  // places left out up to the next token with a slot
+            while (next < end && block_at(next) < 0) ++next;
+            if (next < end)
+                for (int u = o + 1, stop = place(next); u < stop; ++u) earlier(u);
+        }
+        if (p.bounds) {
+            float* mine = write_smem + warp * 2 * D;
+#pragma unroll
+            for (int j = 0; j < E; ++j)
+                if (L::in(lane, j, D)) { mine[L::at(lane, j)] = hi[j]; mine[D + L::at(lane, j)] = lo[j]; }
+            if (lane == 0) s_odd[warp] = odd;
+            __syncthreads();
+            if (warp == 0) {
+                float most = 0.f;
+#pragma unroll
+                for (int j = 0; j < E; ++j) {
+                    if (!L::in(lane, j, D)) { hi[j] = lo[j] = 0.f; continue; }
+                    for (int w = 1; w < kRowWarps; ++w) {
+                        hi[j] = fmaxf(hi[j], write_smem[w * 2 * D + L::at(lane, j)]);
+                        lo[j] = fminf(lo[j], write_smem[w * 2 * D + D + L::at(lane, j)]);
+                        odd |= s_odd[w] != 0;
+                    }
+                    most = fmaxf(most, fmaxf(fabsf(hi[j]), fabsf(lo[j])));
+                }
+                odd = __any_sync(0xffffffffu, odd);
+                most = warp_amax(most);
+                const float step = odd ? NAN : most / 127.0f;
+                int8_t up[E], down[E];
+#pragma unroll
+                for (int j = 0; j < E; ++j) {
+                    const bool some = step > 0.f;
+                    up[j] = some ? static_cast<int8_t>(fminf(fmaxf(ceilf(hi[j] / step), -127.f), 127.f)) : 0;
+                    down[j] = some ? static_cast<int8_t>(fminf(fmaxf(floorf(lo[j] / step), -127.f), 127.f)) : 0;
+                }
+                const int64_t bh = static_cast<int64_t>(blk) * d.num_kv_heads + h;
+                L::store(p.bounds + bh * 2 * D, lane, D, up);
+                L::store(p.bounds + bh * 2 * D + D, lane, D, down);
+                if (lane == 0) p.bound_scale[bh] = step;
+            }
+        }
+        t = end;
+        __syncthreads();  // s_end and the bounds rows are written again
+    }
+}
+
+template <class T, int E, bool VEC>
+__global__ void __launch_bounds__(32 * kRowWarps) read_kernel(const RowsParams p) {
+    using L = Lane<E, VEC>;
+    grid_dependency_wait();
+    allow_dependents();
+    const kvd_paged_rows_desc& d = p.d;
+    const int D = d.head_dim, bs = d.block_size, H = d.num_kv_heads;
+    const int lane = threadIdx.x & 31;
+    const int64_t n_slots = static_cast<int64_t>(d.num_blocks) * bs;
+    const int64_t rows = static_cast<int64_t>(d.num_tokens) * H;
+    for (int64_t r = static_cast<int64_t>(blockIdx.x) * kRowWarps + (threadIdx.x >> 5); r < rows;
+         r += static_cast<int64_t>(gridDim.x) * kRowWarps) {
+        const int t = static_cast<int>(r / H), h = static_cast<int>(r - static_cast<int64_t>(t) * H);
+        const int64_t slot = p.slots[t];
+        float xk[E], xv[E];
+#pragma unroll
+        for (int j = 0; j < E; ++j) xk[j] = xv[j] = 0.f;
+        if (slot >= 0 && slot < n_slots) {
+            const int64_t blk = slot / bs, o = slot - blk * bs;
+            const int64_t at = blk * d.kv_stride_block + h * d.kv_stride_h + o * d.kv_stride_t;
+            const int64_t sc = blk * d.sc_stride_block + h * d.sc_stride_h + o;
+            L::load_codes(p.K + at, lane, D, xk);
+            L::load_codes(p.V + at, lane, D, xv);
+            const float sk = p.ks[sc], sv = p.vs[sc];
+#pragma unroll
+            for (int j = 0; j < E; ++j) { xk[j] *= sk; xv[j] *= sv; }
+        } else if (slot != -1 && h == 0 && lane == 0) {
+            record_status(KVD_STATUS_BAD_BLOCK);
+        }
+        T yk[E], yv[E];
+#pragma unroll
+        for (int j = 0; j < E; ++j) { yk[j] = narrow<T>(xk[j]); yv[j] = narrow<T>(xv[j]); }
+        const int64_t row = t * d.row_stride_t + h * d.row_stride_h;
+        L::store(static_cast<T*>(p.k_out) + row, lane, D, yk);
+        L::store(static_cast<T*>(p.v_out) + row, lane, D, yv);
+    }
+}
+
+template <class T, int E, bool VEC>
+cudaError_t launch_rows(const RowsParams& p, bool write, cudaStream_t st) {
+    const kvd_paged_rows_desc& d = p.d;
+    if (write) {
+        const int64_t grid = static_cast<int64_t>((d.num_tokens + p.tile - 1) / p.tile) * d.num_kv_heads;
+        if (grid > 0x7fffffffLL) return cudaErrorInvalidValue;
+        return launch_after(write_kernel<T, E, VEC>, static_cast<unsigned>(grid), 32 * kRowWarps,
+                            sizeof(float) * kRowWarps * 2 * d.head_dim, 1, st, p);
+    }
+    const int64_t rows = static_cast<int64_t>(d.num_tokens) * d.num_kv_heads;
+    int64_t grid = (rows + kRowWarps - 1) / kRowWarps;
+    const int64_t most = static_cast<int64_t>(device_sm_count()) * 16;
+    if (grid > most) grid = most;
+    return launch_after(read_kernel<T, E, VEC>, static_cast<unsigned>(grid), 32 * kRowWarps, 0, 1, st, p);
+}
+
+template <class T>
+cudaError_t launch_rows_t(const RowsParams& p, bool write, bool vec, cudaStream_t st) {
+    if (vec && p.d.head_dim == 64) return launch_rows<T, 2, true>(p, write, st);
+    if (vec && p.d.head_dim == 128) return launch_rows<T, 4, true>(p, write, st);
+    if (vec && p.d.head_dim == 256) return launch_rows<T, 8, true>(p, write, st);
+    return launch_rows<T, 16, false>(p, write, st);
+}
+
+bool rows_ok(const kvd_paged_rows_desc* d) {
+    if (!d || d->num_tokens < 0 || d->num_kv_heads < 1 || d->head_dim < 1 || d->head_dim > 512) return false;
+    if (d->block_size < 1 || d->num_blocks < 1) return false;
+    return d->flags == 0 || d->flags == KVD_FLAG_Q_BF16 || d->flags == KVD_FLAG_Q_F16;
+}
+
+cudaError_t rows_call(RowsParams& p, const void* a, const void* b, bool write, cudaStream_t st) {
+    const kvd_paged_rows_desc& d = p.d;
+    // Vector access: a lane's E = D/32 elements are one load of at most 16
+    // bytes (two for fp32 rows of 256), so every row starts on 16 bytes.
+    const int64_t es = d.flags ? 2 : 4;
+    auto al = [](const void* x) { return (reinterpret_cast<uintptr_t>(x) & 15) == 0; };
+    const bool vec = al(a) && al(b) && al(p.K) && al(p.V) && al(p.bounds) &&
+                     (((d.row_stride_t | d.row_stride_h) * es) & 15) == 0 &&
+                     ((d.kv_stride_block | d.kv_stride_h | d.kv_stride_t) & 15) == 0;
+    cudaError_t e;
+    if (d.flags & KVD_FLAG_Q_BF16) e = launch_rows_t<__nv_bfloat16>(p, write, vec, st);
+    else if (d.flags & KVD_FLAG_Q_F16) e = launch_rows_t<__half>(p, write, vec, st);
+    else e = launch_rows_t<float>(p, write, vec, st);
+    if (e == cudaSuccess) ++*launch_counter();
+    return e;
+}
+
+// --------------------------------------------------------------------- select
+// A block's bound codes are one row [hi | lo] of 2D int8 values and a query
+// head's one row [max(c, 0) | min(c, 0)], so the bound of q . k is a plain dot
+// product of 2D integers: sum_d max(c hi, c lo) = sum c+ hi + sum c- lo. It
+// runs as int8 m16n8k32 products, 16 blocks by 8 heads; 8 products a tile
+// against 4 KB read (head_dim 128) leave HBM the bound, not the tensor pipe,
+// so a warp keeps its tile in registers: lane (g, t) loads 16-byte pieces of
+// rows g and g+8, and the order in which dims meet the product's k index is
+// the same for both operands, hence free.
+struct SelectParams {
+    kvd_block_select_desc d;
+    const void* Q;
+    const int8_t* bounds;
+    const float* bound_scale;
+    int32_t* sel_table;
+    int32_t* sel_lens;
+    int cap;  // keys a CTA holds
+};
+
+constexpr int kSelThreads = 256;
+constexpr int kSelWarps = kSelThreads / 32;
+constexpr uint32_t kAlways = 0xffffffffu;  // key of a block that is always selected; above every score's
+
+// Order-preserving key of a score: larger is better; NaN counts as +inf, -0 as +0.
+__device__ __forceinline__ uint32_t score_key(float s) {
+    if (isnan(s)) s = INFINITY;
+    const uint32_t u = __float_as_uint(s + 0.f);
+    return u & 0x80000000u ? ~u : u | 0x80000000u;
+}
+
+__device__ __forceinline__ void mma_s8(int (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                       uint32_t b1) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+__device__ __forceinline__ uint4 ld_stream(const void* p) {
+    uint4 v;
+    asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+                 : "l"(p));
+    return v;
+}
+
+// Bytes of one query row in shared memory: the pad keeps two rows' 16-byte
+// pieces on different banks.
+__host__ __device__ __forceinline__ int sel_q_stride(int D) { return 2 * D + 64; }
+
+// ND = D / 32: 64-byte pieces of a bound row; 0: any D, without tensor cores.
+template <int ND>
+__global__ void __launch_bounds__(kSelThreads) select_kernel(const SelectParams p) {
+    extern __shared__ __align__(16) uint8_t sel_smem[];
+    __shared__ uint32_t hist[4][256];
+    __shared__ uint32_t s_range[2][kSelWarps], s_span[2];
+    __shared__ uint32_t s_scan[kSelWarps], s_pick[3];
+    __shared__ uint32_t s_count[2][kSelWarps], s_total[2];
+    const cg::cluster_group cl = cg::this_cluster();
+    const unsigned ranks = cl.num_blocks(), rank = cl.block_rank();
+    const kvd_block_select_desc& d = p.d;
+    const int D = d.head_dim, H = d.num_kv_heads, G = d.num_q_heads / H;
+    const int row = blockIdx.x / ranks;
+    const int b = row / H, h = row - b * H;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    uint32_t* keys = reinterpret_cast<uint32_t*>(sel_smem);
+    uint8_t* s_q = sel_smem + 4 * p.cap;
+    const int GP = (G + 7) & ~7, QS = sel_q_stride(D);
+    float* s_sq = reinterpret_cast<float*>(s_q + GP * QS);
+    grid_dependency_wait();
+    allow_dependents();
+
+    const int bs = d.block_size, MB = d.max_blocks_per_seq, k = d.budget;
+    const int64_t len64 = min(static_cast<int64_t>(max(0, d.seq_lens[b])), static_cast<int64_t>(MB) * bs);
+    const int len = static_cast<int>(len64), n = static_cast<int>((len64 + bs - 1) / bs);
+    const int32_t* table = d.block_table + b * d.block_table_stride;
+    int32_t* out = p.sel_table + static_cast<int64_t>(row) * k;
+    if (rank == 0 && tid == 0) p.sel_lens[row] = n <= k ? len : (k - n) * bs + len;
+    if (n <= k) {  // everything: nothing to score (the same for every CTA of the cluster)
+        if (rank == 0)
+            for (int i = tid; i < k; i += kSelThreads) {
+                const int id = i < n ? table[i] : -1;
+                if (i < n && (id < 0 || id >= d.num_blocks)) record_status(KVD_STATUS_BAD_BLOCK);
+                out[i] = id;
+            }
+        return;
+    }
+
+    // query rows: codes split by sign, zero rows up to a multiple of 8 heads
+    for (int i = tid; i < GP * QS / 4; i += kSelThreads) reinterpret_cast<uint32_t*>(s_q)[i] = 0u;
+    for (int i = tid; i < 4 * 256; i += kSelThreads) (&hist[0][0])[i] = 0u;
+    __syncthreads();
+    for (int g = warp; g < G; g += kSelWarps) {
+        const int64_t q0 = b * d.q_stride_b + static_cast<int64_t>(h * G + g) * d.q_stride_h;
+        float x[16];
+#pragma unroll
+        for (int j = 0; j < 16; ++j) x[j] = lane + 32 * j < D ? load_q(p.Q, q0 + lane + 32 * j, d.flags) : 0.f;
+        const float s = quantise_lanes<16>(x);
+#pragma unroll
+        for (int j = 0; j < 16; ++j) {
+            const int at = lane + 32 * j;
+            if (at < D) {
+                const int c = static_cast<int>(x[j]);
+                s_q[g * QS + at] = static_cast<uint8_t>(static_cast<int8_t>(max(c, 0)));
+                s_q[g * QS + D + at] = static_cast<uint8_t>(static_cast<int8_t>(min(c, 0)));
+            }
+        }
+        if (lane == 0) s_sq[g] = s;
+    }
+    __syncthreads();
+
+    // scores of this CTA's blocks [lo, lo + m)
+    const int per = ((n + static_cast<int>(ranks) - 1) / static_cast<int>(ranks) + 15) & ~15;
+    const int lo = min(n, static_cast<int>(rank) * per), m = min(n, lo + per) - lo;
+    uint32_t kmin = 0xffffffffu, kmax = 0u;
+    auto put = [&](int i, int id, float best) {  // block lo + i, the largest head product (without step)
+        uint32_t key;
+        const int at = lo + i;
+        if (at < d.first || at >= n - d.last) {
+            key = kAlways;
+        } else {
+            key = id < 0 ? 0u : score_key(best * p.bound_scale[static_cast<int64_t>(id) * H + h]);
+            kmin = min(kmin, key);
+            kmax = max(kmax, key);
+        }
+        keys[i] = key;
+    };
+    auto block_id = [&](int i) -> int {  // pool id of block lo + i, -1 when outside the pool
+        if (i >= m) return -1;
+        const int id = table[lo + i];
+        if (id >= 0 && id < d.num_blocks) return id;
+        record_status(KVD_STATUS_BAD_BLOCK);
+        return -1;
+    };
+    if constexpr (ND > 0) {
+        const int g = lane >> 2, t = lane & 3;
+        int ids = block_id(warp * 16 + (lane & 15));
+        for (int i0 = warp * 16; i0 < m; i0 += kSelWarps * 16) {
+            const int next = block_id(i0 + kSelWarps * 16 + (lane & 15));
+            const int id0 = __shfl_sync(0xffffffffu, ids, g), id1 = __shfl_sync(0xffffffffu, ids, g + 8);
+            uint4 a0[ND], a1[ND];
+            const int8_t* r0 = p.bounds + (static_cast<int64_t>(max(id0, 0)) * H + h) * (2 * D) + 16 * t;
+            const int8_t* r1 = p.bounds + (static_cast<int64_t>(max(id1, 0)) * H + h) * (2 * D) + 16 * t;
+#pragma unroll
+            for (int j = 0; j < ND; ++j) { a0[j] = ld_stream(r0 + 64 * j); a1[j] = ld_stream(r1 + 64 * j); }
+            float best0 = -INFINITY, best1 = -INFINITY;
+            for (int g0 = 0; g0 < GP; g0 += 8) {
+                int c[4] = {0, 0, 0, 0};
+                const uint8_t* qr = s_q + (g0 + g) * QS + 16 * t;
+#pragma unroll
+                for (int j = 0; j < ND; ++j) {
+                    const uint4 q = *reinterpret_cast<const uint4*>(qr + 64 * j);
+                    mma_s8(c, a0[j].x, a1[j].x, a0[j].y, a1[j].y, q.x, q.y);
+                    mma_s8(c, a0[j].z, a1[j].z, a0[j].w, a1[j].w, q.z, q.w);
+                }
+#pragma unroll
+                for (int x = 0; x < 2; ++x) {
+                    const int hd = g0 + 2 * t + x;
+                    if (hd < G) {
+                        float v0 = static_cast<float>(c[x]) * s_sq[hd], v1 = static_cast<float>(c[2 + x]) * s_sq[hd];
+                        if (isnan(v0)) v0 = INFINITY;
+                        if (isnan(v1)) v1 = INFINITY;
+                        best0 = fmaxf(best0, v0);
+                        best1 = fmaxf(best1, v1);
+                    }
+                }
+            }
+#pragma unroll
+            for (int o = 1; o < 4; o <<= 1) {
+                best0 = fmaxf(best0, __shfl_xor_sync(0xffffffffu, best0, o));
+                best1 = fmaxf(best1, __shfl_xor_sync(0xffffffffu, best1, o));
+            }
+            if (t == 0 && i0 + g < m) put(i0 + g, id0, best0);
+            if (t == 1 && i0 + g + 8 < m) put(i0 + g + 8, id1, best1);
+            ids = next;
+        }
+    } else {
+        for (int i = warp; i < m; i += kSelWarps) {
+            const int id = block_id(i);
+            const int8_t* r = p.bounds + (static_cast<int64_t>(max(id, 0)) * H + h) * (2 * D);
+            float best = -INFINITY;
+            for (int gg = 0; gg < G; ++gg) {
+                int acc = 0;
+                for (int x = lane; x < 2 * D; x += 32) acc += static_cast<int8_t>(s_q[gg * QS + x]) * r[x];
+                acc = __reduce_add_sync(0xffffffffu, acc);
+                float v = static_cast<float>(acc) * s_sq[gg];
+                if (isnan(v)) v = INFINITY;
+                best = fmaxf(best, v);
+            }
+            if (lane == 0) put(i, id, best);
+        }
+    }
+
+    // Threshold of the `need` best scored keys: 8-bit radix passes from the
+    // highest bit in which any two keys differ, over all CTAs of the cluster.
+    kmin = __reduce_min_sync(0xffffffffu, kmin);
+    kmax = __reduce_max_sync(0xffffffffu, kmax);
+    if (lane == 0) { s_range[0][warp] = kmin; s_range[1][warp] = kmax; }
+    __syncthreads();
+    if (tid == 0) {
+        for (int w = 1; w < kSelWarps; ++w) {
+            kmin = min(kmin, s_range[0][w]);
+            kmax = max(kmax, s_range[1][w]);
+        }
+        s_span[0] = kmin;
+        s_span[1] = kmax;
+    }
+    cl.sync();
+    kmin = 0xffffffffu;
+    kmax = 0u;
+    for (unsigned r = 0; r < ranks; ++r) {
+        const uint32_t* sp = cl.map_shared_rank(s_span, r);
+        kmin = min(kmin, sp[0]);
+        kmax = max(kmax, sp[1]);
+    }
+    uint32_t need = static_cast<uint32_t>(k - d.first - d.last);
+    int top = kmin == kmax ? 0 : 32 - __clz(kmin ^ kmax);
+    uint32_t mask = top >= 32 ? 0u : 0xffffffffu << top;
+    uint32_t prefix = kmax & mask;
+    for (int round = 0; top > 0 && need > 0; ++round) {
+        const int sh = max(0, top - 8);
+        const uint32_t bins = 1u << (top - sh);
+        for (int i = tid; i < m; i += kSelThreads) {
+            const uint32_t key = keys[i];
+            if (key != kAlways && (key & mask) == prefix) atomicAdd(&hist[round][(key >> sh) & (bins - 1)], 1u);
+        }
+        cl.sync();
+        uint32_t x = 0;  // keys in bin 255 - tid
+        for (unsigned r = 0; r < ranks; ++r) x += cl.map_shared_rank(&hist[round][0], r)[255 - tid];
+        uint32_t upto = x;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const uint32_t y = __shfl_up_sync(0xffffffffu, upto, o);
+            if (lane >= o) upto += y;
+        }
+        if (lane == 31) s_scan[warp] = upto;
+        __syncthreads();
+        for (int w = 0; w < warp; ++w) upto += s_scan[w];
+        if (upto >= need && upto - x < need) {
+            s_pick[0] = 255 - tid;
+            s_pick[1] = upto - x;
+            s_pick[2] = x;
+        }
+        __syncthreads();
+        const uint32_t bin = s_pick[0], in_bin = s_pick[2];
+        need -= s_pick[1];
+        prefix |= bin << sh;
+        mask |= (bins - 1) << sh;
+        top = sh;
+        if (in_bin == need) break;  // the whole bin is selected
+    }
+
+    // Selected: always, above the threshold, or among the first `need` at it.
+    // Each warp owns a stretch of the CTA's blocks, so places follow from counts.
+    const int seg = ((m + kSelWarps - 1) / kSelWarps + 31) & ~31;
+    const int s0 = min(m, warp * seg), s1 = min(m, s0 + seg);
+    uint32_t above = 0, equal = 0;
+    for (int i0 = s0; i0 < s1; i0 += 32) {
+        const uint32_t key = i0 + lane < s1 ? keys[i0 + lane] : 0u;
+        const bool in = i0 + lane < s1;
+        above += __popc(__ballot_sync(0xffffffffu, in && (key == kAlways || (key & mask) > prefix)));
+        equal += __popc(__ballot_sync(0xffffffffu, in && key != kAlways && (key & mask) == prefix));
+    }
+    if (lane == 0) { s_count[0][warp] = above; s_count[1][warp] = equal; }
+    __syncthreads();
+    if (tid == 0) {
+        uint32_t a = 0, e = 0;
+        for (int w = 0; w < kSelWarps; ++w) { a += s_count[0][w]; e += s_count[1][w]; }
+        s_total[0] = a;
+        s_total[1] = e;
+    }
+    cl.sync();
+    above = equal = 0;
+    for (unsigned r = 0; r < rank; ++r) {
+        const uint32_t* tt = cl.map_shared_rank(s_total, r);
+        above += tt[0];
+        equal += tt[1];
+    }
+    for (int w = 0; w < warp; ++w) { above += s_count[0][w]; equal += s_count[1][w]; }
+    const uint32_t below = (1u << lane) - 1u;
+    for (int i0 = s0; i0 < s1; i0 += 32) {
+        const bool in = i0 + lane < s1;
+        const uint32_t key = in ? keys[i0 + lane] : 0u;
+        const bool up = in && (key == kAlways || (key & mask) > prefix);
+        const bool eq = in && key != kAlways && (key & mask) == prefix;
+        const uint32_t ub = __ballot_sync(0xffffffffu, up), eb = __ballot_sync(0xffffffffu, eq);
+        const uint32_t e = equal + __popc(eb & below);
+        if (up || (eq && e < need)) out[above + __popc(ub & below) + min(e, need)] = table[lo + i0 + lane];
+        above += __popc(ub);
+        equal += __popc(eb);
+    }
+    cl.sync();  // the other CTAs have read this one's shared memory
+}
+
+template <int ND>
+cudaError_t launch_select(const SelectParams& p, int cluster, size_t smem, cudaStream_t st) {
+    auto kern = select_kernel<ND>;
+    static PerDeviceOnce once;
+    const cudaError_t e = once.run(
+        [kern] { return cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, 200 * 1024); });
+    if (e != cudaSuccess) return e;
+    const int64_t grid = static_cast<int64_t>(p.d.batch) * p.d.num_kv_heads * cluster;
+    return launch_after(kern, static_cast<unsigned>(grid), kSelThreads, smem, static_cast<unsigned>(cluster), st, p);
+}
+
+}  // namespace
+}  // namespace kvd
+
+using namespace kvd;
+
+namespace {
+bool plan_ok(const kvd_paged_plan_desc* d) {
+    if (!d || d->batch < 1 || d->batch > kPlanMaxBatch || d->block_size < 1 || d->num_blocks < 1) return false;
+    if (d->max_blocks_per_seq < 1 || d->num_slots < 0 || d->num_slots == 0x7fffffff) return false;
+    if (d->block_table_stride < d->max_blocks_per_seq) return false;
+    return static_cast<int64_t>(d->max_blocks_per_seq) * d->block_size <= 0x7fffffffLL;
+}
+}  // namespace
+
+extern "C" size_t kvd_paged_plan_workspace_size(const kvd_paged_plan_desc* desc) { return plan_ok(desc) ? 16 : 0; }
+
+extern "C" cudaError_t kvd_paged_plan_launch(const kvd_paged_plan_desc* desc, const int32_t* seq_lens,
+                                             const int32_t* new_lens, int32_t* block_table, int32_t* free_blocks,
+                                             const int32_t* free_count, int64_t* slot_map, int32_t* token_starts,
+                                             int32_t* seq_lens_out, int32_t* free_count_out, void* workspace,
+                                             size_t workspace_bytes, cudaStream_t stream) {
+    *launch_counter() = 0;
+    if (!plan_ok(desc) || !seq_lens || !new_lens || !block_table || !free_blocks || !free_count || !token_starts ||
+        !seq_lens_out || !free_count_out || (!slot_map && desc->num_slots > 0))
+        return cudaErrorInvalidValue;
+    if (!workspace || workspace_bytes < kvd_paged_plan_workspace_size(desc)) return cudaErrorInvalidValue;
+    PlanParams p{*desc, seq_lens, new_lens, block_table, free_blocks, free_count, slot_map, token_starts,
+                 seq_lens_out, free_count_out, static_cast<unsigned int*>(workspace)};
+    const unsigned block = desc->batch <= 256 ? 256 : 1024;
+    const size_t smem = static_cast<size_t>(desc->batch) * 13 + 16;
+    static PerDeviceOnce once;
+    cudaError_t e = once.run([] {
+        return cudaFuncSetAttribute(plan_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kPlanMaxBatch * 13 + 16);
+    });
+    if (e != cudaSuccess) return e;
+    int64_t grid = (static_cast<int64_t>(desc->num_slots) + 4 * block - 1) / (4 * block);
+    if (grid > device_sm_count()) grid = device_sm_count();
+    if (grid < 1) grid = 1;
+    e = launch_after(plan_kernel, static_cast<unsigned>(grid), block, smem, 1, stream, p);
+    if (e == cudaSuccess) *launch_counter() = 1;
+    return e;
+}
+
+extern "C" cudaError_t kvd_paged_write_launch(const kvd_paged_rows_desc* desc, const void* k_new, const void* v_new,
+                                              const int64_t* slot_map, int8_t* K_pool, int8_t* V_pool,
+                                              float* k_scale_pool, float* v_scale_pool, int8_t* bounds,
+                                              float* bound_scale, cudaStream_t stream) {
+    *launch_counter() = 0;
+    if (!rows_ok(desc)) return cudaErrorInvalidValue;
+    if (desc->num_tokens == 0) return cudaSuccess;
+    if (!k_new || !v_new || !slot_map || !K_pool || !V_pool || !k_scale_pool || !v_scale_pool ||
+        (bounds == nullptr) != (bound_scale == nullptr))
+        return cudaErrorInvalidValue;
+    RowsParams p{*desc, k_new, v_new, nullptr, nullptr, slot_map, K_pool, V_pool, k_scale_pool, v_scale_pool,
+                 bounds, bound_scale, 1};
+    const int64_t per = static_cast<int64_t>(desc->num_tokens) * desc->num_kv_heads / (16 * device_sm_count());
+    p.tile = static_cast<int>(per < 1 ? 1 : per > 32 ? 32 : per);
+    return rows_call(p, k_new, v_new, true, stream);
+}
+
+extern "C" cudaError_t kvd_paged_read_launch(const kvd_paged_rows_desc* desc, const int64_t* slot_map,
+                                             const int8_t* K_pool, const int8_t* V_pool, const float* k_scale_pool,
+                                             const float* v_scale_pool, void* k_out, void* v_out,
+                                             cudaStream_t stream) {
+    *launch_counter() = 0;
+    if (!rows_ok(desc)) return cudaErrorInvalidValue;
+    if (desc->num_tokens == 0) return cudaSuccess;
+    if (!slot_map || !K_pool || !V_pool || !k_scale_pool || !v_scale_pool || !k_out || !v_out)
+        return cudaErrorInvalidValue;
+    RowsParams p{*desc, nullptr, nullptr, k_out, v_out, slot_map, const_cast<int8_t*>(K_pool),
+                 const_cast<int8_t*>(V_pool), const_cast<float*>(k_scale_pool), const_cast<float*>(v_scale_pool),
+                 nullptr, nullptr, 1};
+    return rows_call(p, k_out, v_out, false, stream);
+}
+
+extern "C" cudaError_t kvd_block_select_launch(const kvd_block_select_desc* desc, const void* Q, const int8_t* bounds,
+                                               const float* bound_scale, int32_t* sel_table, int32_t* sel_lens,
+                                               cudaStream_t stream) {
+    *launch_counter() = 0;
+    if (!desc || !Q || !bounds || !bound_scale || !sel_table || !sel_lens || !desc->seq_lens || !desc->block_table)
+        return cudaErrorInvalidValue;
+    const kvd_block_select_desc& d = *desc;
+    if (d.batch < 1 || d.num_q_heads < 1 || d.num_kv_heads < 1 || d.num_q_heads % d.num_kv_heads != 0 ||
+        d.head_dim < 1 || d.head_dim > 512 || d.block_size < 1 || d.num_blocks < 1)
+        return cudaErrorInvalidValue;
+    if (d.max_blocks_per_seq < 1 || d.max_blocks_per_seq > 262144 || d.block_table_stride < d.max_blocks_per_seq ||
+        static_cast<int64_t>(d.max_blocks_per_seq) * d.block_size > 0x7fffffffLL)
+        return cudaErrorInvalidValue;
+    if (d.budget < 1 || d.first < 0 || d.last < 1 || d.first > d.budget - d.last) return cudaErrorInvalidValue;
+    if (d.flags != 0 && d.flags != KVD_FLAG_Q_BF16 && d.flags != KVD_FLAG_Q_F16) return cudaErrorInvalidValue;
+    const int64_t rows = static_cast<int64_t>(d.batch) * d.num_kv_heads;
+    if (rows > 0x7fffffffLL / 8) return cudaErrorInvalidValue;
+    // CTAs per row: enough to fill the GPU, at least 128 blocks each, keys within shared memory
+    int c = 1;
+    while (c < 8 && rows * c < 2 * device_sm_count() && d.max_blocks_per_seq >= 256 * c) c *= 2;
+    while (c < 8 && d.max_blocks_per_seq > 32768 * c) c *= 2;
+    SelectParams p{d, Q, bounds, bound_scale, sel_table, sel_lens, 0};
+    p.cap = ((d.max_blocks_per_seq + c - 1) / c + 15) & ~15;
+    const int G = d.num_q_heads / d.num_kv_heads, GP = (G + 7) & ~7;
+    const size_t smem = 4 * static_cast<size_t>(p.cap) + static_cast<size_t>(GP) * sel_q_stride(d.head_dim) +
+                        sizeof(float) * G;
+    if (smem > 200 * 1024) return cudaErrorInvalidValue;
+    const bool vec = (reinterpret_cast<uintptr_t>(bounds) & 15) == 0 && d.head_dim % 32 == 0;
+    cudaError_t e;
+    switch (vec ? d.head_dim : 0) {
+        case 64: e = launch_select<2>(p, c, smem, stream); break;
+        case 96: e = launch_select<3>(p, c, smem, stream); break;
+        case 128: e = launch_select<4>(p, c, smem, stream); break;
+        case 192: e = launch_select<6>(p, c, smem, stream); break;
+        case 256: e = launch_select<8>(p, c, smem, stream); break;
+        default: e = launch_select<0>(p, c, smem, stream); break;
+    }
+    if (e == cudaSuccess) *launch_counter() = 1;
+    return e;
+}

@@ -126,12 +126,14 @@ constexpr int tile_tokens(int D) { return sk_consumer_warps(D) * (32 / (D / 16))
 // max_seq_len is the table's capacity (max_blocks_per_seq * block_size).
 // Token t of sequence b, kv head h: block table[b*bt_stride + t/block_size],
 // codes at blk*kv_sblk + h*kv_sh + (t%block_size)*kv_st, scales at
-// blk*sc_sblk + h*sc_sh + t%block_size.
+// blk*sc_sblk + h*sc_sh + t%block_size. per_head: lengths and table rows are
+// those of sequence b*Hkv + h (blocks selected for each KV head).
 struct PagedView {
     const int32_t* table;
     int64_t bt_stride;
     int block_size, num_blocks;
     int64_t kv_sblk, kv_st, sc_sblk;
+    bool per_head;
 };
 
 // Fused quantise-on-append for launch_gqa_tc: the new token's fp32 K/V rows
@@ -167,7 +169,7 @@ cudaError_t launch_combine_records(const float* base, int nparts, int64_t part_s
                                    int64_t rows, int rows_per_b, int D, void* out, int64_t o_sb, int64_t o_sh,
                                    uint32_t flags, cudaStream_t st, int* launches);
 bool gqa_path_ok(const kvd_decode_desc& d);
-size_t gqa_workspace_size(const kvd_decode_desc& d);
+size_t gqa_workspace_size(const kvd_decode_desc& d, bool sel = false);
 // Split records a dense tensor-core decode left in its workspace when the
 // caller asked it to skip the combine: row r's P records of D+4 floats start
 // at partials + r*P*(D+4). P == 1: the rows were written to `out` directly.

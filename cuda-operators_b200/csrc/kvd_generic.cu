@@ -49,7 +49,8 @@ __device__ __forceinline__ void token_offsets(const GenParams& p, int b, int hk,
         return;
     }
     const int j = t / p.pv.block_size, off = t - j * p.pv.block_size;
-    int blk = p.pv.table[b * p.pv.bt_stride + j];
+    const int64_t seq = p.pv.per_head ? static_cast<int64_t>(b) * (p.Hq / p.group) + hk : b;
+    int blk = p.pv.table[seq * p.pv.bt_stride + j];
     if (blk < 0 || blk >= p.pv.num_blocks) {
         record_status(KVD_STATUS_BAD_BLOCK);
         blk = 0;
@@ -72,7 +73,8 @@ __global__ void __launch_bounds__(kGenThreads) generic_decode_kernel(const GenPa
     const int qi = p.Lq > 0 ? static_cast<int>(u - bh * p.Lq) : 0;
     const int b = static_cast<int>(bh / p.Hq), hq = static_cast<int>(bh % p.Hq);
     const int hk = hq / p.group;
-    int len = p.seq_lens ? min(max(0, p.seq_lens[b]), p.S) : p.S;  // clamp to the capacity
+    const int64_t seq = p.pv.per_head ? static_cast<int64_t>(b) * (p.Hq / p.group) + hk : b;
+    int len = p.seq_lens ? min(max(0, p.seq_lens[seq]), p.S) : p.S;  // clamp to the capacity
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     if (p.Lq > 0) {  // prefill: this query's causal prefix
         const int ql = p.q_lens ? min(max(0, p.q_lens[b]), p.Lq) : p.Lq;

@@ -54,7 +54,8 @@ struct GqaParams {
     float qscale;
     uint32_t flags;
     // Paged cache (table != nullptr): the maps view the pools as
-    // {D, block_size, Hkv, num_blocks}; lbs = log2(block_size) >= 3.
+    // {D, block_size, Hkv, num_blocks}; lbs = log2(block_size) >= 3. Selected
+    // blocks (query mode 2): table rows and lengths are per (b, kv head).
     const int32_t* table;
     int64_t bt_stride, sc_sblk;
     int lbs, nblk;
@@ -104,7 +105,10 @@ struct GqaCfg {
     // N = NP, four accumulator columns per head); QM = 1 (KVD_FLAG_QK_INT8)
     // quantises it to one int8 row per head, so QK has N = 16 and one column
     // per head: head h of warpgroup w is B row / accumulator column w*QPW + h.
-    static constexpr bool QI8 = QM_ != 0;
+    // QM = 2 is QM = 0 over selected blocks: every (b, kv head) is a sequence
+    // of its own, with its own length and block table row.
+    static constexpr bool QI8 = QM_ == 1;
+    static constexpr bool SEL = QM_ == 2;
     static constexpr int NQ = QI8 ? 16 : NP;                      // QK MMA N (<= NP)
     static constexpr int QPW = NQ / NWG;                          // QK rows / columns per warpgroup
     static constexpr int SW = QI8 ? HPW : CPW;                    // score columns an epilogue thread loads
@@ -167,7 +171,7 @@ __device__ __forceinline__ int exp_above(float x) {
 namespace kvd {
 
 struct GItem {
-    int b, hk, split, t_lo, t_hi, ntiles;
+    int b, hk, row, split, t_lo, t_hi, ntiles;  // row: the sequence, whose length and table row are read
 };
 
 // Items are numbered split-major: item = (split * B + k) * Hkv + hk, where k
@@ -191,6 +195,7 @@ __device__ __forceinline__ int split_count(const GqaParams& p, int len) {
     return len > 0 ? (len + p.span - 1) / p.span : 1;
 }
 
+template <bool SEL>
 __device__ __forceinline__ GItem gqa_item(const GqaParams& p, int it) {
     GItem I;
     const int per_split = p.B * p.Hkv;
@@ -198,8 +203,9 @@ __device__ __forceinline__ GItem gqa_item(const GqaParams& p, int it) {
     const int rem = it - I.split * per_split;
     const int k = rem / p.Hkv;
     I.hk = rem - k * p.Hkv;
-    I.b = p.order ? __ldg(p.order + k) : k;
-    const int len = seq_len_of(p, I.b);
+    I.b = !SEL && p.order ? __ldg(p.order + k) : k;
+    I.row = SEL ? rem : I.b;
+    const int len = seq_len_of(p, I.row);
     I.t_lo = I.split * p.span;
     I.t_hi = min(len, I.t_lo + p.span);
     const int n = I.t_hi - I.t_lo;
@@ -208,8 +214,9 @@ __device__ __forceinline__ GItem gqa_item(const GqaParams& p, int it) {
 }
 
 // First non-empty item of this CTA at or after `it` (stepping by the grid).
+template <bool SEL>
 __device__ __forceinline__ int next_item(const GqaParams& p, int it) {
-    while (it < p.n_items && gqa_item(p, it).ntiles == 0) it += p.grid;
+    while (it < p.n_items && gqa_item<SEL>(p, it).ntiles == 0) it += p.grid;
     return it;
 }
 
@@ -242,29 +249,31 @@ struct PTile {
 };
 
 // First tile of this CTA; it = n_items when there is none.
+template <bool SEL>
 __device__ __forceinline__ PTile ptile_first(const GqaParams& p) {
     PTile T;
-    T.it = next_item(p, blockIdx.x);
+    T.it = next_item<SEL>(p, blockIdx.x);
     T.tt = 0;
     T.t0 = 0;
     T.n = 0;
-    T.I = GItem{0, 0, 0, 0, 0, 0};
+    T.I = GItem{0, 0, 0, 0, 0, 0, 0};
     if (T.it < p.n_items) {
-        T.I = gqa_item(p, T.it);
+        T.I = gqa_item<SEL>(p, T.it);
         T.t0 = T.I.t_lo;
         T.n = max(0, min(128, T.I.t_hi - T.t0));
     }
     return T;
 }
 
+template <bool SEL>
 __device__ __forceinline__ PTile ptile_next(const GqaParams& p, const PTile& A) {
     PTile T = A;
     if (T.it >= p.n_items) return T;
     if (++T.tt >= T.I.ntiles) {
         T.tt = 0;
-        T.it = next_item(p, T.it + p.grid);
+        T.it = next_item<SEL>(p, T.it + p.grid);
         if (T.it >= p.n_items) return T;
-        T.I = gqa_item(p, T.it);
+        T.I = gqa_item<SEL>(p, T.it);
     }
     T.t0 = T.I.t_lo + T.tt * 128;
     T.n = max(0, min(128, T.I.t_hi - T.t0));
@@ -275,7 +284,7 @@ __device__ __forceinline__ PTile ptile_next(const GqaParams& p, const PTile& A) 
 __device__ __forceinline__ int ptile_block(const GqaParams& p, const PTile& T, int rows, int lane) {
     const int tok = (lane & 15) * rows;
     if (T.it >= p.n_items || tok >= T.n) return -1;
-    return __ldg(p.table + T.I.b * p.bt_stride + ((T.t0 + tok) >> p.lbs));
+    return __ldg(p.table + T.I.row * p.bt_stride + ((T.t0 + tok) >> p.lbs));
 }
 
 // Scales of tokens 4*lane .. 4*lane+3 of tile T (blocks of 8..64 tokens);
@@ -322,15 +331,15 @@ __device__ __forceinline__ void gqa_producer_paged(const CUtensorMap* kmap, cons
         ++ik;
         return true;
     };
-    PTile T0 = ptile_first(p);
-    PTile T1 = ptile_next(p, T0);
+    PTile T0 = ptile_first<C::SEL>(p);
+    PTile T1 = ptile_next<C::SEL>(p, T0);
     int b0 = ptile_block(p, T0, rows, lane), b1 = ptile_block(p, T1, rows, lane);
     float4 kq0, vq0;
     if (small) ptile_scales(p, T0, b0, lane, kq0, vq0);
     // K runs one tile ahead of V: K(T0) now, then each step issues K(T1) before V(T0).
     bool ok = T0.it >= p.n_items || issue_k(T0, b0);
     while (ok && T0.it < p.n_items) {
-        const PTile T2 = ptile_next(p, T1);
+        const PTile T2 = ptile_next<C::SEL>(p, T1);
         const int b2 = ptile_block(p, T2, rows, lane);  // two tiles ahead
         float4 kq1, vq1;
         if (small) ptile_scales(p, T1, b1, lane, kq1, vq1);  // one tile ahead
@@ -401,8 +410,8 @@ __device__ __forceinline__ void gqa_producer(const CUtensorMap* kmap, const CUte
     bool wrapped = false, ok = true;
     int64_t issued = 0;
     bool appended = p.k_new == nullptr;  // fused append finished (or none)
-    for (int it = next_item(p, blockIdx.x); it < p.n_items && ok; it = next_item(p, it + p.grid)) {
-        const GItem I = gqa_item(p, it);
+    for (int it = next_item<C::SEL>(p, blockIdx.x); it < p.n_items && ok; it = next_item<C::SEL>(p, it + p.grid)) {
+        const GItem I = gqa_item<C::SEL>(p, it);
         const int apos = appended ? -1 : append_pos(p, I.b);
         for (int tt = 0; tt < I.ntiles; ++tt) {
             if (wrapped && !mbar_wait(&empty[s], round_par ^ 1u)) { ok = false; break; }
@@ -486,8 +495,8 @@ __device__ __forceinline__ void gqa_mma(const GqaParams& p, uint8_t* smem, uint3
     constexpr uint32_t idesc_qk = idesc_i8(true, true, false, false, C::NQ, 128);
     int64_t i = 0;
     int kq = 0;
-    for (int it = next_item(p, blockIdx.x); it < p.n_items; it = next_item(p, it + p.grid), ++kq) {
-        const GItem I = gqa_item(p, it);
+    for (int it = next_item<C::SEL>(p, blockIdx.x); it < p.n_items; it = next_item<C::SEL>(p, it + p.grid), ++kq) {
+        const GItem I = gqa_item<C::SEL>(p, it);
         for (int tt = 0; tt < I.ntiles; ++tt, ++i) {
             const int sk = static_cast<int>(i % NK);
             if (!mbar_wait(&bars[C::B_KFULL + sk], static_cast<uint32_t>((i / NK) & 1))) return;
@@ -622,7 +631,7 @@ __device__ __forceinline__ bool gqa_qlimbs(const GqaParams& p, uint8_t* smem, in
     uint64_t* q_full = bars + C::B_QFULL;
     uint64_t* red_bar = bars + C::B_RED + wg;
     float* red = reinterpret_cast<float*>(smem + C::OFF_RED) + wg * 256;
-    const GItem I = gqa_item(p, it);
+    const GItem I = gqa_item<C::SEL>(p, it);
     const int h0 = wg * HPW;
     const int64_t q0 = I.b * p.q_sb + static_cast<int64_t>(I.hk * G + h0) * p.q_sh + r;
     float qv[HPW], am[HPW];
@@ -692,7 +701,7 @@ __device__ __forceinline__ void fused_append_rows(const GqaParams& p, uint8_t* s
         named_bar_sync(1, ET);
         if (base + t < per_cta) {
             const int it = static_cast<int>(blockIdx.x) + (base + t) * p.grid;
-            const GItem I = gqa_item(p, it);
+            const GItem I = gqa_item<C::SEL>(p, it);
             const int apos = append_pos(p, I.b);
             if (apos >= I.t_lo && apos < I.t_hi) {
                 const int e = atomicAdd(count, 1);
@@ -776,8 +785,8 @@ __device__ __forceinline__ bool gqa_pv_epi(const GqaParams& p, uint8_t* smem, ui
         o[h] = fmaf(f, __int_as_float(1065353216 - FA[h] * 8388608), o[h]);
     }
     if (A.flags & 2) {
-        const GItem I = gqa_item(p, A.it);
-        const bool split_row = p.P > 1 && split_count(p, seq_len_of(p, I.b)) > 1;
+        const GItem I = gqa_item<C::SEL>(p, A.it);
+        const bool split_row = p.P > 1 && split_count(p, seq_len_of(p, I.row)) > 1;
         const bool records = split_row || (p.flags & KVD_FLAG_PARTIAL_OUT);
 #pragma unroll
         for (int h = 0; h < HPW; ++h) {
@@ -828,7 +837,7 @@ __device__ __forceinline__ void gqa_epilogue(const GqaParams& p, uint8_t* smem, 
     const uint32_t lane_base = tmem + (static_cast<uint32_t>(wq * 32) << 16) + wg * C::QPW;  // this warpgroup's scores
     uint32_t use = 0;
 
-    if (p.k_new) fused_append_rows<G, NK, NV, QM>(p, smem);
+    if (!C::SEL && p.k_new) fused_append_rows<G, NK, NV, QM>(p, smem);
     const unsigned int tag = *reinterpret_cast<const unsigned int*>(smem + C::OFF_TAG);  // tagged records
 
     // Zero this warpgroup's rows of both query-limb buffers (pad rows stay
@@ -843,7 +852,7 @@ __device__ __forceinline__ void gqa_epilogue(const GqaParams& p, uint8_t* smem, 
         }
     }
     float sEn[HPW];
-    if (!gqa_qlimbs<G, NK, NV, QM>(p, smem, next_item(p, blockIdx.x), 0, use, sEn)) return;
+    if (!gqa_qlimbs<G, NK, NV, QM>(p, smem, next_item<C::SEL>(p, blockIdx.x), 0, use, sEn)) return;
 
     float m[HPW], l[HPW], sE[HPW], o[HPW], mpv[HPW], mA[HPW], LA[HPW];
     int FA[HPW];
@@ -855,8 +864,8 @@ __device__ __forceinline__ void gqa_epilogue(const GqaParams& p, uint8_t* smem, 
     int s = 0;
     uint32_t ph = 0;
     int kq = 0;
-    for (int it = next_item(p, blockIdx.x); it < p.n_items; it = next_item(p, it + p.grid), ++kq) {
-        const GItem I = gqa_item(p, it);
+    for (int it = next_item<C::SEL>(p, blockIdx.x); it < p.n_items; it = next_item<C::SEL>(p, it + p.grid), ++kq) {
+        const GItem I = gqa_item<C::SEL>(p, it);
         for (int tt = 0; tt < I.ntiles; ++tt, ++i) {
             const int bi = static_cast<int>(i & 1);
             // ---- scores of tile i (thread r = token r of the tile)
@@ -942,7 +951,7 @@ __device__ __forceinline__ void gqa_epilogue(const GqaParams& p, uint8_t* smem, 
                 for (int h = 0; h < HPW; ++h) LB[h] = 0.f;
             }
             if (tt == 0) {
-                const int nxt = next_item(p, it + p.grid);
+                const int nxt = next_item<C::SEL>(p, it + p.grid);
                 if (nxt < p.n_items && !gqa_qlimbs<G, NK, NV, QM>(p, smem, nxt, (kq + 1) & 1, use, sEn)) return;
             }
 #pragma unroll
@@ -998,7 +1007,7 @@ __global__ void __launch_bounds__(GqaCfg<G, NK, NV, QM>::THREADS, MINB) gqa_tc_k
         grid_dependency_wait();
         allow_dependents();
     }
-    if (next_item(p, blockIdx.x) >= p.n_items) {  // no (non-empty) item for this CTA (exiting allows the dependents)
+    if (next_item<C::SEL>(p, blockIdx.x) >= p.n_items) {  // no (non-empty) item for this CTA (exiting allows the dependents)
         if (p.k_new) fused_append_finish(p);
         return;
     }
@@ -1047,7 +1056,7 @@ __global__ void __launch_bounds__(GqaCfg<G, NK, NV, QM>::THREADS, MINB) gqa_tc_k
     tc_fence_after();
     const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(smem + C::OFF_TMEM);
     if (warp == EW) {
-        if (p.table) gqa_producer_paged<G, NK, NV, QM>(&kmap, &vmap, p, smem);
+        if (C::SEL || p.table) gqa_producer_paged<G, NK, NV, QM>(&kmap, &vmap, p, smem);
         else if (lane < 2) gqa_producer<G, NK, NV, QM>(&kmap, &vmap, p, smem, lane == 1);
     } else if (warp == EW + 1) {
         if (lane == 0) {
@@ -1104,13 +1113,14 @@ __global__ void __launch_bounds__(1024) seq_order_kernel(const int32_t* seq_lens
 }
 
 // Ragged batches: merge the split records of rows whose sequence had more
-// than one split (single-split rows were written by the decode kernel).
+// than one split (single-split rows were written by the decode kernel). Output
+// rows r*per_seq .. (r+1)*per_seq - 1 belong to sequence r.
 __global__ void __launch_bounds__(128) gqa_ragged_combine_kernel(const float* partials, const int32_t* seq_lens,
-                                                                 int Hq, int P, int span, int S, int D, void* out,
+                                                                 int Hq, int per_seq, int P, int span, int S, int D, void* out,
                                                                  int64_t o_sb, int64_t o_sh, uint32_t flags) {
     const int64_t r = blockIdx.x;
     const int b = static_cast<int>(r / Hq), hq = static_cast<int>(r - static_cast<int64_t>(b) * Hq);
-    const int len = min(max(0, seq_lens[b]), S);
+    const int len = min(max(0, seq_lens[r / per_seq]), S);
     const int ns = len > 0 ? (len + span - 1) / span : 1;
     if (ns <= 1) return;
     const float* first = partials + r * P * static_cast<int64_t>(D + 4);
@@ -1254,6 +1264,13 @@ cudaError_t launch_gqa_g(const CUtensorMap& km, const CUtensorMap& vm, const Gqa
     }
 }
 
+template <int G>
+cudaError_t launch_gqa_mode(int mode, const CUtensorMap& km, const CUtensorMap& vm, const GqaParams& p,
+                            cudaStream_t st) {
+    if (mode == 2) return launch_gqa_g<G, 2>(km, vm, p, st);
+    return mode == 1 ? launch_gqa_g<G, 1>(km, vm, p, st) : launch_gqa_g<G, 0>(km, vm, p, st);
+}
+
 }  // namespace
 
 bool gqa_path_ok(const kvd_decode_desc& d) {
@@ -1271,22 +1288,22 @@ struct GqaPlan {
     size_t order_bytes, rec_bytes;
 };
 
-GqaPlan plan_gqa(const kvd_decode_desc& d, size_t ws_limit) {
+GqaPlan plan_gqa(const kvd_decode_desc& d, size_t ws_limit, bool sel = false) {
     GqaPlan g{};
     const int S = d.max_seq_len > 0 ? d.max_seq_len : 1;
     const int64_t units = static_cast<int64_t>(d.batch) * d.num_kv_heads;
     const int64_t grid = static_cast<int64_t>(device_sm_count()) * kGqaCtas;
     const int s_tiles = (S + 127) / 128;
     // order array + one counter word (fused append)
-    g.order_bytes = (d.seq_lens && d.batch <= 4096) ? ((static_cast<size_t>(d.batch) * 4 + 4 + 255) & ~size_t(255)) : 0;
+    g.order_bytes = (d.seq_lens && d.batch <= 4096 && !sel) ? ((static_cast<size_t>(d.batch) * 4 + 4 + 255) & ~size_t(255)) : 0;
     int span_tiles;
-    if (d.seq_lens) {
+    if (d.seq_lens && !sel) {
         // Ragged: split long sequences into items of at most 16 tiles (fewer if
         // that leaves too few items to balance), longest items dealt first.
         span_tiles = 16;
         while (span_tiles > 1 && units * ((s_tiles + span_tiles - 1) / span_tiles) < 4 * grid) span_tiles /= 2;
         if (span_tiles > s_tiles) span_tiles = s_tiles;
-    } else {
+    } else {  // selections are as long as their budget, but for their last block
         const int P0 = gqa_split_count(d);
         span_tiles = (s_tiles + P0 - 1) / P0;
     }
@@ -1312,8 +1329,8 @@ bool gqa_fused_append_ok(const kvd_decode_desc& d, size_t ws_bytes) {
     return gqa_path_ok(d) && d.seq_lens && plan_gqa(d, ws_bytes).order_bytes > 0;
 }
 
-size_t gqa_workspace_size(const kvd_decode_desc& d) {
-    const GqaPlan g = plan_gqa(d, ~size_t(0));
+size_t gqa_workspace_size(const kvd_decode_desc& d, bool sel) {
+    const GqaPlan g = plan_gqa(d, ~size_t(0), sel);
     return g.order_bytes + g.rec_bytes;
 }
 
@@ -1322,7 +1339,8 @@ cudaError_t launch_gqa_tc(const kvd_decode_desc& d, const void* Q, const int8_t*
                           cudaStream_t st, int* launches, const PagedView* pv, const AppendView* av,
                           SplitRecords* keep_splits) {
     const int G = d.num_q_heads / d.num_kv_heads;
-    const GqaPlan g = plan_gqa(d, ws ? ws_bytes : 0);
+    const bool sel = pv && pv->per_head;
+    const GqaPlan g = plan_gqa(d, ws ? ws_bytes : 0, sel);
     const int S = d.max_seq_len;
     if (av && (pv || !g.order_bytes || !d.seq_lens)) return cudaErrorNotSupported;
     CUtensorMap km, vm;
@@ -1385,13 +1403,13 @@ cudaError_t launch_gqa_tc(const kvd_decode_desc& d, const void* Q, const int8_t*
         if (e != cudaSuccess) return e;
         ++*launches;
     }
-    const bool qi8 = (d.flags & KVD_FLAG_QK_INT8) != 0;
+    const int mode = sel ? 2 : (d.flags & KVD_FLAG_QK_INT8) ? 1 : 0;
     switch (G) {
-        case 1: e = qi8 ? launch_gqa_g<1, 1>(km, vm, p, st) : launch_gqa_g<1, 0>(km, vm, p, st); break;
-        case 2: e = qi8 ? launch_gqa_g<2, 1>(km, vm, p, st) : launch_gqa_g<2, 0>(km, vm, p, st); break;
-        case 4: e = qi8 ? launch_gqa_g<4, 1>(km, vm, p, st) : launch_gqa_g<4, 0>(km, vm, p, st); break;
-        case 8: e = qi8 ? launch_gqa_g<8, 1>(km, vm, p, st) : launch_gqa_g<8, 0>(km, vm, p, st); break;
-        case 16: e = qi8 ? launch_gqa_g<16, 1>(km, vm, p, st) : launch_gqa_g<16, 0>(km, vm, p, st); break;
+        case 1: e = launch_gqa_mode<1>(mode, km, vm, p, st); break;
+        case 2: e = launch_gqa_mode<2>(mode, km, vm, p, st); break;
+        case 4: e = launch_gqa_mode<4>(mode, km, vm, p, st); break;
+        case 8: e = launch_gqa_mode<8>(mode, km, vm, p, st); break;
+        case 16: e = launch_gqa_mode<16>(mode, km, vm, p, st); break;
         default: return cudaErrorInvalidValue;
     }
     if (e != cudaSuccess) return e;
@@ -1406,7 +1424,7 @@ cudaError_t launch_gqa_tc(const kvd_decode_desc& d, const void* Q, const int8_t*
         const int64_t rows = static_cast<int64_t>(d.batch) * d.num_q_heads;
         if (d.seq_lens) {
             gqa_ragged_combine_kernel<<<static_cast<unsigned>(rows), 128, 0, st>>>(
-                p.partials, d.seq_lens, d.num_q_heads, g.P, g.span, S, d.head_dim, out, d.o_stride_b, d.o_stride_h,
+                p.partials, d.seq_lens, d.num_q_heads, sel ? G : d.num_q_heads, g.P, g.span, S, d.head_dim, out, d.o_stride_b, d.o_stride_h,
                 d.flags);
             e = cudaGetLastError();
             if (e == cudaSuccess) ++*launches;

@@ -33,6 +33,7 @@ KVD_STATUS_OK = 0
 KVD_STATUS_WAIT_TIMEOUT = 1
 KVD_STATUS_CACHE_FULL = 2
 KVD_STATUS_BAD_BLOCK = 4
+KVD_STATUS_NO_BLOCKS = 8
 CUDA_ERROR_INVALID_VALUE = 1
 
 c_void_p = ctypes.c_void_p
@@ -139,6 +140,62 @@ class PrefillDesc(ctypes.Structure):
     ]
 
 
+class PagedPlanDesc(ctypes.Structure):
+    """Mirror of ``kvd_paged_plan_desc``."""
+
+    _fields_ = [
+        ("batch", c_int32),
+        ("block_size", c_int32),
+        ("num_blocks", c_int32),
+        ("max_blocks_per_seq", c_int32),
+        ("num_slots", c_int32),
+        ("block_table_stride", c_int64),
+    ]
+
+
+class PagedRowsDesc(ctypes.Structure):
+    """Mirror of ``kvd_paged_rows_desc``."""
+
+    _fields_ = [
+        ("num_tokens", c_int32),
+        ("num_kv_heads", c_int32),
+        ("head_dim", c_int32),
+        ("block_size", c_int32),
+        ("num_blocks", c_int32),
+        ("flags", c_uint32),
+        ("row_stride_t", c_int64),
+        ("row_stride_h", c_int64),
+        ("kv_stride_block", c_int64),
+        ("kv_stride_h", c_int64),
+        ("kv_stride_t", c_int64),
+        ("sc_stride_block", c_int64),
+        ("sc_stride_h", c_int64),
+    ]
+
+
+class BlockSelectDesc(ctypes.Structure):
+    """Mirror of ``kvd_block_select_desc``."""
+
+    _fields_ = [
+        ("batch", c_int32),
+        ("num_q_heads", c_int32),
+        ("num_kv_heads", c_int32),
+        ("head_dim", c_int32),
+        ("block_size", c_int32),
+        ("num_blocks", c_int32),
+        ("max_blocks_per_seq", c_int32),
+        ("budget", c_int32),
+        ("first", c_int32),
+        ("last", c_int32),
+        ("flags", c_uint32),
+        ("seq_lens", c_void_p),
+        ("block_table", c_void_p),
+        ("block_table_stride", c_int64),
+        ("q_stride_b", c_int64),
+        ("q_stride_h", c_int64),
+    ]
+
+
 _SIGNATURES = {
     "solve": (None, [c_void_p] * 6 + [c_int] * 3),
     "kv_int8_split_launch": (c_int, [c_void_p] * 6 + [c_int] * 3 + [c_void_p, c_void_p]),
@@ -174,6 +231,13 @@ _SIGNATURES = {
     "kvd_paged_decode_launch": (c_int, [ctypes.POINTER(PagedDesc)] + [c_void_p] * 7 + [c_size_t, c_void_p]),
     "kvd_paged_append_int8_launch": (c_int, [ctypes.POINTER(PagedDesc), c_void_p, c_void_p, c_int64, c_int64]
                                      + [c_void_p] * 5 + [c_void_p]),
+    "kvd_paged_plan_workspace_size": (c_size_t, [ctypes.POINTER(PagedPlanDesc)]),
+    "kvd_paged_plan_launch": (c_int, [ctypes.POINTER(PagedPlanDesc)] + [c_void_p] * 10 + [c_size_t, c_void_p]),
+    "kvd_paged_write_launch": (c_int, [ctypes.POINTER(PagedRowsDesc)] + [c_void_p] * 9 + [c_void_p]),
+    "kvd_paged_read_launch": (c_int, [ctypes.POINTER(PagedRowsDesc)] + [c_void_p] * 7 + [c_void_p]),
+    "kvd_block_select_launch": (c_int, [ctypes.POINTER(BlockSelectDesc)] + [c_void_p] * 5 + [c_void_p]),
+    "kvd_sparse_workspace_size": (c_size_t, [ctypes.POINTER(PagedDesc)]),
+    "kvd_sparse_decode_launch": (c_int, [ctypes.POINTER(PagedDesc)] + [c_void_p] * 7 + [c_size_t, c_void_p]),
 }
 
 NOALLOC_SCRATCH_BYTES = 512 * 1024
@@ -528,6 +592,232 @@ def paged_append(k_new, v_new, k_pool, v_pool, ks_pool, vs_pool, block_table, se
                                             k_new.stride(1), _ptr(k_pool), _ptr(v_pool), _ptr(ks_pool),
                                             _ptr(vs_pool), _ptr(seq_lens), _stream(stream))
     _check(rc, "kvd_paged_append_int8_launch")
+
+
+# ------------------------------------------- paged serving steps on the GPU
+_ROW_FLAGS = None
+
+
+def _row_flags(dtype) -> int:
+    """KVD_FLAG_Q_* of a row type."""
+    global _ROW_FLAGS
+    if _ROW_FLAGS is None:
+        import torch
+
+        _ROW_FLAGS = {torch.float32: 0, torch.bfloat16: KVD_FLAG_Q_BF16, torch.float16: KVD_FLAG_Q_F16}
+    f = _ROW_FLAGS.get(dtype)
+    if f is None:
+        raise ValueError(f"unsupported row dtype {dtype}")
+    return f
+
+
+def _want(t, dtype, shape, what: str) -> None:
+    """A contiguous tensor of this type and shape."""
+    if t.dtype != dtype or t.shape != shape or not t.is_contiguous():
+        raise ValueError(f"{what} must be contiguous {dtype} of shape {tuple(shape)}, got {t.dtype} {tuple(t.shape)}")
+
+
+def _pool_view(k_pool, ks_pool, layout: str):
+    """(blocks, heads, block_size, head_dim, block stride, head stride, token stride) of a K or V pool."""
+    if layout == "bhtd":
+        NB, H, bs, D = k_pool.shape
+        s_blk, s_h, s_t, s_d = k_pool.stride()
+    elif layout == "bthd":
+        NB, bs, H, D = k_pool.shape
+        s_blk, s_t, s_h, s_d = k_pool.stride()
+    else:
+        raise ValueError(f"unknown pool layout {layout!r}")
+    if ks_pool.shape != (NB, H, bs):
+        raise ValueError(f"scale pool {tuple(ks_pool.shape)} does not match pool {tuple(k_pool.shape)}")
+    if s_d != 1 or ks_pool.stride(2) != 1:
+        raise ValueError("dims and scale tokens must be contiguous")
+    return NB, H, bs, D, s_blk, s_h, s_t
+
+
+def paged_plan(seq_lens, new_lens, block_table, free_blocks, free_count, block_size: int, slot_map, token_starts=None,
+               seq_lens_out=None, free_count_out=None, workspace=None, stream=None):
+    """Block tables and slot maps from request lengths (``kvd_paged_plan_launch``).
+
+    ``seq_lens`` / ``new_lens`` int32 [B] (tokens held, tokens to add; new_lens < 0 ends a request),
+    ``block_table`` int32 [B, max_blocks], ``free_blocks`` int32 [num_blocks] with ``free_count`` int32 [1]
+    ids on it, ``slot_map`` int64 [num_slots]. The table, the free list and, unless other tensors are given for
+    them, the lengths and the count are updated in place. ``workspace``: a zeroed uint8 tensor of 16 bytes that a
+    caller keeps (without one, one is made). Returns (slot_map, token_starts [B + 1])."""
+    import torch
+
+    i32 = torch.int32
+    B = seq_lens.shape[0]
+    if token_starts is None:
+        token_starts = torch.empty(B + 1, dtype=i32, device=seq_lens.device)
+    if seq_lens_out is None:
+        seq_lens_out = seq_lens
+    if free_count_out is None:
+        free_count_out = free_count
+    if workspace is None:
+        workspace = torch.zeros(16, dtype=torch.uint8, device=seq_lens.device)
+    _want(seq_lens, i32, (B,), "seq_lens")
+    _want(new_lens, i32, (B,), "new_lens")
+    _want(seq_lens_out, i32, (B,), "seq_lens_out")
+    _want(token_starts, i32, (B + 1,), "token_starts")
+    _want(free_count, i32, (1,), "free_count")
+    _want(free_count_out, i32, (1,), "free_count_out")
+    if block_table.dtype != i32 or block_table.dim() != 2 or block_table.shape[0] != B or block_table.stride(1) != 1:
+        raise ValueError("block_table must be int32 [B, max_blocks] with contiguous rows")
+    _want(free_blocks, i32, (free_blocks.numel(),), "free_blocks")
+    _want(slot_map, torch.int64, (slot_map.numel(),), "slot_map")
+    desc = PagedPlanDesc(B, block_size, free_blocks.numel(), block_table.shape[1], slot_map.numel(),
+                         block_table.stride(0))
+    rc = lib().kvd_paged_plan_launch(
+        ctypes.byref(desc), seq_lens.data_ptr(), new_lens.data_ptr(), block_table.data_ptr(), free_blocks.data_ptr(),
+        free_count.data_ptr(), slot_map.data_ptr(), token_starts.data_ptr(), seq_lens_out.data_ptr(),
+        free_count_out.data_ptr(), workspace.data_ptr(), workspace.numel(), _stream(stream))
+    _check(rc, "kvd_paged_plan_launch")
+    return slot_map, token_starts
+
+
+def _rows_desc(k, v, slot_map, k_pool, v_pool, ks_pool, vs_pool, layout: str):
+    import torch
+
+    NB, H, bs, D, s_blk, s_h, s_t = _pool_view(k_pool, ks_pool, layout)
+    T = slot_map.shape[0]
+    if k.shape != (T, H, D) or v.shape != k.shape or v.dtype != k.dtype or v.stride() != k.stride() or k.stride(2) != 1:
+        raise ValueError(f"rows must be two [{T}, {H}, {D}] tensors of one type and strides with contiguous dims")
+    if v_pool.stride() != k_pool.stride() or vs_pool.stride() != ks_pool.stride() or v_pool.shape != k_pool.shape \
+            or vs_pool.shape != ks_pool.shape:
+        raise ValueError("K/V pools and their scale pools must share shapes and strides")
+    if k_pool.dtype != torch.int8 or v_pool.dtype != torch.int8 or ks_pool.dtype != torch.float32 \
+            or vs_pool.dtype != torch.float32:
+        raise ValueError("pools are int8, scale pools float32")
+    _want(slot_map, torch.int64, (T,), "slot_map")
+    return PagedRowsDesc(T, H, D, bs, NB, _row_flags(k.dtype), k.stride(0), k.stride(1), s_blk, s_h, s_t,
+                         ks_pool.stride(0), ks_pool.stride(1))
+
+
+def paged_write(k_new, v_new, slot_map, k_pool, v_pool, ks_pool, vs_pool, bounds=None, bound_scale=None,
+                layout: str = "bhtd", stream=None) -> None:
+    """Quantises rows k_new / v_new [T, Hkv, D] (float32, bfloat16 or float16) into the pools' slots
+    ``slot_map`` [T] (-1: skipped). With ``bounds`` int8 [blocks, Hkv, 2, D] and ``bound_scale`` float32
+    [blocks, Hkv] the key bounds of every block written to are kept for :func:`block_select`."""
+    import torch
+
+    desc = _rows_desc(k_new, v_new, slot_map, k_pool, v_pool, ks_pool, vs_pool, layout)
+    if (bounds is None) != (bound_scale is None):
+        raise ValueError("bounds and bound_scale come together")
+    if bounds is not None:
+        _want(bounds, torch.int8, (desc.num_blocks, desc.num_kv_heads, 2, desc.head_dim), "bounds")
+        _want(bound_scale, torch.float32, (desc.num_blocks, desc.num_kv_heads), "bound_scale")
+    rc = lib().kvd_paged_write_launch(ctypes.byref(desc), k_new.data_ptr(), v_new.data_ptr(), slot_map.data_ptr(),
+                                      k_pool.data_ptr(), v_pool.data_ptr(), ks_pool.data_ptr(), vs_pool.data_ptr(),
+                                      _ptr(bounds), _ptr(bound_scale), _stream(stream))
+    _check(rc, "kvd_paged_write_launch")
+
+
+def paged_read(slot_map, k_pool, v_pool, ks_pool, vs_pool, k_out=None, v_out=None, layout: str = "bhtd", dtype=None,
+               stream=None):
+    """Rows of a paged cache by slot as the values that they stand for: returns (k_out, v_out) [T, Hkv, D]
+    (``dtype``, default float32). Slots of -1 read as zeros."""
+    import torch
+
+    if k_out is None or v_out is None:
+        H, D = k_pool.shape[1 if layout == "bhtd" else 2], k_pool.shape[3]
+        shape = (slot_map.shape[0], H, D)
+        k_out = torch.empty(shape, dtype=dtype or torch.float32, device=k_pool.device)
+        v_out = torch.empty_like(k_out)
+    desc = _rows_desc(k_out, v_out, slot_map, k_pool, v_pool, ks_pool, vs_pool, layout)
+    rc = lib().kvd_paged_read_launch(ctypes.byref(desc), slot_map.data_ptr(), k_pool.data_ptr(), v_pool.data_ptr(),
+                                     ks_pool.data_ptr(), vs_pool.data_ptr(), k_out.data_ptr(), v_out.data_ptr(),
+                                     _stream(stream))
+    _check(rc, "kvd_paged_read_launch")
+    return k_out, v_out
+
+
+def block_select(q, bounds, bound_scale, block_table, seq_lens, block_size: int, budget: int, first: int = 1,
+                 last: int = 2, sel_table=None, sel_lens=None, stream=None):
+    """Blocks that one new token per request attends to (``kvd_block_select_launch``): the ``first`` first and
+    ``last`` last blocks and those whose key bounds score highest for ``q`` [B, Hq, D], ``budget`` in all, per
+    KV head. Returns (sel_table int32 [B, Hkv, budget] pool ids, then -1; sel_lens int32 [B, Hkv] tokens)."""
+    import torch
+
+    B, Hq, D = q.shape
+    NB, H, two, Db = bounds.shape
+    if Db != D or Hq % H:
+        raise ValueError(f"shape mismatch q{tuple(q.shape)} bounds{tuple(bounds.shape)}")
+    if q.stride(2) != 1:
+        raise ValueError("dims must be contiguous")
+    if block_table.dtype != torch.int32 or block_table.dim() != 2 or block_table.shape[0] != B \
+            or block_table.stride(1) != 1:
+        raise ValueError("block_table must be int32 [B, max_blocks] with contiguous rows")
+    _want(bounds, torch.int8, (NB, H, 2, D), "bounds")
+    _want(bound_scale, torch.float32, (NB, H), "bound_scale")
+    _want(seq_lens, torch.int32, (B,), "seq_lens")
+    if sel_table is None:
+        sel_table = torch.empty((B, H, budget), dtype=torch.int32, device=q.device)
+    if sel_lens is None:
+        sel_lens = torch.empty((B, H), dtype=torch.int32, device=q.device)
+    _want(sel_table, torch.int32, (B, H, budget), "sel_table")
+    _want(sel_lens, torch.int32, (B, H), "sel_lens")
+    desc = BlockSelectDesc(B, Hq, H, D, block_size, NB, block_table.shape[1], budget, first, last,
+                           _row_flags(q.dtype), seq_lens.data_ptr(), block_table.data_ptr(), block_table.stride(0),
+                           q.stride(0), q.stride(1))
+    rc = lib().kvd_block_select_launch(ctypes.byref(desc), q.data_ptr(), bounds.data_ptr(), bound_scale.data_ptr(),
+                                       sel_table.data_ptr(), sel_lens.data_ptr(), _stream(stream))
+    _check(rc, "kvd_block_select_launch")
+    return sel_table, sel_lens
+
+
+def make_sparse_desc(q, k_pool, ks_pool, out, sel_table, sel_lens, layout: str = "bhtd", softmax_scale: float = 0.0,
+                     partial: bool = False) -> PagedDesc:
+    """Descriptor of a decode over selected blocks: ``sel_table`` int32 [B, Hkv, budget], ``sel_lens`` int32
+    [B, Hkv] (None where only the workspace size is asked for)."""
+    import torch
+
+    B, Hq, D = q.shape
+    NB, H, bs, Dk, s_blk, s_h, s_t = _pool_view(k_pool, ks_pool, layout)
+    if Dk != D or Hq % H:
+        raise ValueError(f"shape mismatch q{tuple(q.shape)} k_pool{tuple(k_pool.shape)}")
+    budget = sel_table.shape[-1]
+    _want(sel_table, torch.int32, (B, H, budget), "sel_table")
+    if sel_lens is not None:
+        _want(sel_lens, torch.int32, (B, H), "sel_lens")
+    if tuple(out.shape) != (B, Hq, D + 4 if partial else D):
+        raise ValueError(f"out must be [{B}, {Hq}, {D + 4 if partial else D}], got {tuple(out.shape)}")
+    if q.stride(2) != 1 or out.stride(2) != 1:
+        raise ValueError("dims must be contiguous")
+    return PagedDesc(B, Hq, H, D, bs, NB, budget, dtype_flags(q, out, partial), _ptr(sel_lens) or sel_table.data_ptr(),
+                     sel_table.data_ptr(), budget, s_blk, s_h, s_t, ks_pool.stride(0), ks_pool.stride(1), q.stride(0),
+                     q.stride(1), out.stride(0), out.stride(1), softmax_scale)
+
+
+def sparse_workspace_size(q, k_pool, sel_table, layout: str = "bhtd") -> int:
+    """Bytes of scratch :func:`sparse_decode` uses for these shapes."""
+    B, Hq, D = q.shape
+    NB, H, bs = (k_pool.shape[i] for i in ((0, 1, 2) if layout == "bhtd" else (0, 2, 1)))
+    p = sel_table.data_ptr()
+    desc = PagedDesc(B, Hq, H, D, bs, NB, sel_table.shape[-1], 0, p, p, sel_table.shape[-1])
+    return int(lib().kvd_sparse_workspace_size(ctypes.byref(desc)))
+
+
+def sparse_decode(q, k_pool, v_pool, ks_pool, vs_pool, sel_table, sel_lens, out=None, layout: str = "bhtd",
+                  softmax_scale: float = 0.0, partial: bool = False, workspace=None, stream=None, out_dtype=None):
+    """INT8 decode attention over selected blocks of a paged cache (:func:`block_select`'s tables); returns
+    ``out`` [B, Hq, D] (or records)."""
+    import torch
+
+    B, Hq, D = q.shape
+    if out is None:
+        out = torch.empty((B, Hq, D + 4 if partial else D), dtype=out_dtype or torch.float32, device=q.device)
+    if v_pool.stride() != k_pool.stride() or vs_pool.stride() != ks_pool.stride() or v_pool.shape != k_pool.shape \
+            or vs_pool.shape != ks_pool.shape:
+        raise ValueError("K/V pools and their scale pools must share shapes and strides")
+    desc = make_sparse_desc(q, k_pool, ks_pool, out, sel_table, sel_lens, layout, softmax_scale, partial)
+    if workspace is None:
+        n = int(lib().kvd_sparse_workspace_size(ctypes.byref(desc)))
+        workspace = torch.empty(max(n, 1), dtype=torch.uint8, device=q.device)
+    rc = lib().kvd_sparse_decode_launch(ctypes.byref(desc), q.data_ptr(), k_pool.data_ptr(), v_pool.data_ptr(),
+                                        ks_pool.data_ptr(), vs_pool.data_ptr(), out.data_ptr(), workspace.data_ptr(),
+                                        workspace.numel(), _stream(stream))
+    _check(rc, "kvd_sparse_decode_launch")
+    return out
 
 
 # ------------------------------------------------------------------ multi-GPU

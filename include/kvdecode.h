@@ -218,6 +218,123 @@ cudaError_t kvd_paged_append_int8_launch(const kvd_paged_desc* desc,
                                          float* k_scale_pool, float* v_scale_pool,
                                          int32_t* seq_lens, cudaStream_t stream);
 
+/* ------------------------------------------------------------------------ */
+/* Paged serving steps on the GPU: block tables and slot maps, slot writes    */
+/* and reads, block selection, decode over selected blocks (no reference      */
+/* counterpart). A slot is block id * block_size + position in the block.     */
+/* ------------------------------------------------------------------------ */
+
+/* Block tables and slot maps from request lengths. Request b holds seq_lens[b]
+ * tokens in the first ceil(seq_lens[b] / block_size) entries of its table row
+ * and gets new_lens[b] more (0 allowed); new_lens[b] < 0 ends the request.
+ * Ended requests' blocks are pushed on the free list (a stack of free_count
+ * ids in `free_blocks`, room for num_blocks), in request and table order, and
+ * their length becomes 0. Then requests are served in order: each new block is
+ * popped from the top of the stack into the request's next table entry, and
+ * the k-th new token overall (all requests' new tokens in order) gets
+ * slot_map[k]. A request is refused as a whole, keeping its length, when it
+ * would pass max_blocks_per_seq blocks or its tokens end past num_slots
+ * (KVD_STATUS_CACHE_FULL), or when the stack runs out in front of it: it needs
+ * blocks and it and the requests before it need more than there are
+ * (KVD_STATUS_NO_BLOCKS). Slots of refused requests' tokens, and slots past
+ * the last token, are -1, and so are slots in a block whose id is outside
+ * [0, num_blocks) (KVD_STATUS_BAD_BLOCK). token_starts [batch + 1] receives
+ * the index of each request's first new token (refused ones count), at most
+ * num_slots. seq_lens_out and free_count_out may be seq_lens and free_count.
+ * At most 8192 requests (cudaErrorInvalidValue above). The workspace of
+ * kvd_paged_plan_workspace_size bytes is zeroed by the caller once; calls
+ * leave it zeroed. Concurrent calls need separate workspaces. */
+#define KVD_STATUS_NO_BLOCKS 8
+typedef struct kvd_paged_plan_desc {
+    int32_t batch, block_size, num_blocks, max_blocks_per_seq;
+    int32_t num_slots;           /* entries of slot_map (>= 0) */
+    int64_t block_table_stride;  /* >= max_blocks_per_seq */
+} kvd_paged_plan_desc;
+size_t kvd_paged_plan_workspace_size(const kvd_paged_plan_desc* desc);
+cudaError_t kvd_paged_plan_launch(const kvd_paged_plan_desc* desc, const int32_t* seq_lens, const int32_t* new_lens,
+                                  int32_t* block_table, int32_t* free_blocks, const int32_t* free_count,
+                                  int64_t* slot_map, int32_t* token_starts, int32_t* seq_lens_out,
+                                  int32_t* free_count_out, void* workspace, size_t workspace_bytes,
+                                  cudaStream_t stream);
+
+/* Rows of a paged cache by slot: row t of [num_tokens][num_kv_heads][head_dim]
+ * belongs to slot_map[t]. Pools as in kvd_paged_desc. flags: element type of
+ * the rows, KVD_FLAG_Q_BF16 or KVD_FLAG_Q_F16 (default fp32). head_dim is at
+ * most 512. */
+typedef struct kvd_paged_rows_desc {
+    int32_t num_tokens, num_kv_heads, head_dim, block_size, num_blocks;
+    uint32_t flags;
+    int64_t row_stride_t, row_stride_h;                 /* k and v rows share strides (elements) */
+    int64_t kv_stride_block, kv_stride_h, kv_stride_t;  /* pools */
+    int64_t sc_stride_block, sc_stride_h;               /* scale pools; token stride 1 */
+} kvd_paged_rows_desc;
+
+/* Quantises rows k_new / v_new with the rule of kvd_append_int8_launch into
+ * their slots. A slot of -1 is skipped; any other slot outside the pools is
+ * skipped and records KVD_STATUS_BAD_BLOCK. A slot must not occur twice.
+ * bounds != NULL also keeps the key bounds that kvd_block_select_launch reads,
+ * bounds [num_blocks][num_kv_heads][2][head_dim] int8 and bound_scale
+ * [num_blocks][num_kv_heads]: for every block written to, over its tokens up
+ * to the last one written, with x_t = code_t * k_scale_t in fp32, hi_d =
+ * max_t x_td, lo_d = min_t x_td and step = max_d max(|hi_d|, |lo_d|) / 127,
+ * codes are clamp(ceil(hi_d / step)) then clamp(floor(lo_d / step)), clamped
+ * to +-127 (step 0: codes 0). A token scale that is not finite makes step NaN
+ * and the codes 0, so that the block is always selected. Tokens of one block
+ * come in order, with no other block's token between them, as
+ * kvd_paged_plan_launch lays them out; places of the block in front of the last
+ * one that the map leaves out hold earlier tokens. */
+cudaError_t kvd_paged_write_launch(const kvd_paged_rows_desc* desc, const void* k_new, const void* v_new,
+                                   const int64_t* slot_map, int8_t* K_pool, int8_t* V_pool, float* k_scale_pool,
+                                   float* v_scale_pool, int8_t* bounds, float* bound_scale, cudaStream_t stream);
+
+/* Reads rows by slot: k_out / v_out row t = code * scale (fp32 product,
+ * rounded once to the rows' type). Slots outside the pools read as zeros; one
+ * that is not -1 records KVD_STATUS_BAD_BLOCK. */
+cudaError_t kvd_paged_read_launch(const kvd_paged_rows_desc* desc, const int64_t* slot_map, const int8_t* K_pool,
+                                  const int8_t* V_pool, const float* k_scale_pool, const float* v_scale_pool,
+                                  void* k_out, void* v_out, cudaStream_t stream);
+
+/* Selects at most `budget` blocks for every (request, KV head) of one new
+ * token per request. The query rows are rounded with the cache's quantiser
+ * (codes c, scale sq); a block's score is an upper bound of q . k over its keys
+ * for the head of the group that could weigh it most, in fp32:
+ *   score = max_g ((sum_d max(c_gd * hi_d, c_gd * lo_d)) * sq_g) * step.
+ * (The integer sum is exact; a NaN score counts as +inf.) Of a request's
+ * n = ceil(seq_lens[b] / block_size) blocks (lengths clamped to the table),
+ * all are selected when n <= budget; else the `first` first ones, the `last`
+ * last ones (first + last <= budget, last >= 1) and the highest scores among
+ * the others, ties to the lower index. sel_table [batch][num_kv_heads][budget]
+ * receives the selected blocks' pool ids in token order, then -1, and sel_lens
+ * [batch][num_kv_heads] the tokens in them: only the last selected block can
+ * be partly filled. A block id outside the pool scores below all others and
+ * records KVD_STATUS_BAD_BLOCK. Tables of up to 262,144 entries per request;
+ * head_dim at most 512. */
+typedef struct kvd_block_select_desc {
+    int32_t batch, num_q_heads, num_kv_heads, head_dim;
+    int32_t block_size, num_blocks, max_blocks_per_seq;
+    int32_t budget, first, last;
+    uint32_t flags;              /* KVD_FLAG_Q_* */
+    const int32_t* seq_lens;     /* device [B] */
+    const int32_t* block_table;  /* device [B][block_table_stride] */
+    int64_t block_table_stride;
+    int64_t q_stride_b, q_stride_h;
+} kvd_block_select_desc;
+cudaError_t kvd_block_select_launch(const kvd_block_select_desc* desc, const void* Q, const int8_t* bounds,
+                                    const float* bound_scale, int32_t* sel_table, int32_t* sel_lens,
+                                    cudaStream_t stream);
+
+/* Decode attention over selected blocks: as kvd_paged_decode_launch, but
+ * every (request, KV head) has its own length and table row:
+ * desc->seq_lens is [batch][num_kv_heads] and desc->block_table
+ * [batch][num_kv_heads][block_table_stride] (sel_lens and sel_table above, with
+ * max_blocks_per_seq = budget). All blocks in front of a row's last one count
+ * as full. KVD_FLAG_QK_INT8 returns cudaErrorNotSupported. */
+size_t kvd_sparse_workspace_size(const kvd_paged_desc* desc);
+cudaError_t kvd_sparse_decode_launch(const kvd_paged_desc* desc,
+                                     const void* Q, const int8_t* K_pool, const int8_t* V_pool,
+                                     const float* k_scale_pool, const float* v_scale_pool, void* out,
+                                     void* workspace, size_t workspace_bytes, cudaStream_t stream);
+
 /* Log-sum-exp combine of `num_parts` partial-record arrays, each [num_heads]
  * records of KVD_PARTIAL_STRIDE(head_dim) floats, part p starting at
  * parts + p*part_stride. Writes normalised rows out[h*out_stride + d] (fp32,
