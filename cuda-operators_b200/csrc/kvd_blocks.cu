@@ -210,6 +210,46 @@ __global__ void __launch_bounds__(1024) plan_kernel(const PlanParams p) {
 }
 
 // ------------------------------------------------------------- rows by slot
+// n / d for n < 2^31, by the multiply-and-shift method of Granlund and
+// Montgomery (1994): mul = floor(2^(31+L) / d) + 1, L = ceil(log2 d).
+struct FastDiv {
+    uint32_t mul, shift;
+    explicit FastDiv(uint32_t d = 1) {
+        uint32_t L = 0;
+        while ((1ull << L) < d) ++L;
+        mul = static_cast<uint32_t>((1ull << (31 + L)) / d + 1);
+        shift = 31 + L;
+    }
+    __device__ __forceinline__ uint32_t div(uint32_t n) const {
+        return static_cast<uint32_t>((static_cast<uint64_t>(n) * mul) >> shift);
+    }
+};
+
+struct RowsParams {
+    kvd_paged_rows_desc d;
+    const void* k_rows;
+    const void* v_rows;
+    void* k_out;
+    void* v_out;
+    const int64_t* slots;
+    int8_t* K;
+    int8_t* V;
+    float* ks;
+    float* vs;
+    int8_t* bounds;      // or nullptr
+    float* bound_scale;
+    int tile;            // tokens whose runs one CTA writes
+    FastDiv by_bs, by_heads;
+    int64_t n_slots;
+};
+
+// Block of a slot, -1 for one outside the pools.
+__device__ __forceinline__ int block_of(const RowsParams& p, int64_t slot) {
+    if (slot < 0 || slot >= p.n_slots) return -1;
+    if (p.n_slots <= 0x7fffffffLL) return static_cast<int>(p.by_bs.div(static_cast<uint32_t>(slot)));
+    return static_cast<int>(slot / p.d.block_size);
+}
+
 template <class T>
 __device__ __forceinline__ float widen(T x);
 template <>
@@ -226,149 +266,323 @@ template <>
 __device__ __forceinline__ __nv_bfloat16 narrow(float x) { return __float2bfloat16_rn(x); }
 template <>
 __device__ __forceinline__ __half narrow(float x) { return __float2half_rn(x); }
+__device__ __forceinline__ uint32_t narrow2(float lo, float hi, __nv_bfloat16) {
+    const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&v);
+}
+__device__ __forceinline__ uint32_t narrow2(float lo, float hi, __half) {
+    const __half2 v = __floats2half2_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&v);
+}
 
-struct RowsParams {
-    kvd_paged_rows_desc d;
-    const void* k_rows;
-    const void* v_rows;
-    void* k_out;
-    void* v_out;
-    const int64_t* slots;
-    int8_t* K;
-    int8_t* V;
-    float* ks;
-    float* vs;
-    int8_t* bounds;      // or nullptr
-    float* bound_scale;
-    int tile;            // tokens whose runs one CTA writes
-};
+// 1.5 * 2^23: adding it rounds a float below 2^22 to a whole number, ties to
+// even, whose low byte is then the sum's low byte.
+constexpr float kRound = 12582912.0f;
 
-// A lane's share of a row of D values: E = D / 32 neighbours (VEC: one load of
-// E elements), or, for other D, every 32nd value (E = 16 covers D <= 512).
-template <int E, bool VEC>
-struct Lane {
-    static __device__ __forceinline__ int at(int lane, int j) { return VEC ? lane * E + j : lane + 32 * j; }
-    static __device__ __forceinline__ bool in(int lane, int j, int D) { return VEC || lane + 32 * j < D; }
+__device__ __forceinline__ uint32_t low_bytes(float2 a, float2 b) {
+    return __byte_perm(__byte_perm(__float_as_uint(a.x), __float_as_uint(a.y), 0x0040),
+                       __byte_perm(__float_as_uint(b.x), __float_as_uint(b.y), 0x0040), 0x5410);
+}
+
+// How a warp holds rows of D values: LPR lanes a row, 8 neighbouring values a
+// lane, 32 / LPR rows at a time (D = 8 * LPR, 16-byte aligned rows); LPR = 0:
+// any D <= 512, one row at a time, every 32nd value a lane.
+template <int LPR>
+struct Rows {
+    static constexpr bool VEC = LPR > 0;
+    static constexpr int LANES = VEC ? LPR : 32;  // lanes a row
+    static constexpr int N = 32 / LANES;          // rows a warp holds
+    static constexpr int E = VEC ? 8 : 16;        // values a lane
+    static __device__ __forceinline__ int at(int l, int j) { return VEC ? l * 8 + j : l + 32 * j; }
+    static __device__ __forceinline__ bool in(int l, int j, int D) { return VEC || l + 32 * j < D; }
     template <class T>
-    static __device__ __forceinline__ void load(const T* row, int lane, int D, float (&x)[E]) {
-        if constexpr (VEC) {
-            struct alignas(sizeof(T) * E < 16 ? sizeof(T) * E : 16) Pack { T v[E]; };
-            const Pack q = *reinterpret_cast<const Pack*>(row + lane * E);
+    static __device__ __forceinline__ void load(const T* row, int l, int D, float (&x)[E]) {
 #pragma unroll
-            for (int j = 0; j < E; ++j) x[j] = widen<T>(q.v[j]);
+        for (int j = 0; j < E; ++j) x[j] = in(l, j, D) ? widen<T>(row[at(l, j)]) : 0.f;
+    }
+    static __device__ __forceinline__ void load_codes(const int8_t* row, int l, int D, float (&x)[E]) {
+        if constexpr (VEC) {
+            const uint2 q = *reinterpret_cast<const uint2*>(row + l * 8);
+            float2 a, b;
+            dequant4(q.x, a, b);
+            x[0] = a.x; x[1] = a.y; x[2] = b.x; x[3] = b.y;
+            dequant4(q.y, a, b);
+            x[4] = a.x; x[5] = a.y; x[6] = b.x; x[7] = b.y;
         } else {
 #pragma unroll
-            for (int j = 0; j < E; ++j) x[j] = in(lane, j, D) ? widen<T>(row[at(lane, j)]) : 0.f;
-        }
-    }
-    static __device__ __forceinline__ void load_codes(const int8_t* row, int lane, int D, float (&x)[E]) {
-        if constexpr (VEC) {
-            struct alignas(E < 16 ? E : 16) Pack { int8_t v[E]; };
-            const Pack q = *reinterpret_cast<const Pack*>(row + lane * E);
-#pragma unroll
-            for (int j = 0; j < E; ++j) x[j] = static_cast<float>(q.v[j]);
-        } else {
-#pragma unroll
-            for (int j = 0; j < E; ++j) x[j] = in(lane, j, D) ? static_cast<float>(row[at(lane, j)]) : 0.f;
+            for (int j = 0; j < E; ++j) x[j] = in(l, j, D) ? static_cast<float>(row[at(l, j)]) : 0.f;
         }
     }
     template <class T>
-    static __device__ __forceinline__ void store(T* row, int lane, int D, const T (&x)[E]) {
-        if constexpr (VEC) {
-            struct alignas(sizeof(T) * E < 16 ? sizeof(T) * E : 16) Pack { T v[E]; };
-            Pack q;
-#pragma unroll
-            for (int j = 0; j < E; ++j) q.v[j] = x[j];
-            *reinterpret_cast<Pack*>(row + lane * E) = q;
+    static __device__ __forceinline__ void store(T* row, int l, int D, const float (&x)[E]) {
+        if constexpr (VEC && sizeof(T) == 4) {
+            float4* out = reinterpret_cast<float4*>(row + l * 8);
+            __stcs(out, make_float4(x[0], x[1], x[2], x[3]));
+            __stcs(out + 1, make_float4(x[4], x[5], x[6], x[7]));
+        } else if constexpr (VEC) {
+            __stcs(reinterpret_cast<uint4*>(row + l * 8),
+                   make_uint4(narrow2(x[0], x[1], T()), narrow2(x[2], x[3], T()), narrow2(x[4], x[5], T()),
+                              narrow2(x[6], x[7], T())));
         } else {
 #pragma unroll
             for (int j = 0; j < E; ++j)
-                if (in(lane, j, D)) row[at(lane, j)] = x[j];
+                if (in(l, j, D)) row[at(l, j)] = narrow<T>(x[j]);
+        }
+    }
+    // x: codes as whole floats
+    static __device__ __forceinline__ void store_codes(int8_t* row, int l, int D, const float (&x)[E]) {
+        if constexpr (VEC) {
+            float2 e[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) e[j] = make_float2(x[2 * j] + kRound, x[2 * j + 1] + kRound);
+            *reinterpret_cast<uint2*>(row + l * 8) = make_uint2(low_bytes(e[0], e[1]), low_bytes(e[2], e[3]));
+        } else {
+#pragma unroll
+            for (int j = 0; j < E; ++j)
+                if (in(l, j, D)) row[at(l, j)] = static_cast<int8_t>(x[j]);
+        }
+    }
+    static __device__ __forceinline__ float amax(float a) {  // over the lanes of a row
+#pragma unroll
+        for (int o = LANES / 2; o > 0; o >>= 1) a = fmaxf(a, __shfl_xor_sync(0xffffffffu, a, o));
+        return a;
+    }
+};
+
+// A lane's 8 neighbouring values of a row, as loaded: words, so that they stay
+// in registers.
+template <class T>
+struct Pack {
+    static constexpr int W = static_cast<int>(sizeof(T)) * 2;  // 32-bit words
+    uint32_t w[W];
+    __device__ __forceinline__ void clear() {
+#pragma unroll
+        for (int j = 0; j < W; ++j) w[j] = 0u;
+    }
+    __device__ __forceinline__ void load(const T* x) {
+#pragma unroll
+        for (int j = 0; j < W; j += 4) {
+            const uint4 q = __ldcs(reinterpret_cast<const uint4*>(x) + j / 4);
+            w[j] = q.x; w[j + 1] = q.y; w[j + 2] = q.z; w[j + 3] = q.w;
+        }
+    }
+    // values 2j and 2j + 1 as floats
+    __device__ __forceinline__ float2 pair(int j) const {
+        if constexpr (sizeof(T) == 4) return make_float2(__uint_as_float(w[2 * j]), __uint_as_float(w[2 * j + 1]));
+        else return widen2(w[j], T());
+    }
+    static __device__ __forceinline__ float2 widen2(uint32_t x, __nv_bfloat16) {
+        return make_float2(__uint_as_float(x << 16), __uint_as_float(x & 0xffff0000u));
+    }
+    static __device__ __forceinline__ float2 widen2(uint32_t x, __half) {
+        return __half22float2(*reinterpret_cast<const __half2*>(&x));
+    }
+    static __device__ __forceinline__ float2 widen2(uint32_t x, float) { return make_float2(__uint_as_float(x), 0.f); }
+    // bits of the largest magnitude as a float: ordered like magnitudes, infinities and NaN on top
+    __device__ __forceinline__ uint32_t most() const {
+        uint32_t m = 0;
+        if constexpr (sizeof(T) == 4) {
+#pragma unroll
+            for (int j = 0; j < W; ++j) m = max(m, w[j] & 0x7fffffffu);
+            return m;
+        } else {
+#pragma unroll
+            for (int j = 0; j < W; ++j) m = __vmaxu2(m, w[j] & 0x7fff7fffu);
+            return __float_as_uint(widen2(max(m & 0xffffu, m >> 16), T()).x);
         }
     }
 };
 
-__device__ __forceinline__ float warp_amax(float a) {
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) a = fmaxf(a, __shfl_xor_sync(0xffffffffu, a, o));
-    return a;
-}
-
-// Quantises a row held across a warp with the rule of kvd_quant.cuh; codes as
-// floats in x. Returns the scale.
-template <int E>
-__device__ __forceinline__ float quantise_lanes(float (&x)[E]) {
+// Any row by the rule of kvd_quant.cuh, divided value by value: x becomes the
+// codes (as floats); returns the scale of the lane's row. All lanes call it.
+template <int LPR>
+__device__ __forceinline__ float quantise_divided(float (&x)[Rows<LPR>::E]) {
+    using R = Rows<LPR>;
     float a = 0.f;
 #pragma unroll
-    for (int j = 0; j < E; ++j) a = fmaxf(a, fabsf(x[j]));
-    a = warp_amax(a);
+    for (int j = 0; j < R::E; ++j) a = fmaxf(a, fabsf(x[j]));  // a NaN is left out
+    a = R::amax(a);
     const float s = a == 0.f ? 0.f : a / 127.0f;
 #pragma unroll
-    for (int j = 0; j < E; ++j) x[j] = a == 0.f ? 0.f : fminf(fmaxf(rintf(x[j] / s), -127.0f), 127.0f);
+    for (int j = 0; j < R::E; ++j) x[j] = a == 0.f ? 0.f : fminf(fmaxf(rintf(x[j] / s), -127.0f), 127.0f);
     return s;
+}
+
+// The K and V rows that a warp holds (LPR lanes each), by the rule of
+// kvd_quant.cuh: code words, the scales of the lane's rows, and in `code` the
+// K codes as floats.
+//  * Even lanes reduce and divide for K, odd lanes for V, so both rows' scales
+//    and reciprocals cost one row's work; 8 or more lanes share a row.
+//  * Every quotient x / s has to be the correctly rounded one (for 16-bit rows
+//    it often lies on a half exactly, where the code depends on its last bit).
+//    With y = 1 / s rounded, q = x y, and twice q += (x - q s) y by fused
+//    multiply-adds, it is (Markstein, IBM J. Res. Dev. 34, 1990: the second
+//    step starts from a neighbour of the quotient and an exact remainder), in
+//    packed pairs and without a branch.
+//  * Rows that are not finite, or so small or large that a remainder or
+//    reciprocal leaves the normal numbers, are divided instead.
+template <class T, int LPR>
+__device__ __forceinline__ void quantise_pair(const Pack<T>& pk, const Pack<T>& pv, float2 (&code)[4], uint2& kw,
+                                              uint2& vw, float& sk, float& sv) {
+    const int lane = threadIdx.x & 31;
+    const bool even = (lane & 1) == 0;
+    const uint32_t mk = pk.most(), mv = pv.most();
+    uint32_t m = max(even ? mk : mv, __shfl_xor_sync(0xffffffffu, even ? mv : mk, 1));
+#pragma unroll
+    for (int o = 2; o < LPR; o <<= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
+    const bool plain = m == 0 || (m >= 0x21800000u && m <= 0x5d800000u);  // 2^-60 .. 2^60
+    if (!__all_sync(0xffffffffu, plain)) {
+        float k[8], v[8];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const float2 a = pk.pair(j), b = pv.pair(j);
+            k[2 * j] = a.x; k[2 * j + 1] = a.y; v[2 * j] = b.x; v[2 * j + 1] = b.y;
+        }
+        sk = quantise_divided<LPR>(k);
+        sv = quantise_divided<LPR>(v);
+        float2 e[8];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            code[j] = make_float2(k[2 * j], k[2 * j + 1]);
+            e[j] = make_float2(k[2 * j] + kRound, k[2 * j + 1] + kRound);
+            e[4 + j] = make_float2(v[2 * j] + kRound, v[2 * j + 1] + kRound);
+        }
+        kw = make_uint2(low_bytes(e[0], e[1]), low_bytes(e[2], e[3]));
+        vw = make_uint2(low_bytes(e[4], e[5]), low_bytes(e[6], e[7]));
+        return;
+    }
+    // m / 127 by one such step: equal to the division for all 2^23 significands
+    const float a = __uint_as_float(m), y127 = 1.0f / 127.0f;
+    float s = a * y127;
+    s = fmaf(fmaf(s, -127.0f, a), y127, s);
+    const float y = m == 0 ? 0.f : 1.0f / s;
+    const int mine = lane & ~1;
+    sk = __shfl_sync(0xffffffffu, s, mine);
+    sv = __shfl_sync(0xffffffffu, s, mine + 1);
+    const float yk = __shfl_sync(0xffffffffu, y, mine), yv = __shfl_sync(0xffffffffu, y, mine + 1);
+    auto quotient = [](float2 x, float2 ns, float2 yy) {  // rounded to a whole number, plus kRound
+        float2 q = __fmul2_rn(x, yy);
+        q = __ffma2_rn(__ffma2_rn(q, ns, x), yy, q);
+        q = __ffma2_rn(__ffma2_rn(q, ns, x), yy, q);
+        return __fadd2_rn(q, make_float2(kRound, kRound));
+    };
+    float2 e[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        e[j] = quotient(pk.pair(j), make_float2(-sk, -sk), make_float2(yk, yk));
+        code[j] = __fadd2_rn(e[j], make_float2(-kRound, -kRound));
+    }
+    kw = make_uint2(low_bytes(e[0], e[1]), low_bytes(e[2], e[3]));
+#pragma unroll
+    for (int j = 0; j < 4; ++j) e[j] = quotient(pv.pair(j), make_float2(-sv, -sv), make_float2(yv, yv));
+    vw = make_uint2(low_bytes(e[0], e[1]), low_bytes(e[2], e[3]));
 }
 
 constexpr int kRowWarps = 4;
 
 // Writes: a run is a maximal stretch of tokens in one block, skipped tokens
-// (slot -1) aside. One CTA per (tile of tokens, KV head) takes the runs that start in its tile, one
-// after the other, its warps the rows of a run in turn. A run's key bounds
-// are then the maximum and minimum over values that the CTA holds in
-// registers (and the block's earlier tokens, read from the pool), so the
-// bounds cost no second pass and no exchange between CTAs. Bound: HBM.
-template <class T, int E, bool VEC>
-__global__ void __launch_bounds__(32 * kRowWarps) write_kernel(const RowsParams p) {
-    using L = Lane<E, VEC>;
-    extern __shared__ float write_smem[];  // [kRowWarps][2][D] bounds of each warp
-    __shared__ int s_end, s_before;
-    __shared__ int s_odd[kRowWarps];
+// (slot -1) aside. One CTA per (tile of tokens, KV head) takes the runs that
+// start in its tile, one after the other, its warps the rows of a run in turn.
+// A run's key bounds are then the maximum and minimum over values that the CTA
+// holds in registers (and the block's earlier tokens, read from the pool), so
+// the bounds cost no second pass and no exchange between CTAs. Heads are the
+// fast index of the grid: CTAs that run together read neighbouring rows. The
+// first rows are loaded beside the slots, before the run is known.
+// Bound: HBM for long maps, the chain of dependent loads for short ones.
+template <class T, int LPR, int W>
+__global__ void __launch_bounds__(32 * W, LPR ? 24 / W : 1) write_kernel(const RowsParams p) {
+    using R = Rows<LPR>;
+    constexpr int E = R::E, STEP = W * R::N;
+    extern __shared__ float write_smem[];  // [W][2][D] bounds of each warp
+    __shared__ int s_odd[W];
     grid_dependency_wait();
     allow_dependents();
     const kvd_paged_rows_desc& d = p.d;
     const int D = d.head_dim, bs = d.block_size, nt = d.num_tokens;
-    const int tiles = (nt + p.tile - 1) / p.tile;
-    const int h = blockIdx.x / tiles;
-    const int t0 = (blockIdx.x - h * tiles) * p.tile, t1 = min(nt, t0 + p.tile);
+    const int tile = static_cast<int>(p.by_heads.div(blockIdx.x));
+    const int h = blockIdx.x - tile * d.num_kv_heads;
+    const int t0 = tile * p.tile, t1 = min(nt, t0 + p.tile);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int64_t n_slots = static_cast<int64_t>(d.num_blocks) * bs;
-    auto block_at = [&](int t) -> int {  // block of token t, -1 for none
-        const int64_t s = p.slots[t];
-        return s >= 0 && s < n_slots ? static_cast<int>(s / bs) : -1;
+    const int sub = lane / R::LANES, l = lane % R::LANES;
+    const T* k_rows = static_cast<const T*>(p.k_rows) + h * d.row_stride_h;
+    const T* v_rows = static_cast<const T*>(p.v_rows) + h * d.row_stride_h;
+    const int r0 = warp * R::N + sub;  // this lane's row of the STEP that the CTA holds
+    // V's rows and codes lie at fixed distances from K's
+    const int64_t v_rows_at = reinterpret_cast<const char*>(v_rows) - reinterpret_cast<const char*>(k_rows);
+    const int64_t v_codes_at = p.V - p.K;
+    const int64_t v_scales_at = reinterpret_cast<char*>(p.vs) - reinterpret_cast<char*>(p.ks);
+    Pack<T> pk, pv;  // this lane's part of the next row
+    auto fetch = [&](const T* row) {
+        if constexpr (R::VEC) {
+            pk.load(row);
+            pv.load(reinterpret_cast<const T*>(reinterpret_cast<const char*>(row) + v_rows_at));
+        }
     };
-    auto odd_slot = [&](int t) {  // a skipped slot that is not -1
-        if (h == 0 && p.slots[t] != -1) record_status(KVD_STATUS_BAD_BLOCK);
-    };
+    auto slot_at = [&](int v) -> int64_t { return v >= 0 && v < nt ? p.slots[v] : -1; };
     bool fresh = false;  // the next token with a slot is known to start a run
     int t = t0;
-    while (t < t1) {
-        const int blk = block_at(t);
-        if (blk < 0) {
-            if (threadIdx.x == 0) odd_slot(t);
-            ++t;
+    while (t < t1) {  // every warp finds the same runs
+        const int64_t here = slot_at(t + lane), s0 = __shfl_sync(0xffffffffu, here, 0);
+        int64_t ahead = slot_at(t + 1 + lane);
+        const T* next_row = k_rows + static_cast<int64_t>(t + r0) * d.row_stride_t + l * 8;
+        if (t + r0 < nt) fetch(next_row);
+        else if constexpr (R::VEC) { pk.clear(); pv.clear(); }
+        const int blk = block_of(p, s0);
+        if (blk < 0) {  // on to the next token with a slot
+            const bool valid = here >= 0 && here < p.n_slots;
+            const uint32_t some = __ballot_sync(0xffffffffu, valid);
+            const int skip = some ? __ffs(some) - 1 : 32;
+            if (lane < skip && here != -1) record_status(KVD_STATUS_BAD_BLOCK);
+            t += skip;
             continue;
         }
-        // end of the run: the first later token of another block
-        if (threadIdx.x == 0) { s_end = nt; s_before = -1; }
-        __syncthreads();
-        for (int u = t + 1;; u += blockDim.x) {
-            const int v = u + static_cast<int>(threadIdx.x);
-            const int at = v < nt ? block_at(v) : -2;
-            const bool other = at != blk && at != -1;
-            if (other) atomicMin(&s_end, v);
-            if (__syncthreads_or(other)) break;
-        }
-        const int end = min(s_end, nt);
-        if (!fresh) {  // the token with a slot before t: a run that started in an earlier tile is its CTA's
-            for (int u = t - 1;; u -= blockDim.x) {
-                const int v = u - static_cast<int>(threadIdx.x);
-                const bool found = v < 0 || block_at(v) >= 0;
-                if (found && v >= 0) atomicMax(&s_before, v);
-                if (__syncthreads_or(found)) break;
+        const int64_t base = static_cast<int64_t>(blk) * bs;
+        const int first = static_cast<int>(s0 - base);
+        // up to the first later token of another block; `last` is the run's last token with a slot
+        int end = t + 1, last = t, held = 1;
+        bool plain = true;
+        for (;;) {
+            const int v = end + lane;
+            const bool valid = ahead >= 0 && ahead < p.n_slots;
+            const bool mine = valid && ahead >= base && ahead < base + bs;
+            if (ahead != -1 && !valid) record_status(KVD_STATUS_BAD_BLOCK);
+            const uint32_t stop = __ballot_sync(0xffffffffu, v >= nt || (valid && !mine));
+            const uint32_t before = stop ? (1u << (__ffs(stop) - 1)) - 1u : 0xffffffffu;
+            const uint32_t mb = __ballot_sync(0xffffffffu, mine) & before;
+            plain &= (__ballot_sync(0xffffffffu, mine && ahead != s0 + (v - t)) & before) == 0;
+            held += __popc(mb);
+            if (mb) last = end + 31 - __clz(mb);
+            if (stop) {
+                end += __ffs(stop) - 1;
+                break;
             }
+            end += 32;
+            ahead = slot_at(end + lane);
+        }
+        plain &= held == last - t + 1;  // token i of the run has place first + i - t
+        if (!fresh) {
+            // A run that started in an earlier tile is its CTA's: look for the token with a slot before
+            // t (tokens of a block come in order, so place 0 starts a run), 128 tokens at a time
+            // because refused requests leave long gaps.
             fresh = true;
-            if (s_before >= 0 && block_at(s_before) == blk) {
+            bool goes_on = false;
+            for (int u = t - 1; first > 0 && u >= 0; u -= 128) {
+                int64_t s[4];
+#pragma unroll
+                for (int x = 0; x < 4; ++x) s[x] = slot_at(u - 32 * x - lane);
+                uint32_t found = 0;
+#pragma unroll
+                for (int x = 0; x < 4; ++x) {
+                    if (found) break;
+                    const bool valid = s[x] >= 0 && s[x] < p.n_slots;
+                    found = __ballot_sync(0xffffffffu, valid);
+                    if (found)
+                        goes_on = __shfl_sync(0xffffffffu, s[x] >= base && s[x] < base + bs, __ffs(found) - 1);
+                }
+                if (found) break;
+            }
+            if (goes_on) {
                 t = end;
-                __syncthreads();
                 continue;
             }
         }
@@ -376,157 +590,258 @@ __global__ void __launch_bounds__(32 * kRowWarps) write_kernel(const RowsParams 
         bool odd = false;  // a token scale that is not finite
 #pragma unroll
         for (int j = 0; j < E; ++j) { hi[j] = -INFINITY; lo[j] = INFINITY; }
-        const int64_t kv0 = blk * d.kv_stride_block + h * d.kv_stride_h;
-        const int64_t sc0 = blk * d.sc_stride_block + h * d.sc_stride_h;
-        auto place = [&](int i) { return static_cast<int>(p.slots[i] - static_cast<int64_t>(blk) * bs); };
-        auto earlier = [&](int o) {  // bounds take in a token that an earlier call wrote
-            float c[E];
-            L::load_codes(p.K + kv0 + o * d.kv_stride_t, lane, D, c);
-            const float s = p.ks[sc0 + o];
+        int8_t* K = p.K + blk * d.kv_stride_block + h * d.kv_stride_h;
+        int8_t* V = p.V + blk * d.kv_stride_block + h * d.kv_stride_h;
+        float* ks = p.ks + blk * d.sc_stride_block + h * d.sc_stride_h;
+        float* vs = p.vs + blk * d.sc_stride_block + h * d.sc_stride_h;
+        auto widen_bounds = [&](const float (&c)[E], float s) {
             odd |= !isfinite(s);
 #pragma unroll
-            for (int j = 0; j < E; ++j) { hi[j] = fmaxf(hi[j], c[j] * s); lo[j] = fminf(lo[j], c[j] * s); }
-        };
-        if (p.bounds)
-            for (int o = warp, first = place(t); o < first; o += kRowWarps) earlier(o);
-        for (int i = t + warp; i < end; i += kRowWarps) {
-            if (block_at(i) < 0) {
-                if (lane == 0) odd_slot(i);
-                continue;
+            for (int j = 0; j < E; ++j) {
+                const float v = c[j] * s;
+                hi[j] = fmaxf(hi[j], v);
+                lo[j] = fminf(lo[j], v);
             }
-            const int o = place(i);
-            const int64_t row = i * d.row_stride_t + h * d.row_stride_h;
-            float xk[E], xv[E];
-            L::load(static_cast<const T*>(p.k_rows) + row, lane, D, xk);
-            L::load(static_cast<const T*>(p.v_rows) + row, lane, D, xv);
-            const float sk = quantise_lanes<E>(xk), sv = quantise_lanes<E>(xv);
-            int8_t ck[E], cv[E];
+        };
+        // the rows in hand, to code row `ko` with scale `so`
+        auto put = [&](bool in, int8_t* ko, float* so) {
+            if constexpr (R::VEC) {
+                float2 code[4];
+                uint2 kw, vw;
+                float sk, sv;
+                quantise_pair<T, LPR>(pk, pv, code, kw, vw, sk, sv);
+                if (!in) return;
+                *reinterpret_cast<uint2*>(ko) = kw;
+                *reinterpret_cast<uint2*>(ko + v_codes_at) = vw;
+                if (l == 0) {
+                    *so = sk;
+                    *reinterpret_cast<float*>(reinterpret_cast<char*>(so) + v_scales_at) = sv;
+                }
+                if (p.bounds) {
+                    odd |= !isfinite(sk);
 #pragma unroll
-            for (int j = 0; j < E; ++j) { ck[j] = static_cast<int8_t>(xk[j]); cv[j] = static_cast<int8_t>(xv[j]); }
-            L::store(p.K + kv0 + o * d.kv_stride_t, lane, D, ck);
-            L::store(p.V + kv0 + o * d.kv_stride_t, lane, D, cv);
-            if (lane == 0) { p.ks[sc0 + o] = sk; p.vs[sc0 + o] = sv; }
-            if (!p.bounds) continue;
-            odd |= !isfinite(sk);
-#pragma unroll
-            for (int j = 0; j < E; ++j) { hi[j] = fmaxf(hi[j], xk[j] * sk); lo[j] = fminf(lo[j], xk[j] * sk); }
-            int next = i + 1;  // places left out up to the next token with a slot
-            while (next < end && block_at(next) < 0) ++next;
-            if (next < end)
-                for (int u = o + 1, stop = place(next); u < stop; ++u) earlier(u);
+                    for (int j = 0; j < 4; ++j) {
+                        const float2 v = __fmul2_rn(code[j], make_float2(sk, sk));
+                        hi[2 * j] = fmaxf(hi[2 * j], v.x);
+                        lo[2 * j] = fminf(lo[2 * j], v.x);
+                        hi[2 * j + 1] = fmaxf(hi[2 * j + 1], v.y);
+                        lo[2 * j + 1] = fminf(lo[2 * j + 1], v.y);
+                    }
+                }
+            }
+        };
+        auto earlier = [&](int o) {  // a token that an earlier call wrote
+            float c[E];
+            R::load_codes(K + o * d.kv_stride_t, l, D, c);
+            widen_bounds(c, ks[o]);
+        };
+        if (p.bounds) {
+#pragma unroll 2
+            for (int o = r0; o < first; o += STEP) earlier(o);
+        }
+        if (R::VEC && plain) {  // consecutive places: pointers advance, the next rows load meanwhile
+            int8_t* ko = K + static_cast<int64_t>(first + r0) * d.kv_stride_t + l * 8;
+            float* so = ks + first + r0;
+            for (int left = last - t + 1; left > 0; left -= STEP) {
+                const Pack<T> ck = pk, cv = pv;
+                const bool more = left - STEP > r0;
+                next_row += STEP * d.row_stride_t;
+                Pack<T> nk = ck, nv = cv;
+                if (more) {
+                    nk.load(next_row);
+                    nv.load(reinterpret_cast<const T*>(reinterpret_cast<const char*>(next_row) + v_rows_at));
+                }
+                put(left > r0, ko, so);
+                pk = nk;
+                pv = nv;
+                ko += STEP * d.kv_stride_t;
+                so += STEP;
+            }
+        } else {
+            for (int i0 = t; i0 <= last; i0 += STEP) {
+                const int i = i0 + r0;
+                const int64_t s = i <= last ? p.slots[i] : -1;
+                const bool in = s >= base && s < base + bs;
+                const int o = in ? static_cast<int>(s - base) : 0;
+                const int64_t row = static_cast<int64_t>(min(i, nt - 1)) * d.row_stride_t;
+                if constexpr (R::VEC) {
+                    fetch(k_rows + row + l * 8);
+                    put(in, K + o * d.kv_stride_t + l * 8, ks + o);
+                } else {
+                    float xk[E], xv[E];
+                    R::load(k_rows + row, l, D, xk);
+                    R::load(v_rows + row, l, D, xv);
+                    const float sk = quantise_divided<LPR>(xk), sv = quantise_divided<LPR>(xv);
+                    if (!in) continue;
+                    R::store_codes(K + o * d.kv_stride_t, l, D, xk);
+                    R::store_codes(V + o * d.kv_stride_t, l, D, xv);
+                    if (l == 0) { ks[o] = sk; vs[o] = sv; }
+                    if (p.bounds) widen_bounds(xk, sk);
+                }
+            }
+        }
+        if (p.bounds && !plain) {  // places left out between the run's tokens hold earlier ones
+            for (int i = t + r0; i < last; i += STEP) {
+                const int64_t s = p.slots[i];
+                if (s < base || s >= base + bs) continue;
+                int next = i + 1;
+                while (next < last && (p.slots[next] < base || p.slots[next] >= base + bs)) ++next;
+                for (int o = static_cast<int>(s - base) + 1, stop = static_cast<int>(p.slots[next] - base); o < stop; ++o)
+                    earlier(o);
+            }
         }
         if (p.bounds) {
-            float* mine = write_smem + warp * 2 * D;
+            __syncwarp();
 #pragma unroll
-            for (int j = 0; j < E; ++j)
-                if (L::in(lane, j, D)) { mine[L::at(lane, j)] = hi[j]; mine[D + L::at(lane, j)] = lo[j]; }
-            if (lane == 0) s_odd[warp] = odd;
-            __syncthreads();
+            for (int x = R::LANES; x < 32; x <<= 1) {  // over the rows that the warp held
+                odd |= __shfl_xor_sync(0xffffffffu, odd, x);
+#pragma unroll
+                for (int j = 0; j < E; ++j) {
+                    hi[j] = fmaxf(hi[j], __shfl_xor_sync(0xffffffffu, hi[j], x));
+                    lo[j] = fminf(lo[j], __shfl_xor_sync(0xffffffffu, lo[j], x));
+                }
+            }
+            if constexpr (W > 1) {
+                float* mine = write_smem + warp * 2 * D;
+                if (sub == 0) {
+#pragma unroll
+                    for (int j = 0; j < E; ++j)
+                        if (R::in(l, j, D)) { mine[R::at(l, j)] = hi[j]; mine[D + R::at(l, j)] = lo[j]; }
+                }
+                if (lane == 0) s_odd[warp] = odd;
+                __syncthreads();
+            }
             if (warp == 0) {
                 float most = 0.f;
 #pragma unroll
                 for (int j = 0; j < E; ++j) {
-                    if (!L::in(lane, j, D)) { hi[j] = lo[j] = 0.f; continue; }
-                    for (int w = 1; w < kRowWarps; ++w) {
-                        hi[j] = fmaxf(hi[j], write_smem[w * 2 * D + L::at(lane, j)]);
-                        lo[j] = fminf(lo[j], write_smem[w * 2 * D + D + L::at(lane, j)]);
-                        odd |= s_odd[w] != 0;
+                    if (!R::in(l, j, D)) { hi[j] = lo[j] = 0.f; continue; }
+#pragma unroll
+                    for (int w = 1; w < W; ++w) {
+                        hi[j] = fmaxf(hi[j], write_smem[w * 2 * D + R::at(l, j)]);
+                        lo[j] = fminf(lo[j], write_smem[w * 2 * D + D + R::at(l, j)]);
                     }
                     most = fmaxf(most, fmaxf(fabsf(hi[j]), fabsf(lo[j])));
                 }
-                odd = __any_sync(0xffffffffu, odd);
-                most = warp_amax(most);
+                for (int w = 1; w < W; ++w) odd |= s_odd[w] != 0;
+                most = R::amax(most);
                 const float step = odd ? NAN : most / 127.0f;
-                int8_t up[E], down[E];
+                int8_t* bound = p.bounds + (static_cast<int64_t>(blk) * d.num_kv_heads + h) * 2 * D;
+                // the upper row as the negated lower row of the negated values; with two or more
+                // rows of lanes a warp, the first rounds one and the second the other
+                auto lower = [&](float (&x)[E], bool flip, int8_t* out) {
 #pragma unroll
-                for (int j = 0; j < E; ++j) {
-                    const bool some = step > 0.f;
-                    up[j] = some ? static_cast<int8_t>(fminf(fmaxf(ceilf(hi[j] / step), -127.f), 127.f)) : 0;
-                    down[j] = some ? static_cast<int8_t>(fminf(fmaxf(floorf(lo[j] / step), -127.f), 127.f)) : 0;
+                    for (int j = 0; j < E; ++j) {
+                        const float v = flip ? -x[j] : x[j];
+                        const float f = step > 0.f ? fminf(fmaxf(floorf(v / step), -127.f), 127.f) : 0.f;
+                        x[j] = flip ? -f : f;
+                    }
+                    R::store_codes(out, l, D, x);
+                };
+                if constexpr (R::N > 1) {
+#pragma unroll
+                    for (int j = 0; j < E; ++j) lo[j] = sub == 0 ? hi[j] : lo[j];
+                    if (sub < 2) lower(lo, sub == 0, bound + sub * D);
+                } else {
+                    lower(hi, true, bound);
+                    lower(lo, false, bound + D);
                 }
-                const int64_t bh = static_cast<int64_t>(blk) * d.num_kv_heads + h;
-                L::store(p.bounds + bh * 2 * D, lane, D, up);
-                L::store(p.bounds + bh * 2 * D + D, lane, D, down);
-                if (lane == 0) p.bound_scale[bh] = step;
+                if (lane == 0) p.bound_scale[static_cast<int64_t>(blk) * d.num_kv_heads + h] = step;
             }
+            if constexpr (W > 1) __syncthreads();  // the bounds rows are written again
         }
         t = end;
-        __syncthreads();  // s_end and the bounds rows are written again
     }
 }
 
-template <class T, int E, bool VEC>
+// Reads: rows (token, head) in order, a warp holding R::N neighbours, four
+// times over so that its loads are in flight together. Bound: HBM.
+template <class T, int LPR>
 __global__ void __launch_bounds__(32 * kRowWarps) read_kernel(const RowsParams p) {
-    using L = Lane<E, VEC>;
+    using R = Rows<LPR>;
+    constexpr int E = R::E, U = R::VEC ? 2 : 1;
     grid_dependency_wait();
     allow_dependents();
     const kvd_paged_rows_desc& d = p.d;
-    const int D = d.head_dim, bs = d.block_size, H = d.num_kv_heads;
-    const int lane = threadIdx.x & 31;
-    const int64_t n_slots = static_cast<int64_t>(d.num_blocks) * bs;
-    const int64_t rows = static_cast<int64_t>(d.num_tokens) * H;
-    for (int64_t r = static_cast<int64_t>(blockIdx.x) * kRowWarps + (threadIdx.x >> 5); r < rows;
-         r += static_cast<int64_t>(gridDim.x) * kRowWarps) {
-        const int t = static_cast<int>(r / H), h = static_cast<int>(r - static_cast<int64_t>(t) * H);
-        const int64_t slot = p.slots[t];
-        float xk[E], xv[E];
+    const int D = d.head_dim, H = d.num_kv_heads;
+    const int lane = threadIdx.x & 31, sub = lane / R::LANES, l = lane % R::LANES;
+    const uint32_t rows = static_cast<uint32_t>(d.num_tokens) * H;
+    const uint32_t step = gridDim.x * kRowWarps * (R::N * U);
+    for (uint32_t r0 = (blockIdx.x * kRowWarps + (threadIdx.x >> 5)) * (R::N * U); r0 < rows; r0 += step) {
+        float xk[U][E], xv[U][E];
+        int64_t row[U];
 #pragma unroll
-        for (int j = 0; j < E; ++j) xk[j] = xv[j] = 0.f;
-        if (slot >= 0 && slot < n_slots) {
-            const int64_t blk = slot / bs, o = slot - blk * bs;
+        for (int u = 0; u < U; ++u) {
+            const uint32_t r = r0 + u * R::N + sub;
+            row[u] = -1;
+#pragma unroll
+            for (int j = 0; j < E; ++j) xk[u][j] = xv[u][j] = 0.f;
+            if (r >= rows) continue;
+            const int t = static_cast<int>(p.by_heads.div(r)), h = static_cast<int>(r) - t * H;
+            row[u] = t * d.row_stride_t + h * d.row_stride_h;
+            const int64_t slot = p.slots[t];
+            const int blk = block_of(p, slot);
+            if (blk < 0) {
+                if (slot != -1 && h == 0 && l == 0) record_status(KVD_STATUS_BAD_BLOCK);
+                continue;
+            }
+            const int64_t o = slot - static_cast<int64_t>(blk) * d.block_size;
             const int64_t at = blk * d.kv_stride_block + h * d.kv_stride_h + o * d.kv_stride_t;
             const int64_t sc = blk * d.sc_stride_block + h * d.sc_stride_h + o;
-            L::load_codes(p.K + at, lane, D, xk);
-            L::load_codes(p.V + at, lane, D, xv);
+            R::load_codes(p.K + at, l, D, xk[u]);
+            R::load_codes(p.V + at, l, D, xv[u]);
             const float sk = p.ks[sc], sv = p.vs[sc];
 #pragma unroll
-            for (int j = 0; j < E; ++j) { xk[j] *= sk; xv[j] *= sv; }
-        } else if (slot != -1 && h == 0 && lane == 0) {
-            record_status(KVD_STATUS_BAD_BLOCK);
+            for (int j = 0; j < E; ++j) { xk[u][j] *= sk; xv[u][j] *= sv; }
         }
-        T yk[E], yv[E];
 #pragma unroll
-        for (int j = 0; j < E; ++j) { yk[j] = narrow<T>(xk[j]); yv[j] = narrow<T>(xv[j]); }
-        const int64_t row = t * d.row_stride_t + h * d.row_stride_h;
-        L::store(static_cast<T*>(p.k_out) + row, lane, D, yk);
-        L::store(static_cast<T*>(p.v_out) + row, lane, D, yv);
+        for (int u = 0; u < U; ++u) {
+            if (row[u] < 0) continue;
+            R::store(static_cast<T*>(p.k_out) + row[u], l, D, xk[u]);
+            R::store(static_cast<T*>(p.v_out) + row[u], l, D, xv[u]);
+        }
     }
 }
 
-template <class T, int E, bool VEC>
+template <class T, int LPR>
 cudaError_t launch_rows(const RowsParams& p, bool write, cudaStream_t st) {
     const kvd_paged_rows_desc& d = p.d;
+    const int64_t rows = static_cast<int64_t>(d.num_tokens) * d.num_kv_heads;
     if (write) {
         const int64_t grid = static_cast<int64_t>((d.num_tokens + p.tile - 1) / p.tile) * d.num_kv_heads;
-        if (grid > 0x7fffffffLL) return cudaErrorInvalidValue;
-        return launch_after(write_kernel<T, E, VEC>, static_cast<unsigned>(grid), 32 * kRowWarps,
+        if (LPR && rows <= 24 * device_sm_count())
+            return launch_after(write_kernel<T, LPR, 1>, static_cast<unsigned>(grid), 32, 0, 1, st, p);
+        return launch_after(write_kernel<T, LPR, kRowWarps>, static_cast<unsigned>(grid), 32 * kRowWarps,
                             sizeof(float) * kRowWarps * 2 * d.head_dim, 1, st, p);
     }
-    const int64_t rows = static_cast<int64_t>(d.num_tokens) * d.num_kv_heads;
-    int64_t grid = (rows + kRowWarps - 1) / kRowWarps;
+    const int64_t per = kRowWarps * Rows<LPR>::N * (LPR ? 2 : 1);
+    int64_t grid = (rows + per - 1) / per;
     const int64_t most = static_cast<int64_t>(device_sm_count()) * 16;
     if (grid > most) grid = most;
-    return launch_after(read_kernel<T, E, VEC>, static_cast<unsigned>(grid), 32 * kRowWarps, 0, 1, st, p);
+    return launch_after(read_kernel<T, LPR>, static_cast<unsigned>(grid), 32 * kRowWarps, 0, 1, st, p);
 }
 
 template <class T>
 cudaError_t launch_rows_t(const RowsParams& p, bool write, bool vec, cudaStream_t st) {
-    if (vec && p.d.head_dim == 64) return launch_rows<T, 2, true>(p, write, st);
-    if (vec && p.d.head_dim == 128) return launch_rows<T, 4, true>(p, write, st);
-    if (vec && p.d.head_dim == 256) return launch_rows<T, 8, true>(p, write, st);
-    return launch_rows<T, 16, false>(p, write, st);
+    if (vec && p.d.head_dim == 64) return launch_rows<T, 8>(p, write, st);
+    if (vec && p.d.head_dim == 128) return launch_rows<T, 16>(p, write, st);
+    if (vec && p.d.head_dim == 256) return launch_rows<T, 32>(p, write, st);
+    return launch_rows<T, 0>(p, write, st);
 }
 
 bool rows_ok(const kvd_paged_rows_desc* d) {
     if (!d || d->num_tokens < 0 || d->num_kv_heads < 1 || d->head_dim < 1 || d->head_dim > 512) return false;
     if (d->block_size < 1 || d->num_blocks < 1) return false;
+    if (static_cast<int64_t>(d->num_tokens) * d->num_kv_heads > 0x7fff0000LL) return false;
     return d->flags == 0 || d->flags == KVD_FLAG_Q_BF16 || d->flags == KVD_FLAG_Q_F16;
 }
 
 cudaError_t rows_call(RowsParams& p, const void* a, const void* b, bool write, cudaStream_t st) {
     const kvd_paged_rows_desc& d = p.d;
-    // Vector access: a lane's E = D/32 elements are one load of at most 16
-    // bytes (two for fp32 rows of 256), so every row starts on 16 bytes.
+    p.by_bs = FastDiv(d.block_size);
+    p.by_heads = FastDiv(d.num_kv_heads);
+    p.n_slots = static_cast<int64_t>(d.num_blocks) * d.block_size;
+    // vector access: every row of values and of codes starts on 16 bytes
     const int64_t es = d.flags ? 2 : 4;
     auto al = [](const void* x) { return (reinterpret_cast<uintptr_t>(x) & 15) == 0; };
     const bool vec = al(a) && al(b) && al(p.K) && al(p.V) && al(p.bounds) &&
@@ -637,7 +952,7 @@ __global__ void __launch_bounds__(kSelThreads) select_kernel(const SelectParams 
         float x[16];
 #pragma unroll
         for (int j = 0; j < 16; ++j) x[j] = lane + 32 * j < D ? load_q(p.Q, q0 + lane + 32 * j, d.flags) : 0.f;
-        const float s = quantise_lanes<16>(x);
+        const float s = quantise_divided<0>(x);
 #pragma unroll
         for (int j = 0; j < 16; ++j) {
             const int at = lane + 32 * j;
@@ -899,9 +1214,10 @@ extern "C" cudaError_t kvd_paged_write_launch(const kvd_paged_rows_desc* desc, c
         (bounds == nullptr) != (bound_scale == nullptr))
         return cudaErrorInvalidValue;
     RowsParams p{*desc, k_new, v_new, nullptr, nullptr, slot_map, K_pool, V_pool, k_scale_pool, v_scale_pool,
-                 bounds, bound_scale, 1};
-    const int64_t per = static_cast<int64_t>(desc->num_tokens) * desc->num_kv_heads / (16 * device_sm_count());
-    p.tile = static_cast<int>(per < 1 ? 1 : per > 32 ? 32 : per);
+                 bounds, bound_scale, 1, FastDiv(), FastDiv(), 0};
+    const int64_t per = static_cast<int64_t>(desc->num_tokens) * desc->num_kv_heads / (24 * device_sm_count());
+    const int most = desc->block_size < 64 ? 64 : desc->block_size > 256 ? 256 : desc->block_size;
+    p.tile = static_cast<int>(per < 1 ? 1 : per > most ? most : per);
     return rows_call(p, k_new, v_new, true, stream);
 }
 
@@ -916,7 +1232,7 @@ extern "C" cudaError_t kvd_paged_read_launch(const kvd_paged_rows_desc* desc, co
         return cudaErrorInvalidValue;
     RowsParams p{*desc, nullptr, nullptr, k_out, v_out, slot_map, const_cast<int8_t*>(K_pool),
                  const_cast<int8_t*>(V_pool), const_cast<float*>(k_scale_pool), const_cast<float*>(v_scale_pool),
-                 nullptr, nullptr, 1};
+                 nullptr, nullptr, 1, FastDiv(), FastDiv(), 0};
     return rows_call(p, k_out, v_out, false, stream);
 }
 
