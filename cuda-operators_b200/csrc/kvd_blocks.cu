@@ -5,8 +5,7 @@
 // No reference counterpart (the reference's caches are dense and complete,
 // kv_cache/new_kvint8.cu:83-84). This file must not be built with fast-math:
 // the quantiser's divisions are IEEE.
-#include <cooperative_groups.h>
-
+#include "kvd_blocks.cuh"
 #include "kvd_common.cuh"
 #include "kvd_decode.cuh"
 #include "kvd_quant.cuh"
@@ -14,11 +13,8 @@
 namespace kvd {
 namespace {
 
-namespace cg = cooperative_groups;
-
 template <class... A, class... B>
-cudaError_t launch_after(void (*kern)(A...), unsigned grid, unsigned block, size_t smem, unsigned cluster,
-                         cudaStream_t st, B... args) {
+cudaError_t launch_after(void (*kern)(A...), unsigned grid, unsigned block, size_t smem, cudaStream_t st, B... args) {
     // Programmatic dependent of the kernel before it; every kernel here waits
     // (griddepcontrol.wait) before its first global access.
     cudaLaunchConfig_t cfg{};
@@ -26,15 +22,11 @@ cudaError_t launch_after(void (*kern)(A...), unsigned grid, unsigned block, size
     cfg.blockDim = dim3(block, 1, 1);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = st;
-    cudaLaunchAttribute attr[2];
+    cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = 1;
-    attr[1].id = cudaLaunchAttributeClusterDimension;
-    attr[1].val.clusterDim.x = cluster;
-    attr[1].val.clusterDim.y = 1;
-    attr[1].val.clusterDim.z = 1;
     cfg.attrs = attr;
-    cfg.numAttrs = cluster > 1 ? 2 : 1;
+    cfg.numAttrs = 1;
     return cudaLaunchKernelEx(&cfg, kern, args...);
 }
 
@@ -408,17 +400,26 @@ __device__ __forceinline__ float quantise_divided(float (&x)[Rows<LPR>::E]) {
     return s;
 }
 
+// Quotients x / s, correctly rounded, then rounded to whole numbers, plus
+// kRound; ns = -s, yy = 1 / s rounded. q = x y, and twice q += (x - q s) y by
+// fused multiply-adds (Markstein, IBM J. Res. Dev. 34, 1990: the second step
+// starts from a neighbour of the quotient and an exact remainder). For
+// magnitudes whose remainders and reciprocals are normal numbers.
+__device__ __forceinline__ float2 quotient(float2 x, float2 ns, float2 yy) {
+    float2 q = __fmul2_rn(x, yy);
+    q = __ffma2_rn(__ffma2_rn(q, ns, x), yy, q);
+    q = __ffma2_rn(__ffma2_rn(q, ns, x), yy, q);
+    return __fadd2_rn(q, make_float2(kRound, kRound));
+}
+
 // The K and V rows that a warp holds (LPR lanes each), by the rule of
 // kvd_quant.cuh: code words, the scales of the lane's rows, and in `code` the
 // K codes as floats.
 //  * Even lanes reduce and divide for K, odd lanes for V, so both rows' scales
 //    and reciprocals cost one row's work; 8 or more lanes share a row.
 //  * Every quotient x / s has to be the correctly rounded one (for 16-bit rows
-//    it often lies on a half exactly, where the code depends on its last bit).
-//    With y = 1 / s rounded, q = x y, and twice q += (x - q s) y by fused
-//    multiply-adds, it is (Markstein, IBM J. Res. Dev. 34, 1990: the second
-//    step starts from a neighbour of the quotient and an exact remainder), in
-//    packed pairs and without a branch.
+//    it often lies on a half exactly, where the code depends on its last bit):
+//    quotient() gives it in packed pairs and without a branch.
 //  * Rows that are not finite, or so small or large that a remainder or
 //    reciprocal leaves the normal numbers, are divided instead.
 template <class T, int LPR>
@@ -460,12 +461,6 @@ __device__ __forceinline__ void quantise_pair(const Pack<T>& pk, const Pack<T>& 
     sk = __shfl_sync(0xffffffffu, s, mine);
     sv = __shfl_sync(0xffffffffu, s, mine + 1);
     const float yk = __shfl_sync(0xffffffffu, y, mine), yv = __shfl_sync(0xffffffffu, y, mine + 1);
-    auto quotient = [](float2 x, float2 ns, float2 yy) {  // rounded to a whole number, plus kRound
-        float2 q = __fmul2_rn(x, yy);
-        q = __ffma2_rn(__ffma2_rn(q, ns, x), yy, q);
-        q = __ffma2_rn(__ffma2_rn(q, ns, x), yy, q);
-        return __fadd2_rn(q, make_float2(kRound, kRound));
-    };
     float2 e[4];
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
@@ -810,15 +805,15 @@ cudaError_t launch_rows(const RowsParams& p, bool write, cudaStream_t st) {
     if (write) {
         const int64_t grid = static_cast<int64_t>((d.num_tokens + p.tile - 1) / p.tile) * d.num_kv_heads;
         if (LPR && rows <= 24 * device_sm_count())
-            return launch_after(write_kernel<T, LPR, 1>, static_cast<unsigned>(grid), 32, 0, 1, st, p);
+            return launch_after(write_kernel<T, LPR, 1>, static_cast<unsigned>(grid), 32, 0, st, p);
         return launch_after(write_kernel<T, LPR, kRowWarps>, static_cast<unsigned>(grid), 32 * kRowWarps,
-                            sizeof(float) * kRowWarps * 2 * d.head_dim, 1, st, p);
+                            sizeof(float) * kRowWarps * 2 * d.head_dim, st, p);
     }
     const int64_t per = kRowWarps * Rows<LPR>::N * (LPR ? 2 : 1);
     int64_t grid = (rows + per - 1) / per;
     const int64_t most = static_cast<int64_t>(device_sm_count()) * 16;
     if (grid > most) grid = most;
-    return launch_after(read_kernel<T, LPR>, static_cast<unsigned>(grid), 32 * kRowWarps, 0, 1, st, p);
+    return launch_after(read_kernel<T, LPR>, static_cast<unsigned>(grid), 32 * kRowWarps, 0, st, p);
 }
 
 template <class T>
@@ -856,308 +851,293 @@ cudaError_t rows_call(RowsParams& p, const void* a, const void* b, bool write, c
 }
 
 // --------------------------------------------------------------------- select
-// A block's bound codes are one row [hi | lo] of 2D int8 values and a query
-// head's one row [max(c, 0) | min(c, 0)], so the bound of q . k is a plain dot
-// product of 2D integers: sum_d max(c hi, c lo) = sum c+ hi + sum c- lo. It
-// runs as int8 m16n8k32 products, 16 blocks by 8 heads; 8 products a tile
-// against 4 KB read (head_dim 128) leave HBM the bound, not the tensor pipe,
-// so a warp keeps its tile in registers: lane (g, t) loads 16-byte pieces of
-// rows g and g+8, and the order in which dims meet the product's k index is
-// the same for both operands, hence free.
-struct SelectParams {
-    kvd_block_select_desc d;
-    const void* Q;
-    const int8_t* bounds;
-    const float* bound_scale;
-    int32_t* sel_table;
-    int32_t* sel_lens;
-    int cap;  // keys a CTA holds
-};
+// Two kernels: scores (kvd_score_tc.cu, or score_any_kernel for other shapes),
+// spread evenly over the GPU whatever the lengths are, then one CTA per
+// (request, KV head) that finds the threshold and writes the table.
 
-constexpr int kSelThreads = 256;
-constexpr int kSelWarps = kSelThreads / 32;
-constexpr uint32_t kAlways = 0xffffffffu;  // key of a block that is always selected; above every score's
-
-// Order-preserving key of a score: larger is better; NaN counts as +inf, -0 as +0.
-__device__ __forceinline__ uint32_t score_key(float s) {
-    if (isnan(s)) s = INFINITY;
-    const uint32_t u = __float_as_uint(s + 0.f);
-    return u & 0x80000000u ? ~u : u | 0x80000000u;
-}
-
-__device__ __forceinline__ void mma_s8(int (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
-                                       uint32_t b1) {
-    asm volatile(
-        "mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-        : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3])
-        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
-}
-
-__device__ __forceinline__ uint4 ld_stream(const void* p) {
-    uint4 v;
-    asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];"
-                 : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
-                 : "l"(p));
-    return v;
-}
-
-// Bytes of one query row in shared memory: the pad keeps two rows' 16-byte
-// pieces on different banks.
-__host__ __device__ __forceinline__ int sel_q_stride(int D) { return 2 * D + 64; }
-
-// ND = D / 32: 64-byte pieces of a bound row; 0: any D, without tensor cores.
-template <int ND>
-__global__ void __launch_bounds__(kSelThreads) select_kernel(const SelectParams p) {
-    extern __shared__ __align__(16) uint8_t sel_smem[];
-    __shared__ uint32_t hist[4][256];
-    __shared__ uint32_t s_range[2][kSelWarps], s_span[2];
-    __shared__ uint32_t s_scan[kSelWarps], s_pick[3];
-    __shared__ uint32_t s_count[2][kSelWarps], s_total[2];
-    const cg::cluster_group cl = cg::this_cluster();
-    const unsigned ranks = cl.num_blocks(), rank = cl.block_rank();
+// Scores for any head_dim: a warp a CTA, query codes in shared memory.
+__global__ void __launch_bounds__(32) score_any_kernel(const SelectParams p) {
+    extern __shared__ int8_t any_smem[];  // [G][D] codes, padded to 4, then [G] scales
     const kvd_block_select_desc& d = p.d;
-    const int D = d.head_dim, H = d.num_kv_heads, G = d.num_q_heads / H;
-    const int row = blockIdx.x / ranks;
-    const int b = row / H, h = row - b * H;
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    uint32_t* keys = reinterpret_cast<uint32_t*>(sel_smem);
-    uint8_t* s_q = sel_smem + 4 * p.cap;
-    const int GP = (G + 7) & ~7, QS = sel_q_stride(D);
-    float* s_sq = reinterpret_cast<float*>(s_q + GP * QS);
+    const int D = d.head_dim, H = d.num_kv_heads, G = d.num_q_heads / H, lane = threadIdx.x;
+    float* scale = reinterpret_cast<float*>(any_smem + ((G * D + 3) & ~3));
+    const int chunks = (d.max_blocks_per_seq + 15) / 16, items = d.batch * H * chunks;
     grid_dependency_wait();
     allow_dependents();
-
-    const int bs = d.block_size, MB = d.max_blocks_per_seq, k = d.budget;
-    const int64_t len64 = min(static_cast<int64_t>(max(0, d.seq_lens[b])), static_cast<int64_t>(MB) * bs);
-    const int len = static_cast<int>(len64), n = static_cast<int>((len64 + bs - 1) / bs);
-    const int32_t* table = d.block_table + b * d.block_table_stride;
-    int32_t* out = p.sel_table + static_cast<int64_t>(row) * k;
-    if (rank == 0 && tid == 0) p.sel_lens[row] = n <= k ? len : (k - n) * bs + len;
-    if (n <= k) {  // everything: nothing to score (the same for every CTA of the cluster)
-        if (rank == 0)
-            for (int i = tid; i < k; i += kSelThreads) {
-                const int id = i < n ? table[i] : -1;
-                if (i < n && (id < 0 || id >= d.num_blocks)) record_status(KVD_STATUS_BAD_BLOCK);
-                out[i] = id;
-            }
-        return;
-    }
-
-    // query rows: codes split by sign, zero rows up to a multiple of 8 heads
-    for (int i = tid; i < GP * QS / 4; i += kSelThreads) reinterpret_cast<uint32_t*>(s_q)[i] = 0u;
-    for (int i = tid; i < 4 * 256; i += kSelThreads) (&hist[0][0])[i] = 0u;
-    __syncthreads();
-    for (int g = warp; g < G; g += kSelWarps) {
-        const int64_t q0 = b * d.q_stride_b + static_cast<int64_t>(h * G + g) * d.q_stride_h;
-        float x[16];
+    for (int it = blockIdx.x; it < items; it += gridDim.x) {  // 16 blocks of a row each
+        ScoreItem I;
+        I.row = it / chunks;
+        I.i0 = (it - I.row * chunks) * 16;
+        I.b = I.row / H;
+        I.h = I.row - I.b * H;
+        int n;
+        select_len(d, I.b, n);
+        if (n <= d.budget || I.i0 >= n) continue;
+        I.m = min(16, n - I.i0);
+        __syncwarp();
+        for (int g = 0; g < G; ++g) {
+            const int64_t q0 = I.b * d.q_stride_b + static_cast<int64_t>(I.h * G + g) * d.q_stride_h;
+            float x[16];
 #pragma unroll
-        for (int j = 0; j < 16; ++j) x[j] = lane + 32 * j < D ? load_q(p.Q, q0 + lane + 32 * j, d.flags) : 0.f;
-        const float s = quantise_divided<0>(x);
+            for (int j = 0; j < 16; ++j) x[j] = lane + 32 * j < D ? load_q(p.Q, q0 + lane + 32 * j, d.flags) : 0.f;
+            const float s = quantise_divided<0>(x);
 #pragma unroll
-        for (int j = 0; j < 16; ++j) {
-            const int at = lane + 32 * j;
-            if (at < D) {
-                const int c = static_cast<int>(x[j]);
-                s_q[g * QS + at] = static_cast<uint8_t>(static_cast<int8_t>(max(c, 0)));
-                s_q[g * QS + D + at] = static_cast<uint8_t>(static_cast<int8_t>(min(c, 0)));
-            }
+            for (int j = 0; j < 16; ++j)
+                if (lane + 32 * j < D) any_smem[g * D + lane + 32 * j] = static_cast<int8_t>(x[j]);
+            if (lane == 0) scale[g] = s;
         }
-        if (lane == 0) s_sq[g] = s;
-    }
-    __syncthreads();
-
-    // scores of this CTA's blocks [lo, lo + m)
-    const int per = ((n + static_cast<int>(ranks) - 1) / static_cast<int>(ranks) + 15) & ~15;
-    const int lo = min(n, static_cast<int>(rank) * per), m = min(n, lo + per) - lo;
-    uint32_t kmin = 0xffffffffu, kmax = 0u;
-    auto put = [&](int i, int id, float best) {  // block lo + i, the largest head product (without step)
-        uint32_t key;
-        const int at = lo + i;
-        if (at < d.first || at >= n - d.last) {
-            key = kAlways;
-        } else {
-            key = id < 0 ? 0u : score_key(best * p.bound_scale[static_cast<int64_t>(id) * H + h]);
-            kmin = min(kmin, key);
-            kmax = max(kmax, key);
-        }
-        keys[i] = key;
-    };
-    auto block_id = [&](int i) -> int {  // pool id of block lo + i, -1 when outside the pool
-        if (i >= m) return -1;
-        const int id = table[lo + i];
-        if (id >= 0 && id < d.num_blocks) return id;
-        record_status(KVD_STATUS_BAD_BLOCK);
-        return -1;
-    };
-    if constexpr (ND > 0) {
-        const int g = lane >> 2, t = lane & 3;
-        int ids = block_id(warp * 16 + (lane & 15));
-        for (int i0 = warp * 16; i0 < m; i0 += kSelWarps * 16) {
-            const int next = block_id(i0 + kSelWarps * 16 + (lane & 15));
-            const int id0 = __shfl_sync(0xffffffffu, ids, g), id1 = __shfl_sync(0xffffffffu, ids, g + 8);
-            uint4 a0[ND], a1[ND];
-            const int8_t* r0 = p.bounds + (static_cast<int64_t>(max(id0, 0)) * H + h) * (2 * D) + 16 * t;
-            const int8_t* r1 = p.bounds + (static_cast<int64_t>(max(id1, 0)) * H + h) * (2 * D) + 16 * t;
-#pragma unroll
-            for (int j = 0; j < ND; ++j) { a0[j] = ld_stream(r0 + 64 * j); a1[j] = ld_stream(r1 + 64 * j); }
-            float best0 = -INFINITY, best1 = -INFINITY;
-            for (int g0 = 0; g0 < GP; g0 += 8) {
-                int c[4] = {0, 0, 0, 0};
-                const uint8_t* qr = s_q + (g0 + g) * QS + 16 * t;
-#pragma unroll
-                for (int j = 0; j < ND; ++j) {
-                    const uint4 q = *reinterpret_cast<const uint4*>(qr + 64 * j);
-                    mma_s8(c, a0[j].x, a1[j].x, a0[j].y, a1[j].y, q.x, q.y);
-                    mma_s8(c, a0[j].z, a1[j].z, a0[j].w, a1[j].w, q.z, q.w);
-                }
-#pragma unroll
-                for (int x = 0; x < 2; ++x) {
-                    const int hd = g0 + 2 * t + x;
-                    if (hd < G) {
-                        float v0 = static_cast<float>(c[x]) * s_sq[hd], v1 = static_cast<float>(c[2 + x]) * s_sq[hd];
-                        if (isnan(v0)) v0 = INFINITY;
-                        if (isnan(v1)) v1 = INFINITY;
-                        best0 = fmaxf(best0, v0);
-                        best1 = fmaxf(best1, v1);
-                    }
-                }
-            }
-#pragma unroll
-            for (int o = 1; o < 4; o <<= 1) {
-                best0 = fmaxf(best0, __shfl_xor_sync(0xffffffffu, best0, o));
-                best1 = fmaxf(best1, __shfl_xor_sync(0xffffffffu, best1, o));
-            }
-            if (t == 0 && i0 + g < m) put(i0 + g, id0, best0);
-            if (t == 1 && i0 + g + 8 < m) put(i0 + g + 8, id1, best1);
-            ids = next;
-        }
-    } else {
-        for (int i = warp; i < m; i += kSelWarps) {
-            const int id = block_id(i);
-            const int8_t* r = p.bounds + (static_cast<int64_t>(max(id, 0)) * H + h) * (2 * D);
+        __syncwarp();
+        const int32_t* table = d.block_table + I.b * d.block_table_stride + I.i0;
+        uint32_t* keys = p.keys + static_cast<int64_t>(I.row) * d.max_blocks_per_seq + I.i0;
+        for (int i = 0; i < I.m; ++i) {
+            const int id = pool_id(d, table, i);
+            const int64_t at = static_cast<int64_t>(max(id, 0)) * H + I.h;
+            const int8_t* r = p.bounds + at * (2 * D);
             float best = -INFINITY;
-            for (int gg = 0; gg < G; ++gg) {
+            for (int g = 0; g < G; ++g) {
                 int acc = 0;
-                for (int x = lane; x < 2 * D; x += 32) acc += static_cast<int8_t>(s_q[gg * QS + x]) * r[x];
-                acc = __reduce_add_sync(0xffffffffu, acc);
-                float v = static_cast<float>(acc) * s_sq[gg];
-                if (isnan(v)) v = INFINITY;
-                best = fmaxf(best, v);
+                for (int x = lane; x < D; x += 32) {
+                    const int c = any_smem[g * D + x];
+                    acc += c * (c > 0 ? r[x] : r[D + x]);
+                }
+                const float v = static_cast<float>(__reduce_add_sync(0xffffffffu, acc)) * scale[g];
+                best = fmaxf(best, isnan(v) ? INFINITY : v);
             }
-            if (lane == 0) put(i, id, best);
+            if (lane == 0) keys[i] = id < 0 ? 0u : score_key(best * p.bound_scale[at]);
         }
     }
-
-    // Threshold of the `need` best scored keys: 8-bit radix passes from the
-    // highest bit in which any two keys differ, over all CTAs of the cluster.
-    kmin = __reduce_min_sync(0xffffffffu, kmin);
-    kmax = __reduce_max_sync(0xffffffffu, kmax);
-    if (lane == 0) { s_range[0][warp] = kmin; s_range[1][warp] = kmax; }
-    __syncthreads();
-    if (tid == 0) {
-        for (int w = 1; w < kSelWarps; ++w) {
-            kmin = min(kmin, s_range[0][w]);
-            kmax = max(kmax, s_range[1][w]);
-        }
-        s_span[0] = kmin;
-        s_span[1] = kmax;
-    }
-    cl.sync();
-    kmin = 0xffffffffu;
-    kmax = 0u;
-    for (unsigned r = 0; r < ranks; ++r) {
-        const uint32_t* sp = cl.map_shared_rank(s_span, r);
-        kmin = min(kmin, sp[0]);
-        kmax = max(kmax, sp[1]);
-    }
-    uint32_t need = static_cast<uint32_t>(k - d.first - d.last);
-    int top = kmin == kmax ? 0 : 32 - __clz(kmin ^ kmax);
-    uint32_t mask = top >= 32 ? 0u : 0xffffffffu << top;
-    uint32_t prefix = kmax & mask;
-    for (int round = 0; top > 0 && need > 0; ++round) {
-        const int sh = max(0, top - 8);
-        const uint32_t bins = 1u << (top - sh);
-        for (int i = tid; i < m; i += kSelThreads) {
-            const uint32_t key = keys[i];
-            if (key != kAlways && (key & mask) == prefix) atomicAdd(&hist[round][(key >> sh) & (bins - 1)], 1u);
-        }
-        cl.sync();
-        uint32_t x = 0;  // keys in bin 255 - tid
-        for (unsigned r = 0; r < ranks; ++r) x += cl.map_shared_rank(&hist[round][0], r)[255 - tid];
-        uint32_t upto = x;
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const uint32_t y = __shfl_up_sync(0xffffffffu, upto, o);
-            if (lane >= o) upto += y;
-        }
-        if (lane == 31) s_scan[warp] = upto;
-        __syncthreads();
-        for (int w = 0; w < warp; ++w) upto += s_scan[w];
-        if (upto >= need && upto - x < need) {
-            s_pick[0] = 255 - tid;
-            s_pick[1] = upto - x;
-            s_pick[2] = x;
-        }
-        __syncthreads();
-        const uint32_t bin = s_pick[0], in_bin = s_pick[2];
-        need -= s_pick[1];
-        prefix |= bin << sh;
-        mask |= (bins - 1) << sh;
-        top = sh;
-        if (in_bin == need) break;  // the whole bin is selected
-    }
-
-    // Selected: always, above the threshold, or among the first `need` at it.
-    // Each warp owns a stretch of the CTA's blocks, so places follow from counts.
-    const int seg = ((m + kSelWarps - 1) / kSelWarps + 31) & ~31;
-    const int s0 = min(m, warp * seg), s1 = min(m, s0 + seg);
-    uint32_t above = 0, equal = 0;
-    for (int i0 = s0; i0 < s1; i0 += 32) {
-        const uint32_t key = i0 + lane < s1 ? keys[i0 + lane] : 0u;
-        const bool in = i0 + lane < s1;
-        above += __popc(__ballot_sync(0xffffffffu, in && (key == kAlways || (key & mask) > prefix)));
-        equal += __popc(__ballot_sync(0xffffffffu, in && key != kAlways && (key & mask) == prefix));
-    }
-    if (lane == 0) { s_count[0][warp] = above; s_count[1][warp] = equal; }
-    __syncthreads();
-    if (tid == 0) {
-        uint32_t a = 0, e = 0;
-        for (int w = 0; w < kSelWarps; ++w) { a += s_count[0][w]; e += s_count[1][w]; }
-        s_total[0] = a;
-        s_total[1] = e;
-    }
-    cl.sync();
-    above = equal = 0;
-    for (unsigned r = 0; r < rank; ++r) {
-        const uint32_t* tt = cl.map_shared_rank(s_total, r);
-        above += tt[0];
-        equal += tt[1];
-    }
-    for (int w = 0; w < warp; ++w) { above += s_count[0][w]; equal += s_count[1][w]; }
-    const uint32_t below = (1u << lane) - 1u;
-    for (int i0 = s0; i0 < s1; i0 += 32) {
-        const bool in = i0 + lane < s1;
-        const uint32_t key = in ? keys[i0 + lane] : 0u;
-        const bool up = in && (key == kAlways || (key & mask) > prefix);
-        const bool eq = in && key != kAlways && (key & mask) == prefix;
-        const uint32_t ub = __ballot_sync(0xffffffffu, up), eb = __ballot_sync(0xffffffffu, eq);
-        const uint32_t e = equal + __popc(eb & below);
-        if (up || (eq && e < need)) out[above + __popc(ub & below) + min(e, need)] = table[lo + i0 + lane];
-        above += __popc(ub);
-        equal += __popc(eb);
-    }
-    cl.sync();  // the other CTAs have read this one's shared memory
 }
 
-template <int ND>
-cudaError_t launch_select(const SelectParams& p, int cluster, size_t smem, cudaStream_t st) {
-    auto kern = select_kernel<ND>;
-    static PerDeviceOnce once;
-    const cudaError_t e = once.run(
-        [kern] { return cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, 200 * 1024); });
-    if (e != cudaSuccess) return e;
-    const int64_t grid = static_cast<int64_t>(p.d.batch) * p.d.num_kv_heads * cluster;
-    return launch_after(kern, static_cast<unsigned>(grid), kSelThreads, smem, static_cast<unsigned>(cluster), st, p);
+// Threshold and table of one row per CTA. The keys are binned evenly between
+// the lowest and highest finite score, which puts the threshold into a bin of
+// few keys as a rule; their ranks then give it exactly. Where the bin holds
+// too many (equal or very uneven scores), 8-bit radix passes over the keys
+// find it instead. Each warp owns a stretch of the row's blocks, so the places
+// of its blocks follow from counts. A row of up to kPickKept blocks is held in
+// registers, keys and pool ids, from one load to the end; longer rows are read
+// again from L2. Bound: latency, three loads in a row and seven barriers.
+constexpr int kPickThreads = 256;
+constexpr int kPickWarps = kPickThreads / 32;
+constexpr int kPickEach = 16;
+constexpr int kPickKept = kPickThreads * kPickEach;
+constexpr int kPickList = 512;
+
+struct PickShared {
+    uint32_t hist[kPickThreads];
+    uint32_t list[kPickList];
+    uint32_t range[2][kPickWarps];
+    uint32_t scan[kPickWarps];
+    uint32_t pick[3], found[2], listed;
+    uint32_t count[2][kPickWarps];
+};
+
+// The bin (a thread each) that the need-th best key lies in: pick = bin, keys above it, keys in it.
+__device__ __forceinline__ void find_bin(PickShared& s, uint32_t need) {
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, bin = kPickThreads - 1 - tid;
+    const uint32_t mine = s.hist[bin];
+    uint32_t upto = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const uint32_t y = __shfl_up_sync(0xffffffffu, upto, o);
+        if (lane >= o) upto += y;
+    }
+    if (lane == 31) s.scan[warp] = upto;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < kPickWarps; ++w)
+        if (w < warp) upto += s.scan[w];
+    if (upto >= need && upto - mine < need) {
+        s.pick[0] = bin;
+        s.pick[1] = upto - mine;
+        s.pick[2] = mine;
+    }
+    __syncthreads();
+}
+
+template <bool KEPT>
+__device__ __forceinline__ void pick_row(const SelectParams& p, PickShared& s, int row, int n, const int32_t* table) {
+    const kvd_block_select_desc& d = p.d;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const uint32_t* all = p.keys + static_cast<int64_t>(row) * d.max_blocks_per_seq;
+    int32_t* out = p.sel_table + static_cast<int64_t>(row) * d.budget;
+    const int seg = ((n + kPickWarps - 1) / kPickWarps + 31) & ~31;  // KEPT: at most 32 * kPickEach
+    const int s0 = min(n, warp * seg), s1 = min(n, s0 + seg);
+    const int lo = d.first, hi = n - d.last;  // scored blocks: [lo, hi); the others are always selected
+    uint32_t key[kPickEach];
+    int id[kPickEach];
+    if constexpr (KEPT) {
+#pragma unroll
+        for (int j = 0; j < kPickEach; ++j) {
+            const int i = s0 + 32 * j + lane;
+            key[j] = i < s1 ? all[i] : 0u;
+            id[j] = i < s1 ? table[i] : 0;
+        }
+    }
+    // fn(block, key, pool id) for this warp's blocks in order, all lanes together; past the end block = n
+    auto each = [&](auto fn, bool with_id) {
+        if constexpr (KEPT) {
+#pragma unroll
+            for (int j = 0; j < kPickEach; ++j) {
+                if (s0 + 32 * j >= s1) break;
+                const int i = s0 + 32 * j + lane;
+                fn(i < s1 ? i : n, key[j], id[j]);
+            }
+        } else {
+            for (int i = s0 + lane; i - lane < s1; i += 32)
+                fn(i < s1 ? i : n, i < s1 ? all[i] : 0u, with_id && i < s1 ? table[i] : 0);
+        }
+    };
+    constexpr uint32_t kInf = 0xff800000u, kNegInf = 0x007fffffu;  // keys of +inf and -inf
+    uint32_t kmin = 0xffffffffu, kmax = 0u;
+    each([&](int i, uint32_t k, int) {
+        if (i >= lo && i < hi && k < kInf && k > kNegInf) {
+            kmin = min(kmin, k);
+            kmax = max(kmax, k);
+        }
+    }, false);
+    kmin = __reduce_min_sync(0xffffffffu, kmin);
+    kmax = __reduce_max_sync(0xffffffffu, kmax);
+    if (lane == 0) { s.range[0][warp] = kmin; s.range[1][warp] = kmax; }
+    __syncthreads();
+    kmin = __reduce_min_sync(0xffffffffu, s.range[0][lane % kPickWarps]);
+    kmax = __reduce_max_sync(0xffffffffu, s.range[1][lane % kPickWarps]);
+    // Bin of a key: scores clamped to the finite ones' range, evenly divided, rounded by the addition
+    // of 2^23 (a bin a thread). It never falls where the key rises. A range that is empty, or whose
+    // width or reciprocal overflows, leaves few bins in use, with products that may be infinite or
+    // NaN: those all end in the last bin.
+    const bool some = kmin <= kmax;
+    const float least = some ? key_score(kmin) : 0.f, most = some ? key_score(kmax) : 0.f, width = most - least;
+    const float per = width > 0.f ? (kPickThreads - 1.5f) / width : 0.f;
+    auto bin_of = [&](uint32_t k) -> uint32_t {
+        const float s = fminf(fmaxf(key_score(k), least), most);  // the key of no block stands for a NaN: least
+        return min(__float_as_uint(fmaf(s - least, per, 8388608.0f)) - 0x4b000000u, kPickThreads - 1u);
+    };
+    uint32_t need = static_cast<uint32_t>(d.budget - d.first - d.last);
+    uint32_t threshold = 0xffffffffu, at_it = 0;  // selected: above the threshold, and the first at_it at it
+    if (need > 0) {
+        each([&](int i, uint32_t k, int) {
+            if (i >= lo && i < hi) atomicAdd(&s.hist[bin_of(k)], 1u);
+        }, false);
+        __syncthreads();
+        find_bin(s, need);
+        const uint32_t bin = s.pick[0], in_bin = s.pick[2];
+        if (in_bin <= kPickList) {
+            const uint32_t rest = need - s.pick[1];
+            each([&](int i, uint32_t k, int) {
+                if (i >= lo && i < hi && bin_of(k) == bin) s.list[atomicAdd(&s.listed, 1u)] = k;
+            }, false);
+            __syncthreads();
+            if (tid < static_cast<int>(in_bin)) {
+                const uint32_t k = s.list[tid];
+                uint32_t more = 0, same = 0;
+#pragma unroll 4
+                for (uint32_t j = 0; j < in_bin; ++j) {
+                    more += s.list[j] > k;
+                    same += s.list[j] == k;
+                }
+                if (more < rest && more + same >= rest) {
+                    s.found[0] = k;
+                    s.found[1] = rest - more;
+                }
+            }
+            __syncthreads();
+            threshold = s.found[0];
+            at_it = s.found[1];
+        } else {
+            uint32_t mask = 0, prefix = 0;
+            for (int sh = 24; sh >= 0; sh -= 8) {
+                s.hist[tid] = 0u;
+                __syncthreads();
+                each([&](int i, uint32_t k, int) {
+                    if (i >= lo && i < hi && (k & mask) == prefix) atomicAdd(&s.hist[(k >> sh) & 255u], 1u);
+                }, false);
+                __syncthreads();
+                find_bin(s, need);
+                prefix |= s.pick[0] << sh;
+                mask |= 255u << sh;
+                need -= s.pick[1];
+            }
+            threshold = prefix;
+            at_it = need;
+        }
+    }
+    auto kind = [&](int i, uint32_t k, bool& up, bool& eq) {
+        const bool scored = i >= lo && i < hi;
+        up = i < n && (!scored || k > threshold);
+        eq = scored && k == threshold;
+    };
+    uint32_t above = 0, equal = 0;
+    each([&](int i, uint32_t k, int) {
+        bool up, eq;
+        kind(i, k, up, eq);
+        above += up;
+        equal += eq;
+    }, false);
+    above = __reduce_add_sync(0xffffffffu, above);
+    equal = __reduce_add_sync(0xffffffffu, equal);
+    if (lane == 0) { s.count[0][warp] = above; s.count[1][warp] = equal; }
+    __syncthreads();
+    above = equal = 0;
+#pragma unroll
+    for (int w = 0; w < kPickWarps; ++w)
+        if (w < warp) { above += s.count[0][w]; equal += s.count[1][w]; }
+    const uint32_t below = (1u << lane) - 1u;
+    each([&](int i, uint32_t k, int block) {
+        bool up, eq;
+        kind(i, k, up, eq);
+        const uint32_t ub = __ballot_sync(0xffffffffu, up), eb = __ballot_sync(0xffffffffu, eq);
+        const uint32_t e = equal + __popc(eb & below);
+        if (up || (eq && e < at_it)) out[above + __popc(ub & below) + min(e, at_it)] = block;
+        above += __popc(ub);
+        equal += __popc(eb);
+    }, true);
+}
+
+__global__ void __launch_bounds__(kPickThreads) pick_kernel(const SelectParams p) {
+    __shared__ PickShared s;
+    const kvd_block_select_desc& d = p.d;
+    const int row = blockIdx.x, b = row / d.num_kv_heads;
+    const int tid = threadIdx.x, k = d.budget;
+    s.hist[tid] = 0u;
+    if (tid == 0) s.listed = 0u;
+    grid_dependency_wait();
+    allow_dependents();
+    int n;
+    const int len = select_len(d, b, n);
+    const int32_t* table = d.block_table + b * d.block_table_stride;
+    if (tid == 0) p.sel_lens[row] = n <= k ? len : (k - n) * d.block_size + len;
+    if (n <= k) {  // everything
+        for (int i = tid; i < k; i += kPickThreads) {
+            p.sel_table[static_cast<int64_t>(row) * k + i] = i < n ? table[i] : -1;
+            if (i < n) pool_id(d, table, i);
+        }
+    } else if (n <= kPickKept) {
+        pick_row<true>(p, s, row, n, table);
+    } else {
+        pick_row<false>(p, s, row, n, table);
+    }
+}
+
+cudaError_t launch_select(const SelectParams& p, cudaStream_t st) {
+    const kvd_block_select_desc& d = p.d;
+    const int64_t rows = static_cast<int64_t>(d.batch) * d.num_kv_heads;
+    cudaError_t e;
+    if (d.max_blocks_per_seq > d.budget) {  // else every row takes all its blocks
+        if (score_tc_ok(p)) {
+            e = launch_score_tc(p, st);
+        } else {
+            const int64_t items = rows * ((d.max_blocks_per_seq + 15) / 16), most = static_cast<int64_t>(device_sm_count()) * 16;
+            const int G = d.num_q_heads / d.num_kv_heads;
+            const size_t smem = ((static_cast<size_t>(G) * d.head_dim + 3) & ~size_t(3)) + sizeof(float) * G;
+            if (smem > 48 * 1024 || items > 0x7fff0000LL) return cudaErrorInvalidValue;
+            e = launch_after(score_any_kernel, static_cast<unsigned>(items < most ? items : most), 32, smem, st, p);
+        }
+        if (e != cudaSuccess) return e;
+        ++*launch_counter();
+    }
+    e = launch_after(pick_kernel, static_cast<unsigned>(rows), kPickThreads, 0, st, p);
+    if (e == cudaSuccess) ++*launch_counter();
+    return e;
 }
 
 }  // namespace
@@ -1198,7 +1178,7 @@ extern "C" cudaError_t kvd_paged_plan_launch(const kvd_paged_plan_desc* desc, co
     int64_t grid = (static_cast<int64_t>(desc->num_slots) + 4 * block - 1) / (4 * block);
     if (grid > device_sm_count()) grid = device_sm_count();
     if (grid < 1) grid = 1;
-    e = launch_after(plan_kernel, static_cast<unsigned>(grid), block, smem, 1, stream, p);
+    e = launch_after(plan_kernel, static_cast<unsigned>(grid), block, smem, stream, p);
     if (e == cudaSuccess) *launch_counter() = 1;
     return e;
 }
@@ -1236,43 +1216,37 @@ extern "C" cudaError_t kvd_paged_read_launch(const kvd_paged_rows_desc* desc, co
     return rows_call(p, k_out, v_out, false, stream);
 }
 
-extern "C" cudaError_t kvd_block_select_launch(const kvd_block_select_desc* desc, const void* Q, const int8_t* bounds,
-                                               const float* bound_scale, int32_t* sel_table, int32_t* sel_lens,
-                                               cudaStream_t stream) {
-    *launch_counter() = 0;
-    if (!desc || !Q || !bounds || !bound_scale || !sel_table || !sel_lens || !desc->seq_lens || !desc->block_table)
-        return cudaErrorInvalidValue;
-    const kvd_block_select_desc& d = *desc;
+namespace {
+bool select_ok(const kvd_block_select_desc* p) {
+    if (!p) return false;
+    const kvd_block_select_desc& d = *p;
     if (d.batch < 1 || d.num_q_heads < 1 || d.num_kv_heads < 1 || d.num_q_heads % d.num_kv_heads != 0 ||
         d.head_dim < 1 || d.head_dim > 512 || d.block_size < 1 || d.num_blocks < 1)
-        return cudaErrorInvalidValue;
-    if (d.max_blocks_per_seq < 1 || d.max_blocks_per_seq > 262144 || d.block_table_stride < d.max_blocks_per_seq ||
+        return false;
+    if (d.max_blocks_per_seq < 1 || d.block_table_stride < d.max_blocks_per_seq ||
         static_cast<int64_t>(d.max_blocks_per_seq) * d.block_size > 0x7fffffffLL)
+        return false;
+    if (d.budget < 1 || d.first < 0 || d.last < 1 || d.first > d.budget - d.last) return false;
+    if (static_cast<int64_t>(d.batch) * d.num_kv_heads > 0x7fffffffLL) return false;
+    return d.flags == 0 || d.flags == KVD_FLAG_Q_BF16 || d.flags == KVD_FLAG_Q_F16;
+}
+}  // namespace
+
+extern "C" size_t kvd_block_select_workspace_size(const kvd_block_select_desc* desc) {
+    if (!select_ok(desc) || desc->max_blocks_per_seq <= desc->budget) return 0;
+    return static_cast<size_t>(desc->batch) * desc->num_kv_heads * desc->max_blocks_per_seq * sizeof(uint32_t);
+}
+
+extern "C" cudaError_t kvd_block_select_launch(const kvd_block_select_desc* desc, const void* Q, const int8_t* bounds,
+                                               const float* bound_scale, int32_t* sel_table, int32_t* sel_lens,
+                                               void* workspace, size_t workspace_bytes, cudaStream_t stream) {
+    *launch_counter() = 0;
+    if (!select_ok(desc) || !Q || !bounds || !bound_scale || !sel_table || !sel_lens || !desc->seq_lens ||
+        !desc->block_table)
         return cudaErrorInvalidValue;
-    if (d.budget < 1 || d.first < 0 || d.last < 1 || d.first > d.budget - d.last) return cudaErrorInvalidValue;
-    if (d.flags != 0 && d.flags != KVD_FLAG_Q_BF16 && d.flags != KVD_FLAG_Q_F16) return cudaErrorInvalidValue;
-    const int64_t rows = static_cast<int64_t>(d.batch) * d.num_kv_heads;
-    if (rows > 0x7fffffffLL / 8) return cudaErrorInvalidValue;
-    // CTAs per row: enough to fill the GPU, at least 128 blocks each, keys within shared memory
-    int c = 1;
-    while (c < 8 && rows * c < 2 * device_sm_count() && d.max_blocks_per_seq >= 256 * c) c *= 2;
-    while (c < 8 && d.max_blocks_per_seq > 32768 * c) c *= 2;
-    SelectParams p{d, Q, bounds, bound_scale, sel_table, sel_lens, 0};
-    p.cap = ((d.max_blocks_per_seq + c - 1) / c + 15) & ~15;
-    const int G = d.num_q_heads / d.num_kv_heads, GP = (G + 7) & ~7;
-    const size_t smem = 4 * static_cast<size_t>(p.cap) + static_cast<size_t>(GP) * sel_q_stride(d.head_dim) +
-                        sizeof(float) * G;
-    if (smem > 200 * 1024) return cudaErrorInvalidValue;
-    const bool vec = (reinterpret_cast<uintptr_t>(bounds) & 15) == 0 && d.head_dim % 32 == 0;
-    cudaError_t e;
-    switch (vec ? d.head_dim : 0) {
-        case 64: e = launch_select<2>(p, c, smem, stream); break;
-        case 96: e = launch_select<3>(p, c, smem, stream); break;
-        case 128: e = launch_select<4>(p, c, smem, stream); break;
-        case 192: e = launch_select<6>(p, c, smem, stream); break;
-        case 256: e = launch_select<8>(p, c, smem, stream); break;
-        default: e = launch_select<0>(p, c, smem, stream); break;
-    }
-    if (e == cudaSuccess) *launch_counter() = 1;
-    return e;
+    const size_t want = kvd_block_select_workspace_size(desc);
+    if (want > 0 && (!workspace || workspace_bytes < want || (reinterpret_cast<uintptr_t>(workspace) & 3) != 0))
+        return cudaErrorInvalidValue;
+    const SelectParams p{*desc, Q, bounds, bound_scale, sel_table, sel_lens, static_cast<uint32_t*>(workspace)};
+    return launch_select(p, stream);
 }

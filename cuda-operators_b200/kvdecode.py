@@ -235,7 +235,8 @@ _SIGNATURES = {
     "kvd_paged_plan_launch": (c_int, [ctypes.POINTER(PagedPlanDesc)] + [c_void_p] * 10 + [c_size_t, c_void_p]),
     "kvd_paged_write_launch": (c_int, [ctypes.POINTER(PagedRowsDesc)] + [c_void_p] * 9 + [c_void_p]),
     "kvd_paged_read_launch": (c_int, [ctypes.POINTER(PagedRowsDesc)] + [c_void_p] * 7 + [c_void_p]),
-    "kvd_block_select_launch": (c_int, [ctypes.POINTER(BlockSelectDesc)] + [c_void_p] * 5 + [c_void_p]),
+    "kvd_block_select_workspace_size": (c_size_t, [ctypes.POINTER(BlockSelectDesc)]),
+    "kvd_block_select_launch": (c_int, [ctypes.POINTER(BlockSelectDesc)] + [c_void_p] * 6 + [c_size_t, c_void_p]),
     "kvd_sparse_workspace_size": (c_size_t, [ctypes.POINTER(PagedDesc)]),
     "kvd_sparse_decode_launch": (c_int, [ctypes.POINTER(PagedDesc)] + [c_void_p] * 7 + [c_size_t, c_void_p]),
 }
@@ -732,7 +733,7 @@ def paged_read(slot_map, k_pool, v_pool, ks_pool, vs_pool, k_out=None, v_out=Non
 
 
 def block_select(q, bounds, bound_scale, block_table, seq_lens, block_size: int, budget: int, first: int = 1,
-                 last: int = 2, sel_table=None, sel_lens=None, stream=None):
+                 last: int = 2, sel_table=None, sel_lens=None, workspace=None, stream=None):
     """Blocks that one new token per request attends to (``kvd_block_select_launch``): the ``first`` first and
     ``last`` last blocks and those whose key bounds score highest for ``q`` [B, Hq, D], ``budget`` in all, per
     KV head. Returns (sel_table int32 [B, Hkv, budget] pool ids, then -1; sel_lens int32 [B, Hkv] tokens)."""
@@ -759,8 +760,12 @@ def block_select(q, bounds, bound_scale, block_table, seq_lens, block_size: int,
     desc = BlockSelectDesc(B, Hq, H, D, block_size, NB, block_table.shape[1], budget, first, last,
                            _row_flags(q.dtype), seq_lens.data_ptr(), block_table.data_ptr(), block_table.stride(0),
                            q.stride(0), q.stride(1))
+    if workspace is None:
+        n = B * H * block_table.shape[1] * 4 if block_table.shape[1] > budget else 1
+        workspace = torch.empty(n, dtype=torch.uint8, device=q.device)
     rc = lib().kvd_block_select_launch(ctypes.byref(desc), q.data_ptr(), bounds.data_ptr(), bound_scale.data_ptr(),
-                                       sel_table.data_ptr(), sel_lens.data_ptr(), _stream(stream))
+                                       sel_table.data_ptr(), sel_lens.data_ptr(), workspace.data_ptr(),
+                                       workspace.numel(), _stream(stream))
     _check(rc, "kvd_block_select_launch")
     return sel_table, sel_lens
 

@@ -279,7 +279,7 @@ typedef struct kvd_paged_rows_desc {
  * max_t x_td, lo_d = min_t x_td and step = max_d max(|hi_d|, |lo_d|) / 127,
  * codes are clamp(ceil(hi_d / step)) then clamp(floor(lo_d / step)), clamped
  * to +-127 (step 0: codes 0). A token scale that is not finite makes step NaN
- * and the codes 0, so that the block is always selected. Tokens of one block
+ * and the codes 0, so that the block is always selected; steps are not negative. Tokens of one block
  * come in order, with no other block's token between them, as
  * kvd_paged_plan_launch lays them out; places of the block in front of the last
  * one that the map leaves out hold earlier tokens. */
@@ -307,8 +307,9 @@ cudaError_t kvd_paged_read_launch(const kvd_paged_rows_desc* desc, const int64_t
  * receives the selected blocks' pool ids in token order, then -1, and sel_lens
  * [batch][num_kv_heads] the tokens in them: only the last selected block can
  * be partly filled. A block id outside the pool scores below all others and
- * records KVD_STATUS_BAD_BLOCK. Tables of up to 262,144 entries per request;
- * head_dim at most 512. */
+ * records KVD_STATUS_BAD_BLOCK. head_dim at most 512. The workspace of
+ * kvd_block_select_workspace_size bytes (a key per table entry and KV head; 0
+ * when no row can hold more than its budget) needs no initialisation. */
 typedef struct kvd_block_select_desc {
     int32_t batch, num_q_heads, num_kv_heads, head_dim;
     int32_t block_size, num_blocks, max_blocks_per_seq;
@@ -319,9 +320,10 @@ typedef struct kvd_block_select_desc {
     int64_t block_table_stride;
     int64_t q_stride_b, q_stride_h;
 } kvd_block_select_desc;
+size_t kvd_block_select_workspace_size(const kvd_block_select_desc* desc);
 cudaError_t kvd_block_select_launch(const kvd_block_select_desc* desc, const void* Q, const int8_t* bounds,
                                     const float* bound_scale, int32_t* sel_table, int32_t* sel_lens,
-                                    cudaStream_t stream);
+                                    void* workspace, size_t workspace_bytes, cudaStream_t stream);
 
 /* Decode attention over selected blocks: as kvd_paged_decode_launch, but
  * every (request, KV head) has its own length and table row:

@@ -254,16 +254,19 @@ def test_symbols_and_refusals():
 
     sel = (2, 8, 2, 64, 16, 40, 20, 8, 1, 2, 0, 256, 256, 20, 512, 64)
     d = kvd.BlockSelectDesc(*sel)
-    for i in range(5):
-        bad = [256] * 5
+    assert L.kvd_block_select_workspace_size(ctypes.byref(d)) == 2 * 2 * 20 * 4
+    for i in range(6):
+        bad = [256] * 6
         bad[i] = None
-        assert L.kvd_block_select_launch(ctypes.byref(d), *bad, None) == EINVAL, i
-    for at, value in [(0, 0), (1, 0), (1, 7), (2, 0), (3, 0), (3, 513), (4, 0), (5, 0), (6, 0), (6, 262145), (7, 0),
+        assert L.kvd_block_select_launch(ctypes.byref(d), *bad, 320, None) == EINVAL, i
+    assert L.kvd_block_select_launch(ctypes.byref(d), *[256] * 6, 319, None) == EINVAL  # workspace too small
+    for at, value in [(0, 0), (1, 0), (1, 7), (2, 0), (3, 0), (3, 513), (4, 0), (5, 0), (6, 0), (6, 1 << 28), (7, 0),
                       (7, 2), (8, -1), (8, 7), (9, 0), (10, 1), (10, 6), (11, None), (12, None), (13, 19)]:
         bad = list(sel)
         bad[at] = value
         d = kvd.BlockSelectDesc(*bad)
-        assert L.kvd_block_select_launch(ctypes.byref(d), *[256] * 5, None) == EINVAL, (at, value)
+        assert L.kvd_block_select_workspace_size(ctypes.byref(d)) == 0 or at in (11, 12)
+        assert L.kvd_block_select_launch(ctypes.byref(d), *[256] * 6, 1 << 30, None) == EINVAL, (at, value)
 
     sp = dict(batch=2, num_q_heads=8, num_kv_heads=2, head_dim=128, block_size=16, num_blocks=64, max_blocks_per_seq=8,
               seq_lens=256, block_table=256, block_table_stride=8, o_stride_h=128)
