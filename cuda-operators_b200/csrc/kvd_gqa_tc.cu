@@ -1212,7 +1212,11 @@ bool make_paged_map(CUtensorMap* m, const int8_t* base, int Hkv, const PagedView
     cuuint32_t estr[4] = {1, 1, 1, 1};
     const CUresult r = fn(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 4, const_cast<int8_t*>(base), dims, strides, box, estr,
                           CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
-                          CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+                          // With tokens outside heads a row's 128 bytes lie between other heads' rows. Their
+                          // CTAs want those soon after, unless every head reads blocks of its own.
+                          pv.per_head && pv.kv_st != 128 ? CU_TENSOR_MAP_L2_PROMOTION_L2_128B
+                                                         : CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                          CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     return r == CUDA_SUCCESS;
 }
 
