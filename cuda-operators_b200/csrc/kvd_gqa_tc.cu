@@ -1118,6 +1118,7 @@ __global__ void __launch_bounds__(1024) seq_order_kernel(const int32_t* seq_lens
 __global__ void __launch_bounds__(128) gqa_ragged_combine_kernel(const float* partials, const int32_t* seq_lens,
                                                                  int Hq, int per_seq, int P, int span, int S, int D, void* out,
                                                                  int64_t o_sb, int64_t o_sh, uint32_t flags) {
+    kvd::grid_dependency_wait();  // launched as a programmatic dependent of the decode that wrote the records
     const int64_t r = blockIdx.x;
     const int b = static_cast<int>(r / Hq), hq = static_cast<int>(r - static_cast<int64_t>(b) * Hq);
     const int len = min(max(0, seq_lens[r / per_seq]), S);
@@ -1427,10 +1428,18 @@ cudaError_t launch_gqa_tc(const kvd_decode_desc& d, const void* Q, const int8_t*
     if (g.P > 1) {
         const int64_t rows = static_cast<int64_t>(d.batch) * d.num_q_heads;
         if (d.seq_lens) {
-            gqa_ragged_combine_kernel<<<static_cast<unsigned>(rows), 128, 0, st>>>(
-                p.partials, d.seq_lens, d.num_q_heads, sel ? G : d.num_q_heads, g.P, g.span, S, d.head_dim, out, d.o_stride_b, d.o_stride_h,
-                d.flags);
-            e = cudaGetLastError();
+            cudaLaunchConfig_t cfg{};
+            cfg.gridDim = dim3(static_cast<unsigned>(rows), 1, 1);
+            cfg.blockDim = dim3(128, 1, 1);
+            cfg.stream = st;
+            cudaLaunchAttribute attr[1];
+            attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+            attr[0].val.programmaticStreamSerializationAllowed = 1;
+            cfg.attrs = attr;
+            cfg.numAttrs = 1;
+            e = cudaLaunchKernelEx(
+                &cfg, gqa_ragged_combine_kernel, static_cast<const float*>(p.partials), d.seq_lens, d.num_q_heads,
+                sel ? G : d.num_q_heads, g.P, g.span, S, d.head_dim, out, d.o_stride_b, d.o_stride_h, d.flags);
             if (e == cudaSuccess) ++*launches;
         } else {
             const int64_t rs = d.head_dim + 4;

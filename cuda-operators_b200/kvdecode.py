@@ -299,7 +299,8 @@ def _stream(stream) -> int | None:
     if stream is None:
         import torch
 
-        return torch.cuda.current_stream().cuda_stream
+        raw = getattr(torch._C, "_cuda_getCurrentRawStream", None)  # a Stream object costs several microseconds
+        return raw(torch.cuda.current_device()) if raw else torch.cuda.current_stream().cuda_stream
     if isinstance(stream, int):
         return stream
     return stream.cuda_stream
@@ -333,19 +334,30 @@ def dtype_flags(q=None, out=None, partial: bool = False) -> int:
     import torch
 
     f = KVD_FLAG_PARTIAL_OUT if partial else 0
-    qmap = {torch.float32: 0, torch.bfloat16: KVD_FLAG_Q_BF16, torch.float16: KVD_FLAG_Q_F16}
-    omap = {torch.float32: 0, torch.bfloat16: KVD_FLAG_OUT_BF16, torch.float16: KVD_FLAG_OUT_F16}
     if q is not None:
-        if q.dtype not in qmap:
+        if q.dtype not in _dtype_map():
             raise ValueError(f"unsupported query dtype {q.dtype}")
-        f |= qmap[q.dtype]
+        f |= _dtype_map()[q.dtype]
     if out is not None and out.device.type != "meta":
-        if out.dtype not in omap:
+        if out.dtype not in _dtype_map():
             raise ValueError(f"unsupported output dtype {out.dtype}")
         if partial and out.dtype != torch.float32:
             raise ValueError("partial records are float32")
-        f |= omap[out.dtype]
+        f |= _dtype_map()[out.dtype] << 2  # KVD_FLAG_OUT_* lie two bits above KVD_FLAG_Q_*
     return f
+
+
+_dtypes = None
+
+
+def _dtype_map() -> dict:
+    """KVD_FLAG_Q_* of each element type."""
+    global _dtypes
+    if _dtypes is None:
+        import torch
+
+        _dtypes = {torch.float32: 0, torch.bfloat16: KVD_FLAG_Q_BF16, torch.float16: KVD_FLAG_Q_F16}
+    return _dtypes
 
 
 def make_desc(q, k, ks, out, seq_lens=None, max_seq_len: int | None = None, softmax_scale: float = 0.0,
@@ -596,17 +608,9 @@ def paged_append(k_new, v_new, k_pool, v_pool, ks_pool, vs_pool, block_table, se
 
 
 # ------------------------------------------- paged serving steps on the GPU
-_ROW_FLAGS = None
-
-
 def _row_flags(dtype) -> int:
     """KVD_FLAG_Q_* of a row type."""
-    global _ROW_FLAGS
-    if _ROW_FLAGS is None:
-        import torch
-
-        _ROW_FLAGS = {torch.float32: 0, torch.bfloat16: KVD_FLAG_Q_BF16, torch.float16: KVD_FLAG_Q_F16}
-    f = _ROW_FLAGS.get(dtype)
+    f = _dtype_map().get(dtype)
     if f is None:
         raise ValueError(f"unsupported row dtype {dtype}")
     return f
