@@ -616,27 +616,64 @@ def _row_flags(dtype) -> int:
     return f
 
 
+_torch = None
+
+
+def _types():
+    """(torch, int8, int32, int64, float32), looked up once: these calls are short, and so are their checks."""
+    global _torch
+    if _torch is None:
+        import torch
+
+        _torch = (torch, torch.int8, torch.int32, torch.int64, torch.float32)
+    return _torch
+
+
 def _want(t, dtype, shape, what: str) -> None:
     """A contiguous tensor of this type and shape."""
-    if t.dtype != dtype or t.shape != shape or not t.is_contiguous():
+    if t.shape != shape or t.dtype != dtype or not t.is_contiguous():
         raise ValueError(f"{what} must be contiguous {dtype} of shape {tuple(shape)}, got {t.dtype} {tuple(t.shape)}")
 
 
-def _pool_view(k_pool, ks_pool, layout: str):
-    """(blocks, heads, block_size, head_dim, block stride, head stride, token stride) of a K or V pool."""
+def _stream_of(stream, t) -> int:
+    """The given stream, or the current one of ``t``'s device."""
+    if stream is not None:
+        return _stream(stream)
+    torch = _types()[0]
+    raw = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+    return raw(t.get_device()) if raw else torch.cuda.current_stream(t.device).cuda_stream
+
+
+def _pools(k_pool, v_pool, ks_pool, vs_pool, layout: str):
+    """(blocks, heads, block_size, head_dim, block stride, head stride, token stride, scale strides) of K and V pools."""
+    _, i8, _, _, f32 = _types()
+    strides, sc_strides = k_pool.stride(), ks_pool.stride()
     if layout == "bhtd":
         NB, H, bs, D = k_pool.shape
-        s_blk, s_h, s_t, s_d = k_pool.stride()
+        s_blk, s_h, s_t, s_d = strides
     elif layout == "bthd":
         NB, bs, H, D = k_pool.shape
-        s_blk, s_t, s_h, s_d = k_pool.stride()
+        s_blk, s_t, s_h, s_d = strides
     else:
         raise ValueError(f"unknown pool layout {layout!r}")
     if ks_pool.shape != (NB, H, bs):
         raise ValueError(f"scale pool {tuple(ks_pool.shape)} does not match pool {tuple(k_pool.shape)}")
-    if s_d != 1 or ks_pool.stride(2) != 1:
+    if s_d != 1 or sc_strides[2] != 1:
         raise ValueError("dims and scale tokens must be contiguous")
-    return NB, H, bs, D, s_blk, s_h, s_t
+    if v_pool.stride() != strides or vs_pool.stride() != sc_strides or v_pool.shape != k_pool.shape \
+            or vs_pool.shape != ks_pool.shape:
+        raise ValueError("K/V pools and their scale pools must share shapes and strides")
+    if k_pool.dtype != i8 or v_pool.dtype != i8 or ks_pool.dtype != f32 or vs_pool.dtype != f32:
+        raise ValueError("pools are int8, scale pools float32")
+    return NB, H, bs, D, s_blk, s_h, s_t, sc_strides[0], sc_strides[1]
+
+
+def _table(block_table, B: int, i32) -> int:
+    """Entries per row of an int32 [B, max_blocks] table."""
+    shape = block_table.shape
+    if block_table.dtype != i32 or len(shape) != 2 or shape[0] != B or block_table.stride(1) != 1:
+        raise ValueError("block_table must be int32 [B, max_blocks] with contiguous rows")
+    return shape[1]
 
 
 def paged_plan(seq_lens, new_lens, block_table, free_blocks, free_count, block_size: int, slot_map, token_starts=None,
@@ -648,54 +685,45 @@ def paged_plan(seq_lens, new_lens, block_table, free_blocks, free_count, block_s
     ids on it, ``slot_map`` int64 [num_slots]. The table, the free list and, unless other tensors are given for
     them, the lengths and the count are updated in place. ``workspace``: a zeroed uint8 tensor of 16 bytes that a
     caller keeps (without one, one is made). Returns (slot_map, token_starts [B + 1])."""
-    import torch
-
-    i32 = torch.int32
+    torch, _, i32, i64, _ = _types()
     B = seq_lens.shape[0]
     if token_starts is None:
         token_starts = torch.empty(B + 1, dtype=i32, device=seq_lens.device)
-    if seq_lens_out is None:
-        seq_lens_out = seq_lens
-    if free_count_out is None:
-        free_count_out = free_count
     if workspace is None:
         workspace = torch.zeros(16, dtype=torch.uint8, device=seq_lens.device)
-    _want(seq_lens, i32, (B,), "seq_lens")
-    _want(new_lens, i32, (B,), "new_lens")
-    _want(seq_lens_out, i32, (B,), "seq_lens_out")
+    rows, one = (B,), (1,)
+    _want(seq_lens, i32, rows, "seq_lens")
+    _want(new_lens, i32, rows, "new_lens")
     _want(token_starts, i32, (B + 1,), "token_starts")
-    _want(free_count, i32, (1,), "free_count")
-    _want(free_count_out, i32, (1,), "free_count_out")
-    if block_table.dtype != i32 or block_table.dim() != 2 or block_table.shape[0] != B or block_table.stride(1) != 1:
-        raise ValueError("block_table must be int32 [B, max_blocks] with contiguous rows")
-    _want(free_blocks, i32, (free_blocks.numel(),), "free_blocks")
-    _want(slot_map, torch.int64, (slot_map.numel(),), "slot_map")
-    desc = PagedPlanDesc(B, block_size, free_blocks.numel(), block_table.shape[1], slot_map.numel(),
-                         block_table.stride(0))
+    _want(free_count, i32, one, "free_count")
+    if seq_lens_out is None:
+        seq_lens_out = seq_lens
+    else:
+        _want(seq_lens_out, i32, rows, "seq_lens_out")
+    if free_count_out is None:
+        free_count_out = free_count
+    else:
+        _want(free_count_out, i32, one, "free_count_out")
+    MB = _table(block_table, B, i32)
+    NB, T = free_blocks.numel(), slot_map.numel()
+    _want(free_blocks, i32, (NB,), "free_blocks")
+    _want(slot_map, i64, (T,), "slot_map")
+    desc = PagedPlanDesc(B, block_size, NB, MB, T, block_table.stride(0))
     rc = lib().kvd_paged_plan_launch(
         ctypes.byref(desc), seq_lens.data_ptr(), new_lens.data_ptr(), block_table.data_ptr(), free_blocks.data_ptr(),
         free_count.data_ptr(), slot_map.data_ptr(), token_starts.data_ptr(), seq_lens_out.data_ptr(),
-        free_count_out.data_ptr(), workspace.data_ptr(), workspace.numel(), _stream(stream))
+        free_count_out.data_ptr(), workspace.data_ptr(), workspace.numel(), _stream_of(stream, seq_lens))
     _check(rc, "kvd_paged_plan_launch")
     return slot_map, token_starts
 
 
 def _rows_desc(k, v, slot_map, k_pool, v_pool, ks_pool, vs_pool, layout: str):
-    import torch
-
-    NB, H, bs, D, s_blk, s_h, s_t = _pool_view(k_pool, ks_pool, layout)
-    T = slot_map.shape[0]
-    if k.shape != (T, H, D) or v.shape != k.shape or v.dtype != k.dtype or v.stride() != k.stride() or k.stride(2) != 1:
+    NB, H, bs, D, s_blk, s_h, s_t, sc_blk, sc_h = _pools(k_pool, v_pool, ks_pool, vs_pool, layout)
+    T, (s_row, s_head, s_dim) = slot_map.shape[0], k.stride()
+    if k.shape != (T, H, D) or v.shape != k.shape or v.dtype != k.dtype or v.stride() != (s_row, s_head, s_dim) or s_dim != 1:
         raise ValueError(f"rows must be two [{T}, {H}, {D}] tensors of one type and strides with contiguous dims")
-    if v_pool.stride() != k_pool.stride() or vs_pool.stride() != ks_pool.stride() or v_pool.shape != k_pool.shape \
-            or vs_pool.shape != ks_pool.shape:
-        raise ValueError("K/V pools and their scale pools must share shapes and strides")
-    if k_pool.dtype != torch.int8 or v_pool.dtype != torch.int8 or ks_pool.dtype != torch.float32 \
-            or vs_pool.dtype != torch.float32:
-        raise ValueError("pools are int8, scale pools float32")
-    _want(slot_map, torch.int64, (T,), "slot_map")
-    return PagedRowsDesc(T, H, D, bs, NB, _row_flags(k.dtype), k.stride(0), k.stride(1), s_blk, s_h, s_t,
-                         ks_pool.stride(0), ks_pool.stride(1))
+    _want(slot_map, _types()[3], (T,), "slot_map")
+    return PagedRowsDesc(T, H, D, bs, NB, _row_flags(k.dtype), s_row, s_head, s_blk, s_h, s_t, sc_blk, sc_h)
 
 
 def paged_write(k_new, v_new, slot_map, k_pool, v_pool, ks_pool, vs_pool, bounds=None, bound_scale=None,
@@ -703,17 +731,18 @@ def paged_write(k_new, v_new, slot_map, k_pool, v_pool, ks_pool, vs_pool, bounds
     """Quantises rows k_new / v_new [T, Hkv, D] (float32, bfloat16 or float16) into the pools' slots
     ``slot_map`` [T] (-1: skipped). With ``bounds`` int8 [blocks, Hkv, 2, D] and ``bound_scale`` float32
     [blocks, Hkv] the key bounds of every block written to are kept for :func:`block_select`."""
-    import torch
-
     desc = _rows_desc(k_new, v_new, slot_map, k_pool, v_pool, ks_pool, vs_pool, layout)
     if (bounds is None) != (bound_scale is None):
         raise ValueError("bounds and bound_scale come together")
+    bounds_ptr = scale_ptr = None
     if bounds is not None:
-        _want(bounds, torch.int8, (desc.num_blocks, desc.num_kv_heads, 2, desc.head_dim), "bounds")
-        _want(bound_scale, torch.float32, (desc.num_blocks, desc.num_kv_heads), "bound_scale")
+        NB, H = desc.num_blocks, desc.num_kv_heads
+        _want(bounds, _types()[1], (NB, H, 2, desc.head_dim), "bounds")
+        _want(bound_scale, _types()[4], (NB, H), "bound_scale")
+        bounds_ptr, scale_ptr = bounds.data_ptr(), bound_scale.data_ptr()
     rc = lib().kvd_paged_write_launch(ctypes.byref(desc), k_new.data_ptr(), v_new.data_ptr(), slot_map.data_ptr(),
                                       k_pool.data_ptr(), v_pool.data_ptr(), ks_pool.data_ptr(), vs_pool.data_ptr(),
-                                      _ptr(bounds), _ptr(bound_scale), _stream(stream))
+                                      bounds_ptr, scale_ptr, _stream_of(stream, k_pool))
     _check(rc, "kvd_paged_write_launch")
 
 
@@ -721,9 +750,8 @@ def paged_read(slot_map, k_pool, v_pool, ks_pool, vs_pool, k_out=None, v_out=Non
                stream=None):
     """Rows of a paged cache by slot as the values that they stand for: returns (k_out, v_out) [T, Hkv, D]
     (``dtype``, default float32). Slots of -1 read as zeros."""
-    import torch
-
     if k_out is None or v_out is None:
+        torch = _types()[0]
         H, D = k_pool.shape[1 if layout == "bhtd" else 2], k_pool.shape[3]
         shape = (slot_map.shape[0], H, D)
         k_out = torch.empty(shape, dtype=dtype or torch.float32, device=k_pool.device)
@@ -731,7 +759,7 @@ def paged_read(slot_map, k_pool, v_pool, ks_pool, vs_pool, k_out=None, v_out=Non
     desc = _rows_desc(k_out, v_out, slot_map, k_pool, v_pool, ks_pool, vs_pool, layout)
     rc = lib().kvd_paged_read_launch(ctypes.byref(desc), slot_map.data_ptr(), k_pool.data_ptr(), v_pool.data_ptr(),
                                      ks_pool.data_ptr(), vs_pool.data_ptr(), k_out.data_ptr(), v_out.data_ptr(),
-                                     _stream(stream))
+                                     _stream_of(stream, k_pool))
     _check(rc, "kvd_paged_read_launch")
     return k_out, v_out
 
@@ -741,60 +769,35 @@ def block_select(q, bounds, bound_scale, block_table, seq_lens, block_size: int,
     """Blocks that one new token per request attends to (``kvd_block_select_launch``): the ``first`` first and
     ``last`` last blocks and those whose key bounds score highest for ``q`` [B, Hq, D], ``budget`` in all, per
     KV head. Returns (sel_table int32 [B, Hkv, budget] pool ids, then -1; sel_lens int32 [B, Hkv] tokens)."""
-    import torch
-
+    torch, i8, i32, _, f32 = _types()
     B, Hq, D = q.shape
-    NB, H, two, Db = bounds.shape
+    NB, H, _, Db = bounds.shape
     if Db != D or Hq % H:
         raise ValueError(f"shape mismatch q{tuple(q.shape)} bounds{tuple(bounds.shape)}")
-    if q.stride(2) != 1:
+    s_b, s_h, s_d = q.stride()
+    if s_d != 1:
         raise ValueError("dims must be contiguous")
-    if block_table.dtype != torch.int32 or block_table.dim() != 2 or block_table.shape[0] != B \
-            or block_table.stride(1) != 1:
-        raise ValueError("block_table must be int32 [B, max_blocks] with contiguous rows")
-    _want(bounds, torch.int8, (NB, H, 2, D), "bounds")
-    _want(bound_scale, torch.float32, (NB, H), "bound_scale")
-    _want(seq_lens, torch.int32, (B,), "seq_lens")
+    MB = _table(block_table, B, i32)
+    _want(bounds, i8, (NB, H, 2, D), "bounds")
+    _want(bound_scale, f32, (NB, H), "bound_scale")
+    _want(seq_lens, i32, (B,), "seq_lens")
     if sel_table is None:
-        sel_table = torch.empty((B, H, budget), dtype=torch.int32, device=q.device)
+        sel_table = torch.empty((B, H, budget), dtype=i32, device=q.device)
+    else:
+        _want(sel_table, i32, (B, H, budget), "sel_table")
     if sel_lens is None:
-        sel_lens = torch.empty((B, H), dtype=torch.int32, device=q.device)
-    _want(sel_table, torch.int32, (B, H, budget), "sel_table")
-    _want(sel_lens, torch.int32, (B, H), "sel_lens")
-    desc = BlockSelectDesc(B, Hq, H, D, block_size, NB, block_table.shape[1], budget, first, last,
-                           _row_flags(q.dtype), seq_lens.data_ptr(), block_table.data_ptr(), block_table.stride(0),
-                           q.stride(0), q.stride(1))
-    if workspace is None:
-        n = B * H * block_table.shape[1] * 4 if block_table.shape[1] > budget else 1
-        workspace = torch.empty(n, dtype=torch.uint8, device=q.device)
+        sel_lens = torch.empty((B, H), dtype=i32, device=q.device)
+    else:
+        _want(sel_lens, i32, (B, H), "sel_lens")
+    desc = BlockSelectDesc(B, Hq, H, D, block_size, NB, MB, budget, first, last, _row_flags(q.dtype),
+                           seq_lens.data_ptr(), block_table.data_ptr(), block_table.stride(0), s_b, s_h)
+    if workspace is None and MB > budget:
+        workspace = torch.empty(B * H * MB, dtype=i32, device=q.device)
     rc = lib().kvd_block_select_launch(ctypes.byref(desc), q.data_ptr(), bounds.data_ptr(), bound_scale.data_ptr(),
-                                       sel_table.data_ptr(), sel_lens.data_ptr(), workspace.data_ptr(),
-                                       workspace.numel(), _stream(stream))
+                                       sel_table.data_ptr(), sel_lens.data_ptr(), _ptr(workspace),
+                                       workspace.nbytes if workspace is not None else 0, _stream_of(stream, q))
     _check(rc, "kvd_block_select_launch")
     return sel_table, sel_lens
-
-
-def make_sparse_desc(q, k_pool, ks_pool, out, sel_table, sel_lens, layout: str = "bhtd", softmax_scale: float = 0.0,
-                     partial: bool = False) -> PagedDesc:
-    """Descriptor of a decode over selected blocks: ``sel_table`` int32 [B, Hkv, budget], ``sel_lens`` int32
-    [B, Hkv] (None where only the workspace size is asked for)."""
-    import torch
-
-    B, Hq, D = q.shape
-    NB, H, bs, Dk, s_blk, s_h, s_t = _pool_view(k_pool, ks_pool, layout)
-    if Dk != D or Hq % H:
-        raise ValueError(f"shape mismatch q{tuple(q.shape)} k_pool{tuple(k_pool.shape)}")
-    budget = sel_table.shape[-1]
-    _want(sel_table, torch.int32, (B, H, budget), "sel_table")
-    if sel_lens is not None:
-        _want(sel_lens, torch.int32, (B, H), "sel_lens")
-    if tuple(out.shape) != (B, Hq, D + 4 if partial else D):
-        raise ValueError(f"out must be [{B}, {Hq}, {D + 4 if partial else D}], got {tuple(out.shape)}")
-    if q.stride(2) != 1 or out.stride(2) != 1:
-        raise ValueError("dims must be contiguous")
-    return PagedDesc(B, Hq, H, D, bs, NB, budget, dtype_flags(q, out, partial), _ptr(sel_lens) or sel_table.data_ptr(),
-                     sel_table.data_ptr(), budget, s_blk, s_h, s_t, ks_pool.stride(0), ks_pool.stride(1), q.stride(0),
-                     q.stride(1), out.stride(0), out.stride(1), softmax_scale)
 
 
 def sparse_workspace_size(q, k_pool, sel_table, layout: str = "bhtd") -> int:
@@ -808,23 +811,34 @@ def sparse_workspace_size(q, k_pool, sel_table, layout: str = "bhtd") -> int:
 
 def sparse_decode(q, k_pool, v_pool, ks_pool, vs_pool, sel_table, sel_lens, out=None, layout: str = "bhtd",
                   softmax_scale: float = 0.0, partial: bool = False, workspace=None, stream=None, out_dtype=None):
-    """INT8 decode attention over selected blocks of a paged cache (:func:`block_select`'s tables); returns
-    ``out`` [B, Hq, D] (or records)."""
-    import torch
-
+    """INT8 decode attention over selected blocks of a paged cache, ``sel_table`` int32 [B, Hkv, budget] and
+    ``sel_lens`` int32 [B, Hkv] (:func:`block_select`'s); returns ``out`` [B, Hq, D] (or records)."""
+    torch, _, i32, _, _ = _types()
     B, Hq, D = q.shape
+    R = D + 4 if partial else D
     if out is None:
-        out = torch.empty((B, Hq, D + 4 if partial else D), dtype=out_dtype or torch.float32, device=q.device)
-    if v_pool.stride() != k_pool.stride() or vs_pool.stride() != ks_pool.stride() or v_pool.shape != k_pool.shape \
-            or vs_pool.shape != ks_pool.shape:
-        raise ValueError("K/V pools and their scale pools must share shapes and strides")
-    desc = make_sparse_desc(q, k_pool, ks_pool, out, sel_table, sel_lens, layout, softmax_scale, partial)
+        out = torch.empty((B, Hq, R), dtype=out_dtype or torch.float32, device=q.device)
+    elif out.shape != (B, Hq, R):
+        raise ValueError(f"out must be [{B}, {Hq}, {R}], got {tuple(out.shape)}")
+    NB, H, bs, Dk, s_blk, s_h, s_t, sc_blk, sc_h = _pools(k_pool, v_pool, ks_pool, vs_pool, layout)
+    if Dk != D or Hq % H:
+        raise ValueError(f"shape mismatch q{tuple(q.shape)} k_pool{tuple(k_pool.shape)}")
+    budget = sel_table.shape[-1]
+    _want(sel_table, i32, (B, H, budget), "sel_table")
+    _want(sel_lens, i32, (B, H), "sel_lens")
+    q_b, q_h, q_d = q.stride()
+    o_b, o_h, o_d = out.stride()
+    if q_d != 1 or o_d != 1:
+        raise ValueError("dims must be contiguous")
+    table = sel_table.data_ptr()
+    desc = PagedDesc(B, Hq, H, D, bs, NB, budget, dtype_flags(q, out, partial), sel_lens.data_ptr(), table, budget,
+                     s_blk, s_h, s_t, sc_blk, sc_h, q_b, q_h, o_b, o_h, softmax_scale)
     if workspace is None:
         n = int(lib().kvd_sparse_workspace_size(ctypes.byref(desc)))
         workspace = torch.empty(max(n, 1), dtype=torch.uint8, device=q.device)
     rc = lib().kvd_sparse_decode_launch(ctypes.byref(desc), q.data_ptr(), k_pool.data_ptr(), v_pool.data_ptr(),
                                         ks_pool.data_ptr(), vs_pool.data_ptr(), out.data_ptr(), workspace.data_ptr(),
-                                        workspace.numel(), _stream(stream))
+                                        workspace.nbytes, _stream_of(stream, q))
     _check(rc, "kvd_sparse_decode_launch")
     return out
 
