@@ -30,178 +30,6 @@ cudaError_t launch_after(void (*kern)(A...), unsigned grid, unsigned block, size
     return cudaLaunchKernelEx(&cfg, kern, args...);
 }
 
-// ----------------------------------------------------------------------- plan
-// Prefix sums over the requests (new tokens, blocks needed, blocks given back)
-// place every slot, table entry and free-list entry independently, so after
-// the sums all writes run in parallel. Every CTA makes the sums itself
-// (24 bytes a request from L2) and writes its share; the CTA that ends last
-// writes the lengths and the count, which may alias the inputs.
-constexpr int kPlanMaxBatch = 8192;
-
-struct PlanParams {
-    kvd_paged_plan_desc d;
-    const int32_t* seq_lens;
-    const int32_t* new_lens;
-    int32_t* table;
-    int32_t* free_blocks;
-    const int32_t* free_count;
-    int64_t* slots;
-    int32_t* starts;
-    int32_t* lens_out;
-    int32_t* count_out;
-    unsigned int* ticket;
-};
-
-// Sums saturate at 2^31 - 1: lengths no pool can hold are refused, not wrapped.
-__device__ __forceinline__ uint32_t sat_add(uint32_t a, uint32_t b) { return min(a + b, 0x7fffffffu); }
-
-// Inclusive prefix sum of one value per thread over the block, plus `carry`.
-__device__ __forceinline__ uint32_t block_scan(uint32_t x, uint32_t carry, uint32_t* warp_sums) {
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, nw = blockDim.x >> 5;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-        const uint32_t y = __shfl_up_sync(0xffffffffu, x, o);
-        if (lane >= o) x = sat_add(x, y);
-    }
-    __syncthreads();  // the sums of the scan before are no longer read
-    if (lane == 31) warp_sums[warp] = x;
-    __syncthreads();
-    uint32_t s = lane < nw ? warp_sums[lane] : 0u;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-        const uint32_t y = __shfl_up_sync(0xffffffffu, s, o);
-        if (lane >= o) s = sat_add(s, y);
-    }
-    const uint32_t before = __shfl_sync(0xffffffffu, s, (warp - 1) & 31);
-    return sat_add(x, warp > 0 ? sat_add(carry, before) : carry);
-}
-
-// First index in [0, n) whose inclusive sum is above v (n when there is none).
-__device__ __forceinline__ int first_above(const uint32_t* sums, int n, uint32_t v) {
-    int lo = 0, hi = n;
-    while (lo < hi) {
-        const int mid = (lo + hi) >> 1;
-        if (sums[mid] > v) hi = mid;
-        else lo = mid + 1;
-    }
-    return lo;
-}
-
-__global__ void __launch_bounds__(1024) plan_kernel(const PlanParams p) {
-    extern __shared__ uint32_t plan_smem[];
-    __shared__ uint32_t warp_sums[32];
-    __shared__ uint32_t s_popped;
-    __shared__ int s_last;
-    grid_dependency_wait();
-    allow_dependents();
-    const int B = p.d.batch, bs = p.d.block_size, MB = p.d.max_blocks_per_seq, NB = p.d.num_blocks;
-    const int64_t cap = static_cast<int64_t>(MB) * bs;
-    uint32_t* tok = plan_smem;   // [B] tokens up to and with request b
-    uint32_t* need = tok + B;    // [B] blocks needed up to and with request b
-    uint32_t* back = need + B;   // [B] blocks given back up to and with request b
-    uint8_t* okay = reinterpret_cast<uint8_t*>(back + B);  // [B] served
-    const bool writer = blockIdx.x == 0;
-    auto length = [&](int b) { return static_cast<int>(min(static_cast<int64_t>(max(0, p.seq_lens[b])), cap)); };
-    auto blocks_of = [&](int64_t tokens) { return static_cast<int>((tokens + bs - 1) / bs); };
-    uint32_t carry_t = 0, carry_n = 0, carry_b = 0;
-    if (threadIdx.x == 0) s_popped = 0;
-    int status = 0;
-    for (int b0 = 0; b0 < B; b0 += blockDim.x) {
-        const int b = b0 + threadIdx.x;
-        const bool in = b < B;
-        const int n = in ? p.new_lens[b] : 0;
-        const int len = in ? length(b) : 0;
-        const uint32_t stop = block_scan(n > 0 ? n : 0, carry_t, warp_sums);
-        const bool over = n > 0 && (len + static_cast<int64_t>(n) > cap || stop > static_cast<uint32_t>(p.d.num_slots));
-        const int held = blocks_of(len);
-        const uint32_t nd = n > 0 && !over ? blocks_of(len + static_cast<int64_t>(n)) - held : 0;
-        const uint32_t nstop = block_scan(nd, carry_n, warp_sums);
-        const uint32_t bstop = block_scan(n < 0 ? held : 0, carry_b, warp_sums);
-        if (in) {
-            tok[b] = stop;
-            need[b] = nstop;
-            back[b] = bstop;
-            okay[b] = over ? 0 : nd > 0 ? 2 : 1;  // 2: served if the blocks suffice
-            if (over) status |= KVD_STATUS_CACHE_FULL;
-        }
-        __syncthreads();
-        const int last = min(B, b0 + static_cast<int>(blockDim.x)) - 1;
-        carry_t = tok[last];
-        carry_n = need[last];
-        carry_b = back[last];
-    }
-    const uint32_t fc = static_cast<uint32_t>(min(max(0, *p.free_count), NB));
-    const uint32_t total = sat_add(fc, carry_b);  // stack height with the ended requests' blocks on top
-    for (int b = threadIdx.x; b < B; b += blockDim.x) {
-        if (okay[b] != 2) continue;
-        if (need[b] <= total) {
-            atomicMax(&s_popped, need[b]);
-        } else {
-            okay[b] = 0;
-            status |= KVD_STATUS_NO_BLOCKS;
-        }
-    }
-    __syncthreads();
-    const uint32_t popped = s_popped, left = total - popped;
-    // Entry i of the stack.
-    auto stack = [&](uint32_t i) -> int {
-        if (i < fc) return p.free_blocks[i];
-        const int b = first_above(back, B, i - fc);
-        const uint32_t before = b > 0 ? back[b - 1] : 0u;
-        return p.table[b * p.d.block_table_stride + (i - fc - before)];
-    };
-    const uint32_t stride = gridDim.x * blockDim.x, me = blockIdx.x * blockDim.x + threadIdx.x;
-    // table entries of the new blocks
-    for (uint32_t k = me; k < popped; k += stride) {
-        const int b = first_above(need, B, k);
-        const uint32_t before = b > 0 ? need[b - 1] : 0u;
-        p.table[b * p.d.block_table_stride + blocks_of(length(b)) + (k - before)] = stack(total - 1 - k);
-    }
-    // ended requests' blocks that stay on the stack
-    for (uint32_t i = fc + me; i < left; i += stride) {
-        if (i < static_cast<uint32_t>(NB)) p.free_blocks[i] = stack(i);
-        else status |= KVD_STATUS_BAD_BLOCK;  // more blocks than the pool has: some were given back twice
-    }
-    // slots
-    const uint32_t tokens = min(tok[B - 1], static_cast<uint32_t>(p.d.num_slots));
-    for (uint32_t t = me; t < static_cast<uint32_t>(p.d.num_slots); t += stride) {
-        int64_t slot = -1;
-        if (t < tokens) {
-            const int b = first_above(tok, B, t);
-            if (okay[b]) {
-                const int len = length(b), held = blocks_of(len);
-                const uint32_t pos = len + (t - (b > 0 ? tok[b - 1] : 0u));
-                const int j = static_cast<int>(pos) / bs;
-                const int id = j < held ? p.table[b * p.d.block_table_stride + j]
-                                        : stack(total - 1 - ((b > 0 ? need[b - 1] : 0u) + (j - held)));
-                if (id >= 0 && id < NB) slot = static_cast<int64_t>(id) * bs + (pos - static_cast<uint32_t>(j) * bs);
-                else status |= KVD_STATUS_BAD_BLOCK;
-            }
-        }
-        p.slots[t] = slot;
-    }
-    if (writer)
-        for (int b = threadIdx.x; b <= B; b += blockDim.x)
-            p.starts[b] = b > 0 ? min(tok[b - 1], static_cast<uint32_t>(p.d.num_slots)) : 0;
-    if (status && writer) record_status(status);
-    else if (status & KVD_STATUS_BAD_BLOCK) record_status(KVD_STATUS_BAD_BLOCK);
-    // lengths and count: after every CTA has read them
-    __syncthreads();
-    if (threadIdx.x == 0) {
-        __threadfence();
-        s_last = gridDim.x == 1 || atomicInc(p.ticket, gridDim.x - 1) == gridDim.x - 1;
-    }
-    __syncthreads();
-    if (!s_last) return;
-    __threadfence();
-    for (int b = threadIdx.x; b < B; b += blockDim.x) {
-        const int n = p.new_lens[b], len = length(b);
-        p.lens_out[b] = n < 0 ? 0 : okay[b] ? len + n : len;
-    }
-    if (threadIdx.x == 0) *p.count_out = static_cast<int32_t>(min(left, static_cast<uint32_t>(NB)));
-}
-
-// ------------------------------------------------------------- rows by slot
 // n / d for n < 2^31, by the multiply-and-shift method of Granlund and
 // Montgomery (1994): mul = floor(2^(31+L) / d) + 1, L = ceil(log2 d).
 struct FastDiv {
@@ -217,6 +45,209 @@ struct FastDiv {
     }
 };
 
+// ----------------------------------------------------------------------- plan
+// Prefix sums over the requests (new tokens, blocks needed, blocks given back)
+// place every slot, table entry and free-list entry independently, so after
+// the sums all writes run in parallel. Every CTA makes the sums itself (8 bytes
+// a request from L2, an exchange through shared memory a sum) and writes its
+// share, a slot per thread where that many threads fit on the GPU. Bound:
+// latency, a chain of three loads and the sums' barriers. Lengths and the count
+// may alias the inputs: the CTA that was last to read the inputs writes them,
+// at its end; the others have counted themselves right after reading.
+constexpr int kPlanMaxBatch = 8192;
+
+struct PlanParams {
+    kvd_paged_plan_desc d;
+    const int32_t* seq_lens;
+    const int32_t* new_lens;
+    int32_t* table;
+    int32_t* free_blocks;
+    const int32_t* free_count;
+    int64_t* slots;
+    int32_t* starts;
+    int32_t* lens_out;
+    int32_t* count_out;
+    unsigned int* ticket;
+    FastDiv by_bs;
+};
+
+// Sums saturate at 2^31 - 1: lengths no pool can hold are refused, not wrapped.
+__device__ __forceinline__ uint32_t sat_add(uint32_t a, uint32_t b) { return min(a + b, 0x7fffffffu); }
+
+// Inclusive prefix sums of N values per thread over the block, on top of `carry`.
+template <int N>
+__device__ __forceinline__ void block_scan(uint32_t (&x)[N], const uint32_t (&carry)[N], uint32_t (*warp_sums)[32]) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, nw = blockDim.x >> 5;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1)
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const uint32_t y = __shfl_up_sync(0xffffffffu, x[i], o);
+            if (lane >= o) x[i] = sat_add(x[i], y);
+        }
+    __syncthreads();  // the sums of the scan before are no longer read
+    if (lane == 31)
+#pragma unroll
+        for (int i = 0; i < N; ++i) warp_sums[i][warp] = x[i];
+    __syncthreads();
+    uint32_t s[N];
+#pragma unroll
+    for (int i = 0; i < N; ++i) s[i] = lane < nw ? warp_sums[i][lane] : 0u;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1)
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const uint32_t y = __shfl_up_sync(0xffffffffu, s[i], o);
+            if (lane >= o) s[i] = sat_add(s[i], y);
+        }
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        const uint32_t before = __shfl_sync(0xffffffffu, s[i], (warp - 1) & 31);
+        x[i] = sat_add(x[i], warp > 0 ? sat_add(carry[i], before) : carry[i]);
+    }
+}
+
+// First index in [0, n) whose inclusive sum is above v (n when there is none).
+__device__ __forceinline__ int first_above(const uint32_t* sums, int n, uint32_t v) {
+    int lo = 0, hi = n;
+    while (lo < hi) {
+        const int mid = (lo + hi) >> 1;
+        if (sums[mid] > v) hi = mid;
+        else lo = mid + 1;
+    }
+    return lo;
+}
+
+// Shared memory of one request: four sums or lengths and a flag.
+constexpr size_t kPlanBytes = 17;
+
+__global__ void __launch_bounds__(1024) plan_kernel(const PlanParams p) {
+    extern __shared__ uint32_t plan_smem[];
+    __shared__ uint32_t warp_sums[2][32];
+    __shared__ uint32_t s_popped;
+    __shared__ int s_last;
+    grid_dependency_wait();
+    allow_dependents();
+    const int B = p.d.batch, bs = p.d.block_size, MB = p.d.max_blocks_per_seq, NB = p.d.num_blocks;
+    const int64_t cap = static_cast<int64_t>(MB) * bs;
+    uint32_t* tok = plan_smem;   // [B] tokens up to and with request b
+    uint32_t* need = tok + B;    // [B] blocks needed up to and with request b
+    uint32_t* back = need + B;   // [B] blocks given back up to and with request b
+    int32_t* held_len = reinterpret_cast<int32_t*>(back + B);  // [B] lengths
+    uint8_t* okay = reinterpret_cast<uint8_t*>(held_len + B);  // [B] 0 refused, 1 or 2 served, 3 ends
+    const uint32_t fc = static_cast<uint32_t>(min(max(0, *p.free_count), NB));
+    auto blocks_of = [&](int tokens) {
+        const int whole = static_cast<int>(p.by_bs.div(static_cast<uint32_t>(tokens)));
+        return whole + (whole * bs != tokens);
+    };
+    uint32_t carry_t[1] = {0}, carry[2] = {0, 0};
+    if (threadIdx.x == 0) s_popped = 0;
+    int status = 0;
+    for (int b0 = 0; b0 < B; b0 += blockDim.x) {
+        const int b = b0 + threadIdx.x;
+        const bool in = b < B;
+        const int n = in ? p.new_lens[b] : 0;
+        const int len = in ? static_cast<int>(min(static_cast<int64_t>(max(0, p.seq_lens[b])), cap)) : 0;
+        uint32_t stop[1] = {n > 0 ? static_cast<uint32_t>(n) : 0u};
+        block_scan<1>(stop, carry_t, warp_sums);
+        const bool over =
+            n > 0 && (len + static_cast<int64_t>(n) > cap || stop[0] > static_cast<uint32_t>(p.d.num_slots));
+        const int held = blocks_of(len);
+        const uint32_t nd = n > 0 && !over ? blocks_of(len + n) - held : 0;
+        uint32_t sums[2] = {nd, n < 0 ? static_cast<uint32_t>(held) : 0u};
+        block_scan<2>(sums, carry, warp_sums);
+        if (in) {
+            tok[b] = stop[0];
+            need[b] = sums[0];
+            back[b] = sums[1];
+            held_len[b] = len;
+            okay[b] = n < 0 ? 3 : over ? 0 : nd > 0 ? 2 : 1;  // 2: served if the blocks suffice
+            if (over) status |= KVD_STATUS_CACHE_FULL;
+        }
+        __syncthreads();
+        const int last = min(B, b0 + static_cast<int>(blockDim.x)) - 1;
+        carry_t[0] = tok[last];
+        carry[0] = need[last];
+        carry[1] = back[last];
+    }
+    // the inputs are read: count this CTA
+    if (threadIdx.x == 0) {
+        s_last = 1;
+        if (gridDim.x > 1) {
+            __threadfence();
+            s_last = atomicInc(p.ticket, gridDim.x - 1) == gridDim.x - 1;
+            __threadfence();
+        }
+    }
+    const uint32_t total = sat_add(fc, carry[1]);  // stack height with the ended requests' blocks on top
+    uint32_t most = 0;
+    for (int b = threadIdx.x; b < B; b += blockDim.x) {
+        if (okay[b] != 2) continue;
+        if (need[b] <= total) {
+            most = max(most, need[b]);
+        } else {
+            okay[b] = 0;
+            status |= KVD_STATUS_NO_BLOCKS;
+        }
+    }
+    most = __reduce_max_sync(0xffffffffu, most);
+    if ((threadIdx.x & 31) == 0) atomicMax(&s_popped, most);
+    __syncthreads();
+    const uint32_t popped = s_popped, left = total - popped;
+    // Entry i of the stack.
+    auto stack = [&](uint32_t i) -> int {
+        if (i < fc) return p.free_blocks[i];
+        const int b = first_above(back, B, i - fc);
+        const uint32_t before = b > 0 ? back[b - 1] : 0u;
+        return p.table[b * p.d.block_table_stride + (i - fc - before)];
+    };
+    const uint32_t stride = gridDim.x * blockDim.x, me = blockIdx.x * blockDim.x + threadIdx.x;
+    // slots
+    const uint32_t tokens = min(tok[B - 1], static_cast<uint32_t>(p.d.num_slots));
+    for (uint32_t t = me; t < static_cast<uint32_t>(p.d.num_slots); t += stride) {
+        int64_t slot = -1;
+        if (t < tokens) {
+            const int b = first_above(tok, B, t);
+            if (okay[b]) {
+                const int len = held_len[b], held = blocks_of(len);
+                const uint32_t pos = len + (t - (b > 0 ? tok[b - 1] : 0u));
+                const int j = static_cast<int>(p.by_bs.div(pos));
+                const int id = j < held ? p.table[b * p.d.block_table_stride + j]
+                                        : stack(total - 1 - ((b > 0 ? need[b - 1] : 0u) + (j - held)));
+                if (id >= 0 && id < NB) slot = static_cast<int64_t>(id) * bs + (pos - static_cast<uint32_t>(j) * bs);
+                else status |= KVD_STATUS_BAD_BLOCK;
+            }
+        }
+        p.slots[t] = slot;
+    }
+    // table entries of the new blocks
+    for (uint32_t k = me; k < popped; k += stride) {
+        const int b = first_above(need, B, k);
+        const uint32_t before = b > 0 ? need[b - 1] : 0u;
+        p.table[b * p.d.block_table_stride + blocks_of(held_len[b]) + (k - before)] = stack(total - 1 - k);
+    }
+    // ended requests' blocks that stay on the stack
+    for (uint32_t i = fc + me; i < left; i += stride) {
+        if (i < static_cast<uint32_t>(NB)) p.free_blocks[i] = stack(i);
+        else status |= KVD_STATUS_BAD_BLOCK;  // more blocks than the pool has: some were given back twice
+    }
+    if (blockIdx.x == 0) {
+        for (int b = threadIdx.x; b <= B; b += blockDim.x)
+            p.starts[b] = b > 0 ? min(tok[b - 1], static_cast<uint32_t>(p.d.num_slots)) : 0;
+        if (status) record_status(status);
+    } else if (status & KVD_STATUS_BAD_BLOCK) {
+        record_status(KVD_STATUS_BAD_BLOCK);
+    }
+    if (!s_last) return;
+    for (int b = threadIdx.x; b < B; b += blockDim.x) {
+        const int len = held_len[b];  // tokens of a served request: its share of the sums
+        const uint32_t n = tok[b] - (b > 0 ? tok[b - 1] : 0u);
+        p.lens_out[b] = okay[b] == 3 ? 0 : okay[b] ? len + static_cast<int>(n) : len;
+    }
+    if (threadIdx.x == 0) *p.count_out = static_cast<int32_t>(min(left, static_cast<uint32_t>(NB)));
+}
+
+// ------------------------------------------------------------- rows by slot
 struct RowsParams {
     kvd_paged_rows_desc d;
     const void* k_rows;
@@ -1167,15 +1198,17 @@ extern "C" cudaError_t kvd_paged_plan_launch(const kvd_paged_plan_desc* desc, co
         return cudaErrorInvalidValue;
     if (!workspace || workspace_bytes < kvd_paged_plan_workspace_size(desc)) return cudaErrorInvalidValue;
     PlanParams p{*desc, seq_lens, new_lens, block_table, free_blocks, free_count, slot_map, token_starts,
-                 seq_lens_out, free_count_out, static_cast<unsigned int*>(workspace)};
+                 seq_lens_out, free_count_out, static_cast<unsigned int*>(workspace),
+                 FastDiv(static_cast<uint32_t>(desc->block_size))};
     const unsigned block = desc->batch <= 256 ? 256 : 1024;
-    const size_t smem = static_cast<size_t>(desc->batch) * 13 + 16;
+    const size_t smem = static_cast<size_t>(desc->batch) * kPlanBytes;
     static PerDeviceOnce once;
     cudaError_t e = once.run([] {
-        return cudaFuncSetAttribute(plan_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kPlanMaxBatch * 13 + 16);
+        return cudaFuncSetAttribute(plan_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                    kPlanMaxBatch * kPlanBytes);
     });
     if (e != cudaSuccess) return e;
-    int64_t grid = (static_cast<int64_t>(desc->num_slots) + 4 * block - 1) / (4 * block);
+    int64_t grid = (static_cast<int64_t>(desc->num_slots) + block - 1) / block;
     if (grid > device_sm_count()) grid = device_sm_count();
     if (grid < 1) grid = 1;
     e = launch_after(plan_kernel, static_cast<unsigned>(grid), block, smem, stream, p);
