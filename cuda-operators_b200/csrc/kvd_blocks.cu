@@ -323,14 +323,16 @@ struct Rows {
 #pragma unroll
         for (int j = 0; j < E; ++j) x[j] = in(l, j, D) ? widen<T>(row[at(l, j)]) : 0.f;
     }
+    static __device__ __forceinline__ void widen_codes(uint2 q, float (&x)[E]) {  // VEC
+        float2 a, b;
+        dequant4(q.x, a, b);
+        x[0] = a.x; x[1] = a.y; x[2] = b.x; x[3] = b.y;
+        dequant4(q.y, a, b);
+        x[4] = a.x; x[5] = a.y; x[6] = b.x; x[7] = b.y;
+    }
     static __device__ __forceinline__ void load_codes(const int8_t* row, int l, int D, float (&x)[E]) {
         if constexpr (VEC) {
-            const uint2 q = *reinterpret_cast<const uint2*>(row + l * 8);
-            float2 a, b;
-            dequant4(q.x, a, b);
-            x[0] = a.x; x[1] = a.y; x[2] = b.x; x[3] = b.y;
-            dequant4(q.y, a, b);
-            x[4] = a.x; x[5] = a.y; x[6] = b.x; x[7] = b.y;
+            widen_codes(*reinterpret_cast<const uint2*>(row + l * 8), x);
         } else {
 #pragma unroll
             for (int j = 0; j < E; ++j) x[j] = in(l, j, D) ? static_cast<float>(row[at(l, j)]) : 0.f;
@@ -780,12 +782,15 @@ __global__ void __launch_bounds__(32 * W, LPR ? 24 / W : 1) write_kernel(const R
     }
 }
 
-// Reads: rows (token, head) in order, a warp holding R::N neighbours, four
-// times over so that its loads are in flight together. Bound: HBM.
+// Reads: rows (token, head) in order, a warp holding U times R::N neighbours,
+// their codes as loaded until all loads are under way. Bound: HBM.
+template <int LPR>
+constexpr int kReadRows = LPR ? 2 : 1;
+
 template <class T, int LPR>
 __global__ void __launch_bounds__(32 * kRowWarps) read_kernel(const RowsParams p) {
     using R = Rows<LPR>;
-    constexpr int E = R::E, U = R::VEC ? 2 : 1;
+    constexpr int E = R::E, U = kReadRows<LPR>;
     grid_dependency_wait();
     allow_dependents();
     const kvd_paged_rows_desc& d = p.d;
@@ -793,18 +798,25 @@ __global__ void __launch_bounds__(32 * kRowWarps) read_kernel(const RowsParams p
     const int lane = threadIdx.x & 31, sub = lane / R::LANES, l = lane % R::LANES;
     const uint32_t rows = static_cast<uint32_t>(d.num_tokens) * H;
     const uint32_t step = gridDim.x * kRowWarps * (R::N * U);
+    const int64_t v_codes_at = p.V - p.K, v_rows_at = static_cast<char*>(p.v_out) - static_cast<char*>(p.k_out);
     for (uint32_t r0 = (blockIdx.x * kRowWarps + (threadIdx.x >> 5)) * (R::N * U); r0 < rows; r0 += step) {
-        float xk[U][E], xv[U][E];
-        int64_t row[U];
+        uint2 kw[U], vw[U];      // VEC
+        float xk[E], xv[E];      // otherwise (U = 1)
+        float sk[U], sv[U];
+        T* out[U];
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             const uint32_t r = r0 + u * R::N + sub;
-            row[u] = -1;
+            out[u] = nullptr;
+            kw[u] = vw[u] = make_uint2(0u, 0u);
+            sk[u] = sv[u] = 0.f;
+            if constexpr (!R::VEC) {
 #pragma unroll
-            for (int j = 0; j < E; ++j) xk[u][j] = xv[u][j] = 0.f;
+                for (int j = 0; j < E; ++j) xk[j] = xv[j] = 0.f;
+            }
             if (r >= rows) continue;
             const int t = static_cast<int>(p.by_heads.div(r)), h = static_cast<int>(r) - t * H;
-            row[u] = t * d.row_stride_t + h * d.row_stride_h;
+            out[u] = static_cast<T*>(p.k_out) + t * d.row_stride_t + h * d.row_stride_h;
             const int64_t slot = p.slots[t];
             const int blk = block_of(p, slot);
             if (blk < 0) {
@@ -812,19 +824,29 @@ __global__ void __launch_bounds__(32 * kRowWarps) read_kernel(const RowsParams p
                 continue;
             }
             const int64_t o = slot - static_cast<int64_t>(blk) * d.block_size;
-            const int64_t at = blk * d.kv_stride_block + h * d.kv_stride_h + o * d.kv_stride_t;
+            const int8_t* at = p.K + blk * d.kv_stride_block + h * d.kv_stride_h + o * d.kv_stride_t;
             const int64_t sc = blk * d.sc_stride_block + h * d.sc_stride_h + o;
-            R::load_codes(p.K + at, l, D, xk[u]);
-            R::load_codes(p.V + at, l, D, xv[u]);
-            const float sk = p.ks[sc], sv = p.vs[sc];
-#pragma unroll
-            for (int j = 0; j < E; ++j) { xk[u][j] *= sk; xv[u][j] *= sv; }
+            if constexpr (R::VEC) {
+                kw[u] = *reinterpret_cast<const uint2*>(at + l * 8);
+                vw[u] = *reinterpret_cast<const uint2*>(at + v_codes_at + l * 8);
+            } else {
+                R::load_codes(at, l, D, xk);
+                R::load_codes(at + v_codes_at, l, D, xv);
+            }
+            sk[u] = p.ks[sc];
+            sv[u] = p.vs[sc];
         }
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-            if (row[u] < 0) continue;
-            R::store(static_cast<T*>(p.k_out) + row[u], l, D, xk[u]);
-            R::store(static_cast<T*>(p.v_out) + row[u], l, D, xv[u]);
+            if (!out[u]) continue;
+            if constexpr (R::VEC) {
+                R::widen_codes(kw[u], xk);
+                R::widen_codes(vw[u], xv);
+            }
+#pragma unroll
+            for (int j = 0; j < E; ++j) { xk[j] *= sk[u]; xv[j] *= sv[u]; }
+            R::store(out[u], l, D, xk);
+            R::store(reinterpret_cast<T*>(reinterpret_cast<char*>(out[u]) + v_rows_at), l, D, xv);
         }
     }
 }
@@ -840,7 +862,7 @@ cudaError_t launch_rows(const RowsParams& p, bool write, cudaStream_t st) {
         return launch_after(write_kernel<T, LPR, kRowWarps>, static_cast<unsigned>(grid), 32 * kRowWarps,
                             sizeof(float) * kRowWarps * 2 * d.head_dim, st, p);
     }
-    const int64_t per = kRowWarps * Rows<LPR>::N * (LPR ? 2 : 1);
+    const int64_t per = kRowWarps * Rows<LPR>::N * kReadRows<LPR>;
     int64_t grid = (rows + per - 1) / per;
     const int64_t most = static_cast<int64_t>(device_sm_count()) * 16;
     if (grid > most) grid = most;
