@@ -239,14 +239,14 @@ kvd_decode_desc paged_as_dense(const kvd_paged_desc& p, PagedView* pv) {
     return d;
 }
 
-bool paged_tc_shape(const kvd_paged_desc& p, const kvd_decode_desc& d) {
+bool paged_tc_shape(const kvd_paged_desc& p, const kvd_decode_desc& d, bool sel = false) {
     const int bs = p.block_size;
-    return bs >= 8 && (bs & (bs - 1)) == 0 && gqa_path_ok(d);
+    return bs >= 8 && (bs & (bs - 1)) == 0 && (sel ? gqa_sel_ok(d) : gqa_path_ok(d));
 }
 
 bool paged_tc_ok(const kvd_paged_desc& p, const kvd_decode_desc& d, const void* Q, const int8_t* K,
-                 const int8_t* V, const float* ks, const float* vs) {
-    if (!paged_tc_shape(p, d)) return false;
+                 const int8_t* V, const float* ks, const float* vs, bool sel = false) {
+    if (!paged_tc_shape(p, d, sel)) return false;
     if (!aligned16(Q) || !aligned16(K) || !aligned16(V) || !aligned16(ks) || !aligned16(vs)) return false;
     if (((p.kv_stride_block | p.kv_stride_h | p.kv_stride_t) & 15) != 0) return false;
     if (p.kv_stride_block <= 0 || p.kv_stride_h <= 0 || p.kv_stride_t <= 0) return false;
@@ -291,7 +291,7 @@ extern "C" size_t kvd_sparse_workspace_size(const kvd_paged_desc* desc) {
     PagedView pv;
     const kvd_decode_desc d = paged_as_dense(*desc, &pv);
     const size_t gen = generic_workspace_size(d);
-    const size_t gqa = paged_tc_shape(*desc, d) ? gqa_workspace_size(d, true) : 0;
+    const size_t gqa = paged_tc_shape(*desc, d, true) ? gqa_workspace_size(d, true) : 0;
     return gen > gqa ? gen : gqa;
 }
 
@@ -310,7 +310,7 @@ extern "C" cudaError_t kvd_sparse_decode_launch(const kvd_paged_desc* desc, cons
     PagedView pv;
     const kvd_decode_desc d = paged_as_dense(*desc, &pv);
     pv.per_head = true;
-    if (paged_tc_ok(*desc, d, Q, K_pool, V_pool, k_scale_pool, v_scale_pool))
+    if (paged_tc_ok(*desc, d, Q, K_pool, V_pool, k_scale_pool, v_scale_pool, true))
         return launch_gqa_tc(d, Q, K_pool, V_pool, k_scale_pool, v_scale_pool, out, workspace, workspace_bytes,
                              stream, &tl_launches, &pv);
     return launch_generic(d, Q, K_pool, V_pool, k_scale_pool, v_scale_pool, out, workspace, workspace_bytes, stream,

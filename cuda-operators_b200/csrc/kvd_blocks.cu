@@ -30,21 +30,6 @@ cudaError_t launch_after(void (*kern)(A...), unsigned grid, unsigned block, size
     return cudaLaunchKernelEx(&cfg, kern, args...);
 }
 
-// n / d for n < 2^31, by the multiply-and-shift method of Granlund and
-// Montgomery (1994): mul = floor(2^(31+L) / d) + 1, L = ceil(log2 d).
-struct FastDiv {
-    uint32_t mul, shift;
-    explicit FastDiv(uint32_t d = 1) {
-        uint32_t L = 0;
-        while ((1ull << L) < d) ++L;
-        mul = static_cast<uint32_t>((1ull << (31 + L)) / d + 1);
-        shift = 31 + L;
-    }
-    __device__ __forceinline__ uint32_t div(uint32_t n) const {
-        return static_cast<uint32_t>((static_cast<uint64_t>(n) * mul) >> shift);
-    }
-};
-
 // ----------------------------------------------------------------------- plan
 // Prefix sums over the requests (new tokens, blocks needed, blocks given back)
 // place every slot, table entry and free-list entry independently, so after

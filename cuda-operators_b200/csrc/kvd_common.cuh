@@ -33,6 +33,21 @@ __device__ __forceinline__ void record_status(int32_t code) {
     atomicOr(&g_status, code);
 }
 
+// n / d for n < 2^31, by the multiply-and-shift method of Granlund and
+// Montgomery (1994): mul = floor(2^(31+L) / d) + 1, L = ceil(log2 d).
+struct FastDiv {
+    uint32_t mul, shift;
+    explicit FastDiv(uint32_t d = 1) {
+        uint32_t L = 0;
+        while ((1ull << L) < d) ++L;
+        mul = static_cast<uint32_t>((1ull << (31 + L)) / d + 1);
+        shift = 31 + L;
+    }
+    __device__ __forceinline__ uint32_t div(uint32_t n) const {
+        return static_cast<uint32_t>((static_cast<uint64_t>(n) * mul) >> shift);
+    }
+};
+
 // ------------------------------------------------- query / output element types
 // Query element `off` of Q, whose type KVD_FLAG_Q_* in `flags` selects.
 __device__ __forceinline__ float load_q(const void* Q, int64_t off, uint32_t flags) {

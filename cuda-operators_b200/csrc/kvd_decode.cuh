@@ -169,6 +169,7 @@ cudaError_t launch_combine_records(const float* base, int nparts, int64_t part_s
                                    int64_t rows, int rows_per_b, int D, void* out, int64_t o_sb, int64_t o_sh,
                                    uint32_t flags, cudaStream_t st, int* launches);
 bool gqa_path_ok(const kvd_decode_desc& d);
+bool gqa_sel_ok(const kvd_decode_desc& d);  // decode over selected blocks: any group of query heads
 size_t gqa_workspace_size(const kvd_decode_desc& d, bool sel = false);
 // Split records a dense tensor-core decode left in its workspace when the
 // caller asked it to skip the combine: row r's P records of D+4 floats start

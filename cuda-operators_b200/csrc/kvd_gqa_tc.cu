@@ -41,6 +41,17 @@
 
 namespace kvd {
 
+// Work rows of a decode over selected blocks (query mode 2). Table rows and
+// lengths are per (b, kv head). A group of more than 8 query heads is cut into
+// `sub` parts of `per` heads (the last may have fewer) that each read the
+// head's blocks; work rows are (part, b, kv head). Heads that a row's form of
+// the kernel has beyond the part's are zero queries whose output is dropped.
+struct SelRows {
+    int sub, per, group;  // sub * per >= group
+    int rows, heads;      // rows = sub * heads, heads = B * Hkv
+    FastDiv by_rows, by_heads, by_hkv;
+};
+
 struct GqaParams {
     const void* Q;                // fp32, bf16 or fp16 (flags)
     const float* ks;
@@ -54,11 +65,11 @@ struct GqaParams {
     float qscale;
     uint32_t flags;
     // Paged cache (table != nullptr): the maps view the pools as
-    // {D, block_size, Hkv, num_blocks}; lbs = log2(block_size) >= 3. Selected
-    // blocks (query mode 2): table rows and lengths are per (b, kv head).
+    // {D, block_size, Hkv, num_blocks}; lbs = log2(block_size) >= 3.
     const int32_t* table;
     int64_t bt_stride, sc_sblk;
     int lbs, nblk;
+    SelRows sel;  // selected blocks (query mode 2)
     // Fused quantise-on-append (k_new != nullptr, dense cache): token
     // seq_lens[b] of every (b, kv head) is quantised from k_new / v_new into
     // the cache before the tile that holds it is loaded, every length reads as
@@ -105,10 +116,12 @@ struct GqaCfg {
     // N = NP, four accumulator columns per head); QM = 1 (KVD_FLAG_QK_INT8)
     // quantises it to one int8 row per head, so QK has N = 16 and one column
     // per head: head h of warpgroup w is B row / accumulator column w*QPW + h.
-    // QM = 2 is QM = 0 over selected blocks: every (b, kv head) is a sequence
-    // of its own, with its own length and block table row.
+    // QM = 2 is QM = 0 over selected blocks (SelRows), QM = 3 that with rows of
+    // fewer than G heads (apart from QM = 2, whose form for 8 heads it would
+    // slow by 2 %: it is at its register limit).
     static constexpr bool QI8 = QM_ == 1;
-    static constexpr bool SEL = QM_ == 2;
+    static constexpr bool SEL = QM_ >= 2;
+    static constexpr bool PAD = QM_ == 3;
     static constexpr int NQ = QI8 ? 16 : NP;                      // QK MMA N (<= NP)
     static constexpr int QPW = NQ / NWG;                          // QK rows / columns per warpgroup
     static constexpr int SW = QI8 ? HPW : CPW;                    // score columns an epilogue thread loads
@@ -171,7 +184,9 @@ __device__ __forceinline__ int exp_above(float x) {
 namespace kvd {
 
 struct GItem {
-    int b, hk, row, split, t_lo, t_hi, ntiles;  // row: the sequence, whose length and table row are read
+    int b, hk, split, t_lo, t_hi, ntiles;
+    int row, kvh;  // the sequence, whose length and table row are read, and its head in the pool
+    int q0, nq;    // PAD: query heads
 };
 
 // Items are numbered split-major: item = (split * B + k) * Hkv + hk, where k
@@ -198,13 +213,26 @@ __device__ __forceinline__ int split_count(const GqaParams& p, int len) {
 template <bool SEL>
 __device__ __forceinline__ GItem gqa_item(const GqaParams& p, int it) {
     GItem I;
-    const int per_split = p.B * p.Hkv;
-    I.split = it / per_split;
-    const int rem = it - I.split * per_split;
-    const int k = rem / p.Hkv;
-    I.hk = rem - k * p.Hkv;
-    I.b = !SEL && p.order ? __ldg(p.order + k) : k;
-    I.row = SEL ? rem : I.b;
+    if constexpr (SEL) {
+        const SelRows& s = p.sel;
+        I.split = static_cast<int>(s.by_rows.div(it));
+        const int r = it - I.split * s.rows, part = static_cast<int>(s.by_heads.div(r));
+        I.row = r - part * s.heads;
+        I.b = static_cast<int>(s.by_hkv.div(I.row));
+        I.kvh = I.row - I.b * p.Hkv;
+        I.hk = I.kvh * s.sub + part;
+        I.q0 = I.kvh * s.group + part * s.per;
+        I.nq = min(s.per, s.group - part * s.per);
+    } else {
+        const int per_split = p.B * p.Hkv;
+        I.split = it / per_split;
+        const int rem = it - I.split * per_split;
+        const int k = rem / p.Hkv;
+        I.hk = rem - k * p.Hkv;
+        I.b = p.order ? __ldg(p.order + k) : k;
+        I.row = I.b;
+        I.kvh = I.hk;
+    }
     const int len = seq_len_of(p, I.row);
     I.t_lo = I.split * p.span;
     I.t_hi = min(len, I.t_lo + p.span);
@@ -256,7 +284,7 @@ __device__ __forceinline__ PTile ptile_first(const GqaParams& p) {
     T.tt = 0;
     T.t0 = 0;
     T.n = 0;
-    T.I = GItem{0, 0, 0, 0, 0, 0, 0};
+    T.I = GItem{};
     if (T.it < p.n_items) {
         T.I = gqa_item<SEL>(p, T.it);
         T.t0 = T.I.t_lo;
@@ -296,7 +324,7 @@ __device__ __forceinline__ void ptile_scales(const GqaParams& p, const PTile& T,
     kq = make_float4(0.f, 0.f, 0.f, 0.f);
     vq = kq;
     if (T.it < p.n_items && tl < T.n && sblk >= 0 && sblk < p.nblk) {
-        const int64_t so = sblk * p.sc_sblk + T.I.hk * p.sc_sh + ((T.t0 + tl) & ((1 << p.lbs) - 1));
+        const int64_t so = sblk * p.sc_sblk + T.I.kvh * p.sc_sh + ((T.t0 + tl) & ((1 << p.lbs) - 1));
         kq = __ldcs(reinterpret_cast<const float4*>(p.ks + so));
         vq = __ldcs(reinterpret_cast<const float4*>(p.vs + so));
     }
@@ -326,7 +354,7 @@ __device__ __forceinline__ void gqa_producer_paged(const CUtensorMap* kmap, cons
         if (lane == 0) mbar_arrive_expect_tx(&bars[C::B_KFULL + sk], bytes);
         __syncwarp();
         if (lane < 16 && good)
-            tma_load_4d(smem + C::OFF_KR + sk * C::TILE_BYTES + tok * C::D, kmap, 0, (T.t0 + tok) & (bs - 1), T.I.hk,
+            tma_load_4d(smem + C::OFF_KR + sk * C::TILE_BYTES + tok * C::D, kmap, 0, (T.t0 + tok) & (bs - 1), T.I.kvh,
                         blk, &bars[C::B_KFULL + sk], pol);
         ++ik;
         return true;
@@ -371,9 +399,9 @@ __device__ __forceinline__ void gqa_producer_paged(const CUtensorMap* kmap, cons
         if (lane == 0) mbar_arrive_expect_tx(&bars[C::B_VFULL + sv], bytes);
         __syncwarp();
         if (good) {
-            const int64_t so = b0 * p.sc_sblk + T0.I.hk * p.sc_sh + off;
+            const int64_t so = b0 * p.sc_sblk + T0.I.kvh * p.sc_sh + off;
             if (lane < 16)
-                tma_load_4d(smem + C::OFF_VR + sv * C::TILE_BYTES + tok * C::D, vmap, 0, off, T0.I.hk, b0,
+                tma_load_4d(smem + C::OFF_VR + sv * C::TILE_BYTES + tok * C::D, vmap, 0, off, T0.I.kvh, b0,
                             &bars[C::B_VFULL + sv], pol);
             if (!small && lane == 0) bulk_g2s(dst, p.ks + so, seg, &bars[C::B_VFULL + sv], pol);
             if (!small && lane == 16) bulk_g2s(dst, p.vs + so, seg, &bars[C::B_VFULL + sv], pol);
@@ -633,11 +661,11 @@ __device__ __forceinline__ bool gqa_qlimbs(const GqaParams& p, uint8_t* smem, in
     float* red = reinterpret_cast<float*>(smem + C::OFF_RED) + wg * 256;
     const GItem I = gqa_item<C::SEL>(p, it);
     const int h0 = wg * HPW;
-    const int64_t q0 = I.b * p.q_sb + static_cast<int64_t>(I.hk * G + h0) * p.q_sh + r;
+    const int64_t q0 = I.b * p.q_sb + static_cast<int64_t>((C::PAD ? I.q0 : I.hk * G) + h0) * p.q_sh + r;
     float qv[HPW], am[HPW];
 #pragma unroll
     for (int h = 0; h < HPW; ++h) {
-        const float x = load_q(p.Q, q0 + h * p.q_sh, p.flags);
+        const float x = !C::PAD || h0 + h < I.nq ? load_q(p.Q, q0 + h * p.q_sh, p.flags) : 0.f;
         qv[h] = C::QI8 ? x : x * p.qscale;  // the int8 query is the raw row, quantised like a cache row
         am[h] = fabsf(qv[h]);
     }
@@ -790,7 +818,8 @@ __device__ __forceinline__ bool gqa_pv_epi(const GqaParams& p, uint8_t* smem, ui
         const bool records = split_row || (p.flags & KVD_FLAG_PARTIAL_OUT);
 #pragma unroll
         for (int h = 0; h < HPW; ++h) {
-            const int hq = I.hk * G + wg * HPW + h;
+            if (C::PAD && wg * HPW + h >= I.nq) continue;
+            const int hq = (C::PAD ? I.q0 : I.hk * G) + wg * HPW + h;
             const int64_t ro = I.b * p.o_sb + static_cast<int64_t>(hq) * p.o_sh;
             if constexpr (G <= kTagMaxGroup) {
                 if (p.tagged) {  // every row of a dense batch, P >= 1 records
@@ -1114,7 +1143,7 @@ __global__ void __launch_bounds__(1024) seq_order_kernel(const int32_t* seq_lens
 
 // Ragged batches: merge the split records of rows whose sequence had more
 // than one split (single-split rows were written by the decode kernel). Output
-// rows r*per_seq .. (r+1)*per_seq - 1 belong to sequence r.
+// row r is of sequence r / per_seq.
 __global__ void __launch_bounds__(128) gqa_ragged_combine_kernel(const float* partials, const int32_t* seq_lens,
                                                                  int Hq, int per_seq, int P, int span, int S, int D, void* out,
                                                                  int64_t o_sb, int64_t o_sh, uint32_t flags) {
@@ -1272,11 +1301,19 @@ cudaError_t launch_gqa_g(const CUtensorMap& km, const CUtensorMap& vm, const Gqa
 template <int G>
 cudaError_t launch_gqa_mode(int mode, const CUtensorMap& km, const CUtensorMap& vm, const GqaParams& p,
                             cudaStream_t st) {
-    if (mode == 2) return launch_gqa_g<G, 2>(km, vm, p, st);
+    if constexpr (G == 4 || G == 8)
+        if (mode == 3) return launch_gqa_g<G, 3>(km, vm, p, st);
+    if constexpr (G <= 8)
+        if (mode == 2) return launch_gqa_g<G, 2>(km, vm, p, st);
     return mode == 1 ? launch_gqa_g<G, 1>(km, vm, p, st) : launch_gqa_g<G, 0>(km, vm, p, st);
 }
 
 }  // namespace
+
+bool gqa_sel_ok(const kvd_decode_desc& d) {
+    return d.head_dim == 128 && d.max_seq_len >= 1 && static_cast<int64_t>(d.batch) * d.num_q_heads <= 0x7fffff &&
+           tensor_map_encoder() != nullptr;
+}
 
 bool gqa_path_ok(const kvd_decode_desc& d) {
     const int G = d.num_q_heads / d.num_kv_heads;
@@ -1292,6 +1329,17 @@ struct GqaPlan {
     int P, span;
     size_t order_bytes, rec_bytes;
 };
+
+// Query heads per work row of a decode over selected blocks: as few parts of
+// at most 8 as make up the group. (The form for 16 spills and took 139 us for
+// 112 rows of 9,536 tokens in 64-token blocks, two parts of 8 107 us; for 512
+// rows of 2,048 tokens in 16-token blocks 139 against 136 us.)
+void sel_heads(const kvd_decode_desc& d, int* sub, int* per, int* form) {
+    const int group = d.num_q_heads / d.num_kv_heads;
+    *sub = (group + 7) / 8;
+    *per = (group + *sub - 1) / *sub;
+    *form = *per > 4 ? 8 : *per > 2 ? 4 : *per;
+}
 
 GqaPlan plan_gqa(const kvd_decode_desc& d, size_t ws_limit, bool sel = false) {
     GqaPlan g{};
@@ -1309,7 +1357,13 @@ GqaPlan plan_gqa(const kvd_decode_desc& d, size_t ws_limit, bool sel = false) {
         while (span_tiles > 1 && units * ((s_tiles + span_tiles - 1) / span_tiles) < 4 * grid) span_tiles /= 2;
         if (span_tiles > s_tiles) span_tiles = s_tiles;
     } else {  // selections are as long as their budget, but for their last block
-        const int P0 = gqa_split_count(d);
+        kvd_decode_desc rows = d;
+        if (sel) {
+            int sub, per, form;
+            sel_heads(d, &sub, &per, &form);
+            rows.num_kv_heads = d.num_kv_heads * sub;
+        }
+        const int P0 = gqa_split_count(rows);
         span_tiles = (s_tiles + P0 - 1) / P0;
     }
     g.span = 128 * span_tiles;
@@ -1343,8 +1397,9 @@ cudaError_t launch_gqa_tc(const kvd_decode_desc& d, const void* Q, const int8_t*
                           const float* ks, const float* vs, void* out, void* ws, size_t ws_bytes,
                           cudaStream_t st, int* launches, const PagedView* pv, const AppendView* av,
                           SplitRecords* keep_splits) {
-    const int G = d.num_q_heads / d.num_kv_heads;
     const bool sel = pv && pv->per_head;
+    int G = d.num_q_heads / d.num_kv_heads, sub = 1, per = G;
+    if (sel) sel_heads(d, &sub, &per, &G);
     const GqaPlan g = plan_gqa(d, ws ? ws_bytes : 0, sel);
     const int S = d.max_seq_len;
     if (av && (pv || !g.order_bytes || !d.seq_lens)) return cudaErrorNotSupported;
@@ -1372,7 +1427,12 @@ cudaError_t launch_gqa_tc(const kvd_decode_desc& d, const void* Q, const int8_t*
     p.partials = g.rec_bytes ? reinterpret_cast<float*>(static_cast<char*>(ws) + g.order_bytes) : nullptr;
     p.seq_lens = d.seq_lens;
     p.B = d.batch; p.Hq = d.num_q_heads; p.Hkv = d.num_kv_heads; p.S = S; p.P = g.P; p.span = g.span;
-    p.n_items = d.batch * d.num_kv_heads * g.P;
+    p.n_items = d.batch * d.num_kv_heads * sub * g.P;
+    if (sel) {
+        const int heads = d.batch * d.num_kv_heads;
+        p.sel = SelRows{sub, per, d.num_q_heads / d.num_kv_heads, sub * heads, heads, FastDiv(sub * heads),
+                        FastDiv(heads), FastDiv(d.num_kv_heads)};
+    }
     const int64_t grid_max = static_cast<int64_t>(device_sm_count()) * kGqaCtas;
     p.grid = static_cast<int>(grid_max < p.n_items ? grid_max : p.n_items);
     p.sc_sb = d.sc_stride_b; p.sc_sh = d.sc_stride_h;
@@ -1408,7 +1468,7 @@ cudaError_t launch_gqa_tc(const kvd_decode_desc& d, const void* Q, const int8_t*
         if (e != cudaSuccess) return e;
         ++*launches;
     }
-    const int mode = sel ? 2 : (d.flags & KVD_FLAG_QK_INT8) ? 1 : 0;
+    const int mode = sel ? (sub * G == d.num_q_heads / d.num_kv_heads ? 2 : 3) : (d.flags & KVD_FLAG_QK_INT8) ? 1 : 0;
     switch (G) {
         case 1: e = launch_gqa_mode<1>(mode, km, vm, p, st); break;
         case 2: e = launch_gqa_mode<2>(mode, km, vm, p, st); break;
@@ -1439,7 +1499,7 @@ cudaError_t launch_gqa_tc(const kvd_decode_desc& d, const void* Q, const int8_t*
             cfg.numAttrs = 1;
             e = cudaLaunchKernelEx(
                 &cfg, gqa_ragged_combine_kernel, static_cast<const float*>(p.partials), d.seq_lens, d.num_q_heads,
-                sel ? G : d.num_q_heads, g.P, g.span, S, d.head_dim, out, d.o_stride_b, d.o_stride_h, d.flags);
+                sel ? d.num_q_heads / d.num_kv_heads : d.num_q_heads, g.P, g.span, S, d.head_dim, out, d.o_stride_b, d.o_stride_h, d.flags);
             if (e == cudaSuccess) ++*launches;
         } else {
             const int64_t rs = d.head_dim + 4;

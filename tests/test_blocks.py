@@ -653,6 +653,15 @@ def test_sparse_decode_lengths(D, G, bs, k):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("G", [3, 5, 6, 7, 9, 12, 16, 20, 33])
+@pytest.mark.parametrize("D,bs,k", [(128, 16, 20), (64, 16, 20)])
+def test_sparse_decode_groups(D, bs, k, G):
+    """Groups of query heads that are no power of two or above the kernels' forms, whole and split rows, records."""
+    _check_sparse(G, 2, 3, G, D, bs, k, [k * bs, 1, 77, 130, 200, k * bs - 3], "bthd", "bfloat16", "float32")
+    _check_sparse(G + 1, 1, 2, G, D, 64, 40, [2560, 2500], "bhtd", "float32", "float32", partial=True)
+
+
+@pytest.mark.gpu
 def test_sparse_decode_small_workspace_and_bad_ids():
     """Less scratch means fewer splits, not other results; a block id outside the pool is not read."""
     import torch
