@@ -290,9 +290,11 @@ extern "C" size_t kvd_sparse_workspace_size(const kvd_paged_desc* desc) {
     if (check_paged(desc) != cudaSuccess) return 0;
     PagedView pv;
     const kvd_decode_desc d = paged_as_dense(*desc, &pv);
-    const size_t gen = generic_workspace_size(d);
-    const size_t gqa = paged_tc_shape(*desc, d, true) ? gqa_workspace_size(d, true) : 0;
-    return gen > gqa ? gen : gqa;
+    // alignment, which the sizes do not show, may move a shape to the next kernel
+    size_t need = generic_workspace_size(d);
+    if (paged_tc_shape(*desc, d, true)) need = need > gqa_workspace_size(d, true) ? need : gqa_workspace_size(d, true);
+    const size_t group = sel_group_workspace_size(d);
+    return need > group ? need : group;
 }
 
 extern "C" cudaError_t kvd_sparse_decode_launch(const kvd_paged_desc* desc, const void* Q, const int8_t* K_pool,
@@ -313,6 +315,9 @@ extern "C" cudaError_t kvd_sparse_decode_launch(const kvd_paged_desc* desc, cons
     if (paged_tc_ok(*desc, d, Q, K_pool, V_pool, k_scale_pool, v_scale_pool, true))
         return launch_gqa_tc(d, Q, K_pool, V_pool, k_scale_pool, v_scale_pool, out, workspace, workspace_bytes,
                              stream, &tl_launches, &pv);
+    if (sel_group_ok(d, pv, K_pool, V_pool))
+        return launch_sel_group(d, Q, K_pool, V_pool, k_scale_pool, v_scale_pool, out, workspace, workspace_bytes,
+                                stream, &tl_launches, pv);
     return launch_generic(d, Q, K_pool, V_pool, k_scale_pool, v_scale_pool, out, workspace, workspace_bytes, stream,
                           &tl_launches, &pv);
 }

@@ -165,6 +165,12 @@ cudaError_t launch_generic(const kvd_decode_desc& d, const void* Q, const int8_t
                            void* ws, size_t ws_bytes, cudaStream_t st, int* launches,
                            const PagedView* pv = nullptr);
 size_t generic_workspace_size(const kvd_decode_desc& d);
+// Decode over selected blocks on CUDA cores (kvd_sel_group.cu).
+bool sel_group_ok(const kvd_decode_desc& d, const PagedView& pv, const int8_t* K, const int8_t* V);
+size_t sel_group_workspace_size(const kvd_decode_desc& d);
+cudaError_t launch_sel_group(const kvd_decode_desc& d, const void* Q, const int8_t* K, const int8_t* V,
+                             const float* ks, const float* vs, void* out, void* ws, size_t ws_bytes, cudaStream_t st,
+                             int* launches, const PagedView& pv);
 cudaError_t launch_combine_records(const float* base, int nparts, int64_t part_stride, int64_t rec_stride,
                                    int64_t rows, int rows_per_b, int D, void* out, int64_t o_sb, int64_t o_sh,
                                    uint32_t flags, cudaStream_t st, int* launches);
