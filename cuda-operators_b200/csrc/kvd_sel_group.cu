@@ -78,35 +78,50 @@ __global__ void __launch_bounds__(kSgThreads) sel_group_kernel(const SgParams p)
     const int quad = tid % QUADS, share = tid / QUADS;
     const int64_t v_at = p.V - p.K;
     const int32_t* table = p.table + row * p.bt_stride;
+    // A chunk's loads depend on one another (block id, then scales and codes), so they run ahead of
+    // their use: block ids two chunks, scales and K codes one, V codes across the scores.
+    auto block_at = [&](int c0) {
+        const int t = c0 + tok;
+        return t < t_hi ? table[p.by_bs.div(t)] : 0;
+    };
+    const int8_t* kr = p.K;
+    float ks = 0.f, vs = 0.f;
+    uint4 code[D / 32];
+    auto fetch = [&](int c0, int blk) {  // this thread's token of the chunk at c0
+        const int t = c0 + tok;
+        kr = p.K;
+        ks = vs = 0.f;
+        if (t >= t_hi) return;
+        const int off = t - static_cast<int>(p.by_bs.div(t)) * p.bs;
+        if (blk >= 0 && blk < p.nblk) {
+            kr = p.K + blk * p.kv_sblk + kvh * p.kv_sh + off * p.kv_st;
+            const int64_t sc = blk * p.sc_sblk + kvh * p.sc_sh + off;
+            ks = p.ks[sc];
+            vs = p.vs[sc];
+        } else {  // score 0 and value 0, as in the other kernels
+            record_status(KVD_STATUS_BAD_BLOCK);
+        }
+#pragma unroll
+        for (int i = 0; i < D / 32; ++i) code[i] = *reinterpret_cast<const uint4*>(kr + 32 * i + 16 * half);
+    };
+    int blk_next = 0;
+    if (t_lo < t_hi) {
+        fetch(t_lo, block_at(t_lo));
+        blk_next = block_at(t_lo + kSgTok);
+    }
     for (int c0 = t_lo; c0 < t_hi; c0 += kSgTok) {
         const int n = min(kSgTok, t_hi - c0);
-        // this thread's token; one past the split, or in a block outside the pool, weighs nothing
-        const int t = c0 + tok;
-        const int8_t* kr = p.K;
-        float ks = 0.f, vs = 0.f;
-        bool in = tok < n;
-        if (in) {
-            const int j = static_cast<int>(p.by_bs.div(t)), off = t - j * p.bs;
-            const int blk = table[j];
-            if (blk >= 0 && blk < p.nblk) {
-                kr = p.K + blk * p.kv_sblk + kvh * p.kv_sh + off * p.kv_st;
-                const int64_t sc = blk * p.sc_sblk + kvh * p.sc_sh + off;
-                ks = p.ks[sc];
-                vs = p.vs[sc];
-            } else {  // score 0 and value 0, as in the other kernels
-                record_status(KVD_STATUS_BAD_BLOCK);
-            }
-        }
+        const bool in = tok < n;
+        const float ks_now = ks, vs_now = vs;
         float2 dot[HP];
 #pragma unroll
         for (int h = 0; h < HP; ++h) dot[h] = make_float2(0.f, 0.f);
         __syncthreads();  // queries are there; the chunk before is done with w_s and the rows
         if (half == 0) vrow[tok] = kr + v_at;
-#pragma unroll 2
+#pragma unroll
         for (int i = 0; i < D / 32; ++i) {
             const int piece = 2 * i + half;
-            const uint4 code = in ? *reinterpret_cast<const uint4*>(kr + 16 * piece) : make_uint4(0u, 0u, 0u, 0u);
-            const uint32_t w[4] = {code.x, code.y, code.z, code.w};
+            const uint32_t w[4] = {code[i].x, code[i].y, code[i].z, code[i].w};
 #pragma unroll
             for (int x = 0; x < 4; ++x) {
                 float2 k0, k1;
@@ -119,16 +134,25 @@ __global__ void __launch_bounds__(kSgThreads) sel_group_kernel(const SgParams p)
                 }
             }
         }
+        fetch(c0 + kSgTok, blk_next);
+        blk_next = block_at(c0 + 2 * kSgTok);
         float s[HP];
 #pragma unroll
         for (int h = 0; h < HP; ++h) {
             float x = dot[h].x + dot[h].y;
             x += __shfl_xor_sync(0xffffffffu, x, 1);
-            s[h] = in ? x * ks : -INFINITY;
+            s[h] = in ? x * ks_now : -INFINITY;
             const float mx = redux_max(s[h]);
             if (lane == 0) red[warp][h] = mx;
         }
         __syncthreads();
+        constexpr int AHEAD = PER < 16 ? PER : 16;
+        uint32_t vcode[AHEAD];
+#pragma unroll
+        for (int i = 0; i < AHEAD; ++i) {
+            const int tt = share * PER + i;
+            vcode[i] = tt < n ? *reinterpret_cast<const uint32_t*>(vrow[tt] + 4 * quad) : 0u;
+        }
 #pragma unroll
         for (int h = 0; h < HP; ++h) {
             const float mx = fmaxf(fmaxf(red[0][h], red[1][h]), fmaxf(red[2][h], red[3][h]));
@@ -138,22 +162,27 @@ __global__ void __launch_bounds__(kSgThreads) sel_group_kernel(const SgParams p)
             m[h] = m_new;
             l[h] = l[h] * alpha + (half == 0 ? pr : 0.f);
             acc[h].x *= alpha; acc[h].y *= alpha; acc[h].z *= alpha; acc[h].w *= alpha;
-            if (half == 0) w_s[tok][h] = in ? pr * vs : 0.f;
+            if (half == 0) w_s[tok][h] = in ? pr * vs_now : 0.f;
         }
         __syncthreads();
-#pragma unroll 4
-        for (int i = 0; i < PER; ++i) {
-            const int tt = share * PER + i;
-            if (tt >= n) break;
-            const uint32_t code = *reinterpret_cast<const uint32_t*>(vrow[tt] + 4 * quad);
-            float2 v0, v1;
-            dequant4(code, v0, v1);
 #pragma unroll
-            for (int h = 0; h < HP; ++h) {
-                const float2 w = make_float2(w_s[tt][h], w_s[tt][h]);
-                const float2 a = __ffma2_rn(w, v0, make_float2(acc[h].x, acc[h].y));
-                const float2 c = __ffma2_rn(w, v1, make_float2(acc[h].z, acc[h].w));
-                acc[h] = make_float4(a.x, a.y, c.x, c.y);
+        for (int i0 = 0; i0 < PER; i0 += AHEAD) {
+#pragma unroll
+            for (int i = 0; i < AHEAD; ++i) {  // a token past the chunk: weight and code 0
+                const int tt = share * PER + i0 + i;
+                float2 v0, v1;
+                dequant4(vcode[i], v0, v1);
+                if (i0 + AHEAD < PER) {
+                    const int later = tt + AHEAD;
+                    vcode[i] = later < n ? *reinterpret_cast<const uint32_t*>(vrow[later] + 4 * quad) : 0u;
+                }
+#pragma unroll
+                for (int h = 0; h < HP; ++h) {
+                    const float2 w = make_float2(w_s[tt][h], w_s[tt][h]);
+                    const float2 a = __ffma2_rn(w, v0, make_float2(acc[h].x, acc[h].y));
+                    const float2 c = __ffma2_rn(w, v1, make_float2(acc[h].z, acc[h].w));
+                    acc[h] = make_float4(a.x, a.y, c.x, c.y);
+                }
             }
         }
     }
