@@ -8,8 +8,8 @@ a copy to the host:
     select  the blocks whose bounds promise the largest products, per KV head      kvdecode.block_select
     decode  attention of each request's new token over the selected blocks        kvdecode.sparse_decode
 
-Queries, keys and values are random (a key direction per request makes some blocks matter more than others,
-as contexts do); a model would compute them. Usage, on a B200 with the library built:
+Queries, keys and values are random (stretches of a prompt have keys along the direction of the request's
+queries, so that some blocks matter more than others); a model would compute them. Usage, on a B200 with the library built:
 
     python examples/paged_serving.py [--steps 40] [--batch 16] [--context 8192] [--budget 32]
 """
@@ -51,7 +51,8 @@ def serve(steps=40, batch=16, context=8192, budget=32, kv_heads=8, group=4, head
         kvd.paged_plan(lens, torch.tensor(new_lens, dtype=i32, device=dev), table, free, count, block_size, slots)
         if total:
             who = torch.repeat_interleave(torch.arange(batch, device=dev), torch.tensor(n, device=dev))
-            k = rnd(total, H, D) + topic[who] * (torch.rand((total, 1, 1), device=dev, generator=gen) < 0.02) * 2
+            hot = torch.arange(total, device=dev) // 200 % 16 == 3  # stretches of a prompt that are to the point
+            k = rnd(total, H, D) + topic[who] * hot.view(-1, 1, 1)
             kvd.paged_write(k, rnd(total, H, D), slots, k_pool, v_pool, ks, vs, bounds, bound_scale)
         if q is None:
             return None
@@ -63,7 +64,7 @@ def serve(steps=40, batch=16, context=8192, budget=32, kv_heads=8, group=4, head
     step(prompts)
     decoded = 0
     for i in range(steps):
-        q = rnd(batch, H * group, D) + topic.repeat_interleave(group, dim=1) * 0.5
+        q = rnd(batch, H * group, D) + topic.repeat_interleave(group, dim=1)
         new = [1] * batch
         if i % 10 == 9 and i + 1 < steps:  # a request ends; the next step starts another in its place
             new[i % batch] = -1
