@@ -33,7 +33,7 @@ struct ScoreCfg {
     static constexpr int NQ = NQ_;                     // heads, padded
     static constexpr int E = D / 32;                   // query values a lane quantises
     static constexpr int STAGES = SL == 4 && NQ > 16 ? 2 : 12 / SL;
-    static constexpr int LW = 4;                       // loading warps
+    static constexpr int LW = 8;                       // loading warps
     static constexpr int LAG = STAGES > 3 ? STAGES - 3 : 1;  // tiles between a tile's issue and the wait for it
     static constexpr int STEPS = 16;                   // tiles whose steps are kept: more than are under way (STAGES + 2)
     static constexpr int SLAB = 128 * 128;             // 128 blocks x 128 bytes
@@ -178,7 +178,7 @@ __device__ __forceinline__ void score_loader(const SelectParams& p, uint8_t* sme
     constexpr int LAG = C::LAG, ROWS = 128 / C::LW;
     constexpr int PIECES = SL * 8;    // 16-byte pieces of a row
     constexpr int RPI = 32 / PIECES;  // rows an instruction covers
-    static_assert(ROWS == 32, "a lane per row");
+    static_assert(ROWS <= 32, "a lane per row");
     uint64_t* bars = reinterpret_cast<uint64_t*>(smem + C::OFF_BAR);
     const int lane = threadIdx.x & 31, H = p.d.num_kv_heads;
     const int sub = lane / PIECES, piece = lane % PIECES;
@@ -230,14 +230,20 @@ __device__ __forceinline__ void score_loader(const SelectParams& p, uint8_t* sme
             uint32_t rid[ROWS / RPI];  // all shuffles first: one before each copy would wait for it
 #pragma unroll
             for (int j = 0; j < ROWS / RPI; ++j) rid[j] = __shfl_sync(0xffffffffu, id, j * RPI + sub);
-#pragma unroll
-            for (int j = 0; j < ROWS; j += RPI) {
+            auto copy = [&](int j) {
                 cp_async16(dst[(j & 7) / RPI] + j * 128, bounds + static_cast<uint64_t>(rid[j / RPI]) * stride);
-                if (j + RPI >= left && left < ROWS) break;  // no rows behind: the same for the whole warp
+            };
+            if (left >= ROWS) {
+#pragma unroll
+                for (int j = 0; j < ROWS; j += RPI) copy(j);
+            } else {
+#pragma unroll
+                for (int j = 0; j < ROWS; j += RPI)
+                    if (j < left) copy(j);  // the same for the whole warp
             }
             float* step = reinterpret_cast<float*>(smem + C::OFF_STEP) + step_in.s * 128 + w * ROWS + lane;
-            if (good) cp_async4(smem_u32(step), p.bound_scale + static_cast<int64_t>(id) * H + I.h);
-            else *step = -1.f;  // no block: below every score
+            if (good && lane < ROWS) cp_async4(smem_u32(step), p.bound_scale + static_cast<int64_t>(id) * H + I.h);
+            else if (lane < ROWS) *step = -1.f;  // no block: below every score
             cp_async_commit();
             step_in.next();
             in.next();
