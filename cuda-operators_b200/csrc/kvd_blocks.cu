@@ -430,6 +430,14 @@ __device__ __forceinline__ float2 quotient(float2 x, float2 ns, float2 yy) {
     return __fadd2_rn(q, make_float2(kRound, kRound));
 }
 
+// The same for 16-bit values, by the reciprocal in two parts, y + ye with
+// ye = (1 - s y) y: q = x y + (x ye), three operations instead of six. Equal to
+// the division's codes for all pairs of 8-bit and of 11-bit significands of
+// value and maximum and all exponents between them (checked exhaustively).
+__device__ __forceinline__ float2 quotient16(float2 x, float2 yy, float2 ye) {
+    return __fadd2_rn(__ffma2_rn(x, yy, __fmul2_rn(x, ye)), make_float2(kRound, kRound));
+}
+
 // The K and V rows that a warp holds (LPR lanes each), by the rule of
 // kvd_quant.cuh: code words, the scales of the lane's rows, and in `code` the
 // K codes as floats.
@@ -479,15 +487,19 @@ __device__ __forceinline__ void quantise_pair(const Pack<T>& pk, const Pack<T>& 
     sk = __shfl_sync(0xffffffffu, s, mine);
     sv = __shfl_sync(0xffffffffu, s, mine + 1);
     const float yk = __shfl_sync(0xffffffffu, y, mine), yv = __shfl_sync(0xffffffffu, y, mine + 1);
+    auto row = [](const Pack<T>& x, float s1, float y1, float2 (&e)[4]) {
+        const float ye = fmaf(-s1, y1, 1.0f) * y1;
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            e[j] = sizeof(T) == 2 ? quotient16(x.pair(j), make_float2(y1, y1), make_float2(ye, ye))
+                                  : quotient(x.pair(j), make_float2(-s1, -s1), make_float2(y1, y1));
+    };
     float2 e[4];
+    row(pk, sk, yk, e);
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-        e[j] = quotient(pk.pair(j), make_float2(-sk, -sk), make_float2(yk, yk));
-        code[j] = __fadd2_rn(e[j], make_float2(-kRound, -kRound));
-    }
+    for (int j = 0; j < 4; ++j) code[j] = __fadd2_rn(e[j], make_float2(-kRound, -kRound));
     kw = make_uint2(low_bytes(e[0], e[1]), low_bytes(e[2], e[3]));
-#pragma unroll
-    for (int j = 0; j < 4; ++j) e[j] = quotient(pv.pair(j), make_float2(-sv, -sv), make_float2(yv, yv));
+    row(pv, sv, yv, e);
     vw = make_uint2(low_bytes(e[0], e[1]), low_bytes(e[2], e[3]));
 }
 
