@@ -515,7 +515,7 @@ constexpr int kRowWarps = 4;
 // first rows are loaded beside the slots, before the run is known.
 // Bound: HBM for long maps, the chain of dependent loads for short ones.
 template <class T, int LPR, int W>
-__global__ void __launch_bounds__(32 * W, LPR ? 24 / W : 1) write_kernel(const RowsParams p) {
+__global__ void __launch_bounds__(32 * W, LPR ? (W == 1 ? 20 : 24 / W) : 1) write_kernel(const RowsParams p) {
     using R = Rows<LPR>;
     constexpr int E = R::E, STEP = W * R::N;
     extern __shared__ float write_smem[];  // [W][2][D] bounds of each warp
