@@ -849,12 +849,28 @@ __global__ void __launch_bounds__(32 * kRowWarps) read_kernel(const RowsParams p
 }
 
 template <class T, int LPR>
-cudaError_t launch_rows(const RowsParams& p, bool write, cudaStream_t st) {
+cudaError_t launch_rows(RowsParams& p, bool write, cudaStream_t st) {
     const kvd_paged_rows_desc& d = p.d;
     const int64_t rows = static_cast<int64_t>(d.num_tokens) * d.num_kv_heads;
     if (write) {
+        // One warp a CTA, or four that share a run. In us, bf16 rows of 8 heads x 128, one warp | four, for
+        // rows that each lie in a block of their own (decode: a run of one and the block's earlier tokens)
+        // and for whole blocks (prompt):
+        //   block_size   decode 256  decode 1,000   prompt 250   prompt 5,000  prompt 20,000
+        //       16         7.6 | 17     21 | 56      6.3 |  7.2     13 | 22       38 | 62
+        //       32         9.1 | 18     25 | 62      9.1 |  7.9     18 | 17       35 | 44
+        //       64          12 | 20     38 | 68       15 |  9.4     27 | 17       34 | 38
+        //      128          19 | 21     67 | 88       25 |  13      41 | 23       57 | 43
+        // Between, blocks of 33 to 127 tokens, small calls are taken for decode steps.
+        const bool one = LPR && (d.block_size <= 32 || (d.block_size < 128 && rows <= 24 * device_sm_count()));
+        // Tiles: about the CTAs that the GPU holds at once (20 of one warp an SM), or twice as many (6 of four):
+        // with 10 or 40 of one warp 1,000 decode rows took 31 or 19 us, 5,000 prompt rows 16 or 18; with 6 or
+        // 24 of four 256 decode rows in blocks of 128 took 28 or 24 us, 20,000 prompt rows 40 or 47.
+        const int64_t per = rows / ((one ? 20 : 12) * device_sm_count());
+        const int most = d.block_size < 64 ? 64 : d.block_size > 256 ? 256 : d.block_size;
+        p.tile = static_cast<int>(per < 1 ? 1 : per > most ? most : per);
         const int64_t grid = static_cast<int64_t>((d.num_tokens + p.tile - 1) / p.tile) * d.num_kv_heads;
-        if (LPR && rows <= 24 * device_sm_count())
+        if (one)
             return launch_after(write_kernel<T, LPR, 1>, static_cast<unsigned>(grid), 32, 0, st, p);
         return launch_after(write_kernel<T, LPR, kRowWarps>, static_cast<unsigned>(grid), 32 * kRowWarps,
                             sizeof(float) * kRowWarps * 2 * d.head_dim, st, p);
@@ -867,7 +883,7 @@ cudaError_t launch_rows(const RowsParams& p, bool write, cudaStream_t st) {
 }
 
 template <class T>
-cudaError_t launch_rows_t(const RowsParams& p, bool write, bool vec, cudaStream_t st) {
+cudaError_t launch_rows_t(RowsParams& p, bool write, bool vec, cudaStream_t st) {
     if (vec && p.d.head_dim == 64) return launch_rows<T, 8>(p, write, st);
     if (vec && p.d.head_dim == 128) return launch_rows<T, 16>(p, write, st);
     if (vec && p.d.head_dim == 256) return launch_rows<T, 32>(p, write, st);
@@ -1247,9 +1263,6 @@ extern "C" cudaError_t kvd_paged_write_launch(const kvd_paged_rows_desc* desc, c
         return cudaErrorInvalidValue;
     RowsParams p{*desc, k_new, v_new, nullptr, nullptr, slot_map, K_pool, V_pool, k_scale_pool, v_scale_pool,
                  bounds, bound_scale, 1, FastDiv(), FastDiv(), 0};
-    const int64_t per = static_cast<int64_t>(desc->num_tokens) * desc->num_kv_heads / (24 * device_sm_count());
-    const int most = desc->block_size < 64 ? 64 : desc->block_size > 256 ? 256 : desc->block_size;
-    p.tile = static_cast<int>(per < 1 ? 1 : per > most ? most : per);
     return rows_call(p, k_new, v_new, true, stream);
 }
 
