@@ -36,7 +36,11 @@ cudaError_t launch_after(void (*kern)(A...), unsigned grid, unsigned block, size
 // the sums all writes run in parallel. Every CTA makes the sums itself (8 bytes
 // a request from L2, an exchange through shared memory a sum) and writes its
 // share, a slot per thread where that many threads fit on the GPU. Bound:
-// latency, a chain of three loads and the sums' barriers. Lengths and the count
+// latency, a chain of three loads and the sums' barriers: 3.3 us for 8 requests
+// and 8.2 us for 1,024 with 65,536 new tokens (one CTA alone: 5.2 and 16.4).
+// Up to 256 requests a CTA has 256 threads, above that 1,024: 8 requests take
+// 3.3 us with 256 and 4.1 with 1,024, 512 take 5.5 and 4.8, 4,096 take 21 and
+// 12. Lengths and the count
 // may alias the inputs: the CTA that was last to read the inputs writes them,
 // at its end; the others have counted themselves right after reading.
 constexpr int kPlanMaxBatch = 8192;
@@ -513,7 +517,13 @@ constexpr int kRowWarps = 4;
 // the bounds cost no second pass and no exchange between CTAs. Heads are the
 // fast index of the grid: CTAs that run together read neighbouring rows. The
 // first rows are loaded beside the slots, before the run is known.
-// Bound: HBM for long maps, the chain of dependent loads for short ones.
+// Bound: for long maps the instructions (59 % of the issue slots, the half-rate
+// integer pipe above all, at 24 warps an SM: 32,768 bf16 rows x 8 heads of 128 in
+// blocks of 64 take 70.5 us, 58.4 of them without bounds; their 204 MB would
+// take 31 at the copy rate); for short ones the chain of dependent loads (256
+// decode rows: 5.9 us, 3.2 without bounds). CTAs of four warps: six an SM (80
+// registers); five, seven and eight took 93, 89 and 93 us when six took 82.
+// CTAs of one: 20 an SM, 256 decode rows 5.9 us, with 24 7.0.
 template <class T, int LPR, int W>
 __global__ void __launch_bounds__(32 * W, LPR ? (W == 1 ? 20 : 24 / W) : 1) write_kernel(const RowsParams p) {
     using R = Rows<LPR>;
@@ -780,14 +790,18 @@ __global__ void __launch_bounds__(32 * W, LPR ? (W == 1 ? 20 : 24 / W) : 1) writ
 }
 
 // Reads: rows (token, head) in order, a warp holding U times R::N neighbours,
-// their codes as loaded until all loads are under way. Bound: HBM.
-template <int LPR>
-constexpr int kReadRows = LPR ? 2 : 1;
+// their codes as loaded until all loads are under way. 16-bit outputs: two
+// rows a lane take 43.9 us for 32,768 x 8 rows of 128 (201 MB, 4.6 TB/s; a
+// plain copy of 134 MB, as many bytes written, takes 41.9), one 47.2, three
+// 46.1; 32-bit ones: two take 7.9 us for 2,000 x 8 rows, one 6.2. Bound: HBM,
+// two thirds of the bytes being writes.
+template <class T, int LPR>
+constexpr int kReadRows = LPR && sizeof(T) == 2 ? 2 : 1;
 
 template <class T, int LPR>
 __global__ void __launch_bounds__(32 * kRowWarps) read_kernel(const RowsParams p) {
     using R = Rows<LPR>;
-    constexpr int E = R::E, U = kReadRows<LPR>;
+    constexpr int E = R::E, U = kReadRows<T, LPR>;
     grid_dependency_wait();
     allow_dependents();
     const kvd_paged_rows_desc& d = p.d;
@@ -875,7 +889,7 @@ cudaError_t launch_rows(RowsParams& p, bool write, cudaStream_t st) {
         return launch_after(write_kernel<T, LPR, kRowWarps>, static_cast<unsigned>(grid), 32 * kRowWarps,
                             sizeof(float) * kRowWarps * 2 * d.head_dim, st, p);
     }
-    const int64_t per = kRowWarps * Rows<LPR>::N * kReadRows<LPR>;
+    const int64_t per = kRowWarps * Rows<LPR>::N * kReadRows<T, LPR>;
     int64_t grid = (rows + per - 1) / per;
     const int64_t most = static_cast<int64_t>(device_sm_count()) * 16;
     if (grid > most) grid = most;
@@ -921,7 +935,9 @@ cudaError_t rows_call(RowsParams& p, const void* a, const void* b, bool write, c
 // spread evenly over the GPU whatever the lengths are, then one CTA per
 // (request, KV head) that finds the threshold and writes the table.
 
-// Scores for any head_dim: a warp a CTA, query codes in shared memory.
+// Scores for head dims other than 64, 128 and 256 and groups of more than 64
+// heads: a warp a CTA, query codes in shared memory. Bound: instructions; 16 x
+// 512 blocks x 8 heads of 128 take 97 us, by tensor cores 12.
 __global__ void __launch_bounds__(32) score_any_kernel(const SelectParams p) {
     extern __shared__ int8_t any_smem[];  // [G][D] codes, padded to 4, then [G] scales
     const kvd_block_select_desc& d = p.d;
@@ -981,7 +997,11 @@ __global__ void __launch_bounds__(32) score_any_kernel(const SelectParams p) {
 // find it instead. Each warp owns a stretch of the row's blocks, so the places
 // of its blocks follow from counts. A row of up to kPickKept blocks is held in
 // registers, keys and pool ids, from one load to the end; longer rows are read
-// again from L2. Bound: latency, three loads in a row and seven barriers.
+// again from L2. Bound: latency, three loads in a row and seven barriers, and
+// for many rows the instructions (56 % of the issue slots).
+// With the scores, 64 requests x 8 heads x 4,096 blocks take 87 us, about 17 of
+// them here: 99 when rows are read again, 94 by radix passes alone; one row of
+// 8,192 blocks a head takes 29 and 37 by radix passes.
 constexpr int kPickThreads = 256;
 constexpr int kPickWarps = kPickThreads / 32;
 constexpr int kPickEach = 16;

@@ -509,6 +509,54 @@ def test_write_skips_and_odd_rows():
     assert kvd.device_status() == 0
 
 
+def _quotient_rows(dtype, rng):
+    """Rows of 128 whose first value is the largest: every significand of the maximum (a sample of float32's), with
+    values of every exponent at which a code can be other than 0, and around the halves between codes."""
+    bits = {"bfloat16": 7, "float16": 10, "float32": 23}[dtype]
+    sigs = 1 << bits
+    top = np.arange(sigs) if sigs <= 1024 else rng.integers(0, sigs, 2000)
+    rows = []
+    for e in range(10):
+        for base in ((-50, 0, 50) if dtype != "float16" else (4,)):
+            val = np.sort(rng.choice(sigs, size=127, replace=False)) if sigs <= 1024 else rng.integers(0, sigs, (len(top), 127))
+            val = np.broadcast_to(val, (len(top), 127))
+            x = np.ldexp(1.0 + val / sigs, base - e)
+            lead = np.ldexp(1.0 + top / sigs, base)[:, None]
+            rows.append(np.concatenate([lead, np.minimum(x, lead)], 1))
+    if dtype == "float32":  # within three units in the last place of a half
+        lead = rows[0][:, :1].astype(np.float32)
+        half = (lead / np.float32(127.0)).astype(np.float64) * (np.arange(127) + 0.5)
+        near = half.astype(np.float32).view(np.int32) + rng.integers(-3, 4, half.shape, dtype=np.int32)
+        rows.append(np.concatenate([lead, np.minimum(near.view(np.float32), lead)], 1))
+    x = np.concatenate(rows).astype(np.float32)
+    return x * np.where(rng.random(x.shape) < 0.5, -1, 1).astype(np.float32)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["bfloat16", "float16", "float32"])
+def test_write_quotients_are_the_divisions(dtype):
+    """Codes and scales equal the IEEE division's bit for bit, also where a quotient lies on or beside a half."""
+    import torch
+
+    x = _quotient_rows(dtype, np.random.default_rng(11))
+    x = x[: x.shape[0] // 16 * 16]
+    k = torch.from_numpy(x).to(getattr(torch, dtype))
+    assert torch.equal(k.float(), torch.from_numpy(x))  # all representable
+    k = k[:, None]
+    v = k.flip(0).contiguous()
+    NB = x.shape[0] // 16
+    slots = torch.arange(x.shape[0], dtype=torch.int64)
+    tk, tv, ts = k.to(DEV), v.to(DEV), slots.to(DEV)
+    K, V = (torch.full((NB, 1, 16, 128), 77, dtype=torch.int8, device=DEV) for _ in range(2))
+    ks, vs = (torch.full((NB, 1, 16), -1.0, device=DEV) for _ in range(2))
+    kvd.paged_write(tk, tv, ts, K, V, ks, vs)
+    codes, scales = po.quantize_rows(x)
+    _same_bits(K.reshape(-1, 128), codes, "K")
+    _same_bits(ks.reshape(-1), scales, "ks")
+    _same_bits(V.reshape(-1, 128), codes[::-1].copy(), "V")
+    _same_bits(vs.reshape(-1), scales[::-1].copy(), "vs")
+
+
 @pytest.mark.gpu
 def test_write_strided_rows_and_streams():
     """Rows that are a part of a wider tensor (vector and scalar access), on a stream that is not the default."""
