@@ -46,6 +46,9 @@ namespace kvd {
 // `sub` parts of `per` heads (the last may have fewer) that each read the
 // head's blocks; work rows are (part, b, kv head). Heads that a row's form of
 // the kernel has beyond the part's are zero queries whose output is dropped.
+// Bound: HBM. 256 x 8 rows of 2,048 tokens, group 8 (1,117 MB): 221 us in blocks
+// of 16, where a K or V box is 2 KB, 197, 192 and 191 us in blocks of 32, 64 and
+// 128 (5.0 to 5.8 TB/s); the paged decode of as many tokens takes 217 to 193.
 struct SelRows {
     int sub, per, group;  // sub * per >= group
     int rows, heads;      // rows = sub * heads, heads = B * Hkv

@@ -279,10 +279,10 @@ typedef struct kvd_paged_rows_desc {
  * max_t x_td, lo_d = min_t x_td and step = max_d max(|hi_d|, |lo_d|) / 127,
  * codes are clamp(ceil(hi_d / step)) then clamp(floor(lo_d / step)), clamped
  * to +-127 (step 0: codes 0). A token scale that is not finite makes step NaN
- * and the codes 0, so that the block is always selected; steps are not negative. Tokens of one block
- * come in order, with no other block's token between them, as
- * kvd_paged_plan_launch lays them out; places of the block in front of the last
- * one that the map leaves out hold earlier tokens. */
+ * and the codes 0, so that the block is always selected; steps are not
+ * negative. Tokens of one block come in order, with no other block's token
+ * between them, as kvd_paged_plan_launch lays them out; places of the block in
+ * front of the last one that the map leaves out hold earlier tokens. */
 cudaError_t kvd_paged_write_launch(const kvd_paged_rows_desc* desc, const void* k_new, const void* v_new,
                                    const int64_t* slot_map, int8_t* K_pool, int8_t* V_pool, float* k_scale_pool,
                                    float* v_scale_pool, int8_t* bounds, float* bound_scale, cudaStream_t stream);
@@ -330,7 +330,10 @@ cudaError_t kvd_block_select_launch(const kvd_block_select_desc* desc, const voi
  * desc->seq_lens is [batch][num_kv_heads] and desc->block_table
  * [batch][num_kv_heads][block_table_stride] (sel_lens and sel_table above, with
  * max_blocks_per_seq = budget). All blocks in front of a row's last one count
- * as full. KVD_FLAG_QK_INT8 returns cudaErrorNotSupported. */
+ * as full. Any group size. head_dim 128 with pools that the paged decode's
+ * tensor-core kernel takes runs on that kernel, head_dim 64, 128 and 256
+ * otherwise on a CUDA-core kernel (pools on 16-byte boundaries), any other on
+ * the generic kernel. KVD_FLAG_QK_INT8 returns cudaErrorNotSupported. */
 size_t kvd_sparse_workspace_size(const kvd_paged_desc* desc);
 cudaError_t kvd_sparse_decode_launch(const kvd_paged_desc* desc,
                                      const void* Q, const int8_t* K_pool, const int8_t* V_pool,
