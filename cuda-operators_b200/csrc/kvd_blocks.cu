@@ -1006,7 +1006,7 @@ constexpr int kPickThreads = 256;
 constexpr int kPickWarps = kPickThreads / 32;
 constexpr int kPickEach = 16;
 constexpr int kPickKept = kPickThreads * kPickEach;
-constexpr int kPickList = 512;
+constexpr int kPickList = kPickThreads;  // keys whose ranks are counted, a thread each
 
 struct PickShared {
     uint32_t hist[kPickThreads];

@@ -639,6 +639,26 @@ def test_select_ties_and_odd_values(MB):
     assert kvd.device_status() == kvd.KVD_STATUS_BAD_BLOCK
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("MB", [3000, 6000])
+def test_select_crowds_at_the_threshold(MB):
+    """A crowd of 100 to 600 blocks with scores next to one another, and the budget ends in it."""
+    crowds = [100, 255, 256, 257, 300, 400, 511, 512, 513, 600]
+    rng = np.random.default_rng(MB)
+    B, bs = len(crowds), 16
+    q, bounds, step, table, lens = select_inputs(2, B, 1, 2, 128, bs, MB, [MB * bs] * B)
+    same = np.broadcast_to(bounds[:1], bounds.shape).copy()
+    for b, m in enumerate(crowds):
+        mine = rng.uniform(0.0, 50.0, MB)
+        where = rng.permutation(np.arange(1, MB - 2))
+        mine[where[:m]] = rng.uniform(100.0, 100.2, m)
+        mine[where[m]] = 200.0
+        step[table[b], 0] = mine
+    for k in (3 + 1 + 7, 3 + 1 + 60, 3 + 1 + 99):
+        _check_select(q, same, step, table, lens, bs, k, 1, 2)
+    assert kvd.device_status() == 0
+
+
 def _check_sparse(seed, B, H, G, D, bs, k, lens, layout, qtype="float32", otype="float32", spare=5, partial=False, ws=None):
     import torch
 
