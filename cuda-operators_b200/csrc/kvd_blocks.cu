@@ -985,7 +985,7 @@ __global__ void __launch_bounds__(32) score_any_kernel(const SelectParams p) {
                 const float v = static_cast<float>(__reduce_add_sync(0xffffffffu, acc)) * scale[g];
                 best = fmaxf(best, isnan(v) ? INFINITY : v);
             }
-            if (lane == 0) keys[i] = id < 0 ? 0u : score_key(best * p.bound_scale[at]);
+            if (lane == 0) keys[i] = id < 0 ? kNoBlockKey : score_key(best * p.bound_scale[at]);
         }
     }
 }
@@ -995,31 +995,39 @@ __global__ void __launch_bounds__(32) score_any_kernel(const SelectParams p) {
 // few keys as a rule; their ranks then give it exactly. Where the bin holds
 // too many (equal or very uneven scores), 8-bit radix passes over the keys
 // find it instead. Each warp owns a stretch of the row's blocks, so the places
-// of its blocks follow from counts. A row of up to kPickKept blocks is held in
+// of its blocks follow from counts. A row of up to 16 blocks a thread is held in
 // registers, keys and pool ids, from one load to the end; longer rows are read
-// again from L2. Bound: latency, three loads in a row and seven barriers, and
-// for many rows the instructions (56 % of the issue slots).
-// With the scores, 64 requests x 8 heads x 4,096 blocks take 87 us, about 17 of
-// them here: 99 when rows are read again, 94 by radix passes alone; one row of
-// 8,192 blocks a head takes 29 and 37 by radix passes.
-constexpr int kPickThreads = 256;
-constexpr int kPickWarps = kPickThreads / 32;
-constexpr int kPickEach = 16;
-constexpr int kPickKept = kPickThreads * kPickEach;
-constexpr int kPickList = kPickThreads;  // keys whose ranks are counted, a thread each
+// again from L2. 256 threads where the table has up to 4,096 blocks a row, above
+// that 1,024. Bound: latency, three loads in a row and seven barriers, and for
+// many rows the instructions (46 % of the issue slots, four CTAs an SM).
+// With the scores, 64 requests x 8 heads x 4,096 blocks take 83 us, about 13 of
+// them here: 92 when rows are read again, 87 by radix passes alone, 93 with 1,024
+// threads a row. One request of 256 blocks a head takes 7.5 us (9.0 with 1,024
+// threads), of 4,096 blocks 11.4 (11.1), of 8,192 15.6 (29 with 256).
+constexpr int kPickEach = 16;  // keys a thread holds
 
+template <int THREADS>
 struct PickShared {
-    uint32_t hist[kPickThreads];
-    uint32_t list[kPickList];
-    uint32_t range[2][kPickWarps];
-    uint32_t scan[kPickWarps];
+    static constexpr int WARPS = THREADS / 32;
+    uint32_t hist[THREADS];  // a bin a thread
+    uint32_t list[THREADS];  // keys whose ranks are counted, a thread each
+    uint32_t range[2][WARPS];
+    uint32_t scan[WARPS];
     uint32_t pick[3], found[2], listed;
-    uint32_t count[2][kPickWarps];
+    uint32_t count[2][WARPS];
 };
 
+// Sum of a number of each warp in front of this one.
+template <int WARPS>
+__device__ __forceinline__ uint32_t before_warp(const uint32_t (&of)[WARPS]) {
+    const int lane = threadIdx.x & 31;
+    return __reduce_add_sync(0xffffffffu, lane < static_cast<int>(threadIdx.x >> 5) ? of[lane % WARPS] : 0u);
+}
+
 // The bin (a thread each) that the need-th best key lies in: pick = bin, keys above it, keys in it.
-__device__ __forceinline__ void find_bin(PickShared& s, uint32_t need) {
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, bin = kPickThreads - 1 - tid;
+template <int THREADS>
+__device__ __forceinline__ void find_bin(PickShared<THREADS>& s, uint32_t need) {
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, bin = THREADS - 1 - tid;
     const uint32_t mine = s.hist[bin];
     uint32_t upto = mine;
 #pragma unroll
@@ -1029,9 +1037,7 @@ __device__ __forceinline__ void find_bin(PickShared& s, uint32_t need) {
     }
     if (lane == 31) s.scan[warp] = upto;
     __syncthreads();
-#pragma unroll
-    for (int w = 0; w < kPickWarps; ++w)
-        if (w < warp) upto += s.scan[w];
+    upto += before_warp(s.scan);
     if (upto >= need && upto - mine < need) {
         s.pick[0] = bin;
         s.pick[1] = upto - mine;
@@ -1040,78 +1046,91 @@ __device__ __forceinline__ void find_bin(PickShared& s, uint32_t need) {
     __syncthreads();
 }
 
-template <bool KEPT>
-__device__ __forceinline__ void pick_row(const SelectParams& p, PickShared& s, int row, int n, const int32_t* table) {
+template <bool KEPT, int THREADS>
+__device__ __forceinline__ void pick_row(const SelectParams& p, PickShared<THREADS>& s, int row, int n,
+                                         const int32_t* table) {
+    constexpr int WARPS = THREADS / 32;
     const kvd_block_select_desc& d = p.d;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const uint32_t* all = p.keys + static_cast<int64_t>(row) * d.max_blocks_per_seq;
     int32_t* out = p.sel_table + static_cast<int64_t>(row) * d.budget;
-    const int seg = ((n + kPickWarps - 1) / kPickWarps + 31) & ~31;  // KEPT: at most 32 * kPickEach
+    const int seg = ((n + WARPS - 1) / WARPS + 31) & ~31;  // KEPT: at most 32 * kPickEach
     const int s0 = min(n, warp * seg), s1 = min(n, s0 + seg);
     const int lo = d.first, hi = n - d.last;  // scored blocks: [lo, hi); the others are always selected
-    uint32_t key[kPickEach];
+    // Keys of blocks that are always selected and of places past the end: above and below all others.
+    constexpr uint32_t kAlways = 0xffffffffu, kOutside = 0u;
+    auto key_at = [&](int i) {
+        const uint32_t k = i < s1 ? all[i] : kOutside;
+        return i < s1 && (i < lo || i >= hi) ? kAlways : k;
+    };
+    auto scored = [](uint32_t k) { return k - 1u < kAlways - 1u; };
+    uint32_t key[kPickEach], bins[kPickEach / 2] = {};  // bins: 16 bits a key
     int id[kPickEach];
     if constexpr (KEPT) {
 #pragma unroll
         for (int j = 0; j < kPickEach; ++j) {
             const int i = s0 + 32 * j + lane;
-            key[j] = i < s1 ? all[i] : 0u;
+            key[j] = key_at(i);
             id[j] = i < s1 ? table[i] : 0;
         }
     }
-    // fn(block, key, pool id) for this warp's blocks in order, all lanes together; past the end block = n
-    auto each = [&](auto fn, bool with_id) {
+    // fn(j, key) for this warp's blocks s0 + 32 j + lane in order, all lanes together
+    auto each = [&](auto fn) {
         if constexpr (KEPT) {
 #pragma unroll
             for (int j = 0; j < kPickEach; ++j) {
                 if (s0 + 32 * j >= s1) break;
-                const int i = s0 + 32 * j + lane;
-                fn(i < s1 ? i : n, key[j], id[j]);
+                fn(j, key[j]);
             }
         } else {
-            for (int i = s0 + lane; i - lane < s1; i += 32)
-                fn(i < s1 ? i : n, i < s1 ? all[i] : 0u, with_id && i < s1 ? table[i] : 0);
+#pragma unroll 4
+            for (int j = 0; s0 + 32 * j < s1; ++j) fn(j, key_at(s0 + 32 * j + lane));
         }
     };
     constexpr uint32_t kInf = 0xff800000u, kNegInf = 0x007fffffu;  // keys of +inf and -inf
     uint32_t kmin = 0xffffffffu, kmax = 0u;
-    each([&](int i, uint32_t k, int) {
-        if (i >= lo && i < hi && k < kInf && k > kNegInf) {
+    each([&](int, uint32_t k) {
+        if (k - (kNegInf + 1) < kInf - (kNegInf + 1)) {
             kmin = min(kmin, k);
             kmax = max(kmax, k);
         }
-    }, false);
+    });
     kmin = __reduce_min_sync(0xffffffffu, kmin);
     kmax = __reduce_max_sync(0xffffffffu, kmax);
     if (lane == 0) { s.range[0][warp] = kmin; s.range[1][warp] = kmax; }
     __syncthreads();
-    kmin = __reduce_min_sync(0xffffffffu, s.range[0][lane % kPickWarps]);
-    kmax = __reduce_max_sync(0xffffffffu, s.range[1][lane % kPickWarps]);
+    kmin = __reduce_min_sync(0xffffffffu, s.range[0][lane % WARPS]);
+    kmax = __reduce_max_sync(0xffffffffu, s.range[1][lane % WARPS]);
     // Bin of a key: scores clamped to the finite ones' range, evenly divided, rounded by the addition
     // of 2^23 (a bin a thread). It never falls where the key rises. A range that is empty, or whose
     // width or reciprocal overflows, leaves few bins in use, with products that may be infinite or
     // NaN: those all end in the last bin.
     const bool some = kmin <= kmax;
     const float least = some ? key_score(kmin) : 0.f, most = some ? key_score(kmax) : 0.f, width = most - least;
-    const float per = width > 0.f ? (kPickThreads - 1.5f) / width : 0.f;
+    const float per = width > 0.f ? (THREADS - 1.5f) / width : 0.f;
     auto bin_of = [&](uint32_t k) -> uint32_t {
         const float s = fminf(fmaxf(key_score(k), least), most);  // the key of no block stands for a NaN: least
-        return min(__float_as_uint(fmaf(s - least, per, 8388608.0f)) - 0x4b000000u, kPickThreads - 1u);
+        return min(__float_as_uint(fmaf(s - least, per, 8388608.0f)) - 0x4b000000u, THREADS - 1u);
     };
     uint32_t need = static_cast<uint32_t>(d.budget - d.first - d.last);
-    uint32_t threshold = 0xffffffffu, at_it = 0;  // selected: above the threshold, and the first at_it at it
+    uint32_t threshold = kAlways - 1u, at_it = 0;  // selected: above the threshold, and the first at_it at it
     if (need > 0) {
-        each([&](int i, uint32_t k, int) {
-            if (i >= lo && i < hi) atomicAdd(&s.hist[bin_of(k)], 1u);
-        }, false);
+        each([&](int j, uint32_t k) {
+            const uint32_t bin = bin_of(k);
+            if constexpr (KEPT) bins[j / 2] |= bin << (j % 2 * 16);
+            if (scored(k)) atomicAdd(&s.hist[bin], 1u);
+        });
         __syncthreads();
         find_bin(s, need);
         const uint32_t bin = s.pick[0], in_bin = s.pick[2];
-        if (in_bin <= kPickList) {
+        if (in_bin <= THREADS) {
             const uint32_t rest = need - s.pick[1];
-            each([&](int i, uint32_t k, int) {
-                if (i >= lo && i < hi && bin_of(k) == bin) s.list[atomicAdd(&s.listed, 1u)] = k;
-            }, false);
+            each([&](int j, uint32_t k) {
+                bool here;
+                if constexpr (KEPT) here = (bins[j / 2] >> (j % 2 * 16) & 0xffffu) == bin;
+                else here = bin_of(k) == bin;
+                if (here && scored(k)) s.list[atomicAdd(&s.listed, 1u)] = k;
+            });
             __syncthreads();
             if (tid < static_cast<int>(in_bin)) {
                 const uint32_t k = s.list[tid];
@@ -1134,9 +1153,9 @@ __device__ __forceinline__ void pick_row(const SelectParams& p, PickShared& s, i
             for (int sh = 24; sh >= 0; sh -= 8) {
                 s.hist[tid] = 0u;
                 __syncthreads();
-                each([&](int i, uint32_t k, int) {
-                    if (i >= lo && i < hi && (k & mask) == prefix) atomicAdd(&s.hist[(k >> sh) & 255u], 1u);
-                }, false);
+                each([&](int, uint32_t k) {
+                    if (scored(k) && (k & mask) == prefix) atomicAdd(&s.hist[(k >> sh) & 255u], 1u);
+                });
                 __syncthreads();
                 find_bin(s, need);
                 prefix |= s.pick[0] << sh;
@@ -1147,40 +1166,36 @@ __device__ __forceinline__ void pick_row(const SelectParams& p, PickShared& s, i
             at_it = need;
         }
     }
-    auto kind = [&](int i, uint32_t k, bool& up, bool& eq) {
-        const bool scored = i >= lo && i < hi;
-        up = i < n && (!scored || k > threshold);
-        eq = scored && k == threshold;
-    };
     uint32_t above = 0, equal = 0;
-    each([&](int i, uint32_t k, int) {
-        bool up, eq;
-        kind(i, k, up, eq);
-        above += up;
-        equal += eq;
-    }, false);
+    each([&](int, uint32_t k) {
+        above += k > threshold;
+        equal += k == threshold;
+    });
     above = __reduce_add_sync(0xffffffffu, above);
     equal = __reduce_add_sync(0xffffffffu, equal);
     if (lane == 0) { s.count[0][warp] = above; s.count[1][warp] = equal; }
     __syncthreads();
-    above = equal = 0;
-#pragma unroll
-    for (int w = 0; w < kPickWarps; ++w)
-        if (w < warp) { above += s.count[0][w]; equal += s.count[1][w]; }
+    above = before_warp(s.count[0]);
+    equal = before_warp(s.count[1]);
     const uint32_t below = (1u << lane) - 1u;
-    each([&](int i, uint32_t k, int block) {
-        bool up, eq;
-        kind(i, k, up, eq);
+    each([&](int j, uint32_t k) {
+        const int i = s0 + 32 * j + lane;
+        int block = 0;
+        if constexpr (KEPT) block = id[j];
+        else if (i < s1) block = table[i];
+        const bool up = k > threshold, eq = k == threshold;
         const uint32_t ub = __ballot_sync(0xffffffffu, up), eb = __ballot_sync(0xffffffffu, eq);
+        if ((ub | eb) == 0) return;
         const uint32_t e = equal + __popc(eb & below);
         if (up || (eq && e < at_it)) out[above + __popc(ub & below) + min(e, at_it)] = block;
         above += __popc(ub);
         equal += __popc(eb);
-    }, true);
+    });
 }
 
-__global__ void __launch_bounds__(kPickThreads) pick_kernel(const SelectParams p) {
-    __shared__ PickShared s;
+template <int THREADS>
+__global__ void __launch_bounds__(THREADS, 1024 / THREADS) pick_kernel(const SelectParams p) {
+    __shared__ PickShared<THREADS> s;
     const kvd_block_select_desc& d = p.d;
     const int row = blockIdx.x, b = row / d.num_kv_heads;
     const int tid = threadIdx.x, k = d.budget;
@@ -1193,14 +1208,14 @@ __global__ void __launch_bounds__(kPickThreads) pick_kernel(const SelectParams p
     const int32_t* table = d.block_table + b * d.block_table_stride;
     if (tid == 0) p.sel_lens[row] = n <= k ? len : (k - n) * d.block_size + len;
     if (n <= k) {  // everything
-        for (int i = tid; i < k; i += kPickThreads) {
+        for (int i = tid; i < k; i += THREADS) {
             p.sel_table[static_cast<int64_t>(row) * k + i] = i < n ? table[i] : -1;
             if (i < n) pool_id(d, table, i);
         }
-    } else if (n <= kPickKept) {
-        pick_row<true>(p, s, row, n, table);
+    } else if (n <= THREADS * kPickEach) {
+        pick_row<true, THREADS>(p, s, row, n, table);
     } else {
-        pick_row<false>(p, s, row, n, table);
+        pick_row<false, THREADS>(p, s, row, n, table);
     }
 }
 
@@ -1221,7 +1236,10 @@ cudaError_t launch_select(const SelectParams& p, cudaStream_t st) {
         if (e != cudaSuccess) return e;
         ++*launch_counter();
     }
-    e = launch_after(pick_kernel, static_cast<unsigned>(rows), kPickThreads, 0, st, p);
+    if (d.max_blocks_per_seq <= 256 * kPickEach)
+        e = launch_after(pick_kernel<256>, static_cast<unsigned>(rows), 256, 0, st, p);
+    else
+        e = launch_after(pick_kernel<1024>, static_cast<unsigned>(rows), 1024, 0, st, p);
     if (e == cudaSuccess) ++*launch_counter();
     return e;
 }

@@ -19,12 +19,13 @@ struct SelectParams {
 };
 
 // Order-preserving key of a score: larger is better; NaN counts as +inf, -0 as
-// +0. 0 is below every score's key: a block outside the pool.
+// +0. Keys lie between those of -inf, 0x007fffff, and +inf, 0xff800000.
 __device__ __forceinline__ uint32_t score_key(float s) {
     if (isnan(s)) s = INFINITY;
     const uint32_t u = __float_as_uint(s + 0.f);
     return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
+constexpr uint32_t kNoBlockKey = 1;  // of a block id outside the pool
 __device__ __forceinline__ float key_score(uint32_t k) { return __uint_as_float(k & 0x80000000u ? k & 0x7fffffffu : ~k); }
 
 // Tokens and blocks of request b.

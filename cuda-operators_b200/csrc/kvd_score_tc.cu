@@ -10,7 +10,7 @@
 // copies, neighbouring lanes on neighbouring pieces of a row, put them into the
 // swizzled operand layout; a thread per block then turns its NQ sums into a
 // score. Bound: HBM, 2D + 4 bytes a block and head: 64 requests x 8 heads x up
-// to 4,096 blocks of 128 dims, 410 MB in rows of 256 bytes, take 79 us, 5.2 TB/s
+// to 4,096 blocks of 128 dims, 410 MB in rows of 256 bytes, take 76 us, 5.4 TB/s
 // (rows so scattered are read at 6.2 to 6.4 TB/s by a kernel that does nothing
 // else). Warp-level int8 products, m16n8k32, took 350 instructions per 16 blocks
 // and 101 us, TMA gathers of four rows 164 us; four loading warps instead of
@@ -37,7 +37,7 @@ struct ScoreCfg {
     static constexpr int E = D / 32;                   // query values a lane quantises
     static constexpr int STAGES = SL == 4 && NQ > 16 ? 2 : 12 / SL;
     static constexpr int LW = 8;                       // loading warps
-    static constexpr int LAG = STAGES > 3 ? STAGES - 3 : 1;  // tiles between a tile's issue and the wait for it
+    static constexpr int LAG = STAGES > 5 ? STAGES - 5 : 1;  // tiles between a tile's issue and the wait for it
     static constexpr int STEPS = 16;                   // tiles whose steps are kept: more than are under way (STAGES + 2)
     static constexpr int SLAB = 128 * 128;             // 128 blocks x 128 bytes
     static constexpr int Q_SLAB = NQ * 128;
@@ -172,8 +172,10 @@ struct Ring {
 // SL * 8 neighbouring lanes, 16 bytes each, to their swizzled places. A tile
 // counts as full once its copies are done and fenced for the tensor cores'
 // reads. The wait for that comes LAG tiles after the issue, LAG below the
-// number of stages by three: the stage that the next tile goes to is then free
-// before it is asked for, and the warps wait for memory only. The blocks' steps
+// number of stages: the stage that the next tile goes to is then free before it
+// is asked for, and the warps wait for memory only (with 6 stages, selecting for
+// 64 requests takes 89.5 us with a LAG of 1, 90.1, 91.4 and 93.3 of 2, 3 and 4;
+// four accumulators instead of two change nothing). The blocks' steps
 // come along, into a ring of their own that the scoring warps read.
 template <int SL, int NQ>
 __device__ __forceinline__ void score_loader(const SelectParams& p, uint8_t* smem, Walk walk, int w) {
@@ -419,7 +421,7 @@ __device__ __forceinline__ void score_epilogue(const SelectParams& p, uint8_t* s
             __syncwarp();
             if (lane == 0) mbar_arrive(&bars[C::B_FREE + acc.s]);
             acc.next();
-            if (i + r < I.m) keys[i + r] = step < 0.f ? 0u : score_key(best * step);
+            if (i + r < I.m) keys[i + r] = step < 0.f ? kNoBlockKey : score_key(best * step);
         }
     }
 }
