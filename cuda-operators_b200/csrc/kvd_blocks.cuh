@@ -32,7 +32,7 @@ __device__ __forceinline__ float key_score(uint32_t k) { return __uint_as_float(
 __device__ __forceinline__ int select_len(const kvd_block_select_desc& d, int b, int& n) {
     const int64_t cap = static_cast<int64_t>(d.max_blocks_per_seq) * d.block_size;
     const int len = static_cast<int>(min(static_cast<int64_t>(max(0, d.seq_lens[b])), cap));
-    n = (len + d.block_size - 1) / d.block_size;
+    n = static_cast<int>((static_cast<uint32_t>(len) + d.block_size - 1) / d.block_size);
     return len;
 }
 
