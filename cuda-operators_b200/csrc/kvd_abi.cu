@@ -286,8 +286,17 @@ extern "C" cudaError_t kvd_paged_decode_launch(const kvd_paged_desc* desc, const
                           &tl_launches, &pv);
 }
 
+namespace {
+// The kernels count a selection's tokens, and the end of a split of them, in 32 bits.
+cudaError_t check_sparse(const kvd_paged_desc* d) {
+    const cudaError_t e = check_paged(d);
+    if (e != cudaSuccess) return e;
+    return static_cast<int64_t>(d->max_blocks_per_seq) * d->block_size > 0x40000000LL ? cudaErrorInvalidValue : cudaSuccess;
+}
+}  // namespace
+
 extern "C" size_t kvd_sparse_workspace_size(const kvd_paged_desc* desc) {
-    if (check_paged(desc) != cudaSuccess) return 0;
+    if (check_sparse(desc) != cudaSuccess) return 0;
     PagedView pv;
     const kvd_decode_desc d = paged_as_dense(*desc, &pv);
     // alignment, which the sizes do not show, may move a shape to the next kernel
@@ -302,7 +311,7 @@ extern "C" cudaError_t kvd_sparse_decode_launch(const kvd_paged_desc* desc, cons
                                                 const float* v_scale_pool, void* out, void* workspace,
                                                 size_t workspace_bytes, cudaStream_t stream) {
     tl_launches = 0;
-    const cudaError_t e = check_paged(desc);
+    const cudaError_t e = check_sparse(desc);
     if (e != cudaSuccess) return e;
     if (!Q || !K_pool || !V_pool || !k_scale_pool || !v_scale_pool || !out) return cudaErrorInvalidValue;
     if (desc->flags & KVD_FLAG_QK_INT8) return cudaErrorNotSupported;

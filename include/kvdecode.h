@@ -330,7 +330,8 @@ cudaError_t kvd_block_select_launch(const kvd_block_select_desc* desc, const voi
  * desc->seq_lens is [batch][num_kv_heads] and desc->block_table
  * [batch][num_kv_heads][block_table_stride] (sel_lens and sel_table above, with
  * max_blocks_per_seq = budget). All blocks in front of a row's last one count
- * as full. Any group size. head_dim 128 with pools that the paged decode's
+ * as full. A budget of more than 2^30 tokens returns cudaErrorInvalidValue.
+ * Any group size. head_dim 128 with pools that the paged decode's
  * tensor-core kernel takes runs on that kernel, head_dim 64, 128 and 256
  * otherwise on a CUDA-core kernel (pools on 16-byte boundaries), any other on
  * the generic kernel. KVD_FLAG_QK_INT8 returns cudaErrorNotSupported. */

@@ -284,6 +284,19 @@ def test_symbols_and_refusals():
     assert L.kvd_sparse_decode_launch(ctypes.byref(d), *[256] * 7, 0, None) == 801  # cudaErrorNotSupported
 
 
+def test_long_budgets_are_refused():
+    """A selection's tokens are counted in 32 bits: budgets above 2^30 tokens do not reach a kernel."""
+    L = kvd.lib()
+    sp = dict(batch=1, num_q_heads=1, num_kv_heads=1, head_dim=80, block_size=1 << 14, num_blocks=64,
+              seq_lens=256, block_table=256, block_table_stride=1 << 17, o_stride_h=80)
+    d = kvd.PagedDesc(**sp, max_blocks_per_seq=1 << 16)
+    assert L.kvd_sparse_workspace_size(ctypes.byref(d)) > 0  # 2^30 tokens
+    for blocks in ((1 << 16) + 1, (1 << 17) - 1):
+        d = kvd.PagedDesc(**sp, max_blocks_per_seq=blocks)
+        assert L.kvd_sparse_workspace_size(ctypes.byref(d)) == 0
+        assert L.kvd_sparse_decode_launch(ctypes.byref(d), *[256] * 7, 1 << 40, None) == EINVAL
+
+
 def test_python_refusals():
     import torch
 
