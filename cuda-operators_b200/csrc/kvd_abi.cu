@@ -321,10 +321,11 @@ extern "C" cudaError_t kvd_sparse_decode_launch(const kvd_paged_desc* desc, cons
     PagedView pv;
     const kvd_decode_desc d = paged_as_dense(*desc, &pv);
     pv.per_head = true;
-    if (paged_tc_ok(*desc, d, Q, K_pool, V_pool, k_scale_pool, v_scale_pool, true))
+    const bool group = sel_group_ok(d, pv, K_pool, V_pool);
+    if (!(group && sel_group_first(d)) && paged_tc_ok(*desc, d, Q, K_pool, V_pool, k_scale_pool, v_scale_pool, true))
         return launch_gqa_tc(d, Q, K_pool, V_pool, k_scale_pool, v_scale_pool, out, workspace, workspace_bytes,
                              stream, &tl_launches, &pv);
-    if (sel_group_ok(d, pv, K_pool, V_pool))
+    if (group)
         return launch_sel_group(d, Q, K_pool, V_pool, k_scale_pool, v_scale_pool, out, workspace, workspace_bytes,
                                 stream, &tl_launches, pv);
     return launch_generic(d, Q, K_pool, V_pool, k_scale_pool, v_scale_pool, out, workspace, workspace_bytes, stream,

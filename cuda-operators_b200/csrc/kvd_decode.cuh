@@ -167,6 +167,7 @@ cudaError_t launch_generic(const kvd_decode_desc& d, const void* Q, const int8_t
 size_t generic_workspace_size(const kvd_decode_desc& d);
 // Decode over selected blocks on CUDA cores (kvd_sel_group.cu).
 bool sel_group_ok(const kvd_decode_desc& d, const PagedView& pv, const int8_t* K, const int8_t* V);
+bool sel_group_first(const kvd_decode_desc& d);  // little work: before the tensor-core kernel
 size_t sel_group_workspace_size(const kvd_decode_desc& d);
 cudaError_t launch_sel_group(const kvd_decode_desc& d, const void* Q, const int8_t* K, const int8_t* V,
                              const float* ks, const float* vs, void* out, void* ws, size_t ws_bytes, cudaStream_t st,

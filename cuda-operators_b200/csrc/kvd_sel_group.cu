@@ -16,8 +16,8 @@
 // blocks of 16, groups of 1, 2, 4, 8, 16: head_dim 64 (151 MB) 51, 63, 84, 141,
 // 244 us; head_dim 256 (554 MB) 187 us for 1, 491 for 8; head_dim 128 in blocks
 // of 24 112 and 259. Where both run, the tensor-core kernel takes 47 and 64 us
-// (group 1 and 8, blocks of 16) against 65 and 237 here; only a lone short row is
-// faster here (1 x 8 rows of 1,024 tokens, group 1: 5.8 against 8.3).
+// (group 1 and 8, blocks of 16) against 65 and 237 here; little work is done
+// sooner here (sel_group_first).
 #include "kvd_common.cuh"
 #include "kvd_decode.cuh"
 
@@ -267,6 +267,21 @@ bool sel_group_ok(const kvd_decode_desc& d, const PagedView& pv, const int8_t* K
     if (((reinterpret_cast<uintptr_t>(K) | reinterpret_cast<uintptr_t>(V)) & 15) != 0) return false;
     if (((pv.kv_sblk | d.kv_stride_h | pv.kv_st) & 15) != 0) return false;
     return static_cast<int64_t>(d.batch) * d.num_q_heads <= 0x7fffffff;
+}
+
+// Little work is a matter of latency, and this kernel's splits of 64 tokens and
+// short set-up end sooner than the tensor-core kernel's tiles of 128: head_dim
+// 128, 8 KV heads, blocks of 16, us here | there, for requests x tokens:
+//            1 x 512      1 x 2,048    1 x 4,096    4 x 512     8 x 512     8 x 1,024
+//   1 head   5.3 | 8.2    7.4 | 9.4    11 | 11      5.9 | 8.9   6.9 | 10    11 | 11
+//   2        6.0 | 8.7    8.4 | 9.8    12 | 12      6.6 | 9.4   8.1 | 10    13 | 12
+//   4        7.2 | 9.5    10 | 11      17 | 13      8.4 | 10    13 | 11     20 | 13
+//   8        10 | 9.6     13 | 11      23 | 14      12 | 10     20 | 12     35 | 14
+bool sel_group_first(const kvd_decode_desc& d) {
+    int sub, per;
+    group_parts(d, &sub, &per);
+    const int64_t tokens = static_cast<int64_t>(d.batch) * d.num_kv_heads * sub * d.max_seq_len;
+    return per <= 4 && tokens <= (per <= 2 ? 32768 : 16384);
 }
 
 size_t sel_group_workspace_size(const kvd_decode_desc& d) {

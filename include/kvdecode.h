@@ -332,9 +332,9 @@ cudaError_t kvd_block_select_launch(const kvd_block_select_desc* desc, const voi
  * max_blocks_per_seq = budget). All blocks in front of a row's last one count
  * as full. A budget of more than 2^30 tokens returns cudaErrorInvalidValue.
  * Any group size. head_dim 128 with pools that the paged decode's
- * tensor-core kernel takes runs on that kernel, head_dim 64, 128 and 256
- * otherwise on a CUDA-core kernel (pools on 16-byte boundaries), any other on
- * the generic kernel. KVD_FLAG_QK_INT8 returns cudaErrorNotSupported. */
+ * tensor-core kernel takes runs on that kernel unless there is little work,
+ * head_dim 64, 128 and 256 otherwise on a CUDA-core kernel (pools on 16-byte
+ * boundaries), any other on the generic kernel. KVD_FLAG_QK_INT8 returns cudaErrorNotSupported. */
 size_t kvd_sparse_workspace_size(const kvd_paged_desc* desc);
 cudaError_t kvd_sparse_decode_launch(const kvd_paged_desc* desc,
                                      const void* Q, const int8_t* K_pool, const int8_t* V_pool,

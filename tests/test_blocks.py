@@ -743,6 +743,17 @@ def test_sparse_decode_groups(D, bs, k, G):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("G", [1, 2, 3, 4])
+@pytest.mark.parametrize("B,k", [(2, 60), (2, 90), (4, 130)])
+def test_sparse_decode_either_side_of_little_work(B, k, G):
+    """Budgets at which small groups change from one kernel to the other."""
+    rng = np.random.default_rng(k)
+    lens = rng.integers(0, k * 16 + 1, (B, 8))
+    lens[0, :4] = 0, 1, k * 16, k * 16 - 15
+    _check_sparse(k + G, B, 8, G, 128, 16, k, lens, "bhtd")
+
+
+@pytest.mark.gpu
 def test_sparse_decode_small_workspace_and_bad_ids():
     """Less scratch means fewer splits, not other results; a block id outside the pool is not read."""
     import torch
