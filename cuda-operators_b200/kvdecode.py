@@ -647,25 +647,25 @@ def _stream_of(stream, t) -> int:
 def _pools(k_pool, v_pool, ks_pool, vs_pool, layout: str):
     """(blocks, heads, block_size, head_dim, block stride, head stride, token stride, scale strides) of K and V pools."""
     _, i8, _, _, f32 = _types()
-    strides, sc_strides = k_pool.stride(), ks_pool.stride()
+    shape, strides, sc_shape, sc_strides = k_pool.shape, k_pool.stride(), ks_pool.shape, ks_pool.stride()
     if layout == "bhtd":
-        NB, H, bs, D = k_pool.shape
+        NB, H, bs, D = shape
         s_blk, s_h, s_t, s_d = strides
     elif layout == "bthd":
-        NB, bs, H, D = k_pool.shape
+        NB, bs, H, D = shape
         s_blk, s_t, s_h, s_d = strides
     else:
         raise ValueError(f"unknown pool layout {layout!r}")
-    if ks_pool.shape != (NB, H, bs):
-        raise ValueError(f"scale pool {tuple(ks_pool.shape)} does not match pool {tuple(k_pool.shape)}")
-    if s_d != 1 or sc_strides[2] != 1:
+    if sc_shape != (NB, H, bs):
+        raise ValueError(f"scale pool {tuple(sc_shape)} does not match pool {tuple(shape)}")
+    sc_blk, sc_h, sc_t = sc_strides
+    if s_d != 1 or sc_t != 1:
         raise ValueError("dims and scale tokens must be contiguous")
-    if v_pool.stride() != strides or vs_pool.stride() != sc_strides or v_pool.shape != k_pool.shape \
-            or vs_pool.shape != ks_pool.shape:
+    if v_pool.stride() != strides or vs_pool.stride() != sc_strides or v_pool.shape != shape or vs_pool.shape != sc_shape:
         raise ValueError("K/V pools and their scale pools must share shapes and strides")
-    if k_pool.dtype != i8 or v_pool.dtype != i8 or ks_pool.dtype != f32 or vs_pool.dtype != f32:
+    if k_pool.dtype is not i8 or v_pool.dtype is not i8 or ks_pool.dtype is not f32 or vs_pool.dtype is not f32:
         raise ValueError("pools are int8, scale pools float32")
-    return NB, H, bs, D, s_blk, s_h, s_t, sc_strides[0], sc_strides[1]
+    return NB, H, bs, D, s_blk, s_h, s_t, sc_blk, sc_h
 
 
 def _table(block_table, B: int, i32) -> int:
@@ -813,7 +813,7 @@ def sparse_decode(q, k_pool, v_pool, ks_pool, vs_pool, sel_table, sel_lens, out=
                   softmax_scale: float = 0.0, partial: bool = False, workspace=None, stream=None, out_dtype=None):
     """INT8 decode attention over selected blocks of a paged cache, ``sel_table`` int32 [B, Hkv, budget] and
     ``sel_lens`` int32 [B, Hkv] (:func:`block_select`'s); returns ``out`` [B, Hq, D] (or records)."""
-    torch, _, i32, _, _ = _types()
+    torch, _, i32, _, f32 = _types()
     B, Hq, D = q.shape
     R = D + 4 if partial else D
     if out is None:
@@ -830,8 +830,11 @@ def sparse_decode(q, k_pool, v_pool, ks_pool, vs_pool, sel_table, sel_lens, out=
     o_b, o_h, o_d = out.stride()
     if q_d != 1 or o_d != 1:
         raise ValueError("dims must be contiguous")
+    if partial and out.dtype is not f32:
+        raise ValueError("partial records are float32")
+    flags = _row_flags(q.dtype) | _row_flags(out.dtype) << 2 | (KVD_FLAG_PARTIAL_OUT if partial else 0)  # OUT_*: two bits up
     table = sel_table.data_ptr()
-    desc = PagedDesc(B, Hq, H, D, bs, NB, budget, dtype_flags(q, out, partial), sel_lens.data_ptr(), table, budget,
+    desc = PagedDesc(B, Hq, H, D, bs, NB, budget, flags, sel_lens.data_ptr(), table, budget,
                      s_blk, s_h, s_t, sc_blk, sc_h, q_b, q_h, o_b, o_h, softmax_scale)
     if workspace is None:
         n = int(lib().kvd_sparse_workspace_size(ctypes.byref(desc)))
