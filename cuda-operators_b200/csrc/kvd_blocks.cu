@@ -37,12 +37,11 @@ cudaError_t launch_after(void (*kern)(A...), unsigned grid, unsigned block, size
 // a request from L2, an exchange through shared memory a sum) and writes its
 // share, a slot per thread where that many threads fit on the GPU. Bound:
 // latency, a chain of three loads and the sums' barriers: 3.3 us for 8 requests
-// and 8.2 us for 1,024 with 65,536 new tokens (one CTA alone: 5.2 and 16.4).
-// Up to 256 requests a CTA has 256 threads, above that 1,024: 8 requests take
-// 3.3 us with 256 and 4.1 with 1,024, 512 take 5.5 and 4.8, 4,096 take 21 and
-// 12. Lengths and the count
-// may alias the inputs: the CTA that was last to read the inputs writes them,
-// at its end; the others have counted themselves right after reading.
+// and 8.2 us for 1,024 with 65,536 new tokens. Up to 256 requests a CTA has 256
+// threads, above that 1,024: 8 requests take 3.3 us with 256 and 4.1 with 1,024,
+// 512 take 5.5 and 4.8, 4,096 take 21 and 12. Lengths and the count may alias the
+// inputs: the CTA that was last to read the inputs writes them, at its end; the
+// others have counted themselves right after reading.
 constexpr int kPlanMaxBatch = 8192;
 
 struct PlanParams {
