@@ -874,8 +874,9 @@ cudaError_t launch_rows(RowsParams& p, bool write, cudaStream_t st) {
         //       32         9.1 | 18     25 | 62      9.1 |  7.9     18 | 17       35 | 44
         //       64          12 | 20     38 | 68       15 |  9.4     27 | 17       34 | 38
         //      128          19 | 21     67 | 88       25 |  13      41 | 23       57 | 43
-        // Between, blocks of 33 to 127 tokens, small calls are taken for decode steps.
-        const bool one = LPR && (d.block_size <= 32 || (d.block_size < 128 && rows <= 24 * device_sm_count()));
+        // Between, blocks of 33 to 127 tokens, calls of up to 64 rows an SM are taken for decode steps, which
+        // gain more by it than a prompt loses (1,000 tokens in blocks of 64: 38 | 68 against 19 | 11).
+        const bool one = LPR && (d.block_size <= 32 || (d.block_size < 128 && rows <= 64 * device_sm_count()));
         // Tiles: about the CTAs that the GPU holds at once (20 of one warp an SM), or twice as many (6 of four):
         // with 10 or 40 of one warp 1,000 decode rows took 31 or 19 us, 5,000 prompt rows 16 or 18; with 6 or
         // 24 of four 256 decode rows in blocks of 128 took 28 or 24 us, 20,000 prompt rows 40 or 47.
