@@ -999,7 +999,7 @@ __global__ void __launch_bounds__(32) score_any_kernel(const SelectParams p) {
 // registers, keys and pool ids, from one load to the end; longer rows are read
 // again from L2. 256 threads where the table has up to 4,096 blocks a row, above
 // that 1,024. Bound: latency, three loads in a row and seven barriers, and for
-// many rows the instructions (46 % of the issue slots, four CTAs an SM).
+// many rows the instructions (57 % of the issue slots, four CTAs an SM).
 // With the scores, 64 requests x 8 heads x 4,096 blocks take 83 us, about 13 of
 // them here: 92 when rows are read again, 87 by radix passes alone, 93 with 1,024
 // threads a row. One request of 256 blocks a head takes 7.5 us (9.0 with 1,024
