@@ -644,6 +644,24 @@ def _stream_of(stream, t) -> int:
     return raw(t.get_device()) if raw else torch.cuda.current_stream(t.device).cuda_stream
 
 
+def _made(make, stream, t, kept: bool = False):
+    """``make()``'s tensor, for a call on ``stream``: made with that stream current, so that what fills it runs there
+    too and its memory goes back to that stream's pool. ``kept``: the caller gets it, and may use it on the stream that
+    is current now."""
+    if stream is not None and _stream(stream) != _stream_of(None, t):
+        torch = _types()[0]
+        if not isinstance(stream, torch.cuda.Stream):
+            handle = _stream(stream)
+            stream = torch.cuda.ExternalStream(handle, t.device) if handle else torch.cuda.default_stream(t.device)
+        here = torch.cuda.current_stream(t.device)
+        with torch.cuda.stream(stream):
+            made = make()
+        if kept:
+            made.record_stream(here)
+        return made
+    return make()
+
+
 def _pools(k_pool, v_pool, ks_pool, vs_pool, layout: str):
     """(blocks, heads, block_size, head_dim, block stride, head stride, token stride, scale strides) of K and V pools."""
     _, i8, _, _, f32 = _types()
@@ -689,8 +707,8 @@ def paged_plan(seq_lens, new_lens, block_table, free_blocks, free_count, block_s
     B = seq_lens.shape[0]
     if token_starts is None:
         token_starts = torch.empty(B + 1, dtype=i32, device=seq_lens.device)
-    if workspace is None:
-        workspace = torch.zeros(16, dtype=torch.uint8, device=seq_lens.device)
+    if workspace is None:  # zeroed on the call's stream
+        workspace = _made(lambda: torch.zeros(16, dtype=torch.uint8, device=seq_lens.device), stream, seq_lens)
     rows, one = (B,), (1,)
     _want(seq_lens, i32, rows, "seq_lens")
     _want(new_lens, i32, rows, "new_lens")
