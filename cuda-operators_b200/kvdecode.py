@@ -706,7 +706,7 @@ def paged_plan(seq_lens, new_lens, block_table, free_blocks, free_count, block_s
     torch, _, i32, i64, _ = _types()
     B = seq_lens.shape[0]
     if token_starts is None:
-        token_starts = torch.empty(B + 1, dtype=i32, device=seq_lens.device)
+        token_starts = _made(lambda: torch.empty(B + 1, dtype=i32, device=seq_lens.device), stream, seq_lens, True)
     if workspace is None:  # zeroed on the call's stream
         workspace = _made(lambda: torch.zeros(16, dtype=torch.uint8, device=seq_lens.device), stream, seq_lens)
     rows, one = (B,), (1,)
@@ -772,8 +772,8 @@ def paged_read(slot_map, k_pool, v_pool, ks_pool, vs_pool, k_out=None, v_out=Non
         torch = _types()[0]
         H, D = k_pool.shape[1 if layout == "bhtd" else 2], k_pool.shape[3]
         shape = (slot_map.shape[0], H, D)
-        k_out = torch.empty(shape, dtype=dtype or torch.float32, device=k_pool.device)
-        v_out = torch.empty_like(k_out)
+        k_out, v_out = (_made(lambda: torch.empty(shape, dtype=dtype or torch.float32, device=k_pool.device), stream,
+                              k_pool, True) for _ in range(2))
     desc = _rows_desc(k_out, v_out, slot_map, k_pool, v_pool, ks_pool, vs_pool, layout)
     rc = lib().kvd_paged_read_launch(ctypes.byref(desc), slot_map.data_ptr(), k_pool.data_ptr(), v_pool.data_ptr(),
                                      ks_pool.data_ptr(), vs_pool.data_ptr(), k_out.data_ptr(), v_out.data_ptr(),
@@ -800,17 +800,17 @@ def block_select(q, bounds, bound_scale, block_table, seq_lens, block_size: int,
     _want(bound_scale, f32, (NB, H), "bound_scale")
     _want(seq_lens, i32, (B,), "seq_lens")
     if sel_table is None:
-        sel_table = torch.empty((B, H, budget), dtype=i32, device=q.device)
+        sel_table = _made(lambda: torch.empty((B, H, budget), dtype=i32, device=q.device), stream, q, True)
     else:
         _want(sel_table, i32, (B, H, budget), "sel_table")
     if sel_lens is None:
-        sel_lens = torch.empty((B, H), dtype=i32, device=q.device)
+        sel_lens = _made(lambda: torch.empty((B, H), dtype=i32, device=q.device), stream, q, True)
     else:
         _want(sel_lens, i32, (B, H), "sel_lens")
     desc = BlockSelectDesc(B, Hq, H, D, block_size, NB, MB, budget, first, last, _row_flags(q.dtype),
                            seq_lens.data_ptr(), block_table.data_ptr(), block_table.stride(0), s_b, s_h)
     if workspace is None and MB > budget:
-        workspace = torch.empty(B * H * MB, dtype=i32, device=q.device)
+        workspace = _made(lambda: torch.empty(B * H * MB, dtype=i32, device=q.device), stream, q)
     rc = lib().kvd_block_select_launch(ctypes.byref(desc), q.data_ptr(), bounds.data_ptr(), bound_scale.data_ptr(),
                                        sel_table.data_ptr(), sel_lens.data_ptr(), _ptr(workspace),
                                        workspace.nbytes if workspace is not None else 0, _stream_of(stream, q))
@@ -835,7 +835,7 @@ def sparse_decode(q, k_pool, v_pool, ks_pool, vs_pool, sel_table, sel_lens, out=
     B, Hq, D = q.shape
     R = D + 4 if partial else D
     if out is None:
-        out = torch.empty((B, Hq, R), dtype=out_dtype or torch.float32, device=q.device)
+        out = _made(lambda: torch.empty((B, Hq, R), dtype=out_dtype or torch.float32, device=q.device), stream, q, True)
     elif out.shape != (B, Hq, R):
         raise ValueError(f"out must be [{B}, {Hq}, {R}], got {tuple(out.shape)}")
     NB, H, bs, Dk, s_blk, s_h, s_t, sc_blk, sc_h = _pools(k_pool, v_pool, ks_pool, vs_pool, layout)
@@ -856,7 +856,7 @@ def sparse_decode(q, k_pool, v_pool, ks_pool, vs_pool, sel_table, sel_lens, out=
                      s_blk, s_h, s_t, sc_blk, sc_h, q_b, q_h, o_b, o_h, softmax_scale)
     if workspace is None:
         n = int(lib().kvd_sparse_workspace_size(ctypes.byref(desc)))
-        workspace = torch.empty(max(n, 1), dtype=torch.uint8, device=q.device)
+        workspace = _made(lambda: torch.empty(max(n, 1), dtype=torch.uint8, device=q.device), stream, q)
     rc = lib().kvd_sparse_decode_launch(ctypes.byref(desc), q.data_ptr(), k_pool.data_ptr(), v_pool.data_ptr(),
                                         ks_pool.data_ptr(), vs_pool.data_ptr(), out.data_ptr(), workspace.data_ptr(),
                                         workspace.nbytes, _stream_of(stream, q))

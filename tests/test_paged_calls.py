@@ -30,3 +30,88 @@ def test_plan_on_a_side_stream_without_a_workspace(as_handle):
     got = (*(t.cpu().numpy() for t in (table, free)), int(count), *(t.cpu().numpy() for t in (lens, starts, slots)),
            kvd.device_status())
     _same_plan(got, plan_oracle(*args, 16, 20000))
+
+
+class _Spy:
+    """The library, with the arguments of every launch kept."""
+
+    def __init__(self, lib):
+        self.lib, self.args = lib, []
+
+    def __getattr__(self, name):
+        fn = getattr(self.lib, name)
+        if not name.endswith("_launch"):
+            return fn
+
+        def call(*args):
+            self.args.append(args)
+            return fn(*args)
+
+        return call
+
+
+def _step_inputs(B=2, H=2, G=2, D=64, bs=16, MB=300):
+    """Pools, bounds, tables, rows and queries of a serving step, on the GPU."""
+    import torch
+
+    g = torch.Generator(device=DEV).manual_seed(1)
+    NB = B * MB
+    x = dict(K=torch.randint(-127, 128, (NB, H, bs, D), dtype=torch.int8, device=DEV, generator=g),
+             V=torch.randint(-127, 128, (NB, H, bs, D), dtype=torch.int8, device=DEV, generator=g),
+             ks=torch.rand((NB, H, bs), device=DEV, generator=g) * 0.02,
+             vs=torch.rand((NB, H, bs), device=DEV, generator=g) * 0.02,
+             bounds=torch.randint(-127, 128, (NB, H, 2, D), dtype=torch.int8, device=DEV, generator=g),
+             step=torch.rand((NB, H), device=DEV, generator=g),
+             table=torch.randperm(NB, device=DEV, generator=g).to(torch.int32).view(B, MB),
+             lens=torch.tensor([MB * bs, MB * bs - 7], dtype=torch.int32, device=DEV),
+             slots=torch.randperm(NB * bs, device=DEV, generator=g)[:5000].to(torch.int64),
+             q=torch.randn((B, H * G, D), device=DEV, generator=g), bs=bs)
+    x["bounds"] = x["bounds"].sort(dim=2, descending=True).values.contiguous()
+    return x
+
+
+def _step_calls(x, stream):
+    """Every call that makes scratch or outputs of its own, as (outputs, pointers of the scratch)."""
+    import torch
+
+    spy = _Spy(kvd.lib())
+    kvd._lib, real = spy, kvd._lib
+    try:
+        grow = torch.zeros_like(x["lens"])
+        count = torch.zeros(1, dtype=torch.int32, device=DEV)
+        free = torch.empty(x["K"].shape[0], dtype=torch.int32, device=DEV)
+        slots = torch.empty(600, dtype=torch.int64, device=DEV)
+        torch.cuda.synchronize()
+        _, starts = kvd.paged_plan(x["lens"], grow, x["table"], free, count, x["bs"], slots, stream=stream)
+        rows = kvd.paged_read(x["slots"], x["K"], x["V"], x["ks"], x["vs"], stream=stream)
+        sel, sl = kvd.block_select(x["q"], x["bounds"], x["step"], x["table"], x["lens"], x["bs"], 40, stream=stream)
+        out = kvd.sparse_decode(x["q"], x["K"], x["V"], x["ks"], x["vs"], sel, sl, stream=stream)
+    finally:
+        kvd._lib = real
+    scratch = [args[-3] for args in (spy.args[0], spy.args[2], spy.args[3])]
+    torch.cuda.synchronize()
+    return (starts, *rows, sel, sl, out), scratch
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("as_handle", [False, True])
+def test_what_a_call_makes_belongs_to_its_stream(as_handle):
+    """Scratch and outputs of calls on a side stream are memory of that stream: once dropped they are not handed to
+    the current stream, on which nothing waits for the call. The results are those of the current stream's calls."""
+    import torch
+
+    x = _step_inputs()
+    want, _ = _step_calls(x, None)
+    side = torch.cuda.Stream()
+    got, scratch = _step_calls(x, side.cuda_stream if as_handle else side)
+    for a, b in zip(got, want):
+        assert torch.equal(a, b)
+    sizes = [t.nbytes for t in got] + [16, 2 * 2 * 300 * 4]
+    at = {t.data_ptr() for t in got} | set(scratch)
+    assert None not in at and 0 not in at
+    del got, a, b
+    for n in sizes:  # what the calls had is not handed out here
+        again = [torch.empty(n, dtype=torch.uint8, device=DEV) for _ in range(8)]
+        assert not at & {t.data_ptr() for t in again}
+    side.synchronize()
+    assert kvd.device_status() == 0
