@@ -306,6 +306,58 @@ def _stream(stream) -> int | None:
     return stream.cuda_stream
 
 
+_torch = None
+
+
+def _types():
+    """(torch, int8, int32, int64, float32), looked up once: these calls are short, and so are their checks."""
+    global _torch
+    if _torch is None:
+        import torch
+
+        _torch = (torch, torch.int8, torch.int32, torch.int64, torch.float32)
+    return _torch
+
+
+def _stream_of(stream, t) -> int:
+    """The given stream, or the current one of ``t``'s device."""
+    if stream is not None:
+        return _stream(stream)
+    torch = _types()[0]
+    raw = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+    return raw(t.get_device()) if raw else torch.cuda.current_stream(t.device).cuda_stream
+
+
+def _made(make, stream, t, kept: bool = False):
+    """``make()``'s tensor, for a call on ``stream``: made with that stream current, so that what fills it runs there
+    too and its memory goes back to that stream's pool. ``kept``: the caller gets it, and may use it on the stream that
+    is current now."""
+    if stream is not None and _stream(stream) != _stream_of(None, t):
+        torch = _types()[0]
+        if not isinstance(stream, torch.cuda.Stream):
+            handle = _stream(stream)
+            stream = torch.cuda.ExternalStream(handle, t.device) if handle else torch.cuda.default_stream(t.device)
+        here = torch.cuda.current_stream(t.device)
+        with torch.cuda.stream(stream):
+            made = make()
+        if kept:
+            made.record_stream(here)
+        return made
+    return make()
+
+
+def _out(shape, dtype, t, stream):
+    """An output (``dtype``, default float32) of a call on ``stream`` whose data lie where ``t`` does."""
+    torch = _types()[0]
+    return _made(lambda: torch.empty(shape, dtype=dtype or torch.float32, device=t.device), stream, t, kept=True)
+
+
+def _scratch(n: int, t, stream):
+    """``n`` bytes (at least one) of scratch for a call on ``stream``."""
+    torch = _types()[0]
+    return _made(lambda: torch.empty(max(n, 1), dtype=torch.uint8, device=t.device), stream, t)
+
+
 # ---------------------------------------------------------------- reference ABI
 def solve(Q, K_int8, V_int8, k_scale, v_scale, output, num_heads: int, seq_len: int, head_dim: int) -> None:
     """``solve`` of kv_cache/*.cu: default stream, no synchronisation, no return value."""
@@ -393,17 +445,15 @@ def decode(q, k, v, ks, vs, out=None, seq_lens=None, softmax_scale: float = 0.0,
     """Split-KV INT8 decode attention; returns ``out`` ([B,Hq,D], or [B,Hq,D+4] records if partial).
     ``q`` may be float32, bfloat16 or float16; the output type is ``out``'s (or ``out_dtype``,
     default float32). ``qk_int8`` selects the INT8 Q.K mode (looser, stated tolerance)."""
-    import torch
-
     B, Hq, D = q.shape
     if out is None:
-        out = torch.empty((B, Hq, D + 4 if partial else D), dtype=out_dtype or torch.float32, device=q.device)
+        out = _out((B, Hq, D + 4 if partial else D), out_dtype, q, stream)
     if v.stride() != k.stride() or vs.stride() != ks.stride():
         raise ValueError("K/V and k_scale/v_scale must share strides")
     desc = make_desc(q, k, ks, out, seq_lens, max_seq_len, softmax_scale, partial, qk_int8)
     if workspace is None:
         n = workspace_size(desc)
-        workspace = torch.empty(max(n, 1), dtype=torch.uint8, device=q.device)
+        workspace = _scratch(n, q, stream)
     rc = lib().kvd_decode_launch(ctypes.byref(desc), _ptr(q), _ptr(k), _ptr(v), _ptr(ks), _ptr(vs), _ptr(out),
                                  _ptr(workspace), workspace.numel(), _stream(stream))
     _check(rc, "kvd_decode_launch")
@@ -427,12 +477,10 @@ def decode_noalloc(q, k, v, ks, vs, out, seq_lens=None, softmax_scale: float = 0
 
 def combine(parts, out=None, partial: bool = False, stream=None, out_dtype=None):
     """LSE-combine records ``parts`` [P, H, D+4] into out [H, D] (or [H, D+4] records)."""
-    import torch
-
     P, H, R = parts.shape
     D = R - 4
     if out is None:
-        out = torch.empty((H, R if partial else D), dtype=out_dtype or torch.float32, device=parts.device)
+        out = _out((H, R if partial else D), out_dtype, parts, stream)
     rc = lib().kvd_combine_launch(_ptr(parts), P, parts.stride(0), H, D, _ptr(out), out.stride(0),
                                   dtype_flags(None, out, partial), _stream(stream))
     _check(rc, "kvd_combine_launch")
@@ -458,16 +506,14 @@ def append_decode(k_new, v_new, q, k, v, ks, vs, seq_lens, out=None, workspace=N
                   partial: bool = False, stream=None, out_dtype=None, qk_int8: bool = False):
     """Quantise-on-append of one token per (b, kv head) and the decode over the grown
     cache in one decode launch (``kvd_append_decode_launch``); ``seq_lens`` is updated."""
-    import torch
-
     B, Hq, D = q.shape
     if out is None:
-        out = torch.empty((B, Hq, D + 4 if partial else D), dtype=out_dtype or torch.float32, device=q.device)
+        out = _out((B, Hq, D + 4 if partial else D), out_dtype, q, stream)
     if v.stride() != k.stride() or vs.stride() != ks.stride() or v_new.stride() != k_new.stride():
         raise ValueError("K/V (and their scales, and the new rows) must share strides")
     desc = make_desc(q, k, ks, out, seq_lens, None, softmax_scale, partial, qk_int8)
     if workspace is None:
-        workspace = torch.empty(max(workspace_size(desc), 1), dtype=torch.uint8, device=q.device)
+        workspace = _scratch(workspace_size(desc), q, stream)
     rc = lib().kvd_append_decode_launch(ctypes.byref(desc), _ptr(k_new), _ptr(v_new), k_new.stride(0),
                                         k_new.stride(1), _ptr(q), _ptr(k), _ptr(v), _ptr(ks), _ptr(vs), _ptr(out),
                                         _ptr(workspace), workspace.numel(), _stream(stream))
@@ -500,16 +546,13 @@ def prefill(q, k, v, ks, vs, seq_lens=None, q_lens=None, out=None, softmax_scale
             workspace=None, stream=None):
     """Causal prefill attention over the INT8 cache; q [B,Hq,Lq,D] holds the last q_lens[b]
     (default Lq) of the seq_lens[b] (default cap) cached tokens. Returns out [B,Hq,Lq,D]."""
-    import torch
-
     if out is None:
-        out = torch.empty(q.shape, dtype=out_dtype or torch.float32, device=q.device)
+        out = _out(q.shape, out_dtype, q, stream)
     if v.stride() != k.stride() or vs.stride() != ks.stride():
         raise ValueError("K/V and k_scale/v_scale must share strides")
     desc = make_prefill_desc(q, k, ks, out, seq_lens, q_lens, softmax_scale)
     if workspace is None:
-        workspace = torch.empty(max(int(lib().kvd_prefill_workspace_size(ctypes.byref(desc))), 1),
-                                dtype=torch.uint8, device=q.device)
+        workspace = _scratch(int(lib().kvd_prefill_workspace_size(ctypes.byref(desc))), q, stream)
     rc = lib().kvd_prefill_launch(ctypes.byref(desc), _ptr(q), _ptr(k), _ptr(v), _ptr(ks), _ptr(vs), _ptr(out),
                                   _ptr(workspace), workspace.numel(), _stream(stream))
     _check(rc, "kvd_prefill_launch")
@@ -522,9 +565,9 @@ def quantize_rows(x, codes=None, scales=None, stream=None):
 
     rows, dim = x.shape
     if codes is None:
-        codes = torch.empty((rows, dim), dtype=torch.int8, device=x.device)
+        codes = _out((rows, dim), torch.int8, x, stream)
     if scales is None:
-        scales = torch.empty((rows,), dtype=torch.float32, device=x.device)
+        scales = _out((rows,), torch.float32, x, stream)
     rc = lib().kvd_quantize_rows_launch(_ptr(x), rows, dim, x.stride(0), _ptr(codes), codes.stride(0),
                                         _ptr(scales), _stream(stream))
     _check(rc, "kvd_quantize_rows_launch")
@@ -574,16 +617,14 @@ def paged_decode(q, k_pool, v_pool, ks_pool, vs_pool, block_table, seq_lens, out
                  softmax_scale: float = 0.0, partial: bool = False, workspace=None, stream=None, out_dtype=None,
                  qk_int8: bool = False):
     """INT8 decode attention over a paged cache; returns ``out`` [B,Hq,D] (or records)."""
-    import torch
-
     B, Hq, D = q.shape
     if out is None:
-        out = torch.empty((B, Hq, D + 4 if partial else D), dtype=out_dtype or torch.float32, device=q.device)
+        out = _out((B, Hq, D + 4 if partial else D), out_dtype, q, stream)
     if v_pool.stride() != k_pool.stride() or vs_pool.stride() != ks_pool.stride():
         raise ValueError("K/V pools and their scale pools must share strides")
     desc = make_paged_desc(q, k_pool, ks_pool, out, block_table, seq_lens, layout, softmax_scale, partial, qk_int8)
     if workspace is None:
-        workspace = torch.empty(max(paged_workspace_size(desc), 1), dtype=torch.uint8, device=q.device)
+        workspace = _scratch(paged_workspace_size(desc), q, stream)
     rc = lib().kvd_paged_decode_launch(ctypes.byref(desc), _ptr(q), _ptr(k_pool), _ptr(v_pool), _ptr(ks_pool),
                                        _ptr(vs_pool), _ptr(out), _ptr(workspace), workspace.numel(),
                                        _stream(stream))
@@ -616,50 +657,10 @@ def _row_flags(dtype) -> int:
     return f
 
 
-_torch = None
-
-
-def _types():
-    """(torch, int8, int32, int64, float32), looked up once: these calls are short, and so are their checks."""
-    global _torch
-    if _torch is None:
-        import torch
-
-        _torch = (torch, torch.int8, torch.int32, torch.int64, torch.float32)
-    return _torch
-
-
 def _want(t, dtype, shape, what: str) -> None:
     """A contiguous tensor of this type and shape."""
     if t.shape != shape or t.dtype != dtype or not t.is_contiguous():
         raise ValueError(f"{what} must be contiguous {dtype} of shape {tuple(shape)}, got {t.dtype} {tuple(t.shape)}")
-
-
-def _stream_of(stream, t) -> int:
-    """The given stream, or the current one of ``t``'s device."""
-    if stream is not None:
-        return _stream(stream)
-    torch = _types()[0]
-    raw = getattr(torch._C, "_cuda_getCurrentRawStream", None)
-    return raw(t.get_device()) if raw else torch.cuda.current_stream(t.device).cuda_stream
-
-
-def _made(make, stream, t, kept: bool = False):
-    """``make()``'s tensor, for a call on ``stream``: made with that stream current, so that what fills it runs there
-    too and its memory goes back to that stream's pool. ``kept``: the caller gets it, and may use it on the stream that
-    is current now."""
-    if stream is not None and _stream(stream) != _stream_of(None, t):
-        torch = _types()[0]
-        if not isinstance(stream, torch.cuda.Stream):
-            handle = _stream(stream)
-            stream = torch.cuda.ExternalStream(handle, t.device) if handle else torch.cuda.default_stream(t.device)
-        here = torch.cuda.current_stream(t.device)
-        with torch.cuda.stream(stream):
-            made = make()
-        if kept:
-            made.record_stream(here)
-        return made
-    return make()
 
 
 def _pools(k_pool, v_pool, ks_pool, vs_pool, layout: str):
@@ -706,7 +707,7 @@ def paged_plan(seq_lens, new_lens, block_table, free_blocks, free_count, block_s
     torch, _, i32, i64, _ = _types()
     B = seq_lens.shape[0]
     if token_starts is None:
-        token_starts = _made(lambda: torch.empty(B + 1, dtype=i32, device=seq_lens.device), stream, seq_lens, True)
+        token_starts = _out((B + 1,), i32, seq_lens, stream)
     if workspace is None:  # zeroed on the call's stream
         workspace = _made(lambda: torch.zeros(16, dtype=torch.uint8, device=seq_lens.device), stream, seq_lens)
     rows, one = (B,), (1,)
@@ -772,8 +773,7 @@ def paged_read(slot_map, k_pool, v_pool, ks_pool, vs_pool, k_out=None, v_out=Non
         torch = _types()[0]
         H, D = k_pool.shape[1 if layout == "bhtd" else 2], k_pool.shape[3]
         shape = (slot_map.shape[0], H, D)
-        k_out, v_out = (_made(lambda: torch.empty(shape, dtype=dtype or torch.float32, device=k_pool.device), stream,
-                              k_pool, True) for _ in range(2))
+        k_out, v_out = (_out(shape, dtype, k_pool, stream) for _ in range(2))
     desc = _rows_desc(k_out, v_out, slot_map, k_pool, v_pool, ks_pool, vs_pool, layout)
     rc = lib().kvd_paged_read_launch(ctypes.byref(desc), slot_map.data_ptr(), k_pool.data_ptr(), v_pool.data_ptr(),
                                      ks_pool.data_ptr(), vs_pool.data_ptr(), k_out.data_ptr(), v_out.data_ptr(),
@@ -800,17 +800,17 @@ def block_select(q, bounds, bound_scale, block_table, seq_lens, block_size: int,
     _want(bound_scale, f32, (NB, H), "bound_scale")
     _want(seq_lens, i32, (B,), "seq_lens")
     if sel_table is None:
-        sel_table = _made(lambda: torch.empty((B, H, budget), dtype=i32, device=q.device), stream, q, True)
+        sel_table = _out((B, H, budget), i32, q, stream)
     else:
         _want(sel_table, i32, (B, H, budget), "sel_table")
     if sel_lens is None:
-        sel_lens = _made(lambda: torch.empty((B, H), dtype=i32, device=q.device), stream, q, True)
+        sel_lens = _out((B, H), i32, q, stream)
     else:
         _want(sel_lens, i32, (B, H), "sel_lens")
     desc = BlockSelectDesc(B, Hq, H, D, block_size, NB, MB, budget, first, last, _row_flags(q.dtype),
                            seq_lens.data_ptr(), block_table.data_ptr(), block_table.stride(0), s_b, s_h)
     if workspace is None and MB > budget:
-        workspace = _made(lambda: torch.empty(B * H * MB, dtype=i32, device=q.device), stream, q)
+        workspace = _scratch(B * H * MB * 4, q, stream)
     rc = lib().kvd_block_select_launch(ctypes.byref(desc), q.data_ptr(), bounds.data_ptr(), bound_scale.data_ptr(),
                                        sel_table.data_ptr(), sel_lens.data_ptr(), _ptr(workspace),
                                        workspace.nbytes if workspace is not None else 0, _stream_of(stream, q))
@@ -835,7 +835,7 @@ def sparse_decode(q, k_pool, v_pool, ks_pool, vs_pool, sel_table, sel_lens, out=
     B, Hq, D = q.shape
     R = D + 4 if partial else D
     if out is None:
-        out = _made(lambda: torch.empty((B, Hq, R), dtype=out_dtype or torch.float32, device=q.device), stream, q, True)
+        out = _out((B, Hq, R), out_dtype, q, stream)
     elif out.shape != (B, Hq, R):
         raise ValueError(f"out must be [{B}, {Hq}, {R}], got {tuple(out.shape)}")
     NB, H, bs, Dk, s_blk, s_h, s_t, sc_blk, sc_h = _pools(k_pool, v_pool, ks_pool, vs_pool, layout)
@@ -856,7 +856,7 @@ def sparse_decode(q, k_pool, v_pool, ks_pool, vs_pool, sel_table, sel_lens, out=
                      s_blk, s_h, s_t, sc_blk, sc_h, q_b, q_h, o_b, o_h, softmax_scale)
     if workspace is None:
         n = int(lib().kvd_sparse_workspace_size(ctypes.byref(desc)))
-        workspace = _made(lambda: torch.empty(max(n, 1), dtype=torch.uint8, device=q.device), stream, q)
+        workspace = _scratch(n, q, stream)
     rc = lib().kvd_sparse_decode_launch(ctypes.byref(desc), q.data_ptr(), k_pool.data_ptr(), v_pool.data_ptr(),
                                         ks_pool.data_ptr(), vs_pool.data_ptr(), out.data_ptr(), workspace.data_ptr(),
                                         workspace.nbytes, _stream_of(stream, q))
@@ -895,15 +895,13 @@ def seq_split_decode(comm: MgpuComm, q, k, v, ks, vs, out=None, seq_lens=None, w
                      out_dtype=None):
     """Sequence-split decode (kvd_mgpu_seq_split_decode): this rank passes its own token
     range of the cache; every rank gets the merged output rows."""
-    import torch
-
     B, Hq, D = q.shape
     if out is None:
-        out = torch.empty((B, Hq, D), dtype=out_dtype or torch.float32, device=q.device)
+        out = _out((B, Hq, D), out_dtype, q, stream)
     desc = make_desc(q, k, ks, out, seq_lens)
     if workspace is None:
         n = int(lib().kvd_mgpu_seq_split_workspace_size(ctypes.byref(desc), comm.nranks))
-        workspace = torch.empty(max(n, 1), dtype=torch.uint8, device=q.device)
+        workspace = _scratch(n, q, stream)
     rc = lib().kvd_mgpu_seq_split_decode(ctypes.byref(desc), _ptr(q), _ptr(k), _ptr(v), _ptr(ks), _ptr(vs),
                                          _ptr(out), _ptr(workspace), workspace.numel(), comm.handle, comm.nranks,
                                          _stream(stream))
@@ -922,15 +920,13 @@ class P2PExchange:
         self._ws = None
 
     def decode(self, q, k, v, ks, vs, out=None, seq_lens=None, stream=None, out_dtype=None):
-        import torch
-
         B, Hq, D = q.shape
         if out is None:
-            out = torch.empty((B, Hq, D), dtype=out_dtype or torch.float32, device=q.device)
+            out = _out((B, Hq, D), out_dtype, q, stream)
         desc = make_desc(q, k, ks, out, seq_lens)
         n = int(lib().kvd_mgpu_p2p_workspace_size(ctypes.byref(desc)))
         if self._ws is None or self._ws.numel() < n:
-            self._ws = torch.empty(max(n, 1), dtype=torch.uint8, device=q.device)
+            self._ws = _scratch(n, q, stream)
         rc = lib().kvd_mgpu_p2p_seq_split_decode(self.handle, ctypes.byref(desc), _ptr(q), _ptr(k), _ptr(v),
                                                  _ptr(ks), _ptr(vs), _ptr(out), _ptr(self._ws), self._ws.numel(),
                                                  _stream(stream))
@@ -969,12 +965,12 @@ class P2PGroup:
         with torch.cuda.device(self.devices[rank]):
             B, Hq, D = q.shape
             if out is None:
-                out = torch.empty((B, Hq, D), dtype=out_dtype or torch.float32, device=q.device)
+                out = _out((B, Hq, D), out_dtype, q, stream)
             desc = make_desc(q, k, ks, out, seq_lens)
             n = int(lib().kvd_mgpu_p2p_workspace_size(ctypes.byref(desc)))
             ws = self._ws.get(rank)
             if ws is None or ws.numel() < n:
-                ws = self._ws[rank] = torch.empty(max(n, 1), dtype=torch.uint8, device=q.device)
+                ws = self._ws[rank] = _scratch(n, q, stream)
             rc = lib().kvd_mgpu_p2p_seq_split_decode(self.handles[rank], ctypes.byref(desc), _ptr(q), _ptr(k),
                                                      _ptr(v), _ptr(ks), _ptr(vs), _ptr(out), _ptr(ws), ws.numel(),
                                                      _stream(stream))

@@ -115,3 +115,52 @@ def test_what_a_call_makes_belongs_to_its_stream(as_handle):
         assert not at & {t.data_ptr() for t in again}
     side.synchronize()
     assert kvd.device_status() == 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("as_handle", [False, True])
+def test_scratch_of_the_dense_and_paged_calls_belongs_to_their_stream(as_handle):
+    """The same of the decode, append-decode, paged decode, prefill, combine and row quantiser."""
+    import torch
+
+    B, H, G, S, D, bs = 2, 2, 4, 4096, 128, 16
+    g = torch.Generator(device=DEV).manual_seed(2)
+    rnd = lambda *shape: torch.randn(shape, device=DEV, generator=g)  # noqa: E731
+    K, V = (torch.randint(-127, 128, (B, H, S, D), dtype=torch.int8, device=DEV, generator=g) for _ in range(2))
+    ks, vs = (torch.rand((B, H, S), device=DEV, generator=g) * 0.02 for _ in range(2))
+    Kp, Vp = (t.view(B, H, S // bs, bs, D).transpose(1, 2).reshape(-1, H, bs, D).contiguous() for t in (K, V))
+    ksp, vsp = (t.view(B, H, S // bs, bs).transpose(1, 2).reshape(-1, H, bs).contiguous() for t in (ks, vs))
+    table = torch.arange(B * S // bs, dtype=torch.int32, device=DEV).view(B, -1)
+    full = torch.full((B,), S, dtype=torch.int32, device=DEV)
+    q, kn, vn, qp = rnd(B, H * G, D), rnd(B, H, D), rnd(B, H, D), rnd(B, H * G, 64, D)
+    parts, rows = rnd(3, 5, D + 4).abs(), rnd(7, D)
+
+    def calls(stream):
+        spy = _Spy(kvd.lib())
+        kvd._lib, real = spy, kvd._lib
+        try:
+            lens = full - 1
+            k2, v2, ks2, vs2 = K.clone(), V.clone(), ks.clone(), vs.clone()
+            torch.cuda.synchronize()
+            outs = [kvd.decode(q, K, V, ks, vs, stream=stream),
+                    kvd.append_decode(kn, vn, q, k2, v2, ks2, vs2, lens, stream=stream),
+                    kvd.prefill(qp, K, V, ks, vs, stream=stream),
+                    kvd.paged_decode(q, Kp, Vp, ksp, vsp, table, full, stream=stream),
+                    kvd.combine(parts, stream=stream), *kvd.quantize_rows(rows, stream=stream)]
+        finally:
+            kvd._lib = real
+        torch.cuda.synchronize()
+        return outs, [args[-3] for args in spy.args[:4]], [args[-2] for args in spy.args[:4]]  # workspaces
+
+    want, _, _ = calls(None)
+    side = torch.cuda.Stream()
+    got, scratch, bytes_ = calls(side.cuda_stream if as_handle else side)
+    for a, b in zip(got, want):
+        assert torch.equal(a, b)
+    at = {t.data_ptr() for t in got} | set(scratch)
+    sizes = [t.nbytes for t in got] + bytes_
+    del got, a, b
+    for n in sizes:
+        again = [torch.empty(n, dtype=torch.uint8, device=DEV) for _ in range(8)]
+        assert not at & {t.data_ptr() for t in again}
+    assert kvd.device_status() == 0
