@@ -319,43 +319,48 @@ def _types():
     return _torch
 
 
-def _stream_of(stream, t) -> int:
-    """The given stream, or the current one of ``t``'s device."""
-    if stream is not None:
-        return _stream(stream)
-    torch = _types()[0]
-    raw = getattr(torch._C, "_cuda_getCurrentRawStream", None)
-    return raw(t.get_device()) if raw else torch.cuda.current_stream(t.device).cuda_stream
+_cuda = None
 
 
-def _made(make, stream, t, kept: bool = False):
-    """``make()``'s tensor, for a call on ``stream``: made with that stream current, so that what fills it runs there
-    too and its memory goes back to that stream's pool. ``kept``: the caller gets it, and may use it on the stream that
-    is current now."""
-    if stream is not None and _stream(stream) != _stream_of(None, t):
+def _cuda_state():
+    """(current stream's handle of a device, current device), looked up once: the public forms take longer than a check."""
+    global _cuda
+    if _cuda is None:
         torch = _types()[0]
-        if not isinstance(stream, torch.cuda.Stream):
-            handle = _stream(stream)
-            stream = torch.cuda.ExternalStream(handle, t.device) if handle else torch.cuda.default_stream(t.device)
-        here = torch.cuda.current_stream(t.device)
-        with torch.cuda.stream(stream):
-            made = make()
-        if kept:
-            made.record_stream(here)
-        return made
-    return make()
+        _cuda = (getattr(torch._C, "_cuda_getCurrentRawStream", None)
+                 or (lambda device: torch.cuda.current_stream(device).cuda_stream),
+                 getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device)
+    return _cuda
+
+
+def _made(make, shape, dtype, t, stream, kept: bool = False):
+    """A tensor of ``make`` (torch.empty, torch.zeros) on ``t``'s device for a call on ``stream``: made with that
+    stream current, so that what fills it runs there too and its memory goes back to that stream's pool. ``kept``: the
+    caller gets it, and may use it on the stream that is current now."""
+    if stream is None or _stream(stream) == _cuda_state()[0](t.get_device()):
+        return make(shape, dtype=dtype, device=t.device)
+    cuda = _types()[0].cuda
+    if not isinstance(stream, cuda.Stream):
+        handle = _stream(stream)
+        stream = cuda.ExternalStream(handle, t.device) if handle else cuda.default_stream(t.device)
+    here = cuda.current_stream(t.device)
+    with cuda.stream(stream):
+        made = make(shape, dtype=dtype, device=t.device)
+    if kept:
+        made.record_stream(here)
+    return made
 
 
 def _out(shape, dtype, t, stream):
     """An output (``dtype``, default float32) of a call on ``stream`` whose data lie where ``t`` does."""
-    torch = _types()[0]
-    return _made(lambda: torch.empty(shape, dtype=dtype or torch.float32, device=t.device), stream, t, kept=True)
+    types = _torch or _types()
+    return _made(types[0].empty, shape, dtype or types[4], t, stream, True)
 
 
 def _scratch(n: int, t, stream):
     """``n`` bytes (at least one) of scratch for a call on ``stream``."""
-    torch = _types()[0]
-    return _made(lambda: torch.empty(max(n, 1), dtype=torch.uint8, device=t.device), stream, t)
+    torch = (_torch or _types())[0]
+    return _made(torch.empty, n or 1, torch.uint8, t, stream)
 
 
 # ---------------------------------------------------------------- reference ABI
@@ -657,15 +662,33 @@ def _row_flags(dtype) -> int:
     return f
 
 
-def _want(t, dtype, shape, what: str) -> None:
-    """A contiguous tensor of this type and shape."""
-    if t.shape != shape or t.dtype != dtype or not t.is_contiguous():
-        raise ValueError(f"{what} must be contiguous {dtype} of shape {tuple(shape)}, got {t.dtype} {tuple(t.shape)}")
+def _want(device: int, dtype, *wanted) -> None:
+    """Contiguous tensors of this device and type: a (tensor, shape, name) each, tensors that are None aside."""
+    for t, shape, what in wanted:
+        if t is None:
+            continue
+        if t.shape != shape or t.dtype is not dtype or not t.is_contiguous():
+            raise ValueError(f"{what} must be contiguous {dtype} of shape {tuple(shape)}, got {t.dtype} {tuple(t.shape)}")
+        if t.get_device() != device:
+            raise _elsewhere(t)
 
 
-def _pools(k_pool, v_pool, ks_pool, vs_pool, layout: str):
+def _elsewhere(t) -> ValueError:
+    return ValueError(f"all tensors must be on one device, got another on {t.device}")
+
+
+def _handle(device: int, stream) -> int:
+    """The given stream, or the current one, of the tensors' device, which has to be the current device: launches go
+    there, and their sizes are its own."""
+    raw_stream, current_device = _cuda or _cuda_state()
+    if device < 0 or current_device() != device:
+        raise ValueError("tensors must be on the current CUDA device")
+    return raw_stream(device) if stream is None else _stream(stream)
+
+
+def _pools(device: int, k_pool, v_pool, ks_pool, vs_pool, layout: str):
     """(blocks, heads, block_size, head_dim, block stride, head stride, token stride, scale strides) of K and V pools."""
-    _, i8, _, _, f32 = _types()
+    _, i8, _, _, f32 = _torch or _types()
     shape, strides, sc_shape, sc_strides = k_pool.shape, k_pool.stride(), ks_pool.shape, ks_pool.stride()
     if layout == "bhtd":
         NB, H, bs, D = shape
@@ -682,16 +705,21 @@ def _pools(k_pool, v_pool, ks_pool, vs_pool, layout: str):
         raise ValueError("dims and scale tokens must be contiguous")
     if v_pool.stride() != strides or vs_pool.stride() != sc_strides or v_pool.shape != shape or vs_pool.shape != sc_shape:
         raise ValueError("K/V pools and their scale pools must share shapes and strides")
+    for t in (k_pool, v_pool, ks_pool, vs_pool):
+        if t.get_device() != device:
+            raise _elsewhere(t)
     if k_pool.dtype is not i8 or v_pool.dtype is not i8 or ks_pool.dtype is not f32 or vs_pool.dtype is not f32:
         raise ValueError("pools are int8, scale pools float32")
     return NB, H, bs, D, s_blk, s_h, s_t, sc_blk, sc_h
 
 
-def _table(block_table, B: int, i32) -> int:
+def _table(device: int, block_table, B: int, i32) -> int:
     """Entries per row of an int32 [B, max_blocks] table."""
     shape = block_table.shape
     if block_table.dtype != i32 or len(shape) != 2 or shape[0] != B or block_table.stride(1) != 1:
         raise ValueError("block_table must be int32 [B, max_blocks] with contiguous rows")
+    if block_table.get_device() != device:
+        raise _elsewhere(block_table)
     return shape[1]
 
 
@@ -704,44 +732,44 @@ def paged_plan(seq_lens, new_lens, block_table, free_blocks, free_count, block_s
     ids on it, ``slot_map`` int64 [num_slots]. The table, the free list and, unless other tensors are given for
     them, the lengths and the count are updated in place. ``workspace``: a zeroed uint8 tensor of 16 bytes that a
     caller keeps (without one, one is made). Returns (slot_map, token_starts [B + 1])."""
-    torch, _, i32, i64, _ = _types()
-    B = seq_lens.shape[0]
+    torch, _, i32, i64, _ = _torch or _types()
+    device, B = seq_lens.get_device(), seq_lens.shape[0]
+    MB = _table(device, block_table, B, i32)
+    NB, T = free_blocks.numel(), slot_map.numel()
+    rows, one = (B,), (1,)
+    _want(device, i32, (seq_lens, rows, "seq_lens"), (new_lens, rows, "new_lens"), (free_blocks, (NB,), "free_blocks"),
+          (free_count, one, "free_count"), (token_starts, (B + 1,), "token_starts"), (seq_lens_out, rows, "seq_lens_out"),
+          (free_count_out, one, "free_count_out"))
+    _want(device, i64, (slot_map, (T,), "slot_map"))
+    if workspace is not None and workspace.get_device() != device:
+        raise _elsewhere(workspace)
+    handle = _handle(device, stream)
+    if seq_lens_out is None:
+        seq_lens_out = seq_lens
+    if free_count_out is None:
+        free_count_out = free_count
     if token_starts is None:
         token_starts = _out((B + 1,), i32, seq_lens, stream)
     if workspace is None:  # zeroed on the call's stream
-        workspace = _made(lambda: torch.zeros(16, dtype=torch.uint8, device=seq_lens.device), stream, seq_lens)
-    rows, one = (B,), (1,)
-    _want(seq_lens, i32, rows, "seq_lens")
-    _want(new_lens, i32, rows, "new_lens")
-    _want(token_starts, i32, (B + 1,), "token_starts")
-    _want(free_count, i32, one, "free_count")
-    if seq_lens_out is None:
-        seq_lens_out = seq_lens
-    else:
-        _want(seq_lens_out, i32, rows, "seq_lens_out")
-    if free_count_out is None:
-        free_count_out = free_count
-    else:
-        _want(free_count_out, i32, one, "free_count_out")
-    MB = _table(block_table, B, i32)
-    NB, T = free_blocks.numel(), slot_map.numel()
-    _want(free_blocks, i32, (NB,), "free_blocks")
-    _want(slot_map, i64, (T,), "slot_map")
+        workspace = _made(torch.zeros, 16, torch.uint8, seq_lens, stream)
     desc = PagedPlanDesc(B, block_size, NB, MB, T, block_table.stride(0))
-    rc = lib().kvd_paged_plan_launch(
+    rc = (_lib or lib()).kvd_paged_plan_launch(
         ctypes.byref(desc), seq_lens.data_ptr(), new_lens.data_ptr(), block_table.data_ptr(), free_blocks.data_ptr(),
         free_count.data_ptr(), slot_map.data_ptr(), token_starts.data_ptr(), seq_lens_out.data_ptr(),
-        free_count_out.data_ptr(), workspace.data_ptr(), workspace.numel(), _stream_of(stream, seq_lens))
-    _check(rc, "kvd_paged_plan_launch")
+        free_count_out.data_ptr(), workspace.data_ptr(), workspace.nbytes, handle)
+    if rc:
+        _check(rc, "kvd_paged_plan_launch")
     return slot_map, token_starts
 
 
-def _rows_desc(k, v, slot_map, k_pool, v_pool, ks_pool, vs_pool, layout: str):
-    NB, H, bs, D, s_blk, s_h, s_t, sc_blk, sc_h = _pools(k_pool, v_pool, ks_pool, vs_pool, layout)
+def _rows_desc(device: int, k, v, slot_map, k_pool, v_pool, ks_pool, vs_pool, layout: str):
+    NB, H, bs, D, s_blk, s_h, s_t, sc_blk, sc_h = _pools(device, k_pool, v_pool, ks_pool, vs_pool, layout)
     T, (s_row, s_head, s_dim) = slot_map.shape[0], k.stride()
     if k.shape != (T, H, D) or v.shape != k.shape or v.dtype != k.dtype or v.stride() != (s_row, s_head, s_dim) or s_dim != 1:
         raise ValueError(f"rows must be two [{T}, {H}, {D}] tensors of one type and strides with contiguous dims")
-    _want(slot_map, _types()[3], (T,), "slot_map")
+    _want(device, _torch[3], (slot_map, (T,), "slot_map"))
+    if k.get_device() != device or v.get_device() != device:
+        raise _elsewhere(v if k.get_device() == device else k)
     return PagedRowsDesc(T, H, D, bs, NB, _row_flags(k.dtype), s_row, s_head, s_blk, s_h, s_t, sc_blk, sc_h)
 
 
@@ -750,35 +778,38 @@ def paged_write(k_new, v_new, slot_map, k_pool, v_pool, ks_pool, vs_pool, bounds
     """Quantises rows k_new / v_new [T, Hkv, D] (float32, bfloat16 or float16) into the pools' slots
     ``slot_map`` [T] (-1: skipped). With ``bounds`` int8 [blocks, Hkv, 2, D] and ``bound_scale`` float32
     [blocks, Hkv] the key bounds of every block written to are kept for :func:`block_select`."""
-    desc = _rows_desc(k_new, v_new, slot_map, k_pool, v_pool, ks_pool, vs_pool, layout)
+    device = k_pool.get_device()
+    desc = _rows_desc(device, k_new, v_new, slot_map, k_pool, v_pool, ks_pool, vs_pool, layout)
     if (bounds is None) != (bound_scale is None):
         raise ValueError("bounds and bound_scale come together")
     bounds_ptr = scale_ptr = None
     if bounds is not None:
         NB, H = desc.num_blocks, desc.num_kv_heads
-        _want(bounds, _types()[1], (NB, H, 2, desc.head_dim), "bounds")
-        _want(bound_scale, _types()[4], (NB, H), "bound_scale")
+        _want(device, _torch[1], (bounds, (NB, H, 2, desc.head_dim), "bounds"))
+        _want(device, _torch[4], (bound_scale, (NB, H), "bound_scale"))
         bounds_ptr, scale_ptr = bounds.data_ptr(), bound_scale.data_ptr()
-    rc = lib().kvd_paged_write_launch(ctypes.byref(desc), k_new.data_ptr(), v_new.data_ptr(), slot_map.data_ptr(),
+    rc = (_lib or lib()).kvd_paged_write_launch(ctypes.byref(desc), k_new.data_ptr(), v_new.data_ptr(), slot_map.data_ptr(),
                                       k_pool.data_ptr(), v_pool.data_ptr(), ks_pool.data_ptr(), vs_pool.data_ptr(),
-                                      bounds_ptr, scale_ptr, _stream_of(stream, k_pool))
-    _check(rc, "kvd_paged_write_launch")
+                                      bounds_ptr, scale_ptr, _handle(device, stream))
+    if rc:
+        _check(rc, "kvd_paged_write_launch")
 
 
 def paged_read(slot_map, k_pool, v_pool, ks_pool, vs_pool, k_out=None, v_out=None, layout: str = "bhtd", dtype=None,
                stream=None):
     """Rows of a paged cache by slot as the values that they stand for: returns (k_out, v_out) [T, Hkv, D]
     (``dtype``, default float32). Slots of -1 read as zeros."""
+    device = k_pool.get_device()
+    handle = _handle(device, stream)
     if k_out is None or v_out is None:
-        torch = _types()[0]
         H, D = k_pool.shape[1 if layout == "bhtd" else 2], k_pool.shape[3]
         shape = (slot_map.shape[0], H, D)
         k_out, v_out = (_out(shape, dtype, k_pool, stream) for _ in range(2))
-    desc = _rows_desc(k_out, v_out, slot_map, k_pool, v_pool, ks_pool, vs_pool, layout)
-    rc = lib().kvd_paged_read_launch(ctypes.byref(desc), slot_map.data_ptr(), k_pool.data_ptr(), v_pool.data_ptr(),
-                                     ks_pool.data_ptr(), vs_pool.data_ptr(), k_out.data_ptr(), v_out.data_ptr(),
-                                     _stream_of(stream, k_pool))
-    _check(rc, "kvd_paged_read_launch")
+    desc = _rows_desc(device, k_out, v_out, slot_map, k_pool, v_pool, ks_pool, vs_pool, layout)
+    rc = (_lib or lib()).kvd_paged_read_launch(ctypes.byref(desc), slot_map.data_ptr(), k_pool.data_ptr(), v_pool.data_ptr(),
+                                     ks_pool.data_ptr(), vs_pool.data_ptr(), k_out.data_ptr(), v_out.data_ptr(), handle)
+    if rc:
+        _check(rc, "kvd_paged_read_launch")
     return k_out, v_out
 
 
@@ -787,7 +818,7 @@ def block_select(q, bounds, bound_scale, block_table, seq_lens, block_size: int,
     """Blocks that one new token per request attends to (``kvd_block_select_launch``): the ``first`` first and
     ``last`` last blocks and those whose key bounds score highest for ``q`` [B, Hq, D], ``budget`` in all, per
     KV head. Returns (sel_table int32 [B, Hkv, budget] pool ids, then -1; sel_lens int32 [B, Hkv] tokens)."""
-    torch, i8, i32, _, f32 = _types()
+    torch, i8, i32, _, f32 = _torch or _types()
     B, Hq, D = q.shape
     NB, H, _, Db = bounds.shape
     if Db != D or Hq % H:
@@ -795,26 +826,28 @@ def block_select(q, bounds, bound_scale, block_table, seq_lens, block_size: int,
     s_b, s_h, s_d = q.stride()
     if s_d != 1:
         raise ValueError("dims must be contiguous")
-    MB = _table(block_table, B, i32)
-    _want(bounds, i8, (NB, H, 2, D), "bounds")
-    _want(bound_scale, f32, (NB, H), "bound_scale")
-    _want(seq_lens, i32, (B,), "seq_lens")
+    device = q.get_device()
+    MB = _table(device, block_table, B, i32)
+    _want(device, i8, (bounds, (NB, H, 2, D), "bounds"))
+    _want(device, f32, (bound_scale, (NB, H), "bound_scale"))
+    _want(device, i32, (seq_lens, (B,), "seq_lens"), (sel_table, (B, H, budget), "sel_table"),
+          (sel_lens, (B, H), "sel_lens"))
+    if workspace is not None and workspace.get_device() != device:
+        raise _elsewhere(workspace)
+    handle = _handle(device, stream)
     if sel_table is None:
         sel_table = _out((B, H, budget), i32, q, stream)
-    else:
-        _want(sel_table, i32, (B, H, budget), "sel_table")
     if sel_lens is None:
         sel_lens = _out((B, H), i32, q, stream)
-    else:
-        _want(sel_lens, i32, (B, H), "sel_lens")
     desc = BlockSelectDesc(B, Hq, H, D, block_size, NB, MB, budget, first, last, _row_flags(q.dtype),
                            seq_lens.data_ptr(), block_table.data_ptr(), block_table.stride(0), s_b, s_h)
     if workspace is None and MB > budget:
         workspace = _scratch(B * H * MB * 4, q, stream)
-    rc = lib().kvd_block_select_launch(ctypes.byref(desc), q.data_ptr(), bounds.data_ptr(), bound_scale.data_ptr(),
+    rc = (_lib or lib()).kvd_block_select_launch(ctypes.byref(desc), q.data_ptr(), bounds.data_ptr(), bound_scale.data_ptr(),
                                        sel_table.data_ptr(), sel_lens.data_ptr(), _ptr(workspace),
-                                       workspace.nbytes if workspace is not None else 0, _stream_of(stream, q))
-    _check(rc, "kvd_block_select_launch")
+                                       workspace.nbytes if workspace is not None else 0, handle)
+    if rc:
+        _check(rc, "kvd_block_select_launch")
     return sel_table, sel_lens
 
 
@@ -831,19 +864,23 @@ def sparse_decode(q, k_pool, v_pool, ks_pool, vs_pool, sel_table, sel_lens, out=
                   softmax_scale: float = 0.0, partial: bool = False, workspace=None, stream=None, out_dtype=None):
     """INT8 decode attention over selected blocks of a paged cache, ``sel_table`` int32 [B, Hkv, budget] and
     ``sel_lens`` int32 [B, Hkv] (:func:`block_select`'s); returns ``out`` [B, Hq, D] (or records)."""
-    torch, _, i32, _, f32 = _types()
+    torch, _, i32, _, f32 = _torch or _types()
     B, Hq, D = q.shape
     R = D + 4 if partial else D
-    if out is None:
-        out = _out((B, Hq, R), out_dtype, q, stream)
-    elif out.shape != (B, Hq, R):
+    if out is not None and out.shape != (B, Hq, R):
         raise ValueError(f"out must be [{B}, {Hq}, {R}], got {tuple(out.shape)}")
-    NB, H, bs, Dk, s_blk, s_h, s_t, sc_blk, sc_h = _pools(k_pool, v_pool, ks_pool, vs_pool, layout)
+    device = q.get_device()
+    NB, H, bs, Dk, s_blk, s_h, s_t, sc_blk, sc_h = _pools(device, k_pool, v_pool, ks_pool, vs_pool, layout)
     if Dk != D or Hq % H:
         raise ValueError(f"shape mismatch q{tuple(q.shape)} k_pool{tuple(k_pool.shape)}")
     budget = sel_table.shape[-1]
-    _want(sel_table, i32, (B, H, budget), "sel_table")
-    _want(sel_lens, i32, (B, H), "sel_lens")
+    _want(device, i32, (sel_table, (B, H, budget), "sel_table"), (sel_lens, (B, H), "sel_lens"))
+    for t in (out, workspace):
+        if t is not None and t.get_device() != device:
+            raise _elsewhere(t)
+    handle = _handle(device, stream)
+    if out is None:
+        out = _out((B, Hq, R), out_dtype, q, stream)
     q_b, q_h, q_d = q.stride()
     o_b, o_h, o_d = out.stride()
     if q_d != 1 or o_d != 1:
@@ -857,10 +894,11 @@ def sparse_decode(q, k_pool, v_pool, ks_pool, vs_pool, sel_table, sel_lens, out=
     if workspace is None:
         n = int(lib().kvd_sparse_workspace_size(ctypes.byref(desc)))
         workspace = _scratch(n, q, stream)
-    rc = lib().kvd_sparse_decode_launch(ctypes.byref(desc), q.data_ptr(), k_pool.data_ptr(), v_pool.data_ptr(),
+    rc = (_lib or lib()).kvd_sparse_decode_launch(ctypes.byref(desc), q.data_ptr(), k_pool.data_ptr(), v_pool.data_ptr(),
                                         ks_pool.data_ptr(), vs_pool.data_ptr(), out.data_ptr(), workspace.data_ptr(),
-                                        workspace.nbytes, _stream_of(stream, q))
-    _check(rc, "kvd_sparse_decode_launch")
+                                        workspace.nbytes, handle)
+    if rc:
+        _check(rc, "kvd_sparse_decode_launch")
     return out
 
 

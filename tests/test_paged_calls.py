@@ -6,6 +6,87 @@ import kvdecode as kvd
 from test_blocks import DEV, _same_plan, plan_inputs, plan_oracle
 
 
+class _NoLaunch:
+    """A library whose launches are counted and not made."""
+
+    def __init__(self):
+        self.names = []
+
+    def __getattr__(self, name):
+        if name.endswith("_size"):
+            return lambda *args: 64
+        return lambda *args: self.names.append(name) or 0
+
+
+def _every_call():
+    """(call, names of its tensors, tensors) of every paged serving step, all on the host."""
+    import torch
+
+    B, H, G, D, bs, MB, NB, T, k = 2, 2, 2, 64, 8, 4, 9, 3, 2
+    i8, i32, i64 = torch.int8, torch.int32, torch.int64
+    z = lambda *shape, dtype=torch.float32: torch.zeros(shape, dtype=dtype)  # noqa: E731
+    pools = lambda: dict(k_pool=z(NB, H, bs, D, dtype=i8), v_pool=z(NB, H, bs, D, dtype=i8),  # noqa: E731
+                         ks_pool=z(NB, H, bs), vs_pool=z(NB, H, bs))
+    return [
+        (lambda **t: kvd.paged_plan(block_size=bs, **t),
+         dict(seq_lens=z(B, dtype=i32), new_lens=z(B, dtype=i32), block_table=z(B, MB, dtype=i32),
+              free_blocks=z(NB, dtype=i32), free_count=z(1, dtype=i32), slot_map=z(T, dtype=i64),
+              token_starts=z(B + 1, dtype=i32), seq_lens_out=z(B, dtype=i32), free_count_out=z(1, dtype=i32),
+              workspace=z(16, dtype=torch.uint8))),
+        (kvd.paged_write, dict(k_new=z(T, H, D), v_new=z(T, H, D), slot_map=z(T, dtype=i64), **pools(),
+                               bounds=z(NB, H, 2, D, dtype=i8), bound_scale=z(NB, H))),
+        (kvd.paged_read, dict(slot_map=z(T, dtype=i64), **pools(), k_out=z(T, H, D), v_out=z(T, H, D))),
+        (lambda **t: kvd.block_select(block_size=bs, budget=k, last=1, **t),
+         dict(q=z(B, H * G, D), bounds=z(NB, H, 2, D, dtype=i8), bound_scale=z(NB, H), block_table=z(B, MB, dtype=i32),
+              seq_lens=z(B, dtype=i32), sel_table=z(B, H, k, dtype=i32), sel_lens=z(B, H, dtype=i32),
+              workspace=z(256, dtype=torch.uint8))),
+        (kvd.sparse_decode, dict(q=z(B, H * G, D), **pools(), sel_table=z(B, H, k, dtype=i32),
+                                 sel_lens=z(B, H, dtype=i32), out=z(B, H * G, D), workspace=z(64, dtype=torch.uint8)))]
+
+
+@pytest.mark.parametrize("which", range(5))
+def test_tensors_of_another_device_are_refused(which, monkeypatch):
+    """A tensor left on the host, or on another GPU than the rest, is a ValueError and nothing is launched: the
+    library would take its address for one of the GPU's. Devices are pretended."""
+    import torch
+
+    call, tensors = _every_call()[which]
+    lib = _NoLaunch()
+    monkeypatch.setattr(kvd, "_lib", lib)
+    monkeypatch.setattr(kvd, "_cuda", (None, lambda: 0), raising=False)
+    with pytest.raises(ValueError):
+        call(**tensors, stream=0)  # all on the host
+    where = {}
+    monkeypatch.setattr(torch.Tensor, "get_device", lambda t: where.get(id(t), 0))
+    call(**tensors, stream=0)
+    assert len(lib.names) == 1
+    for name, t in tensors.items():
+        for device in (-1, 1):
+            where = {id(t): device}
+            with pytest.raises(ValueError):
+                call(**tensors, stream=0)
+    assert len(lib.names) == 1
+
+
+@pytest.mark.parametrize("which", range(5))
+def test_tensors_of_a_gpu_that_is_not_current_are_refused(which, monkeypatch):
+    """Launches go to the current device and are sized for it: tensors of another GPU are a ValueError there."""
+    import torch
+
+    call, tensors = _every_call()[which]
+    lib = _NoLaunch()
+    monkeypatch.setattr(kvd, "_lib", lib)
+    monkeypatch.setattr(kvd, "_cuda", (None, lambda: 0), raising=False)
+    for index, launches in ((0, 1), (1, 1)):
+        monkeypatch.setattr(torch.Tensor, "get_device", lambda t: index)
+        if index == 0:
+            call(**tensors, stream=0)
+        else:
+            with pytest.raises(ValueError):
+                call(**tensors, stream=0)
+        assert len(lib.names) == launches
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("as_handle", [False, True])
 def test_plan_on_a_side_stream_without_a_workspace(as_handle):
@@ -163,4 +244,19 @@ def test_scratch_of_the_dense_and_paged_calls_belongs_to_their_stream(as_handle)
     for n in sizes:
         again = [torch.empty(n, dtype=torch.uint8, device=DEV) for _ in range(8)]
         assert not at & {t.data_ptr() for t in again}
+    assert kvd.device_status() == 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("which", range(5))
+def test_host_tensors_among_the_gpu_s_are_refused(which):
+    """As above with real devices: every tensor in turn is left on the host. Refused before anything is launched."""
+    import torch
+
+    call, tensors = _every_call()[which]
+    there = {name: t.to(DEV) for name, t in tensors.items()}
+    for name in tensors:
+        with pytest.raises(ValueError):
+            call(**{**there, name: tensors[name]})
+    torch.cuda.synchronize()
     assert kvd.device_status() == 0
