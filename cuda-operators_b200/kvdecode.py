@@ -788,9 +788,9 @@ def paged_write(k_new, v_new, slot_map, k_pool, v_pool, ks_pool, vs_pool, bounds
         _want(device, _torch[1], (bounds, (NB, H, 2, desc.head_dim), "bounds"))
         _want(device, _torch[4], (bound_scale, (NB, H), "bound_scale"))
         bounds_ptr, scale_ptr = bounds.data_ptr(), bound_scale.data_ptr()
-    rc = (_lib or lib()).kvd_paged_write_launch(ctypes.byref(desc), k_new.data_ptr(), v_new.data_ptr(), slot_map.data_ptr(),
-                                      k_pool.data_ptr(), v_pool.data_ptr(), ks_pool.data_ptr(), vs_pool.data_ptr(),
-                                      bounds_ptr, scale_ptr, _handle(device, stream))
+    rc = (_lib or lib()).kvd_paged_write_launch(
+        ctypes.byref(desc), k_new.data_ptr(), v_new.data_ptr(), slot_map.data_ptr(), k_pool.data_ptr(),
+        v_pool.data_ptr(), ks_pool.data_ptr(), vs_pool.data_ptr(), bounds_ptr, scale_ptr, _handle(device, stream))
     if rc:
         _check(rc, "kvd_paged_write_launch")
 
@@ -798,16 +798,26 @@ def paged_write(k_new, v_new, slot_map, k_pool, v_pool, ks_pool, vs_pool, bounds
 def paged_read(slot_map, k_pool, v_pool, ks_pool, vs_pool, k_out=None, v_out=None, layout: str = "bhtd", dtype=None,
                stream=None):
     """Rows of a paged cache by slot as the values that they stand for: returns (k_out, v_out) [T, Hkv, D]
-    (``dtype``, default float32). Slots of -1 read as zeros."""
+    (``dtype``, default float32; an output that is given sets the type and strides of the other). Slots of -1 read as
+    zeros."""
     device = k_pool.get_device()
     handle = _handle(device, stream)
-    if k_out is None or v_out is None:
+    if k_out is None and v_out is None:
         H, D = k_pool.shape[1 if layout == "bhtd" else 2], k_pool.shape[3]
         shape = (slot_map.shape[0], H, D)
         k_out, v_out = (_out(shape, dtype, k_pool, stream) for _ in range(2))
+    else:
+        given = v_out if k_out is None else k_out
+        if dtype is not None and given.dtype is not dtype:
+            raise ValueError(f"outputs of {given.dtype} are given, {dtype} is asked for")
+        if k_out is None or v_out is None:
+            make = lambda shape, **how: (_torch or _types())[0].empty_strided(shape, given.stride(), **how)  # noqa: E731
+            other = _made(make, given.shape, given.dtype, k_pool, stream, True)
+            k_out, v_out = (other, v_out) if k_out is None else (k_out, other)
     desc = _rows_desc(device, k_out, v_out, slot_map, k_pool, v_pool, ks_pool, vs_pool, layout)
-    rc = (_lib or lib()).kvd_paged_read_launch(ctypes.byref(desc), slot_map.data_ptr(), k_pool.data_ptr(), v_pool.data_ptr(),
-                                     ks_pool.data_ptr(), vs_pool.data_ptr(), k_out.data_ptr(), v_out.data_ptr(), handle)
+    rc = (_lib or lib()).kvd_paged_read_launch(
+        ctypes.byref(desc), slot_map.data_ptr(), k_pool.data_ptr(), v_pool.data_ptr(), ks_pool.data_ptr(),
+        vs_pool.data_ptr(), k_out.data_ptr(), v_out.data_ptr(), handle)
     if rc:
         _check(rc, "kvd_paged_read_launch")
     return k_out, v_out
@@ -843,9 +853,9 @@ def block_select(q, bounds, bound_scale, block_table, seq_lens, block_size: int,
                            seq_lens.data_ptr(), block_table.data_ptr(), block_table.stride(0), s_b, s_h)
     if workspace is None and MB > budget:
         workspace = _scratch(B * H * MB * 4, q, stream)
-    rc = (_lib or lib()).kvd_block_select_launch(ctypes.byref(desc), q.data_ptr(), bounds.data_ptr(), bound_scale.data_ptr(),
-                                       sel_table.data_ptr(), sel_lens.data_ptr(), _ptr(workspace),
-                                       workspace.nbytes if workspace is not None else 0, handle)
+    rc = (_lib or lib()).kvd_block_select_launch(
+        ctypes.byref(desc), q.data_ptr(), bounds.data_ptr(), bound_scale.data_ptr(), sel_table.data_ptr(),
+        sel_lens.data_ptr(), _ptr(workspace), workspace.nbytes if workspace is not None else 0, handle)
     if rc:
         _check(rc, "kvd_block_select_launch")
     return sel_table, sel_lens
@@ -894,9 +904,9 @@ def sparse_decode(q, k_pool, v_pool, ks_pool, vs_pool, sel_table, sel_lens, out=
     if workspace is None:
         n = int(lib().kvd_sparse_workspace_size(ctypes.byref(desc)))
         workspace = _scratch(n, q, stream)
-    rc = (_lib or lib()).kvd_sparse_decode_launch(ctypes.byref(desc), q.data_ptr(), k_pool.data_ptr(), v_pool.data_ptr(),
-                                        ks_pool.data_ptr(), vs_pool.data_ptr(), out.data_ptr(), workspace.data_ptr(),
-                                        workspace.nbytes, handle)
+    rc = (_lib or lib()).kvd_sparse_decode_launch(
+        ctypes.byref(desc), q.data_ptr(), k_pool.data_ptr(), v_pool.data_ptr(), ks_pool.data_ptr(), vs_pool.data_ptr(),
+        out.data_ptr(), workspace.data_ptr(), workspace.nbytes, handle)
     if rc:
         _check(rc, "kvd_sparse_decode_launch")
     return out

@@ -87,6 +87,51 @@ def test_tensors_of_a_gpu_that_is_not_current_are_refused(which, monkeypatch):
         assert len(lib.names) == launches
 
 
+@pytest.mark.parametrize("given", ["k_out", "v_out"])
+def test_read_makes_the_output_that_is_missing(given, monkeypatch):
+    """One output given, part of a wider tensor: it is the one that the call fills and returns, and the other is made
+    with its type and strides. Devices are pretended, nothing is launched."""
+    import torch
+
+    _, tensors = _every_call()[2]
+    buffer = torch.empty((3, 4, 64), dtype=torch.bfloat16)[:, 1:3]
+    tensors = {n: t for n, t in tensors.items() if n not in ("k_out", "v_out")}
+    args = []
+
+    class Lib:
+        kvd_paged_read_launch = staticmethod(lambda *a: args.append(a) or 0)
+
+    monkeypatch.setattr(kvd, "_lib", Lib())
+    monkeypatch.setattr(kvd, "_cuda", (lambda device: 0, lambda: 0), raising=False)
+    monkeypatch.setattr(torch.Tensor, "get_device", lambda t: 0)
+    out = kvd.paged_read(**tensors, **{given: buffer})
+    at = 0 if given == "k_out" else 1
+    assert out[at] is buffer and out[0].data_ptr() != out[1].data_ptr()
+    assert out[1 - at].dtype == torch.bfloat16 and out[1 - at].stride() == buffer.stride()
+    assert args[0][6:8] == (out[0].data_ptr(), out[1].data_ptr())
+    with pytest.raises(ValueError):
+        kvd.paged_read(**tensors, **{given: buffer}, dtype=torch.float32)
+    with pytest.raises(ValueError):
+        kvd.paged_read(**tensors, k_out=buffer, v_out=torch.empty_like(buffer), dtype=torch.float16)
+    assert len(args) == 1
+
+
+@pytest.mark.gpu
+def test_read_into_one_given_output():
+    """On the GPU: the given half of a fused buffer gets the rows, the other output the same as a call without any."""
+    import torch
+
+    x = _step_inputs()
+    pools = (x["K"], x["V"], x["ks"], x["vs"])
+    want = kvd.paged_read(x["slots"], *pools, dtype=torch.bfloat16)
+    for at in (0, 1):
+        wide = torch.zeros((5000, 3, 2, 64), dtype=torch.bfloat16, device=DEV)
+        given = wide[:, 1]
+        got = kvd.paged_read(x["slots"], *pools, **{("k_out", "v_out")[at]: given})
+        assert got[at] is given and torch.equal(given, want[at]) and torch.equal(got[1 - at], want[1 - at])
+        assert not wide[:, 0].any() and not wide[:, 2].any()
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("as_handle", [False, True])
 def test_plan_on_a_side_stream_without_a_workspace(as_handle):
