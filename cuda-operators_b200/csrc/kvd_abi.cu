@@ -317,6 +317,7 @@ extern "C" cudaError_t kvd_sparse_decode_launch(const kvd_paged_desc* desc, cons
     if (desc->flags & KVD_FLAG_QK_INT8) return cudaErrorNotSupported;
     if ((desc->flags & KVD_FLAG_PARTIAL_OUT) && desc->num_q_heads > 1 && desc->o_stride_h < desc->head_dim + 4)
         return cudaErrorInvalidValue;
+    if ((reinterpret_cast<uintptr_t>(workspace) & 3) != 0) return cudaErrorInvalidValue;
     if (!workspace) workspace_bytes = 0;
     PagedView pv;
     const kvd_decode_desc d = paged_as_dense(*desc, &pv);

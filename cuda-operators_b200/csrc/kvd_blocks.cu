@@ -1269,7 +1269,9 @@ extern "C" cudaError_t kvd_paged_plan_launch(const kvd_paged_plan_desc* desc, co
     if (!plan_ok(desc) || !seq_lens || !new_lens || !block_table || !free_blocks || !free_count || !token_starts ||
         !seq_lens_out || !free_count_out || (!slot_map && desc->num_slots > 0))
         return cudaErrorInvalidValue;
-    if (!workspace || workspace_bytes < kvd_paged_plan_workspace_size(desc)) return cudaErrorInvalidValue;
+    if (!workspace || workspace_bytes < kvd_paged_plan_workspace_size(desc) ||
+        (reinterpret_cast<uintptr_t>(workspace) & 3) != 0)
+        return cudaErrorInvalidValue;
     PlanParams p{*desc, seq_lens, new_lens, block_table, free_blocks, free_count, slot_map, token_starts,
                  seq_lens_out, free_count_out, static_cast<unsigned int*>(workspace),
                  FastDiv(static_cast<uint32_t>(desc->block_size))};

@@ -673,6 +673,16 @@ def _want(device: int, dtype, *wanted) -> None:
             raise _elsewhere(t)
 
 
+def _own_scratch(device: int, workspace) -> None:
+    """A caller's workspace: bytes that lie together, on the device."""
+    if workspace is None:
+        return
+    if not workspace.is_contiguous():
+        raise ValueError("workspace must be contiguous")
+    if workspace.get_device() != device:
+        raise _elsewhere(workspace)
+
+
 def _elsewhere(t) -> ValueError:
     return ValueError(f"all tensors must be on one device, got another on {t.device}")
 
@@ -741,8 +751,7 @@ def paged_plan(seq_lens, new_lens, block_table, free_blocks, free_count, block_s
           (free_count, one, "free_count"), (token_starts, (B + 1,), "token_starts"), (seq_lens_out, rows, "seq_lens_out"),
           (free_count_out, one, "free_count_out"))
     _want(device, i64, (slot_map, (T,), "slot_map"))
-    if workspace is not None and workspace.get_device() != device:
-        raise _elsewhere(workspace)
+    _own_scratch(device, workspace)
     handle = _handle(device, stream)
     if seq_lens_out is None:
         seq_lens_out = seq_lens
@@ -842,8 +851,7 @@ def block_select(q, bounds, bound_scale, block_table, seq_lens, block_size: int,
     _want(device, f32, (bound_scale, (NB, H), "bound_scale"))
     _want(device, i32, (seq_lens, (B,), "seq_lens"), (sel_table, (B, H, budget), "sel_table"),
           (sel_lens, (B, H), "sel_lens"))
-    if workspace is not None and workspace.get_device() != device:
-        raise _elsewhere(workspace)
+    _own_scratch(device, workspace)
     handle = _handle(device, stream)
     if sel_table is None:
         sel_table = _out((B, H, budget), i32, q, stream)
@@ -885,9 +893,9 @@ def sparse_decode(q, k_pool, v_pool, ks_pool, vs_pool, sel_table, sel_lens, out=
         raise ValueError(f"shape mismatch q{tuple(q.shape)} k_pool{tuple(k_pool.shape)}")
     budget = sel_table.shape[-1]
     _want(device, i32, (sel_table, (B, H, budget), "sel_table"), (sel_lens, (B, H), "sel_lens"))
-    for t in (out, workspace):
-        if t is not None and t.get_device() != device:
-            raise _elsewhere(t)
+    if out is not None and out.get_device() != device:
+        raise _elsewhere(out)
+    _own_scratch(device, workspace)
     handle = _handle(device, stream)
     if out is None:
         out = _out((B, Hq, R), out_dtype, q, stream)

@@ -242,7 +242,8 @@ cudaError_t kvd_paged_append_int8_launch(const kvd_paged_desc* desc,
  * the index of each request's first new token (refused ones count), at most
  * num_slots. seq_lens_out and free_count_out may be seq_lens and free_count.
  * At most 8192 requests (cudaErrorInvalidValue above). The workspace of
- * kvd_paged_plan_workspace_size bytes is zeroed by the caller once; calls
+ * kvd_paged_plan_workspace_size bytes, on a 4-byte boundary as every workspace
+ * of this section (cudaErrorInvalidValue), is zeroed by the caller once; calls
  * leave it zeroed. Concurrent calls need separate workspaces. */
 #define KVD_STATUS_NO_BLOCKS 8
 typedef struct kvd_paged_plan_desc {

@@ -1,5 +1,6 @@
 """The bindings of the paged serving steps: streams, scratch, devices and outputs (no reference counterpart)."""
-import numpy as np
+import ctypes
+
 import pytest
 
 import kvdecode as kvd
@@ -85,6 +86,36 @@ def test_tensors_of_a_gpu_that_is_not_current_are_refused(which, monkeypatch):
             with pytest.raises(ValueError):
                 call(**tensors, stream=0)
         assert len(lib.names) == launches
+
+
+def test_workspaces_off_their_boundary_are_refused():
+    """Workspaces hold 32-bit words: one on another boundary would be a misaligned access in the kernels. Host checks
+    alone, nothing is launched."""
+    L = kvd.lib()
+    plan = kvd.PagedPlanDesc(4, 16, 8, 4, 10, 4)
+    sparse = kvd.PagedDesc(batch=2, num_q_heads=8, num_kv_heads=2, head_dim=128, block_size=16, num_blocks=64,
+                           max_blocks_per_seq=8, seq_lens=256, block_table=256, block_table_stride=8, o_stride_h=128)
+    select = kvd.BlockSelectDesc(2, 8, 2, 64, 16, 40, 20, 8, 1, 2, 0, 256, 256, 20, 512, 64)
+    for at in (257, 258, 259):
+        assert L.kvd_paged_plan_launch(ctypes.byref(plan), *[256] * 9, at, 64, None) == kvd.CUDA_ERROR_INVALID_VALUE
+        assert L.kvd_sparse_decode_launch(ctypes.byref(sparse), *[256] * 6, at, 1 << 20, None) == kvd.CUDA_ERROR_INVALID_VALUE
+        assert L.kvd_block_select_launch(ctypes.byref(select), *[256] * 5, at, 1 << 20, None) == kvd.CUDA_ERROR_INVALID_VALUE
+
+
+@pytest.mark.parametrize("which", [0, 3, 4])
+def test_workspaces_with_gaps_are_refused(which, monkeypatch):
+    """A strided view's bytes do not lie together; nothing is launched for it."""
+    import torch
+
+    call, tensors = _every_call()[which]
+    lib = _NoLaunch()
+    monkeypatch.setattr(kvd, "_lib", lib)
+    monkeypatch.setattr(kvd, "_cuda", (None, lambda: 0), raising=False)
+    monkeypatch.setattr(torch.Tensor, "get_device", lambda t: 0)
+    for gaps in (torch.zeros((512, 2), dtype=torch.uint8)[:, 0], torch.zeros(1, dtype=torch.uint8).expand(512)):
+        with pytest.raises(ValueError):
+            call(**{**tensors, "workspace": gaps}, stream=0)
+    assert not lib.names
 
 
 @pytest.mark.parametrize("given", ["k_out", "v_out"])
