@@ -1332,6 +1332,8 @@ bool select_ok(const kvd_block_select_desc* p) {
         static_cast<int64_t>(d.max_blocks_per_seq) * d.block_size > 0x7fffffffLL)
         return false;
     if (d.budget < 1 || d.first < 0 || d.last < 1 || d.first > d.budget - d.last) return false;
+    // the kernels step over blocks and entries in ints, up to 1,024 threads and a tile past the last
+    if (d.max_blocks_per_seq > 0x40000000 || d.budget > 0x40000000) return false;
     if (static_cast<int64_t>(d.batch) * d.num_kv_heads > 0x7fffffffLL) return false;
     return d.flags == 0 || d.flags == KVD_FLAG_Q_BF16 || d.flags == KVD_FLAG_Q_F16;
 }

@@ -308,7 +308,8 @@ cudaError_t kvd_paged_read_launch(const kvd_paged_rows_desc* desc, const int64_t
  * receives the selected blocks' pool ids in token order, then -1, and sel_lens
  * [batch][num_kv_heads] the tokens in them: only the last selected block can
  * be partly filled. A block id outside the pool scores below all others and
- * records KVD_STATUS_BAD_BLOCK. head_dim at most 512. The workspace of
+ * records KVD_STATUS_BAD_BLOCK. head_dim at most 512; tables and budgets of
+ * more than 2^30 blocks return cudaErrorInvalidValue. The workspace of
  * kvd_block_select_workspace_size bytes (a key per table entry and KV head; 0
  * when no row can hold more than its budget) needs no initialisation. */
 typedef struct kvd_block_select_desc {

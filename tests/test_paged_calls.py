@@ -102,6 +102,23 @@ def test_workspaces_off_their_boundary_are_refused():
         assert L.kvd_block_select_launch(ctypes.byref(select), *[256] * 5, at, 1 << 20, None) == kvd.CUDA_ERROR_INVALID_VALUE
 
 
+def test_selections_past_two_to_the_30_blocks_are_refused():
+    """The kernels count blocks in 32 bits: a table of nearly 2^31 blocks of one token, or a budget of as many, would
+    pass them. Such sizes do not reach a kernel; 2^30 do."""
+    L = kvd.lib()
+
+    def size(blocks, budget):
+        d = kvd.BlockSelectDesc(1, 1, 1, 64, 1, 40, blocks, budget, 1, 2, 0, 256, 256, blocks, 64, 64)
+        if blocks > 1 << 30 or budget > 1 << 30:
+            assert L.kvd_block_select_launch(ctypes.byref(d), *[256] * 6, 1 << 62, None) == kvd.CUDA_ERROR_INVALID_VALUE
+        return L.kvd_block_select_workspace_size(ctypes.byref(d))
+
+    assert size(1 << 30, 8) == 4 << 30
+    for blocks in ((1 << 30) + 1, (1 << 31) - 128, (1 << 31) - 1):
+        assert size(blocks, 8) == 0
+        size(100, blocks)
+
+
 @pytest.mark.parametrize("which", [0, 3, 4])
 def test_workspaces_with_gaps_are_refused(which, monkeypatch):
     """A strided view's bytes do not lie together; nothing is launched for it."""
