@@ -936,13 +936,14 @@ cudaError_t rows_call(RowsParams& p, const void* a, const void* b, bool write, c
 // (request, KV head) that finds the threshold and writes the table.
 
 // Scores for head dims other than 64, 128 and 256 and groups of more than 64
-// heads: a warp a CTA, query codes in shared memory. Bound: instructions; 16 x
-// 512 blocks x 8 heads of 128 take 97 us, by tensor cores 12.
-__global__ void __launch_bounds__(32) score_any_kernel(const SelectParams p) {
-    extern __shared__ int8_t any_smem[];  // [G][D] codes, padded to 4, then [G] scales
+// heads: a warp a CTA, query codes in shared memory, as many heads at a time as
+// 48 KB hold (95 of 512 dims). Bound: instructions; 16 x 512 blocks x 8 heads of
+// 128 take 97 us, by tensor cores 12.
+__global__ void __launch_bounds__(32) score_any_kernel(const SelectParams p, int heads) {
+    extern __shared__ int8_t any_smem[];  // [heads][D] codes, padded to 4, then [heads] scales
     const kvd_block_select_desc& d = p.d;
     const int D = d.head_dim, H = d.num_kv_heads, G = d.num_q_heads / H, lane = threadIdx.x;
-    float* scale = reinterpret_cast<float*>(any_smem + ((G * D + 3) & ~3));
+    float* scale = reinterpret_cast<float*>(any_smem + ((heads * D + 3) & ~3));
     const int chunks = (d.max_blocks_per_seq + 15) / 16, items = d.batch * H * chunks;
     grid_dependency_wait();
     allow_dependents();
@@ -956,37 +957,41 @@ __global__ void __launch_bounds__(32) score_any_kernel(const SelectParams p) {
         select_len(d, I.b, n);
         if (n <= d.budget || I.i0 >= n) continue;
         I.m = min(16, n - I.i0);
-        __syncwarp();
-        for (int g = 0; g < G; ++g) {
-            const int64_t q0 = I.b * d.q_stride_b + static_cast<int64_t>(I.h * G + g) * d.q_stride_h;
-            float x[16];
-#pragma unroll
-            for (int j = 0; j < 16; ++j) x[j] = lane + 32 * j < D ? load_q(p.Q, q0 + lane + 32 * j, d.flags) : 0.f;
-            const float s = quantise_divided<0>(x);
-#pragma unroll
-            for (int j = 0; j < 16; ++j)
-                if (lane + 32 * j < D) any_smem[g * D + lane + 32 * j] = static_cast<int8_t>(x[j]);
-            if (lane == 0) scale[g] = s;
-        }
-        __syncwarp();
         const int32_t* table = d.block_table + I.b * d.block_table_stride + I.i0;
-        uint32_t* keys = p.keys + static_cast<int64_t>(I.row) * d.max_blocks_per_seq + I.i0;
-        for (int i = 0; i < I.m; ++i) {
-            const int id = pool_id(d, table, i);
-            const int64_t at = static_cast<int64_t>(max(id, 0)) * H + I.h;
-            const int8_t* r = p.bounds + at * (2 * D);
-            float best = -INFINITY;
-            for (int g = 0; g < G; ++g) {
-                int acc = 0;
-                for (int x = lane; x < D; x += 32) {
-                    const int c = any_smem[g * D + x];
-                    acc += c * (c > 0 ? r[x] : r[D + x]);
-                }
-                const float v = static_cast<float>(__reduce_add_sync(0xffffffffu, acc)) * scale[g];
-                best = fmaxf(best, isnan(v) ? INFINITY : v);
+        const int id = lane < I.m ? pool_id(d, table, lane) : -1;  // of this lane's block
+        float best = -INFINITY;                                    // its score over the heads so far
+        for (int g0 = 0; g0 < G; g0 += heads) {
+            const int m = min(heads, G - g0);
+            __syncwarp();
+            for (int g = 0; g < m; ++g) {
+                const int64_t q0 = I.b * d.q_stride_b + static_cast<int64_t>(I.h * G + g0 + g) * d.q_stride_h;
+                float x[16];
+#pragma unroll
+                for (int j = 0; j < 16; ++j) x[j] = lane + 32 * j < D ? load_q(p.Q, q0 + lane + 32 * j, d.flags) : 0.f;
+                const float s = quantise_divided<0>(x);
+#pragma unroll
+                for (int j = 0; j < 16; ++j)
+                    if (lane + 32 * j < D) any_smem[g * D + lane + 32 * j] = static_cast<int8_t>(x[j]);
+                if (lane == 0) scale[g] = s;
             }
-            if (lane == 0) keys[i] = id < 0 ? kNoBlockKey : score_key(best * p.bound_scale[at]);
+            __syncwarp();
+            for (int i = 0; i < I.m; ++i) {
+                const int64_t at = static_cast<int64_t>(max(__shfl_sync(0xffffffffu, id, i), 0)) * H + I.h;
+                const int8_t* r = p.bounds + at * (2 * D);
+                for (int g = 0; g < m; ++g) {
+                    int acc = 0;
+                    for (int x = lane; x < D; x += 32) {
+                        const int c = any_smem[g * D + x];
+                        acc += c * (c > 0 ? r[x] : r[D + x]);
+                    }
+                    const float v = static_cast<float>(__reduce_add_sync(0xffffffffu, acc)) * scale[g];
+                    if (lane == i) best = fmaxf(best, isnan(v) ? INFINITY : v);
+                }
+            }
         }
+        if (lane < I.m)
+            p.keys[static_cast<int64_t>(I.row) * d.max_blocks_per_seq + I.i0 + lane] =
+                id < 0 ? kNoBlockKey : score_key(best * p.bound_scale[static_cast<int64_t>(id) * H + I.h]);
     }
 }
 
@@ -1228,10 +1233,11 @@ cudaError_t launch_select(const SelectParams& p, cudaStream_t st) {
             e = launch_score_tc(p, st);
         } else {
             const int64_t items = rows * ((d.max_blocks_per_seq + 15) / 16), most = static_cast<int64_t>(device_sm_count()) * 16;
-            const int G = d.num_q_heads / d.num_kv_heads;
-            const size_t smem = ((static_cast<size_t>(G) * d.head_dim + 3) & ~size_t(3)) + sizeof(float) * G;
-            if (smem > 48 * 1024 || items > 0x7fff0000LL) return cudaErrorInvalidValue;
-            e = launch_after(score_any_kernel, static_cast<unsigned>(items < most ? items : most), 32, smem, st, p);
+            const int G = d.num_q_heads / d.num_kv_heads, most_heads = (48 * 1024 - 4) / (d.head_dim + 4);
+            const int heads = G < most_heads ? G : most_heads;
+            const size_t smem = ((static_cast<size_t>(heads) * d.head_dim + 3) & ~size_t(3)) + sizeof(float) * heads;
+            if (items > 0x7fff0000LL) return cudaErrorInvalidValue;
+            e = launch_after(score_any_kernel, static_cast<unsigned>(items < most ? items : most), 32, smem, st, p, heads);
         }
         if (e != cudaSuccess) return e;
         ++*launch_counter();

@@ -4,7 +4,7 @@ import ctypes
 import pytest
 
 import kvdecode as kvd
-from test_blocks import DEV, _same_plan, plan_inputs, plan_oracle
+from test_blocks import DEV, _check_select, _same_plan, plan_inputs, plan_oracle, select_inputs
 
 
 class _NoLaunch:
@@ -353,3 +353,17 @@ def test_host_tensors_among_the_gpu_s_are_refused(which):
             call(**{**there, name: tensors[name]})
     torch.cuda.synchronize()
     assert kvd.device_status() == 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("G,D,MB", [(97, 512, 40), (200, 256, 40), (800, 64, 37), (480, 100, 50), (65, 128, 90)])
+def test_select_of_wide_groups(G, D, MB):
+    """Groups whose query codes do not fit into shared memory together are scored a part at a time."""
+    bs, k = 16, 9
+    lens = [MB * bs, (k + 1) * bs - 3, k * bs]
+    q, bounds, step, table, lens = select_inputs(G, 3, 2, G, D, bs, MB, lens)
+    q *= 0.1 + 0.9 * (abs(q[:, :, :1]) > 1.8)  # the heads that weigh most lie anywhere in the group
+    step[3::11] = float("nan")
+    table[0, 5], table[1, 2] = -1, 10 ** 8
+    _check_select(q, bounds, step, table, lens, bs, k, 1, 2)
+    assert kvd.device_status() == kvd.KVD_STATUS_BAD_BLOCK
