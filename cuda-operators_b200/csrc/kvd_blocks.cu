@@ -36,9 +36,9 @@ cudaError_t launch_after(void (*kern)(A...), unsigned grid, unsigned block, size
 // the sums all writes run in parallel. Every CTA makes the sums itself (8 bytes
 // a request from L2, an exchange through shared memory a sum) and writes its
 // share, a slot per thread where that many threads fit on the GPU. Bound:
-// latency, a chain of three loads and the sums' barriers: 3.3 us for 8 requests
-// and 8.2 us for 1,024 with 65,536 new tokens. Up to 256 requests a CTA has 256
-// threads, above that 1,024: 8 requests take 3.3 us with 256 and 4.1 with 1,024,
+// latency, a chain of three loads and the sums' barriers: 3.7 us for 8 requests
+// and 8.7 us for 1,024 with 65,536 new tokens. Up to 256 requests a CTA has 256
+// threads, above that 1,024: 8 requests took 3.3 us with 256 and 4.1 with 1,024,
 // 512 take 5.5 and 4.8, 4,096 take 21 and 12. Lengths and the count may alias the
 // inputs: the CTA that was last to read the inputs writes them, at its end; the
 // others have counted themselves right after reading.
@@ -516,13 +516,17 @@ constexpr int kRowWarps = 4;
 // the bounds cost no second pass and no exchange between CTAs. Heads are the
 // fast index of the grid: CTAs that run together read neighbouring rows. The
 // first rows are loaded beside the slots, before the run is known.
-// Bound: for long maps the instructions (59 % of the issue slots, the half-rate
-// integer pipe above all, at 24 warps an SM: 32,768 bf16 rows x 8 heads of 128 in
-// blocks of 64 take 70.5 us, 58.4 of them without bounds; their 204 MB would
-// take 31 at the copy rate); for short ones the chain of dependent loads (256
-// decode rows: 5.9 us, 3.2 without bounds). CTAs of four warps: six an SM (80
-// registers); five, seven and eight took 93, 89 and 93 us when six took 82.
-// CTAs of one: 20 an SM, 256 decode rows 5.9 us, with 24 7.0.
+// Bound: latency. For long maps no resource is full: 59 % of the issue slots,
+// 24 % of the DRAM rate, a third of the warps at 24 an SM, so too little is under
+// way (32,768 bf16 rows x 8 heads of 128 in blocks of 64 take 70.9 us, 58.5
+// without bounds; their 204 MB would take 31 at the copy rate). For short ones it
+// is the chain of dependent loads (256 decode rows in a pool of 512 blocks of 16:
+// 6.2 us, 3.4 without bounds). A refused prompt's slots of -1 are looked through
+// 32 at a time behind a run and 128 in front of one, a load after the other:
+// 30,000 of them between prompts of 1,990 tokens cost 235 us (8,000: 56 to 58).
+// CTAs of four warps: six an SM (80 registers, 52 to 104 bytes spilled); five,
+// seven and eight took 93, 89 and 93 us when six took 82. CTAs of one: 20 an SM
+// (4 to 32 bytes spilled), 256 decode rows 5.9 us when 24 took 7.0.
 template <class T, int LPR, int W>
 __global__ void __launch_bounds__(32 * W, LPR ? (W == 1 ? 20 : 24 / W) : 1) write_kernel(const RowsParams p) {
     using R = Rows<LPR>;
@@ -868,7 +872,7 @@ cudaError_t launch_rows(RowsParams& p, bool write, cudaStream_t st) {
     if (write) {
         // One warp a CTA, or four that share a run. In us, bf16 rows of 8 heads x 128, one warp | four, for
         // rows that each lie in a block of their own (decode: a run of one and the block's earlier tokens)
-        // and for whole blocks (prompt):
+        // and for whole blocks (prompt), anywhere in a pool of 131,072 tokens:
         //   block_size   decode 256  decode 1,000   prompt 250   prompt 5,000  prompt 20,000
         //       16         7.6 | 17     21 | 56      6.3 |  7.2     13 | 22       38 | 62
         //       32         9.1 | 18     25 | 62      9.1 |  7.9     18 | 17       35 | 44
@@ -937,8 +941,8 @@ cudaError_t rows_call(RowsParams& p, const void* a, const void* b, bool write, c
 
 // Scores for head dims other than 64, 128 and 256 and groups of more than 64
 // heads: a warp a CTA, query codes in shared memory, as many heads at a time as
-// 48 KB hold (95 of 512 dims). Bound: instructions; 16 x 512 blocks x 8 heads of
-// 128 take 97 us, by tensor cores 12.
+// 48 KB hold (95 of 512 dims). Bound: instructions; 16 x 512 blocks x 8 KV heads in
+// groups of 4 take 97 us at head_dim 96 and 94 at 128, by tensor cores 12.
 __global__ void __launch_bounds__(32) score_any_kernel(const SelectParams p, int heads) {
     extern __shared__ int8_t any_smem[];  // [heads][D] codes, padded to 4, then [heads] scales
     const kvd_block_select_desc& d = p.d;
@@ -1005,10 +1009,10 @@ __global__ void __launch_bounds__(32) score_any_kernel(const SelectParams p, int
 // again from L2. 256 threads where the table has up to 4,096 blocks a row, above
 // that 1,024. Bound: latency, three loads in a row and seven barriers, and for
 // many rows the instructions (57 % of the issue slots, four CTAs an SM).
-// With the scores, 64 requests x 8 heads x 4,096 blocks take 83 us, about 13 of
-// them here: 92 when rows are read again, 87 by radix passes alone, 93 with 1,024
-// threads a row. One request of 256 blocks a head takes 7.5 us (9.0 with 1,024
-// threads), of 4,096 blocks 11.4 (11.1), of 8,192 15.6 (29 with 256).
+// With the scores, 64 requests x 8 heads x up to 4,096 blocks take 89.4 us, 11 of
+// them here: 100 when rows are read again, 93 by radix passes alone, 97 with 1,024
+// threads a row. One request of 256 blocks a head takes 7.7 us (9.0 with 1,024
+// threads), of 4,096 blocks 11.4 (11.0), of 8,192 15.4 (37 with 256).
 constexpr int kPickEach = 16;  // keys a thread holds
 
 template <int THREADS>

@@ -1359,7 +1359,10 @@ GqaPlan plan_gqa(const kvd_decode_desc& d, size_t ws_limit, bool sel = false) {
         span_tiles = 16;
         while (span_tiles > 1 && units * ((s_tiles + span_tiles - 1) / span_tiles) < 4 * grid) span_tiles /= 2;
         if (span_tiles > s_tiles) span_tiles = s_tiles;
-    } else {  // selections are as long as their budget, but for their last block
+    } else {
+        // Selections are taken to be as long as their budget, as those of long requests are, but for the last
+        // block. A few long rows among short ones are not split for it: 256 requests x 8 KV heads, groups of 8,
+        // blocks of 16, four with 2,048 tokens and the others with 64, take 61 us, the four alone 14.
         kvd_decode_desc rows = d;
         if (sel) {
             int sub, per, form;

@@ -10,7 +10,7 @@
 // copies, neighbouring lanes on neighbouring pieces of a row, put them into the
 // swizzled operand layout; a thread per block then turns its NQ sums into a
 // score. Bound: HBM, 2D + 4 bytes a block and head: 64 requests x 8 heads x up
-// to 4,096 blocks of 128 dims, 410 MB in rows of 256 bytes, take 76 us, 5.4 TB/s
+// to 4,096 blocks of 128 dims, 410 MB in rows of 256 bytes, take 78 us, 5.2 TB/s
 // (rows so scattered are read at 6.2 to 6.4 TB/s by a kernel that does nothing
 // else). Warp-level int8 products, m16n8k32, took 350 instructions per 16 blocks
 // and 101 us, TMA gathers of four rows 164 us; four loading warps instead of

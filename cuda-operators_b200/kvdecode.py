@@ -323,7 +323,7 @@ _cuda = None
 
 
 def _cuda_state():
-    """(current stream's handle of a device, current device), looked up once: the public forms take longer than a check."""
+    """(current stream's handle of a device, current device), looked up once: the public forms take longer."""
     global _cuda
     if _cuda is None:
         torch = _types()[0]
@@ -748,8 +748,8 @@ def paged_plan(seq_lens, new_lens, block_table, free_blocks, free_count, block_s
     NB, T = free_blocks.numel(), slot_map.numel()
     rows, one = (B,), (1,)
     _want(device, i32, (seq_lens, rows, "seq_lens"), (new_lens, rows, "new_lens"), (free_blocks, (NB,), "free_blocks"),
-          (free_count, one, "free_count"), (token_starts, (B + 1,), "token_starts"), (seq_lens_out, rows, "seq_lens_out"),
-          (free_count_out, one, "free_count_out"))
+          (free_count, one, "free_count"), (token_starts, (B + 1,), "token_starts"),
+          (seq_lens_out, rows, "seq_lens_out"), (free_count_out, one, "free_count_out"))
     _want(device, i64, (slot_map, (T,), "slot_map"))
     _own_scratch(device, workspace)
     handle = _handle(device, stream)

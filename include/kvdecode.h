@@ -33,11 +33,10 @@
  * kvd_paged_write_launch, kvd_paged_read_launch, kvd_block_select_launch,
  * kvd_sparse_decode_launch; the generic decode kernel aside): they are launched
  * with the attribute, wait before any global memory access, and let the next
- * kernel launch from then on. A
- * caller's kernel that follows one of these calls with the attribute must wait
- * before it reads what the call writes (tables, slots, lengths, codes, scales,
- * bounds, rows, selections, output) and before it overwrites what the call
- * reads.
+ * kernel launch from then on. A caller's kernel that follows one of these calls
+ * with the attribute must wait before it reads what the call writes (tables,
+ * slots, lengths, codes, scales, bounds, rows, selections, output) and before it
+ * overwrites what the call reads.
  */
 #ifndef KVDECODE_H
 #define KVDECODE_H

@@ -4,7 +4,7 @@ import ctypes
 import pytest
 
 import kvdecode as kvd
-from test_blocks import DEV, _check_select, _same_plan, plan_inputs, plan_oracle, select_inputs
+from test_blocks import DEV, EINVAL, _check_select, _same_plan, plan_inputs, plan_oracle, select_inputs
 
 
 class _NoLaunch:
@@ -97,9 +97,9 @@ def test_workspaces_off_their_boundary_are_refused():
                            max_blocks_per_seq=8, seq_lens=256, block_table=256, block_table_stride=8, o_stride_h=128)
     select = kvd.BlockSelectDesc(2, 8, 2, 64, 16, 40, 20, 8, 1, 2, 0, 256, 256, 20, 512, 64)
     for at in (257, 258, 259):
-        assert L.kvd_paged_plan_launch(ctypes.byref(plan), *[256] * 9, at, 64, None) == kvd.CUDA_ERROR_INVALID_VALUE
-        assert L.kvd_sparse_decode_launch(ctypes.byref(sparse), *[256] * 6, at, 1 << 20, None) == kvd.CUDA_ERROR_INVALID_VALUE
-        assert L.kvd_block_select_launch(ctypes.byref(select), *[256] * 5, at, 1 << 20, None) == kvd.CUDA_ERROR_INVALID_VALUE
+        assert L.kvd_paged_plan_launch(ctypes.byref(plan), *[256] * 9, at, 64, None) == EINVAL
+        assert L.kvd_sparse_decode_launch(ctypes.byref(sparse), *[256] * 6, at, 1 << 20, None) == EINVAL
+        assert L.kvd_block_select_launch(ctypes.byref(select), *[256] * 5, at, 1 << 20, None) == EINVAL
 
 
 def test_selections_past_two_to_the_30_blocks_are_refused():
@@ -110,7 +110,7 @@ def test_selections_past_two_to_the_30_blocks_are_refused():
     def size(blocks, budget):
         d = kvd.BlockSelectDesc(1, 1, 1, 64, 1, 40, blocks, budget, 1, 2, 0, 256, 256, blocks, 64, 64)
         if blocks > 1 << 30 or budget > 1 << 30:
-            assert L.kvd_block_select_launch(ctypes.byref(d), *[256] * 6, 1 << 62, None) == kvd.CUDA_ERROR_INVALID_VALUE
+            assert L.kvd_block_select_launch(ctypes.byref(d), *[256] * 6, 1 << 62, None) == EINVAL
         return L.kvd_block_select_workspace_size(ctypes.byref(d))
 
     assert size(1 << 30, 8) == 4 << 30
