@@ -168,3 +168,78 @@ def test_write_several_runs_a_cta(T, H, D, bs, requests, dtype, layout):
 def test_plan_of_the_largest_batches(B, num_slots):
     args = plan_inputs(B, B, 16, 9, B, B // 9, B // 5, 40)
     _same_plan(_run_plan(*args, 16, num_slots), plan_oracle(*args, 16, num_slots))
+
+
+def _high_and_low(NB, n, seed):
+    """n block ids, the first and the last ones of the pool among them, in random order."""
+    rng = np.random.default_rng(seed)
+    ids = np.concatenate([np.arange(n // 2), NB - 1 - np.arange(n - n // 2)])
+    return rng.permutation(ids)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("layout", ["bhtd", "bthd"])
+@pytest.mark.parametrize("NB,H,bs,D", [(70000, 8, 64, 128), (140000, 8, 64, 64), (2200000, 8, 1, 128), (90000, 8, 80, 80)])
+def test_pools_past_32_bits(NB, H, bs, D, layout):
+    """Pools, or bounds, of more than 2^32 bytes: rows written, read, scored and attended to in their first and last
+    blocks are, bit for bit, those of a small pool that holds the same blocks."""
+    import torch
+
+    n, B, G, k = 40, 2, 4, 9
+    g = torch.Generator(device=DEV).manual_seed(1)
+    ids = torch.from_numpy(_high_and_low(NB, n, NB)).to(DEV)
+    shape = lambda blocks: (blocks, H, bs, D) if layout == "bhtd" else (blocks, bs, H, D)  # noqa: E731
+
+    def made(blocks):
+        K, V = (torch.zeros(shape(blocks), dtype=torch.int8, device=DEV) for _ in range(2))
+        ks, vs = (torch.zeros((blocks, H, bs), device=DEV) for _ in range(2))
+        return [K, V, ks, vs], [torch.zeros((blocks, H, 2, D), dtype=torch.int8, device=DEV),
+                                torch.zeros((blocks, H), device=DEV)]
+
+    big, small = made(NB), made(n)
+    assert max(t.nbytes for t in (*big[0], *big[1])) > 1 << 32
+    T = n * bs - bs // 3
+    k_new, v_new = (torch.randn((T, H, D), device=DEV, generator=g).to(torch.bfloat16) for _ in range(2))
+    q = torch.randn((B, H * G, D), device=DEV, generator=g)
+    lens = torch.tensor([n // 2 * bs, T - n // 2 * bs], dtype=torch.int32, device=DEV)
+    got = []
+    for (pool, bound), blocks in ((big, ids), (small, torch.arange(n, device=DEV))):
+        slots = (blocks[:, None] * bs + torch.arange(bs, device=DEV)).reshape(-1)[:T].contiguous()
+        kvd.paged_write(k_new, v_new, slots, *pool, *bound, layout=layout)
+        rows = kvd.paged_read(slots, *pool, layout=layout)
+        table = blocks.view(B, n // B).to(torch.int32)
+        sel, sl = kvd.block_select(q, *bound, table, lens, bs, k)
+        out = kvd.sparse_decode(q, *pool, sel, sl, layout=layout)
+        got.append([*rows, out, sl] + [t[blocks] for t in (*pool, *bound)] + [sel])
+    for a, b in zip(got[0][:-1], got[1][:-1]):
+        assert torch.equal(a, b)
+    assert torch.equal(got[0][-1], ids[got[1][-1].long()].to(torch.int32))
+    assert got[0][0].abs().max() > 1 and kvd.device_status() == 0
+
+
+@pytest.mark.gpu
+def test_slots_past_32_bits():
+    """More than 2^31 slots: blocks of a slot are found by 64-bit division; rows of 4 values in the last blocks."""
+    import torch
+
+    bs, D, n = 64, 4, 30
+    NB = (1 << 25) + 100
+    K, V = (torch.zeros((NB, 1, bs, D), dtype=torch.int8, device=DEV) for _ in range(2))
+    ks, vs = (torch.zeros((NB, 1, bs), device=DEV) for _ in range(2))
+    ids = torch.from_numpy(_high_and_low(NB, n, 3)).to(DEV)
+    slots = (ids[:, None] * bs + torch.arange(bs, device=DEV)).reshape(-1)[: n * bs - 5].contiguous()
+    assert int(slots.max()) >= 1 << 31
+    slots[100:120] = -1
+    slots[500] = NB * bs
+    x, y = (torch.randn((len(slots), 1, D), device=DEV) for _ in range(2))
+    kvd.paged_write(x, y, slots, K, V, ks, vs)
+    ok = ((slots >= 0) & (slots < NB * bs)).cpu().numpy()
+    at = slots[torch.from_numpy(ok).to(DEV)]
+    for rows, pool, scales in ((x, K, ks), (y, V, vs)):
+        codes, sc = po.quantize_rows(rows.cpu().numpy()[ok])
+        assert np.array_equal(pool[at // bs, 0, at % bs].cpu().numpy(), codes[:, 0])
+        assert np.array_equal(scales[at // bs, 0, at % bs].cpu().numpy(), sc[:, 0])
+    got, _ = kvd.paged_read(slots, K, V, ks, vs)
+    codes, sc = po.quantize_rows(x.cpu().numpy())
+    assert np.array_equal(got.cpu().numpy(), np.where(ok[:, None, None], codes.astype(np.float32) * sc[..., None], np.float32(0)))
+    assert kvd.device_status() == kvd.KVD_STATUS_BAD_BLOCK
