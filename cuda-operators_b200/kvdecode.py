@@ -196,6 +196,57 @@ class BlockSelectDesc(ctypes.Structure):
     ]
 
 
+class PagedPrefillDesc(ctypes.Structure):
+    """Mirror of ``kvd_paged_prefill_desc``."""
+
+    _fields_ = [
+        ("batch", c_int32),
+        ("num_q_heads", c_int32),
+        ("num_kv_heads", c_int32),
+        ("head_dim", c_int32),
+        ("num_rows", c_int32),
+        ("block_size", c_int32),
+        ("num_blocks", c_int32),
+        ("max_blocks_per_seq", c_int32),
+        ("causal", c_int32),
+        ("flags", c_uint32),
+        ("seq_lens", c_void_p),
+        ("row_starts", c_void_p),
+        ("block_table", c_void_p),
+        ("block_table_stride", c_int64),
+        ("kv_stride_block", c_int64),
+        ("kv_stride_h", c_int64),
+        ("kv_stride_t", c_int64),
+        ("sc_stride_block", c_int64),
+        ("sc_stride_h", c_int64),
+        ("q_stride_t", c_int64),
+        ("q_stride_h", c_int64),
+        ("o_stride_t", c_int64),
+        ("o_stride_h", c_int64),
+        ("softmax_scale", c_float),
+    ]
+
+
+class PagesDesc(ctypes.Structure):
+    """Mirror of ``kvd_pages_desc``."""
+
+    _fields_ = [
+        ("batch", c_int32),
+        ("num_kv_heads", c_int32),
+        ("head_dim", c_int32),
+        ("block_size", c_int32),
+        ("num_blocks", c_int32),
+        ("max_blocks_per_seq", c_int32),
+        ("block_table_stride", c_int64),
+        ("block_table_out_stride", c_int64),
+        ("kv_stride_block", c_int64),
+        ("kv_stride_h", c_int64),
+        ("kv_stride_t", c_int64),
+        ("sc_stride_block", c_int64),
+        ("sc_stride_h", c_int64),
+    ]
+
+
 _SIGNATURES = {
     "solve": (None, [c_void_p] * 6 + [c_int] * 3),
     "kv_int8_split_launch": (c_int, [c_void_p] * 6 + [c_int] * 3 + [c_void_p, c_void_p]),
@@ -239,6 +290,12 @@ _SIGNATURES = {
     "kvd_block_select_launch": (c_int, [ctypes.POINTER(BlockSelectDesc)] + [c_void_p] * 6 + [c_size_t, c_void_p]),
     "kvd_sparse_workspace_size": (c_size_t, [ctypes.POINTER(PagedDesc)]),
     "kvd_sparse_decode_launch": (c_int, [ctypes.POINTER(PagedDesc)] + [c_void_p] * 7 + [c_size_t, c_void_p]),
+    "kvd_paged_prefill_workspace_size": (c_size_t, [ctypes.POINTER(PagedPrefillDesc)]),
+    "kvd_paged_prefill_launch": (c_int, [ctypes.POINTER(PagedPrefillDesc)] + [c_void_p] * 7 + [c_size_t, c_void_p]),
+    "kvd_paged_fork_workspace_size": (c_size_t, [ctypes.POINTER(PagesDesc)]),
+    "kvd_paged_fork_launch": (c_int, [ctypes.POINTER(PagesDesc)] + [c_void_p] * 15 + [c_size_t, c_void_p]),
+    "kvd_paged_compact_workspace_size": (c_size_t, [ctypes.POINTER(PagesDesc)]),
+    "kvd_paged_compact_launch": (c_int, [ctypes.POINTER(PagesDesc)] + [c_void_p] * 14 + [c_size_t, c_void_p]),
 }
 
 NOALLOC_SCRATCH_BYTES = 512 * 1024
@@ -918,6 +975,170 @@ def sparse_decode(q, k_pool, v_pool, ks_pool, vs_pool, sel_table, sel_lens, out=
     if rc:
         _check(rc, "kvd_sparse_decode_launch")
     return out
+
+
+def _prefill_desc(q, k_pool, block_table, layout: str, causal: bool = True):
+    """Descriptor of the sizes alone, for the workspace."""
+    T, Hq, D = q.shape
+    NB, H, bs = (k_pool.shape[i] for i in ((0, 1, 2) if layout == "bhtd" else (0, 2, 1)))
+    B, MB = block_table.shape
+    p = block_table.data_ptr() or 16
+    desc = PagedPrefillDesc(B, Hq, H, D, T, bs, NB, MB, int(causal), _row_flags(q.dtype), p, p, p, MB)
+    return desc
+
+
+def paged_prefill_workspace_size(q, k_pool, block_table, layout: str = "bhtd") -> int:
+    """Bytes of scratch :func:`paged_prefill` uses for these shapes."""
+    return int(lib().kvd_paged_prefill_workspace_size(ctypes.byref(_prefill_desc(q, k_pool, block_table, layout))))
+
+
+def paged_prefill(q, k_pool, v_pool, ks_pool, vs_pool, block_table, seq_lens, token_starts, out=None, layout: str = "bhtd",
+                  causal: bool = True, softmax_scale: float = 0.0, workspace=None, stream=None, out_dtype=None):
+    """Attention of the new tokens of every request over a paged INT8 cache (``kvd_paged_prefill_launch``).
+
+    ``q`` [T, Hq, D] (float32, bfloat16 or float16) holds the requests' rows one after the other, request b's from
+    ``token_starts``[b] to ``token_starts``[b + 1] (int32 [B + 1], :func:`paged_plan`'s), any number of them, single
+    tokens among them. They are the last of its ``seq_lens``[b] tokens, whose K/V rows the cache holds already; each
+    attends to the tokens up to its own, or with ``causal=False`` to all of them (an encoder's states). Returns ``out``
+    [T, Hq, D]; rows that belong to no request are left as they are."""
+    torch, _, i32, _, _ = _torch or _types()
+    T, Hq, D = q.shape
+    device = q.get_device()
+    NB, H, bs, Dk, s_blk, s_h, s_t, sc_blk, sc_h = _pools(device, k_pool, v_pool, ks_pool, vs_pool, layout)
+    if Dk != D or Hq % H:
+        raise ValueError(f"shape mismatch q{tuple(q.shape)} k_pool{tuple(k_pool.shape)}")
+    B = seq_lens.shape[0]
+    MB = _table(device, block_table, B, i32)
+    _want(device, i32, (seq_lens, (B,), "seq_lens"), (token_starts, (B + 1,), "token_starts"))
+    if out is not None:
+        if out.shape != (T, Hq, D):
+            raise ValueError(f"out must be [{T}, {Hq}, {D}], got {tuple(out.shape)}")
+        if out.get_device() != device:
+            raise _elsewhere(out)
+        if out_dtype is not None and out.dtype is not out_dtype:
+            raise ValueError(f"an output of {out.dtype} is given, {out_dtype} is asked for")
+    _own_scratch(device, workspace)
+    handle = _handle(device, stream)
+    if out is None:
+        out = _out((T, Hq, D), out_dtype, q, stream)
+    q_t, q_h, q_d = q.stride()
+    o_t, o_h, o_d = out.stride()
+    if q_d != 1 or o_d != 1:
+        raise ValueError("dims must be contiguous")
+    flags = _row_flags(q.dtype) | _row_flags(out.dtype) << 2  # KVD_FLAG_OUT_* lie two bits above KVD_FLAG_Q_*
+    desc = PagedPrefillDesc(B, Hq, H, D, T, bs, NB, MB, 1 if causal else 0, flags, seq_lens.data_ptr(),
+                            token_starts.data_ptr(), block_table.data_ptr(), block_table.stride(0), s_blk, s_h, s_t,
+                            sc_blk, sc_h, q_t, q_h, o_t, o_h, softmax_scale)
+    if workspace is None:
+        workspace = _scratch(int(lib().kvd_paged_prefill_workspace_size(ctypes.byref(desc))), q, stream)
+    rc = (_lib or lib()).kvd_paged_prefill_launch(
+        ctypes.byref(desc), q.data_ptr(), k_pool.data_ptr(), v_pool.data_ptr(), ks_pool.data_ptr(), vs_pool.data_ptr(),
+        out.data_ptr(), workspace.data_ptr(), workspace.nbytes, handle)
+    if rc:
+        _check(rc, "kvd_paged_prefill_launch")
+    return out
+
+
+def _pages_desc(device: int, seq_lens, block_table, block_table_out, free_blocks, free_count, k_pool, v_pool, ks_pool,
+                vs_pool, bounds, bound_scale, layout: str, i32, i8, f32):
+    """Checked descriptor of a call on whole blocks."""
+    NB, H, bs, D, s_blk, s_h, s_t, sc_blk, sc_h = _pools(device, k_pool, v_pool, ks_pool, vs_pool, layout)
+    B = seq_lens.shape[0]
+    MB = _table(device, block_table, B, i32)
+    if block_table_out is not block_table and _table(device, block_table_out, B, i32) != MB:
+        raise ValueError(f"block_table_out must be [{B}, {MB}], got {tuple(block_table_out.shape)}")
+    if (bounds is None) != (bound_scale is None):
+        raise ValueError("bounds and bound_scale come together")
+    _want(device, i32, (seq_lens, (B,), "seq_lens"), (free_blocks, (NB,), "free_blocks"), (free_count, (1,), "free_count"))
+    _want(device, i8, (bounds, (NB, H, 2, D), "bounds"))
+    _want(device, f32, (bound_scale, (NB, H), "bound_scale"))
+    return PagesDesc(B, H, D, bs, NB, MB, block_table.stride(0), block_table_out.stride(0), s_blk, s_h, s_t, sc_blk, sc_h)
+
+
+def _pages_size(name: str, block_table, free_blocks) -> int:
+    B, MB = block_table.shape
+    desc = PagesDesc(B, 1, 1, 1, free_blocks.numel(), MB, MB, MB)
+    return int(getattr(lib(), name)(ctypes.byref(desc)))
+
+
+def paged_fork_workspace_size(block_table, free_blocks) -> int:
+    """Bytes of zeroed scratch that :func:`paged_fork` keeps between calls for these shapes."""
+    return _pages_size("kvd_paged_fork_workspace_size", block_table, free_blocks)
+
+
+def paged_compact_workspace_size(block_table, free_blocks) -> int:
+    """Bytes of zeroed scratch that :func:`paged_compact` keeps between calls for these shapes."""
+    return _pages_size("kvd_paged_compact_workspace_size", block_table, free_blocks)
+
+
+def paged_fork(parents, seq_lens, block_table, free_blocks, free_count, k_pool, v_pool, ks_pool, vs_pool, bounds=None,
+               bound_scale=None, layout: str = "bhtd", seq_lens_out=None, block_table_out=None, free_count_out=None,
+               workspace=None, stream=None):
+    """Rows of the block table become copies of other rows (``kvd_paged_fork_launch``): row b continues row
+    ``parents``[b] (int32 [B]; b itself: it goes on as it is; -1: it ends). Full blocks are shared, partly filled last ones are copied
+    into blocks from the free list, and blocks that no row names any more go back on it. Lengths, table and count
+    are updated in place unless other tensors are given for them. Requests that may share blocks are ended here, not
+    by :func:`paged_plan`. ``workspace``: a zeroed uint8 tensor of :func:`paged_fork_workspace_size` bytes that a
+    caller keeps (without one, one is made). Returns (block_table_out, seq_lens_out)."""
+    torch, i8, i32, _, f32 = _torch or _types()
+    device = seq_lens.get_device()
+    if block_table_out is None:
+        block_table_out = block_table
+    desc = _pages_desc(device, seq_lens, block_table, block_table_out, free_blocks, free_count, k_pool, v_pool, ks_pool,
+                       vs_pool, bounds, bound_scale, layout, i32, i8, f32)
+    rows = (desc.batch,)
+    _want(device, i32, (parents, rows, "parents"), (seq_lens_out, rows, "seq_lens_out"),
+          (free_count_out, (1,), "free_count_out"))
+    _own_scratch(device, workspace)
+    handle = _handle(device, stream)
+    if seq_lens_out is None:
+        seq_lens_out = seq_lens
+    if free_count_out is None:
+        free_count_out = free_count
+    if workspace is None:  # zeroed on the call's stream
+        n = int(lib().kvd_paged_fork_workspace_size(ctypes.byref(desc)))
+        workspace = _made(torch.zeros, n or 1, torch.uint8, seq_lens, stream)
+    rc = (_lib or lib()).kvd_paged_fork_launch(
+        ctypes.byref(desc), parents.data_ptr(), seq_lens.data_ptr(), block_table.data_ptr(), free_blocks.data_ptr(),
+        free_count.data_ptr(), k_pool.data_ptr(), v_pool.data_ptr(), ks_pool.data_ptr(), vs_pool.data_ptr(), _ptr(bounds),
+        _ptr(bound_scale), seq_lens_out.data_ptr(), block_table_out.data_ptr(), free_count_out.data_ptr(),
+        workspace.data_ptr(), workspace.nbytes, handle)
+    if rc:
+        _check(rc, "kvd_paged_fork_launch")
+    return block_table_out, seq_lens_out
+
+
+def paged_compact(seq_lens, block_table, free_blocks, free_count, k_pool, v_pool, ks_pool, vs_pool, bounds=None,
+                  bound_scale=None, layout: str = "bhtd", block_table_out=None, free_blocks_out=None, used=None,
+                  workspace=None, stream=None):
+    """Moves the blocks that the table names to the lowest ids among those and the free ones
+    (``kvd_paged_compact_launch``). Table and free list are updated in place unless other tensors are given for
+    them, ``free_count`` always is. ``workspace``: a zeroed uint8 tensor of :func:`paged_compact_workspace_size`
+    bytes that a caller keeps. Returns ``used`` int32 [1]: the blocks that the pools then need."""
+    torch, i8, i32, _, f32 = _torch or _types()
+    device = seq_lens.get_device()
+    if block_table_out is None:
+        block_table_out = block_table
+    if free_blocks_out is None:
+        free_blocks_out = free_blocks
+    desc = _pages_desc(device, seq_lens, block_table, block_table_out, free_blocks, free_count, k_pool, v_pool, ks_pool,
+                       vs_pool, bounds, bound_scale, layout, i32, i8, f32)
+    _want(device, i32, (free_blocks_out, (desc.num_blocks,), "free_blocks_out"), (used, (1,), "used"))
+    _own_scratch(device, workspace)
+    handle = _handle(device, stream)
+    if used is None:
+        used = _out((1,), i32, seq_lens, stream)
+    if workspace is None:  # zeroed on the call's stream
+        n = int(lib().kvd_paged_compact_workspace_size(ctypes.byref(desc)))
+        workspace = _made(torch.zeros, n or 1, torch.uint8, seq_lens, stream)
+    rc = (_lib or lib()).kvd_paged_compact_launch(
+        ctypes.byref(desc), seq_lens.data_ptr(), block_table.data_ptr(), free_blocks.data_ptr(), free_count.data_ptr(),
+        k_pool.data_ptr(), v_pool.data_ptr(), ks_pool.data_ptr(), vs_pool.data_ptr(), _ptr(bounds), _ptr(bound_scale),
+        block_table_out.data_ptr(), free_blocks_out.data_ptr(), used.data_ptr(), workspace.data_ptr(), workspace.nbytes,
+        handle)
+    if rc:
+        _check(rc, "kvd_paged_compact_launch")
+    return used
 
 
 # ------------------------------------------------------------------ multi-GPU

@@ -351,6 +351,102 @@ cudaError_t kvd_sparse_decode_launch(const kvd_paged_desc* desc,
                                      const float* k_scale_pool, const float* v_scale_pool, void* out,
                                      void* workspace, size_t workspace_bytes, cudaStream_t stream);
 
+/* Attention of a chunk of new tokens of every request over a paged cache: the
+ * tokens' K/V rows are in the cache already (kvd_paged_write_launch). The rows
+ * of all requests are packed: rows [row_starts[b], row_starts[b + 1]) of Q
+ * [num_rows][num_q_heads][head_dim] are request b's, any number of them, in
+ * ascending order (kvd_paged_plan_launch's token_starts). With causal != 0 they
+ * are the last of its seq_lens[b] tokens: of n rows, row i attends to tokens
+ * [0, seq_lens[b] - n + i]. With causal == 0 every row attends to all
+ * seq_lens[b] tokens (states of an encoder that the cache holds).
+ *   out[t][h] = softmax_j((q . K[j]) * ks[j] * scale) . (V[j] * vs[j])
+ * A row that sees no token is written as 0. Rows that belong to no request (in
+ * front of row_starts[0], from row_starts[batch] on) are left as they are;
+ * starts are clamped to [0, num_rows], lengths to the table. A block id
+ * outside the pool counts as in kvd_paged_decode_launch
+ * (KVD_STATUS_BAD_BLOCK). head_dim at most 512. Sums and softmax statistics
+ * are fp32; 16-bit queries enter the products unrounded, 32-bit ones as two
+ * 16-bit terms (22 bits); weights as one 16-bit term (11 bits) where the output
+ * has 16 bits, else as two. head_dim 64 and 128 with pools on 16-byte
+ * boundaries and 16-byte multiples of strides run on tensor cores, any other
+ * shape on CUDA cores. The workspace of kvd_paged_prefill_workspace_size bytes,
+ * on a 16-byte boundary, needs no initialisation; concurrent calls need
+ * separate ones. num_rows 0 does nothing. */
+typedef struct kvd_paged_prefill_desc {
+    int32_t batch, num_q_heads, num_kv_heads, head_dim;
+    int32_t num_rows;            /* rows of Q and out, >= 0 */
+    int32_t block_size, num_blocks, max_blocks_per_seq;
+    int32_t causal;
+    uint32_t flags;              /* KVD_FLAG_Q_*, KVD_FLAG_OUT_* */
+    const int32_t* seq_lens;     /* device [B] */
+    const int32_t* row_starts;   /* device [B + 1] */
+    const int32_t* block_table;  /* device [B][block_table_stride] */
+    int64_t block_table_stride;  /* >= max_blocks_per_seq */
+    int64_t kv_stride_block, kv_stride_h, kv_stride_t;  /* pools as in kvd_paged_desc */
+    int64_t sc_stride_block, sc_stride_h;
+    int64_t q_stride_t, q_stride_h, o_stride_t, o_stride_h;
+    float softmax_scale;         /* <= 0 selects 1/sqrt(D) */
+} kvd_paged_prefill_desc;
+size_t kvd_paged_prefill_workspace_size(const kvd_paged_prefill_desc* desc);
+cudaError_t kvd_paged_prefill_launch(const kvd_paged_prefill_desc* desc, const void* Q, const int8_t* K_pool,
+                                     const int8_t* V_pool, const float* k_scale_pool, const float* v_scale_pool,
+                                     void* out, void* workspace, size_t workspace_bytes, cudaStream_t stream);
+
+/* Rows of a block table that become copies of other rows (samples of a prompt,
+ * beams), and the blocks that nobody holds afterwards back on the free list.
+ * Row b continues row parents[b] (b itself: it goes on as it is); a parent
+ * outside [0, batch) ends row b. Full blocks are shared: several rows name
+ * them. A row's partly filled last block, which the next token is written to,
+ * belongs to one row: it stays with the row itself where that goes on, else
+ * with the lowest row that continues it, and every other one gets a copy of its
+ * tokens (codes, scales, and the key bounds where given) in a block from the
+ * free list. In this order: blocks that only ended rows name are pushed on the
+ * free list (the stack of kvd_paged_plan_launch) by ascending id; then copies
+ * are popped from its top in the order of the rows. A row whose copy finds the
+ * stack empty ends (length 0, KVD_STATUS_NO_BLOCKS). Of a row's table entries
+ * those of its blocks are written, of free_blocks those from free_count on.
+ * seq_lens_out, block_table_out and free_count_out may be seq_lens,
+ * block_table and free_count. Table ids outside the pool are passed on and
+ * never followed (KVD_STATUS_BAD_BLOCK). The table has to name every holder of a
+ * block. kvd_paged_plan_launch gives back all blocks of a request that it ends,
+ * so requests that may share blocks are ended here instead. The workspace of
+ * kvd_paged_fork_workspace_size bytes, on a 4-byte boundary, is zeroed by the
+ * caller once; calls leave its counters zeroed. Concurrent calls need separate ones. At
+ * most 8192 rows, 2^30 blocks and tokens of a row below 2^31, 2^30 codes in a block's head
+ * (cudaErrorInvalidValue above). */
+typedef struct kvd_pages_desc {
+    int32_t batch, num_kv_heads, head_dim;
+    int32_t block_size, num_blocks, max_blocks_per_seq;
+    int64_t block_table_stride, block_table_out_stride;  /* >= max_blocks_per_seq */
+    int64_t kv_stride_block, kv_stride_h, kv_stride_t;   /* pools as in kvd_paged_desc */
+    int64_t sc_stride_block, sc_stride_h;
+} kvd_pages_desc;
+size_t kvd_paged_fork_workspace_size(const kvd_pages_desc* desc);
+cudaError_t kvd_paged_fork_launch(const kvd_pages_desc* desc, const int32_t* parents, const int32_t* seq_lens,
+                                  const int32_t* block_table, int32_t* free_blocks, const int32_t* free_count,
+                                  int8_t* K_pool, int8_t* V_pool, float* k_scale_pool, float* v_scale_pool,
+                                  int8_t* bounds, float* bound_scale, int32_t* seq_lens_out,
+                                  int32_t* block_table_out, int32_t* free_count_out, void* workspace,
+                                  size_t workspace_bytes, cudaStream_t stream);
+
+/* Moves the blocks that the table's rows name to the lowest ids among those
+ * and the free ones, so that pools can shrink: of the blocks in use and the
+ * free ones together, the lowest ids as many as are in use become the ones in
+ * use; the k-th block in use above them moves, whole, to the k-th free one among
+ * them. Blocks that neither the table nor the free list names belong to others
+ * and stay. block_table_out gets the new ids (rows share a block as before),
+ * free_blocks_out the free ones in descending order (the lowest id is the next
+ * one handed out), free_count their number and used[0] the number of blocks that the pools
+ * then need: the highest id in use, plus one. block_table_out and
+ * free_blocks_out may be block_table and free_blocks. Pools, bounds, limits and workspace
+ * (kvd_paged_compact_workspace_size bytes) as for kvd_paged_fork_launch. */
+cudaError_t kvd_paged_compact_launch(const kvd_pages_desc* desc, const int32_t* seq_lens, const int32_t* block_table,
+                                     const int32_t* free_blocks, int32_t* free_count, int8_t* K_pool, int8_t* V_pool,
+                                     float* k_scale_pool, float* v_scale_pool, int8_t* bounds, float* bound_scale,
+                                     int32_t* block_table_out, int32_t* free_blocks_out, int32_t* used,
+                                     void* workspace, size_t workspace_bytes, cudaStream_t stream);
+size_t kvd_paged_compact_workspace_size(const kvd_pages_desc* desc);
+
 /* Log-sum-exp combine of `num_parts` partial-record arrays, each [num_heads]
  * records of KVD_PARTIAL_STRIDE(head_dim) floats, part p starting at
  * parts + p*part_stride. Writes normalised rows out[h*out_stride + d] (fp32,
