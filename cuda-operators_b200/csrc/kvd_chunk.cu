@@ -96,6 +96,214 @@ __global__ void __launch_bounds__(kAnyThreads) chunk_any_kernel(const ChunkParam
     }
 }
 
+// ---------------------------------------------------------------- plan
+// Which kernel takes a request, and how its tokens are split: one CTA sums the
+// work of all requests (tokens times units), which gives the stretch that a
+// unit may have, then places every request's units and records by prefix sums.
+// A stretch is at least work / target, so split units are fewer than 2 target:
+// the room for their records. Bound: latency (loads, two sums, one scan).
+__global__ void __launch_bounds__(1024) chunk_plan_kernel(const ChunkParams p) {
+    __shared__ unsigned long long work[2];
+    __shared__ int sums[4][32];
+    grid_dependency_wait();
+    allow_dependents();
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    if (tid < 2) work[tid] = 0;
+    __syncthreads();
+    auto shape = [&](int b, int& rows, int& units, bool& few) {
+        const ChunkRows r = chunk_rows(p, b);
+        rows = r.n * p.G;
+        few = rows <= p.few_most;
+        units = (few ? (rows + kFewRows - 1) / kFewRows : (rows + p.tile_rows - 1) / p.tile_rows) * p.Hkv;
+        return r.len;
+    };
+    unsigned long long w[2] = {0, 0};
+    for (int b = tid; b < p.B; b += blockDim.x) {
+        int rows, units;
+        bool few;
+        const int len = shape(b, rows, units, few);
+        w[few ? 0 : 1] += static_cast<unsigned long long>(units) * len;
+    }
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) w[i] += __shfl_xor_sync(0xffffffffu, w[i], o);
+        if (lane == 0 && w[i]) atomicAdd(&work[i], w[i]);
+    }
+    __syncthreads();
+    auto span_of = [](unsigned long long x, int target, int least) {
+        const unsigned long long s = (x + target - 1) / target;
+        return static_cast<int>(min(max(s, static_cast<unsigned long long>(least)), 0x40000000ull));
+    };
+    const int few_span = span_of(work[0], p.few_target, kFewMinSpan), tile_span = span_of(work[1], p.tile_target, kTileMinSpan);
+    int carry[4] = {0, 0, 0, 0};
+    for (int b0 = 0; b0 < p.B; b0 += blockDim.x) {
+        const int b = b0 + tid;
+        int x[4] = {0, 0, 0, 0};
+        if (b < p.B) {
+            int rows, units, each;
+            bool few;
+            const int len = shape(b, rows, units, few);
+            const int n = few ? chunk_splits(len, few_span, kFewStep, each) : chunk_splits(len, tile_span, kTile, each);
+            x[few ? 0 : 2] = units * n;
+            x[few ? 1 : 3] = n > 1 ? units * n : 0;
+        }
+        int inc[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            inc[i] = x[i];
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const int y = __shfl_up_sync(0xffffffffu, inc[i], o);
+                if (lane >= o) inc[i] += y;
+            }
+        }
+        __syncthreads();
+        if (lane == 31)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) sums[i][warp] = inc[i];
+        __syncthreads();
+        int32_t* const first[4] = {p.few_first, p.few_rec, p.tile_first, p.tile_rec};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            int s = sums[i][lane];
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const int y = __shfl_up_sync(0xffffffffu, s, o);
+                if (lane >= o) s += y;
+            }
+            const int upto = __shfl_sync(0xffffffffu, s, (warp - 1) & 31), all = __shfl_sync(0xffffffffu, s, 31);
+            if (b < p.B) first[i][b] = carry[i] + (warp > 0 ? upto : 0) + inc[i] - x[i];
+            carry[i] += all;
+        }
+    }
+    if (tid == 0) {
+        p.few_first[p.B] = carry[0];
+        p.few_rec[p.B] = carry[1];
+        p.tile_first[p.B] = carry[2];
+        p.tile_rec[p.B] = carry[3];
+        *p.head = ChunkHead{carry[0], few_span, carry[2], tile_span, carry[1], carry[3], 0, 0};
+    }
+}
+
+// ------------------------------------------------------------- split work
+// Merges the records of units that were split along the tokens: 16 rows a CTA,
+// out = sum_s 2^(m_s - M) o_s / sum_s 2^(m_s - M) l_s.
+template <int D>
+__global__ void __launch_bounds__(128) chunk_merge_kernel(const ChunkParams p) {
+    grid_dependency_wait();
+    allow_dependents();
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int few = p.head->few_recs, groups = p.tile_rows / kFewRows;
+    const int64_t units = few + static_cast<int64_t>(p.head->tile_recs) * groups;
+    for (int64_t u = blockIdx.x; u < units; u += gridDim.x) {
+        const bool is_few = u < few;
+        const int slot = is_few ? static_cast<int>(u) : static_cast<int>((u - few) / groups);
+        const int group = is_few ? 0 : static_cast<int>(u - few - static_cast<int64_t>(slot) * groups);
+        const int32_t* first = is_few ? p.few_rec : p.tile_rec;
+        const int b = warp_find(first, p.B, slot);
+        const ChunkRows R = chunk_rows(p, b);
+        const int unit_rows = is_few ? kFewRows : p.tile_rows;
+        const int rows = R.n * p.G, nrb = (rows + unit_rows - 1) / unit_rows;
+        int each;
+        const int nsplit = is_few ? chunk_splits(R.len, p.head->few_span, kFewStep, each)
+                                  : chunk_splits(R.len, p.head->tile_span, kTile, each);
+        const int local = slot - first[b], item = local / nsplit;
+        if (local != item * nsplit) continue;  // the first record of a unit stands for all
+        const int hk = item / nrb, rb = item - hk * nrb;
+        const float* o = is_few ? p.few_o : p.tile_o;
+        const float2* ml = is_few ? p.few_ml : p.tile_ml;
+        for (int r = group * kFewRows + warp; r < (group + 1) * kFewRows; r += 4) {
+            const int row = rb * unit_rows + r;
+            if (row >= rows) break;
+            const int64_t at = static_cast<int64_t>(slot) * unit_rows + r;
+            float M = -INFINITY;
+            for (int s = lane; s < nsplit; s += 32) M = fmaxf(M, ml[at + static_cast<int64_t>(s) * unit_rows].x);
+#pragma unroll
+            for (int i = 16; i > 0; i >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, i));
+            float L = 0.f, acc[D / 32] = {};
+#pragma unroll 4
+            for (int s = 0; s < nsplit; ++s) {
+                const int64_t rec = at + static_cast<int64_t>(s) * unit_rows;
+                const float2 v = ml[rec];
+                const float f = v.x == -INFINITY ? 0.f : exp2f(v.x - M);
+                L = fmaf(v.y, f, L);
+#pragma unroll
+                for (int d = 0; d < D / 32; ++d) {
+                    const float x = o[rec * D + d * 32 + lane];
+                    if (f != 0.f) acc[d] = fmaf(x, f, acc[d]);
+                }
+            }
+            const int i = static_cast<int>(p.by_g.div(static_cast<uint32_t>(row))), g = row - i * p.G;
+            const int64_t o_at = static_cast<int64_t>(R.t0 + i) * p.o_st + static_cast<int64_t>(hk * p.G + g) * p.o_sh;
+            const float inv = L == 0.f ? 0.f : 1.f / L;  // no token in sight
+#pragma unroll
+            for (int d = 0; d < D / 32; ++d) store_out(p.out, o_at + d * 32 + lane, acc[d] * inv, p.flags);
+        }
+    }
+}
+
+template <class... A, class... B>
+cudaError_t launch_after(void (*kern)(A...), unsigned grid, unsigned block, size_t smem, cudaStream_t st, B... args) {
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(grid, 1, 1);
+    cfg.blockDim = dim3(block, 1, 1);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = st;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, kern, args...);
+}
+
+constexpr int kNever = 0x7fffffff;
+
+bool tensor_shape(const kvd_paged_prefill_desc& d) {
+    return (d.head_dim == 64 || d.head_dim == 128) && d.kv_stride_block >= 0 && d.kv_stride_h >= 0 && d.kv_stride_t >= 0 &&
+           ((d.kv_stride_block | d.kv_stride_h | d.kv_stride_t) & 15) == 0;
+}
+
+int64_t round16(int64_t x) { return (x + 15) & ~static_cast<int64_t>(15); }
+
+// Lays the workspace out from `base` (0: to learn its size); returns the end.
+int64_t lay_out(const kvd_paged_prefill_desc& d, ChunkParams* p, uint8_t* base) {
+    const int sms = device_sm_count();
+    const int64_t G = d.num_q_heads / d.num_kv_heads, D = d.head_dim, entries = static_cast<int64_t>(d.batch) + 1;
+    const int64_t cap = static_cast<int64_t>(d.max_blocks_per_seq) * d.block_size;
+    p->few_target = 2 * sms;
+    p->tile_target = sms;
+    p->tile_rows = kTileRows;
+    p->few_most = kNever;
+    const bool tiles = static_cast<int64_t>(d.num_rows) * G > p->few_most;
+    auto records = [&](int64_t target, int64_t unit_rows, int64_t least) {
+        // no more units than rows give, and no more splits of each than the longest length gives
+        const int64_t units = (d.num_rows * G / unit_rows + (d.batch < d.num_rows ? d.batch : d.num_rows)) * d.num_kv_heads;
+        const int64_t splits = (cap + least - 1) / least;
+        const int64_t most = units * splits;
+        return splits <= 1 ? 0 : most < 2 * target ? most : 2 * target;
+    };
+    p->max_few_recs = static_cast<int>(records(p->few_target, kFewRows, kFewMinSpan));
+    p->max_tile_recs = tiles ? static_cast<int>(records(p->tile_target, p->tile_rows, kTileMinSpan)) : 0;
+    int64_t at = 0;
+    auto take = [&](int64_t bytes) {
+        uint8_t* here = base + at;
+        at += round16(bytes);
+        return here;
+    };
+    p->head = reinterpret_cast<ChunkHead*>(take(sizeof(ChunkHead)));
+    p->few_first = reinterpret_cast<int32_t*>(take(4 * entries));
+    p->few_rec = reinterpret_cast<int32_t*>(take(4 * entries));
+    p->tile_first = reinterpret_cast<int32_t*>(take(4 * entries));
+    p->tile_rec = reinterpret_cast<int32_t*>(take(4 * entries));
+    p->few_o = reinterpret_cast<float*>(take(4 * D * kFewRows * p->max_few_recs));
+    p->few_ml = reinterpret_cast<float2*>(take(8 * kFewRows * static_cast<int64_t>(p->max_few_recs)));
+    p->tile_o = reinterpret_cast<float*>(take(4 * D * p->tile_rows * p->max_tile_recs));
+    p->tile_ml = reinterpret_cast<float2*>(take(8 * p->tile_rows * static_cast<int64_t>(p->max_tile_recs)));
+    return at;
+}
+
 cudaError_t check_chunk(const kvd_paged_prefill_desc* d) {
     if (!d || d->batch < 1 || d->num_q_heads < 1 || d->num_kv_heads < 1 || d->head_dim < 1 || d->head_dim > kAnyMaxD ||
         d->num_q_heads % d->num_kv_heads != 0 || d->num_rows < 0 || d->block_size < 1 || d->num_blocks < 1 ||
@@ -118,7 +326,8 @@ using namespace kvd;
 
 extern "C" size_t kvd_paged_prefill_workspace_size(const kvd_paged_prefill_desc* d) {
     if (check_chunk(d) != cudaSuccess) return 0;
-    return 0;
+    ChunkParams p{};
+    return d->head_dim == 64 || d->head_dim == 128 ? static_cast<size_t>(lay_out(*d, &p, nullptr)) : 0;
 }
 
 extern "C" cudaError_t kvd_paged_prefill_launch(const kvd_paged_prefill_desc* d, const void* Q, const int8_t* K_pool,
@@ -148,8 +357,23 @@ extern "C" cudaError_t kvd_paged_prefill_launch(const kvd_paged_prefill_desc* d,
     p.flags = d->flags;
     p.by_bs = FastDiv(static_cast<uint32_t>(p.bs));
     p.by_g = FastDiv(static_cast<uint32_t>(p.G));
-    chunk_any_kernel<<<static_cast<unsigned>(p.T * p.Hq), kAnyThreads, 0, stream>>>(p);
-    e = cudaGetLastError();
+    const int64_t per16 = (d->flags & (KVD_FLAG_Q_BF16 | KVD_FLAG_Q_F16)) ? 8 : 4;  // elements of a row in 16 bytes
+    p.vec_q = (reinterpret_cast<uintptr_t>(Q) & 15) == 0 && d->q_stride_t % per16 == 0 && d->q_stride_h % per16 == 0;
+    const bool aligned = ((reinterpret_cast<uintptr_t>(K_pool) | reinterpret_cast<uintptr_t>(V_pool)) & 15) == 0;
+    if (!tensor_shape(*d) || !aligned) {
+        e = launch_after(chunk_any_kernel, static_cast<unsigned>(p.T * p.Hq), kAnyThreads, 0, stream, p);
+        if (e == cudaSuccess) ++*launches;
+        return e;
+    }
+    lay_out(*d, &p, static_cast<uint8_t*>(workspace));
+    e = launch_after(chunk_plan_kernel, 1, 1024, 0, stream, p);
+    if (e != cudaSuccess) return e;
+    ++*launches;
+    e = launch_chunk_few(p, stream, launches);
+    if (e != cudaSuccess || p.max_few_recs + p.max_tile_recs == 0) return e;
+    const unsigned grid = 8u * device_sm_count();
+    e = p.D == 128 ? launch_after(chunk_merge_kernel<128>, grid, 128, 0, stream, p)
+                   : launch_after(chunk_merge_kernel<64>, grid, 128, 0, stream, p);
     if (e == cudaSuccess) ++*launches;
     return e;
 }
