@@ -461,6 +461,7 @@ extern "C" cudaError_t kvd_device_status(int32_t* status) {
     if (e != cudaSuccess) return e;
     const int32_t zero = 0;
     e = cudaMemcpyToSymbol(g_status, &zero, sizeof(zero));
+    if (e == cudaSuccess) e = take_chunk_tile_status(&v);
     *status = v;
     return e;
 }

@@ -258,8 +258,6 @@ cudaError_t launch_after(void (*kern)(A...), unsigned grid, unsigned block, size
     return cudaLaunchKernelEx(&cfg, kern, args...);
 }
 
-constexpr int kNever = 0x7fffffff;
-
 bool tensor_shape(const kvd_paged_prefill_desc& d) {
     return (d.head_dim == 64 || d.head_dim == 128) && d.kv_stride_block >= 0 && d.kv_stride_h >= 0 && d.kv_stride_t >= 0 &&
            ((d.kv_stride_block | d.kv_stride_h | d.kv_stride_t) & 15) == 0;
@@ -274,8 +272,9 @@ int64_t lay_out(const kvd_paged_prefill_desc& d, ChunkParams* p, uint8_t* base) 
     const int64_t cap = static_cast<int64_t>(d.max_blocks_per_seq) * d.block_size;
     p->few_target = 2 * sms;
     p->tile_target = sms;
-    p->tile_rows = kTileRows;
-    p->few_most = kNever;
+    constexpr uint32_t q16 = KVD_FLAG_Q_BF16 | KVD_FLAG_Q_F16, o16 = KVD_FLAG_OUT_BF16 | KVD_FLAG_OUT_F16;
+    p->tile_rows = (d.flags & q16) != 0 && (d.flags & o16) != 0 ? 256 : 128;
+    p->few_most = 32;
     const bool tiles = static_cast<int64_t>(d.num_rows) * G > p->few_most;
     auto records = [&](int64_t target, int64_t unit_rows, int64_t least) {
         // no more units than rows give, and no more splits of each than the longest length gives
@@ -286,6 +285,12 @@ int64_t lay_out(const kvd_paged_prefill_desc& d, ChunkParams* p, uint8_t* base) 
     };
     p->max_few_recs = static_cast<int>(records(p->few_target, kFewRows, kFewMinSpan));
     p->max_tile_recs = tiles ? static_cast<int>(records(p->tile_target, p->tile_rows, kTileMinSpan)) : 0;
+    // the size is the same for all types of rows and output
+    int64_t tile_rows = 0;
+    for (int64_t r = 128; tiles && r <= 256; r += 128) {
+        const int64_t x = r * records(p->tile_target, r, kTileMinSpan);
+        tile_rows = x > tile_rows ? x : tile_rows;
+    }
     int64_t at = 0;
     auto take = [&](int64_t bytes) {
         uint8_t* here = base + at;
@@ -299,8 +304,8 @@ int64_t lay_out(const kvd_paged_prefill_desc& d, ChunkParams* p, uint8_t* base) 
     p->tile_rec = reinterpret_cast<int32_t*>(take(4 * entries));
     p->few_o = reinterpret_cast<float*>(take(4 * D * kFewRows * p->max_few_recs));
     p->few_ml = reinterpret_cast<float2*>(take(8 * kFewRows * static_cast<int64_t>(p->max_few_recs)));
-    p->tile_o = reinterpret_cast<float*>(take(4 * D * p->tile_rows * p->max_tile_recs));
-    p->tile_ml = reinterpret_cast<float2*>(take(8 * p->tile_rows * static_cast<int64_t>(p->max_tile_recs)));
+    p->tile_o = reinterpret_cast<float*>(take(4 * D * tile_rows));
+    p->tile_ml = reinterpret_cast<float2*>(take(8 * tile_rows));
     return at;
 }
 
@@ -359,6 +364,8 @@ extern "C" cudaError_t kvd_paged_prefill_launch(const kvd_paged_prefill_desc* d,
     p.by_g = FastDiv(static_cast<uint32_t>(p.G));
     const int64_t per16 = (d->flags & (KVD_FLAG_Q_BF16 | KVD_FLAG_Q_F16)) ? 8 : 4;  // elements of a row in 16 bytes
     p.vec_q = (reinterpret_cast<uintptr_t>(Q) & 15) == 0 && d->q_stride_t % per16 == 0 && d->q_stride_h % per16 == 0;
+    const int64_t per16o = (d->flags & (KVD_FLAG_OUT_BF16 | KVD_FLAG_OUT_F16)) ? 8 : 4;
+    p.vec_out = (reinterpret_cast<uintptr_t>(out) & 15) == 0 && d->o_stride_t % per16o == 0 && d->o_stride_h % per16o == 0;
     const bool aligned = ((reinterpret_cast<uintptr_t>(K_pool) | reinterpret_cast<uintptr_t>(V_pool)) & 15) == 0;
     if (!tensor_shape(*d) || !aligned) {
         e = launch_after(chunk_any_kernel, static_cast<unsigned>(p.T * p.Hq), kAnyThreads, 0, stream, p);
@@ -370,7 +377,12 @@ extern "C" cudaError_t kvd_paged_prefill_launch(const kvd_paged_prefill_desc* d,
     if (e != cudaSuccess) return e;
     ++*launches;
     e = launch_chunk_few(p, stream, launches);
-    if (e != cudaSuccess || p.max_few_recs + p.max_tile_recs == 0) return e;
+    if (e != cudaSuccess) return e;
+    if (static_cast<int64_t>(p.T) * p.G > p.few_most) {  // a request may have many rows
+        e = launch_chunk_tile(p, stream, launches);
+        if (e != cudaSuccess) return e;
+    }
+    if (p.max_few_recs + p.max_tile_recs == 0) return cudaSuccess;
     const unsigned grid = 8u * device_sm_count();
     e = p.D == 128 ? launch_after(chunk_merge_kernel<128>, grid, 128, 0, stream, p)
                    : launch_after(chunk_merge_kernel<64>, grid, 128, 0, stream, p);

@@ -33,7 +33,7 @@ struct ChunkParams {
     float qscale;  // softmax_scale * log2(e)
     uint32_t flags;
     FastDiv by_bs, by_g;
-    int vec_q;  // query rows on 16-byte boundaries
+    int vec_q, vec_out;  // rows on 16-byte boundaries
     // plan
     ChunkHead* head;
     int32_t* few_first;   // [B + 1] units in front of request b's
@@ -51,7 +51,6 @@ struct ChunkParams {
 };
 
 constexpr int kFewRows = 16;     // rows of a unit of the kernel for few rows
-constexpr int kTileRows = 256;   // rows of a unit of the kernel for many rows, 16-bit products
 constexpr int kFewStep = 32;     // tokens of a step of that kernel
 constexpr int kFewMinSpan = 256; // tokens that a split has at least
 constexpr int kTileMinSpan = 512;

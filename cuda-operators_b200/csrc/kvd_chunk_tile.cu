@@ -1,0 +1,807 @@
+// kvd_chunk_tile.cu -- attention of packed new tokens over a paged cache for
+// requests with many rows a KV head, on the tcgen05 tensor cores.
+//
+// A unit is (request, KV head, block of rows, stretch of tokens); rows are the
+// request's tokens times the group's heads, so a tile of the cache is read and
+// widened once for all of them. With u_j = q . K_j (fp32 accumulators of fp16
+// products; q times a power of two per row, codes exact), s_j = u_j ks_j rf in
+// base 2 and p_j = 2^(s_j - m):
+//   l = sum p_j,   O = sum fp16(p_j vs_j 2^e) V_j,   out = O 2^-e / l,
+// with m a running maximum that may trail by 8 and 2^e a power of two that keeps
+// the weights in fp16's range (it falls when larger value scales come).
+//
+// Outputs of 16 bits (TERMS 1): one fp16 term of the queries (exact for 16-bit
+// ones) and of the weights; 256 rows, 128 to each of two softmax warpgroups,
+// share a tile. Outputs of 32 bits or fp32 queries (TERMS 2): two terms of both
+// (22 bits), 128 rows, the warpgroups take tiles in turn with their own m, l
+// and O and are merged at the end. Blocks of at most 128 rows go that way too
+// with one term. So there are always two score tiles in flight: while one
+// warpgroup turns its scores into weights the tensor cores work for the other.
+//
+// One CTA an SM, 16 warps:
+//   0-7   softmax, a row a thread (= TMEM lane): S from tensor memory, weights
+//         back into the columns that S had, from where they are an MMA operand;
+//   8-11  widen INT8 rows, straight from global memory (a tile ahead in
+//         registers), into fp16 tiles in shared memory: 128-byte swizzled rows of
+//         tokens, the K-major operand of q K^T and the MN-major one of P V; and
+//         the unit's queries;
+//   12    issues the MMAs;
+//   13    looks the tile's blocks up ahead: row offsets, scales.
+// Every wait is bounded; on expiry the kernel records KVD_STATUS_WAIT_TIMEOUT
+// and unwinds.
+#include "kvd_chunk.cuh"
+#include "kvd_decode.cuh"
+#include "kvd_tc.cuh"
+
+namespace kvd {
+namespace {
+
+constexpr int kThreads = 512;
+constexpr int kMetaStages = 4;
+
+// What is known of a tile before it is read.
+struct TileMeta {
+    float ks[kTile];
+    float vs[kTile];     // times 2^ve
+    int64_t row[kTile];  // offset of the token's row in the pools, -1: zeros
+    int ve;
+    int pad[15];
+};
+
+template <int D>
+struct TileSmem {
+    static constexpr int kRows = 128 * D * 2;  // fp16 tile: 128 rows, D/64 columns of 128 bytes
+    static constexpr int kQ = 0;               // [2]
+    static constexpr int kK = 2 * kRows;       // [2]
+    static constexpr int kV = 4 * kRows;       // [2]
+    static constexpr int kMeta = 6 * kRows;
+    static constexpr int kRf = kMeta + kMetaStages * static_cast<int>(sizeof(TileMeta));  // [2][256]
+    static constexpr int kMl = kRf + 2 * 256 * 4;                                         // [2][128] m, l, ve
+    static constexpr int kBar = kMl + 2 * 128 * 16;
+    static constexpr int kBars = 2 * kMetaStages + 8 + 4 + 2 + 2 + 3;
+    static constexpr int kTmem = kBar + kBars * 8;
+    static constexpr int kBytes = kTmem + 16 + 1024;  // slack to align the base
+};
+static_assert(sizeof(TileMeta) % 16 == 0, "alignment");
+static_assert(TileSmem<128>::kBytes <= 232448, "shared memory");
+
+enum Bars {
+    kMetaFull = 0,
+    kMetaEmpty = kMetaFull + kMetaStages,
+    kKFull = kMetaEmpty + kMetaStages,
+    kKEmpty = kKFull + 2,
+    kVFull = kKEmpty + 2,
+    kVEmpty = kVFull + 2,
+    kSFull = kVEmpty + 2,
+    kPFull = kSFull + 2,
+    kQFull = kPFull + 2,
+    kQEmpty = kQFull + 1,
+    kOFull = kQEmpty + 1,
+    kMerge = kOFull + 2,
+    kDone = kMerge + 1,
+    kDrain = kDone + 1,
+};
+
+constexpr uint32_t kColO = 256;  // S and P: columns 0 and 128; O: 256 and 384
+
+__host__ __device__ constexpr uint32_t idesc_fp16(int N, int M, bool b_mn) {
+    return (1u << 4) | ((b_mn ? 1u : 0u) << 16) | (static_cast<uint32_t>(N >> 3) << 17) | (static_cast<uint32_t>(M >> 4) << 24);
+}
+
+__device__ __forceinline__ void mma_f16_ss_warp(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc, uint32_t idesc, bool accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p, e;\n\t.reg .b32 r;\n\t"
+        "elect.sync r|e, 0xffffffff;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "@e tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
+        ::"r"(d_tmem), "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate ? 1u : 0u)
+        : "memory");
+}
+
+__device__ __forceinline__ void mbar_arrive_n(uint64_t* bar, uint32_t n) {
+    asm volatile("mbarrier.arrive.release.cta.shared::cta.b64 _, [%0], %1;" ::"r"(smem_u32(bar)), "r"(n) : "memory");
+}
+
+__device__ __forceinline__ bool mbar_wait_all(uint64_t* bar, uint32_t parity) {
+    return __all_sync(0xffffffffu, mbar_wait(bar, parity));
+}
+
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float r;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    return r;
+}
+
+template <int N>
+__device__ __forceinline__ void regs_more() {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N));
+}
+template <int N>
+__device__ __forceinline__ void regs_less() {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
+}
+
+struct TileUnit {
+    int b, hk, rb, split, nsplit, nrb;
+    ChunkRows R;
+    int rows;            // of the request and KV head
+    int begin, end, nt;  // tokens, tiles
+    bool alt;            // the warpgroups take tiles in turn
+};
+
+// Later blocks of rows see more tokens and come first; blocks of one KV head lie together, for L2.
+template <int TERMS>
+__device__ __forceinline__ TileUnit tile_unit(const ChunkParams& p, int unit) {
+    constexpr int ROWS = TERMS == 1 ? 256 : 128;
+    TileUnit u;
+    u.b = warp_find(p.tile_first, p.B, unit);
+    u.R = chunk_rows(p, u.b);
+    u.rows = u.R.n * p.G;
+    u.nrb = (u.rows + ROWS - 1) / ROWS;
+    int each;
+    u.nsplit = chunk_splits(u.R.len, p.head->tile_span, kTile, each);
+    int rest = unit - p.tile_first[u.b];
+    u.rb = u.nrb - 1 - rest % u.nrb;
+    rest /= u.nrb;
+    u.hk = rest % p.Hkv;
+    u.split = rest / p.Hkv;
+    const int last = min(u.rows, (u.rb + 1) * ROWS) - 1;
+    const int most = chunk_sees(p, u.R, static_cast<int>(p.by_g.div(static_cast<uint32_t>(last))));
+    u.begin = u.split * each;
+    u.end = min(min(u.begin + each, u.R.len), most);
+    u.nt = u.end > u.begin ? (u.end - u.begin + kTile - 1) / kTile : 0;
+    u.alt = TERMS == 2 || u.rows - u.rb * ROWS <= 128;
+    return u;
+}
+
+// ------------------------------------------------------------------ look-ahead
+__device__ __forceinline__ void tile_scout(const ChunkParams& p, const TileUnit& u, TileMeta* meta, uint64_t* bars, int& j, bool& ok) {
+    const int lane = threadIdx.x & 31;
+    const int32_t* table = p.table + u.b * p.bt_stride;
+    constexpr int N = kTile / 32;
+    int id[N], off[N];
+    auto look_up = [&](int i) {
+#pragma unroll
+        for (int x = 0; x < N; ++x) {
+            const int t = u.begin + i * kTile + 32 * x + lane;
+            id[x] = -1;
+            off[x] = 0;
+            if (t < u.end) {
+                const int k = static_cast<int>(p.by_bs.div(static_cast<uint32_t>(t)));
+                off[x] = t - k * p.bs;
+                id[x] = table[k];
+            }
+        }
+    };
+    int ve = 126;
+    look_up(0);
+    for (int i = 0; i < u.nt && ok; ++i, ++j) {
+        TileMeta* m = meta + (j & (kMetaStages - 1));
+        float ks[N], vs[N];
+        int64_t row[N];
+        bool bad = false;
+#pragma unroll
+        for (int x = 0; x < N; ++x) {
+            const bool there = id[x] >= 0 && id[x] < p.NB;
+            bad |= !there && u.begin + i * kTile + 32 * x + lane < u.end;
+            const int64_t s = there ? id[x] * p.sc_sblk + u.hk * p.sc_sh + off[x] : 0;
+            row[x] = there ? id[x] * p.kv_sblk + u.hk * p.kv_sh + off[x] * p.kv_st : -1;
+            ks[x] = there ? p.ks[s] : 0.f;
+            vs[x] = there ? p.vs[s] : 0.f;
+        }
+        if (bad) record_status(KVD_STATUS_BAD_BLOCK);
+        if (i + 1 < u.nt) look_up(i + 1);  // on its way while this tile's scales come
+        float top = 0.f;
+#pragma unroll
+        for (int x = 0; x < N; ++x) {
+            const float a = fabsf(vs[x]);
+            if (a < INFINITY) top = fmaxf(top, a);  // what is not finite has no say
+        }
+        const int bits = __reduce_max_sync(0xffffffffu, __float_as_int(top));
+        if (bits != 0) ve = min(ve, fit_exponent(__int_as_float(bits), 7));
+        const float f = pow2i(ve);
+        ok = j < kMetaStages || mbar_wait_all(&bars[kMetaEmpty + (j & (kMetaStages - 1))], ((j / kMetaStages) - 1) & 1);
+        if (!ok) break;
+#pragma unroll
+        for (int x = 0; x < N; ++x) {
+            m->ks[32 * x + lane] = ks[x];
+            m->vs[32 * x + lane] = vs[x] * f;
+            m->row[32 * x + lane] = row[x];
+        }
+        if (lane == 0) m->ve = ve;
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&bars[kMetaFull + (j & (kMetaStages - 1))]);
+    }
+}
+
+// ------------------------------------------------------------------ converters
+// Place of 16-byte piece ch (of 8) of column col of row r in an fp16 tile.
+__device__ __forceinline__ int piece_at(int r, int col, int ch) {
+    return col * 16384 + (r >> 3) * 1024 + (r & 7) * 128 + ((ch ^ (r & 7)) << 4);
+}
+
+// Sixteen codes of row r, dims 16 c16 .., as two pieces. Eight lanes that store together take the two in an
+// order that meets eight different places.
+template <int D>
+__device__ __forceinline__ void store_codes(uint8_t* tile, int r, int c16, uint4 w) {
+    uint4 a, b;
+    // words hold dims 4i..4i+3: pairs (0,1) and (2,3) in the order of the dims
+    auto two = [](uint32_t x, uint32_t& lo, uint32_t& hi) {
+        const uint32_t y = x ^ 0x80808080u;
+        uint32_t l = __byte_perm(y, 0x64646464u, 0x4140), h = __byte_perm(y, 0x64646464u, 0x4342);
+        const __half2 k = __half2half2(__ushort_as_half(0x6480));
+        const __half2 hl = __hsub2(*reinterpret_cast<const __half2*>(&l), k), hh = __hsub2(*reinterpret_cast<const __half2*>(&h), k);
+        lo = *reinterpret_cast<const uint32_t*>(&hl);
+        hi = *reinterpret_cast<const uint32_t*>(&hh);
+    };
+    two(w.x, a.x, a.y);
+    two(w.y, a.z, a.w);
+    two(w.z, b.x, b.y);
+    two(w.w, b.z, b.w);
+    const int col = c16 >> 2, ch = (c16 & 3) * 2;
+    const bool swap = D == 128 && col != 0;
+    *reinterpret_cast<uint4*>(tile + piece_at(r, col, swap ? ch + 1 : ch)) = swap ? b : a;
+    *reinterpret_cast<uint4*>(tile + piece_at(r, col, swap ? ch : ch + 1)) = swap ? a : b;
+}
+
+template <int D>
+struct Codes {
+    static constexpr int PER = D / 16;          // lanes a row
+    static constexpr int N = 128 * PER / 128;   // pieces of 16 codes a thread
+    uint4 w[N];
+    __device__ __forceinline__ void load(const int8_t* pool, const TileMeta* m, int ct) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const int r = ct / PER + i * (128 / PER);
+            const int64_t at = m->row[r];
+            w[i] = at >= 0 ? *reinterpret_cast<const uint4*>(pool + at + (ct % PER) * 16) : make_uint4(0u, 0u, 0u, 0u);
+        }
+    }
+    __device__ __forceinline__ void store(uint8_t* tile, int ct) const {
+#pragma unroll
+        for (int i = 0; i < N; ++i) store_codes<D>(tile, ct / PER + i * (128 / PER), ct % PER, w[i]);
+    }
+};
+
+// The unit's rows as fp16, each times its power of two, and what the scores are multiplied with instead.
+template <int D, int TERMS>
+__device__ __forceinline__ void load_queries(const ChunkParams& p, const TileUnit& u, uint8_t* q, float* rf, int ct) {
+    constexpr int ROWS = TERMS == 1 ? 256 : 128;
+    constexpr int PER = D / 16;
+    const int there = min(ROWS, u.rows - u.rb * ROWS), most = TERMS == 1 && there > 128 ? 256 : 128;
+    const int c16 = ct % PER;
+#pragma unroll 2
+    for (int r = ct / PER; r < most; r += 128 / PER) {
+        float x[16];
+#pragma unroll
+        for (int d = 0; d < 16; ++d) x[d] = 0.f;
+        if (r < there) {
+            const int row = u.rb * ROWS + r;
+            const int i = static_cast<int>(p.by_g.div(static_cast<uint32_t>(row))), g = row - i * p.G;
+            const int64_t at = static_cast<int64_t>(u.R.t0 + i) * p.q_st + static_cast<int64_t>(u.hk * p.G + g) * p.q_sh + c16 * 16;
+            if (!p.vec_q) {
+#pragma unroll
+                for (int d = 0; d < 16; ++d) x[d] = load_q(p.Q, at + d, p.flags);
+            } else if (p.flags & (KVD_FLAG_Q_BF16 | KVD_FLAG_Q_F16)) {
+                const uint4* src = reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p.Q) + at);
+#pragma unroll
+                for (int k = 0; k < 2; ++k) {
+                    const uint4 v = src[k];
+                    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+                    for (int y = 0; y < 4; ++y) {
+                        float2 f;
+                        if (p.flags & KVD_FLAG_Q_BF16)
+                            f = make_float2(__uint_as_float(w[y] << 16), __uint_as_float(w[y] & 0xffff0000u));
+                        else
+                            f = __half22float2(*reinterpret_cast<const __half2*>(&w[y]));
+                        x[8 * k + 2 * y] = f.x;
+                        x[8 * k + 2 * y + 1] = f.y;
+                    }
+                }
+            } else {
+                const float4* src = reinterpret_cast<const float4*>(static_cast<const float*>(p.Q) + at);
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    const float4 v = src[k];
+                    x[4 * k] = v.x; x[4 * k + 1] = v.y; x[4 * k + 2] = v.z; x[4 * k + 3] = v.w;
+                }
+            }
+        }
+        float top = 0.f;
+#pragma unroll
+        for (int d = 0; d < 16; ++d) top = fmaxf(top, fabsf(x[d]));
+#pragma unroll
+        for (int o = 1; o < PER; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+        const int k = fit_exponent(top, 15);
+        const float f = pow2i(k);
+        if (c16 == 0) rf[r] = p.qscale * pow2i(-k);
+        uint32_t hi[8], lo[8];
+#pragma unroll
+        for (int d = 0; d < 8; ++d) {
+            hi[d] = pack_half(x[2 * d] * f, x[2 * d + 1] * f);
+            if (TERMS == 2) lo[d] = pack_rest(x[2 * d] * f, x[2 * d + 1] * f, hi[d]);
+        }
+        uint8_t* tile = q + (r >> 7) * TileSmem<D>::kRows;
+        const int col = c16 >> 2, ch = (c16 & 3) * 2, rr = r & 127;
+        *reinterpret_cast<uint4*>(tile + piece_at(rr, col, ch)) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+        *reinterpret_cast<uint4*>(tile + piece_at(rr, col, ch + 1)) = make_uint4(hi[4], hi[5], hi[6], hi[7]);
+        if constexpr (TERMS == 2) {
+            uint8_t* rest = q + TileSmem<D>::kRows;
+            *reinterpret_cast<uint4*>(rest + piece_at(rr, col, ch)) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+            *reinterpret_cast<uint4*>(rest + piece_at(rr, col, ch + 1)) = make_uint4(lo[4], lo[5], lo[6], lo[7]);
+        }
+    }
+}
+
+// Tiles in the order in which the MMAs want them: K of the first two, then V of a tile and K of the second next.
+template <int D, int TERMS>
+__device__ __forceinline__ bool tile_convert(const ChunkParams& p, const TileUnit& u, uint8_t* smem, uint64_t* bars, int j0, int nu) {
+    using S = TileSmem<D>;
+    const int ct = threadIdx.x - 256, lane = ct & 31;
+    const TileMeta* meta = reinterpret_cast<const TileMeta*>(smem + S::kMeta);
+    const int jobs = 2 * u.nt;
+    auto job = [&](int q, int& tile, bool& v) {
+        v = q == jobs - 1 || (q >= 2 && (q & 1) == 0);
+        tile = v ? (q == jobs - 1 ? u.nt - 1 : (q - 2) >> 1) : (q == 0 ? 0 : (q + 1) >> 1);
+    };
+    auto load = [&](int q, Codes<D>& c) -> bool {
+        if (q >= jobs) return true;
+        int tile;
+        bool v;
+        job(q, tile, v);
+        const int j = j0 + tile, st = j & (kMetaStages - 1);
+        if (!v && !mbar_wait(&bars[kMetaFull + st], (j / kMetaStages) & 1)) return false;
+        c.load(v ? p.V : p.K, meta + st, ct);
+        if (v) {
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&bars[kMetaEmpty + st]);
+        }
+        return true;
+    };
+    auto store = [&](int q, const Codes<D>& c) -> bool {
+        int tile;
+        bool v;
+        job(q, tile, v);
+        const int j = j0 + tile, st = j & 1;
+        if (j >= 2 && !mbar_wait(&bars[(v ? kVEmpty : kKEmpty) + st], ((j >> 1) - 1) & 1)) return false;
+        c.store(smem + (v ? S::kV : S::kK) + st * S::kRows, ct);
+        fence_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&bars[(v ? kVFull : kKFull) + st]);
+        return true;
+    };
+    Codes<D> a, b;
+    if (!load(0, a)) return false;
+    if (nu > 0 && !mbar_wait(&bars[kQEmpty], (nu - 1) & 1)) return false;
+    load_queries<D, TERMS>(p, u, smem + S::kQ, reinterpret_cast<float*>(smem + S::kRf) + (nu & 1) * 256, ct);
+    fence_async_smem();
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&bars[kQFull]);
+#pragma unroll 1
+    for (int q = 0; q < jobs; q += 2) {  // an even number of jobs
+        if (!load(q + 1, b) || !store(q, a) || !load(q + 2, a) || !store(q + 1, b)) return false;
+    }
+    return true;
+}
+
+// ------------------------------------------------------------------ MMA issuer
+// Step i works for warpgroup i & 1: on tile i when the warpgroups take tiles in turn, else on tile i / 2. The
+// scores of step i + 2 are issued behind the weights' product of step i, which reads the columns they overwrite.
+template <int D, int TERMS>
+__device__ __forceinline__ bool tile_mma(const TileUnit& u, uint8_t* smem, uint32_t tmem, uint64_t* bars, int j0, int nu, int (&np)[2], int nq) {
+    using S = TileSmem<D>;
+    constexpr uint32_t id_s = idesc_fp16(kTile, 128, false), id_o = idesc_fp16(D, 128, true);
+    const int steps = u.alt ? u.nt : 2 * u.nt;
+    if (!mbar_wait_all(&bars[kQFull], nu & 1)) return false;
+    auto scores = [&](int i) -> bool {
+        const int w = i & 1, j = j0 + (u.alt ? i : i >> 1), st = j & 1;
+        if ((u.alt || w == 0) && !mbar_wait_all(&bars[kKFull + st], (j >> 1) & 1)) return false;
+        tc_fence_after();
+        const uint64_t kd = smem_desc(smem_u32(smem + S::kK + st * S::kRows), 16u, 1024u, kLayoutSw128);
+#pragma unroll
+        for (int t = 0; t < TERMS; ++t) {
+            if (t < nq) {
+                const int tile = TERMS == 2 ? t : (u.alt ? 0 : w);
+                const uint64_t qd = smem_desc(smem_u32(smem + S::kQ + tile * S::kRows), 16u, 1024u, kLayoutSw128);
+#pragma unroll
+                for (int k = 0; k < D / 16; ++k) {
+                    const uint64_t step = ((k >> 2) * 16384u + (k & 3) * 32u) >> 4;
+                    mma_f16_ss_warp(tmem + w * 128u, qd + step, kd + step, id_s, t > 0 || k > 0);
+                }
+            }
+        }
+        mma_commit_warp(&bars[kSFull + w]);
+        if (u.alt || w == 1) mma_commit_warp(&bars[kKEmpty + st]);
+        return true;
+    };
+    if (!scores(0)) return false;
+    if (steps > 1 && !scores(1)) return false;
+    if (steps <= 2) mma_commit_warp(&bars[kQEmpty]);
+    for (int i = 0; i < steps; ++i) {
+        const int w = i & 1, j = j0 + (u.alt ? i : i >> 1), st = j & 1;
+        if (!mbar_wait_all(&bars[kPFull + w], np[w] & 1)) return false;
+        ++np[w];
+        if ((u.alt || w == 0) && !mbar_wait_all(&bars[kVFull + st], (j >> 1) & 1)) return false;
+        tc_fence_after();
+        // 16 tokens: two groups of 8 rows (1,024 bytes each); dims 64.. one column on
+        const uint64_t vd = smem_desc(smem_u32(smem + S::kV + st * S::kRows), 16384u, 1024u, kLayoutSw128);
+#pragma unroll
+        for (int t = 0; t < TERMS; ++t)
+#pragma unroll
+            for (int k = 0; k < kTile / 16; ++k)
+                mma_f16_ts_warp(tmem + kColO + w * 128u, tmem + w * 128u + 64u * t + 8u * k, vd + (2048u * k >> 4), id_o,
+                                i >= 2 || t > 0 || k > 0);
+        if (u.alt || w == 1) mma_commit_warp(&bars[kVEmpty + st]);
+        if (i + 2 < steps) {
+            if (!scores(i + 2)) return false;
+            if (i + 3 == steps) mma_commit_warp(&bars[kQEmpty]);
+        } else {
+            mma_commit_warp(&bars[kOFull + w]);
+        }
+    }
+    return true;
+}
+
+// ------------------------------------------------------------------ softmax
+// Columns d0 .. d0 + 31 of a row.
+__device__ __forceinline__ void store_row32(const ChunkParams& p, int64_t at, const float (&x)[32]) {
+    const bool o16 = (p.flags & (KVD_FLAG_OUT_BF16 | KVD_FLAG_OUT_F16)) != 0;
+    if (!p.vec_out) {
+#pragma unroll
+        for (int d = 0; d < 32; ++d) store_out(p.out, at + d, x[d], p.flags);
+    } else if (!o16) {
+        float4* dst = reinterpret_cast<float4*>(static_cast<float*>(p.out) + at);
+#pragma unroll
+        for (int d = 0; d < 8; ++d) dst[d] = make_float4(x[4 * d], x[4 * d + 1], x[4 * d + 2], x[4 * d + 3]);
+    } else {
+        uint32_t w[16];
+#pragma unroll
+        for (int d = 0; d < 16; ++d) {
+            if (p.flags & KVD_FLAG_OUT_BF16) {
+                const __nv_bfloat162 h = __floats2bfloat162_rn(x[2 * d], x[2 * d + 1]);
+                w[d] = *reinterpret_cast<const uint32_t*>(&h);
+            } else {
+                w[d] = pack_half(x[2 * d], x[2 * d + 1]);
+            }
+        }
+        uint4* dst = reinterpret_cast<uint4*>(static_cast<uint16_t*>(p.out) + at);
+#pragma unroll
+        for (int d = 0; d < 4; ++d) dst[d] = make_uint4(w[4 * d], w[4 * d + 1], w[4 * d + 2], w[4 * d + 3]);
+    }
+}
+
+// The two softmax warpgroups meet (a bounded wait).
+__device__ __forceinline__ bool both_here(uint64_t* bars, int& count) {
+    tc_fence_before();
+    __syncwarp();
+    if ((threadIdx.x & 31) == 0) mbar_arrive(&bars[kMerge]);
+    const bool ok = mbar_wait(&bars[kMerge], count & 1);
+    ++count;
+    tc_fence_after();
+    return ok;
+}
+
+template <int D, int TERMS>
+__device__ __forceinline__ bool tile_softmax(const ChunkParams& p, const TileUnit& u, uint8_t* smem, uint32_t tmem, uint64_t* bars, int j0,
+                                             int nu, int& ns, int& no, int& nm_sync) {
+    using S = TileSmem<D>;
+    constexpr int ROWS = TERMS == 1 ? 256 : 128;
+    const int w = threadIdx.x >> 7, r = threadIdx.x & 127, lane = r & 31;
+    const uint32_t lanes = tmem + (static_cast<uint32_t>(r & ~31) << 16);
+    const uint32_t col_s = lanes + w * 128u, col_o = lanes + kColO + w * 128u;
+    const TileMeta* meta = reinterpret_cast<const TileMeta*>(smem + S::kMeta);
+    const int in_unit = u.alt ? r : w * 128 + r, row = u.rb * ROWS + in_unit;
+    const int i = static_cast<int>(p.by_g.div(static_cast<uint32_t>(row))), g = row - i * p.G;
+    const bool there = row < u.rows;
+    const int64_t o_at = static_cast<int64_t>(u.R.t0 + i) * p.o_st + static_cast<int64_t>(u.hk * p.G + g) * p.o_sh;
+    const int slot = u.nsplit > 1 ? p.tile_rec[u.b] + (u.hk * u.nrb + u.rb) * u.nsplit + u.split : -1;
+    const int64_t rec = static_cast<int64_t>(slot) * ROWS + in_unit;
+    if (u.nt == 0) {  // nothing in sight
+        if (there && (!u.alt || w == 0)) {
+            if (slot >= 0) {
+                p.tile_ml[rec] = make_float2(-INFINITY, 0.f);
+            } else {
+                const float none[32] = {};
+#pragma unroll 1
+                for (int d = 0; d < D; d += 32) store_row32(p, o_at + d, none);
+            }
+        }
+        return true;
+    }
+    if (!mbar_wait(&bars[kQFull], nu & 1)) return false;
+    const float rf = reinterpret_cast<const float*>(smem + S::kRf)[(nu & 1) * 256 + in_unit];
+    const int sees = chunk_sees(p, u.R, min(i, u.R.n - 1));  // rows that are not there see what the last one does
+    const int first_row = u.rb * ROWS + (u.alt ? 0 : w * 128);
+    const int least = min(u.end, chunk_sees(p, u.R, min(u.R.n - 1, static_cast<int>(p.by_g.div(static_cast<uint32_t>(first_row))))));
+    float m = -INFINITY;
+    float2 lp[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+    int ve = 126;
+    bool any = false;  // O holds sums of this unit
+    for (int tile = u.alt ? w : 0; tile < u.nt; tile += u.alt ? 2 : 1) {
+        const int j = j0 + tile, st = j & (kMetaStages - 1), t0 = u.begin + tile * kTile;
+        if (!mbar_wait(&bars[kMetaFull + st], (j / kMetaStages) & 1)) return false;
+        const float4* ks4 = reinterpret_cast<const float4*>(meta[st].ks);
+        const float4* vs4 = reinterpret_cast<const float4*>(meta[st].vs);
+        const int ve_now = meta[st].ve;
+        if (!mbar_wait(&bars[kSFull + w], ns & 1)) return false;
+        ++ns;
+        tc_fence_after();
+        uint32_t sr[kTile];
+#pragma unroll
+        for (int x = 0; x < 4; ++x) tmem_ld32(col_s + 32u * x, *reinterpret_cast<uint32_t(*)[32]>(&sr[32 * x]));
+        tmem_wait_ld();
+        float tm[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+        const bool masked = t0 + kTile > least;
+        if (masked) {
+            const int lim = min(sees, u.end) - t0;
+#pragma unroll
+            for (int k = 0; k < kTile / 4; ++k) {
+                const float4 kq = ks4[k];
+                const float2 a = __fmul2_rn(make_float2(__uint_as_float(sr[4 * k]), __uint_as_float(sr[4 * k + 1])), make_float2(kq.x, kq.y));
+                const float2 b = __fmul2_rn(make_float2(__uint_as_float(sr[4 * k + 2]), __uint_as_float(sr[4 * k + 3])), make_float2(kq.z, kq.w));
+                const float v0 = 4 * k < lim ? a.x : -INFINITY, v1 = 4 * k + 1 < lim ? a.y : -INFINITY;
+                const float v2 = 4 * k + 2 < lim ? b.x : -INFINITY, v3 = 4 * k + 3 < lim ? b.y : -INFINITY;
+                sr[4 * k] = __float_as_uint(v0);
+                sr[4 * k + 1] = __float_as_uint(v1);
+                sr[4 * k + 2] = __float_as_uint(v2);
+                sr[4 * k + 3] = __float_as_uint(v3);
+                tm[k & 3] = max3(max3(tm[k & 3], v0, v1), v2, v3);
+            }
+        } else {
+#pragma unroll
+            for (int k = 0; k < kTile / 4; ++k) {
+                const float4 kq = ks4[k];
+                const float2 a = __fmul2_rn(make_float2(__uint_as_float(sr[4 * k]), __uint_as_float(sr[4 * k + 1])), make_float2(kq.x, kq.y));
+                const float2 b = __fmul2_rn(make_float2(__uint_as_float(sr[4 * k + 2]), __uint_as_float(sr[4 * k + 3])), make_float2(kq.z, kq.w));
+                sr[4 * k] = __float_as_uint(a.x);
+                sr[4 * k + 1] = __float_as_uint(a.y);
+                sr[4 * k + 2] = __float_as_uint(b.x);
+                sr[4 * k + 3] = __float_as_uint(b.y);
+                tm[k & 3] = max3(max3(tm[k & 3], a.x, a.y), b.x, b.y);
+            }
+        }
+        const float top = fmaxf(fmaxf(tm[0], tm[1]), fmaxf(tm[2], tm[3])) * rf;  // rf > 0: -inf stays
+        const bool move = top > m + (m == -INFINITY ? 0.f : 8.f);
+        if (any && __any_sync(0xffffffffu, (move && m != -INFINITY) || ve_now != ve)) {
+            // this warpgroup's products before this tile's scores are complete: O may change
+            const float f = move && m != -INFINITY ? ex2_fast(m - top) : 1.f;
+            const float fo = f * (ve - ve_now > 126 ? 0.f : pow2i(ve_now - ve));
+#pragma unroll 1
+            for (int d = 0; d < D; d += 32) {
+                uint32_t o[32];
+                tmem_ld32(col_o + d, o);
+                tmem_wait_ld();
+#pragma unroll
+                for (int x = 0; x < 32; ++x) o[x] = __float_as_uint(__uint_as_float(o[x]) * fo);
+                tmem_st32(col_o + d, o);
+            }
+            lp[0] = __fmul2_rn(lp[0], make_float2(f, f));
+            lp[1] = __fmul2_rn(lp[1], make_float2(f, f));
+        }
+        any = true;
+        ve = ve_now;
+        if (move) m = top;
+        const float me = m == -INFINITY ? 0.f : m;
+        const float2 nm = make_float2(-me, -me), rf2 = make_float2(rf, rf);
+        const int hidden_from = masked ? min(sees, u.end) - t0 : kTile;
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {  // 32 tokens at a time: 16 columns of pairs
+            uint32_t hi[16], lo[16];
+#pragma unroll
+            for (int k = 0; k < 16; ++k) {
+                const int c = 16 * q + k;
+                const float2 d = __ffma2_rn(make_float2(__uint_as_float(sr[2 * c]), __uint_as_float(sr[2 * c + 1])), rf2, nm);
+                const float2 pp = make_float2(ex2_fast(d.x), ex2_fast(d.y));
+                lp[k & 1] = __fadd2_rn(lp[k & 1], pp);
+                const float4 vq = vs4[c >> 1];
+                float2 x = __fmul2_rn(pp, (c & 1) ? make_float2(vq.z, vq.w) : make_float2(vq.x, vq.y));
+                if (masked) {  // a hidden token's scale may be anything
+                    if (2 * c >= hidden_from) x.x = 0.f;
+                    if (2 * c + 1 >= hidden_from) x.y = 0.f;
+                }
+                hi[k] = pack_half(x.x, x.y);
+                if constexpr (TERMS == 2) lo[k] = pack_rest(x.x, x.y, hi[k]);
+            }
+            tmem_st16(col_s + 16u * q, hi);
+            if constexpr (TERMS == 2) tmem_st16(col_s + 64u + 16u * q, lo);
+        }
+        tmem_wait_st();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) {
+            mbar_arrive(&bars[kPFull + w]);
+            mbar_arrive_n(&bars[kMetaEmpty + st], u.alt ? 2u : 1u);
+        }
+    }
+    // ---- the rows
+    if (any) {
+        if (!mbar_wait(&bars[kOFull + w], no & 1)) return false;
+        ++no;
+    }
+    tc_fence_after();
+    float l = (lp[0].x + lp[0].y) + (lp[1].x + lp[1].y);
+    float back = pow2i(-ve), other_back = 0.f;
+    int d0 = 0, d1 = D;
+    if (u.alt) {  // the two warpgroups' sums, half of the dims each
+        float4* ml = reinterpret_cast<float4*>(smem + S::kMl);
+        ml[w * 128 + r] = make_float4(m, l, __int_as_float(ve), 0.f);
+        if (!both_here(bars, nm_sync)) return false;
+        const float4 other = ml[(w ^ 1) * 128 + r];
+        const int other_ve = __float_as_int(other.z);
+        const float M = fmaxf(m, other.x);
+        const float f0 = m == -INFINITY ? 0.f : ex2_fast(m - M), f1 = other.x == -INFINITY ? 0.f : ex2_fast(other.x - M);
+        l = l * f0 + other.y * f1;
+        m = M;
+        back *= f0;
+        other_back = u.nt > 1 ? pow2i(-other_ve) * f1 : 0.f;
+        if (!any) back = 0.f;
+        if (any && u.nt == 1) other_back = 0.f;
+        if (!any) other_back = pow2i(-other_ve) * f1;
+        d0 = w * (D / 2);
+        d1 = d0 + D / 2;
+    }
+    const float inv = slot >= 0 ? 1.f : (l == 0.f ? 0.f : 1.f / l);  // no token in sight: 0; NaN stays
+    const bool both = u.alt && u.nt > 1;
+#pragma unroll 1
+    for (int d = d0; d < d1; d += 32) {
+        float x[32];
+        {
+            uint32_t o[32];
+            tmem_ld32(lanes + kColO + (u.alt && !any ? (w ^ 1) : w) * 128u + d, o);
+            tmem_wait_ld();
+            const float f = u.alt && !any ? other_back : back;
+#pragma unroll
+            for (int y = 0; y < 32; ++y) x[y] = f == 0.f ? 0.f : __uint_as_float(o[y]) * f;
+        }
+        if (both) {
+            uint32_t o[32];
+            tmem_ld32(lanes + kColO + (w ^ 1) * 128u + d, o);
+            tmem_wait_ld();
+#pragma unroll
+            for (int y = 0; y < 32; ++y) x[y] = other_back == 0.f ? x[y] : fmaf(__uint_as_float(o[y]), other_back, x[y]);
+        }
+        if (there) {
+            if (slot >= 0) {
+                float4* dst = reinterpret_cast<float4*>(p.tile_o + rec * D + d);
+#pragma unroll
+                for (int y = 0; y < 8; ++y) dst[y] = make_float4(x[4 * y], x[4 * y + 1], x[4 * y + 2], x[4 * y + 3]);
+            } else {
+#pragma unroll
+                for (int y = 0; y < 32; ++y) x[y] *= inv;
+                store_row32(p, o_at + d, x);
+            }
+        }
+    }
+    if (slot >= 0 && there && (!u.alt || w == 0)) p.tile_ml[rec] = make_float2(m, l);
+    tc_fence_before();
+    return !u.alt || both_here(bars, nm_sync);  // both have read both
+}
+
+template <int D, int TERMS>
+__global__ void __launch_bounds__(kThreads, 1) chunk_tile_kernel(const __grid_constant__ ChunkParams p) {
+    using S = TileSmem<D>;
+    extern __shared__ uint8_t tile_smem[];
+    uint8_t* smem = tile_smem + ((1024u - (smem_u32(tile_smem) & 1023u)) & 1023u);
+    uint64_t* bars = reinterpret_cast<uint64_t*>(smem + S::kBar);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < kMetaStages; ++s) {
+            mbar_init(&bars[kMetaFull + s], 1);
+            mbar_init(&bars[kMetaEmpty + s], 4 + 8);  // converter and softmax warps
+        }
+        for (int s = 0; s < 2; ++s) {
+            mbar_init(&bars[kKFull + s], 4);
+            mbar_init(&bars[kKEmpty + s], 1);
+            mbar_init(&bars[kVFull + s], 4);
+            mbar_init(&bars[kVEmpty + s], 1);
+            mbar_init(&bars[kSFull + s], 1);
+            mbar_init(&bars[kPFull + s], 4);
+            mbar_init(&bars[kOFull + s], 1);
+        }
+        mbar_init(&bars[kQFull], 4);
+        mbar_init(&bars[kQEmpty], 1);
+        mbar_init(&bars[kMerge], 8);
+        mbar_init(&bars[kDone], 8);
+        mbar_init(&bars[kDrain], 1);
+        fence_mbar_init();
+    }
+    if (warp == 12) tmem_alloc(reinterpret_cast<uint32_t*>(smem + S::kTmem), 512);
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(smem + S::kTmem);
+    grid_dependency_wait();
+    allow_dependents();
+    const int units = p.head->tile_units;
+    if (warp < 8) {
+        regs_more<184>();
+        int j = 0, nu = 0, ns = 0, no = 0, nm = 0;
+        for (int unit = blockIdx.x; unit < units; unit += gridDim.x) {
+            const TileUnit u = tile_unit<TERMS>(p, unit);
+            if (!tile_softmax<D, TERMS>(p, u, smem, tmem, bars, j, nu, ns, no, nm)) break;
+            j += u.nt;
+            nu += u.nt > 0;
+        }
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&bars[kDone]);
+    } else if (warp < 12) {
+        regs_less<88>();
+        int j = 0, nu = 0;
+        for (int unit = blockIdx.x; unit < units; unit += gridDim.x) {
+            const TileUnit u = tile_unit<TERMS>(p, unit);
+            if (u.nt == 0) continue;
+            if (!tile_convert<D, TERMS>(p, u, smem, bars, j, nu)) break;
+            j += u.nt;
+            ++nu;
+        }
+    } else {
+        regs_less<56>();
+        if (warp == 12) {
+            const int nq = p.flags & (KVD_FLAG_Q_BF16 | KVD_FLAG_Q_F16) ? 1 : 2;
+            int j = 0, nu = 0, np[2] = {0, 0};
+            for (int unit = blockIdx.x; unit < units; unit += gridDim.x) {
+                const TileUnit u = tile_unit<TERMS>(p, unit);
+                if (u.nt == 0) continue;
+                if (!tile_mma<D, TERMS>(u, smem, tmem, bars, j, nu, np, nq)) break;
+                j += u.nt;
+                ++nu;
+            }
+            mma_commit_warp(&bars[kDrain]);  // arrives once every MMA issued above has completed
+            mbar_wait(&bars[kDrain], 0);
+            mbar_wait(&bars[kDone], 0);  // the softmax warps have finished with tensor memory
+            __syncwarp();
+            tc_fence_after();
+            tmem_dealloc(tmem, 512);
+        } else if (warp == 13) {
+            int j = 0;
+            bool ok = true;
+            for (int unit = blockIdx.x; unit < units && ok; unit += gridDim.x) {
+                const TileUnit u = tile_unit<TERMS>(p, unit);
+                tile_scout(p, u, reinterpret_cast<TileMeta*>(smem + S::kMeta), bars, j, ok);
+            }
+        }
+    }
+}
+
+template <int D, int TERMS>
+cudaError_t launch_tile(const ChunkParams& p, cudaStream_t st) {
+    auto kern = chunk_tile_kernel<D, TERMS>;
+    static PerDeviceOnce once;
+    cudaError_t e = once.run([kern] {
+        return cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, TileSmem<D>::kBytes);
+    });
+    if (e != cudaSuccess) return e;
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(device_sm_count(), 1, 1);
+    cfg.blockDim = dim3(kThreads, 1, 1);
+    cfg.dynamicSmemBytes = TileSmem<D>::kBytes;
+    cfg.stream = st;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, kern, p);
+}
+
+}  // namespace
+
+cudaError_t take_chunk_tile_status(int32_t* status) {
+    int32_t v = 0;
+    const int32_t zero = 0;
+    const cudaError_t e = cudaMemcpyFromSymbol(&v, g_status, sizeof(v));
+    if (e != cudaSuccess) return e;
+    *status |= v;
+    return v ? cudaMemcpyToSymbol(g_status, &zero, sizeof(zero)) : cudaSuccess;
+}
+
+cudaError_t launch_chunk_tile(const ChunkParams& p, cudaStream_t st, int* launches) {
+    const bool two = p.tile_rows == 128;
+    const cudaError_t e = p.D == 128 ? (two ? launch_tile<128, 2>(p, st) : launch_tile<128, 1>(p, st))
+                                     : (two ? launch_tile<64, 2>(p, st) : launch_tile<64, 1>(p, st));
+    if (e == cudaSuccess) ++*launches;
+    return e;
+}
+
+}  // namespace kvd

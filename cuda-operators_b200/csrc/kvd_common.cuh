@@ -15,7 +15,13 @@ namespace kvd {
 
 // Device status word (KVD_STATUS_*). Kernels OR a code into it instead of
 // trapping; kvd_device_status() reads and clears it.
+// A file that is compiled as a whole program (so that ptxas honours
+// setmaxnreg) has a word of its own, which kvd_device_status() reads too.
+#ifdef KVD_WHOLE_PROGRAM
+static __device__ int32_t g_status;
+#else
 extern __device__ int32_t g_status;
+#endif
 
 constexpr uint64_t kWaitTimeoutNs = 2000000000ull;  // 2 s bound on every spin-wait
 

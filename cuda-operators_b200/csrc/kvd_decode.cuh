@@ -215,4 +215,7 @@ cudaError_t launch_combine_parts(const float* parts, int num_parts, int64_t part
                                  int head_dim, void* out, int64_t out_stride, uint32_t flags,
                                  cudaStream_t st, int* launches);
 
+// Adds the status bits of the kernel for many new rows (kvd_chunk_tile.cu), which keeps a word of its own, and clears them.
+cudaError_t take_chunk_tile_status(int32_t* status);
+
 }  // namespace kvd
