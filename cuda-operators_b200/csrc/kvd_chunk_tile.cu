@@ -18,15 +18,15 @@
 // with one term. So there are always two score tiles in flight: while one
 // warpgroup turns its scores into weights the tensor cores work for the other.
 //
-// One CTA an SM, 16 warps:
+// One CTA an SM, 20 warps:
 //   0-7   softmax, a row a thread (= TMEM lane): S from tensor memory, weights
 //         back into the columns that S had, from where they are an MMA operand;
-//   8-11  widen INT8 rows, straight from global memory (a tile ahead in
+//   8-15  widen INT8 rows, straight from global memory (a tile ahead in
 //         registers), into fp16 tiles in shared memory: 128-byte swizzled rows of
 //         tokens, the K-major operand of q K^T and the MN-major one of P V; and
 //         the unit's queries;
-//   12    issues the MMAs;
-//   13    looks the tile's blocks up ahead: row offsets, scales.
+//   16    issues the MMAs;
+//   17    looks the tile's blocks up ahead: row offsets, scales.
 // Every wait is bounded; on expiry the kernel records KVD_STATUS_WAIT_TIMEOUT
 // and unwinds.
 #include "kvd_chunk.cuh"
@@ -36,16 +36,21 @@
 namespace kvd {
 namespace {
 
-constexpr int kThreads = 512;
+constexpr int kThreads = 640;
+constexpr int kConvWarps = 8, kConvThreads = 32 * kConvWarps;
+// Registers a thread has after the split, of 96 at launch: 256 x 136 + 256 x 72 + 128 x 64 = 640 x 96.
+constexpr int kSoftmaxRegs = 136, kConvRegs = 72, kOtherRegs = 64;
+static_assert(256 * kSoftmaxRegs + kConvThreads * kConvRegs + 128 * kOtherRegs <= kThreads * 96, "registers of the launch");
 constexpr int kMetaStages = 4;
 
 // What is known of a tile before it is read.
 struct TileMeta {
     float ks[kTile];
-    float vs[kTile];     // times 2^ve
+    float vs[kTile];     // times 2^ve, 0 where it is not finite
     int64_t row[kTile];  // offset of the token's row in the pools, -1: zeros
+    uint32_t odd[kTile / 32];  // tokens whose value scale is not finite
     int ve;
-    int pad[15];
+    int pad[11];
 };
 
 template <int D>
@@ -192,10 +197,13 @@ __device__ __forceinline__ void tile_scout(const ChunkParams& p, const TileUnit&
         if (bad) record_status(KVD_STATUS_BAD_BLOCK);
         if (i + 1 < u.nt) look_up(i + 1);  // on its way while this tile's scales come
         float top = 0.f;
+        uint32_t odd[N];
 #pragma unroll
         for (int x = 0; x < N; ++x) {
-            const float a = fabsf(vs[x]);
-            if (a < INFINITY) top = fmaxf(top, a);  // what is not finite has no say
+            const bool fine = fabsf(vs[x]) < INFINITY;
+            odd[x] = __ballot_sync(0xffffffffu, !fine);
+            if (!fine) vs[x] = 0.f;
+            top = fmaxf(top, fabsf(vs[x]));
         }
         const int bits = __reduce_max_sync(0xffffffffu, __float_as_int(top));
         if (bits != 0) ve = min(ve, fit_exponent(__int_as_float(bits), 7));
@@ -207,6 +215,7 @@ __device__ __forceinline__ void tile_scout(const ChunkParams& p, const TileUnit&
             m->ks[32 * x + lane] = ks[x];
             m->vs[32 * x + lane] = vs[x] * f;
             m->row[32 * x + lane] = row[x];
+            if (lane == 0) m->odd[x] = odd[x];
         }
         if (lane == 0) m->ve = ve;
         __syncwarp();
@@ -247,19 +256,20 @@ __device__ __forceinline__ void store_codes(uint8_t* tile, int r, int c16, uint4
 template <int D>
 struct Codes {
     static constexpr int PER = D / 16;          // lanes a row
-    static constexpr int N = 128 * PER / 128;   // pieces of 16 codes a thread
+    static constexpr int N = 128 * PER / kConvThreads;  // pieces of 16 codes a thread
+    static constexpr int STEP = kConvThreads / PER;     // rows of all threads together
     uint4 w[N];
     __device__ __forceinline__ void load(const int8_t* pool, const TileMeta* m, int ct) {
 #pragma unroll
         for (int i = 0; i < N; ++i) {
-            const int r = ct / PER + i * (128 / PER);
+            const int r = ct / PER + i * STEP;
             const int64_t at = m->row[r];
             w[i] = at >= 0 ? *reinterpret_cast<const uint4*>(pool + at + (ct % PER) * 16) : make_uint4(0u, 0u, 0u, 0u);
         }
     }
     __device__ __forceinline__ void store(uint8_t* tile, int ct) const {
 #pragma unroll
-        for (int i = 0; i < N; ++i) store_codes<D>(tile, ct / PER + i * (128 / PER), ct % PER, w[i]);
+        for (int i = 0; i < N; ++i) store_codes<D>(tile, ct / PER + i * STEP, ct % PER, w[i]);
     }
 };
 
@@ -270,8 +280,8 @@ __device__ __forceinline__ void load_queries(const ChunkParams& p, const TileUni
     constexpr int PER = D / 16;
     const int there = min(ROWS, u.rows - u.rb * ROWS), most = TERMS == 1 && there > 128 ? 256 : 128;
     const int c16 = ct % PER;
-#pragma unroll 2
-    for (int r = ct / PER; r < most; r += 128 / PER) {
+#pragma unroll 1
+    for (int r = ct / PER; r < most; r += kConvThreads / PER) {
         float x[16];
 #pragma unroll
         for (int d = 0; d < 16; ++d) x[d] = 0.f;
@@ -417,7 +427,7 @@ __device__ __forceinline__ bool tile_mma(const TileUnit& u, uint8_t* smem, uint3
     };
     if (!scores(0)) return false;
     if (steps > 1 && !scores(1)) return false;
-    if (steps <= 2) mma_commit_warp(&bars[kQEmpty]);
+    bool loaded = true;  // the unit's queries are still needed
     for (int i = 0; i < steps; ++i) {
         const int w = i & 1, j = j0 + (u.alt ? i : i >> 1), st = j & 1;
         if (!mbar_wait_all(&bars[kPFull + w], np[w] & 1)) return false;
@@ -435,9 +445,14 @@ __device__ __forceinline__ bool tile_mma(const TileUnit& u, uint8_t* smem, uint3
         if (u.alt || w == 1) mma_commit_warp(&bars[kVEmpty + st]);
         if (i + 2 < steps) {
             if (!scores(i + 2)) return false;
-            if (i + 3 == steps) mma_commit_warp(&bars[kQEmpty]);
         } else {
             mma_commit_warp(&bars[kOFull + w]);
+        }
+        // Behind the last scores, and behind weights of every warpgroup that has any: these have then waited for
+        // this unit's queries, whose barrier may not complete twice before they do.
+        if (loaded && i + 3 >= steps && (i >= 1 || steps == 1)) {
+            mma_commit_warp(&bars[kQEmpty]);
+            loaded = false;
         }
     }
     return true;
@@ -469,6 +484,62 @@ __device__ __forceinline__ void store_row32(const ChunkParams& p, int64_t at, co
 #pragma unroll
         for (int d = 0; d < 4; ++d) dst[d] = make_uint4(w[4 * d], w[4 * d + 1], w[4 * d + 2], w[4 * d + 3]);
     }
+}
+
+// Scores of 32 tokens of this thread's row: the largest u ks (raw products times the tokens' scales) of the first
+// `lim` ones.
+template <bool MASK>
+__device__ __forceinline__ float top32(uint32_t col, const float4* ks4, int lim) {
+    uint32_t s[32];
+    tmem_ld32(col, s);
+    tmem_wait_ld();
+    float tm[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+        const float4 kq = ks4[k];
+        const float2 a = __fmul2_rn(make_float2(__uint_as_float(s[4 * k]), __uint_as_float(s[4 * k + 1])), make_float2(kq.x, kq.y));
+        const float2 b = __fmul2_rn(make_float2(__uint_as_float(s[4 * k + 2]), __uint_as_float(s[4 * k + 3])), make_float2(kq.z, kq.w));
+        const float v0 = !MASK || 4 * k < lim ? a.x : -INFINITY, v1 = !MASK || 4 * k + 1 < lim ? a.y : -INFINITY;
+        const float v2 = !MASK || 4 * k + 2 < lim ? b.x : -INFINITY, v3 = !MASK || 4 * k + 3 < lim ? b.y : -INFINITY;
+        tm[k & 1] = max3(max3(tm[k & 1], v0, v1), v2, v3);
+    }
+    return fmaxf(tm[0], tm[1]);
+}
+
+// Weights of 32 tokens with reference m: their sum onto `sum`, p vs 2^ve as fp16 pairs (and their rests). Returns
+// the largest u ks.
+template <bool MASK>
+__device__ __forceinline__ float weights32(uint32_t col, const float4* ks4, const float4* vs4, int lim, float rf, float m,
+                                           float2 (&sum)[2], uint32_t (&hi)[16], uint32_t* lo) {
+    uint32_t s[32];
+    tmem_ld32(col, s);
+    tmem_wait_ld();
+    const float2 nm = make_float2(-m, -m), rf2 = make_float2(rf, rf);
+    float tm[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+        const float4 kq = ks4[k], vq = vs4[k];
+        float2 a = __fmul2_rn(make_float2(__uint_as_float(s[4 * k]), __uint_as_float(s[4 * k + 1])), make_float2(kq.x, kq.y));
+        float2 b = __fmul2_rn(make_float2(__uint_as_float(s[4 * k + 2]), __uint_as_float(s[4 * k + 3])), make_float2(kq.z, kq.w));
+        if (MASK) {
+            a = make_float2(4 * k < lim ? a.x : -INFINITY, 4 * k + 1 < lim ? a.y : -INFINITY);
+            b = make_float2(4 * k + 2 < lim ? b.x : -INFINITY, 4 * k + 3 < lim ? b.y : -INFINITY);
+        }
+        tm[k & 1] = max3(max3(tm[k & 1], a.x, a.y), b.x, b.y);
+        a = __ffma2_rn(a, rf2, nm);
+        b = __ffma2_rn(b, rf2, nm);
+        const float2 pa = make_float2(ex2_fast(a.x), ex2_fast(a.y)), pb = make_float2(ex2_fast(b.x), ex2_fast(b.y));
+        sum[0] = __fadd2_rn(sum[0], pa);
+        sum[1] = __fadd2_rn(sum[1], pb);
+        const float2 x = __fmul2_rn(pa, make_float2(vq.x, vq.y)), y = __fmul2_rn(pb, make_float2(vq.z, vq.w));
+        hi[2 * k] = pack_half(x.x, x.y);
+        hi[2 * k + 1] = pack_half(y.x, y.y);
+        if (lo) {
+            lo[2 * k] = pack_rest(x.x, x.y, hi[2 * k]);
+            lo[2 * k + 1] = pack_rest(y.x, y.y, hi[2 * k + 1]);
+        }
+    }
+    return fmaxf(tm[0], tm[1]);
 }
 
 // The two softmax warpgroups meet (a bounded wait).
@@ -509,7 +580,8 @@ __device__ __forceinline__ bool tile_softmax(const ChunkParams& p, const TileUni
         }
         return true;
     }
-    if (!mbar_wait(&bars[kQFull], nu & 1)) return false;
+    // (a warpgroup without tiles does not wait: nothing holds the barrier up for it)
+    if ((!u.alt || w < u.nt) && !mbar_wait(&bars[kQFull], nu & 1)) return false;
     const float rf = reinterpret_cast<const float*>(smem + S::kRf)[(nu & 1) * 256 + in_unit];
     const int sees = chunk_sees(p, u.R, min(i, u.R.n - 1));  // rows that are not there see what the last one does
     const int first_row = u.rb * ROWS + (u.alt ? 0 : w * 128);
@@ -527,84 +599,86 @@ __device__ __forceinline__ bool tile_softmax(const ChunkParams& p, const TileUni
         if (!mbar_wait(&bars[kSFull + w], ns & 1)) return false;
         ++ns;
         tc_fence_after();
-        uint32_t sr[kTile];
-#pragma unroll
-        for (int x = 0; x < 4; ++x) tmem_ld32(col_s + 32u * x, *reinterpret_cast<uint32_t(*)[32]>(&sr[32 * x]));
-        tmem_wait_ld();
-        float tm[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+        const int lim = min(sees, u.end) - t0;  // tokens of the tile that the row sees
         const bool masked = t0 + kTile > least;
-        if (masked) {
-            const int lim = min(sees, u.end) - t0;
+        bool done = false;
+        if constexpr (TERMS == 1) {
+            // With the reference of the tiles before: one pass. It stands unless a score is above it by more than 8.
+            if (!masked && __all_sync(0xffffffffu, m != -INFINITY) && ve_now == ve) {
+                uint32_t pk[kTile / 2];
+                float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+                float top = -INFINITY;
 #pragma unroll
-            for (int k = 0; k < kTile / 4; ++k) {
-                const float4 kq = ks4[k];
-                const float2 a = __fmul2_rn(make_float2(__uint_as_float(sr[4 * k]), __uint_as_float(sr[4 * k + 1])), make_float2(kq.x, kq.y));
-                const float2 b = __fmul2_rn(make_float2(__uint_as_float(sr[4 * k + 2]), __uint_as_float(sr[4 * k + 3])), make_float2(kq.z, kq.w));
-                const float v0 = 4 * k < lim ? a.x : -INFINITY, v1 = 4 * k + 1 < lim ? a.y : -INFINITY;
-                const float v2 = 4 * k + 2 < lim ? b.x : -INFINITY, v3 = 4 * k + 3 < lim ? b.y : -INFINITY;
-                sr[4 * k] = __float_as_uint(v0);
-                sr[4 * k + 1] = __float_as_uint(v1);
-                sr[4 * k + 2] = __float_as_uint(v2);
-                sr[4 * k + 3] = __float_as_uint(v3);
-                tm[k & 3] = max3(max3(tm[k & 3], v0, v1), v2, v3);
-            }
-        } else {
-#pragma unroll
-            for (int k = 0; k < kTile / 4; ++k) {
-                const float4 kq = ks4[k];
-                const float2 a = __fmul2_rn(make_float2(__uint_as_float(sr[4 * k]), __uint_as_float(sr[4 * k + 1])), make_float2(kq.x, kq.y));
-                const float2 b = __fmul2_rn(make_float2(__uint_as_float(sr[4 * k + 2]), __uint_as_float(sr[4 * k + 3])), make_float2(kq.z, kq.w));
-                sr[4 * k] = __float_as_uint(a.x);
-                sr[4 * k + 1] = __float_as_uint(a.y);
-                sr[4 * k + 2] = __float_as_uint(b.x);
-                sr[4 * k + 3] = __float_as_uint(b.y);
-                tm[k & 3] = max3(max3(tm[k & 3], a.x, a.y), b.x, b.y);
+                for (int q = 0; q < 4; ++q)
+                    top = fmaxf(top, weights32<false>(col_s + 32u * q, ks4 + 8 * q, vs4 + 8 * q, 0, rf, m, sum,
+                                                      *reinterpret_cast<uint32_t(*)[16]>(&pk[16 * q]), nullptr));
+                done = !__any_sync(0xffffffffu, top * rf > m + 8.f);
+                if (done) {
+                    lp[0] = __fadd2_rn(lp[0], sum[0]);
+                    lp[1] = __fadd2_rn(lp[1], sum[1]);
+                    tmem_st32(col_s, *reinterpret_cast<uint32_t(*)[32]>(&pk[0]));
+                    tmem_st32(col_s + 32u, *reinterpret_cast<uint32_t(*)[32]>(&pk[32]));
+                }
             }
         }
-        const float top = fmaxf(fmaxf(tm[0], tm[1]), fmaxf(tm[2], tm[3])) * rf;  // rf > 0: -inf stays
-        const bool move = top > m + (m == -INFINITY ? 0.f : 8.f);
-        if (any && __any_sync(0xffffffffu, (move && m != -INFINITY) || ve_now != ve)) {
-            // this warpgroup's products before this tile's scores are complete: O may change
-            const float f = move && m != -INFINITY ? ex2_fast(m - top) : 1.f;
-            const float fo = f * (ve - ve_now > 126 ? 0.f : pow2i(ve_now - ve));
+        if (!done) {
+            float top = -INFINITY;
+            if (masked) {
 #pragma unroll 1
-            for (int d = 0; d < D; d += 32) {
-                uint32_t o[32];
-                tmem_ld32(col_o + d, o);
-                tmem_wait_ld();
-#pragma unroll
-                for (int x = 0; x < 32; ++x) o[x] = __float_as_uint(__uint_as_float(o[x]) * fo);
-                tmem_st32(col_o + d, o);
+                for (int q = 0; q < 4; ++q) top = fmaxf(top, top32<true>(col_s + 32u * q, ks4 + 8 * q, lim - 32 * q));
+            } else {
+#pragma unroll 1
+                for (int q = 0; q < 4; ++q) top = fmaxf(top, top32<false>(col_s + 32u * q, ks4 + 8 * q, 0));
             }
-            lp[0] = __fmul2_rn(lp[0], make_float2(f, f));
-            lp[1] = __fmul2_rn(lp[1], make_float2(f, f));
+            top *= rf;  // rf > 0: -inf stays
+            const bool move = top > m + (m == -INFINITY ? 0.f : 8.f);
+            if (any && __any_sync(0xffffffffu, (move && m != -INFINITY) || ve_now != ve)) {
+                // this warpgroup's products before this tile's scores are complete: O may change
+                const float f = move && m != -INFINITY ? ex2_fast(m - top) : 1.f;
+                const float fo = f * (ve - ve_now > 126 ? 0.f : pow2i(ve_now - ve));
+#pragma unroll 1
+                for (int d = 0; d < D; d += 32) {
+                    uint32_t o[32];
+                    tmem_ld32(col_o + d, o);
+                    tmem_wait_ld();
+#pragma unroll
+                    for (int x = 0; x < 32; ++x) o[x] = __float_as_uint(__uint_as_float(o[x]) * fo);
+                    tmem_st32(col_o + d, o);
+                }
+                lp[0] = __fmul2_rn(lp[0], make_float2(f, f));
+                lp[1] = __fmul2_rn(lp[1], make_float2(f, f));
+            }
+            ve = ve_now;
+            if (move) m = top;
+            const float me = m == -INFINITY ? 0.f : m;
+            // hidden tokens (weight 0) and their value scales, which are finite here, leave no trace
+            uint32_t hi[16], rest[TERMS == 2 ? 3 : 1][16];
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                uint32_t* lo = TERMS == 2 ? rest[q < 3 ? q : 2] : nullptr;
+                if (TERMS == 2 && q == 3) {  // the columns that these terms go to have been read by now
+                    tmem_st16(col_s + 64u, rest[0]);
+                    tmem_st16(col_s + 80u, rest[1]);
+                    uint32_t last[16];
+                    if (masked) weights32<true>(col_s + 96u, ks4 + 24, vs4 + 24, lim - 96, rf, me, lp, hi, last);
+                    else weights32<false>(col_s + 96u, ks4 + 24, vs4 + 24, 0, rf, me, lp, hi, last);
+                    tmem_st16(col_s + 96u, rest[2]);
+                    tmem_st16(col_s + 112u, last);
+                } else if (masked) {
+                    weights32<true>(col_s + 32u * q, ks4 + 8 * q, vs4 + 8 * q, lim - 32 * q, rf, me, lp, hi, lo);
+                } else {
+                    weights32<false>(col_s + 32u * q, ks4 + 8 * q, vs4 + 8 * q, 0, rf, me, lp, hi, lo);
+                }
+                tmem_st16(col_s + 16u * q, hi);
+            }
         }
         any = true;
-        ve = ve_now;
-        if (move) m = top;
-        const float me = m == -INFINITY ? 0.f : m;
-        const float2 nm = make_float2(-me, -me), rf2 = make_float2(rf, rf);
-        const int hidden_from = masked ? min(sees, u.end) - t0 : kTile;
+        if (meta[st].odd[0] | meta[st].odd[1] | meta[st].odd[2] | meta[st].odd[3]) {
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {  // 32 tokens at a time: 16 columns of pairs
-            uint32_t hi[16], lo[16];
-#pragma unroll
-            for (int k = 0; k < 16; ++k) {
-                const int c = 16 * q + k;
-                const float2 d = __ffma2_rn(make_float2(__uint_as_float(sr[2 * c]), __uint_as_float(sr[2 * c + 1])), rf2, nm);
-                const float2 pp = make_float2(ex2_fast(d.x), ex2_fast(d.y));
-                lp[k & 1] = __fadd2_rn(lp[k & 1], pp);
-                const float4 vq = vs4[c >> 1];
-                float2 x = __fmul2_rn(pp, (c & 1) ? make_float2(vq.z, vq.w) : make_float2(vq.x, vq.y));
-                if (masked) {  // a hidden token's scale may be anything
-                    if (2 * c >= hidden_from) x.x = 0.f;
-                    if (2 * c + 1 >= hidden_from) x.y = 0.f;
-                }
-                hi[k] = pack_half(x.x, x.y);
-                if constexpr (TERMS == 2) lo[k] = pack_rest(x.x, x.y, hi[k]);
+            for (int x = 0; x < kTile / 32; ++x) {
+                const int n = lim - 32 * x;
+                if (meta[st].odd[x] & (n >= 32 ? 0xffffffffu : n <= 0 ? 0u : (1u << n) - 1u)) lp[0].x = NAN;
             }
-            tmem_st16(col_s + 16u * q, hi);
-            if constexpr (TERMS == 2) tmem_st16(col_s + 64u + 16u * q, lo);
         }
         tmem_wait_st();
         tc_fence_before();
@@ -688,25 +762,25 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_tile_kernel(const __grid_co
     if (threadIdx.x == 0) {
         for (int s = 0; s < kMetaStages; ++s) {
             mbar_init(&bars[kMetaFull + s], 1);
-            mbar_init(&bars[kMetaEmpty + s], 4 + 8);  // converter and softmax warps
+            mbar_init(&bars[kMetaEmpty + s], kConvWarps + 8);  // converter and softmax warps
         }
         for (int s = 0; s < 2; ++s) {
-            mbar_init(&bars[kKFull + s], 4);
+            mbar_init(&bars[kKFull + s], kConvWarps);
             mbar_init(&bars[kKEmpty + s], 1);
-            mbar_init(&bars[kVFull + s], 4);
+            mbar_init(&bars[kVFull + s], kConvWarps);
             mbar_init(&bars[kVEmpty + s], 1);
             mbar_init(&bars[kSFull + s], 1);
             mbar_init(&bars[kPFull + s], 4);
             mbar_init(&bars[kOFull + s], 1);
         }
-        mbar_init(&bars[kQFull], 4);
+        mbar_init(&bars[kQFull], kConvWarps);
         mbar_init(&bars[kQEmpty], 1);
         mbar_init(&bars[kMerge], 8);
         mbar_init(&bars[kDone], 8);
         mbar_init(&bars[kDrain], 1);
         fence_mbar_init();
     }
-    if (warp == 12) tmem_alloc(reinterpret_cast<uint32_t*>(smem + S::kTmem), 512);
+    if (warp == 16) tmem_alloc(reinterpret_cast<uint32_t*>(smem + S::kTmem), 512);
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(smem + S::kTmem);
@@ -714,7 +788,7 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_tile_kernel(const __grid_co
     allow_dependents();
     const int units = p.head->tile_units;
     if (warp < 8) {
-        regs_more<184>();
+        regs_more<kSoftmaxRegs>();
         int j = 0, nu = 0, ns = 0, no = 0, nm = 0;
         for (int unit = blockIdx.x; unit < units; unit += gridDim.x) {
             const TileUnit u = tile_unit<TERMS>(p, unit);
@@ -725,8 +799,8 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_tile_kernel(const __grid_co
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(&bars[kDone]);
-    } else if (warp < 12) {
-        regs_less<88>();
+    } else if (warp < 8 + kConvWarps) {
+        regs_less<kConvRegs>();
         int j = 0, nu = 0;
         for (int unit = blockIdx.x; unit < units; unit += gridDim.x) {
             const TileUnit u = tile_unit<TERMS>(p, unit);
@@ -736,8 +810,8 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_tile_kernel(const __grid_co
             ++nu;
         }
     } else {
-        regs_less<56>();
-        if (warp == 12) {
+        regs_less<kOtherRegs>();
+        if (warp == 16) {
             const int nq = p.flags & (KVD_FLAG_Q_BF16 | KVD_FLAG_Q_F16) ? 1 : 2;
             int j = 0, nu = 0, np[2] = {0, 0};
             for (int unit = blockIdx.x; unit < units; unit += gridDim.x) {
@@ -753,7 +827,7 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_tile_kernel(const __grid_co
             __syncwarp();
             tc_fence_after();
             tmem_dealloc(tmem, 512);
-        } else if (warp == 13) {
+        } else if (warp == 17) {
             int j = 0;
             bool ok = true;
             for (int unit = blockIdx.x; unit < units && ok; unit += gridDim.x) {
