@@ -47,7 +47,7 @@ constexpr int kMetaStages = 4;
 struct TileMeta {
     float ks[kTile];
     float vs[kTile];     // times 2^ve, 0 where it is not finite
-    int64_t row[kTile];  // offset of the token's row in the pools, -1: zeros
+    int64_t row[kTile];  // offset of the token's row in the pools; where there is none 0, and its scales are 0
     uint32_t odd[kTile / 32];  // tokens whose value scale is not finite
     int ve;
     int pad[11];
@@ -190,7 +190,7 @@ __device__ __forceinline__ void tile_scout(const ChunkParams& p, const TileUnit&
             const bool there = id[x] >= 0 && id[x] < p.NB;
             bad |= !there && u.begin + i * kTile + 32 * x + lane < u.end;
             const int64_t s = there ? id[x] * p.sc_sblk + u.hk * p.sc_sh + off[x] : 0;
-            row[x] = there ? id[x] * p.kv_sblk + u.hk * p.kv_sh + off[x] * p.kv_st : -1;
+            row[x] = there ? id[x] * p.kv_sblk + u.hk * p.kv_sh + off[x] * p.kv_st : 0;
             ks[x] = there ? p.ks[s] : 0.f;
             vs[x] = there ? p.vs[s] : 0.f;
         }
@@ -229,9 +229,7 @@ __device__ __forceinline__ int piece_at(int r, int col, int ch) {
     return col * 16384 + (r >> 3) * 1024 + (r & 7) * 128 + ((ch ^ (r & 7)) << 4);
 }
 
-// Sixteen codes of row r, dims 16 c16 .., as two pieces. Eight lanes that store together take the two in an
-// order that meets eight different places.
-template <int D>
+// Sixteen codes of row r, dims 16 c16 .., as two pieces.
 __device__ __forceinline__ void store_codes(uint8_t* tile, int r, int c16, uint4 w) {
     uint4 a, b;
     // words hold dims 4i..4i+3: pairs (0,1) and (2,3) in the order of the dims
@@ -248,28 +246,40 @@ __device__ __forceinline__ void store_codes(uint8_t* tile, int r, int c16, uint4
     two(w.z, b.x, b.y);
     two(w.w, b.z, b.w);
     const int col = c16 >> 2, ch = (c16 & 3) * 2;
-    const bool swap = D == 128 && col != 0;
-    *reinterpret_cast<uint4*>(tile + piece_at(r, col, swap ? ch + 1 : ch)) = swap ? b : a;
-    *reinterpret_cast<uint4*>(tile + piece_at(r, col, swap ? ch : ch + 1)) = swap ? a : b;
+    *reinterpret_cast<uint4*>(tile + piece_at(r, col, ch)) = a;
+    *reinterpret_cast<uint4*>(tile + piece_at(r, col, ch + 1)) = b;
 }
 
+// The pieces of 16 codes that a thread takes of a tile. Eight lanes that store together take four pieces of a row
+// of even number and the other four of the next one (all four of both at 64 dims), which are eight different places
+// of the swizzle; a warp's loads cover whole rows.
 template <int D>
 struct Codes {
-    static constexpr int PER = D / 16;          // lanes a row
-    static constexpr int N = 128 * PER / kConvThreads;  // pieces of 16 codes a thread
+    static constexpr int PER = D / 16;                  // pieces of a row
+    static constexpr int N = 128 * PER / kConvThreads;  // pieces a thread
     static constexpr int STEP = kConvThreads / PER;     // rows of all threads together
     uint4 w[N];
-    __device__ __forceinline__ void load(const int8_t* pool, const TileMeta* m, int ct) {
-#pragma unroll
-        for (int i = 0; i < N; ++i) {
-            const int r = ct / PER + i * STEP;
-            const int64_t at = m->row[r];
-            w[i] = at >= 0 ? *reinterpret_cast<const uint4*>(pool + at + (ct % PER) * 16) : make_uint4(0u, 0u, 0u, 0u);
+    static __device__ __forceinline__ void place(int ct, int& r, int& c16) {
+        if constexpr (D == 128) {
+            const int odd = (ct >> 2) & 1;
+            r = 2 * (ct >> 4) + odd;
+            c16 = (ct & 3) + 4 * (odd ^ ((ct >> 3) & 1));
+        } else {
+            r = ct >> 2;
+            c16 = ct & 3;
         }
     }
-    __device__ __forceinline__ void store(uint8_t* tile, int ct) const {
+    __device__ __forceinline__ void load(const int8_t* pool, const TileMeta* m, int ct) {
+        int r, c16;
+        place(ct, r, c16);
 #pragma unroll
-        for (int i = 0; i < N; ++i) store_codes<D>(tile, ct / PER + i * STEP, ct % PER, w[i]);
+        for (int i = 0; i < N; ++i) w[i] = *reinterpret_cast<const uint4*>(pool + m->row[r + i * STEP] + c16 * 16);
+    }
+    __device__ __forceinline__ void store(uint8_t* tile, int ct) const {
+        int r, c16;
+        place(ct, r, c16);
+#pragma unroll
+        for (int i = 0; i < N; ++i) store_codes(tile, r + i * STEP, c16, w[i]);
     }
 };
 
