@@ -229,15 +229,21 @@ __device__ __forceinline__ int piece_at(int r, int col, int ch) {
     return col * 16384 + (r >> 3) * 1024 + (r & 7) * 128 + ((ch ^ (r & 7)) << 4);
 }
 
-// Sixteen codes of row r, dims 16 c16 .., as two pieces.
-__device__ __forceinline__ void store_codes(uint8_t* tile, int r, int c16, uint4 w) {
+// Sixteen codes of row r, dims 16 c16 .., as two pieces; FOLD: times the row's scale, rounded.
+template <bool FOLD>
+__device__ __forceinline__ void store_codes(uint8_t* tile, int r, int c16, uint4 w, float scale) {
     uint4 a, b;
+    const __half2 f = __float2half2_rn(scale);
     // words hold dims 4i..4i+3: pairs (0,1) and (2,3) in the order of the dims
-    auto two = [](uint32_t x, uint32_t& lo, uint32_t& hi) {
+    auto two = [f](uint32_t x, uint32_t& lo, uint32_t& hi) {
         const uint32_t y = x ^ 0x80808080u;
         uint32_t l = __byte_perm(y, 0x64646464u, 0x4140), h = __byte_perm(y, 0x64646464u, 0x4342);
         const __half2 k = __half2half2(__ushort_as_half(0x6480));
-        const __half2 hl = __hsub2(*reinterpret_cast<const __half2*>(&l), k), hh = __hsub2(*reinterpret_cast<const __half2*>(&h), k);
+        __half2 hl = __hsub2(*reinterpret_cast<const __half2*>(&l), k), hh = __hsub2(*reinterpret_cast<const __half2*>(&h), k);
+        if (FOLD) {
+            hl = __hmul2(hl, f);
+            hh = __hmul2(hh, f);
+        }
         lo = *reinterpret_cast<const uint32_t*>(&hl);
         hi = *reinterpret_cast<const uint32_t*>(&hh);
     };
@@ -275,11 +281,12 @@ struct Codes {
 #pragma unroll
         for (int i = 0; i < N; ++i) w[i] = *reinterpret_cast<const uint4*>(pool + m->row[r + i * STEP] + c16 * 16);
     }
-    __device__ __forceinline__ void store(uint8_t* tile, int ct) const {
+    template <bool FOLD>
+    __device__ __forceinline__ void store(uint8_t* tile, int ct, const float* scale) const {
         int r, c16;
         place(ct, r, c16);
 #pragma unroll
-        for (int i = 0; i < N; ++i) store_codes(tile, r + i * STEP, c16, w[i]);
+        for (int i = 0; i < N; ++i) store_codes<FOLD>(tile, r + i * STEP, c16, w[i], FOLD ? scale[r + i * STEP] : 0.f);
     }
 };
 
@@ -355,7 +362,7 @@ __device__ __forceinline__ void load_queries(const ChunkParams& p, const TileUni
 }
 
 // Tiles in the order in which the MMAs want them: K of the first two, then V of a tile and K of the second next.
-template <int D, int TERMS>
+template <int D, int TERMS, bool FOLD>
 __device__ __forceinline__ bool tile_convert(const ChunkParams& p, const TileUnit& u, uint8_t* smem, uint64_t* bars, int j0, int nu) {
     using S = TileSmem<D>;
     const int ct = threadIdx.x - 256, lane = ct & 31;
@@ -373,7 +380,7 @@ __device__ __forceinline__ bool tile_convert(const ChunkParams& p, const TileUni
         const int j = j0 + tile, st = j & (kMetaStages - 1);
         if (!v && !mbar_wait(&bars[kMetaFull + st], (j / kMetaStages) & 1)) return false;
         c.load(v ? p.V : p.K, meta + st, ct);
-        if (v) {
+        if (v && !FOLD) {
             __syncwarp();
             if (lane == 0) mbar_arrive(&bars[kMetaEmpty + st]);
         }
@@ -385,10 +392,15 @@ __device__ __forceinline__ bool tile_convert(const ChunkParams& p, const TileUni
         job(q, tile, v);
         const int j = j0 + tile, st = j & 1;
         if (j >= 2 && !mbar_wait(&bars[(v ? kVEmpty : kKEmpty) + st], ((j >> 1) - 1) & 1)) return false;
-        c.store(smem + (v ? S::kV : S::kK) + st * S::kRows, ct);
+        uint8_t* to = smem + (v ? S::kV : S::kK) + st * S::kRows;
+        if (FOLD && v) c.template store<true>(to, ct, meta[j & (kMetaStages - 1)].vs);
+        else c.template store<false>(to, ct, nullptr);
         fence_async_smem();
         __syncwarp();
-        if (lane == 0) mbar_arrive(&bars[(v ? kVFull : kKFull) + st]);
+        if (lane == 0) {
+            mbar_arrive(&bars[(v ? kVFull : kKFull) + st]);
+            if (FOLD && v) mbar_arrive(&bars[kMetaEmpty + (j & (kMetaStages - 1))]);
+        }
         return true;
     };
     Codes<D> a, b;
@@ -518,7 +530,7 @@ __device__ __forceinline__ float top32(uint32_t col, const float4* ks4, int lim)
 
 // Weights of 32 tokens with reference m: their sum onto `sum`, p vs 2^ve as fp16 pairs (and their rests). Returns
 // the largest u ks.
-template <bool MASK>
+template <bool MASK, bool FOLD>
 __device__ __forceinline__ float weights32(uint32_t col, const float4* ks4, const float4* vs4, int lim, float rf, float m,
                                            float2 (&sum)[2], uint32_t (&hi)[16], uint32_t* lo) {
     uint32_t s[32];
@@ -528,7 +540,7 @@ __device__ __forceinline__ float weights32(uint32_t col, const float4* ks4, cons
     float tm[2] = {-INFINITY, -INFINITY};
 #pragma unroll
     for (int k = 0; k < 8; ++k) {
-        const float4 kq = ks4[k], vq = vs4[k];
+        const float4 kq = ks4[k], vq = FOLD ? make_float4(1.f, 1.f, 1.f, 1.f) : vs4[k];
         float2 a = __fmul2_rn(make_float2(__uint_as_float(s[4 * k]), __uint_as_float(s[4 * k + 1])), make_float2(kq.x, kq.y));
         float2 b = __fmul2_rn(make_float2(__uint_as_float(s[4 * k + 2]), __uint_as_float(s[4 * k + 3])), make_float2(kq.z, kq.w));
         if (MASK) {
@@ -541,7 +553,7 @@ __device__ __forceinline__ float weights32(uint32_t col, const float4* ks4, cons
         const float2 pa = make_float2(ex2_fast(a.x), ex2_fast(a.y)), pb = make_float2(ex2_fast(b.x), ex2_fast(b.y));
         sum[0] = __fadd2_rn(sum[0], pa);
         sum[1] = __fadd2_rn(sum[1], pb);
-        const float2 x = __fmul2_rn(pa, make_float2(vq.x, vq.y)), y = __fmul2_rn(pb, make_float2(vq.z, vq.w));
+        const float2 x = FOLD ? pa : __fmul2_rn(pa, make_float2(vq.x, vq.y)), y = FOLD ? pb : __fmul2_rn(pb, make_float2(vq.z, vq.w));
         hi[2 * k] = pack_half(x.x, x.y);
         hi[2 * k + 1] = pack_half(y.x, y.y);
         if (lo) {
@@ -563,7 +575,7 @@ __device__ __forceinline__ bool both_here(uint64_t* bars, int& count) {
     return ok;
 }
 
-template <int D, int TERMS>
+template <int D, int TERMS, bool FOLD>
 __device__ __forceinline__ bool tile_softmax(const ChunkParams& p, const TileUnit& u, uint8_t* smem, uint32_t tmem, uint64_t* bars, int j0,
                                              int nu, int& ns, int& no, int& nm_sync) {
     using S = TileSmem<D>;
@@ -620,7 +632,7 @@ __device__ __forceinline__ bool tile_softmax(const ChunkParams& p, const TileUni
                 float top = -INFINITY;
 #pragma unroll
                 for (int q = 0; q < 4; ++q)
-                    top = fmaxf(top, weights32<false>(col_s + 32u * q, ks4 + 8 * q, vs4 + 8 * q, 0, rf, m, sum,
+                    top = fmaxf(top, weights32<false, FOLD>(col_s + 32u * q, ks4 + 8 * q, vs4 + 8 * q, 0, rf, m, sum,
                                                       *reinterpret_cast<uint32_t(*)[16]>(&pk[16 * q]), nullptr));
                 done = !__any_sync(0xffffffffu, top * rf > m + 8.f);
                 if (done) {
@@ -670,14 +682,14 @@ __device__ __forceinline__ bool tile_softmax(const ChunkParams& p, const TileUni
                     tmem_st16(col_s + 64u, rest[0]);
                     tmem_st16(col_s + 80u, rest[1]);
                     uint32_t last[16];
-                    if (masked) weights32<true>(col_s + 96u, ks4 + 24, vs4 + 24, lim - 96, rf, me, lp, hi, last);
-                    else weights32<false>(col_s + 96u, ks4 + 24, vs4 + 24, 0, rf, me, lp, hi, last);
+                    if (masked) weights32<true, FOLD>(col_s + 96u, ks4 + 24, vs4 + 24, lim - 96, rf, me, lp, hi, last);
+                    else weights32<false, FOLD>(col_s + 96u, ks4 + 24, vs4 + 24, 0, rf, me, lp, hi, last);
                     tmem_st16(col_s + 96u, rest[2]);
                     tmem_st16(col_s + 112u, last);
                 } else if (masked) {
-                    weights32<true>(col_s + 32u * q, ks4 + 8 * q, vs4 + 8 * q, lim - 32 * q, rf, me, lp, hi, lo);
+                    weights32<true, FOLD>(col_s + 32u * q, ks4 + 8 * q, vs4 + 8 * q, lim - 32 * q, rf, me, lp, hi, lo);
                 } else {
-                    weights32<false>(col_s + 32u * q, ks4 + 8 * q, vs4 + 8 * q, 0, rf, me, lp, hi, lo);
+                    weights32<false, FOLD>(col_s + 32u * q, ks4 + 8 * q, vs4 + 8 * q, 0, rf, me, lp, hi, lo);
                 }
                 tmem_st16(col_s + 16u * q, hi);
             }
@@ -762,7 +774,7 @@ __device__ __forceinline__ bool tile_softmax(const ChunkParams& p, const TileUni
     return !u.alt || both_here(bars, nm_sync);  // both have read both
 }
 
-template <int D, int TERMS>
+template <int D, int TERMS, bool FOLD>
 __global__ void __launch_bounds__(kThreads, 1) chunk_tile_kernel(const __grid_constant__ ChunkParams p) {
     using S = TileSmem<D>;
     extern __shared__ uint8_t tile_smem[];
@@ -802,7 +814,7 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_tile_kernel(const __grid_co
         int j = 0, nu = 0, ns = 0, no = 0, nm = 0;
         for (int unit = blockIdx.x; unit < units; unit += gridDim.x) {
             const TileUnit u = tile_unit<TERMS>(p, unit);
-            if (!tile_softmax<D, TERMS>(p, u, smem, tmem, bars, j, nu, ns, no, nm)) break;
+            if (!tile_softmax<D, TERMS, FOLD>(p, u, smem, tmem, bars, j, nu, ns, no, nm)) break;
             j += u.nt;
             nu += u.nt > 0;
         }
@@ -815,7 +827,7 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_tile_kernel(const __grid_co
         for (int unit = blockIdx.x; unit < units; unit += gridDim.x) {
             const TileUnit u = tile_unit<TERMS>(p, unit);
             if (u.nt == 0) continue;
-            if (!tile_convert<D, TERMS>(p, u, smem, bars, j, nu)) break;
+            if (!tile_convert<D, TERMS, FOLD>(p, u, smem, bars, j, nu)) break;
             j += u.nt;
             ++nu;
         }
@@ -848,9 +860,9 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_tile_kernel(const __grid_co
     }
 }
 
-template <int D, int TERMS>
+template <int D, int TERMS, bool FOLD>
 cudaError_t launch_tile(const ChunkParams& p, cudaStream_t st) {
-    auto kern = chunk_tile_kernel<D, TERMS>;
+    auto kern = chunk_tile_kernel<D, TERMS, FOLD>;
     static PerDeviceOnce once;
     cudaError_t e = once.run([kern] {
         return cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, TileSmem<D>::kBytes);
@@ -881,9 +893,9 @@ cudaError_t take_chunk_tile_status(int32_t* status) {
 }
 
 cudaError_t launch_chunk_tile(const ChunkParams& p, cudaStream_t st, int* launches) {
-    const bool two = p.tile_rows == 128;
-    const cudaError_t e = p.D == 128 ? (two ? launch_tile<128, 2>(p, st) : launch_tile<128, 1>(p, st))
-                                     : (two ? launch_tile<64, 2>(p, st) : launch_tile<64, 1>(p, st));
+    const bool two = p.tile_rows == 128, fold = !two && (p.flags & KVD_FLAG_OUT_BF16) != 0;
+    const cudaError_t e = p.D == 128 ? (two ? launch_tile<128, 2, false>(p, st) : fold ? launch_tile<128, 1, true>(p, st) : launch_tile<128, 1, false>(p, st))
+                                     : (two ? launch_tile<64, 2, false>(p, st) : fold ? launch_tile<64, 1, true>(p, st) : launch_tile<64, 1, false>(p, st));
     if (e == cudaSuccess) ++*launches;
     return e;
 }
