@@ -97,60 +97,100 @@ __global__ void __launch_bounds__(kAnyThreads) chunk_any_kernel(const ChunkParam
 }
 
 // ---------------------------------------------------------------- plan
-// Which kernel takes a request, and how its tokens are split: one CTA sums the
-// work of all requests (tokens times units), which gives the stretch that a
-// unit may have, then places every request's units and records by prefix sums.
-// A stretch is at least work / target, so split units are fewer than 2 target:
-// the room for their records. Bound: latency (loads, two sums, one scan).
+// Which kernel takes a request, and how its tokens are split: one CTA looks at
+// all requests and, for each kernel, at five stretches that a unit may have at
+// most: no limit, and the work (tokens times units) over 1, 2, 3 and 4 times
+// the CTAs that run at once (1 and 2 for many rows). It takes the one whose estimate is least,
+//   max(longest stretch, rounds of CTAs x mean stretch),
+// each stretch with what a unit costs beside its tokens, then places every
+// request's units and records by prefix sums. Split units are fewer than twice
+// the work over the stretch: the room for their records. Bound: latency (loads,
+// two rounds of sums, one scan).
+constexpr int kSpans = 5;
+// The records of many rows are large: those are split into twice the CTAs' units at most.
+__host__ __device__ constexpr int span_parts(int cls, int k) { return cls == kMany && k > 2 ? 2 : k; }
+
+struct ChunkShape {
+    int rows, units, len, cls;
+};
+
+__device__ __forceinline__ ChunkShape chunk_shape(const ChunkParams& p, int b) {
+    const ChunkRows r = chunk_rows(p, b);
+    ChunkShape s;
+    s.len = r.len;
+    s.rows = r.n * p.G;
+    s.cls = chunk_class(p, s.rows);
+    const int per = s.cls == 0 ? p.unit_rows[0] : s.cls == 1 ? p.unit_rows[1] : p.unit_rows[kMany];
+    s.units = (s.rows + per - 1) / per * p.Hkv;
+    return s;
+}
+
+__device__ __forceinline__ int chunk_step(int cls) { return cls == kMany ? kTile : kFewStep; }
+
 __global__ void __launch_bounds__(1024) chunk_plan_kernel(const ChunkParams p) {
-    __shared__ unsigned long long work[2];
-    __shared__ int sums[4][32];
+    __shared__ unsigned long long work[kClasses];
+    __shared__ int units_at[kClasses * kSpans], longest_at[kClasses * kSpans], span[kClasses];
+    __shared__ int sums[2 * kClasses][32];
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, nw = blockDim.x >> 5;
+    if (tid < kClasses) work[tid] = 0;
+    if (tid < kClasses * kSpans) units_at[tid] = longest_at[tid] = 0;
     grid_dependency_wait();
     allow_dependents();
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    if (tid < 2) work[tid] = 0;
     __syncthreads();
-    auto shape = [&](int b, int& rows, int& units, bool& few) {
-        const ChunkRows r = chunk_rows(p, b);
-        rows = r.n * p.G;
-        few = rows <= p.few_most;
-        units = (few ? (rows + kFewRows - 1) / kFewRows : (rows + p.tile_rows - 1) / p.tile_rows) * p.Hkv;
-        return r.len;
-    };
-    unsigned long long w[2] = {0, 0};
     for (int b = tid; b < p.B; b += blockDim.x) {
-        int rows, units;
-        bool few;
-        const int len = shape(b, rows, units, few);
-        w[few ? 0 : 1] += static_cast<unsigned long long>(units) * len;
-    }
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) w[i] += __shfl_xor_sync(0xffffffffu, w[i], o);
-        if (lane == 0 && w[i]) atomicAdd(&work[i], w[i]);
+        const ChunkShape s = chunk_shape(p, b);
+        if (s.units) atomicAdd(&work[s.cls], static_cast<unsigned long long>(s.units) * s.len);
     }
     __syncthreads();
-    auto span_of = [](unsigned long long x, int target, int least) {
-        const unsigned long long s = (x + target - 1) / target;
-        return static_cast<int>(min(max(s, static_cast<unsigned long long>(least)), 0x40000000ull));
+    auto span_of = [&](int cls, int k) {
+        if (k == 0) return 0x40000000;
+        const unsigned long long parts = static_cast<unsigned long long>(span_parts(cls, k)) * (cls == 0 ? p.ctas[0] : cls == 1 ? p.ctas[1] : p.ctas[kMany]);
+        const unsigned long long s = (work[cls] + parts - 1) / parts, least = cls == kMany ? kTileMinSpan : kFewMinSpan;
+        return static_cast<int>(min(max(s, least), 0x40000000ull));
     };
-    const int few_span = span_of(work[0], p.few_target, kFewMinSpan), tile_span = span_of(work[1], p.tile_target, kTileMinSpan);
-    int carry[4] = {0, 0, 0, 0};
+    for (int64_t i = tid; i < static_cast<int64_t>(p.B) * kSpans; i += blockDim.x) {  // a thread per request and stretch
+        const int b = static_cast<int>(i / kSpans), k = static_cast<int>(i - static_cast<int64_t>(b) * kSpans);
+        const ChunkShape s = chunk_shape(p, b);
+        if (s.units == 0) continue;
+        int each;
+        const int n = chunk_splits(s.len, span_of(s.cls, k), chunk_step(s.cls), each);
+        atomicAdd(&units_at[s.cls * kSpans + k], s.units * n);
+        atomicMax(&longest_at[s.cls * kSpans + k], min(each, s.len));
+    }
+    __syncthreads();
+    if (tid < kClasses) {
+        const float extra = tid == kMany ? kTileExtra : kFewExtra;
+        const int ctas = tid == 0 ? p.ctas[0] : tid == 1 ? p.ctas[1] : p.ctas[kMany];
+        int best = 0;
+        float least = INFINITY;
+        for (int k = 0; k < kSpans; ++k) {
+            const int units = max(1, units_at[tid * kSpans + k]);
+            const float mean = static_cast<float>(work[tid]) / static_cast<float>(units);
+            const float cost = fmaxf(longest_at[tid * kSpans + k] + extra, static_cast<float>((units + ctas - 1) / ctas) * (mean + extra));
+            if (cost < least) {
+                least = cost;
+                best = k;
+            }
+        }
+        span[tid] = span_of(tid, best);
+    }
+    __syncthreads();
+    int carry[2 * kClasses] = {};
     for (int b0 = 0; b0 < p.B; b0 += blockDim.x) {
         const int b = b0 + tid;
-        int x[4] = {0, 0, 0, 0};
+        int x[2 * kClasses] = {}, inc[2 * kClasses];
         if (b < p.B) {
-            int rows, units, each;
-            bool few;
-            const int len = shape(b, rows, units, few);
-            const int n = few ? chunk_splits(len, few_span, kFewStep, each) : chunk_splits(len, tile_span, kTile, each);
-            x[few ? 0 : 2] = units * n;
-            x[few ? 1 : 3] = n > 1 ? units * n : 0;
-        }
-        int inc[4];
+            const ChunkShape s = chunk_shape(p, b);
+            int each;
+            const int n = chunk_splits(s.len, span[s.cls], chunk_step(s.cls), each);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
+            for (int c = 0; c < kClasses; ++c) {
+                x[2 * c] = c == s.cls ? s.units * n : 0;
+                x[2 * c + 1] = c == s.cls && n > 1 ? s.units * n : 0;
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < 2 * kClasses; ++i) {
             inc[i] = x[i];
 #pragma unroll
             for (int o = 1; o < 32; o <<= 1) {
@@ -161,85 +201,93 @@ __global__ void __launch_bounds__(1024) chunk_plan_kernel(const ChunkParams p) {
         __syncthreads();
         if (lane == 31)
 #pragma unroll
-            for (int i = 0; i < 4; ++i) sums[i][warp] = inc[i];
+            for (int i = 0; i < 2 * kClasses; ++i) sums[i][warp] = inc[i];
         __syncthreads();
-        int32_t* const first[4] = {p.few_first, p.few_rec, p.tile_first, p.tile_rec};
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            int s = sums[i][lane];
+        for (int i = 0; i < 2 * kClasses; ++i) {
+            int s = lane < nw ? sums[i][lane] : 0;
 #pragma unroll
             for (int o = 1; o < 32; o <<= 1) {
                 const int y = __shfl_up_sync(0xffffffffu, s, o);
                 if (lane >= o) s += y;
             }
             const int upto = __shfl_sync(0xffffffffu, s, (warp - 1) & 31), all = __shfl_sync(0xffffffffu, s, 31);
-            if (b < p.B) first[i][b] = carry[i] + (warp > 0 ? upto : 0) + inc[i] - x[i];
+            int32_t* to = i & 1 ? p.rec[i >> 1] : p.first[i >> 1];
+            if (b < p.B) to[b] = carry[i] + (warp > 0 ? upto : 0) + inc[i] - x[i];
             carry[i] += all;
         }
     }
     if (tid == 0) {
-        p.few_first[p.B] = carry[0];
-        p.few_rec[p.B] = carry[1];
-        p.tile_first[p.B] = carry[2];
-        p.tile_rec[p.B] = carry[3];
-        *p.head = ChunkHead{carry[0], few_span, carry[2], tile_span, carry[1], carry[3], 0, 0};
+        ChunkHead h{};
+#pragma unroll
+        for (int c = 0; c < kClasses; ++c) {
+            p.first[c][p.B] = h.units[c] = carry[2 * c];
+            p.rec[c][p.B] = h.recs[c] = carry[2 * c + 1];
+            h.span[c] = span[c];
+        }
+        *p.head = h;
     }
 }
 
 // ------------------------------------------------------------- split work
-// Merges the records of units that were split along the tokens: 16 rows a CTA,
-// out = sum_s 2^(m_s - M) o_s / sum_s 2^(m_s - M) l_s.
+// Merges the records of units that were split along the tokens: eight rows a
+// CTA, out = sum_s 2^(m_s - M) o_s / sum_s 2^(m_s - M) l_s.
+constexpr int kMergeRows = 8;
+
 template <int D>
 __global__ void __launch_bounds__(128) chunk_merge_kernel(const ChunkParams p) {
     grid_dependency_wait();
     allow_dependents();
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int few = p.head->few_recs, groups = p.tile_rows / kFewRows;
-    const int64_t units = few + static_cast<int64_t>(p.head->tile_recs) * groups;
-    for (int64_t u = blockIdx.x; u < units; u += gridDim.x) {
-        const bool is_few = u < few;
-        const int slot = is_few ? static_cast<int>(u) : static_cast<int>((u - few) / groups);
-        const int group = is_few ? 0 : static_cast<int>(u - few - static_cast<int64_t>(slot) * groups);
-        const int32_t* first = is_few ? p.few_rec : p.tile_rec;
-        const int b = warp_find(first, p.B, slot);
-        const ChunkRows R = chunk_rows(p, b);
-        const int unit_rows = is_few ? kFewRows : p.tile_rows;
-        const int rows = R.n * p.G, nrb = (rows + unit_rows - 1) / unit_rows;
-        int each;
-        const int nsplit = is_few ? chunk_splits(R.len, p.head->few_span, kFewStep, each)
-                                  : chunk_splits(R.len, p.head->tile_span, kTile, each);
-        const int local = slot - first[b], item = local / nsplit;
-        if (local != item * nsplit) continue;  // the first record of a unit stands for all
-        const int hk = item / nrb, rb = item - hk * nrb;
-        const float* o = is_few ? p.few_o : p.tile_o;
-        const float2* ml = is_few ? p.few_ml : p.tile_ml;
-        for (int r = group * kFewRows + warp; r < (group + 1) * kFewRows; r += 4) {
-            const int row = rb * unit_rows + r;
-            if (row >= rows) break;
-            const int64_t at = static_cast<int64_t>(slot) * unit_rows + r;
-            float M = -INFINITY;
-            for (int s = lane; s < nsplit; s += 32) M = fmaxf(M, ml[at + static_cast<int64_t>(s) * unit_rows].x);
+    int64_t before = 0;  // units of the classes in front
 #pragma unroll
-            for (int i = 16; i > 0; i >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, i));
-            float L = 0.f, acc[D / 32] = {};
+    for (int c = 0; c < kClasses; ++c) {
+        const int unit_rows = p.unit_rows[c], groups = unit_rows / kMergeRows, span = p.head->span[c];
+        const int64_t units = static_cast<int64_t>(p.head->recs[c]) * groups;
+        // every CTA goes on in the next class where it stopped in this one
+        int64_t u = blockIdx.x + (gridDim.x - before % gridDim.x);
+        if (u >= gridDim.x) u -= gridDim.x;
+        for (; u < units; u += gridDim.x) {
+            const int slot = static_cast<int>(u / groups), group = static_cast<int>(u - static_cast<int64_t>(slot) * groups);
+            const int b = warp_find(p.rec[c], p.B, slot);
+            const ChunkRows R = chunk_rows(p, b);
+            const int rows = R.n * p.G, nrb = (rows + unit_rows - 1) / unit_rows;
+            int each;
+            const int nsplit = chunk_splits(R.len, span, chunk_step(c), each);
+            const int local = slot - p.rec[c][b], item = local / nsplit;
+            if (local != item * nsplit) continue;  // the first record of a unit stands for all
+            const int hk = item / nrb, rb = item - hk * nrb;
+            const float* o = p.part_o[c];
+            const float2* ml = p.part_ml[c];
+            for (int r = group * kMergeRows + warp; r < (group + 1) * kMergeRows; r += 4) {
+                const int row = rb * unit_rows + r;
+                if (row >= rows) break;
+                const int64_t at = static_cast<int64_t>(slot) * unit_rows + r;
+                float M = -INFINITY;
+                for (int s = lane; s < nsplit; s += 32) M = fmaxf(M, ml[at + static_cast<int64_t>(s) * unit_rows].x);
+#pragma unroll
+                for (int i = 16; i > 0; i >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, i));
+                float L = 0.f, acc[D / 32] = {};
 #pragma unroll 4
-            for (int s = 0; s < nsplit; ++s) {
-                const int64_t rec = at + static_cast<int64_t>(s) * unit_rows;
-                const float2 v = ml[rec];
-                const float f = v.x == -INFINITY ? 0.f : exp2f(v.x - M);
-                L = fmaf(v.y, f, L);
+                for (int s = 0; s < nsplit; ++s) {
+                    const int64_t rec = at + static_cast<int64_t>(s) * unit_rows;
+                    const float2 v = ml[rec];
+                    const float f = v.x == -INFINITY ? 0.f : exp2f(v.x - M);
+                    L = fmaf(v.y, f, L);
 #pragma unroll
-                for (int d = 0; d < D / 32; ++d) {
-                    const float x = o[rec * D + d * 32 + lane];
-                    if (f != 0.f) acc[d] = fmaf(x, f, acc[d]);
+                    for (int d = 0; d < D / 32; ++d) {
+                        const float x = o[rec * D + d * 32 + lane];
+                        if (f != 0.f) acc[d] = fmaf(x, f, acc[d]);
+                    }
                 }
-            }
-            const int i = static_cast<int>(p.by_g.div(static_cast<uint32_t>(row))), g = row - i * p.G;
-            const int64_t o_at = static_cast<int64_t>(R.t0 + i) * p.o_st + static_cast<int64_t>(hk * p.G + g) * p.o_sh;
-            const float inv = L == 0.f ? 0.f : 1.f / L;  // no token in sight
+                const int i = static_cast<int>(p.by_g.div(static_cast<uint32_t>(row))), g = row - i * p.G;
+                const int64_t o_at = static_cast<int64_t>(R.t0 + i) * p.o_st + static_cast<int64_t>(hk * p.G + g) * p.o_sh;
+                const float inv = L == 0.f ? 0.f : 1.f / L;  // no token in sight
 #pragma unroll
-            for (int d = 0; d < D / 32; ++d) store_out(p.out, o_at + d * 32 + lane, acc[d] * inv, p.flags);
+                for (int d = 0; d < D / 32; ++d) store_out(p.out, o_at + d * 32 + lane, acc[d] * inv, p.flags);
+            }
         }
+        before += units;
     }
 }
 
@@ -263,34 +311,38 @@ bool tensor_shape(const kvd_paged_prefill_desc& d) {
            ((d.kv_stride_block | d.kv_stride_h | d.kv_stride_t) & 15) == 0;
 }
 
+// Rows of a KV head up to which a request has few.
+constexpr int kFewMost = 64;
+
+// Whether a request of the call may be of a class, by what the host knows.
+bool has_class(const kvd_paged_prefill_desc& d, int cls) {
+    const int64_t G = d.num_q_heads / d.num_kv_heads, most = d.num_rows * G;
+    return cls == 0 ? G <= 8 : cls == 1 ? most > 8 && G <= kFewMost : most > kFewMost;
+}
+
 int64_t round16(int64_t x) { return (x + 15) & ~static_cast<int64_t>(15); }
 
-// Lays the workspace out from `base` (0: to learn its size); returns the end.
+// Lays the workspace out from `base` (nullptr: to learn its size, which is the same for all types of rows and
+// output); returns its bytes.
 int64_t lay_out(const kvd_paged_prefill_desc& d, ChunkParams* p, uint8_t* base) {
     const int sms = device_sm_count();
     const int64_t G = d.num_q_heads / d.num_kv_heads, D = d.head_dim, entries = static_cast<int64_t>(d.batch) + 1;
     const int64_t cap = static_cast<int64_t>(d.max_blocks_per_seq) * d.block_size;
-    p->few_target = 2 * sms;
-    p->tile_target = sms;
     constexpr uint32_t q16 = KVD_FLAG_Q_BF16 | KVD_FLAG_Q_F16, o16 = KVD_FLAG_OUT_BF16 | KVD_FLAG_OUT_F16;
-    p->tile_rows = (d.flags & q16) != 0 && (d.flags & o16) != 0 ? 256 : 128;
-    p->few_most = 32;
-    const bool tiles = static_cast<int64_t>(d.num_rows) * G > p->few_most;
-    auto records = [&](int64_t target, int64_t unit_rows, int64_t least) {
-        // no more units than rows give, and no more splits of each than the longest length gives
+    p->unit_rows[0] = 8;
+    p->unit_rows[1] = 16;
+    p->unit_rows[kMany] = (d.flags & q16) != 0 && (d.flags & o16) != 0 ? 256 : 128;
+    p->ctas[0] = sms * chunk_few_ctas(static_cast<int>(D), 0);
+    p->ctas[1] = sms * chunk_few_ctas(static_cast<int>(D), 1);
+    p->ctas[kMany] = sms;
+    p->few_most = kFewMost;
+    // no more units than rows give, and no more splits of each than the longest length gives
+    auto records = [&](int cls, int64_t unit_rows) -> int64_t {
+        const int64_t least = cls == kMany ? kTileMinSpan : kFewMinSpan;
         const int64_t units = (d.num_rows * G / unit_rows + (d.batch < d.num_rows ? d.batch : d.num_rows)) * d.num_kv_heads;
-        const int64_t splits = (cap + least - 1) / least;
-        const int64_t most = units * splits;
-        return splits <= 1 ? 0 : most < 2 * target ? most : 2 * target;
+        const int64_t splits = (cap + least - 1) / least, most = units * splits, room = 2LL * span_parts(cls, kSpans - 1) * p->ctas[cls];
+        return splits <= 1 || !has_class(d, cls) ? 0 : most < room ? most : room;
     };
-    p->max_few_recs = static_cast<int>(records(p->few_target, kFewRows, kFewMinSpan));
-    p->max_tile_recs = tiles ? static_cast<int>(records(p->tile_target, p->tile_rows, kTileMinSpan)) : 0;
-    // the size is the same for all types of rows and output
-    int64_t tile_rows = 0;
-    for (int64_t r = 128; tiles && r <= 256; r += 128) {
-        const int64_t x = r * records(p->tile_target, r, kTileMinSpan);
-        tile_rows = x > tile_rows ? x : tile_rows;
-    }
     int64_t at = 0;
     auto take = [&](int64_t bytes) {
         uint8_t* here = base + at;
@@ -298,14 +350,19 @@ int64_t lay_out(const kvd_paged_prefill_desc& d, ChunkParams* p, uint8_t* base) 
         return here;
     };
     p->head = reinterpret_cast<ChunkHead*>(take(sizeof(ChunkHead)));
-    p->few_first = reinterpret_cast<int32_t*>(take(4 * entries));
-    p->few_rec = reinterpret_cast<int32_t*>(take(4 * entries));
-    p->tile_first = reinterpret_cast<int32_t*>(take(4 * entries));
-    p->tile_rec = reinterpret_cast<int32_t*>(take(4 * entries));
-    p->few_o = reinterpret_cast<float*>(take(4 * D * kFewRows * p->max_few_recs));
-    p->few_ml = reinterpret_cast<float2*>(take(8 * kFewRows * static_cast<int64_t>(p->max_few_recs)));
-    p->tile_o = reinterpret_cast<float*>(take(4 * D * tile_rows));
-    p->tile_ml = reinterpret_cast<float2*>(take(8 * tile_rows));
+    p->records = false;
+    for (int c = 0; c < kClasses; ++c) {
+        p->first[c] = reinterpret_cast<int32_t*>(take(4 * entries));
+        p->rec[c] = reinterpret_cast<int32_t*>(take(4 * entries));
+        int64_t rows = records(c, p->unit_rows[c]) * p->unit_rows[c];
+        if (c == kMany) {
+            const int64_t x = 128 * records(c, 128), y = 256 * records(c, 256);
+            rows = x > y ? x : y;
+        }
+        p->part_o[c] = reinterpret_cast<float*>(take(4 * D * rows));
+        p->part_ml[c] = reinterpret_cast<float2*>(take(8 * rows));
+        p->records |= rows > 0;
+    }
     return at;
 }
 
@@ -373,16 +430,15 @@ extern "C" cudaError_t kvd_paged_prefill_launch(const kvd_paged_prefill_desc* d,
         return e;
     }
     lay_out(*d, &p, static_cast<uint8_t*>(workspace));
-    e = launch_after(chunk_plan_kernel, 1, 1024, 0, stream, p);
+    e = launch_after(chunk_plan_kernel, 1, p.B <= 256 ? 256 : 1024, 0, stream, p);
     if (e != cudaSuccess) return e;
     ++*launches;
-    e = launch_chunk_few(p, stream, launches);
-    if (e != cudaSuccess) return e;
-    if (static_cast<int64_t>(p.T) * p.G > p.few_most) {  // a request may have many rows
-        e = launch_chunk_tile(p, stream, launches);
+    for (int c = 0; c < kClasses; ++c) {
+        if (!has_class(*d, c)) continue;
+        e = c == kMany ? launch_chunk_tile(p, stream, launches) : launch_chunk_few(p, c, stream, launches);
         if (e != cudaSuccess) return e;
     }
-    if (p.max_few_recs + p.max_tile_recs == 0) return cudaSuccess;
+    if (!p.records) return cudaSuccess;
     const unsigned grid = 8u * device_sm_count();
     e = p.D == 128 ? launch_after(chunk_merge_kernel<128>, grid, 128, 0, stream, p)
                    : launch_after(chunk_merge_kernel<64>, grid, 128, 0, stream, p);

@@ -9,12 +9,17 @@
 
 namespace kvd {
 
-// Work of a call, in the workspace: a header, then six arrays of B + 1 entries.
+// Requests by their rows (new tokens times heads of a group) of a KV head: up to 8, few, many. Each class has a
+// kernel of its own.
+constexpr int kClasses = 3;
+constexpr int kMany = 2;
+
+// Work of a call, in the workspace: this, then for each class two arrays of B + 1 entries.
 struct ChunkHead {
-    int32_t few_units, few_span;    // units of the kernel for few rows, and tokens of a split at most
-    int32_t tile_units, tile_span;  // units of the kernel for many rows, and tokens of a split at most
-    int32_t few_recs, tile_recs;    // records of split work
-    int32_t ticket, pad;
+    int32_t units[kClasses];  // units: blocks of rows x KV heads x stretches of tokens
+    int32_t span[kClasses];   // tokens of a stretch at most
+    int32_t recs[kClasses];   // records of units whose tokens are split
+    int32_t pad[3];
 };
 
 struct ChunkParams {
@@ -36,24 +41,21 @@ struct ChunkParams {
     int vec_q, vec_out;  // rows on 16-byte boundaries
     // plan
     ChunkHead* head;
-    int32_t* few_first;   // [B + 1] units in front of request b's
-    int32_t* few_rec;     // [B + 1] records in front of request b's
-    int32_t* tile_first;  // the same for the requests with many rows
-    int32_t* tile_rec;
-    float* few_o;   // records: [slot][kFewRows][D] sums of weighted values
-    float2* few_ml; // and [slot][kFewRows] (reference in base 2, sum of weights)
-    float* tile_o;
-    float2* tile_ml;
-    int few_most;      // rows (of one KV head) up to which a request goes to the kernel for few rows
-    int tile_rows;     // rows of a unit of the kernel for many rows
-    int few_target, tile_target;  // units that splitting aims at
-    int max_few_recs, max_tile_recs;
+    int32_t* first[kClasses];   // [B + 1] units in front of request b's
+    int32_t* rec[kClasses];     // [B + 1] records in front of request b's
+    float* part_o[kClasses];    // records: [slot][unit_rows][D] sums of weighted values
+    float2* part_ml[kClasses];  // and [slot][unit_rows] (reference in base 2, sum of weights)
+    int unit_rows[kClasses];
+    int ctas[kClasses];         // CTAs that run at once
+    int few_most;               // rows up to which a request has few
+    bool records;               // some unit may be split
 };
 
-constexpr int kFewRows = 16;     // rows of a unit of the kernel for few rows
-constexpr int kFewStep = 32;     // tokens of a step of that kernel
+constexpr int kFewStep = 32;     // tokens of a step of the kernels for few rows
 constexpr int kFewMinSpan = 256; // tokens that a split has at least
 constexpr int kTileMinSpan = 512;
+// What a unit costs beside its tokens, in tokens.
+constexpr float kFewExtra = 200.f, kTileExtra = 400.f;
 constexpr int kTile = 128;       // tokens of a tile of the kernel for many rows
 
 // Rows [t0, t0 + n) of request b and its tokens.
@@ -73,6 +75,8 @@ __device__ __forceinline__ ChunkRows chunk_rows(const ChunkParams& p, int b) {
 __device__ __forceinline__ int chunk_sees(const ChunkParams& p, const ChunkRows& r, int i) {
     return p.causal ? max(0, min(r.len, r.len - r.n + i + 1)) : r.len;
 }
+
+__device__ __forceinline__ int chunk_class(const ChunkParams& p, int rows) { return rows <= 8 ? 0 : rows <= p.few_most ? 1 : kMany; }
 
 // Splits of a request's tokens, and the tokens of each (a multiple of `step`).
 __device__ __forceinline__ int chunk_splits(int len, int span, int step, int& each) {
@@ -124,7 +128,8 @@ __device__ __forceinline__ int fit_exponent(float most, int top) {
     return min(max(top - (e - 126), -126), 126);
 }
 
-cudaError_t launch_chunk_few(const ChunkParams& p, cudaStream_t st, int* launches);
+cudaError_t launch_chunk_few(const ChunkParams& p, int cls, cudaStream_t st, int* launches);
+int chunk_few_ctas(int D, int cls);  // per SM
 cudaError_t launch_chunk_tile(const ChunkParams& p, cudaStream_t st, int* launches);
 
 }  // namespace kvd

@@ -2,18 +2,21 @@
 // requests with few rows a KV head (single tokens, drafted tokens, short
 // chunks): bound by the cache's bytes.
 //
-// A unit is (request, 16 rows of a KV head, stretch of tokens); its rows are
-// the request's tokens times the group's heads, so a token's codes are read once
-// for up to 16 of them. Each of the CTA's warps walks every fourth step of 32
+// A unit is (request, 8 or 16 rows of a KV head, stretch of tokens); its rows
+// are the request's tokens times the group's heads, so a token's codes are read
+// once for all of them. Each of the CTA's warps walks every fourth step of 32
 // tokens with its own running maximum, sum and output: with s_j = (q . K_j)
 // ks_j scale in base 2, p_j = 2^(s_j - m),
 //   l = sum p_j,  o = sum (p_j vs_j) V_j,
 // and the four are merged at the end. Codes come through a ring in shared memory
-// that only this warp uses (16-byte cp.async, three steps ahead), are widened to
-// fp16 exactly and multiplied with mma.m16n8k16: 16 rows are all that a unit has,
-// where tcgen05's smallest tile is 64. The order of dims in q . K, and of
-// dims over the output's columns, is whatever makes a lane's operands neighbours
-// in memory; the scores' accumulators are the weights' operand as they lie.
+// that only this warp uses (16-byte cp.async, a step or two ahead), are widened
+// to fp16 exactly and multiplied with mma.m16n8k16, tokens and then dims as its
+// 16 rows and the queries' rows as its 8 columns: S^T = K q^T, O^T = V^T P^T (the
+// smallest tile of tcgen05 has 64). The order of dims within a product is
+// whatever makes a lane's operands neighbours in memory, and movmatrix turns the
+// weights into the second product's operand. Requests of up to 8 rows have
+// a kernel of their own, which holds half the output in registers, so more warps
+// fit beside each other.
 #include "kvd_chunk.cuh"
 #include "kvd_decode.cuh"
 #include "kvd_tc.cuh"
@@ -23,8 +26,6 @@ namespace {
 
 constexpr int kFewWarps = 4;
 constexpr int kStep = kFewStep;
-constexpr int kStages = 3;  // steps of a warp's ring
-
 __device__ __forceinline__ void mma_16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
     asm volatile(
         "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
@@ -46,14 +47,26 @@ __device__ __forceinline__ void async_wait() {
     asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
 }
 
-template <int D>
+// NR: 8-row groups of a unit. Stages of a warp's ring, and CTAs of an SM, are what 227 KB of shared memory and 64 K
+// registers hold.
+template <int D, int NR>
 struct FewSmem {
-    static constexpr int kCodes = kStep * D;                // one of K or V
+    static constexpr int kRows = 8 * NR;
+    static constexpr int kCtas = NR == 2 ? 2 : D == 128 ? 3 : 4;
+    static constexpr int kStages = NR == 1 && D == 128 ? 2 : 3;  // steps
+    static constexpr int kCodes = kStep * D;                     // of K or V
     static constexpr int kStage = 2 * kCodes + 2 * kStep * 4;
     static constexpr int kRing = kFewWarps * kStages * kStage;
-    static constexpr int kMerge = kFewWarps * kFewRows * (D + 4) * 4;  // after the ring is done with
+    static constexpr int kMerge = kFewWarps * kRows * (D + 4) * 4;  // after the ring is done with
     static constexpr int kBytes = kRing > kMerge ? kRing : kMerge;
 };
+
+// The transposed 8 x 8 matrix of fp16 pairs that the warp holds.
+__device__ __forceinline__ uint32_t transposed(uint32_t x) {
+    uint32_t y;
+    asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+    return y;
+}
 
 // Places of 16-byte chunk c of token row r in a stage, chosen so that the eight lanes that read together meet
 // eight different places: rows 2i and 2i+1 for K, rows 0, 2, 4 and 6 for V.
@@ -62,48 +75,42 @@ __device__ __forceinline__ int k_at(int r, int c) { return r * D + (D == 128 ? (
 template <int D>
 __device__ __forceinline__ int v_at(int r, int c) { return r * D + (D == 128 ? (c ^ (r & 6)) : (c ^ ((r >> 1) & 3))) * 16; }
 
-template <int D, int NQ, int NP>
-__global__ void __launch_bounds__(kFewWarps * 32, 2) chunk_few_kernel(const ChunkParams p) {
+template <int D, int NR, int NQ, int NP>
+__global__ void __launch_bounds__(kFewWarps * 32, FewSmem<D, NR>::kCtas) chunk_few_kernel(const ChunkParams p) {
     extern __shared__ __align__(16) uint8_t few_smem[];
     constexpr int KS = D / 16;      // steps of 16 dims of a product
     constexpr int CH = D / 64;      // 16-byte chunks of a K row that a lane holds
     constexpr int PER = D / 16;     // 16-byte chunks of a row
     constexpr int COPIES = kStep * PER / 32;  // chunks of K, and of V, that a lane copies
-    using S = FewSmem<D>;
+    constexpr int CLS = NR - 1;
+    using S = FewSmem<D, NR>;
+    constexpr int ROWS = S::kRows, STAGES = S::kStages;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, quad = lane >> 2, c = lane & 3;
-    uint8_t* ring = few_smem + warp * kStages * S::kStage;
+    uint8_t* ring = few_smem + warp * STAGES * S::kStage;
     grid_dependency_wait();
     allow_dependents();
-    const int units = p.head->few_units, span = p.head->few_span;
+    const int units = p.head->units[CLS], span = p.head->span[CLS];
     for (int unit = blockIdx.x; unit < units; unit += gridDim.x) {
-        const int b = warp_find(p.few_first, p.B, unit);
+        const int b = warp_find(p.first[CLS], p.B, unit);
         const ChunkRows R = chunk_rows(p, b);
         int each;
-        const int rows = R.n * p.G, nrb = (rows + kFewRows - 1) / kFewRows, nsplit = chunk_splits(R.len, span, kStep, each);
-        int rest = unit - p.few_first[b];
+        const int rows = R.n * p.G, nrb = (rows + ROWS - 1) / ROWS, nsplit = chunk_splits(R.len, span, kStep, each);
+        int rest = unit - p.first[CLS][b];
         const int rb = rest % nrb;
         rest /= nrb;
         const int hk = rest % p.Hkv, split = rest / p.Hkv;
-        // the two rows of this lane: token of the request, head of the group, tokens that it sees
-        int sees[2];
-        int64_t q_at[2];
-        bool there[2];
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-            const int r = rb * kFewRows + quad + 8 * e;
-            const int i = static_cast<int>(p.by_g.div(static_cast<uint32_t>(r))), g = r - i * p.G;
-            there[e] = r < rows;
-            sees[e] = chunk_sees(p, R, min(i, R.n - 1));  // rows that are not there see what the last one does
-            q_at[e] = static_cast<int64_t>(R.t0 + i) * p.q_st + static_cast<int64_t>(hk * p.G + g) * p.q_sh;
-        }
-        const int last_row = min(rows, (rb + 1) * kFewRows) - 1;
+        const int last_row = min(rows, (rb + 1) * ROWS) - 1;
         const int most = chunk_sees(p, R, static_cast<int>(p.by_g.div(static_cast<uint32_t>(last_row))));
-        const int least = chunk_sees(p, R, static_cast<int>(p.by_g.div(static_cast<uint32_t>(rb * kFewRows))));
+        const int least = chunk_sees(p, R, static_cast<int>(p.by_g.div(static_cast<uint32_t>(rb * ROWS))));
         const int begin = split * each, end = min(min(begin + each, R.len), most);
         // ---- tokens into the ring. Lane l looks up token l of the step that is copied next.
         const int steps = end > begin ? (end - begin + kStep - 1) / kStep : 0;
         const int mine = steps > warp ? (steps - warp + kFewWarps - 1) / kFewWarps : 0;
         const int32_t* table = p.table + b * p.bt_stride;
+        const int8_t* K = p.K + hk * p.kv_sh;
+        const int8_t* V = p.V + hk * p.kv_sh;
+        const float* ks = p.ks + hk * p.sc_sh;
+        const float* vs = p.vs + hk * p.sc_sh;
         auto look_up = [&](int k, int& off) {  // block of this lane's token of its k-th step, -1: none
             const int t = begin + (warp + k * kFewWarps) * kStep + lane;
             if (k >= mine || t >= end) return -1;
@@ -117,65 +124,65 @@ __global__ void __launch_bounds__(kFewWarps * 32, 2) chunk_few_kernel(const Chun
         int next_off = 0, next_id = look_up(0, next_off);
         auto fetch = [&](int k) {
             if (k < mine) {
-                uint8_t* st = ring + (k % kStages) * S::kStage;
-                const int64_t row = next_id < 0 ? -1 : next_id * p.kv_sblk + hk * p.kv_sh + next_off * p.kv_st;
-                const int64_t sc = next_id < 0 ? 0 : next_id * p.sc_sblk + hk * p.sc_sh + next_off;
+                uint8_t* st = ring + (k % STAGES) * S::kStage;
+                // where there is no token its scales are zeros, and any codes do
+                const int id = max(next_id, 0), off = next_id < 0 ? 0 : next_off;
+                const int64_t row = id * p.kv_sblk + off * p.kv_st, sc = id * p.sc_sblk + off;
 #pragma unroll
                 for (int u = 0; u < COPIES; ++u) {
                     const int i = lane + 32 * u, r = i / PER, ch = i % PER;
-                    const int64_t at = __shfl_sync(0xffffffffu, row, r);
-                    const bool ok = at >= 0;
-                    const int64_t from = (ok ? at : 0) + ch * 16;
-                    async_copy<16>(st + k_at<D>(r, ch), p.K + from, ok);
-                    async_copy<16>(st + S::kCodes + v_at<D>(r, ch), p.V + from, ok);
+                    const int64_t at = __shfl_sync(0xffffffffu, row, r) + ch * 16;
+                    async_copy<16>(st + k_at<D>(r, ch), K + at, true);
+                    async_copy<16>(st + S::kCodes + v_at<D>(r, ch), V + at, true);
                 }
                 float* scales = reinterpret_cast<float*>(st + 2 * S::kCodes);
-                async_copy<4>(scales + lane, p.ks + sc, next_id >= 0);
-                async_copy<4>(scales + kStep + lane, p.vs + sc, next_id >= 0);
+                async_copy<4>(scales + lane, ks + sc, next_id >= 0);
+                async_copy<4>(scales + kStep + lane, vs + sc, next_id >= 0);
                 next_id = look_up(k + 1, next_off);
             }
             async_commit();
         };
 #pragma unroll 1
-        for (int k = 0; k < kStages - 1; ++k) fetch(k);
-        // ---- queries: this lane's dims of its rows, a power of two times them so that fp16 holds them
-        uint32_t qa[NQ][KS][4];
-        float rf[2];
+        for (int k = 0; k < STAGES - 1; ++k) fetch(k);
+        // ---- queries: this lane's dims of row quad of each group, a power of two times them so that fp16 holds them
+        uint32_t qb[NQ][NR][KS][2];
+        float factor[NR];  // what the scores of row quad are multiplied with instead
 #pragma unroll
-        for (int e = 0; e < 2; ++e) {
+        for (int e = 0; e < NR; ++e) {
+            const int r = rb * ROWS + 8 * e + quad;
+            const int i = static_cast<int>(p.by_g.div(static_cast<uint32_t>(r))), g = r - i * p.G;
+            const int64_t q_at = static_cast<int64_t>(R.t0 + i) * p.q_st + static_cast<int64_t>(hk * p.G + g) * p.q_sh;
             float x[CH * 16];
 #pragma unroll
-            for (int h = 0; h < CH; ++h)
-#pragma unroll
-                for (int d = 0; d < 16; ++d) x[h * 16 + d] = 0.f;
-            if (there[e]) {
+            for (int d = 0; d < CH * 16; ++d) x[d] = 0.f;
+            if (r < rows) {
                 if (p.vec_q) {
 #pragma unroll
                     for (int h = 0; h < CH; ++h) {
-                        const int64_t at = q_at[e] + h * 64 + c * 16;
+                        const int64_t at = q_at + h * 64 + c * 16;
                         if constexpr (NQ == 2) {
                             const float4* src = reinterpret_cast<const float4*>(static_cast<const float*>(p.Q) + at);
 #pragma unroll
-                            for (int i = 0; i < 4; ++i) {
-                                const float4 v = src[i];
-                                x[h * 16 + 4 * i] = v.x; x[h * 16 + 4 * i + 1] = v.y;
-                                x[h * 16 + 4 * i + 2] = v.z; x[h * 16 + 4 * i + 3] = v.w;
+                            for (int y = 0; y < 4; ++y) {
+                                const float4 v = src[y];
+                                x[h * 16 + 4 * y] = v.x; x[h * 16 + 4 * y + 1] = v.y;
+                                x[h * 16 + 4 * y + 2] = v.z; x[h * 16 + 4 * y + 3] = v.w;
                             }
                         } else {
                             const uint4* src = reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p.Q) + at);
 #pragma unroll
-                            for (int i = 0; i < 2; ++i) {
-                                const uint4 v = src[i];
+                            for (int y = 0; y < 2; ++y) {
+                                const uint4 v = src[y];
                                 const uint32_t w[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
-                                for (int y = 0; y < 4; ++y) {
+                                for (int z = 0; z < 4; ++z) {
                                     float2 f;
                                     if (p.flags & KVD_FLAG_Q_BF16)
-                                        f = make_float2(__uint_as_float(w[y] << 16), __uint_as_float(w[y] & 0xffff0000u));
+                                        f = make_float2(__uint_as_float(w[z] << 16), __uint_as_float(w[z] & 0xffff0000u));
                                     else
-                                        f = __half22float2(*reinterpret_cast<const __half2*>(&w[y]));
-                                    x[h * 16 + 8 * i + 2 * y] = f.x;
-                                    x[h * 16 + 8 * i + 2 * y + 1] = f.y;
+                                        f = __half22float2(*reinterpret_cast<const __half2*>(&w[z]));
+                                    x[h * 16 + 8 * y + 2 * z] = f.x;
+                                    x[h * 16 + 8 * y + 2 * z + 1] = f.y;
                                 }
                             }
                         }
@@ -184,7 +191,7 @@ __global__ void __launch_bounds__(kFewWarps * 32, 2) chunk_few_kernel(const Chun
 #pragma unroll
                     for (int h = 0; h < CH; ++h)
 #pragma unroll
-                        for (int d = 0; d < 16; ++d) x[h * 16 + d] = load_q(p.Q, q_at[e] + h * 64 + c * 16 + d, p.flags);
+                        for (int d = 0; d < 16; ++d) x[h * 16 + d] = load_q(p.Q, q_at + h * 64 + c * 16 + d, p.flags);
                 }
             }
             float top = 0.f;
@@ -194,121 +201,152 @@ __global__ void __launch_bounds__(kFewWarps * 32, 2) chunk_few_kernel(const Chun
             top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
             const int k = fit_exponent(top, 15);  // below 2^15: products of 128 dims stay far from fp32's end
             const float f = pow2i(k);
-            rf[e] = p.qscale * pow2i(-k);
+            factor[e] = p.qscale * pow2i(-k);
 #pragma unroll
             for (int s = 0; s < KS; ++s) {  // a word of four codes is a step: even dims in one pair, odd ones in the other
                 const float* y = x + s * 4;
-                const uint32_t ev = pack_half(y[0] * f, y[2] * f), od = pack_half(y[1] * f, y[3] * f);
-                qa[0][s][e] = ev;
-                qa[0][s][2 + e] = od;
+                qb[0][e][s][0] = pack_half(y[0] * f, y[2] * f);
+                qb[0][e][s][1] = pack_half(y[1] * f, y[3] * f);
                 if constexpr (NQ == 2) {
-                    qa[1][s][e] = pack_rest(y[0] * f, y[2] * f, ev);
-                    qa[1][s][2 + e] = pack_rest(y[1] * f, y[3] * f, od);
+                    qb[1][e][s][0] = pack_rest(y[0] * f, y[2] * f, qb[0][e][s][0]);
+                    qb[1][e][s][1] = pack_rest(y[1] * f, y[3] * f, qb[0][e][s][1]);
                 }
             }
         }
-        // ---- the walk
-        float o[D / 8][4];
+        // the columns of this lane in the products: rows 2c and 2c + 1 of each group
+        float rf[NR][2], m[NR][2], l[NR][2];
+        int sees[NR][2];
 #pragma unroll
-        for (int j = 0; j < D / 8; ++j) o[j][0] = o[j][1] = o[j][2] = o[j][3] = 0.f;
-        float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+        for (int e = 0; e < NR; ++e)
+#pragma unroll
+            for (int y = 0; y < 2; ++y) {
+                rf[e][y] = __shfl_sync(0xffffffffu, factor[e], 4 * (2 * c + y));
+                const int i = static_cast<int>(p.by_g.div(static_cast<uint32_t>(rb * ROWS + 8 * e + 2 * c + y)));
+                // rows that are not there see what the last one does
+                sees[e][y] = min(end, chunk_sees(p, R, min(i, R.n - 1)));
+                m[e][y] = -INFINITY;
+                l[e][y] = 0.f;
+            }
+        // ---- the walk
+        float o[NR][D / 16][4];
+#pragma unroll
+        for (int e = 0; e < NR; ++e)
+#pragma unroll
+            for (int j = 0; j < D / 16; ++j) o[e][j][0] = o[e][j][1] = o[e][j][2] = o[e][j][3] = 0.f;
         int ve = 126;  // value scales times 2^ve are below 2^7, so that weights up to 2^8 fit fp16
 #pragma unroll 1
         for (int k = 0; k < mine; ++k) {
-            async_wait<kStages - 2>();
+            async_wait<STAGES - 2>();
             __syncwarp();  // every lane's copies of step k are there, and step k - 1 has been read
-            fetch(k + kStages - 1);
-            const uint8_t* st = ring + (k % kStages) * S::kStage;
+            fetch(k + STAGES - 1);
+            const uint8_t* st = ring + (k % STAGES) * S::kStage;
             const float* scales = reinterpret_cast<const float*>(st + 2 * S::kCodes);
             const int t0 = begin + (warp + k * kFewWarps) * kStep;
-            float s[kStep / 8][4];
+            // scores: s[mt][e][x] is token 16 mt + quad + 8 (x >> 1), row 2c + (x & 1) of group e
+            float s[2][NR][4];
 #pragma unroll
-            for (int n = 0; n < kStep / 8; ++n) {
-                s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.f;
+            for (int mt = 0; mt < 2; ++mt) {
+#pragma unroll
+                for (int e = 0; e < NR; ++e) s[mt][e][0] = s[mt][e][1] = s[mt][e][2] = s[mt][e][3] = 0.f;
 #pragma unroll
                 for (int h = 0; h < CH; ++h) {
-                    const uint4 w4 = *reinterpret_cast<const uint4*>(st + k_at<D>(n * 8 + quad, h * 4 + c));
-                    const uint32_t w[4] = {w4.x, w4.y, w4.z, w4.w};
+                    const uint4 a4 = *reinterpret_cast<const uint4*>(st + k_at<D>(mt * 16 + quad, h * 4 + c));
+                    const uint4 b4 = *reinterpret_cast<const uint4*>(st + k_at<D>(mt * 16 + quad + 8, h * 4 + c));
+                    const uint32_t wa[4] = {a4.x, a4.y, a4.z, a4.w}, wb[4] = {b4.x, b4.y, b4.z, b4.w};
 #pragma unroll
                     for (int x = 0; x < 4; ++x) {
-                        const uint32_t b0 = half_pair(w[x]), b1 = half_pair(w[x] >> 8);
-                        mma_16816(s[n], qa[0][h * 4 + x], b0, b1);
-                        if constexpr (NQ == 2) mma_16816(s[n], qa[1][h * 4 + x], b0, b1);
+                        const uint32_t a[4] = {half_pair(wa[x]), half_pair(wb[x]), half_pair(wa[x] >> 8), half_pair(wb[x] >> 8)};
+#pragma unroll
+                        for (int e = 0; e < NR; ++e) {
+                            mma_16816(s[mt][e], a, qb[0][e][h * 4 + x][0], qb[0][e][h * 4 + x][1]);
+                            if constexpr (NQ == 2) mma_16816(s[mt][e], a, qb[1][e][h * 4 + x][0], qb[1][e][h * 4 + x][1]);
+                        }
                     }
                 }
             }
-            // scores; -inf where a row does not see the token
-            float top[2] = {-INFINITY, -INFINITY};
+            float top[NR][2];
+#pragma unroll
+            for (int e = 0; e < NR; ++e) top[e][0] = top[e][1] = -INFINITY;
             const bool masked = t0 + kStep > min(least, end);
 #pragma unroll
-            for (int n = 0; n < kStep / 8; ++n) {
-                const float2 kq = *reinterpret_cast<const float2*>(scales + n * 8 + 2 * c);
+            for (int mt = 0; mt < 2; ++mt)
 #pragma unroll
-                for (int x = 0; x < 4; ++x) {
-                    float v = s[n][x] * ((x & 1) ? kq.y : kq.x) * rf[x >> 1];
-                    if (masked && t0 + n * 8 + 2 * c + (x & 1) >= min(sees[x >> 1], end)) v = -INFINITY;
-                    s[n][x] = v;
-                    top[x >> 1] = fmaxf(top[x >> 1], v);
+                for (int half = 0; half < 2; ++half) {
+                    const int t = 16 * mt + quad + 8 * half;
+                    const float kq = scales[t];
+#pragma unroll
+                    for (int e = 0; e < NR; ++e)
+#pragma unroll
+                        for (int y = 0; y < 2; ++y) {
+                            float v = s[mt][e][2 * half + y] * kq * rf[e][y];
+                            if (masked && t0 + t >= sees[e][y]) v = -INFINITY;  // the row does not see the token
+                            s[mt][e][2 * half + y] = v;
+                            top[e][y] = fmaxf(top[e][y], v);
+                        }
                 }
-            }
-#pragma unroll
-            for (int e = 0; e < 2; ++e) {
-                top[e] = fmaxf(top[e], __shfl_xor_sync(0xffffffffu, top[e], 1));
-                top[e] = fmaxf(top[e], __shfl_xor_sync(0xffffffffu, top[e], 2));
-            }
             // largest value scale of the step (what is not finite has no say)
             float v_top = fabsf(scales[kStep + lane]);
             if (!(v_top < INFINITY)) v_top = 0.f;
             const int v_bits = __reduce_max_sync(0xffffffffu, __float_as_int(v_top));
             const int v_fit = v_bits == 0 ? 126 : fit_exponent(__int_as_float(v_bits), 7);
             const bool grow = v_fit < ve;
-            bool move[2];
+            bool move = grow;
 #pragma unroll
-            for (int e = 0; e < 2; ++e) move[e] = top[e] > m[e] + (m[e] == -INFINITY ? 0.f : 8.f);
-            if (__any_sync(0xffffffffu, grow || move[0] || move[1])) {
+            for (int e = 0; e < NR; ++e)
+#pragma unroll
+                for (int y = 0; y < 2; ++y) move |= top[e][y] > m[e][y] + (m[e][y] == -INFINITY ? 0.f : 8.f);
+            if (__any_sync(0xffffffffu, move)) {
                 const float fv = grow ? (ve - v_fit > 126 ? 0.f : pow2i(v_fit - ve)) : 1.f;
                 if (grow) ve = v_fit;
 #pragma unroll
-                for (int e = 0; e < 2; ++e) {
-                    const float f = move[e] ? (m[e] == -INFINITY ? 0.f : ex2_fast(m[e] - top[e])) : 1.f;
-                    if (move[e]) m[e] = top[e];
-                    l[e] *= f;
+                for (int e = 0; e < NR; ++e)
 #pragma unroll
-                    for (int j = 0; j < D / 8; ++j) {
-                        o[j][2 * e] *= f * fv;
-                        o[j][2 * e + 1] *= f * fv;
+                    for (int y = 0; y < 2; ++y) {
+                        float to = top[e][y];
+                        to = fmaxf(to, __shfl_xor_sync(0xffffffffu, to, 4));
+                        to = fmaxf(to, __shfl_xor_sync(0xffffffffu, to, 8));
+                        to = fmaxf(to, __shfl_xor_sync(0xffffffffu, to, 16));
+                        const bool go = to > m[e][y] + (m[e][y] == -INFINITY ? 0.f : 8.f);
+                        const float f = go ? (m[e][y] == -INFINITY ? 0.f : ex2_fast(m[e][y] - to)) : 1.f;
+                        if (go) m[e][y] = to;
+                        l[e][y] *= f;
+#pragma unroll
+                        for (int j = 0; j < D / 16; ++j) {
+                            o[e][j][y] *= f * fv;
+                            o[e][j][2 + y] *= f * fv;
+                        }
                     }
-                }
             }
             const float vf = pow2i(ve);
-            // weights, and the sums of values
 #pragma unroll
-            for (int g = 0; g < kStep / 16; ++g) {
-                uint32_t pa[NP][4];
+            for (int mt = 0; mt < 2; ++mt) {
+                // weights of 16 tokens
+                uint32_t pb[NP][NR][2];
 #pragma unroll
                 for (int half = 0; half < 2; ++half) {
-                    const int n = 2 * g + half;
-                    const float2 vq = *reinterpret_cast<const float2*>(scales + kStep + n * 8 + 2 * c);
+                    const float vq = scales[kStep + 16 * mt + quad + 8 * half] * vf;
 #pragma unroll
-                    for (int e = 0; e < 2; ++e) {
-                        const float me = m[e] == -INFINITY ? 0.f : m[e];
-                        const float p0 = ex2_fast(s[n][2 * e] - me), p1 = ex2_fast(s[n][2 * e + 1] - me);
-                        l[e] += p0 + p1;
-                        float w0 = p0 * (vq.x * vf), w1 = p1 * (vq.y * vf);
-                        if (masked) {  // a hidden token's scale may be anything
-                            if (s[n][2 * e] == -INFINITY) w0 = 0.f;
-                            if (s[n][2 * e + 1] == -INFINITY) w1 = 0.f;
+                    for (int e = 0; e < NR; ++e) {
+                        float w[2];
+#pragma unroll
+                        for (int y = 0; y < 2; ++y) {
+                            const float x = s[mt][e][2 * half + y];
+                            const float pr = ex2_fast(x - (m[e][y] == -INFINITY ? 0.f : m[e][y]));
+                            l[e][y] += pr;
+                            w[y] = pr * vq;
+                            if (masked && x == -INFINITY) w[y] = 0.f;  // a hidden token's scale may be anything
                         }
-                        pa[0][2 * half + e] = pack_half(w0, w1);
-                        if constexpr (NP == 2) pa[1][2 * half + e] = pack_rest(w0, w1, pa[0][2 * half + e]);
+                        const uint32_t hi = pack_half(w[0], w[1]);
+                        pb[0][e][half] = transposed(hi);
+                        if constexpr (NP == 2) pb[1][e][half] = transposed(pack_rest(w[0], w[1], hi));
                     }
                 }
-                // tokens 2c, 2c+1, 2c+8, 2c+9 of these 16; dims quad * D/8 .. of each
+                // values: tokens 2c, 2c+1, 2c+8, 2c+9 of the 16; dims quad * D/8 .. of each
                 constexpr int W = D / 32;  // words of a lane's dims
                 uint32_t v[4][W];
 #pragma unroll
                 for (int x = 0; x < 4; ++x) {
-                    const int r = g * 16 + 2 * c + (x & 1) + (x >> 1) * 8;
+                    const int r = mt * 16 + 2 * c + (x & 1) + (x >> 1) * 8;
                     const uint8_t* src = st + S::kCodes;
                     if constexpr (D == 128) {
                         const uint4 w = *reinterpret_cast<const uint4*>(src + v_at<D>(r, quad));
@@ -319,51 +357,51 @@ __global__ void __launch_bounds__(kFewWarps * 32, 2) chunk_few_kernel(const Chun
                     }
                 }
 #pragma unroll
-                for (int y = 0; y < W; ++y) {
-                    const uint32_t lo01 = __byte_perm(v[0][y], v[1][y], 0x5410), lo23 = __byte_perm(v[0][y], v[1][y], 0x7632);
-                    const uint32_t hi01 = __byte_perm(v[2][y], v[3][y], 0x5410), hi23 = __byte_perm(v[2][y], v[3][y], 0x7632);
-                    const uint32_t b0[4] = {half_pair(lo01), half_pair(lo01 >> 8), half_pair(lo23), half_pair(lo23 >> 8)};
-                    const uint32_t b1[4] = {half_pair(hi01), half_pair(hi01 >> 8), half_pair(hi23), half_pair(hi23 >> 8)};
+                for (int y = 0; y < W; ++y)
 #pragma unroll
-                    for (int d = 0; d < 4; ++d) {
-                        mma_16816(o[4 * y + d], pa[0], b0[d], b1[d]);
-                        if constexpr (NP == 2) mma_16816(o[4 * y + d], pa[1], b0[d], b1[d]);
+                    for (int z = 0; z < 2; ++z) {  // dims 4y + 2z and the next one: rows quad and quad + 8 of a product
+                        const uint32_t lo = __byte_perm(v[0][y], v[1][y], z ? 0x7632 : 0x5410);
+                        const uint32_t hi = __byte_perm(v[2][y], v[3][y], z ? 0x7632 : 0x5410);
+                        const uint32_t a[4] = {half_pair(lo), half_pair(lo >> 8), half_pair(hi), half_pair(hi >> 8)};
+#pragma unroll
+                        for (int e = 0; e < NR; ++e) {
+                            mma_16816(o[e][2 * y + z], a, pb[0][e][0], pb[0][e][1]);
+                            if constexpr (NP == 2) mma_16816(o[e][2 * y + z], a, pb[1][e][0], pb[1][e][1]);
+                        }
                     }
-                }
             }
         }
         async_wait<0>();
-        // ---- merge of the warps. Column n of product j is dim n * D/8 + j.
+        // ---- merge of the warps
         __syncthreads();  // every warp is done with its ring
         float* merge = reinterpret_cast<float*>(few_smem);  // [warp][row][D + 4]: dims, then m and l
         const float back = pow2i(-ve);
 #pragma unroll
-        for (int e = 0; e < 2; ++e) {
-            l[e] += __shfl_xor_sync(0xffffffffu, l[e], 1);
-            l[e] += __shfl_xor_sync(0xffffffffu, l[e], 2);
-            float* row = merge + (warp * kFewRows + quad + 8 * e) * (D + 4);
+        for (int e = 0; e < NR; ++e)
 #pragma unroll
-            for (int j = 0; j < D / 8; ++j) {
-                row[(2 * c) * (D / 8) + j] = o[j][2 * e] * back;
-                row[(2 * c + 1) * (D / 8) + j] = o[j][2 * e + 1] * back;
+            for (int y = 0; y < 2; ++y) {
+                float sum = l[e][y];
+                sum += __shfl_xor_sync(0xffffffffu, sum, 4);
+                sum += __shfl_xor_sync(0xffffffffu, sum, 8);
+                sum += __shfl_xor_sync(0xffffffffu, sum, 16);
+                float* row = merge + (warp * ROWS + 8 * e + 2 * c + y) * (D + 4);
+#pragma unroll
+                for (int j = 0; j < D / 16; ++j)
+                    *reinterpret_cast<float2*>(row + quad * (D / 8) + 2 * j) = make_float2(o[e][j][y] * back, o[e][j][2 + y] * back);
+                if (quad == 0) *reinterpret_cast<float2*>(row + D) = make_float2(m[e][y], sum);
             }
-            if (c == 0) {
-                row[D] = m[e];
-                row[D + 1] = l[e];
-            }
-        }
         __syncthreads();
-        const int slot = nsplit > 1 ? p.few_rec[b] + (hk * nrb + rb) * nsplit + split : -1;
-        for (int r = warp; r < kFewRows; r += kFewWarps) {
-            const int row = rb * kFewRows + r;
+        const int slot = nsplit > 1 ? p.rec[CLS][b] + (hk * nrb + rb) * nsplit + split : -1;
+        for (int r = warp; r < ROWS; r += kFewWarps) {
+            const int row = rb * ROWS + r;
             if (row >= rows) break;
             float M = -INFINITY;
 #pragma unroll
-            for (int w = 0; w < kFewWarps; ++w) M = fmaxf(M, merge[(w * kFewRows + r) * (D + 4) + D]);
+            for (int w = 0; w < kFewWarps; ++w) M = fmaxf(M, merge[(w * ROWS + r) * (D + 4) + D]);
             float f[kFewWarps], L = 0.f;
 #pragma unroll
             for (int w = 0; w < kFewWarps; ++w) {
-                const float* src = merge + (w * kFewRows + r) * (D + 4);
+                const float* src = merge + (w * ROWS + r) * (D + 4);
                 f[w] = src[D] == -INFINITY ? 0.f : ex2_fast(src[D] - M);
                 L += src[D + 1] * f[w];
             }
@@ -376,28 +414,29 @@ __global__ void __launch_bounds__(kFewWarps * 32, 2) chunk_few_kernel(const Chun
                 float x = 0.f;
 #pragma unroll
                 for (int w = 0; w < kFewWarps; ++w)
-                    if (f[w] != 0.f) x = fmaf(merge[(w * kFewRows + r) * (D + 4) + d], f[w], x);
-                if (slot >= 0) p.few_o[(static_cast<int64_t>(slot) * kFewRows + r) * D + d] = x;
+                    if (f[w] != 0.f) x = fmaf(merge[(w * ROWS + r) * (D + 4) + d], f[w], x);
+                if (slot >= 0) p.part_o[CLS][(static_cast<int64_t>(slot) * ROWS + r) * D + d] = x;
                 else store_out(p.out, o_at + d, x * inv, p.flags);
             }
-            if (slot >= 0 && lane == 0) p.few_ml[slot * kFewRows + r] = make_float2(M, L);
+            if (slot >= 0 && lane == 0) p.part_ml[CLS][static_cast<int64_t>(slot) * ROWS + r] = make_float2(M, L);
         }
         __syncthreads();  // the ring may be filled again
     }
 }
 
-template <int D, int NQ, int NP>
+template <int D, int NR, int NQ, int NP>
 cudaError_t launch_few(const ChunkParams& p, cudaStream_t st) {
-    auto kern = chunk_few_kernel<D, NQ, NP>;
+    auto kern = chunk_few_kernel<D, NR, NQ, NP>;
+    using S = FewSmem<D, NR>;
     static PerDeviceOnce once;
     cudaError_t e = once.run([kern] {
-        return cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, FewSmem<D>::kBytes);
+        return cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kBytes);
     });
     if (e != cudaSuccess) return e;
     cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3(2u * device_sm_count(), 1, 1);
+    cfg.gridDim = dim3(static_cast<unsigned>(p.ctas[NR - 1]), 1, 1);
     cfg.blockDim = dim3(kFewWarps * 32, 1, 1);
-    cfg.dynamicSmemBytes = FewSmem<D>::kBytes;
+    cfg.dynamicSmemBytes = S::kBytes;
     cfg.stream = st;
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -407,17 +446,22 @@ cudaError_t launch_few(const ChunkParams& p, cudaStream_t st) {
     return cudaLaunchKernelEx(&cfg, kern, p);
 }
 
+template <int D, int NR>
+cudaError_t launch_few_of(const ChunkParams& p, cudaStream_t st) {
+    const bool q16 = (p.flags & (KVD_FLAG_Q_BF16 | KVD_FLAG_Q_F16)) != 0, o16 = (p.flags & (KVD_FLAG_OUT_BF16 | KVD_FLAG_OUT_F16)) != 0;
+    return q16 ? (o16 ? launch_few<D, NR, 1, 1>(p, st) : launch_few<D, NR, 1, 2>(p, st))
+               : (o16 ? launch_few<D, NR, 2, 1>(p, st) : launch_few<D, NR, 2, 2>(p, st));
+}
+
 }  // namespace
 
-cudaError_t launch_chunk_few(const ChunkParams& p, cudaStream_t st, int* launches) {
-    const bool q16 = (p.flags & (KVD_FLAG_Q_BF16 | KVD_FLAG_Q_F16)) != 0, o16 = (p.flags & (KVD_FLAG_OUT_BF16 | KVD_FLAG_OUT_F16)) != 0;
-    cudaError_t e;
-    if (p.D == 128)
-        e = q16 ? (o16 ? launch_few<128, 1, 1>(p, st) : launch_few<128, 1, 2>(p, st))
-                : (o16 ? launch_few<128, 2, 1>(p, st) : launch_few<128, 2, 2>(p, st));
-    else
-        e = q16 ? (o16 ? launch_few<64, 1, 1>(p, st) : launch_few<64, 1, 2>(p, st))
-                : (o16 ? launch_few<64, 2, 1>(p, st) : launch_few<64, 2, 2>(p, st));
+int chunk_few_ctas(int D, int cls) {
+    return D == 128 ? (cls ? FewSmem<128, 2>::kCtas : FewSmem<128, 1>::kCtas) : (cls ? FewSmem<64, 2>::kCtas : FewSmem<64, 1>::kCtas);
+}
+
+cudaError_t launch_chunk_few(const ChunkParams& p, int cls, cudaStream_t st, int* launches) {
+    const cudaError_t e = p.D == 128 ? (cls ? launch_few_of<128, 2>(p, st) : launch_few_of<128, 1>(p, st))
+                                     : (cls ? launch_few_of<64, 2>(p, st) : launch_few_of<64, 1>(p, st));
     if (e == cudaSuccess) ++*launches;
     return e;
 }

@@ -139,13 +139,13 @@ template <int TERMS>
 __device__ __forceinline__ TileUnit tile_unit(const ChunkParams& p, int unit) {
     constexpr int ROWS = TERMS == 1 ? 256 : 128;
     TileUnit u;
-    u.b = warp_find(p.tile_first, p.B, unit);
+    u.b = warp_find(p.first[kMany], p.B, unit);
     u.R = chunk_rows(p, u.b);
     u.rows = u.R.n * p.G;
     u.nrb = (u.rows + ROWS - 1) / ROWS;
     int each;
-    u.nsplit = chunk_splits(u.R.len, p.head->tile_span, kTile, each);
-    int rest = unit - p.tile_first[u.b];
+    u.nsplit = chunk_splits(u.R.len, p.head->span[kMany], kTile, each);
+    int rest = unit - p.first[kMany][u.b];
     u.rb = u.nrb - 1 - rest % u.nrb;
     rest /= u.nrb;
     u.hk = rest % p.Hkv;
@@ -588,12 +588,12 @@ __device__ __forceinline__ bool tile_softmax(const ChunkParams& p, const TileUni
     const int i = static_cast<int>(p.by_g.div(static_cast<uint32_t>(row))), g = row - i * p.G;
     const bool there = row < u.rows;
     const int64_t o_at = static_cast<int64_t>(u.R.t0 + i) * p.o_st + static_cast<int64_t>(u.hk * p.G + g) * p.o_sh;
-    const int slot = u.nsplit > 1 ? p.tile_rec[u.b] + (u.hk * u.nrb + u.rb) * u.nsplit + u.split : -1;
+    const int slot = u.nsplit > 1 ? p.rec[kMany][u.b] + (u.hk * u.nrb + u.rb) * u.nsplit + u.split : -1;
     const int64_t rec = static_cast<int64_t>(slot) * ROWS + in_unit;
     if (u.nt == 0) {  // nothing in sight
         if (there && (!u.alt || w == 0)) {
             if (slot >= 0) {
-                p.tile_ml[rec] = make_float2(-INFINITY, 0.f);
+                p.part_ml[kMany][rec] = make_float2(-INFINITY, 0.f);
             } else {
                 const float none[32] = {};
 #pragma unroll 1
@@ -759,7 +759,7 @@ __device__ __forceinline__ bool tile_softmax(const ChunkParams& p, const TileUni
         }
         if (there) {
             if (slot >= 0) {
-                float4* dst = reinterpret_cast<float4*>(p.tile_o + rec * D + d);
+                float4* dst = reinterpret_cast<float4*>(p.part_o[kMany] + rec * D + d);
 #pragma unroll
                 for (int y = 0; y < 8; ++y) dst[y] = make_float4(x[4 * y], x[4 * y + 1], x[4 * y + 2], x[4 * y + 3]);
             } else {
@@ -769,7 +769,7 @@ __device__ __forceinline__ bool tile_softmax(const ChunkParams& p, const TileUni
             }
         }
     }
-    if (slot >= 0 && there && (!u.alt || w == 0)) p.tile_ml[rec] = make_float2(m, l);
+    if (slot >= 0 && there && (!u.alt || w == 0)) p.part_ml[kMany][rec] = make_float2(m, l);
     tc_fence_before();
     return !u.alt || both_here(bars, nm_sync);  // both have read both
 }
@@ -808,7 +808,7 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_tile_kernel(const __grid_co
     const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(smem + S::kTmem);
     grid_dependency_wait();
     allow_dependents();
-    const int units = p.head->tile_units;
+    const int units = p.head->units[kMany];
     if (warp < 8) {
         regs_more<kSoftmaxRegs>();
         int j = 0, nu = 0, ns = 0, no = 0, nm = 0;
@@ -893,7 +893,7 @@ cudaError_t take_chunk_tile_status(int32_t* status) {
 }
 
 cudaError_t launch_chunk_tile(const ChunkParams& p, cudaStream_t st, int* launches) {
-    const bool two = p.tile_rows == 128, fold = !two && (p.flags & KVD_FLAG_OUT_BF16) != 0;
+    const bool two = p.unit_rows[kMany] == 128, fold = !two && (p.flags & KVD_FLAG_OUT_BF16) != 0;
     const cudaError_t e = p.D == 128 ? (two ? launch_tile<128, 2, false>(p, st) : fold ? launch_tile<128, 1, true>(p, st) : launch_tile<128, 1, false>(p, st))
                                      : (two ? launch_tile<64, 2, false>(p, st) : fold ? launch_tile<64, 1, true>(p, st) : launch_tile<64, 1, false>(p, st));
     if (e == cudaSuccess) ++*launches;
