@@ -101,8 +101,9 @@ __global__ void __launch_bounds__(kAnyThreads) chunk_any_kernel(const ChunkParam
 // all requests and, for each kernel, at five stretches that a unit may have at
 // most: no limit, and the work (tokens times units) over 1, 2, 3 and 4 times
 // the CTAs that run at once (1 and 2 for many rows). It takes the one whose estimate is least,
-//   max(longest stretch, rounds of CTAs x mean stretch),
-// each stretch with what a unit costs beside its tokens, then places every
+//   max(longest stretch, rounds of CTAs x mean stretch)
+// for many rows (for few: the mean work of a CTA and half of the longest
+// stretch), each stretch with what a unit costs beside its tokens, then places every
 // request's units and records by prefix sums. Split units are fewer than twice
 // the work over the stretch: the room for their records. Bound: latency (loads,
 // two rounds of sums, one scan).
@@ -127,7 +128,10 @@ __device__ __forceinline__ ChunkShape chunk_shape(const ChunkParams& p, int b) {
 
 __device__ __forceinline__ int chunk_step(int cls) { return cls == kMany ? kTile : kFewStep; }
 
+constexpr int kPlanShapes = 1024;  // requests whose shapes the plan keeps in shared memory
+
 __global__ void __launch_bounds__(1024) chunk_plan_kernel(const ChunkParams p) {
+    __shared__ ChunkShape shapes[kPlanShapes];
     __shared__ unsigned long long work[kClasses];
     __shared__ int units_at[kClasses * kSpans], longest_at[kClasses * kSpans], span[kClasses];
     __shared__ int sums[2 * kClasses][32];
@@ -137,11 +141,14 @@ __global__ void __launch_bounds__(1024) chunk_plan_kernel(const ChunkParams p) {
     grid_dependency_wait();
     allow_dependents();
     __syncthreads();
+    const bool kept = p.B <= kPlanShapes;
     for (int b = tid; b < p.B; b += blockDim.x) {
         const ChunkShape s = chunk_shape(p, b);
+        if (kept) shapes[b] = s;
         if (s.units) atomicAdd(&work[s.cls], static_cast<unsigned long long>(s.units) * s.len);
     }
     __syncthreads();
+    auto shape_of = [&](int b) { return kept ? shapes[b] : chunk_shape(p, b); };
     auto span_of = [&](int cls, int k) {
         if (k == 0) return 0x40000000;
         const unsigned long long parts = static_cast<unsigned long long>(span_parts(cls, k)) * (cls == 0 ? p.ctas[0] : cls == 1 ? p.ctas[1] : p.ctas[kMany]);
@@ -150,7 +157,7 @@ __global__ void __launch_bounds__(1024) chunk_plan_kernel(const ChunkParams p) {
     };
     for (int64_t i = tid; i < static_cast<int64_t>(p.B) * kSpans; i += blockDim.x) {  // a thread per request and stretch
         const int b = static_cast<int>(i / kSpans), k = static_cast<int>(i - static_cast<int64_t>(b) * kSpans);
-        const ChunkShape s = chunk_shape(p, b);
+        const ChunkShape s = shape_of(b);
         if (s.units == 0) continue;
         int each;
         const int n = chunk_splits(s.len, span_of(s.cls, k), chunk_step(s.cls), each);
@@ -166,7 +173,11 @@ __global__ void __launch_bounds__(1024) chunk_plan_kernel(const ChunkParams p) {
         for (int k = 0; k < kSpans; ++k) {
             const int units = max(1, units_at[tid * kSpans + k]);
             const float mean = static_cast<float>(work[tid]) / static_cast<float>(units);
-            const float cost = fmaxf(longest_at[tid * kSpans + k] + extra, static_cast<float>((units + ctas - 1) / ctas) * (mean + extra));
+            const float longest = longest_at[tid * kSpans + k] + extra;
+            // one CTA of many rows an SM works in rounds; several of few rows share their SM's rate
+            const float all = tid == kMany ? static_cast<float>((units + ctas - 1) / ctas) * (mean + extra)
+                                           : static_cast<float>(units) / ctas * (mean + extra) + 0.5f * longest;
+            const float cost = fmaxf(longest, all);
             if (cost < least) {
                 least = cost;
                 best = k;
@@ -180,7 +191,7 @@ __global__ void __launch_bounds__(1024) chunk_plan_kernel(const ChunkParams p) {
         const int b = b0 + tid;
         int x[2 * kClasses] = {}, inc[2 * kClasses];
         if (b < p.B) {
-            const ChunkShape s = chunk_shape(p, b);
+            const ChunkShape s = shape_of(b);
             int each;
             const int n = chunk_splits(s.len, span[s.cls], chunk_step(s.cls), each);
 #pragma unroll
@@ -217,6 +228,9 @@ __global__ void __launch_bounds__(1024) chunk_plan_kernel(const ChunkParams p) {
             carry[i] += all;
         }
     }
+#pragma unroll
+    for (int c = 0; c < kMany; ++c)  // nobody has arrived yet
+        for (int i = tid; i < carry[2 * c + 1]; i += blockDim.x) p.arrived[c][i] = 0;
     if (tid == 0) {
         ChunkHead h{};
 #pragma unroll
@@ -230,8 +244,9 @@ __global__ void __launch_bounds__(1024) chunk_plan_kernel(const ChunkParams p) {
 }
 
 // ------------------------------------------------------------- split work
-// Merges the records of units that were split along the tokens: eight rows a
-// CTA, out = sum_s 2^(m_s - M) o_s / sum_s 2^(m_s - M) l_s.
+// Merges the records of units of many rows that were split along the tokens:
+// eight rows a CTA, out = sum_s 2^(m_s - M) o_s / sum_s 2^(m_s - M) l_s. (Units of
+// few rows are merged by the CTA that is last to write one.)
 constexpr int kMergeRows = 8;
 
 template <int D>
@@ -239,55 +254,19 @@ __global__ void __launch_bounds__(128) chunk_merge_kernel(const ChunkParams p) {
     grid_dependency_wait();
     allow_dependents();
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    int64_t before = 0;  // units of the classes in front
-#pragma unroll
-    for (int c = 0; c < kClasses; ++c) {
-        const int unit_rows = p.unit_rows[c], groups = unit_rows / kMergeRows, span = p.head->span[c];
-        const int64_t units = static_cast<int64_t>(p.head->recs[c]) * groups;
-        // every CTA goes on in the next class where it stopped in this one
-        int64_t u = blockIdx.x + (gridDim.x - before % gridDim.x);
-        if (u >= gridDim.x) u -= gridDim.x;
-        for (; u < units; u += gridDim.x) {
-            const int slot = static_cast<int>(u / groups), group = static_cast<int>(u - static_cast<int64_t>(slot) * groups);
-            const int b = warp_find(p.rec[c], p.B, slot);
-            const ChunkRows R = chunk_rows(p, b);
-            const int rows = R.n * p.G, nrb = (rows + unit_rows - 1) / unit_rows;
-            int each;
-            const int nsplit = chunk_splits(R.len, span, chunk_step(c), each);
-            const int local = slot - p.rec[c][b], item = local / nsplit;
-            if (local != item * nsplit) continue;  // the first record of a unit stands for all
-            const int hk = item / nrb, rb = item - hk * nrb;
-            const float* o = p.part_o[c];
-            const float2* ml = p.part_ml[c];
-            for (int r = group * kMergeRows + warp; r < (group + 1) * kMergeRows; r += 4) {
-                const int row = rb * unit_rows + r;
-                if (row >= rows) break;
-                const int64_t at = static_cast<int64_t>(slot) * unit_rows + r;
-                float M = -INFINITY;
-                for (int s = lane; s < nsplit; s += 32) M = fmaxf(M, ml[at + static_cast<int64_t>(s) * unit_rows].x);
-#pragma unroll
-                for (int i = 16; i > 0; i >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, i));
-                float L = 0.f, acc[D / 32] = {};
-#pragma unroll 4
-                for (int s = 0; s < nsplit; ++s) {
-                    const int64_t rec = at + static_cast<int64_t>(s) * unit_rows;
-                    const float2 v = ml[rec];
-                    const float f = v.x == -INFINITY ? 0.f : exp2f(v.x - M);
-                    L = fmaf(v.y, f, L);
-#pragma unroll
-                    for (int d = 0; d < D / 32; ++d) {
-                        const float x = o[rec * D + d * 32 + lane];
-                        if (f != 0.f) acc[d] = fmaf(x, f, acc[d]);
-                    }
-                }
-                const int i = static_cast<int>(p.by_g.div(static_cast<uint32_t>(row))), g = row - i * p.G;
-                const int64_t o_at = static_cast<int64_t>(R.t0 + i) * p.o_st + static_cast<int64_t>(hk * p.G + g) * p.o_sh;
-                const float inv = L == 0.f ? 0.f : 1.f / L;  // no token in sight
-#pragma unroll
-                for (int d = 0; d < D / 32; ++d) store_out(p.out, o_at + d * 32 + lane, acc[d] * inv, p.flags);
-            }
-        }
-        before += units;
+    const int unit_rows = p.unit_rows[kMany], groups = unit_rows / kMergeRows, span = p.head->span[kMany];
+    const int64_t units = static_cast<int64_t>(p.head->recs[kMany]) * groups;
+    for (int64_t u = blockIdx.x; u < units; u += gridDim.x) {
+        const int slot = static_cast<int>(u / groups), group = static_cast<int>(u - static_cast<int64_t>(slot) * groups);
+        const int b = warp_find(p.rec[kMany], p.B, slot);
+        const ChunkRows R = chunk_rows(p, b);
+        const int rows = R.n * p.G, nrb = (rows + unit_rows - 1) / unit_rows;
+        int each;
+        const int nsplit = chunk_splits(R.len, span, kTile, each);
+        const int local = slot - p.rec[kMany][b], item = local / nsplit;
+        if (local != item * nsplit) continue;  // the first record of a unit stands for all
+        const int hk = item / nrb, rb = item - hk * nrb, r0 = group * kMergeRows + warp * 2;
+        merge_records<D, 2>(p, R, p.part_o[kMany], p.part_ml[kMany], slot, nsplit, unit_rows, hk, rb * unit_rows, r0, rows, lane);
     }
 }
 
@@ -311,20 +290,35 @@ bool tensor_shape(const kvd_paged_prefill_desc& d) {
            ((d.kv_stride_block | d.kv_stride_h | d.kv_stride_t) & 15) == 0;
 }
 
-// Rows of a KV head up to which a request has few.
-constexpr int kFewMost = 64;
+int64_t group_rows(const kvd_paged_prefill_desc& d) { return static_cast<int64_t>(d.num_rows) * (d.num_q_heads / d.num_kv_heads); }
+
+// Rows of a KV head up to which a request has few: 64. (512 tokens of 8,192 in groups of 8: 16 rows a unit re-read and
+// re-widen what a tile shares; figures beside the kernels.) A call whose requests have up to 32 rows on average and 256
+// in all takes them all for few, which saves two launches.
+int few_most(const kvd_paged_prefill_desc& d) {
+    const int64_t rows = group_rows(d);
+    return rows <= 256 && rows <= 32LL * d.batch ? 256 : 64;
+}
+
+// Rows up to which a request goes to the kernel for units of 8: 8, unless there are too few requests to fill the GPU
+// and others beside them; one launch less then counts more.
+int tiny_most(const kvd_paged_prefill_desc& d) {
+    const bool alone = d.num_rows <= d.batch;  // single tokens
+    return alone || static_cast<int64_t>(d.batch) * d.num_kv_heads >= 2LL * device_sm_count() ? 8 : 0;
+}
 
 // Whether a request of the call may be of a class, by what the host knows.
 bool has_class(const kvd_paged_prefill_desc& d, int cls) {
-    const int64_t G = d.num_q_heads / d.num_kv_heads, most = d.num_rows * G;
-    return cls == 0 ? G <= 8 : cls == 1 ? most > 8 && G <= kFewMost : most > kFewMost;
+    const int64_t G = d.num_q_heads / d.num_kv_heads, most = group_rows(d);
+    return cls == 0 ? G <= tiny_most(d) : cls == 1 ? most > tiny_most(d) && G <= few_most(d) : most > few_most(d);
 }
 
 int64_t round16(int64_t x) { return (x + 15) & ~static_cast<int64_t>(15); }
 
 // Lays the workspace out from `base` (nullptr: to learn its size, which is the same for all types of rows and
 // output); returns its bytes.
-int64_t lay_out(const kvd_paged_prefill_desc& d, ChunkParams* p, uint8_t* base) {
+int64_t lay_out(const kvd_paged_prefill_desc& d, ChunkParams* p, uint8_t* base, bool& split) {
+    split = false;  // whether units of many rows may be
     const int sms = device_sm_count();
     const int64_t G = d.num_q_heads / d.num_kv_heads, D = d.head_dim, entries = static_cast<int64_t>(d.batch) + 1;
     const int64_t cap = static_cast<int64_t>(d.max_blocks_per_seq) * d.block_size;
@@ -332,15 +326,16 @@ int64_t lay_out(const kvd_paged_prefill_desc& d, ChunkParams* p, uint8_t* base) 
     p->unit_rows[0] = 8;
     p->unit_rows[1] = 16;
     p->unit_rows[kMany] = (d.flags & q16) != 0 && (d.flags & o16) != 0 ? 256 : 128;
-    p->ctas[0] = sms * chunk_few_ctas(static_cast<int>(D), 0);
-    p->ctas[1] = sms * chunk_few_ctas(static_cast<int>(D), 1);
+    for (int c = 0; c < kMany; ++c) p->ctas[c] = sms * chunk_few_ctas(d.head_dim, c, (d.flags & q16) != 0);
     p->ctas[kMany] = sms;
-    p->few_most = kFewMost;
+    p->tiny_most = tiny_most(d);
+    p->few_most = few_most(d);
     // no more units than rows give, and no more splits of each than the longest length gives
     auto records = [&](int cls, int64_t unit_rows) -> int64_t {
         const int64_t least = cls == kMany ? kTileMinSpan : kFewMinSpan;
         const int64_t units = (d.num_rows * G / unit_rows + (d.batch < d.num_rows ? d.batch : d.num_rows)) * d.num_kv_heads;
-        const int64_t splits = (cap + least - 1) / least, most = units * splits, room = 2LL * span_parts(cls, kSpans - 1) * p->ctas[cls];
+        const int64_t splits = (cap + least - 1) / least, most = units * splits;
+        const int64_t ctas = cls == kMany ? sms : sms * chunk_few_ctas(d.head_dim, cls, true), room = 2 * span_parts(cls, kSpans - 1) * ctas;
         return splits <= 1 || !has_class(d, cls) ? 0 : most < room ? most : room;
     };
     int64_t at = 0;
@@ -350,7 +345,6 @@ int64_t lay_out(const kvd_paged_prefill_desc& d, ChunkParams* p, uint8_t* base) 
         return here;
     };
     p->head = reinterpret_cast<ChunkHead*>(take(sizeof(ChunkHead)));
-    p->records = false;
     for (int c = 0; c < kClasses; ++c) {
         p->first[c] = reinterpret_cast<int32_t*>(take(4 * entries));
         p->rec[c] = reinterpret_cast<int32_t*>(take(4 * entries));
@@ -361,7 +355,8 @@ int64_t lay_out(const kvd_paged_prefill_desc& d, ChunkParams* p, uint8_t* base) 
         }
         p->part_o[c] = reinterpret_cast<float*>(take(4 * D * rows));
         p->part_ml[c] = reinterpret_cast<float2*>(take(8 * rows));
-        p->records |= rows > 0;
+        if (c < kMany) p->arrived[c] = reinterpret_cast<int32_t*>(take(4 * rows / p->unit_rows[c]));
+        else split |= rows > 0;
     }
     return at;
 }
@@ -389,7 +384,8 @@ using namespace kvd;
 extern "C" size_t kvd_paged_prefill_workspace_size(const kvd_paged_prefill_desc* d) {
     if (check_chunk(d) != cudaSuccess) return 0;
     ChunkParams p{};
-    return d->head_dim == 64 || d->head_dim == 128 ? static_cast<size_t>(lay_out(*d, &p, nullptr)) : 0;
+    bool split;
+    return d->head_dim == 64 || d->head_dim == 128 ? static_cast<size_t>(lay_out(*d, &p, nullptr, split)) : 0;
 }
 
 extern "C" cudaError_t kvd_paged_prefill_launch(const kvd_paged_prefill_desc* d, const void* Q, const int8_t* K_pool,
@@ -429,7 +425,8 @@ extern "C" cudaError_t kvd_paged_prefill_launch(const kvd_paged_prefill_desc* d,
         if (e == cudaSuccess) ++*launches;
         return e;
     }
-    lay_out(*d, &p, static_cast<uint8_t*>(workspace));
+    bool split;
+    lay_out(*d, &p, static_cast<uint8_t*>(workspace), split);
     e = launch_after(chunk_plan_kernel, 1, p.B <= 256 ? 256 : 1024, 0, stream, p);
     if (e != cudaSuccess) return e;
     ++*launches;
@@ -438,7 +435,7 @@ extern "C" cudaError_t kvd_paged_prefill_launch(const kvd_paged_prefill_desc* d,
         e = c == kMany ? launch_chunk_tile(p, stream, launches) : launch_chunk_few(p, c, stream, launches);
         if (e != cudaSuccess) return e;
     }
-    if (!p.records) return cudaSuccess;
+    if (!split) return cudaSuccess;
     const unsigned grid = 8u * device_sm_count();
     e = p.D == 128 ? launch_after(chunk_merge_kernel<128>, grid, 128, 0, stream, p)
                    : launch_after(chunk_merge_kernel<64>, grid, 128, 0, stream, p);

@@ -47,15 +47,15 @@ struct ChunkParams {
     float2* part_ml[kClasses];  // and [slot][unit_rows] (reference in base 2, sum of weights)
     int unit_rows[kClasses];
     int ctas[kClasses];         // CTAs that run at once
-    int few_most;               // rows up to which a request has few
-    bool records;               // some unit may be split
+    int32_t* arrived[kMany];    // [slot] units of the classes with few rows that have written their records
+    int tiny_most, few_most;    // rows up to which a request is of the first class, of the second
 };
 
 constexpr int kFewStep = 32;     // tokens of a step of the kernels for few rows
 constexpr int kFewMinSpan = 256; // tokens that a split has at least
 constexpr int kTileMinSpan = 512;
 // What a unit costs beside its tokens, in tokens.
-constexpr float kFewExtra = 200.f, kTileExtra = 400.f;
+constexpr float kFewExtra = 512.f, kTileExtra = 400.f;
 constexpr int kTile = 128;       // tokens of a tile of the kernel for many rows
 
 // Rows [t0, t0 + n) of request b and its tokens.
@@ -76,7 +76,9 @@ __device__ __forceinline__ int chunk_sees(const ChunkParams& p, const ChunkRows&
     return p.causal ? max(0, min(r.len, r.len - r.n + i + 1)) : r.len;
 }
 
-__device__ __forceinline__ int chunk_class(const ChunkParams& p, int rows) { return rows <= 8 ? 0 : rows <= p.few_most ? 1 : kMany; }
+__device__ __forceinline__ int chunk_class(const ChunkParams& p, int rows) {
+    return rows <= p.tiny_most ? 0 : rows <= p.few_most ? 1 : kMany;
+}
 
 // Splits of a request's tokens, and the tokens of each (a multiple of `step`).
 __device__ __forceinline__ int chunk_splits(int len, int span, int step, int& each) {
@@ -128,8 +130,75 @@ __device__ __forceinline__ int fit_exponent(float most, int top) {
     return min(max(top - (e - 126), -126), 126);
 }
 
+// Four neighbouring dims of an output row.
+__device__ __forceinline__ void store_out4(const ChunkParams& p, int64_t at, float4 x) {
+    if (!p.vec_out) {
+        store_out(p.out, at, x.x, p.flags);
+        store_out(p.out, at + 1, x.y, p.flags);
+        store_out(p.out, at + 2, x.z, p.flags);
+        store_out(p.out, at + 3, x.w, p.flags);
+    } else if (p.flags & KVD_FLAG_OUT_BF16) {
+        const __nv_bfloat162 a = __floats2bfloat162_rn(x.x, x.y), b = __floats2bfloat162_rn(x.z, x.w);
+        *reinterpret_cast<uint2*>(static_cast<uint16_t*>(p.out) + at) =
+            make_uint2(*reinterpret_cast<const uint32_t*>(&a), *reinterpret_cast<const uint32_t*>(&b));
+    } else if (p.flags & KVD_FLAG_OUT_F16) {
+        *reinterpret_cast<uint2*>(static_cast<uint16_t*>(p.out) + at) = make_uint2(pack_half(x.x, x.y), pack_half(x.z, x.w));
+    } else {
+        *reinterpret_cast<float4*>(static_cast<float*>(p.out) + at) = x;
+    }
+}
+
+// N rows from r0 on (of the unit's; row0: its first one of the request's) of a split unit, by a warp: the records
+// slot, slot + 1, .. of its splits, weighed by their references.
+template <int D, int N>
+__device__ __forceinline__ void merge_records(const ChunkParams& p, const ChunkRows& R, const float* o, const float2* ml, int slot,
+                                              int nsplit, int unit_rows, int hk, int row0, int r0, int rows, int lane) {
+    constexpr int E = D / 32;  // neighbouring dims a lane
+    float M[N], L[N] = {}, acc[N][E] = {};
+    int64_t at[N];
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        at[i] = static_cast<int64_t>(slot) * unit_rows + min(r0 + i, rows - 1 - row0);  // the last one again where there is none
+        M[i] = -INFINITY;
+        for (int s = lane; s < nsplit; s += 32) M[i] = fmaxf(M[i], __ldcg(&ml[at[i] + static_cast<int64_t>(s) * unit_rows]).x);
+#pragma unroll
+        for (int x = 16; x > 0; x >>= 1) M[i] = fmaxf(M[i], __shfl_xor_sync(0xffffffffu, M[i], x));
+    }
+#pragma unroll 4
+    for (int s = 0; s < nsplit; ++s) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const int64_t rec = at[i] + static_cast<int64_t>(s) * unit_rows;
+            const float2 v = __ldcg(&ml[rec]);
+            float x[E];
+            if constexpr (E == 4) {
+                const float4 y = __ldcg(reinterpret_cast<const float4*>(o + rec * D) + lane);
+                x[0] = y.x; x[1] = y.y; x[2] = y.z; x[3] = y.w;
+            } else {
+                const float2 y = __ldcg(reinterpret_cast<const float2*>(o + rec * D) + lane);
+                x[0] = y.x; x[1] = y.y;
+            }
+            const float f = v.x == -INFINITY ? 0.f : exp2f(v.x - M[i]);
+            L[i] = fmaf(v.y, f, L[i]);
+#pragma unroll
+            for (int d = 0; d < E; ++d)
+                if (f != 0.f) acc[i][d] = fmaf(x[d], f, acc[i][d]);
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        const int row = row0 + r0 + i;
+        if (row >= rows) break;
+        const int t = static_cast<int>(p.by_g.div(static_cast<uint32_t>(row))), g = row - t * p.G;
+        const int64_t to = static_cast<int64_t>(R.t0 + t) * p.o_st + static_cast<int64_t>(hk * p.G + g) * p.o_sh + lane * E;
+        const float inv = L[i] == 0.f ? 0.f : 1.f / L[i];  // no token in sight: 0; NaN stays
+#pragma unroll
+        for (int d = 0; d < E; ++d) store_out(p.out, to + d, acc[i][d] * inv, p.flags);
+    }
+}
+
 cudaError_t launch_chunk_few(const ChunkParams& p, int cls, cudaStream_t st, int* launches);
-int chunk_few_ctas(int D, int cls);  // per SM
+int chunk_few_ctas(int D, int cls, bool q16);  // CTAs of an SM
 cudaError_t launch_chunk_tile(const ChunkParams& p, cudaStream_t st, int* launches);
 
 }  // namespace kvd

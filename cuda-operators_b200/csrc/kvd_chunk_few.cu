@@ -49,11 +49,11 @@ __device__ __forceinline__ void async_wait() {
 
 // NR: 8-row groups of a unit. Stages of a warp's ring, and CTAs of an SM, are what 227 KB of shared memory and 64 K
 // registers hold.
-template <int D, int NR>
+template <int D, int NR, int NQ>
 struct FewSmem {
     static constexpr int kRows = 8 * NR;
-    static constexpr int kCtas = NR == 2 ? 2 : D == 128 ? 3 : 4;
-    static constexpr int kStages = NR == 1 && D == 128 ? 2 : 3;  // steps
+    static constexpr int kCtas = D == 64 ? (NR == 1 ? 4 : 3) : NR == 2 && NQ == 2 ? 2 : 3;
+    static constexpr int kStages = D == 128 && kCtas == 3 ? 2 : 3;  // steps
     static constexpr int kCodes = kStep * D;                     // of K or V
     static constexpr int kStage = 2 * kCodes + 2 * kStep * 4;
     static constexpr int kRing = kFewWarps * kStages * kStage;
@@ -76,14 +76,14 @@ template <int D>
 __device__ __forceinline__ int v_at(int r, int c) { return r * D + (D == 128 ? (c ^ (r & 6)) : (c ^ ((r >> 1) & 3))) * 16; }
 
 template <int D, int NR, int NQ, int NP>
-__global__ void __launch_bounds__(kFewWarps * 32, FewSmem<D, NR>::kCtas) chunk_few_kernel(const ChunkParams p) {
+__global__ void __launch_bounds__(kFewWarps * 32, FewSmem<D, NR, NQ>::kCtas) chunk_few_kernel(const ChunkParams p) {
     extern __shared__ __align__(16) uint8_t few_smem[];
     constexpr int KS = D / 16;      // steps of 16 dims of a product
     constexpr int CH = D / 64;      // 16-byte chunks of a K row that a lane holds
     constexpr int PER = D / 16;     // 16-byte chunks of a row
     constexpr int COPIES = kStep * PER / 32;  // chunks of K, and of V, that a lane copies
     constexpr int CLS = NR - 1;
-    using S = FewSmem<D, NR>;
+    using S = FewSmem<D, NR, NQ>;
     constexpr int ROWS = S::kRows, STAGES = S::kStages;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, quad = lane >> 2, c = lane & 3;
     uint8_t* ring = few_smem + warp * STAGES * S::kStage;
@@ -122,7 +122,8 @@ __global__ void __launch_bounds__(kFewWarps * 32, FewSmem<D, NR>::kCtas) chunk_f
             return -1;
         };
         int next_off = 0, next_id = look_up(0, next_off);
-        auto fetch = [&](int k) {
+        int ahead_off = 0, ahead_id = STAGES > 2 ? look_up(1, ahead_off) : -1;  // on its way together with the first
+        auto fetch = [&](int k, bool first = false) {
             if (k < mine) {
                 uint8_t* st = ring + (k % STAGES) * S::kStage;
                 // where there is no token its scales are zeros, and any codes do
@@ -138,15 +139,20 @@ __global__ void __launch_bounds__(kFewWarps * 32, FewSmem<D, NR>::kCtas) chunk_f
                 float* scales = reinterpret_cast<float*>(st + 2 * S::kCodes);
                 async_copy<4>(scales + lane, ks + sc, next_id >= 0);
                 async_copy<4>(scales + kStep + lane, vs + sc, next_id >= 0);
-                next_id = look_up(k + 1, next_off);
+                if (first && STAGES > 2) {
+                    next_id = ahead_id;
+                    next_off = ahead_off;
+                } else {
+                    next_id = look_up(k + 1, next_off);
+                }
             }
             async_commit();
         };
-#pragma unroll 1
-        for (int k = 0; k < STAGES - 1; ++k) fetch(k);
         // ---- queries: this lane's dims of row quad of each group, a power of two times them so that fp16 holds them
         uint32_t qb[NQ][NR][KS][2];
         float factor[NR];  // what the scores of row quad are multiplied with instead
+        fetch(0, true);
+        if (STAGES > 2) fetch(1);
 #pragma unroll
         for (int e = 0; e < NR; ++e) {
             const int r = rb * ROWS + 8 * e + quad;
@@ -247,7 +253,9 @@ __global__ void __launch_bounds__(kFewWarps * 32, FewSmem<D, NR>::kCtas) chunk_f
 #pragma unroll
             for (int mt = 0; mt < 2; ++mt) {
 #pragma unroll
-                for (int e = 0; e < NR; ++e) s[mt][e][0] = s[mt][e][1] = s[mt][e][2] = s[mt][e][3] = 0.f;
+                for (int e = 0; e < NR; ++e) {
+                    s[mt][e][0] = s[mt][e][1] = s[mt][e][2] = s[mt][e][3] = 0.f;
+                }
 #pragma unroll
                 for (int h = 0; h < CH; ++h) {
                     const uint4 a4 = *reinterpret_cast<const uint4*>(st + k_at<D>(mt * 16 + quad, h * 4 + c));
@@ -392,42 +400,60 @@ __global__ void __launch_bounds__(kFewWarps * 32, FewSmem<D, NR>::kCtas) chunk_f
             }
         __syncthreads();
         const int slot = nsplit > 1 ? p.rec[CLS][b] + (hk * nrb + rb) * nsplit + split : -1;
-        for (int r = warp; r < ROWS; r += kFewWarps) {
-            const int row = rb * ROWS + r;
-            if (row >= rows) break;
-            float M = -INFINITY;
-#pragma unroll
-            for (int w = 0; w < kFewWarps; ++w) M = fmaxf(M, merge[(w * ROWS + r) * (D + 4) + D]);
-            float f[kFewWarps], L = 0.f;
+        constexpr int TPR = kFewWarps * 32 / ROWS;  // threads a row, four dims at a time each
+        const int r = threadIdx.x / TPR, tx = threadIdx.x % TPR, row = rb * ROWS + r;
+        if (row < rows) {
+            float M = -INFINITY, f[kFewWarps], L = 0.f;
+            float2 ml[kFewWarps];
 #pragma unroll
             for (int w = 0; w < kFewWarps; ++w) {
-                const float* src = merge + (w * ROWS + r) * (D + 4);
-                f[w] = src[D] == -INFINITY ? 0.f : ex2_fast(src[D] - M);
-                L += src[D + 1] * f[w];
+                ml[w] = *reinterpret_cast<const float2*>(merge + (w * ROWS + r) * (D + 4) + D);
+                M = fmaxf(M, ml[w].x);
+            }
+#pragma unroll
+            for (int w = 0; w < kFewWarps; ++w) {
+                f[w] = ml[w].x == -INFINITY ? 0.f : ex2_fast(ml[w].x - M);
+                L += ml[w].y * f[w];
             }
             const int i = static_cast<int>(p.by_g.div(static_cast<uint32_t>(row))), g = row - i * p.G;
             const int64_t o_at = static_cast<int64_t>(R.t0 + i) * p.o_st + static_cast<int64_t>(hk * p.G + g) * p.o_sh;
             // a sum of weights that is 0 belongs to a row that sees nothing; NaN stays
-            const float inv = L == 0.f ? 0.f : 1.f / L;
+            const float inv = slot >= 0 ? 1.f : L == 0.f ? 0.f : 1.f / L;
 #pragma unroll
-            for (int d = lane; d < D; d += 32) {
-                float x = 0.f;
+            for (int j = 0; j < D / 4 / TPR; ++j) {
+                const int d = (tx + j * TPR) * 4;
+                float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-                for (int w = 0; w < kFewWarps; ++w)
-                    if (f[w] != 0.f) x = fmaf(merge[(w * ROWS + r) * (D + 4) + d], f[w], x);
-                if (slot >= 0) p.part_o[CLS][(static_cast<int64_t>(slot) * ROWS + r) * D + d] = x;
-                else store_out(p.out, o_at + d, x * inv, p.flags);
+                for (int w = 0; w < kFewWarps; ++w) {
+                    const float4 y = *reinterpret_cast<const float4*>(merge + (w * ROWS + r) * (D + 4) + d);
+                    if (f[w] != 0.f) x = make_float4(fmaf(y.x, f[w], x.x), fmaf(y.y, f[w], x.y), fmaf(y.z, f[w], x.z), fmaf(y.w, f[w], x.w));
+                }
+                x = make_float4(x.x * inv, x.y * inv, x.z * inv, x.w * inv);
+                if (slot >= 0) *reinterpret_cast<float4*>(p.part_o[CLS] + (static_cast<int64_t>(slot) * ROWS + r) * D + d) = x;
+                else store_out4(p, o_at + d, x);
             }
-            if (slot >= 0 && lane == 0) p.part_ml[CLS][static_cast<int64_t>(slot) * ROWS + r] = make_float2(M, L);
+            if (slot >= 0 && tx == 0) p.part_ml[CLS][static_cast<int64_t>(slot) * ROWS + r] = make_float2(M, L);
         }
         __syncthreads();  // the ring may be filled again
+        if (slot >= 0) {  // the CTA that is last to write a record of the unit merges them
+            __shared__ int s_last;
+            if (threadIdx.x == 0) {  // releases this CTA's records, acquires the others'
+                int before;
+                asm volatile("atom.acq_rel.gpu.global.add.s32 %0, [%1], 1;" : "=r"(before) : "l"(&p.arrived[CLS][slot - split]) : "memory");
+                s_last = before == nsplit - 1;
+            }
+            __syncthreads();
+            if (s_last)
+                merge_records<D, ROWS / kFewWarps>(p, R, p.part_o[CLS], p.part_ml[CLS], slot - split, nsplit, ROWS, hk, rb * ROWS,
+                                                   warp * (ROWS / kFewWarps), rows, lane);
+        }
     }
 }
 
 template <int D, int NR, int NQ, int NP>
 cudaError_t launch_few(const ChunkParams& p, cudaStream_t st) {
     auto kern = chunk_few_kernel<D, NR, NQ, NP>;
-    using S = FewSmem<D, NR>;
+    using S = FewSmem<D, NR, NQ>;
     static PerDeviceOnce once;
     cudaError_t e = once.run([kern] {
         return cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kBytes);
@@ -455,8 +481,9 @@ cudaError_t launch_few_of(const ChunkParams& p, cudaStream_t st) {
 
 }  // namespace
 
-int chunk_few_ctas(int D, int cls) {
-    return D == 128 ? (cls ? FewSmem<128, 2>::kCtas : FewSmem<128, 1>::kCtas) : (cls ? FewSmem<64, 2>::kCtas : FewSmem<64, 1>::kCtas);
+int chunk_few_ctas(int D, int cls, bool q16) {
+    if (D == 64) return cls ? FewSmem<64, 2, 1>::kCtas : FewSmem<64, 1, 1>::kCtas;
+    return cls == 0 ? FewSmem<128, 1, 1>::kCtas : q16 ? FewSmem<128, 2, 1>::kCtas : FewSmem<128, 2, 2>::kCtas;
 }
 
 cudaError_t launch_chunk_few(const ChunkParams& p, int cls, cudaStream_t st, int* launches) {
