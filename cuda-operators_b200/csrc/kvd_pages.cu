@@ -19,6 +19,7 @@ namespace {
 
 constexpr int kPagesMaxBatch = 8192;  // rows: four bytes each in the shared memory of a CTA, twice
 constexpr int kMarkThreads = 512;
+constexpr int kWords = 4;  // words of a bitmap that a thread holds at a time
 constexpr int kApplyThreads = 256;
 constexpr int kEntries = 256;  // table entries a warp takes at a time, eight loads a lane
 constexpr int kNoHeir = 0x7fffffff;
@@ -34,6 +35,7 @@ struct Pools {
     int64_t sblk, sh, st, sc_blk, sc_h;
     int H, D;
     FastDiv by_vecs;  // D / bytes a lane copies at a time
+    bool bounds16;    // a head's bounds lie on 16-byte boundaries
 };
 
 struct PagesParams {
@@ -139,6 +141,23 @@ __device__ __forceinline__ void my_words(const PagesParams& p, int64_t& first, i
     last = min(p.words, first + n);
 }
 
+// kWords words of a bitmap from w on, zeros behind its end; written by other CTAs.
+__device__ __forceinline__ void load_words(const PagesParams& p, const uint32_t* bits, int64_t w, uint32_t (&x)[kWords]) {
+#pragma unroll
+    for (int i = 0; i < kWords; ++i) x[i] = w + i < p.words ? __ldcg(bits + w + i) : 0u;
+}
+
+// A row's entries from e0 on that a warp marks: its unit u of all rows' stretches.
+__device__ __forceinline__ int unit_row(const PagesParams& p, int64_t u, int& e0) {
+    if (p.chunks == 1) {
+        e0 = 0;
+        return static_cast<int>(u);
+    }
+    const int b = static_cast<int>(u / p.chunks);
+    e0 = static_cast<int>(u - static_cast<int64_t>(b) * p.chunks) * kEntries;
+    return b;
+}
+
 // ------------------------------------------------------------------------ fork
 // heir[p]: the row that takes over row p's partly filled last block, -1 for row
 // p itself, else the lowest of the rows that copy it; kNoHeir: row p ends.
@@ -163,7 +182,8 @@ __global__ void __launch_bounds__(kMarkThreads) fork_mark_kernel(const PagesPara
     int status = 0;
     const int64_t units = static_cast<int64_t>(p.B) * p.chunks;
     for (int64_t u = blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5); u < units; u += warps) {
-        const int b = static_cast<int>(u / p.chunks), e0 = static_cast<int>(u - static_cast<int64_t>(b) * p.chunks) * kEntries;
+        int e0;
+        const int b = unit_row(p, u, e0);
         const int n = blocks_of(p, len[b]);
         uint32_t* bits = heir[b] == kNoHeir ? p.bits_b : p.bits_a;
         const int32_t* row = p.table + b * p.stride;
@@ -189,59 +209,79 @@ __global__ void __launch_bounds__(kMarkThreads) fork_mark_kernel(const PagesPara
     status = 0;
     // blocks that only ended rows held go on the stack, in the order of their ids
     const int fc = min(max(0, *p.count_in), p.NB);
-    int64_t w0, w1;
-    my_words(p, w0, w1);
-    int freed[1] = {0}, total[1];
-    for (int64_t w = w0; w < w1; ++w) freed[0] += __popc(__ldcg(p.bits_b + w) & ~__ldcg(p.bits_a + w));
-    cta_scan<1>(freed, total, sums);
-    int at = fc + freed[0];
-    for (int64_t w = w0; w < w1; ++w) {
-        uint32_t bits = __ldcg(p.bits_b + w) & ~__ldcg(p.bits_a + w);
-        p.bits_a[w] = p.bits_b[w] = 0;
-        for (; bits; bits &= bits - 1, ++at) {
-            if (at < p.NB) p.free_out[at] = static_cast<int32_t>(w * 32) + __ffs(bits) - 1;
-            else status |= KVD_STATUS_BAD_BLOCK;  // the list held blocks that rows held too
+    int pushed = 0;
+    for (int64_t base = 0; base < p.words; base += static_cast<int64_t>(blockDim.x) * kWords) {
+        const int64_t w = base + static_cast<int64_t>(threadIdx.x) * kWords;
+        uint32_t bits[kWords], on[kWords];
+        load_words(p, p.bits_b, w, bits);
+        load_words(p, p.bits_a, w, on);
+        int freed[1] = {0}, total[1];
+#pragma unroll
+        for (int i = 0; i < kWords; ++i) {
+            if (bits[i]) p.bits_b[w + i] = 0;
+            if (on[i]) p.bits_a[w + i] = 0;
+            bits[i] &= ~on[i];
+            freed[0] += __popc(bits[i]);
         }
+        cta_scan<1>(freed, total, sums);
+        int at = fc + pushed + freed[0];
+#pragma unroll
+        for (int i = 0; i < kWords; ++i)
+            for (; bits[i]; bits[i] &= bits[i] - 1, ++at) {
+                if (at < p.NB) p.free_out[at] = static_cast<int32_t>((w + i) * 32) + __ffs(bits[i]) - 1;
+                else status |= KVD_STATUS_BAD_BLOCK;  // the list held blocks that rows held too
+            }
+        pushed += total[0];
     }
-    const int height = min(p.NB, fc + total[0]);
+    const int height = min(p.NB, fc + pushed);
     __syncthreads();
     // a fresh block, from the top of the stack, for every row that needs a copy of a partly filled block
+    constexpr int N = 4;  // neighbouring rows a thread
     int carry = 0;
-    for (int b0 = 0; b0 < p.B; b0 += blockDim.x) {
-        const int b = b0 + threadIdx.x;
-        int from = -1, tail = 0, tail_id = -1;
-        if (b < p.B) {
-            from = p.parents[b];
-            if (from < 0 || from >= p.B) from = -1;
-        }
+    for (int base = 0; base < p.B; base += blockDim.x * N) {
+        int from[N], tail[N], tail_id[N];
         int copies[1] = {0}, all[1];
-        if (from >= 0) {
-            const int whole = static_cast<int>(p.by_bs.div(static_cast<uint32_t>(len[from])));
-            tail = len[from] - whole * p.bs;
-            const bool takes_over = heir[from] == -1 ? from == b : heir[from] == b;
-            if (tail > 0 && !takes_over) {
-                tail_id = p.table[from * p.stride + whole];
-                copies[0] = in_pool(p, tail_id);  // a bad id is passed on as it is
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const int b = base + threadIdx.x * N + i;
+            from[i] = -1;
+            tail[i] = 0;
+            tail_id[i] = -1;  // no copy; a bad id is passed on as it is
+            if (b >= p.B) continue;
+            const int f = p.parents[b];
+            if (f < 0 || f >= p.B) continue;
+            from[i] = f;
+            const int whole = static_cast<int>(p.by_bs.div(static_cast<uint32_t>(len[f])));
+            tail[i] = len[f] - whole * p.bs;
+            const bool takes_over = heir[f] == -1 ? f == b : heir[f] == b;
+            if (tail[i] > 0 && !takes_over) {
+                const int id = p.table[f * p.stride + whole];
+                if (in_pool(p, id)) tail_id[i] = id;
             }
         }
-        const bool wants = copies[0] != 0;
+#pragma unroll
+        for (int i = 0; i < N; ++i) copies[0] += tail_id[i] >= 0;
         cta_scan<1>(copies, all, sums);
-        const int k = carry + copies[0];
+        int k = carry + copies[0];
         carry += all[0];
-        if (b < p.B) {
-            const bool refused = wants && k >= height;
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const int b = base + threadIdx.x * N + i;
+            if (b >= p.B) continue;
+            const bool wants = tail_id[i] >= 0, refused = wants && k >= height;
             int id = kNoBlock;
             if (wants && !refused) {
                 id = p.free_out[height - 1 - k];
                 const bool good = in_pool(p, id);
                 if (!good) status |= KVD_STATUS_BAD_BLOCK;
-                p.src[k] = tail_id;
+                p.src[k] = tail_id[i];
                 p.dst[k] = id;
-                p.tokens[k] = good ? tail : 0;
+                p.tokens[k] = good ? tail[i] : 0;
             }
+            k += wants;
             if (refused) status |= KVD_STATUS_NO_BLOCKS;
             p.fresh[b] = id;
-            p.lens_out[b] = from >= 0 && !refused ? len[from] : 0;
+            p.lens_out[b] = from[i] >= 0 && !refused ? len[from[i]] : 0;
         }
     }
     if (threadIdx.x == 0) {
@@ -286,7 +326,10 @@ __device__ __forceinline__ void copy_head(const Pools& q, int from, int to, int 
     for (int t = lane; t < n; t += 32) d[t] = s[t];
     if (!v_side && q.bounds) {
         const int64_t a = (static_cast<int64_t>(from) * q.H + h) * 2 * q.D, b = (static_cast<int64_t>(to) * q.H + h) * 2 * q.D;
-        for (int i = lane; i < 2 * q.D; i += 32) q.bounds[b + i] = q.bounds[a + i];
+        const int pieces = q.bounds16 ? 2 * q.D / 16 : 0;
+        for (int i = lane; i < pieces; i += 32)
+            reinterpret_cast<uint4*>(q.bounds + b)[i] = reinterpret_cast<const uint4*>(q.bounds + a)[i];
+        for (int i = pieces * 16 + lane; i < 2 * q.D; i += 32) q.bounds[b + i] = q.bounds[a + i];
         if (lane == 0) q.bound_scale[static_cast<int64_t>(to) * q.H + h] = q.bound_scale[static_cast<int64_t>(from) * q.H + h];
     }
 }
@@ -296,9 +339,11 @@ __device__ __forceinline__ void copy_blocks(const PagesParams& p, const Pools& q
     const int lane = threadIdx.x & 31, per = 2 * q.H;
     const int64_t units = static_cast<int64_t>(*p.n_copies) * per, warps = gridDim.x * (blockDim.x >> 5);
     for (int64_t u = blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5); u < units; u += warps) {
-        const int k = static_cast<int>(u / per), rest = static_cast<int>(u - static_cast<int64_t>(k) * per);
+        const int k = units < 0x7fffffff ? static_cast<int>(static_cast<uint32_t>(u) / static_cast<uint32_t>(per)) : static_cast<int>(u / per);
+        const int rest = static_cast<int>(u - static_cast<int64_t>(k) * per);
         const int n = p.tokens ? p.tokens[k] : p.bs;
-        if (n > 0) copy_head<Vec>(q, p.src[k], p.dst[k], n, rest >= q.H, rest >= q.H ? rest - q.H : rest, lane);
+        const int from = p.src[k], to = p.dst[k];
+        if (n > 0) copy_head<Vec>(q, from, to, n, rest >= q.H, rest >= q.H ? rest - q.H : rest, lane);
     }
 }
 
@@ -310,7 +355,8 @@ __global__ void __launch_bounds__(kApplyThreads) fork_apply_kernel(const PagesPa
     const int lane = threadIdx.x & 31, warps = gridDim.x * (blockDim.x >> 5);
     const int64_t units = static_cast<int64_t>(p.B) * p.chunks;
     for (int64_t u = blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5); u < units; u += warps) {
-        const int b = static_cast<int>(u / p.chunks), e0 = static_cast<int>(u - static_cast<int64_t>(b) * p.chunks) * kEntries;
+        int e0;
+        const int b = unit_row(p, u, e0);
         const int from = p.parents[b];
         if (from < 0 || from >= p.B || (p.staged && from == b)) continue;
         const int n = blocks_of(p, p.lens_out[b]), fresh = p.fresh[b];
@@ -336,7 +382,8 @@ __global__ void __launch_bounds__(kMarkThreads) compact_mark_kernel(const PagesP
     int status = 0;
     const int64_t units = static_cast<int64_t>(p.B) * p.chunks;
     for (int64_t u = me; u < units; u += warps) {
-        const int b = static_cast<int>(u / p.chunks), e0 = static_cast<int>(u - static_cast<int64_t>(b) * p.chunks) * kEntries;
+        int e0;
+        const int b = unit_row(p, u, e0);
         const int n = blocks_of(p, row_len(p, b));
         if (e0 >= n) continue;
         const int32_t* row = p.table + b * p.stride;
@@ -422,7 +469,8 @@ __global__ void __launch_bounds__(kApplyThreads) compact_apply_kernel(const Page
     const int64_t units = static_cast<int64_t>(p.B) * p.chunks;
     const bool moved_only = p.table_out == p.table;
     for (int64_t u = blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5); u < units; u += warps) {
-        const int b = static_cast<int>(u / p.chunks), e0 = static_cast<int>(u - static_cast<int64_t>(b) * p.chunks) * kEntries;
+        int e0;
+        const int b = unit_row(p, u, e0);
         const int n = blocks_of(p, row_len(p, b));
         for (int e = e0 + lane; e < min(n, e0 + kEntries); e += 32) {
             const int id = p.table[b * p.stride + e];
@@ -495,7 +543,8 @@ int vec_bytes(const kvd_pages_desc& d, const void* K, const void* V) {
 Pools make_pools(const kvd_pages_desc& d, int8_t* K, int8_t* V, float* ks, float* vs, int8_t* bounds, float* bound_scale,
                  int vec) {
     return Pools{K, V, ks, vs, bounds, bound_scale, d.kv_stride_block, d.kv_stride_h, d.kv_stride_t, d.sc_stride_block,
-                 d.sc_stride_h, d.num_kv_heads, d.head_dim, FastDiv(static_cast<uint32_t>(d.head_dim / vec))};
+                 d.sc_stride_h, d.num_kv_heads, d.head_dim, FastDiv(static_cast<uint32_t>(d.head_dim / vec)),
+                 (reinterpret_cast<uintptr_t>(bounds) & 15) == 0 && d.head_dim % 8 == 0};
 }
 
 unsigned mark_grid(const PagesParams& p) {
