@@ -19,7 +19,8 @@ struct ChunkHead {
     int32_t units[kClasses];  // units: blocks of rows x KV heads x stretches of tokens
     int32_t span[kClasses];   // tokens of a stretch at most
     int32_t recs[kClasses];   // records of units whose tokens are split
-    int32_t pad[3];
+    int32_t ticket;           // units of many rows that have been taken
+    int32_t pad[2];
 };
 
 struct ChunkParams {

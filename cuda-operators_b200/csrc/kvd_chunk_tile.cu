@@ -26,7 +26,8 @@
 //         tokens, the K-major operand of q K^T and the MN-major one of P V; and
 //         the unit's queries;
 //   16    issues the MMAs;
-//   17    looks the tile's blocks up ahead: row offsets, scales.
+//   17    takes units from a ticket that all CTAs share, for the whole CTA, and
+//         looks its tiles' blocks up ahead: row offsets, scales.
 // Every wait is bounded; on expiry the kernel records KVD_STATUS_WAIT_TIMEOUT
 // and unwinds.
 #include "kvd_chunk.cuh"
@@ -42,6 +43,7 @@ constexpr int kConvWarps = 8, kConvThreads = 32 * kConvWarps;
 constexpr int kSoftmaxRegs = 136, kConvRegs = 72, kOtherRegs = 64;
 static_assert(256 * kSoftmaxRegs + kConvThreads * kConvRegs + 128 * kOtherRegs <= kThreads * 96, "registers of the launch");
 constexpr int kMetaStages = 4;
+constexpr int kUnitStages = 4;
 
 // What is known of a tile before it is read.
 struct TileMeta {
@@ -62,8 +64,9 @@ struct TileSmem {
     static constexpr int kMeta = 6 * kRows;
     static constexpr int kRf = kMeta + kMetaStages * static_cast<int>(sizeof(TileMeta));  // [2][256]
     static constexpr int kMl = kRf + 2 * 256 * 4;                                         // [2][128] m, l, ve
-    static constexpr int kBar = kMl + 2 * 128 * 16;
-    static constexpr int kBars = 2 * kMetaStages + 8 + 4 + 2 + 2 + 3;
+    static constexpr int kUnits = kMl + 2 * 128 * 16;  // [kUnitStages]
+    static constexpr int kBar = kUnits + kUnitStages * 4;
+    static constexpr int kBars = 2 * kMetaStages + 8 + 4 + 2 + 2 + 3 + 2 * kUnitStages;
     static constexpr int kTmem = kBar + kBars * 8;
     static constexpr int kBytes = kTmem + 16 + 1024;  // slack to align the base
 };
@@ -85,6 +88,8 @@ enum Bars {
     kMerge = kOFull + 2,
     kDone = kMerge + 1,
     kDrain = kDone + 1,
+    kUnitFull = kDrain + 1,
+    kUnitEmpty = kUnitFull + kUnitStages,
 };
 
 constexpr uint32_t kColO = 256;  // S and P: columns 0 and 128; O: 256 and 384
@@ -134,7 +139,7 @@ struct TileUnit {
     bool alt;            // the warpgroups take tiles in turn
 };
 
-// Later blocks of rows see more tokens and come first; blocks of one KV head lie together, for L2.
+// Later blocks of rows see more tokens and come first, so that the last units to be taken are short ones.
 template <int TERMS>
 __device__ __forceinline__ TileUnit tile_unit(const ChunkParams& p, int unit) {
     constexpr int ROWS = TERMS == 1 ? 256 : 128;
@@ -146,10 +151,10 @@ __device__ __forceinline__ TileUnit tile_unit(const ChunkParams& p, int unit) {
     int each;
     u.nsplit = chunk_splits(u.R.len, p.head->span[kMany], kTile, each);
     int rest = unit - p.first[kMany][u.b];
-    u.rb = u.nrb - 1 - rest % u.nrb;
-    rest /= u.nrb;
     u.hk = rest % p.Hkv;
-    u.split = rest / p.Hkv;
+    rest /= p.Hkv;
+    u.split = rest % u.nsplit;
+    u.rb = u.nrb - 1 - rest / u.nsplit;
     const int last = min(u.rows, (u.rb + 1) * ROWS) - 1;
     const int most = chunk_sees(p, u.R, static_cast<int>(p.by_g.div(static_cast<uint32_t>(last))));
     u.begin = u.split * each;
@@ -157,6 +162,18 @@ __device__ __forceinline__ TileUnit tile_unit(const ChunkParams& p, int unit) {
     u.nt = u.end > u.begin ? (u.end - u.begin + kTile - 1) / kTile : 0;
     u.alt = TERMS == 2 || u.rows - u.rb * ROWS <= 128;
     return u;
+}
+
+// The CTA's n-th unit, -1 behind the last one, for a warp; every role's warps ask for all of them.
+template <int D>
+__device__ __forceinline__ int next_unit(uint8_t* smem, uint64_t* bars, int& n) {
+    const int st = n & (kUnitStages - 1);
+    if (!mbar_wait_all(&bars[kUnitFull + st], (n / kUnitStages) & 1)) return -1;
+    const int unit = reinterpret_cast<const int*>(smem + TileSmem<D>::kUnits)[st];
+    __syncwarp();
+    if ((threadIdx.x & 31) == 0) mbar_arrive(&bars[kUnitEmpty + st]);
+    ++n;
+    return unit;
 }
 
 // ------------------------------------------------------------------ look-ahead
@@ -800,6 +817,10 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_tile_kernel(const __grid_co
         mbar_init(&bars[kMerge], 8);
         mbar_init(&bars[kDone], 8);
         mbar_init(&bars[kDrain], 1);
+        for (int s = 0; s < kUnitStages; ++s) {
+            mbar_init(&bars[kUnitFull + s], 1);
+            mbar_init(&bars[kUnitEmpty + s], 8 + kConvWarps + 1);  // softmax, converters, MMA issuer
+        }
         fence_mbar_init();
     }
     if (warp == 16) tmem_alloc(reinterpret_cast<uint32_t*>(smem + S::kTmem), 512);
@@ -812,7 +833,7 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_tile_kernel(const __grid_co
     if (warp < 8) {
         regs_more<kSoftmaxRegs>();
         int j = 0, nu = 0, ns = 0, no = 0, nm = 0;
-        for (int unit = blockIdx.x; unit < units; unit += gridDim.x) {
+        for (int n = 0, unit = next_unit<D>(smem, bars, n); unit >= 0; unit = next_unit<D>(smem, bars, n)) {
             const TileUnit u = tile_unit<TERMS>(p, unit);
             if (!tile_softmax<D, TERMS, FOLD>(p, u, smem, tmem, bars, j, nu, ns, no, nm)) break;
             j += u.nt;
@@ -824,7 +845,7 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_tile_kernel(const __grid_co
     } else if (warp < 8 + kConvWarps) {
         regs_less<kConvRegs>();
         int j = 0, nu = 0;
-        for (int unit = blockIdx.x; unit < units; unit += gridDim.x) {
+        for (int n = 0, unit = next_unit<D>(smem, bars, n); unit >= 0; unit = next_unit<D>(smem, bars, n)) {
             const TileUnit u = tile_unit<TERMS>(p, unit);
             if (u.nt == 0) continue;
             if (!tile_convert<D, TERMS, FOLD>(p, u, smem, bars, j, nu)) break;
@@ -836,7 +857,7 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_tile_kernel(const __grid_co
         if (warp == 16) {
             const int nq = p.flags & (KVD_FLAG_Q_BF16 | KVD_FLAG_Q_F16) ? 1 : 2;
             int j = 0, nu = 0, np[2] = {0, 0};
-            for (int unit = blockIdx.x; unit < units; unit += gridDim.x) {
+            for (int n = 0, unit = next_unit<D>(smem, bars, n); unit >= 0; unit = next_unit<D>(smem, bars, n)) {
                 const TileUnit u = tile_unit<TERMS>(p, unit);
                 if (u.nt == 0) continue;
                 if (!tile_mma<D, TERMS>(u, smem, tmem, bars, j, nu, np, nq)) break;
@@ -852,7 +873,18 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_tile_kernel(const __grid_co
         } else if (warp == 17) {
             int j = 0;
             bool ok = true;
-            for (int unit = blockIdx.x; unit < units && ok; unit += gridDim.x) {
+            for (int n = 0; ok; ++n) {
+                int unit = 0;
+                if (lane == 0) unit = atomicAdd(&p.head->ticket, 1);
+                unit = __shfl_sync(0xffffffffu, unit, 0);
+                const int st = n & (kUnitStages - 1);
+                ok = n < kUnitStages || mbar_wait_all(&bars[kUnitEmpty + st], ((n / kUnitStages) - 1) & 1);
+                if (!ok) break;
+                if (lane == 0) {
+                    reinterpret_cast<int*>(smem + S::kUnits)[st] = unit < units ? unit : -1;
+                    mbar_arrive(&bars[kUnitFull + st]);
+                }
+                if (unit >= units) break;
                 const TileUnit u = tile_unit<TERMS>(p, unit);
                 tile_scout(p, u, reinterpret_cast<TileMeta*>(smem + S::kMeta), bars, j, ok);
             }
