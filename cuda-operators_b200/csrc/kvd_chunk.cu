@@ -98,18 +98,21 @@ __global__ void __launch_bounds__(kAnyThreads) chunk_any_kernel(const ChunkParam
 
 // ---------------------------------------------------------------- plan
 // Which kernel takes a request, and how its tokens are split: one CTA looks at
-// all requests and, for each kernel, at five stretches that a unit may have at
-// most: no limit, and the work (tokens times units) over 1, 2, 3 and 4 times
-// the CTAs that run at once (1 and 2 for many rows). It takes the one whose estimate is least,
+// all requests and, for each kernel, at six stretches that a unit may have at
+// most: no limit, and the work (tokens times units) over a half to four times
+// the CTAs that run at once (twice for many rows). It takes the one whose estimate is least,
 //   max(longest stretch, rounds of CTAs x mean stretch)
 // for many rows (for few: the mean work of a CTA and half of the longest
 // stretch), each stretch with what a unit costs beside its tokens, then places every
 // request's units and records by prefix sums. Split units are fewer than twice
 // the work over the stretch: the room for their records. Bound: latency (loads,
 // two rounds of sums, one scan).
-constexpr int kSpans = 5;
-// The records of many rows are large: those are split into twice the CTAs' units at most.
-__host__ __device__ constexpr int span_parts(int cls, int k) { return cls == kMany && k > 2 ? 2 : k; }
+constexpr int kSpans = 6;
+// Units that stretch k aims at, in quarters of the CTAs that run at once (0: no limit). The records of many rows are
+// large: those are split into twice the CTAs' units at most.
+__host__ __device__ constexpr int span_quarters(int cls, int k) {
+    return k == 0 ? 0 : k == 1 ? 2 : k == 2 ? 3 : k == 3 ? 4 : cls == kMany ? 8 : k == 4 ? 8 : 16;
+}
 
 struct ChunkShape {
     int rows, units, len, cls;
@@ -151,8 +154,8 @@ __global__ void __launch_bounds__(1024) chunk_plan_kernel(const ChunkParams p) {
     auto shape_of = [&](int b) { return kept ? shapes[b] : chunk_shape(p, b); };
     auto span_of = [&](int cls, int k) {
         if (k == 0) return 0x40000000;
-        const unsigned long long parts = static_cast<unsigned long long>(span_parts(cls, k)) * (cls == 0 ? p.ctas[0] : cls == 1 ? p.ctas[1] : p.ctas[kMany]);
-        const unsigned long long s = (work[cls] + parts - 1) / parts, least = cls == kMany ? kTileMinSpan : kFewMinSpan;
+        const unsigned long long parts = static_cast<unsigned long long>(span_quarters(cls, k)) * (cls == 0 ? p.ctas[0] : cls == 1 ? p.ctas[1] : p.ctas[kMany]);
+        const unsigned long long s = (4 * work[cls] + parts - 1) / parts, least = cls == kMany ? kTileMinSpan : kFewMinSpan;
         return static_cast<int>(min(max(s, least), 0x40000000ull));
     };
     for (int64_t i = tid; i < static_cast<int64_t>(p.B) * kSpans; i += blockDim.x) {  // a thread per request and stretch
@@ -335,7 +338,7 @@ int64_t lay_out(const kvd_paged_prefill_desc& d, ChunkParams* p, uint8_t* base, 
         const int64_t least = cls == kMany ? kTileMinSpan : kFewMinSpan;
         const int64_t units = (d.num_rows * G / unit_rows + (d.batch < d.num_rows ? d.batch : d.num_rows)) * d.num_kv_heads;
         const int64_t splits = (cap + least - 1) / least, most = units * splits;
-        const int64_t ctas = cls == kMany ? sms : sms * chunk_few_ctas(d.head_dim, cls, true), room = 2 * span_parts(cls, kSpans - 1) * ctas;
+        const int64_t ctas = cls == kMany ? sms : sms * chunk_few_ctas(d.head_dim, cls, true), room = 2 * span_quarters(cls, kSpans - 1) * ctas / 4;
         return splits <= 1 || !has_class(d, cls) ? 0 : most < room ? most : room;
     };
     int64_t at = 0;
