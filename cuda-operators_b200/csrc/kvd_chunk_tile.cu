@@ -581,6 +581,20 @@ __device__ __forceinline__ float weights32(uint32_t col, const float4* ks4, cons
     return fmaxf(tm[0], tm[1]);
 }
 
+// 32 columns of a warp's 32 rows in pieces: lane l has rows l/4, +8, +16, +24 and, of every eight columns, 2 (l % 4)
+// and the next one.
+__device__ __forceinline__ void tmem_ld_rows(uint32_t col, uint32_t (&r)[32]) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+        asm volatile(
+            "tcgen05.ld.sync.aligned.16x256b.x4.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+            : "=r"(r[16 * h]), "=r"(r[16 * h + 1]), "=r"(r[16 * h + 2]), "=r"(r[16 * h + 3]), "=r"(r[16 * h + 4]),
+              "=r"(r[16 * h + 5]), "=r"(r[16 * h + 6]), "=r"(r[16 * h + 7]), "=r"(r[16 * h + 8]), "=r"(r[16 * h + 9]),
+              "=r"(r[16 * h + 10]), "=r"(r[16 * h + 11]), "=r"(r[16 * h + 12]), "=r"(r[16 * h + 13]),
+              "=r"(r[16 * h + 14]), "=r"(r[16 * h + 15])
+            : "r"(col + (static_cast<uint32_t>(16 * h) << 16)));
+}
+
 // The two softmax warpgroups meet (a bounded wait).
 __device__ __forceinline__ bool both_here(uint64_t* bars, int& count) {
     tc_fence_before();
@@ -756,20 +770,52 @@ __device__ __forceinline__ bool tile_softmax(const ChunkParams& p, const TileUni
     }
     const float inv = slot >= 0 ? 1.f : (l == 0.f ? 0.f : 1.f / l);  // no token in sight: 0; NaN stays
     const bool both = u.alt && u.nt > 1;
+    const uint32_t own = lanes + kColO + (u.alt && !any ? (w ^ 1) : w) * 128u, second = lanes + kColO + (w ^ 1) * 128u;
+    const float own_back = u.alt && !any ? other_back : back;
+    if constexpr (TERMS == 2)
+    if ((slot >= 0 || (p.vec_out && (p.flags & (KVD_FLAG_OUT_BF16 | KVD_FLAG_OUT_F16)) == 0))) {
+        // 32-bit rows: four lanes write 32 bytes of a row together, where a row a lane would write half sectors
+        // (one term has no registers left for this)
+        float* row_to = !there ? nullptr : slot >= 0 ? p.part_o[kMany] + rec * D : static_cast<float*>(p.out) + o_at;
+        float fa[4], fb[4];
+        float* to[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int from = 8 * i + (lane >> 2);
+            fa[i] = __shfl_sync(0xffffffffu, own_back * inv, from);
+            fb[i] = __shfl_sync(0xffffffffu, other_back * inv, from);
+            to[i] = reinterpret_cast<float*>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(row_to), from));
+        }
+#pragma unroll 1
+        for (int d = d0; d < d1; d += 32) {
+            uint32_t o[32], o2[32];
+            tmem_ld_rows(own + d, o);
+            if (both) tmem_ld_rows(second + d, o2);
+            tmem_wait_ld();
+#pragma unroll
+            for (int y = 0; y < 32; y += 2) {
+                const int i = 2 * (y >> 4) + ((y >> 1) & 1), k = (y >> 2) & 3;
+                float2 x = fa[i] == 0.f ? make_float2(0.f, 0.f) : make_float2(__uint_as_float(o[y]) * fa[i], __uint_as_float(o[y + 1]) * fa[i]);
+                if (both && fb[i] != 0.f)
+                    x = make_float2(fmaf(__uint_as_float(o2[y]), fb[i], x.x), fmaf(__uint_as_float(o2[y + 1]), fb[i], x.y));
+                if (to[i]) *reinterpret_cast<float2*>(to[i] + d + 8 * k + 2 * (lane & 3)) = x;
+            }
+        }
+        d1 = d0;  // done
+    }
 #pragma unroll 1
     for (int d = d0; d < d1; d += 32) {
         float x[32];
         {
             uint32_t o[32];
-            tmem_ld32(lanes + kColO + (u.alt && !any ? (w ^ 1) : w) * 128u + d, o);
+            tmem_ld32(own + d, o);
             tmem_wait_ld();
-            const float f = u.alt && !any ? other_back : back;
 #pragma unroll
-            for (int y = 0; y < 32; ++y) x[y] = f == 0.f ? 0.f : __uint_as_float(o[y]) * f;
+            for (int y = 0; y < 32; ++y) x[y] = own_back == 0.f ? 0.f : __uint_as_float(o[y]) * own_back;
         }
         if (both) {
             uint32_t o[32];
-            tmem_ld32(lanes + kColO + (w ^ 1) * 128u + d, o);
+            tmem_ld32(second + d, o);
             tmem_wait_ld();
 #pragma unroll
             for (int y = 0; y < 32; ++y) x[y] = other_back == 0.f ? x[y] : fmaf(__uint_as_float(o[y]), other_back, x[y]);
