@@ -135,11 +135,12 @@ constexpr int kPlanShapes = 1024;  // requests whose shapes the plan keeps in sh
 
 __global__ void __launch_bounds__(1024) chunk_plan_kernel(const ChunkParams p) {
     __shared__ ChunkShape shapes[kPlanShapes];
-    __shared__ unsigned long long work[kClasses];
+    __shared__ unsigned long long work[kClasses], claimed;
     __shared__ int units_at[kClasses * kSpans], longest_at[kClasses * kSpans], span[kClasses];
     __shared__ int sums[2 * kClasses][32];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, nw = blockDim.x >> 5;
     if (tid < kClasses) work[tid] = 0;
+    if (tid == 0) claimed = 0;
     if (tid < kClasses * kSpans) units_at[tid] = longest_at[tid] = 0;
     grid_dependency_wait();
     allow_dependents();
@@ -148,9 +149,14 @@ __global__ void __launch_bounds__(1024) chunk_plan_kernel(const ChunkParams p) {
     for (int b = tid; b < p.B; b += blockDim.x) {
         const ChunkShape s = chunk_shape(p, b);
         if (kept) shapes[b] = s;
-        if (s.units) atomicAdd(&work[s.cls], static_cast<unsigned long long>(s.units) * s.len);
+        if (s.units) {
+            atomicAdd(&work[s.cls], static_cast<unsigned long long>(s.units) * s.len);
+            atomicAdd(&claimed, static_cast<unsigned long long>(s.units));
+        }
     }
     __syncthreads();
+    // Rows times heads are at most 2^30, so starts that ascend give fewer units than this; others may give nothing.
+    const bool sane = claimed < 0x50000000ull;
     auto shape_of = [&](int b) { return kept ? shapes[b] : chunk_shape(p, b); };
     auto span_of = [&](int cls, int k) {
         if (k == 0) return 0x40000000;
@@ -161,7 +167,7 @@ __global__ void __launch_bounds__(1024) chunk_plan_kernel(const ChunkParams p) {
     for (int64_t i = tid; i < static_cast<int64_t>(p.B) * kSpans; i += blockDim.x) {  // a thread per request and stretch
         const int b = static_cast<int>(i / kSpans), k = static_cast<int>(i - static_cast<int64_t>(b) * kSpans);
         const ChunkShape s = shape_of(b);
-        if (s.units == 0) continue;
+        if (s.units == 0 || !sane) continue;
         int each;
         const int n = chunk_splits(s.len, span_of(s.cls, k), chunk_step(s.cls), each);
         atomicAdd(&units_at[s.cls * kSpans + k], s.units * n);
@@ -189,46 +195,59 @@ __global__ void __launch_bounds__(1024) chunk_plan_kernel(const ChunkParams p) {
         span[tid] = span_of(tid, best);
     }
     __syncthreads();
-    int carry[2 * kClasses] = {};
-    for (int b0 = 0; b0 < p.B; b0 += blockDim.x) {
-        const int b = b0 + tid;
-        int x[2 * kClasses] = {}, inc[2 * kClasses];
-        if (b < p.B) {
-            const ChunkShape s = shape_of(b);
-            int each;
-            const int n = chunk_splits(s.len, span[s.cls], chunk_step(s.cls), each);
+    // Starts that do not ascend may give more rows than the call has, and more records than there is room for: no
+    // stretch has a limit then.
+    int carry[2 * kClasses];
+    bool fits = false;
+    for (int attempt = 0; attempt < 2 && !fits; ++attempt) {
 #pragma unroll
-            for (int c = 0; c < kClasses; ++c) {
-                x[2 * c] = c == s.cls ? s.units * n : 0;
-                x[2 * c + 1] = c == s.cls && n > 1 ? s.units * n : 0;
+        for (int i = 0; i < 2 * kClasses; ++i) carry[i] = 0;
+        for (int b0 = 0; b0 < p.B; b0 += blockDim.x) {
+            const int b = b0 + tid;
+            int x[2 * kClasses] = {}, inc[2 * kClasses];
+            if (b < p.B && sane) {
+                const ChunkShape s = shape_of(b);
+                int each;
+                const int n = chunk_splits(s.len, span[s.cls], chunk_step(s.cls), each);
+#pragma unroll
+                for (int c = 0; c < kClasses; ++c) {
+                    x[2 * c] = c == s.cls ? s.units * n : 0;
+                    x[2 * c + 1] = c == s.cls && n > 1 ? s.units * n : 0;
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < 2 * kClasses; ++i) {
+                inc[i] = x[i];
+#pragma unroll
+                for (int o = 1; o < 32; o <<= 1) {
+                    const int y = __shfl_up_sync(0xffffffffu, inc[i], o);
+                    if (lane >= o) inc[i] += y;
+                }
+            }
+            __syncthreads();
+            if (lane == 31)
+#pragma unroll
+                for (int i = 0; i < 2 * kClasses; ++i) sums[i][warp] = inc[i];
+            __syncthreads();
+#pragma unroll
+            for (int i = 0; i < 2 * kClasses; ++i) {
+                int s = lane < nw ? sums[i][lane] : 0;
+#pragma unroll
+                for (int o = 1; o < 32; o <<= 1) {
+                    const int y = __shfl_up_sync(0xffffffffu, s, o);
+                    if (lane >= o) s += y;
+                }
+                const int upto = __shfl_sync(0xffffffffu, s, (warp - 1) & 31), all = __shfl_sync(0xffffffffu, s, 31);
+                int32_t* to = i & 1 ? p.rec[i >> 1] : p.first[i >> 1];
+                if (b < p.B) to[b] = carry[i] + (warp > 0 ? upto : 0) + inc[i] - x[i];
+                carry[i] += all;
             }
         }
-#pragma unroll
-        for (int i = 0; i < 2 * kClasses; ++i) {
-            inc[i] = x[i];
-#pragma unroll
-            for (int o = 1; o < 32; o <<= 1) {
-                const int y = __shfl_up_sync(0xffffffffu, inc[i], o);
-                if (lane >= o) inc[i] += y;
-            }
-        }
-        __syncthreads();
-        if (lane == 31)
-#pragma unroll
-            for (int i = 0; i < 2 * kClasses; ++i) sums[i][warp] = inc[i];
-        __syncthreads();
-#pragma unroll
-        for (int i = 0; i < 2 * kClasses; ++i) {
-            int s = lane < nw ? sums[i][lane] : 0;
-#pragma unroll
-            for (int o = 1; o < 32; o <<= 1) {
-                const int y = __shfl_up_sync(0xffffffffu, s, o);
-                if (lane >= o) s += y;
-            }
-            const int upto = __shfl_sync(0xffffffffu, s, (warp - 1) & 31), all = __shfl_sync(0xffffffffu, s, 31);
-            int32_t* to = i & 1 ? p.rec[i >> 1] : p.first[i >> 1];
-            if (b < p.B) to[b] = carry[i] + (warp > 0 ? upto : 0) + inc[i] - x[i];
-            carry[i] += all;
+        fits = carry[1] <= p.max_recs[0] && carry[3] <= p.max_recs[1] && carry[5] <= p.max_recs[kMany];
+        if (!fits) {
+            __syncthreads();
+            if (tid < kClasses) span[tid] = 0x40000000;
+            __syncthreads();
         }
     }
 #pragma unroll
@@ -354,6 +373,7 @@ int64_t lay_out(const kvd_paged_prefill_desc& d, ChunkParams* p, uint8_t* base, 
         p->first[c] = reinterpret_cast<int32_t*>(take(4 * entries));
         p->rec[c] = reinterpret_cast<int32_t*>(take(4 * entries));
         int64_t rows = records(c, p->unit_rows[c]) * p->unit_rows[c];
+        p->max_recs[c] = static_cast<int>(rows / p->unit_rows[c]);
         if (c == kMany) {
             const int64_t x = 128 * records(c, 128), y = 256 * records(c, 256);
             rows = x > y ? x : y;

@@ -49,6 +49,7 @@ struct ChunkParams {
     int unit_rows[kClasses];
     int ctas[kClasses];         // CTAs that run at once
     int32_t* arrived[kMany];    // [slot] units of the classes with few rows that have written their records
+    int max_recs[kClasses];     // room for records
     int tiny_most, few_most;    // rows up to which a request is of the first class, of the second
 };
 

@@ -394,6 +394,23 @@ def test_starts_that_do_not_fit_are_clamped():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("T,B", [(3, 40), (200, 40)])
+def test_starts_that_go_back_and_forth_stay_inside_the_workspace(T, B):
+    """Every second request claims all rows: their work must not need more records than the workspace has room for."""
+    import torch
+
+    s = make_case(B, [T] * B, [9000] * B, 2, 4, 128, 16, "bfloat16", seed=21)
+    q = s["q"][:T].contiguous()
+    starts = torch.tensor([0, T] * (B // 2) + [0], dtype=torch.int32, device=DEV)
+    size = kvd.paged_prefill_workspace_size(q, s["K"], s["table"])
+    ws = torch.full((size + (64 << 20),), 171, dtype=torch.uint8, device=DEV)
+    out = kvd.paged_prefill(q, s["K"], s["V"], s["ks"], s["vs"], s["table"], s["lens"], starts, workspace=ws[:size])
+    torch.cuda.synchronize()
+    assert bool((ws[size:] == 171).all()) and torch.isfinite(out).all()
+    assert kvd.device_status() == 0
+
+
+@pytest.mark.gpu
 def test_no_rows():
     import torch
 
