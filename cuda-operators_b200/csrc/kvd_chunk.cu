@@ -146,13 +146,20 @@ __global__ void __launch_bounds__(1024) chunk_plan_kernel(const ChunkParams p) {
     allow_dependents();
     __syncthreads();
     const bool kept = p.B <= kPlanShapes;
+    unsigned long long mine[kClasses + 1] = {};  // work of each class, units of all
     for (int b = tid; b < p.B; b += blockDim.x) {
         const ChunkShape s = chunk_shape(p, b);
         if (kept) shapes[b] = s;
-        if (s.units) {
-            atomicAdd(&work[s.cls], static_cast<unsigned long long>(s.units) * s.len);
-            atomicAdd(&claimed, static_cast<unsigned long long>(s.units));
-        }
+#pragma unroll
+        for (int c = 0; c < kClasses; ++c)
+            if (c == s.cls) mine[c] += static_cast<unsigned long long>(s.units) * s.len;
+        mine[kClasses] += s.units;
+    }
+#pragma unroll
+    for (int c = 0; c <= kClasses; ++c) {  // (64-bit adds to shared memory are slow: one a warp)
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) mine[c] += __shfl_xor_sync(0xffffffffu, mine[c], o);
+        if (lane == 0 && mine[c]) atomicAdd(c < kClasses ? &work[c] : &claimed, mine[c]);
     }
     __syncthreads();
     // Rows times heads are at most 2^30, so starts that ascend give fewer units than this; others may give nothing.

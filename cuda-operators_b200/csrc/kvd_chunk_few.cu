@@ -205,17 +205,23 @@ __global__ void __launch_bounds__(kFewWarps * 32, FewSmem<D, NR, NQ>::kCtas) chu
             for (int d = 0; d < CH * 16; ++d) top = fmaxf(top, fabsf(x[d]));
             top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
             top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-            const int k = fit_exponent(top, 15);  // below 2^15: products of 128 dims stay far from fp32's end
+            // Two terms: whole numbers below 2^11, whose products with the codes add up without loss, and what is left.
+            // One: below 2^15, products of 128 dims stay far from fp32's end.
+            const int k = fit_exponent(top, NQ == 2 ? 11 : 15);
             const float f = pow2i(k);
             factor[e] = p.qscale * pow2i(-k);
 #pragma unroll
             for (int s = 0; s < KS; ++s) {  // a word of four codes is a step: even dims in one pair, odd ones in the other
                 const float* y = x + s * 4;
-                qb[0][e][s][0] = pack_half(y[0] * f, y[2] * f);
-                qb[0][e][s][1] = pack_half(y[1] * f, y[3] * f);
+                const float a = y[0] * f, b = y[1] * f, c2 = y[2] * f, d = y[3] * f;
                 if constexpr (NQ == 2) {
-                    qb[1][e][s][0] = pack_rest(y[0] * f, y[2] * f, qb[0][e][s][0]);
-                    qb[1][e][s][1] = pack_rest(y[1] * f, y[3] * f, qb[0][e][s][1]);
+                    qb[0][e][s][0] = pack_half(rintf(a), rintf(c2));
+                    qb[0][e][s][1] = pack_half(rintf(b), rintf(d));
+                    qb[1][e][s][0] = pack_rest(a, c2, qb[0][e][s][0]);
+                    qb[1][e][s][1] = pack_rest(b, d, qb[0][e][s][1]);
+                } else {
+                    qb[0][e][s][0] = pack_half(a, c2);
+                    qb[0][e][s][1] = pack_half(b, d);
                 }
             }
         }
@@ -253,9 +259,9 @@ __global__ void __launch_bounds__(kFewWarps * 32, FewSmem<D, NR, NQ>::kCtas) chu
 #pragma unroll
             for (int mt = 0; mt < 2; ++mt) {
 #pragma unroll
-                for (int e = 0; e < NR; ++e) {
-                    s[mt][e][0] = s[mt][e][1] = s[mt][e][2] = s[mt][e][3] = 0.f;
-                }
+                for (int e = 0; e < NR; ++e) s[mt][e][0] = s[mt][e][1] = s[mt][e][2] = s[mt][e][3] = 0.f;
+                // the second term's sum by itself: a sum is cut off, not rounded, behind every step, by a unit of its size
+                float s2[NR][4] = {};
 #pragma unroll
                 for (int h = 0; h < CH; ++h) {
                     const uint4 a4 = *reinterpret_cast<const uint4*>(st + k_at<D>(mt * 16 + quad, h * 4 + c));
@@ -267,10 +273,15 @@ __global__ void __launch_bounds__(kFewWarps * 32, FewSmem<D, NR, NQ>::kCtas) chu
 #pragma unroll
                         for (int e = 0; e < NR; ++e) {
                             mma_16816(s[mt][e], a, qb[0][e][h * 4 + x][0], qb[0][e][h * 4 + x][1]);
-                            if constexpr (NQ == 2) mma_16816(s[mt][e], a, qb[1][e][h * 4 + x][0], qb[1][e][h * 4 + x][1]);
+                            if constexpr (NQ == 2) mma_16816(s2[e], a, qb[1][e][h * 4 + x][0], qb[1][e][h * 4 + x][1]);
                         }
                     }
                 }
+                if constexpr (NQ == 2)
+#pragma unroll
+                    for (int e = 0; e < NR; ++e)
+#pragma unroll
+                        for (int x = 0; x < 4; ++x) s[mt][e][x] += s2[e][x];
             }
             float top[NR][2];
 #pragma unroll

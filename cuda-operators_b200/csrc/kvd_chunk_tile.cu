@@ -357,14 +357,18 @@ __device__ __forceinline__ void load_queries(const ChunkParams& p, const TileUni
         for (int d = 0; d < 16; ++d) top = fmaxf(top, fabsf(x[d]));
 #pragma unroll
         for (int o = 1; o < PER; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-        const int k = fit_exponent(top, 15);
+        // Two terms (32-bit rows): whole numbers below 2^11, whose products with the codes add up without loss, and what
+        // is left. (A product's sum is cut off, not rounded, behind every step, by a unit of its size.)
+        const bool whole = TERMS == 2 && (p.flags & (KVD_FLAG_Q_BF16 | KVD_FLAG_Q_F16)) == 0;
+        const int k = fit_exponent(top, whole ? 11 : 15);
         const float f = pow2i(k);
         if (c16 == 0) rf[r] = p.qscale * pow2i(-k);
         uint32_t hi[8], lo[8];
 #pragma unroll
         for (int d = 0; d < 8; ++d) {
-            hi[d] = pack_half(x[2 * d] * f, x[2 * d + 1] * f);
-            if (TERMS == 2) lo[d] = pack_rest(x[2 * d] * f, x[2 * d + 1] * f, hi[d]);
+            const float a = x[2 * d] * f, b = x[2 * d + 1] * f;
+            hi[d] = whole ? pack_half(rintf(a), rintf(b)) : pack_half(a, b);
+            if (TERMS == 2) lo[d] = pack_rest(a, b, hi[d]);
         }
         uint8_t* tile = q + (r >> 7) * TileSmem<D>::kRows;
         const int col = c16 >> 2, ch = (c16 & 3) * 2, rr = r & 127;
@@ -448,15 +452,16 @@ __device__ __forceinline__ bool tile_mma(const TileUnit& u, uint8_t* smem, uint3
         if ((u.alt || w == 0) && !mbar_wait_all(&bars[kKFull + st], (j >> 1) & 1)) return false;
         tc_fence_after();
         const uint64_t kd = smem_desc(smem_u32(smem + S::kK + st * S::kRows), 16u, 1024u, kLayoutSw128);
+        // the smaller term first
 #pragma unroll
-        for (int t = 0; t < TERMS; ++t) {
+        for (int t = TERMS - 1; t >= 0; --t) {
             if (t < nq) {
                 const int tile = TERMS == 2 ? t : (u.alt ? 0 : w);
                 const uint64_t qd = smem_desc(smem_u32(smem + S::kQ + tile * S::kRows), 16u, 1024u, kLayoutSw128);
 #pragma unroll
                 for (int k = 0; k < D / 16; ++k) {
                     const uint64_t step = ((k >> 2) * 16384u + (k & 3) * 32u) >> 4;
-                    mma_f16_ss_warp(tmem + w * 128u, qd + step, kd + step, id_s, t > 0 || k > 0);
+                    mma_f16_ss_warp(tmem + w * 128u, qd + step, kd + step, id_s, t < nq - 1 || k > 0);
                 }
             }
         }
