@@ -390,6 +390,8 @@ int64_t lay_out(const kvd_paged_prefill_desc& d, ChunkParams* p, uint8_t* base, 
         if (c < kMany) p->arrived[c] = reinterpret_cast<int32_t*>(take(4 * rows / p->unit_rows[c]));
         else split |= rows > 0;
     }
+    p->aside = reinterpret_cast<float4*>(take(has_class(d, kMany) && cap > kAsideTiles * kTile ? 4LL * sms * 2 * 128 * D : 0));
+    p->aside_tiles = (d.flags & o16) != 0 ? kAsideTiles16 : kAsideTiles;
     return at;
 }
 

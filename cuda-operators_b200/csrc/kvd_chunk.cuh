@@ -50,6 +50,8 @@ struct ChunkParams {
     int ctas[kClasses];         // CTAs that run at once
     int32_t* arrived[kMany];    // [slot] units of the classes with few rows that have written their records
     int max_recs[kClasses];     // room for records
+    float4* aside;              // [CTA][2][D / 4][128] sums that the kernel for many rows puts aside
+    int aside_tiles;            // after how many tiles
     int tiny_most, few_most;    // rows up to which a request is of the first class, of the second
 };
 
@@ -59,6 +61,11 @@ constexpr int kTileMinSpan = 512;
 // What a unit costs beside its tokens, in tokens.
 constexpr float kFewExtra = 512.f, kTileExtra = 400.f;
 constexpr int kTile = 128;       // tokens of a tile of the kernel for many rows
+// A product of 16 tokens on the tensor cores cuts the sum that it adds to off, towards zero: 32,768 tokens of values
+// above zero, in one stretch of two terms, came out 1.07e-4 too small. So a warpgroup puts its sums aside, added with
+// rounding, and starts again from zero after this many of its tiles, 64 products of a 32-bit output (1.5e-6 then),
+// 512 of a 16-bit one. Powers of two.
+constexpr int kAsideTiles = 4, kAsideTiles16 = 64;
 
 // Rows [t0, t0 + n) of request b and its tokens.
 struct ChunkRows {

@@ -384,8 +384,15 @@ __global__ void __launch_bounds__(kFewWarps * 32, FewSmem<D, NR, NQ>::kCtas) chu
                         const uint32_t a[4] = {half_pair(lo), half_pair(lo >> 8), half_pair(hi), half_pair(hi >> 8)};
 #pragma unroll
                         for (int e = 0; e < NR; ++e) {
-                            mma_16816(o[e][2 * y + z], a, pb[0][e][0], pb[0][e][1]);
-                            if constexpr (NP == 2) mma_16816(o[e][2 * y + z], a, pb[1][e][0], pb[1][e][1]);
+                            if constexpr (NP == 1) {
+                                mma_16816(o[e][2 * y + z], a, pb[0][e][0], pb[0][e][1]);
+                            } else {  // sums by themselves: a product cuts off what it adds to, towards zero
+                                float sum[4] = {};
+                                mma_16816(sum, a, pb[1][e][0], pb[1][e][1]);
+                                mma_16816(sum, a, pb[0][e][0], pb[0][e][1]);
+#pragma unroll
+                                for (int x = 0; x < 4; ++x) o[e][2 * y + z][x] += sum[x];
+                            }
                         }
                     }
             }

@@ -611,6 +611,52 @@ __device__ __forceinline__ bool both_here(uint64_t* bars, int& count) {
     return ok;
 }
 
+// What sums that were put aside with the reference and the exponent `of` (x, z) are worth with these.
+__device__ __forceinline__ float aside_factor(const float4& of, float m, int ve) {
+    const int fall = __float_as_int(of.z) - ve;
+    return of.x == -INFINITY || fall > 126 ? 0.f : ex2_fast(of.x - m) * pow2i(-fall);
+}
+
+// Adds this thread's row of O to the sums that it has put aside, and starts O again from zero. The sums keep the
+// reference and exponent of the first time (`of`), which O is raised to on its way, so that nothing waits for
+// them; once that is too far, they are read and lowered instead.
+template <int D>
+__device__ __forceinline__ void put_aside(float4* aside, float4* of, uint32_t col_o, bool first, float m, int ve) {
+    float f = 0.f;  // times the old sums, or times O
+    bool read = false;
+    if (!first) {
+        const float4 was = *of;
+        const float up = m - was.x;
+        const int fall = __float_as_int(was.z) - ve;
+        read = __any_sync(0xffffffffu, m != -INFINITY && !(up + static_cast<float>(fall) <= 60.f));
+        f = read ? aside_factor(was, m, ve) : m == -INFINITY ? 0.f : ex2_fast(up) * pow2i(fall);
+    }
+    if (first || read) *of = make_float4(m, 0.f, __int_as_float(ve), 0.f);
+#pragma unroll 1
+    for (int d = 0; d < D; d += 32) {
+        uint32_t o[32];
+        tmem_ld32(col_o + d, o);
+        tmem_wait_ld();
+#pragma unroll
+        for (int x = 0; x < 32; x += 4) {
+            float4* at = aside + (d + x) / 4 * 128;
+            float4 y = make_float4(__uint_as_float(o[x]), __uint_as_float(o[x + 1]), __uint_as_float(o[x + 2]), __uint_as_float(o[x + 3]));
+            if (first || read) {
+                if (f != 0.f) {
+                    const float4 z = __ldcg(at);
+                    y = make_float4(fmaf(z.x, f, y.x), fmaf(z.y, f, y.y), fmaf(z.z, f, y.z), fmaf(z.w, f, y.w));
+                }
+                __stcg(at, y);
+            } else {
+                asm volatile("red.relaxed.gpu.global.add.v4.f32 [%0], {%1, %2, %3, %4};" ::"l"(at), "f"(y.x * f), "f"(y.y * f),
+                             "f"(y.z * f), "f"(y.w * f) : "memory");
+            }
+            o[x] = o[x + 1] = o[x + 2] = o[x + 3] = 0u;
+        }
+        tmem_st32(col_o + d, o);
+    }
+}
+
 template <int D, int TERMS, bool FOLD>
 __device__ __forceinline__ bool tile_softmax(const ChunkParams& p, const TileUnit& u, uint8_t* smem, uint32_t tmem, uint64_t* bars, int j0,
                                              int nu, int& ns, int& no, int& nm_sync) {
@@ -659,10 +705,12 @@ __device__ __forceinline__ bool tile_softmax(const ChunkParams& p, const TileUni
         tc_fence_after();
         const int lim = min(sees, u.end) - t0;  // tokens of the tile that the row sees
         const bool masked = t0 + kTile > least;
+        const int own_tile = u.alt ? tile >> 1 : tile;
+        const bool full = own_tile != 0 && (own_tile & (p.aside_tiles - 1)) == 0;  // O holds as many as it should
         bool done = false;
         if constexpr (TERMS == 1) {
             // With the reference of the tiles before: one pass. It stands unless a score is above it by more than 8.
-            if (!masked && __all_sync(0xffffffffu, m != -INFINITY) && ve_now == ve) {
+            if (!masked && !full && __all_sync(0xffffffffu, m != -INFINITY) && ve_now == ve) {
                 uint32_t pk[kTile / 2];
                 float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
                 float top = -INFINITY;
@@ -689,6 +737,9 @@ __device__ __forceinline__ bool tile_softmax(const ChunkParams& p, const TileUni
                 for (int q = 0; q < 4; ++q) top = fmaxf(top, top32<false>(col_s + 32u * q, ks4 + 8 * q, 0));
             }
             top *= rf;  // rf > 0: -inf stays
+            if (full)  // this warpgroup's products before this tile's scores are complete: O may change
+                put_aside<D>(p.aside + (blockIdx.x * 2 + w) * (D / 4) * 128 + r, reinterpret_cast<float4*>(smem + S::kMl) + w * 128 + r,
+                             col_o, own_tile == p.aside_tiles, m, ve);
             const bool move = top > m + (m == -INFINITY ? 0.f : 8.f);
             if (any && __any_sync(0xffffffffu, (move && m != -INFINITY) || ve_now != ve)) {
                 // this warpgroup's products before this tile's scores are complete: O may change
@@ -752,6 +803,28 @@ __device__ __forceinline__ bool tile_softmax(const ChunkParams& p, const TileUni
         ++no;
     }
     tc_fence_after();
+    if ((u.alt ? (u.nt - w + 1) / 2 : u.nt) > p.aside_tiles) {  // sums were put aside: they come back
+        const float4* aside = p.aside + (blockIdx.x * 2 + w) * (D / 4) * 128 + r;
+        const float f = aside_factor(reinterpret_cast<const float4*>(smem + S::kMl)[w * 128 + r], m, ve);
+#pragma unroll 1
+        for (int d = 0; d < D; d += 32) {
+            uint32_t o[32];
+            tmem_ld32(col_o + d, o);
+            tmem_wait_ld();
+#pragma unroll
+            for (int x = 0; x < 32; x += 4) {
+                const float4 y = __ldcg(aside + (d + x) / 4 * 128);
+                if (f != 0.f) {
+                    o[x] = __float_as_uint(fmaf(y.x, f, __uint_as_float(o[x])));
+                    o[x + 1] = __float_as_uint(fmaf(y.y, f, __uint_as_float(o[x + 1])));
+                    o[x + 2] = __float_as_uint(fmaf(y.z, f, __uint_as_float(o[x + 2])));
+                    o[x + 3] = __float_as_uint(fmaf(y.w, f, __uint_as_float(o[x + 3])));
+                }
+            }
+            tmem_st32(col_o + d, o);
+        }
+        tmem_wait_st();
+    }
     float l = (lp[0].x + lp[0].y) + (lp[1].x + lp[1].y);
     float back = pow2i(-ve), other_back = 0.f;
     int d0 = 0, d1 = D;

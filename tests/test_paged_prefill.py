@@ -17,6 +17,11 @@ per element, against it:
 * where the output is bf16 a value's scale and its product with the code enter as
   fp16 too: two more half steps, 3 2^-11 sum_j p_j |v_j| with the weights' (whose
   products with each other, below 2^-20, the first term covers);
+* 32-bit outputs have two fp16 terms of a weight, whose steps end at 2^-24: half of
+  that, 2^-25, of a reference that is at least 2^6 of the largest value scale, is
+  2^-31 of the largest |v| a token, however small the weight: 2^-31 len max |v|.
+  (It shows where a token that outweighs all others has a code of 0 and values are
+  far above 1, so that 2e-5 is nothing);
 * the scores: with A = max_j sum_d |q_d k_jd| ks_j scale, rounding the queries to
   two fp16 terms (22 bits) moves a score by at most 2^-22 A, and each of the 16
   fp32 sums of 16 dims (8, times 2 terms) by half a step of at most 2^-24 A:
@@ -116,6 +121,8 @@ def close(got, s, want, dtype=None):
     if dtype != torch.float32:
         tol = tol + torch.finfo(dtype).eps / 2 * out.abs() + 2.0 ** -25 + 2.0 ** -17 * top
         tol = tol + (3 if dtype == torch.bfloat16 else 1) * 2.0 ** -11 * mean
+    else:
+        tol = tol + 2.0 ** -31 * float(s["len"].max()) * top
     rows = torch.zeros(got.shape[0], dtype=torch.bool, device=DEV)
     for b in range(len(s["n"])):
         rows[int(s["starts_host"][b]): int(s["starts_host"][b + 1])] = True
@@ -199,6 +206,44 @@ def test_scales_of_very_different_sizes(dtype, n):
     check(s)
     s["vs"].zero_()
     check(s)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("D", [128, 64])
+@pytest.mark.parametrize("later_k,later_v", [(1.0, 1.0), (100.0, 1.0), (1.0, 1e22), (1.0, 1e-22), (100.0, 1e22)])
+def test_sums_of_long_rows_when_later_tokens_weigh_more(D, later_k, later_v):
+    # 32-bit outputs of long rows are summed in parts, with references that may lie far from each other
+    s = make_case(18, [128] * 18, [6000 - 130 * (b % 3) for b in range(18)], 8, 1, D, 16, "float32", seed=4)
+    late = s["table"].long()[:, 200:375].clamp(0, s["ks"].shape[0] - 1).flatten()  # blocks of tokens from 3,200 on
+    if later_v > 1:
+        s["vs"] *= 1e-11  # so that their sums stay far from fp32's end
+    s["ks"][late] *= later_k
+    s["vs"][late] *= later_v
+    check(s)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("n,dtype,products", [(2, "float32", 64), (128, "float32", 64), (128, "float16", 512)])
+def test_sums_of_long_rows_do_not_drift(n, dtype, products):
+    # A product on the tensor cores cuts a sum off, at 2^-23 of it at most, always towards zero. With values above
+    # zero all losses of a row have one sign: 32,768 tokens are 2,048 products of 16, or twice as many in two terms.
+    # Sums in parts of at most so many products lose 2^-23 of a part each (parts are added with rounding to nearest,
+    # whose error has no sign, and neither has that of fp16 weights and outputs: 2^-11 over the root of 10^6 values);
+    # weights of two terms (2^-22), exponentials (2^-22) and the sum of weights are counted as 2^-20.
+    import torch
+
+    H = torch.cuda.get_device_properties(0).multi_processor_count  # a unit of work a CTA: rows are not split
+    s = make_case(1, [n], [32768], H, 1, 64, 64, dtype, seed=3)
+    s["V"] = s["V"].abs()
+    got = prefill(s, causal=False)
+    ids = s["table"][0, :512].long()
+    loss = []
+    for h in range(H):
+        k, v = ((s[x][ids, h].double() * s[y][ids, h].double().unsqueeze(-1)).reshape(-1, 64) for x, y in (("K", "ks"), ("V", "vs")))
+        want = torch.softmax(s["q"][:, h].double() @ k.T / 8, -1) @ v
+        loss.append((got[:, h].double() / want - 1).mean())
+    assert abs(float(torch.stack(loss).mean())) <= products * 2.0 ** -23 + 2.0 ** -20
+    assert kvd.device_status() == 0
 
 
 @pytest.mark.gpu
