@@ -506,8 +506,8 @@ cudaError_t check_pages(const kvd_pages_desc* d) {
         d->num_blocks < 1 || d->max_blocks_per_seq < 1 || d->block_table_stride < d->max_blocks_per_seq ||
         d->block_table_out_stride < d->max_blocks_per_seq)
         return cudaErrorInvalidValue;
-    // sums of blocks, a copy's bytes and a row's tokens are counted in 32 bits
-    if (d->num_blocks > 0x40000000 || static_cast<int64_t>(d->block_size) * d->head_dim > 0x3fffffffLL ||
+    // sums of blocks, a row's entries and tokens, and a copy's bytes are counted in 32 bits
+    if (d->num_blocks > 0x40000000 || d->max_blocks_per_seq > 0x40000000 || static_cast<int64_t>(d->block_size) * d->head_dim > 0x3fffffffLL ||
         static_cast<int64_t>(d->max_blocks_per_seq) * d->block_size > 0x7fffffffLL)
         return cudaErrorInvalidValue;
     return cudaSuccess;

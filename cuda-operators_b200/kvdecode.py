@@ -797,7 +797,8 @@ def paged_plan(seq_lens, new_lens, block_table, free_blocks, free_count, block_s
     ``seq_lens`` / ``new_lens`` int32 [B] (tokens held, tokens to add; new_lens < 0 ends a request),
     ``block_table`` int32 [B, max_blocks], ``free_blocks`` int32 [num_blocks] with ``free_count`` int32 [1]
     ids on it, ``slot_map`` int64 [num_slots]. The table, the free list and, unless other tensors are given for
-    them, the lengths and the count are updated in place. ``workspace``: a zeroed uint8 tensor of 16 bytes that a
+    them, the lengths and the count are updated in place. An ended request gives all its blocks back; requests that
+    share blocks are ended by :func:`paged_fork`. ``workspace``: a zeroed uint8 tensor of 16 bytes that a
     caller keeps (without one, one is made). Returns (slot_map, token_starts [B + 1])."""
     torch, _, i32, i64, _ = _torch or _types()
     device, B = seq_lens.get_device(), seq_lens.shape[0]
@@ -1075,11 +1076,12 @@ def paged_fork(parents, seq_lens, block_table, free_blocks, free_count, k_pool, 
                bound_scale=None, layout: str = "bhtd", seq_lens_out=None, block_table_out=None, free_count_out=None,
                workspace=None, stream=None):
     """Rows of the block table become copies of other rows (``kvd_paged_fork_launch``): row b continues row
-    ``parents``[b] (int32 [B]; b itself: it goes on as it is; -1: it ends). Full blocks are shared, partly filled last ones are copied
-    into blocks from the free list, and blocks that no row names any more go back on it. Lengths, table and count
-    are updated in place unless other tensors are given for them. Requests that may share blocks are ended here, not
-    by :func:`paged_plan`. ``workspace``: a zeroed uint8 tensor of :func:`paged_fork_workspace_size` bytes that a
-    caller keeps (without one, one is made). Returns (block_table_out, seq_lens_out)."""
+    ``parents``[b] (int32 [B]; b itself: it goes on as it is; -1: it ends). Full blocks are shared, partly filled
+    last ones are copied into blocks from the free list, and blocks that no row names any more go back on it.
+    Lengths, table and count are updated in place unless other tensors are given for them (as for all layers but
+    the last where several share a table). Requests that may share blocks are ended here, not by
+    :func:`paged_plan`. ``workspace``: a zeroed uint8 tensor of :func:`paged_fork_workspace_size` bytes that a
+    caller keeps for pools of as many blocks (without one, one is made). Returns (block_table_out, seq_lens_out)."""
     torch, i8, i32, _, f32 = _torch or _types()
     device = seq_lens.get_device()
     if block_table_out is None:

@@ -31,7 +31,8 @@
  * caller's kernel that follows it with the attribute must wait in the same way.
  * So do the kernels of the paged serving steps (kvd_paged_plan_launch,
  * kvd_paged_write_launch, kvd_paged_read_launch, kvd_block_select_launch,
- * kvd_sparse_decode_launch; the generic decode kernel aside): they are launched
+ * kvd_sparse_decode_launch, kvd_paged_prefill_launch, kvd_paged_fork_launch,
+ * kvd_paged_compact_launch; the generic decode kernel aside): they are launched
  * with the attribute, wait before any global memory access, and let the next
  * kernel launch from then on. A caller's kernel that follows one of these calls
  * with the attribute must wait before it reads what the call writes (tables,
@@ -364,14 +365,19 @@ cudaError_t kvd_sparse_decode_launch(const kvd_paged_desc* desc,
  * front of row_starts[0], from row_starts[batch] on) are left as they are;
  * starts are clamped to [0, num_rows], lengths to the table. A block id
  * outside the pool counts as in kvd_paged_decode_launch
- * (KVD_STATUS_BAD_BLOCK). head_dim at most 512. Sums and softmax statistics
- * are fp32; 16-bit queries enter the products unrounded, 32-bit ones as two
- * 16-bit terms (22 bits); weights as one 16-bit term (11 bits) where the output
- * has 16 bits, else as two. head_dim 64 and 128 with pools on 16-byte
- * boundaries and 16-byte multiples of strides run on tensor cores, any other
- * shape on CUDA cores. The workspace of kvd_paged_prefill_workspace_size bytes,
- * on a 16-byte boundary, needs no initialisation; concurrent calls need
- * separate ones. num_rows 0 does nothing. */
+ * (KVD_STATUS_BAD_BLOCK). Starts that do not ascend give rows of any of the
+ * requests that claim them, or leave them as they are. head_dim at most 512.
+ * Sums and softmax statistics are fp32; 16-bit queries enter the products
+ * unrounded, 32-bit ones as two terms of 11 bits each; weights times value
+ * scales (weights and, for bf16 outputs, value scales times codes) as one
+ * 16-bit term of 11 bits where the output has 16 bits, else as two. Tensor cores
+ * cut a sum off at every product that they add, so 32-bit outputs are summed in
+ * parts of at most 64 products of 16 tokens. head_dim 64 and 128 with pools on
+ * 16-byte boundaries and 16-byte multiples of strides run on tensor cores, any
+ * other shape on CUDA cores (where the cache is read again for every row and
+ * head). The workspace of kvd_paged_prefill_workspace_size bytes, on a 16-byte
+ * boundary, needs no initialisation; concurrent calls need separate ones.
+ * num_rows 0 does nothing. */
 typedef struct kvd_paged_prefill_desc {
     int32_t batch, num_q_heads, num_kv_heads, head_dim;
     int32_t num_rows;            /* rows of Q and out, >= 0 */
@@ -409,11 +415,16 @@ cudaError_t kvd_paged_prefill_launch(const kvd_paged_prefill_desc* desc, const v
  * block_table and free_count. Table ids outside the pool are passed on and
  * never followed (KVD_STATUS_BAD_BLOCK). The table has to name every holder of a
  * block. kvd_paged_plan_launch gives back all blocks of a request that it ends,
- * so requests that may share blocks are ended here instead. The workspace of
+ * so requests that may share blocks are ended here instead. Where the pools of
+ * several layers share one table, each layer has a call, all but the last with
+ * outputs of their own (kvd_paged_compact_launch: and with a copy of
+ * free_count); they all copy the same blocks. The workspace of
  * kvd_paged_fork_workspace_size bytes, on a 4-byte boundary, is zeroed by the
- * caller once; calls leave its counters zeroed. Concurrent calls need separate ones. At
- * most 8192 rows, 2^30 blocks and tokens of a row below 2^31, 2^30 codes in a block's head
- * (cudaErrorInvalidValue above). */
+ * caller once; calls leave its counters and bitmaps zeroed. It serves calls with
+ * the same num_blocks, kvd_paged_compact_launch's too where it is large enough;
+ * concurrent calls need separate ones. At most 8192 rows, 2^30 blocks in the
+ * pool and in a row, below 2^31 tokens of a row and below 2^30 codes in a
+ * block's head (cudaErrorInvalidValue above). */
 typedef struct kvd_pages_desc {
     int32_t batch, num_kv_heads, head_dim;
     int32_t block_size, num_blocks, max_blocks_per_seq;
@@ -436,10 +447,10 @@ cudaError_t kvd_paged_fork_launch(const kvd_pages_desc* desc, const int32_t* par
  * them. Blocks that neither the table nor the free list names belong to others
  * and stay. block_table_out gets the new ids (rows share a block as before),
  * free_blocks_out the free ones in descending order (the lowest id is the next
- * one handed out), free_count their number and used[0] the number of blocks that the pools
- * then need: the highest id in use, plus one. block_table_out and
- * free_blocks_out may be block_table and free_blocks. Pools, bounds, limits and workspace
- * (kvd_paged_compact_workspace_size bytes) as for kvd_paged_fork_launch. */
+ * one handed out), free_count their number and used[0] the number of blocks
+ * that the pools then need: the highest id in use, plus one. block_table_out and
+ * free_blocks_out may be block_table and free_blocks. Pools, bounds, limits and
+ * workspace (kvd_paged_compact_workspace_size bytes) as for kvd_paged_fork_launch. */
 cudaError_t kvd_paged_compact_launch(const kvd_pages_desc* desc, const int32_t* seq_lens, const int32_t* block_table,
                                      const int32_t* free_blocks, int32_t* free_count, int8_t* K_pool, int8_t* V_pool,
                                      float* k_scale_pool, float* v_scale_pool, int8_t* bounds, float* bound_scale,

@@ -461,6 +461,55 @@ def test_blocks_past_32_bits():
     assert kvd.device_status() == 0
 
 
+@pytest.mark.gpu
+def test_fork_and_compact_share_a_workspace():
+    import torch
+
+    rng, B, MB, bs, NB = np.random.default_rng(5), 9, 40, 8, 500
+    ws = torch.zeros(max(f(torch.empty((B, MB)), torch.empty(NB)) for f in (
+        kvd.paged_fork_workspace_size, kvd.paged_compact_workspace_size)), dtype=torch.uint8, device=DEV)
+    pools = make_pools(NB, 2, bs, 64, "bhtd", 6)
+    lens = rng.integers(0, MB * bs + 1, size=B)
+    table, left = random_rows(rng, B, MB, bs, NB, lens, share=0.4)
+    free, count = np.full(NB, -1, np.int32), len(left)
+    free[:count] = left
+    for step in range(3):  # every step takes over what the one before left
+        table, lens, free, count, *_ = check_fork(rng.integers(-1, B, size=B), lens, table, free, count, bs, pools, "bhtd",
+                                                  True, ws)
+        table, free, count, *_ = check_compact(lens, table, free, count, bs, pools, "bhtd", True, ws)
+
+
+@pytest.mark.gpu
+def test_pools_of_two_layers_share_a_table():
+    import torch
+
+    rng, B, MB, bs, NB = np.random.default_rng(8), 6, 12, 16, 90
+    layers = [make_pools(NB, 2, bs, 32, "bhtd", s) for s in (1, 2)]
+    lens = rng.integers(1, MB * bs + 1, size=B)
+    table, left = random_rows(rng, B, MB, bs, NB, lens)
+    free, count = np.full(NB, -1, np.int32), len(left)
+    free[:count] = left
+    parents = rng.integers(0, B, size=B)
+    fork = fork_oracle(parents, lens, table, free, count, bs)
+    move = compact_oracle(fork[1], *fork[:1], fork[2], fork[3], bs)
+    before = [snapshot(p) for p in layers]
+    t = [dev(lens), dev(table), dev(free), dev([count])]
+    other = [torch.empty_like(x) for x in t]
+    for i, pools in enumerate(layers):  # the last one updates what they share
+        own = {} if i else dict(seq_lens_out=other[0], block_table_out=other[1], free_count_out=other[3])
+        kvd.paged_fork(dev(parents), *t, *pools[:4], bounds=pools[4], bound_scale=pools[5], **own)
+    for x, w in zip((t[1], t[0], t[2], t[3]), fork):
+        np.testing.assert_array_equal(x.cpu().numpy().reshape(-1), np.asarray(w, np.int32).reshape(-1))
+    for i, pools in enumerate(layers):
+        own = {} if i else dict(block_table_out=other[1], free_blocks_out=other[2])
+        kvd.paged_compact(t[0], t[1], t[2], t[3] if i else t[3].clone(), *pools[:4], bounds=pools[4], bound_scale=pools[5], **own)
+    for x, w in zip((t[1], t[2], t[3]), move):
+        np.testing.assert_array_equal(x.cpu().numpy().reshape(-1), np.asarray(w, np.int32).reshape(-1))
+    for pools, was in zip(layers, before):
+        same(pools, apply_copies(apply_copies(was, fork[4], "bhtd", bs), [(s, d, bs) for s, d in move[4]], "bhtd", bs))
+    assert kvd.device_status() == 0
+
+
 # ------------------------------------------------------------------------ CPU
 def pages_desc(**kw):
     d = kvd.PagesDesc(4, 2, 64, 16, 100, 8, 8, 8, 2 * 16 * 64, 16 * 64, 64, 32, 16)
@@ -472,6 +521,8 @@ def pages_desc(**kw):
 @pytest.mark.parametrize("kw", [dict(batch=0), dict(batch=8193), dict(num_kv_heads=0), dict(head_dim=0), dict(block_size=0),
                                 dict(num_blocks=0), dict(num_blocks=(1 << 30) + 1), dict(max_blocks_per_seq=0),
                                 dict(block_table_stride=7), dict(block_table_out_stride=7),
+                                dict(block_size=1, max_blocks_per_seq=(1 << 30) + 1, block_table_stride=1 << 31,
+                                     block_table_out_stride=1 << 31),
                                 dict(max_blocks_per_seq=1 << 28, block_table_stride=1 << 28, block_table_out_stride=1 << 28),
                                 dict(block_size=1 << 24, head_dim=64, max_blocks_per_seq=2)])
 def test_bad_descriptors_are_refused(kw):
