@@ -87,11 +87,24 @@ __device__ __forceinline__ int blocks_of(const PagesParams& p, int len) {
 
 __device__ __forceinline__ bool in_pool(const PagesParams& p, int id) { return id >= 0 && id < p.NB; }
 
-// Many rows may name a block: the bit is read first, so that most of them write nothing.
-__device__ __forceinline__ void mark(uint32_t* bits, int id) {
-    uint32_t* w = bits + (id >> 5);
-    const uint32_t bit = 1u << (id & 31);
-    if (!(*reinterpret_cast<volatile uint32_t*>(w) & bit)) atomicOr(w, bit);
+// Marks the blocks id[i] with 32 i < n; returns whether one lies outside the pool. Many rows may name a block: the bits
+// are read first, all of them at once, so that most rows write nothing. (A bit that looks unset may be set by now.)
+template <int N>
+__device__ __forceinline__ bool mark(const PagesParams& p, uint32_t* bits, const int (&id)[N], int n) {
+    uint32_t word[N];
+    bool bad = false;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        const bool there = 32 * i < n, good = there && in_pool(p, id[i]);
+        word[i] = good ? __ldcg(bits + (id[i] >> 5)) : 0xffffffffu;
+        bad |= there && !good;
+    }
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        const uint32_t bit = 1u << (id[i] & 31);
+        if (!(word[i] & bit)) atomicOr(bits + (id[i] >> 5), bit);
+    }
+    return bad;
 }
 
 // Exclusive prefix sums of N values a thread over the CTA; total: the sums of all.
@@ -174,14 +187,23 @@ __global__ void __launch_bounds__(kMarkThreads) fork_mark_kernel(const PagesPara
     int32_t* len = heir + p.B;
     grid_dependency_wait();
     allow_dependents();
-    for (int b = threadIdx.x; b < p.B; b += blockDim.x) {
-        heir[b] = kNoHeir;
-        len[b] = row_len(p, b);
-    }
+    for (int b = threadIdx.x; b < p.B; b += blockDim.x) heir[b] = kNoHeir;
     __syncthreads();
-    for (int b = threadIdx.x; b < p.B; b += blockDim.x) {
-        const int from = p.parents[b];
-        if (from >= 0 && from < p.B) atomicMin(&heir[from], from == b ? -1 : b);
+    constexpr int R = 4;  // rows a thread has under way
+    for (int b0 = threadIdx.x; b0 < p.B; b0 += R * blockDim.x) {
+        int from[R], tokens[R];
+#pragma unroll
+        for (int i = 0; i < R; ++i) {
+            const int b = b0 + i * blockDim.x;
+            from[i] = b < p.B ? p.parents[b] : -1;
+            tokens[i] = b < p.B ? row_len(p, b) : 0;
+        }
+#pragma unroll
+        for (int i = 0; i < R; ++i) {
+            const int b = b0 + i * blockDim.x;
+            if (b < p.B) len[b] = tokens[i];
+            if (from[i] >= 0 && from[i] < p.B) atomicMin(&heir[from[i]], from[i] == b ? -1 : b);
+        }
     }
     __syncthreads();
     const int lane = threadIdx.x & 31, warps = gridDim.x * (blockDim.x >> 5);
@@ -196,12 +218,8 @@ __global__ void __launch_bounds__(kMarkThreads) fork_mark_kernel(const PagesPara
         if (e0 < n) {
             int id[kEntries / 32];
 #pragma unroll
-            for (int i = 0; i < kEntries / 32; ++i) id[i] = e0 + 32 * i + lane < n ? row[e0 + 32 * i + lane] : kNoBlock;
-#pragma unroll
-            for (int i = 0; i < kEntries / 32; ++i) {
-                if (in_pool(p, id[i])) mark(bits, id[i]);
-                else if (id[i] != kNoBlock) status |= KVD_STATUS_BAD_BLOCK;
-            }
+            for (int i = 0; i < kEntries / 32; ++i) id[i] = 32 * i < n - e0 - lane ? row[e0 + 32 * i + lane] : -1;
+            if (mark(p, bits, id, n - e0 - lane)) status |= KVD_STATUS_BAD_BLOCK;
         }
         const int from = p.staged ? p.parents[b] : b;
         if (from != b && from >= 0 && from < p.B) {
@@ -395,18 +413,13 @@ __global__ void __launch_bounds__(kMarkThreads) compact_mark_kernel(const PagesP
         const int32_t* row = p.table + b * p.stride;
         int id[kEntries / 32];
 #pragma unroll
-        for (int i = 0; i < kEntries / 32; ++i) id[i] = e0 + 32 * i + lane < n ? row[e0 + 32 * i + lane] : kNoBlock;
-#pragma unroll
-        for (int i = 0; i < kEntries / 32; ++i) {
-            if (in_pool(p, id[i])) mark(p.bits_a, id[i]);
-            else if (id[i] != kNoBlock) status |= KVD_STATUS_BAD_BLOCK;
-        }
+        for (int i = 0; i < kEntries / 32; ++i) id[i] = 32 * i < n - e0 - lane ? row[e0 + 32 * i + lane] : -1;
+        if (mark(p, p.bits_a, id, n - e0 - lane)) status |= KVD_STATUS_BAD_BLOCK;
     }
     const int fc = min(max(0, *p.count_in), p.NB);
     for (int64_t i = static_cast<int64_t>(me) * 32 + lane; i < fc; i += static_cast<int64_t>(warps) * 32) {
-        const int id = p.free_in[i];
-        if (in_pool(p, id)) mark(p.bits_b, id);
-        else status |= KVD_STATUS_BAD_BLOCK;
+        const int id[1] = {p.free_in[i]};
+        if (mark(p, p.bits_b, id, 1)) status |= KVD_STATUS_BAD_BLOCK;
     }
     if (status) record_status(status);
     if (!last_cta(p.ticket)) return;
