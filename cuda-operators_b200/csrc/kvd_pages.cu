@@ -13,10 +13,10 @@
 // table rows and copies blocks, a warp per (block, K or V, head).
 //
 // Bound: latency of the two launches and of the last CTA's sums, then HBM. Fork:
-// 32 rows 13 us, 256 rows that become copies of 32 with their partly filled
-// blocks 16 us (0.03 GB), 2,048 rows 33 us. Compact: 2,048 blocks of 16 tokens 21 us;
+// 32 rows 11 us, 256 rows that become copies of 32 with their partly filled
+// blocks 15 us (0.03 GB), 2,048 rows 29 us. Compact: 2,048 blocks of 16 tokens 21 us;
 // 4,096 of 8,192 blocks of 64 tokens x 8 heads x 128 dims in use, half of them
-// moved, 104 us: 5.3 TB/s. Marks by 1,024 threads a CTA were slower.
+// moved, 103 us: 5.4 TB/s. Marks by 1,024 threads a CTA were slower.
 #include "kvd_common.cuh"
 #include "kvd_decode.cuh"
 
