@@ -668,6 +668,7 @@ __device__ __forceinline__ void put_aside(float4* aside, float4* of, uint32_t co
         }
         tmem_st32(col_o + d, o);
     }
+    tmem_wait_st();  // O may be read again in the same tile, and only this wait puts a load behind the stores
 }
 
 template <int D, int TERMS, bool FOLD>
