@@ -469,7 +469,6 @@ extern "C" cudaError_t kvd_paged_prefill_launch(const kvd_paged_prefill_desc* d,
         if (!has_class(*d, c)) continue;
         e = c == kMany ? launch_chunk_tile(p, stream, launches) : launch_chunk_few(p, c, stream, launches);
         if (e != cudaSuccess) return e;
-        p.follows = 1;
     }
     if (!split) return cudaSuccess;
     const unsigned grid = 8u * device_sm_count();

@@ -52,7 +52,6 @@ struct ChunkParams {
     int max_recs[kClasses];     // room for records
     float4* aside;              // [CTA][2][D / 4][128] sums that the kernel for many rows puts aside
     int aside_tiles;            // after how many tiles
-    int follows;                // the kernel before this one reads the same plan
     int tiny_most, few_most;    // rows up to which a request is of the first class, of the second
 };
 
@@ -67,23 +66,6 @@ constexpr int kTile = 128;       // tokens of a tile of the kernel for many rows
 // rounding, and starts again from zero after this many of its tiles, 64 products of a 32-bit output (1.5e-6 then),
 // 512 of a 16-bit one. Powers of two.
 constexpr int kAsideTiles = 4, kAsideTiles16 = 64;
-
-// The kernels of the classes write nothing that the others read, so one need not wait until the one before it ends: it
-// takes the SMs that the other leaves. That it has been launched says that all CTAs of the other have got here, where
-// they (or those of the one before them) had waited for the plan. It ends after the other, so whoever waits for it
-// waits for both.
-__device__ __forceinline__ void class_begins(const ChunkParams& p) {
-    if (p.follows) {  // (a fence takes 2 us more where a kernel has nothing to do)
-        [[maybe_unused]] int units;
-        asm volatile("ld.acquire.gpu.global.s32 %0, [%1];" : "=r"(units) : "l"(&p.head->units[0]) : "memory");
-    } else {
-        grid_dependency_wait();
-    }
-    allow_dependents();
-}
-__device__ __forceinline__ void class_ends(const ChunkParams& p) {
-    if (p.follows) grid_dependency_wait();
-}
 
 // Rows [t0, t0 + n) of request b and its tokens.
 struct ChunkRows {

@@ -2,12 +2,16 @@
 
 Inputs, oracle and tolerances are those of test_paged_prefill.py; where a test needs another bound it derives it."""
 import ctypes
+import re
+from pathlib import Path
 
 import numpy as np
 import pytest
 
 import kvdecode as kvd
 from test_paged_prefill import DEV, TYPES, close, make_case, oracle, prefill, prefill_desc
+
+CSRC = Path(__file__).resolve().parents[1] / "cuda-operators_b200" / "csrc"
 
 
 def tokens(s, b=0):
@@ -44,4 +48,47 @@ def test_references_that_move_where_sums_are_put_aside(dtype, n, every, what, ti
     else:
         s["vs"][blk, :, off] *= (2.0 ** (10 * level.float())).unsqueeze(-1)
     close(prefill(s, causal=False), s, oracle(s, causal=False))
+    assert kvd.device_status() == 0
+
+
+def test_kernels_wait_for_the_one_before_them():
+    # Every kernel that is launched with the programmatic attribute waits for its predecessor, whatever its arguments
+    # say, before it lets the next one begin and before it looks at memory that others write.
+    found = 0
+    for name in ("kvd_chunk.cu", "kvd_chunk_few.cu", "kvd_chunk_tile.cu", "kvd_pages.cu"):
+        source = (CSRC / name).read_text()
+        for part in source.split("__global__")[1:]:
+            body = part[part.index("{\n"): part.index("\n}\n")]
+            wait, allow = body.find("\n    grid_dependency_wait();"), body.find("\n    allow_dependents();")
+            assert 0 <= wait < allow, (name, part[:100])
+            assert not re.search(r"\bp\.(head|first|rec|starts|seq_lens|table|lens|parents|Q|K|V|ks|vs|bits_a|free_in)\b", body[:wait])
+            found += 1
+    assert found >= 9
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES)
+def test_plans_of_calls_that_follow_each_other(dtype):
+    # Requests of every class in each call, two calls in turn with other lengths and rows, in one graph with one
+    # workspace: a kernel that read the plan of the call before would take other units.
+    import torch
+
+    n = [[1, 8, 30, 1, 120, 2, 50, 1] * 4, [50, 1, 1, 9, 2, 140, 1, 20] * 4]
+    cases = [make_case(32, x, np.asarray(x) + 300 * (1 + i), 8, 4, 128, 16, dtype, seed=40 + i) for i, x in enumerate(n)]
+    wants = [oracle(s) for s in cases]
+    outs = [torch.empty_like(s["q"]) for s in cases]
+    ws = torch.full((max(kvd.paged_prefill_workspace_size(s["q"], s["K"], s["table"]) for s in cases),), 255,
+                    dtype=torch.uint8, device=DEV)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        for _ in range(3):
+            for s, o in zip(cases, outs):
+                o.fill_(float("nan"))
+                prefill(s, out=o, workspace=ws)
+    for _ in range(4):
+        graph.replay()
+        for s, o, w in zip(cases, outs, wants):
+            close(o, s, w)
     assert kvd.device_status() == 0
