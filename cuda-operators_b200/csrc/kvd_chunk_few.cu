@@ -234,7 +234,7 @@ __global__ void __launch_bounds__(kFewWarps * 32, FewSmem<D, NR, NQ>::kCtas) chu
         }
         // the columns of this lane in the products: rows 2c and 2c + 1 of each group
         float rf[NR][2], m[NR][2], l[NR][2];
-        int sees[NR][2];
+        int sees[NR][2], ve[NR][2];  // value scales that the row has seen, times 2^ve, are below 2^7: weights up to 2^8 fit fp16
 #pragma unroll
         for (int e = 0; e < NR; ++e)
 #pragma unroll
@@ -245,6 +245,7 @@ __global__ void __launch_bounds__(kFewWarps * 32, FewSmem<D, NR, NQ>::kCtas) chu
                 sees[e][y] = min(end, chunk_sees(p, R, min(i, R.n - 1)));
                 m[e][y] = -INFINITY;
                 l[e][y] = 0.f;
+                ve[e][y] = 126;
             }
         // ---- the walk
         float o[NR][D / 16][4];
@@ -252,7 +253,6 @@ __global__ void __launch_bounds__(kFewWarps * 32, FewSmem<D, NR, NQ>::kCtas) chu
         for (int e = 0; e < NR; ++e)
 #pragma unroll
             for (int j = 0; j < D / 16; ++j) o[e][j][0] = o[e][j][1] = o[e][j][2] = o[e][j][3] = 0.f;
-        int ve = 126;  // value scales times 2^ve are below 2^7, so that weights up to 2^8 fit fp16
 #pragma unroll 1
         for (int k = 0; k < mine; ++k) {
             async_wait<STAGES - 2>();
@@ -310,20 +310,38 @@ __global__ void __launch_bounds__(kFewWarps * 32, FewSmem<D, NR, NQ>::kCtas) chu
                             top[e][y] = fmaxf(top[e][y], v);
                         }
                 }
-            // largest value scale of the step (what is not finite has no say)
+            // largest value scale of the step (what is not finite has no say), and the exponents that it asks for: a row's
+            // are its own where rows see different tokens, so that no hidden one costs it bits
             float v_top = fabsf(scales[kStep + lane]);
             if (!(v_top < INFINITY)) v_top = 0.f;
-            const int v_bits = __reduce_max_sync(0xffffffffu, __float_as_int(v_top));
-            const int v_fit = v_bits == 0 ? 126 : fit_exponent(__int_as_float(v_bits), 7);
-            const bool grow = v_fit < ve;
-            bool move = grow;
+            int fit[NR][2];
+            if (!masked) {
+                const int bits = __reduce_max_sync(0xffffffffu, __float_as_int(v_top));
+                fit[0][0] = bits == 0 ? 126 : fit_exponent(__int_as_float(bits), 7);
+#pragma unroll
+                for (int e = 0; e < NR; ++e) fit[e][0] = fit[e][1] = fit[0][0];
+            } else {
+#pragma unroll
+                for (int x = 1; x < 32; x <<= 1) {  // lane i: the largest of tokens 0 .. i
+                    const float y = __shfl_up_sync(0xffffffffu, v_top, x);
+                    if (lane >= x) v_top = fmaxf(v_top, y);
+                }
+#pragma unroll
+                for (int e = 0; e < NR; ++e)
+#pragma unroll
+                    for (int y = 0; y < 2; ++y) {
+                        const int lim = sees[e][y] - t0;
+                        const float seen = __shfl_sync(0xffffffffu, v_top, min(max(lim, 1), 32) - 1);
+                        fit[e][y] = lim <= 0 || seen == 0.f ? 126 : fit_exponent(seen, 7);
+                    }
+            }
+            bool move = false;
 #pragma unroll
             for (int e = 0; e < NR; ++e)
 #pragma unroll
-                for (int y = 0; y < 2; ++y) move |= top[e][y] > m[e][y] + (m[e][y] == -INFINITY ? 0.f : 8.f);
+                for (int y = 0; y < 2; ++y)
+                    move |= fit[e][y] < ve[e][y] || top[e][y] > m[e][y] + (m[e][y] == -INFINITY ? 0.f : 8.f);
             if (__any_sync(0xffffffffu, move)) {
-                const float fv = grow ? (ve - v_fit > 126 ? 0.f : pow2i(v_fit - ve)) : 1.f;
-                if (grow) ve = v_fit;
 #pragma unroll
                 for (int e = 0; e < NR; ++e)
 #pragma unroll
@@ -334,23 +352,25 @@ __global__ void __launch_bounds__(kFewWarps * 32, FewSmem<D, NR, NQ>::kCtas) chu
                         to = fmaxf(to, __shfl_xor_sync(0xffffffffu, to, 16));
                         const bool go = to > m[e][y] + (m[e][y] == -INFINITY ? 0.f : 8.f);
                         const float f = go ? (m[e][y] == -INFINITY ? 0.f : ex2_fast(m[e][y] - to)) : 1.f;
+                        const int fall = max(ve[e][y] - fit[e][y], 0);
+                        const float fo = fall > 126 ? 0.f : f * pow2i(-fall);
                         if (go) m[e][y] = to;
+                        ve[e][y] -= fall;
                         l[e][y] *= f;
 #pragma unroll
                         for (int j = 0; j < D / 16; ++j) {
-                            o[e][j][y] *= f * fv;
-                            o[e][j][2 + y] *= f * fv;
+                            o[e][j][y] *= fo;
+                            o[e][j][2 + y] *= fo;
                         }
                     }
             }
-            const float vf = pow2i(ve);
 #pragma unroll
             for (int mt = 0; mt < 2; ++mt) {
                 // weights of 16 tokens
                 uint32_t pb[NP][NR][2];
 #pragma unroll
                 for (int half = 0; half < 2; ++half) {
-                    const float vq = scales[kStep + 16 * mt + quad + 8 * half] * vf;
+                    const float vq = scales[kStep + 16 * mt + quad + 8 * half];
 #pragma unroll
                     for (int e = 0; e < NR; ++e) {
                         float w[2];
@@ -359,7 +379,7 @@ __global__ void __launch_bounds__(kFewWarps * 32, FewSmem<D, NR, NQ>::kCtas) chu
                             const float x = s[mt][e][2 * half + y];
                             const float pr = ex2_fast(x - (m[e][y] == -INFINITY ? 0.f : m[e][y]));
                             l[e][y] += pr;
-                            w[y] = pr * vq;
+                            w[y] = pr * (vq * pow2i(ve[e][y]));
                             if (masked && x == -INFINITY) w[y] = 0.f;  // a hidden token's scale may be anything
                         }
                         const uint32_t hi = pack_half(w[0], w[1]);
@@ -408,7 +428,6 @@ __global__ void __launch_bounds__(kFewWarps * 32, FewSmem<D, NR, NQ>::kCtas) chu
         // ---- merge of the warps
         __syncthreads();  // every warp is done with its ring
         float* merge = reinterpret_cast<float*>(few_smem);  // [warp][row][D + 4]: dims, then m and l
-        const float back = pow2i(-ve);
 #pragma unroll
         for (int e = 0; e < NR; ++e)
 #pragma unroll
@@ -417,6 +436,7 @@ __global__ void __launch_bounds__(kFewWarps * 32, FewSmem<D, NR, NQ>::kCtas) chu
                 sum += __shfl_xor_sync(0xffffffffu, sum, 4);
                 sum += __shfl_xor_sync(0xffffffffu, sum, 8);
                 sum += __shfl_xor_sync(0xffffffffu, sum, 16);
+                const float back = pow2i(-ve[e][y]);
                 float* row = merge + (warp * ROWS + 8 * e + 2 * c + y) * (D + 4);
 #pragma unroll
                 for (int j = 0; j < D / 16; ++j)

@@ -92,3 +92,50 @@ def test_plans_of_calls_that_follow_each_other(dtype):
         for s, o, w in zip(cases, outs, wants):
             close(o, s, w)
     assert kvd.device_status() == 0
+
+
+FEW = [(128, 4, 2), (128, 4, 10), (64, 1, 7), (64, 2, 21)]  # dims, heads a KV head, rows: 8 to 42 rows a KV head
+
+
+def hidden_scales(D, G, n, dtype, value):
+    """Whose last tokens' value scales are far above what the rows in front of them see. "steps": each new token's is
+    four times the one before it, so every row has a largest of its own."""
+    s = make_case(1, [n], [203], 2, G, D, 16, dtype, seed=51)
+    blk, off = tokens(s)
+    if value == "steps":
+        s["vs"] *= 1e-6
+        for i in range(n):
+            s["vs"][blk[203 - n + i], :, off[203 - n + i]] *= 4.0 ** min(i + 1, 8 if dtype == "float16" else 40)
+    else:
+        s["vs"][blk[-1], :, off[-1]] = value
+    return s
+
+
+def check_hidden_scales(D, G, n, dtype, value):
+    # Causal rows: what a row gets does not depend on value scales of tokens behind it. A small weight is off by 2^-25 of
+    # a reference that is at least 2^6 of the largest value scale that the row sees, times a code of at most 127: 2^-31
+    # of 127 times that scale a token, in every dim, also where the code of the token with that scale is 0. So the
+    # largest |v| of the tolerance is 127 times the largest scale in sight.
+    import torch
+
+    s = hidden_scales(D, G, n, dtype, value)
+    out, mean, _, size = oracle(s)
+    blk, off = tokens(s)
+    sees = 127.0 * s["vs"][blk, :, off].double().cummax(0).values[-n:].repeat_interleave(G, 1)
+    want = out, mean, sees.unsqueeze(-1).expand_as(out), size
+    got = prefill(s)
+    s["n"], s["starts_host"] = np.array([n - 1]), np.array([0, n - 1])  # every row but the last: the large ones are hidden
+    close(got, s, want)
+    if dtype != "float16" or value == "steps":  # the last row's fit the output
+        close(got, {**s, "n": np.array([n]), "starts_host": np.array([0, n])}, want)
+    s["n"], s["starts_host"] = np.array([n]), np.array([0, n])
+    close(prefill(s, out_dtype=torch.float32), s, want)
+    assert kvd.device_status() == 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("D,G,n", FEW)
+@pytest.mark.parametrize("value", ["steps", 1e10, 1e20, 1e36])
+def test_value_scales_of_hidden_tokens_with_few_rows(D, G, n, dtype, value):
+    check_hidden_scales(D, G, n, dtype, value)
