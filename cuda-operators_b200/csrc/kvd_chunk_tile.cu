@@ -61,11 +61,12 @@ constexpr int kUnitStages = 4;
 // What is known of a tile before it is read.
 struct TileMeta {
     float ks[kTile];
-    float vs[kTile];     // times 2^ve, 0 where it is not finite
+    float vs[kTile];     // times 2^ve, or as they are where `vary`; 0 where it is not finite
     int64_t row[kTile];  // offset of the token's row in the pools; where there is none 0, and its scales are 0
     uint32_t odd[kTile / 32];  // tokens whose value scale is not finite
     int ve;
-    int pad[11];
+    int vary;  // tokens that some rows do not see have the largest scales: each row has an exponent of its own
+    int pad[10];
 };
 
 template <int D>
@@ -149,6 +150,7 @@ struct TileUnit {
     ChunkRows R;
     int rows;            // of the request and KV head
     int begin, end, nt;  // tokens, tiles
+    int least;           // tokens in front of this one are seen by every row
     bool alt;            // the warpgroups take tiles in turn
 };
 
@@ -172,6 +174,7 @@ __device__ __forceinline__ TileUnit tile_unit(const ChunkParams& p, int unit) {
     const int most = chunk_sees(p, u.R, static_cast<int>(p.by_g.div(static_cast<uint32_t>(last))));
     u.begin = u.split * each;
     u.end = min(min(u.begin + each, u.R.len), most);
+    u.least = min(u.end, chunk_sees(p, u.R, static_cast<int>(p.by_g.div(static_cast<uint32_t>(u.rb * ROWS)))));
     u.nt = u.end > u.begin ? (u.end - u.begin + kTile - 1) / kTile : 0;
     u.alt = TERMS == 2 || u.rows - u.rb * ROWS <= 128;
     return u;
@@ -208,7 +211,10 @@ __device__ __forceinline__ void tile_scout(const ChunkParams& p, const TileUnit&
             }
         }
     };
-    int ve = 126;
+    // Exponents for the scales of tokens that every row sees, and of all. Where the second is smaller, rows choose for
+    // themselves, so that no hidden token costs a row bits. From then on it stays smaller: every later token is hidden
+    // from some row.
+    int ve = 126, ve_all = 126;
     look_up(0);
     for (int i = 0; i < u.nt && ok; ++i, ++j) {
         TileMeta* m = meta + (j & (kMetaStages - 1));
@@ -226,18 +232,22 @@ __device__ __forceinline__ void tile_scout(const ChunkParams& p, const TileUnit&
         }
         if (bad) record_status(KVD_STATUS_BAD_BLOCK);
         if (i + 1 < u.nt) look_up(i + 1);  // on its way while this tile's scales come
-        float top = 0.f;
+        float top = 0.f, top_all = 0.f;
         uint32_t odd[N];
 #pragma unroll
         for (int x = 0; x < N; ++x) {
             const bool fine = fabsf(vs[x]) < INFINITY;
             odd[x] = __ballot_sync(0xffffffffu, !fine);
             if (!fine) vs[x] = 0.f;
-            top = fmaxf(top, fabsf(vs[x]));
+            if (u.begin + i * kTile + 32 * x + lane < u.least) top = fmaxf(top, fabsf(vs[x]));
+            top_all = fmaxf(top_all, fabsf(vs[x]));
         }
         const int bits = __reduce_max_sync(0xffffffffu, __float_as_int(top));
+        const int bits_all = __reduce_max_sync(0xffffffffu, __float_as_int(top_all));
         if (bits != 0) ve = min(ve, fit_exponent(__int_as_float(bits), 7));
-        const float f = pow2i(ve);
+        if (bits_all != 0) ve_all = min(ve_all, fit_exponent(__int_as_float(bits_all), 7));
+        const bool vary = ve_all < ve;
+        const float f = vary ? 1.f : pow2i(ve);
         ok = j < kMetaStages || mbar_wait_all(&bars[kMetaEmpty + (j & (kMetaStages - 1))], ((j / kMetaStages) - 1) & 1);
         if (!ok) break;
 #pragma unroll
@@ -247,7 +257,10 @@ __device__ __forceinline__ void tile_scout(const ChunkParams& p, const TileUnit&
             m->row[32 * x + lane] = row[x];
             if (lane == 0) m->odd[x] = odd[x];
         }
-        if (lane == 0) m->ve = ve;
+        if (lane == 0) {
+            m->ve = ve;
+            m->vary = vary;
+        }
         __syncwarp();
         if (lane == 0) mbar_arrive(&bars[kMetaFull + (j & (kMetaStages - 1))]);
     }
@@ -427,7 +440,9 @@ __device__ __forceinline__ bool tile_convert(const ChunkParams& p, const TileUni
         const int j = j0 + tile, st = j & 1;
         if (j >= 2 && !mbar_wait(&bars[(v ? kVEmpty : kKEmpty) + st], ((j >> 1) - 1) & 1)) return false;
         uint8_t* to = smem + (v ? S::kV : S::kK) + st * S::kRows;
-        if (FOLD && v) c.template store<true>(to, ct, meta[j & (kMetaStages - 1)].vs);
+        // (where exponents vary the value scales are the weights')
+        if (FOLD && v && !(u.begin + (tile + 1) * kTile > u.least && meta[j & (kMetaStages - 1)].vary))
+            c.template store<true>(to, ct, meta[j & (kMetaStages - 1)].vs);
         else c.template store<false>(to, ct, nullptr);
         fence_async_smem();
         __syncwarp();
@@ -564,10 +579,10 @@ __device__ __forceinline__ float top32(uint32_t col, const float4* ks4, int lim)
 }
 
 // Weights of 32 tokens with reference m: their sum onto `sum`, p vs 2^ve as fp16 pairs (and their rests). Returns
-// the largest u ks.
+// the largest u ks. MASK: the first `lim` tokens only; vf is 2^ve where the exponent is the row's own (`vary`), else 1.
 template <bool MASK, bool FOLD>
-__device__ __forceinline__ float weights32(uint32_t col, const float4* ks4, const float4* vs4, int lim, float rf, float m,
-                                           float2 (&sum)[2], uint32_t (&hi)[16], uint32_t* lo) {
+__device__ __forceinline__ float weights32(uint32_t col, const float4* ks4, const float4* vs4, int lim, float vf, bool vary, float rf,
+                                           float m, float2 (&sum)[2], uint32_t (&hi)[16], uint32_t* lo) {
     uint32_t s[32];
     tmem_ld32(col, s);
     tmem_wait_ld();
@@ -575,7 +590,12 @@ __device__ __forceinline__ float weights32(uint32_t col, const float4* ks4, cons
     float tm[2] = {-INFINITY, -INFINITY};
 #pragma unroll
     for (int k = 0; k < 8; ++k) {
-        const float4 kq = ks4[k], vq = FOLD ? make_float4(1.f, 1.f, 1.f, 1.f) : vs4[k];
+        const float4 kq = ks4[k];
+        float4 vq = make_float4(1.f, 1.f, 1.f, 1.f);
+        if (!FOLD || (MASK && vary)) vq = vs4[k];
+        if (MASK)  // a hidden token's scale may be too large for 2^ve
+            vq = make_float4(4 * k < lim ? vq.x * vf : 0.f, 4 * k + 1 < lim ? vq.y * vf : 0.f, 4 * k + 2 < lim ? vq.z * vf : 0.f,
+                             4 * k + 3 < lim ? vq.w * vf : 0.f);
         float2 a = __fmul2_rn(make_float2(__uint_as_float(s[4 * k]), __uint_as_float(s[4 * k + 1])), make_float2(kq.x, kq.y));
         float2 b = __fmul2_rn(make_float2(__uint_as_float(s[4 * k + 2]), __uint_as_float(s[4 * k + 3])), make_float2(kq.z, kq.w));
         if (MASK) {
@@ -588,7 +608,8 @@ __device__ __forceinline__ float weights32(uint32_t col, const float4* ks4, cons
         const float2 pa = make_float2(ex2_fast(a.x), ex2_fast(a.y)), pb = make_float2(ex2_fast(b.x), ex2_fast(b.y));
         sum[0] = __fadd2_rn(sum[0], pa);
         sum[1] = __fadd2_rn(sum[1], pb);
-        const float2 x = FOLD ? pa : __fmul2_rn(pa, make_float2(vq.x, vq.y)), y = FOLD ? pb : __fmul2_rn(pb, make_float2(vq.z, vq.w));
+        const bool plain = FOLD && !MASK;
+        const float2 x = plain ? pa : __fmul2_rn(pa, make_float2(vq.x, vq.y)), y = plain ? pb : __fmul2_rn(pb, make_float2(vq.z, vq.w));
         hi[2 * k] = pack_half(x.x, x.y);
         hi[2 * k + 1] = pack_half(y.x, y.y);
         if (lo) {
@@ -702,8 +723,6 @@ __device__ __forceinline__ bool tile_softmax(const ChunkParams& p, const TileUni
     if ((!u.alt || w < u.nt) && !mbar_wait(&bars[kQFull], nu & 1)) return false;
     const float rf = reinterpret_cast<const float*>(smem + S::kRf)[(nu & 1) * 256 + in_unit];
     const int sees = chunk_sees(p, u.R, min(i, u.R.n - 1));  // rows that are not there see what the last one does
-    const int first_row = u.rb * ROWS + (u.alt ? 0 : w * 128);
-    const int least = min(u.end, chunk_sees(p, u.R, min(u.R.n - 1, static_cast<int>(p.by_g.div(static_cast<uint32_t>(first_row))))));
     float m = -INFINITY;
     float2 lp[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
     int ve = 126;
@@ -713,24 +732,23 @@ __device__ __forceinline__ bool tile_softmax(const ChunkParams& p, const TileUni
         if (!mbar_wait(&bars[kMetaFull + st], (j / kMetaStages) & 1)) return false;
         const float4* ks4 = reinterpret_cast<const float4*>(meta[st].ks);
         const float4* vs4 = reinterpret_cast<const float4*>(meta[st].vs);
-        const int ve_now = meta[st].ve;
+        const int lim = min(sees, u.end) - t0;  // tokens of the tile that the row sees
+        const bool masked = t0 + kTile > u.least;
         if (!mbar_wait(&bars[kSFull + w], ns & 1)) return false;
         ++ns;
         tc_fence_after();
-        const int lim = min(sees, u.end) - t0;  // tokens of the tile that the row sees
-        const bool masked = t0 + kTile > least;
         const int own_tile = u.alt ? tile >> 1 : tile;
         const bool full = own_tile != 0 && (own_tile & (p.aside_tiles - 1)) == 0;  // O holds as many as it should
         bool done = false;
         if constexpr (TERMS == 1) {
             // With the reference of the tiles before: one pass. It stands unless a score is above it by more than 8.
-            if (!masked && !full && __all_sync(0xffffffffu, m != -INFINITY) && ve_now == ve) {
+            if (!masked && !full && __all_sync(0xffffffffu, m != -INFINITY) && meta[st].ve == ve) {
                 uint32_t pk[kTile / 2];
                 float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
                 float top = -INFINITY;
 #pragma unroll
                 for (int q = 0; q < 4; ++q)
-                    top = fmaxf(top, weights32<false, FOLD>(col_s + 32u * q, ks4 + 8 * q, vs4 + 8 * q, 0, rf, m, sum,
+                    top = fmaxf(top, weights32<false, FOLD>(col_s + 32u * q, ks4 + 8 * q, vs4 + 8 * q, 0, 1.f, false, rf, m, sum,
                                                       *reinterpret_cast<uint32_t(*)[16]>(&pk[16 * q]), nullptr));
                 done = !__any_sync(0xffffffffu, top * rf > m + 8.f);
                 if (done) {
@@ -742,6 +760,21 @@ __device__ __forceinline__ bool tile_softmax(const ChunkParams& p, const TileUni
             }
         }
         if (!done) {
+            int ve_now = meta[st].ve;
+            const bool vary = masked && meta[st].vary;
+            if (vary) {
+                float seen = 0.f;
+#pragma unroll 4
+                for (int x = 0; x < kTile / 4; ++x) {
+                    const float4 v = vs4[x];
+                    if (4 * x < lim) seen = fmaxf(seen, fabsf(v.x));
+                    if (4 * x + 1 < lim) seen = fmaxf(seen, fabsf(v.y));
+                    if (4 * x + 2 < lim) seen = fmaxf(seen, fabsf(v.z));
+                    if (4 * x + 3 < lim) seen = fmaxf(seen, fabsf(v.w));
+                }
+                ve_now = seen == 0.f ? ve : min(ve, fit_exponent(seen, 7));
+            }
+            const float vf = vary ? pow2i(ve_now) : 1.f;
             float top = -INFINITY;
             if (masked) {
 #pragma unroll 1
@@ -776,21 +809,22 @@ __device__ __forceinline__ bool tile_softmax(const ChunkParams& p, const TileUni
             const float me = m == -INFINITY ? 0.f : m;
             // hidden tokens (weight 0) and their value scales, which are finite here, leave no trace
             uint32_t hi[16], rest[TERMS == 2 ? 3 : 1][16];
-#pragma unroll
+            // (one copy of this rare path where it can be: unrolled, its registers cost the path above 500 us of 4,790)
+#pragma unroll (TERMS == 2 ? 4 : 1)
             for (int q = 0; q < 4; ++q) {
                 uint32_t* lo = TERMS == 2 ? rest[q < 3 ? q : 2] : nullptr;
                 if (TERMS == 2 && q == 3) {  // the columns that these terms go to have been read by now
                     tmem_st16(col_s + 64u, rest[0]);
                     tmem_st16(col_s + 80u, rest[1]);
                     uint32_t last[16];
-                    if (masked) weights32<true, FOLD>(col_s + 96u, ks4 + 24, vs4 + 24, lim - 96, rf, me, lp, hi, last);
-                    else weights32<false, FOLD>(col_s + 96u, ks4 + 24, vs4 + 24, 0, rf, me, lp, hi, last);
+                    if (masked) weights32<true, FOLD>(col_s + 96u, ks4 + 24, vs4 + 24, lim - 96, vf, vary, rf, me, lp, hi, last);
+                    else weights32<false, FOLD>(col_s + 96u, ks4 + 24, vs4 + 24, 0, 1.f, false, rf, me, lp, hi, last);
                     tmem_st16(col_s + 96u, rest[2]);
                     tmem_st16(col_s + 112u, last);
                 } else if (masked) {
-                    weights32<true, FOLD>(col_s + 32u * q, ks4 + 8 * q, vs4 + 8 * q, lim - 32 * q, rf, me, lp, hi, lo);
+                    weights32<true, FOLD>(col_s + 32u * q, ks4 + 8 * q, vs4 + 8 * q, lim - 32 * q, vf, vary, rf, me, lp, hi, lo);
                 } else {
-                    weights32<false, FOLD>(col_s + 32u * q, ks4 + 8 * q, vs4 + 8 * q, 0, rf, me, lp, hi, lo);
+                    weights32<false, FOLD>(col_s + 32u * q, ks4 + 8 * q, vs4 + 8 * q, 0, 1.f, false, rf, me, lp, hi, lo);
                 }
                 tmem_st16(col_s + 16u * q, hi);
             }

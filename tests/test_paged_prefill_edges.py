@@ -100,12 +100,13 @@ FEW = [(128, 4, 2), (128, 4, 10), (64, 1, 7), (64, 2, 21)]  # dims, heads a KV h
 def hidden_scales(D, G, n, dtype, value):
     """Whose last tokens' value scales are far above what the rows in front of them see. "steps": each new token's is
     four times the one before it, so every row has a largest of its own."""
-    s = make_case(1, [n], [203], 2, G, D, 16, dtype, seed=51)
+    ln = max(203, n + 33)
+    s = make_case(1, [n], [ln], 2, G, D, 16, dtype, seed=51)
     blk, off = tokens(s)
     if value == "steps":
         s["vs"] *= 1e-6
         for i in range(n):
-            s["vs"][blk[203 - n + i], :, off[203 - n + i]] *= 4.0 ** min(i + 1, 8 if dtype == "float16" else 40)
+            s["vs"][blk[ln - n + i], :, off[ln - n + i]] *= 4.0 ** min(i + 1, 8 if dtype == "float16" else 40)
     else:
         s["vs"][blk[-1], :, off[-1]] = value
     return s
@@ -138,4 +139,15 @@ def check_hidden_scales(D, G, n, dtype, value):
 @pytest.mark.parametrize("D,G,n", FEW)
 @pytest.mark.parametrize("value", ["steps", 1e10, 1e20, 1e36])
 def test_value_scales_of_hidden_tokens_with_few_rows(D, G, n, dtype, value):
+    check_hidden_scales(D, G, n, dtype, value)
+
+
+MANY = [(128, 4, 40), (128, 1, 300), (64, 1, 130), (64, 8, 70)]  # 130 to 560 rows a KV head
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("D,G,n", MANY)
+@pytest.mark.parametrize("value", ["steps", 1e10, 1e20, 1e36])
+def test_value_scales_of_hidden_tokens_with_many_rows(D, G, n, dtype, value):
     check_hidden_scales(D, G, n, dtype, value)
