@@ -345,10 +345,21 @@ bool has_class(const kvd_paged_prefill_desc& d, int cls) {
     return cls == 0 ? G <= tiny_most(d) : cls == 1 ? most > tiny_most(d) && G <= few_most(d) : most > few_most(d);
 }
 
+// Rows that requests of a class have at most in any call like this one with as many rows or fewer. Room for records goes
+// by this, not by has_class, so that scratch for a loop's largest step serves the smaller ones, which may be of other
+// classes: single tokens are tiny in a step by themselves (tiny_most), and 256 rows of a KV head few (few_most).
+int64_t class_rows(const kvd_paged_prefill_desc& d, int cls) {
+    const int64_t T = d.num_rows, B = d.batch, G = d.num_q_heads / d.num_kv_heads;
+    const int64_t alone = T < B ? T : B, few = (B < 8 ? 32 * B : 256) / G;
+    if (cls == 0) return G > 8 ? 0 : B * d.num_kv_heads >= 2LL * device_sm_count() ? T : alone;
+    if (cls == 1) return G <= 48 ? T : T < few ? T : few;
+    return has_class(d, kMany) ? T : 0;  // never in a call of fewer rows than one that has it not
+}
+
 int64_t round16(int64_t x) { return (x + 15) & ~static_cast<int64_t>(15); }
 
 // Lays the workspace out from `base` (nullptr: to learn its size, which is the same for all types of rows and
-// output); returns its bytes.
+// output and does not fall as rows are added); returns its bytes.
 int64_t lay_out(const kvd_paged_prefill_desc& d, ChunkParams* p, uint8_t* base, bool& split) {
     split = false;  // whether units of many rows may be
     const int sms = device_sm_count();
@@ -365,10 +376,10 @@ int64_t lay_out(const kvd_paged_prefill_desc& d, ChunkParams* p, uint8_t* base, 
     // no more units than rows give, and no more splits of each than the longest length gives
     auto records = [&](int cls, int64_t unit_rows) -> int64_t {
         const int64_t least = cls == kMany ? kTileMinSpan : kFewMinSpan;
-        const int64_t units = (d.num_rows * G / unit_rows + (d.batch < d.num_rows ? d.batch : d.num_rows)) * d.num_kv_heads;
+        const int64_t rows = class_rows(d, cls), units = (rows * G / unit_rows + (d.batch < rows ? d.batch : rows)) * d.num_kv_heads;
         const int64_t splits = (cap + least - 1) / least, most = units * splits;
         const int64_t ctas = cls == kMany ? sms : sms * chunk_few_ctas(d.head_dim, cls, true), room = 2 * span_quarters(cls, kSpans - 1) * ctas / 4;
-        return splits <= 1 || !has_class(d, cls) ? 0 : most < room ? most : room;
+        return splits <= 1 ? 0 : most < room ? most : room;
     };
     int64_t at = 0;
     auto take = [&](int64_t bytes) {

@@ -989,7 +989,8 @@ def _prefill_desc(q, k_pool, block_table, layout: str, causal: bool = True):
 
 
 def paged_prefill_workspace_size(q, k_pool, block_table, layout: str = "bhtd") -> int:
-    """Bytes of scratch :func:`paged_prefill` uses for these shapes."""
+    """Bytes of scratch :func:`paged_prefill` uses for these shapes. They do not fall as ``q`` gets rows, so scratch for a
+    loop's largest step serves the others."""
     return int(lib().kvd_paged_prefill_workspace_size(ctypes.byref(_prefill_desc(q, k_pool, block_table, layout))))
 
 

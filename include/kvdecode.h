@@ -376,8 +376,9 @@ cudaError_t kvd_sparse_decode_launch(const kvd_paged_desc* desc,
  * 16-byte boundaries and 16-byte multiples of strides run on tensor cores, any
  * other shape on CUDA cores (where the cache is read again for every row and
  * head). The workspace of kvd_paged_prefill_workspace_size bytes, on a 16-byte
- * boundary, needs no initialisation; concurrent calls need separate ones.
- * num_rows 0 does nothing. */
+ * boundary, needs no initialisation; concurrent calls need separate ones. The
+ * size is the same for all types and does not fall as num_rows grows, so the
+ * largest step's serves a loop. num_rows 0 does nothing. */
 typedef struct kvd_paged_prefill_desc {
     int32_t batch, num_q_heads, num_kv_heads, head_dim;
     int32_t num_rows;            /* rows of Q and out, >= 0 */

@@ -151,3 +151,47 @@ MANY = [(128, 4, 40), (128, 1, 300), (64, 1, 130), (64, 8, 70)]  # 130 to 560 ro
 @pytest.mark.parametrize("value", ["steps", 1e10, 1e20, 1e36])
 def test_value_scales_of_hidden_tokens_with_many_rows(D, G, n, dtype, value):
     check_hidden_scales(D, G, n, dtype, value)
+
+
+def sizes(rows, **kw):
+    L = kvd.lib()
+    return [int(L.kvd_paged_prefill_workspace_size(ctypes.byref(prefill_desc(num_rows=t, **kw)))) for t in rows]
+
+
+SHAPES = [(8, 8, 8, 257, 128), (128, 1, 8, 257, 128), (1, 2, 1, 600, 64), (300, 8, 4, 600, 128), (64, 16, 1, 94, 64),
+          (4, 2, 64, 300, 128), (2, 1, 100, 300, 64), (40, 1, 7, 3, 128)]
+
+
+def check_sizes(B, H, G, MB, D, flags):
+    # scratch for a loop's largest step serves every smaller one
+    rows = [*range(0, 700), *range(700, 70000, 331)]
+    got = sizes(rows, batch=B, num_q_heads=H * G, num_kv_heads=H, max_blocks_per_seq=MB, block_table_stride=MB, head_dim=D,
+                flags=flags)
+    assert got[0] > 0 and all(x <= y for x, y in zip(got, got[1:]))
+
+
+@pytest.mark.parametrize("B,H,G,MB,D", SHAPES)
+@pytest.mark.parametrize("flags", [0, kvd.KVD_FLAG_Q_BF16 | kvd.KVD_FLAG_OUT_BF16])
+def test_workspace_does_not_shrink_with_more_rows(B, H, G, MB, D, flags):
+    check_sizes(B, H, G, MB, D, flags)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("B,H,G,MB,D", SHAPES)
+def test_workspace_does_not_shrink_with_more_rows_on_the_gpu(B, H, G, MB, D):
+    check_sizes(B, H, G, MB, D, 0)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES)
+def test_one_workspace_serves_chunks_and_then_single_tokens(dtype):
+    import torch
+
+    chunk = make_case(8, [16, 1, 1, 1, 1, 1, 1, 1], [4000, 900, 17, 300, 1, 2222, 64, 4100], 8, 8, 128, 16, dtype, seed=63)
+    one = make_case(8, [1] * 8, [4001, 901, 18, 301, 2, 2223, 65, 4100], 8, 8, 128, 16, dtype, seed=64)
+    chunk["table"] = torch.nn.functional.pad(chunk["table"], (0, one["table"].shape[1] - chunk["table"].shape[1]))
+    size = kvd.paged_prefill_workspace_size(chunk["q"], chunk["K"], chunk["table"])
+    ws = torch.full((size,), 255, dtype=torch.uint8, device=DEV)
+    for s in (chunk, one, chunk):
+        close(prefill(s, workspace=ws), s, oracle(s))
+    assert kvd.device_status() == 0
