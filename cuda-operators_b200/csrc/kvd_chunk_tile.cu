@@ -697,6 +697,9 @@ __device__ __forceinline__ bool tile_softmax(const ChunkParams& p, const TileUni
                                              int nu, int& ns, int& no, int& nm_sync) {
     using S = TileSmem<D>;
     constexpr int ROWS = TERMS == 1 ? 256 : 128;
+    // Weights up to 2^8 times value scales below 2^7 fit fp16. Weights without the scales have the room of these, so the
+    // reference lies 2^7 below the largest score: small ones stay normal numbers for as long as the others do.
+    constexpr int kBelow = FOLD ? 7 : 0;
     const int w = threadIdx.x >> 7, r = threadIdx.x & 127, lane = r & 31;
     const uint32_t lanes = tmem + (static_cast<uint32_t>(r & ~31) << 16);
     const uint32_t col_s = lanes + w * 128u, col_o = lanes + kColO + w * 128u;
@@ -750,7 +753,7 @@ __device__ __forceinline__ bool tile_softmax(const ChunkParams& p, const TileUni
                 for (int q = 0; q < 4; ++q)
                     top = fmaxf(top, weights32<false, FOLD>(col_s + 32u * q, ks4 + 8 * q, vs4 + 8 * q, 0, 1.f, false, rf, m, sum,
                                                       *reinterpret_cast<uint32_t(*)[16]>(&pk[16 * q]), nullptr));
-                done = !__any_sync(0xffffffffu, top * rf > m + 8.f);
+                done = !__any_sync(0xffffffffu, top * rf > m + (8.f + kBelow));
                 if (done) {
                     lp[0] = __fadd2_rn(lp[0], sum[0]);
                     lp[1] = __fadd2_rn(lp[1], sum[1]);
@@ -772,7 +775,7 @@ __device__ __forceinline__ bool tile_softmax(const ChunkParams& p, const TileUni
                     if (4 * x + 2 < lim) seen = fmaxf(seen, fabsf(v.z));
                     if (4 * x + 3 < lim) seen = fmaxf(seen, fabsf(v.w));
                 }
-                ve_now = seen == 0.f ? ve : min(ve, fit_exponent(seen, 7));
+                ve_now = seen == 0.f ? ve : min(ve, fit_exponent(seen, 7 - kBelow));
             }
             const float vf = vary ? pow2i(ve_now) : 1.f;
             float top = -INFINITY;
@@ -787,10 +790,11 @@ __device__ __forceinline__ bool tile_softmax(const ChunkParams& p, const TileUni
             if (full)  // this warpgroup's products before this tile's scores are complete: O may change
                 put_aside<D>(p.aside + (blockIdx.x * 2 + w) * (D / 4) * 128 + r, reinterpret_cast<float4*>(smem + S::kMl) + w * 128 + r,
                              col_o, own_tile == p.aside_tiles, m, ve);
-            const bool move = top > m + (m == -INFINITY ? 0.f : 8.f);
+            const bool move = top > m + (m == -INFINITY ? 0.f : 8.f + kBelow);
+            const float to = top - kBelow;
             if (any && __any_sync(0xffffffffu, (move && m != -INFINITY) || ve_now != ve)) {
                 // this warpgroup's products before this tile's scores are complete: O may change
-                const float f = move && m != -INFINITY ? ex2_fast(m - top) : 1.f;
+                const float f = move && m != -INFINITY ? ex2_fast(m - to) : 1.f;
                 const float fo = f * (ve - ve_now > 126 ? 0.f : pow2i(ve_now - ve));
 #pragma unroll 1
                 for (int d = 0; d < D; d += 32) {
@@ -805,7 +809,7 @@ __device__ __forceinline__ bool tile_softmax(const ChunkParams& p, const TileUni
                 lp[1] = __fmul2_rn(lp[1], make_float2(f, f));
             }
             ve = ve_now;
-            if (move) m = top;
+            if (move) m = to;
             const float me = m == -INFINITY ? 0.f : m;
             // hidden tokens (weight 0) and their value scales, which are finite here, leave no trace
             uint32_t hi[16], rest[TERMS == 2 ? 3 : 1][16];

@@ -195,3 +195,34 @@ def test_one_workspace_serves_chunks_and_then_single_tokens(dtype):
     for s in (chunk, one, chunk):
         close(prefill(s, workspace=ws), s, oracle(s))
     assert kvd.device_status() == 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["bfloat16", "float16"])
+@pytest.mark.parametrize("n", [1, 32])
+def test_many_small_weights_beside_a_large_one(dtype, n):
+    # 2^20 tokens of weight 2^-25.5 beside one of weight 1, all values the same: the small weights are 2.2 percent of
+    # their sum, and the output is the value. As one fp16 term a weight is off by half a step (2^-11 of it) or, below the
+    # smallest normal fp16, by 2^-25 of a reference that is at least 2^6 of the large weight: 2^20 tokens x 2^-31, 2^-11.
+    # (The same for the scale of bf16's values and its product with the code, and half a step of the output.) Nearly all entries of the table name
+    # one block, so that the pool is small; a unit of work a CTA: rows of 32 tokens are not split.
+    import torch
+
+    H, bs, D, G = torch.cuda.get_device_properties(0).multi_processor_count, 128, 64, 8
+    MB = (1 << 20) // bs
+    K, V = (torch.zeros((2, H, bs, D), dtype=torch.int8, device=DEV) for _ in range(2))
+    V.fill_(64)
+    K[0, :, 0, 0] = 100
+    ks = torch.full((2, H, bs), 25.5 * np.log(2) / 100, device=DEV)  # 8 x 100 ks / sqrt(64) = 25.5 ln 2
+    vs = torch.full((2, H, bs), 0.01, device=DEV)
+    table = torch.ones((1, MB), dtype=torch.int32, device=DEV)
+    table[0, 0] = 0
+    q = torch.zeros((n, H * G, D), dtype=getattr(torch, dtype), device=DEV)
+    q[..., 0] = 8.0
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32, device=DEV)  # noqa: E731
+    got = kvd.paged_prefill(q, K, V, ks, vs, table, i32([1 << 20]), i32([0, n]), causal=False, out_dtype=q.dtype).double()
+    want = 64 * float(vs[0, 0, 0])
+    eps = torch.finfo(q.dtype).eps / 2
+    tol = 1e-4 + 2.0 ** -11 + (0.0 if dtype == "float32" else eps + 3 * 2.0 ** -11)
+    assert float((got / want - 1).abs().max()) <= tol
+    assert kvd.device_status() == 0
