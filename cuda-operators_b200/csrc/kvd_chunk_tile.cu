@@ -727,7 +727,9 @@ __device__ __forceinline__ bool tile_softmax(const ChunkParams& p, const TileUni
     const float rf = reinterpret_cast<const float*>(smem + S::kRf)[(nu & 1) * 256 + in_unit];
     const int sees = chunk_sees(p, u.R, min(i, u.R.n - 1));  // rows that are not there see what the last one does
     float m = -INFINITY;
+    // One term: sums of a thread's four tokens in turn (few tiles add to them one token at a time). Two: one sum.
     float2 lp[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+    float l = 0.f;
     int ve = 126;
     bool any = false;  // O holds sums of this unit
     for (int tile = u.alt ? w : 0; tile < u.nt; tile += u.alt ? 2 : 1) {
@@ -805,12 +807,19 @@ __device__ __forceinline__ bool tile_softmax(const ChunkParams& p, const TileUni
                     for (int x = 0; x < 32; ++x) o[x] = __float_as_uint(__uint_as_float(o[x]) * fo);
                     tmem_st32(col_o + d, o);
                 }
-                lp[0] = __fmul2_rn(lp[0], make_float2(f, f));
-                lp[1] = __fmul2_rn(lp[1], make_float2(f, f));
+                if constexpr (TERMS == 1) {
+                    lp[0] = __fmul2_rn(lp[0], make_float2(f, f));
+                    lp[1] = __fmul2_rn(lp[1], make_float2(f, f));
+                } else {
+                    l *= f;
+                }
             }
             ve = ve_now;
             if (move) m = to;
             const float me = m == -INFINITY ? 0.f : m;
+            // two terms: small weights of a tile are added to each other before they meet a sum that may be far larger
+            float2 two[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+            float2(&tp)[2] = TERMS == 1 ? lp : two;
             // hidden tokens (weight 0) and their value scales, which are finite here, leave no trace
             uint32_t hi[16], rest[TERMS == 2 ? 3 : 1][16];
             // (one copy of this rare path where it can be: unrolled, its registers cost the path above 500 us of 4,790)
@@ -821,24 +830,25 @@ __device__ __forceinline__ bool tile_softmax(const ChunkParams& p, const TileUni
                     tmem_st16(col_s + 64u, rest[0]);
                     tmem_st16(col_s + 80u, rest[1]);
                     uint32_t last[16];
-                    if (masked) weights32<true, FOLD>(col_s + 96u, ks4 + 24, vs4 + 24, lim - 96, vf, vary, rf, me, lp, hi, last);
-                    else weights32<false, FOLD>(col_s + 96u, ks4 + 24, vs4 + 24, 0, 1.f, false, rf, me, lp, hi, last);
+                    if (masked) weights32<true, FOLD>(col_s + 96u, ks4 + 24, vs4 + 24, lim - 96, vf, vary, rf, me, tp, hi, last);
+                    else weights32<false, FOLD>(col_s + 96u, ks4 + 24, vs4 + 24, 0, 1.f, false, rf, me, tp, hi, last);
                     tmem_st16(col_s + 96u, rest[2]);
                     tmem_st16(col_s + 112u, last);
                 } else if (masked) {
-                    weights32<true, FOLD>(col_s + 32u * q, ks4 + 8 * q, vs4 + 8 * q, lim - 32 * q, vf, vary, rf, me, lp, hi, lo);
+                    weights32<true, FOLD>(col_s + 32u * q, ks4 + 8 * q, vs4 + 8 * q, lim - 32 * q, vf, vary, rf, me, tp, hi, lo);
                 } else {
-                    weights32<false, FOLD>(col_s + 32u * q, ks4 + 8 * q, vs4 + 8 * q, 0, 1.f, false, rf, me, lp, hi, lo);
+                    weights32<false, FOLD>(col_s + 32u * q, ks4 + 8 * q, vs4 + 8 * q, 0, 1.f, false, rf, me, tp, hi, lo);
                 }
                 tmem_st16(col_s + 16u * q, hi);
             }
+            if (TERMS == 2) l += (tp[0].x + tp[0].y) + (tp[1].x + tp[1].y);
         }
         any = true;
         if (meta[st].odd[0] | meta[st].odd[1] | meta[st].odd[2] | meta[st].odd[3]) {
 #pragma unroll
             for (int x = 0; x < kTile / 32; ++x) {
                 const int n = lim - 32 * x;
-                if (meta[st].odd[x] & (n >= 32 ? 0xffffffffu : n <= 0 ? 0u : (1u << n) - 1u)) lp[0].x = NAN;
+                if (meta[st].odd[x] & (n >= 32 ? 0xffffffffu : n <= 0 ? 0u : (1u << n) - 1u)) (TERMS == 1 ? lp[0].x : l) = NAN;
             }
         }
         tmem_wait_st();
@@ -877,7 +887,7 @@ __device__ __forceinline__ bool tile_softmax(const ChunkParams& p, const TileUni
         }
         tmem_wait_st();
     }
-    float l = (lp[0].x + lp[0].y) + (lp[1].x + lp[1].y);
+    if (TERMS == 1) l = (lp[0].x + lp[0].y) + (lp[1].x + lp[1].y);
     float back = pow2i(-ve), other_back = 0.f;
     int d0 = 0, d1 = D;
     if (u.alt) {  // the two warpgroups' sums, half of the dims each

@@ -198,7 +198,7 @@ def test_one_workspace_serves_chunks_and_then_single_tokens(dtype):
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("dtype", ["bfloat16", "float16"])
+@pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("n", [1, 32])
 def test_many_small_weights_beside_a_large_one(dtype, n):
     # 2^20 tokens of weight 2^-25.5 beside one of weight 1, all values the same: the small weights are 2.2 percent of
