@@ -71,7 +71,7 @@ __global__ void __launch_bounds__(kAnyThreads) chunk_any_kernel(const ChunkParam
         const float alpha = m == -INFINITY ? 0.f : exp2f(m - top);
         if (tid < c) {  // into arrays of their own: other threads may still read the scores
             const float e = exp2f(score[tid] - top);
-            prob[tid] = e;
+            prob[tid] = fabsf(vscl[tid]) < INFINITY ? e : NAN;
             weight[tid] = e * vscl[tid];
         }
         __syncthreads();

@@ -33,6 +33,7 @@ namespace {
 
 constexpr int kFewWarps = 4;
 constexpr int kStep = kFewStep;
+constexpr int kInfBits = 0x7f800000;
 __device__ __forceinline__ void mma_16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
     asm volatile(
         "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
@@ -310,17 +311,24 @@ __global__ void __launch_bounds__(kFewWarps * 32, FewSmem<D, NR, NQ>::kCtas) chu
                             top[e][y] = fmaxf(top[e][y], v);
                         }
                 }
-            // largest value scale of the step (what is not finite has no say), and the exponents that it asks for: a row's
-            // are its own where rows see different tokens, so that no hidden one costs it bits
+            // largest value scale of the step, and the exponents that it asks for: a row's are its own where rows see
+            // different tokens, so that no hidden one costs it bits. A scale that is not finite has no say, but makes
+            // the sum of weights of the rows that see it NaN.
             float v_top = fabsf(scales[kStep + lane]);
-            if (!(v_top < INFINITY)) v_top = 0.f;
             int fit[NR][2];
             if (!masked) {
-                const int bits = __reduce_max_sync(0xffffffffu, __float_as_int(v_top));
+                int bits = __reduce_max_sync(0xffffffffu, __float_as_int(v_top));
+                if (bits >= kInfBits) {
+#pragma unroll
+                    for (int e = 0; e < NR; ++e) l[e][0] = l[e][1] = NAN;
+                    bits = __reduce_max_sync(0xffffffffu, v_top < INFINITY ? __float_as_int(v_top) : 0);
+                }
                 fit[0][0] = bits == 0 ? 126 : fit_exponent(__int_as_float(bits), 7);
 #pragma unroll
                 for (int e = 0; e < NR; ++e) fit[e][0] = fit[e][1] = fit[0][0];
             } else {
+                const unsigned odd = __ballot_sync(0xffffffffu, !(v_top < INFINITY));
+                if (!(v_top < INFINITY)) v_top = 0.f;
 #pragma unroll
                 for (int x = 1; x < 32; x <<= 1) {  // lane i: the largest of tokens 0 .. i
                     const float y = __shfl_up_sync(0xffffffffu, v_top, x);
@@ -333,6 +341,7 @@ __global__ void __launch_bounds__(kFewWarps * 32, FewSmem<D, NR, NQ>::kCtas) chu
                         const int lim = sees[e][y] - t0;
                         const float seen = __shfl_sync(0xffffffffu, v_top, min(max(lim, 1), 32) - 1);
                         fit[e][y] = lim <= 0 || seen == 0.f ? 126 : fit_exponent(seen, 7);
+                        if (odd & (lim >= 32 ? 0xffffffffu : lim <= 0 ? 0u : (1u << lim) - 1u)) l[e][y] = NAN;
                     }
             }
             bool move = false;

@@ -361,7 +361,8 @@ cudaError_t kvd_sparse_decode_launch(const kvd_paged_desc* desc,
  * [0, seq_lens[b] - n + i]. With causal == 0 every row attends to all
  * seq_lens[b] tokens (states of an encoder that the cache holds).
  *   out[t][h] = softmax_j((q . K[j]) * ks[j] * scale) . (V[j] * vs[j])
- * A row that sees no token is written as 0. Rows that belong to no request (in
+ * A row that sees no token is written as 0, one that sees a token whose value
+ * scale is not finite as NaN. Rows that belong to no request (in
  * front of row_starts[0], from row_starts[batch] on) are left as they are;
  * starts are clamped to [0, num_rows], lengths to the table. A block id
  * outside the pool counts as in kvd_paged_decode_launch

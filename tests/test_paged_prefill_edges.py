@@ -226,3 +226,34 @@ def test_many_small_weights_beside_a_large_one(dtype, n):
     tol = 1e-4 + 2.0 ** -11 + (0.0 if dtype == "float32" else eps + 3 * 2.0 ** -11)
     assert float((got / want - 1).abs().max()) <= tol
     assert kvd.device_status() == 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("D,G,n", [(128, 4, 1), (128, 4, 10), (64, 1, 7), (128, 4, 40), (64, 1, 300), (96, 2, 6)])
+@pytest.mark.parametrize("value", [float("inf"), float("-inf"), float("nan")])
+def test_value_scales_that_are_not_finite(D, G, n, dtype, value):
+    # a row that sees such a token is NaN in every dim, also where its code is 0 or the weight vanishes; others are as ever
+    import torch
+
+    for small in (False, True):
+        s = make_case(2, [n, 3], [703, 90], 2, G, D, 16, dtype, seed=61)
+        want = oracle(s)
+        blk, off = tokens(s)
+        at = 703 - n // 2 - 1  # the rows from n - 1 - n // 2 on see it
+        s["vs"][blk[at], 1, off[at]] = value
+        s["V"][blk[at], 1, off[at], :9] = 0
+        if small:
+            s["ks"][blk[at], 1, off[at]] = 0.0  # score 0, where other tokens of its rows have hundreds
+            s["q"] *= 40.0
+            want = None
+        got = prefill(s)
+        assert torch.isnan(got[n - 1 - n // 2: n, G:]).all()
+        rest = got.clone()
+        rest[n - 1 - n // 2: n, G:] = 0.0
+        assert torch.isfinite(rest).all()
+        if want is not None:
+            out = want[0].clone()
+            out[n - 1 - n // 2: n, G:] = 0.0
+            close(rest, s, (out, *want[1:]))
+    assert kvd.device_status() == 0
