@@ -388,7 +388,7 @@ __device__ __forceinline__ void load_queries(const ChunkParams& p, const TileUni
         const bool whole = TERMS == 2 && (p.flags & (KVD_FLAG_Q_BF16 | KVD_FLAG_Q_F16)) == 0;
         const int k = fit_exponent(top, whole ? 11 : 15);
         const float f = pow2i(k);
-        if (c16 == 0) rf[r] = p.qscale * pow2i(-k);
+        if (c16 == 0) rf[r] = fmaxf(p.qscale * pow2i(-k), 0x1p-126f);  // never 0, which would make -inf times it NaN
         uint32_t hi[8], lo[8];
 #pragma unroll
         for (int d = 0; d < 8; ++d) {

@@ -9,7 +9,7 @@ import numpy as np
 import pytest
 
 import kvdecode as kvd
-from test_paged_prefill import DEV, TYPES, close, make_case, oracle, prefill, prefill_desc
+from test_paged_prefill import DEV, TYPES, check, close, make_case, oracle, prefill, prefill_desc
 
 CSRC = Path(__file__).resolve().parents[1] / "cuda-operators_b200" / "csrc"
 
@@ -257,3 +257,13 @@ def test_value_scales_that_are_not_finite(D, G, n, dtype, value):
             out[n - 1 - n // 2: n, G:] = 0.0
             close(rest, s, (out, *want[1:]))
     assert kvd.device_status() == 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+@pytest.mark.parametrize("n", [2, 20, 200])
+def test_rows_and_scales_near_the_smallest_number(dtype, n):
+    # query rows of 1e-34 with a softmax scale of 1e-9: all scores vanish, and the weights of what a row sees are equal
+    s = make_case(1, [n], [n + 150], 2, 2, 128, 16, dtype, seed=62)
+    s["q"] *= 1e-34
+    check(s, scale=1e-9)
