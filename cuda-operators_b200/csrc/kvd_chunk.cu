@@ -5,7 +5,10 @@
 // fp32 with no KV cache). With s_j = (q . K_j) ks_j scale over the tokens that a
 // row sees, out = sum_j 2^(s_j - m) vs_j V_j / sum_j 2^(s_j - m) in base 2 (the
 // scale holds log2(e)), m the running maximum: one pass over the tokens.
+#include <atomic>
+#include <chrono>
 #include <cmath>
+#include <random>
 
 #include "kvd_chunk.cuh"
 #include "kvd_decode.cuh"
@@ -271,6 +274,8 @@ __global__ void __launch_bounds__(1024) chunk_plan_kernel(const ChunkParams p) {
         }
         *p.head = h;
     }
+    __syncthreads();  // all of the plan, then the stamp
+    if (tid == 0) asm volatile("st.release.gpu.global.u64 [%0], %1;" ::"l"(&p.head->ready), "l"(p.stamp) : "memory");
 }
 
 // ------------------------------------------------------------- split work
@@ -407,6 +412,21 @@ int64_t lay_out(const kvd_paged_prefill_desc& d, ChunkParams* p, uint8_t* base, 
     return at;
 }
 
+// A number that no other call has. Scratch may hold anything, so the numbers start where chance says.
+uint64_t next_stamp() {
+    static std::atomic<uint64_t> stamp{[]() -> uint64_t {
+        try {
+            std::random_device chance;
+            return static_cast<uint64_t>(chance()) << 32 | chance();
+        } catch (...) {  // no source of chance: the time
+            return static_cast<uint64_t>(std::chrono::system_clock::now().time_since_epoch().count()) * 0x9e3779b97f4a7c15ull;
+        }
+    }()};
+    uint64_t s = 0;
+    while (s == 0) s = stamp.fetch_add(1, std::memory_order_relaxed);  // 0: none
+    return s;
+}
+
 cudaError_t check_chunk(const kvd_paged_prefill_desc* d) {
     if (!d || d->batch < 1 || d->num_q_heads < 1 || d->num_kv_heads < 1 || d->head_dim < 1 || d->head_dim > kAnyMaxD ||
         d->num_q_heads % d->num_kv_heads != 0 || d->num_rows < 0 || d->block_size < 1 || d->num_blocks < 1 ||
@@ -473,13 +493,16 @@ extern "C" cudaError_t kvd_paged_prefill_launch(const kvd_paged_prefill_desc* d,
     }
     bool split;
     lay_out(*d, &p, static_cast<uint8_t*>(workspace), split);
+    p.stamp = next_stamp();
     e = launch_after(chunk_plan_kernel, 1, p.B <= 256 ? 256 : 1024, 0, stream, p);
     if (e != cudaSuccess) return e;
     ++*launches;
     for (int c = 0; c < kClasses; ++c) {
         if (!has_class(*d, c)) continue;
+        p.last = c == kMany || !(has_class(*d, kMany) || (c == 0 && has_class(*d, 1)));
         e = c == kMany ? launch_chunk_tile(p, stream, launches) : launch_chunk_few(p, c, stream, launches);
         if (e != cudaSuccess) return e;
+        p.follows = 1;
     }
     if (!split) return cudaSuccess;
     const unsigned grid = 8u * device_sm_count();

@@ -16,12 +16,15 @@ constexpr int kMany = 2;
 
 // Work of a call, in the workspace: this, then for each class two arrays of B + 1 entries.
 struct ChunkHead {
+    uint64_t ready;           // the call's stamp once the plan is there
     int32_t units[kClasses];  // units: blocks of rows x KV heads x stretches of tokens
     int32_t span[kClasses];   // tokens of a stretch at most
     int32_t recs[kClasses];   // records of units whose tokens are split
     int32_t ticket;           // units of many rows that have been taken
-    int32_t pad[2];
+    int32_t ended;            // CTAs of the last class's kernel that have ended
+    int32_t pad[3];
 };
+static_assert(sizeof(ChunkHead) % 16 == 0, "alignment");
 
 struct ChunkParams {
     const void* Q;
@@ -52,6 +55,9 @@ struct ChunkParams {
     int max_recs[kClasses];     // room for records
     float4* aside;              // [CTA][2][D / 4][128] sums that the kernel for many rows puts aside
     int aside_tiles;            // after how many tiles
+    uint64_t stamp;             // of the call: no other has it
+    int follows;                // the kernel before this one reads the same plan
+    int last;                   // no kernel of a class comes after this one
     int tiny_most, few_most;    // rows up to which a request is of the first class, of the second
 };
 
@@ -66,6 +72,34 @@ constexpr int kTile = 128;       // tokens of a tile of the kernel for many rows
 // rounding, and starts again from zero after this many of its tiles, 64 products of a 32-bit output (1.5e-6 then),
 // 512 of a 16-bit one. Powers of two.
 constexpr int kAsideTiles = 4, kAsideTiles16 = 64;
+
+// The kernels of the classes write nothing that the others read, so one need not wait until the one before it ends: it
+// takes the SMs that the other leaves. What puts its reads behind the plan, and with it behind all that the plan has
+// waited for, is the stamp that the plan releases and this acquires. A kernel that does not find the stamp waits for
+// the one before it. No stamp is left over from a call before: calls have stamps of their own, and a captured one, which
+// keeps its stamp, takes it back when its last class ends. Every kernel ends after the one before it, so whoever
+// waits for the last waits for all.
+__device__ __forceinline__ void class_begins(const ChunkParams& p) {
+    if (p.follows) {
+        __shared__ int s_ready;
+        if (threadIdx.x == 0) {
+            unsigned long long stamp;
+            asm volatile("ld.acquire.gpu.global.u64 %0, [%1];" : "=l"(stamp) : "l"(&p.head->ready) : "memory");
+            s_ready = stamp == p.stamp;
+        }
+        __syncthreads();
+        if (!s_ready) grid_dependency_wait();
+    } else {
+        grid_dependency_wait();
+    }
+    allow_dependents();
+}
+__device__ __forceinline__ void class_ends(const ChunkParams& p) {
+    if (!p.follows) return;
+    grid_dependency_wait();
+    // (the last kernel's CTAs have all seen the stamp when each has counted itself, and earlier kernels have ended)
+    if (p.last && threadIdx.x == 0 && atomicAdd(&p.head->ended, 1) == static_cast<int>(gridDim.x) - 1) p.head->ready = 0;
+}
 
 // Rows [t0, t0 + n) of request b and its tokens.
 struct ChunkRows {

@@ -95,8 +95,7 @@ __global__ void __launch_bounds__(kFewWarps * 32, FewSmem<D, NR, NQ>::kCtas) chu
     constexpr int ROWS = S::kRows, STAGES = S::kStages;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, quad = lane >> 2, c = lane & 3;
     uint8_t* ring = few_smem + warp * STAGES * S::kStage;
-    grid_dependency_wait();
-    allow_dependents();
+    class_begins(p);
     const int units = p.head->units[CLS], span = p.head->span[CLS];
     for (int unit = blockIdx.x; unit < units; unit += gridDim.x) {
         const int b = warp_find(p.first[CLS], p.B, unit);
@@ -502,6 +501,7 @@ __global__ void __launch_bounds__(kFewWarps * 32, FewSmem<D, NR, NQ>::kCtas) chu
                                                    warp * (ROWS / kFewWarps), rows, lane);
         }
     }
+    class_ends(p);
 }
 
 template <int D, int NR, int NQ, int NP>

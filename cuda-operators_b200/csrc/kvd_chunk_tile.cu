@@ -1013,8 +1013,7 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_tile_kernel(const __grid_co
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(smem + S::kTmem);
-    grid_dependency_wait();
-    allow_dependents();
+    class_begins(p);
     const int units = p.head->units[kMany];
     if (warp < 8) {
         regs_more<kSoftmaxRegs>();
@@ -1076,6 +1075,7 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_tile_kernel(const __grid_co
             }
         }
     }
+    class_ends(p);
 }
 
 template <int D, int TERMS, bool FOLD>

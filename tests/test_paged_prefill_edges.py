@@ -53,13 +53,22 @@ def test_references_that_move_where_sums_are_put_aside(dtype, n, every, what, ti
 
 def test_kernels_wait_for_the_one_before_them():
     # Every kernel that is launched with the programmatic attribute waits for its predecessor, whatever its arguments
-    # say, before it lets the next one begin and before it looks at memory that others write.
+    # say, before it lets the next one begin and before it looks at memory that others write; or, where a class of
+    # requests follows another, it acquires the stamp that the plan released, and waits where it does not find it.
+    begins = (CSRC / "kvd_chunk.cuh").read_text().split("void class_begins")[1].split("\n}\n")[0]
+    at = [begins.find(x) for x in ("ld.acquire.gpu.global.u64", "stamp == p.stamp", "__syncthreads();",
+                                   "if (!s_ready) grid_dependency_wait();", "} else {\n        grid_dependency_wait();", "\n    allow_dependents();")]
+    assert at[0] >= 0 and at == sorted(at)
+    assert "st.release.gpu.global.u64" in (CSRC / "kvd_chunk.cu").read_text()
     found = 0
     for name in ("kvd_chunk.cu", "kvd_chunk_few.cu", "kvd_chunk_tile.cu", "kvd_pages.cu"):
         source = (CSRC / name).read_text()
         for part in source.split("__global__")[1:]:
             body = part[part.index("{\n"): part.index("\n}\n")]
             wait, allow = body.find("\n    grid_dependency_wait();"), body.find("\n    allow_dependents();")
+            if wait < 0:
+                wait, allow = body.find("\n    class_begins(p);"), len(body)
+                assert body.endswith("\n    class_ends(p);")
             assert 0 <= wait < allow, (name, part[:100])
             assert not re.search(r"\bp\.(head|first|rec|starts|seq_lens|table|lens|parents|Q|K|V|ks|vs|bits_a|free_in)\b", body[:wait])
             found += 1
@@ -70,7 +79,8 @@ def test_kernels_wait_for_the_one_before_them():
 @pytest.mark.parametrize("dtype", TYPES)
 def test_plans_of_calls_that_follow_each_other(dtype):
     # Requests of every class in each call, two calls in turn with other lengths and rows, in one graph with one
-    # workspace: a kernel that read the plan of the call before would take other units.
+    # workspace, and replays with other lengths: a kernel that read the plan of a call before would take other units.
+    # What says that a plan is there is gone when the call has ended.
     import torch
 
     n = [[1, 8, 30, 1, 120, 2, 50, 1] * 4, [50, 1, 1, 9, 2, 140, 1, 20] * 4]
@@ -91,6 +101,14 @@ def test_plans_of_calls_that_follow_each_other(dtype):
         graph.replay()
         for s, o, w in zip(cases, outs, wants):
             close(o, s, w)
+        assert int(ws[:8].view(torch.int64)) == 0
+        for s in cases:
+            s["lens"].sub_(17)
+            s["len"] = s["len"] - 17
+        wants = [oracle(s) for s in cases]
+    for s, w in zip(cases, wants):  # calls outside of graphs
+        close(prefill(s, workspace=ws), s, w)
+        assert int(ws[:8].view(torch.int64)) == 0
     assert kvd.device_status() == 0
 
 
