@@ -43,7 +43,8 @@ __device__ __forceinline__ void record_status(int32_t code) {
 // Montgomery (1994): mul = floor(2^(31+L) / d) + 1, L = ceil(log2 d).
 struct FastDiv {
     uint32_t mul, shift;
-    explicit FastDiv(uint32_t d = 1) {
+    FastDiv() : FastDiv(1) {}
+    explicit FastDiv(uint32_t d) {
         uint32_t L = 0;
         while ((1ull << L) < d) ++L;
         mul = static_cast<uint32_t>((1ull << (31 + L)) / d + 1);

@@ -58,7 +58,7 @@ struct PagesParams {
     uint32_t* bits_a;  // fork: blocks of rows that go on; compact: blocks in use
     uint32_t* bits_b;  // fork: blocks of rows that end; compact: free blocks
     int64_t words;
-    FastDiv by_bs, by_chunks;
+    FastDiv by_bs;
     // fork
     const int32_t* parents;
     int32_t* lens_out;
