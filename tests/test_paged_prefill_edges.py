@@ -285,3 +285,49 @@ def test_rows_and_scales_near_the_smallest_number(dtype, n):
     s = make_case(1, [n], [n + 150], 2, 2, 128, 16, dtype, seed=62)
     s["q"] *= 1e-34
     check(s, scale=1e-9)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("D,layout", [(257, "bhtd"), (384, "bthd"), (511, "bhtd"), (512, "bhtd")])
+def test_wide_heads(dtype, D, layout):
+    # more dims than the CUDA-core kernel has threads, three and four times
+    check(make_case(3, [1, 9, 5], [70, 9, 130], 2, 2, D, 16, dtype, layout, seed=71, extra=2), causal=True)
+    check(make_case(2, [3, 1], [2, 200], 1, 3, D, 7, dtype, layout, seed=72), causal=False)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("D,G,n", [(128, 4, 2), (128, 4, 11), (64, 1, 300), (128, 8, 70), (96, 1, 5)])
+def test_codes_of_minus_128(dtype, D, G, n):
+    # the lowest code, which the quantiser does not make and the layout allows
+    s = make_case(2, [n, 1], [n + 290, 40], 2, G, D, 16, dtype, seed=73)
+    for x in ("K", "V"):
+        s[x][:, :, ::3] = -128
+        s[x][..., 5] = -128
+    check(s)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES)
+def test_more_requests_than_the_plan_keeps(dtype):
+    # over 1,024 requests the plan looks lengths up again instead of keeping them; some have no rows, some no tokens
+    rng = np.random.default_rng(74)
+    n = rng.integers(0, 4, size=2500)
+    n[::500] = 90
+    lens = np.maximum(0, n + rng.integers(-2, 60, size=2500))
+    lens[7] = 9000
+    check(make_case(2500, n, lens, 1, 2, 64, 16, dtype, seed=74))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES)
+def test_what_a_request_gets_beside_others(dtype):
+    # The plan splits tokens by the work of the whole call, so a row's bits depend on the other requests; its value does not.
+    s = make_case(6, [40, 1, 300, 2, 9, 64], [4000, 9000, 1300, 64, 700, 64], 2, 4, 128, 16, dtype, seed=75)
+    want = oracle(s)
+    for b in range(6):
+        one = {**s, "n": s["n"][b:b + 1], "len": s["len"][b:b + 1], "starts_host": s["starts_host"][b:b + 2],
+               "table": s["table"][b:b + 1], "lens": s["lens"][b:b + 1], "starts": s["starts"][b:b + 2].contiguous()}
+        close(prefill(one), one, want)
+    assert kvd.device_status() == 0
