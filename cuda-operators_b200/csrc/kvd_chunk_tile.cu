@@ -383,8 +383,8 @@ __device__ __forceinline__ void load_queries(const ChunkParams& p, const TileUni
         for (int d = 0; d < 16; ++d) top = fmaxf(top, fabsf(x[d]));
 #pragma unroll
         for (int o = 1; o < PER; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-        // Two terms (32-bit rows): whole numbers below 2^11, whose products with the codes add up without loss, and what
-        // is left. (A product's sum is cut off, not rounded, behind every step, by a unit of its size.)
+        // Two terms (32-bit rows): whole numbers up to 2^11 and what is left. A product's sum is cut off, not rounded,
+        // behind every step, by a unit of its size, which whole numbers alone would not feel below 2^24.
         const bool whole = TERMS == 2 && (p.flags & (KVD_FLAG_Q_BF16 | KVD_FLAG_Q_F16)) == 0;
         const int k = fit_exponent(top, whole ? 11 : 15);
         const float f = pow2i(k);
@@ -480,7 +480,8 @@ __device__ __forceinline__ bool tile_mma(const TileUnit& u, uint8_t* smem, uint3
         if ((u.alt || w == 0) && !mbar_wait_all(&bars[kKFull + st], (j >> 1) & 1)) return false;
         tc_fence_after();
         const uint64_t kd = smem_desc(smem_u32(smem + S::kK + st * S::kRows), 16u, 1024u, kLayoutSw128);
-        // the smaller term first
+        // The smaller term first: errors of 9.7e-7 against 3.3e-6 for scores of hundreds, of 6.0e-7 against 8.5e-7 for
+        // ordinary ones (128 dims; fp32 matrix products 2.9e-6 and 5.1e-7).
 #pragma unroll
         for (int t = TERMS - 1; t >= 0; --t) {
             if (t < nq) {
