@@ -1081,7 +1081,8 @@ def paged_fork(parents, seq_lens, block_table, free_blocks, free_count, k_pool, 
     last ones are copied into blocks from the free list, and blocks that no row names any more go back on it.
     Lengths, table and count are updated in place unless other tensors are given for them (as for all layers but
     the last where several share a table). Requests that may share blocks are ended here, not by
-    :func:`paged_plan`. ``workspace``: a zeroed uint8 tensor of :func:`paged_fork_workspace_size` bytes that a
+    :func:`paged_plan`. A length that is lowered by hand (refused drafts) stays inside a last block that no other row
+    names: blocks behind it are lost to the pool, and a shared one that it ends in would be written to. ``workspace``: a zeroed uint8 tensor of :func:`paged_fork_workspace_size` bytes that a
     caller keeps for pools of as many blocks (without one, one is made). Returns (block_table_out, seq_lens_out)."""
     torch, i8, i32, _, f32 = _torch or _types()
     device = seq_lens.get_device()

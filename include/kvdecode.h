@@ -417,9 +417,14 @@ cudaError_t kvd_paged_prefill_launch(const kvd_paged_prefill_desc* desc, const v
  * block_table and free_count. Table ids outside the pool are passed on and
  * never followed (KVD_STATUS_BAD_BLOCK). The table has to name every holder of a
  * block. kvd_paged_plan_launch gives back all blocks of a request that it ends,
- * so requests that may share blocks are ended here instead. Where the pools of
- * several layers share one table, each layer has a call, all but the last with
- * outputs of their own (kvd_paged_compact_launch: and with a copy of
+ * so requests that may share blocks are ended here instead. A caller who lowers
+ * a length (drafted tokens that are refused) stays inside a last block that no
+ * other row names. Entries behind the new length are not looked at: their blocks
+ * are lost to the pool unless the caller pushes those that no row names any more
+ * on the free list. A length that ends inside a block which other rows name too
+ * (a full one, shared) lets the next write change their tokens. Where the pools
+ * of several layers share one table, each layer has a call, all but the last
+ * with outputs of their own (kvd_paged_compact_launch: and with a copy of
  * free_count); they all copy the same blocks. The workspace of
  * kvd_paged_fork_workspace_size bytes, on a 4-byte boundary, is zeroed by the
  * caller once; calls leave its counters and bitmaps zeroed. It serves calls with
