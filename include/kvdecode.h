@@ -34,7 +34,9 @@
  * kvd_sparse_decode_launch, kvd_paged_prefill_launch, kvd_paged_fork_launch,
  * kvd_paged_compact_launch; the generic decode kernel aside): they are launched
  * with the attribute, wait before any global memory access, and let the next
- * kernel launch from then on. A caller's kernel that follows one of these calls
+ * kernel launch from then on. (In kvd_paged_prefill_launch a kernel behind the
+ * second may instead begin on what the first one, which has waited, released to
+ * it; it waits before it ends.) A caller's kernel that follows one of these calls
  * with the attribute must wait before it reads what the call writes (tables,
  * slots, lengths, codes, scales, bounds, rows, selections, output) and before it
  * overwrites what the call reads.
@@ -373,7 +375,10 @@ cudaError_t kvd_sparse_decode_launch(const kvd_paged_desc* desc,
  * scales (weights and, for bf16 outputs, value scales times codes) as one
  * 16-bit term of 11 bits where the output has 16 bits, else as two. Tensor cores
  * cut a sum off at every product that they add, so 32-bit outputs are summed in
- * parts of at most 64 products of 16 tokens. head_dim 64 and 128 with pools on
+ * parts of at most 64 products of 16 tokens. Equal calls give equal bits; tokens
+ * are split by the work of the whole call, so the last bits of a row may change
+ * with the other requests. A causal row does not depend on the codes and scales
+ * of tokens behind it. head_dim 64 and 128 with pools on
  * 16-byte boundaries and 16-byte multiples of strides run on tensor cores, any
  * other shape on CUDA cores (where the cache is read again for every row and
  * head). The workspace of kvd_paged_prefill_workspace_size bytes, on a 16-byte
