@@ -115,10 +115,9 @@ def test_plans_of_calls_that_follow_each_other(dtype):
 FEW = [(128, 4, 2), (128, 4, 10), (64, 1, 7), (64, 2, 21)]  # dims, heads a KV head, rows: 8 to 42 rows a KV head
 
 
-def hidden_scales(D, G, n, dtype, value):
+def hidden_scales(D, G, n, dtype, value, ln):
     """Whose last tokens' value scales are far above what the rows in front of them see. "steps": each new token's is
     four times the one before it, so every row has a largest of its own."""
-    ln = max(203, n + 33)
     s = make_case(1, [n], [ln], 2, G, D, 16, dtype, seed=51)
     blk, off = tokens(s)
     if value == "steps":
@@ -130,14 +129,14 @@ def hidden_scales(D, G, n, dtype, value):
     return s
 
 
-def check_hidden_scales(D, G, n, dtype, value):
+def check_hidden_scales(D, G, n, dtype, value, ln=None):
     # Causal rows: what a row gets does not depend on value scales of tokens behind it. A small weight is off by 2^-25 of
     # a reference that is at least 2^6 of the largest value scale that the row sees, times a code of at most 127: 2^-31
     # of 127 times that scale a token, in every dim, also where the code of the token with that scale is 0. So the
     # largest |v| of the tolerance is 127 times the largest scale in sight.
     import torch
 
-    s = hidden_scales(D, G, n, dtype, value)
+    s = hidden_scales(D, G, n, dtype, value, ln or max(203, n + 33))
     out, mean, _, size = oracle(s)
     blk, off = tokens(s)
     sees = 127.0 * s["vs"][blk, :, off].double().cummax(0).values[-n:].repeat_interleave(G, 1)
@@ -213,6 +212,15 @@ def test_one_workspace_serves_chunks_and_then_single_tokens(dtype):
     for s in (chunk, one, chunk):
         close(prefill(s, workspace=ws), s, oracle(s))
     assert kvd.device_status() == 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("D,G,n,ln", [(128, 4, 2, 9001), (128, 4, 40, 9001), (64, 1, 300, 20011), (128, 1, 1000, 3000)])
+@pytest.mark.parametrize("value", ["steps", 1e20])
+def test_value_scales_of_hidden_tokens_of_long_rows(D, G, n, ln, dtype, value):
+    # tokens in stretches, some of which no row sees as a whole
+    check_hidden_scales(D, G, n, dtype, value, ln)
 
 
 @pytest.mark.gpu
@@ -331,3 +339,13 @@ def test_what_a_request_gets_beside_others(dtype):
                "table": s["table"][b:b + 1], "lens": s["lens"][b:b + 1], "starts": s["starts"][b:b + 2].contiguous()}
         close(prefill(one), one, want)
     assert kvd.device_status() == 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("D,G,n", [(128, 4, 2), (128, 4, 80), (64, 1, 11), (64, 2, 200)])
+def test_value_scales_over_eight_powers_of_ten(dtype, D, G, n):
+    s = make_case(2, [n, n], [1500, 333], 1, G, D, 16, dtype, seed=76, v_spread=1e4)
+    check(s)
+    s["ks"].zero_()  # equal weights
+    check(s)
