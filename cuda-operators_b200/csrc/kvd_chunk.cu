@@ -328,9 +328,9 @@ bool tensor_shape(const kvd_paged_prefill_desc& d) {
 int64_t group_rows(const kvd_paged_prefill_desc& d) { return static_cast<int64_t>(d.num_rows) * (d.num_q_heads / d.num_kv_heads); }
 
 // Rows of a KV head up to which a request has few: 48. Units of 16 rows re-read and re-widen what a tile shares: 16
-// requests of 8,192 bf16 tokens x 8 KV heads, 128 dims, take 85, 133, 175 and 246 us with 16, 32, 48 and 64 rows each
-// by the kernel for few, 165, 172, 173 and 176 by the one for many (fp32 105, 170, 212, 287 and 215 to 227; 64 dims 61,
-// 89, 116, 157 and 145 to 153). A call whose requests have up to 32 rows on average and 256 in all takes them all for
+// requests of 4,096 to 8,192 bf16 tokens x 8 KV heads, 128 dims, take 89, 138, 181 and 252 us with 16, 32, 48 and 64
+// rows each by the kernel for few, 177, 187, 187 and 191 by the one for many (fp32 118, 186, 233, 311 and 229 to 244; 64
+// dims 63, 94, 121, 166 and 145 to 153). A call whose requests have up to 32 rows on average and 256 in all takes them all for
 // few, which saves two launches.
 int few_most(const kvd_paged_prefill_desc& d) {
     const int64_t rows = group_rows(d);

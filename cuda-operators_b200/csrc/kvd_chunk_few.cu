@@ -237,7 +237,12 @@ __global__ void __launch_bounds__(kFewWarps * 32, FewSmem<D, NR, NQ>::kCtas) chu
         }
         // the columns of this lane in the products: rows 2c and 2c + 1 of each group
         float rf[NR][2], m[NR][2], l[NR][2];
-        int sees[NR][2], ve[NR][2];  // value scales that the row has seen, times 2^ve, are below 2^7: weights up to 2^8 fit fp16
+        int sees[NR][2];
+        // Exponents of the four rows, a byte each, plus 127: value scales that a row has seen, times 2^ve, are below 2^7,
+        // so that weights up to 2^8 fit fp16. (Registers are short here: 16 requests of 16 rows take 89 us, 93 with a word
+        // for each and 96 with one exponent for all and a copy of the loop below for rows that differ; 86 with one alone.)
+        uint32_t ve4 = 253u * 0x01010101u;
+        auto scale_of = [&](int e, int y) { return __uint_as_float(__byte_perm(ve4, 0u, (2 * e + y) << 12 | 0x0444) >> 1); };
 #pragma unroll
         for (int e = 0; e < NR; ++e)
 #pragma unroll
@@ -248,7 +253,6 @@ __global__ void __launch_bounds__(kFewWarps * 32, FewSmem<D, NR, NQ>::kCtas) chu
                 sees[e][y] = min(end, chunk_sees(p, R, min(i, R.n - 1)));
                 m[e][y] = -INFINITY;
                 l[e][y] = 0.f;
-                ve[e][y] = 126;
             }
         // ---- the walk
         float o[NR][D / 16][4];
@@ -317,7 +321,7 @@ __global__ void __launch_bounds__(kFewWarps * 32, FewSmem<D, NR, NQ>::kCtas) chu
             // different tokens, so that no hidden one costs it bits. A scale that is not finite has no say, but makes
             // the sum of weights of the rows that see it NaN.
             float v_top = fabsf(scales[kStep + lane]);
-            int fit[NR][2];
+            uint32_t fit4 = 0u;
             if (!masked) {
                 int bits = __reduce_max_sync(0xffffffffu, __float_as_int(v_top));
                 if (bits >= kInfBits) {
@@ -325,9 +329,7 @@ __global__ void __launch_bounds__(kFewWarps * 32, FewSmem<D, NR, NQ>::kCtas) chu
                     for (int e = 0; e < NR; ++e) l[e][0] = l[e][1] = NAN;
                     bits = __reduce_max_sync(0xffffffffu, v_top < INFINITY ? __float_as_int(v_top) : 0);
                 }
-                fit[0][0] = bits == 0 ? 126 : fit_exponent(__int_as_float(bits), 7);
-#pragma unroll
-                for (int e = 0; e < NR; ++e) fit[e][0] = fit[e][1] = fit[0][0];
+                fit4 = (bits == 0 ? 253u : fit_exponent(__int_as_float(bits), 7) + 127u) * 0x01010101u;
             } else {
                 const unsigned odd = __ballot_sync(0xffffffffu, !(v_top < INFINITY));
                 if (!(v_top < INFINITY)) v_top = 0.f;
@@ -342,16 +344,17 @@ __global__ void __launch_bounds__(kFewWarps * 32, FewSmem<D, NR, NQ>::kCtas) chu
                     for (int y = 0; y < 2; ++y) {
                         const int lim = sees[e][y] - t0;
                         const float seen = __shfl_sync(0xffffffffu, v_top, min(max(lim, 1), 32) - 1);
-                        fit[e][y] = lim <= 0 || seen == 0.f ? 126 : fit_exponent(seen, 7);
+                        fit4 |= (lim <= 0 || seen == 0.f ? 253u : fit_exponent(seen, 7) + 127u) << (8 * (2 * e + y));
                         if (odd & (lim >= 32 ? 0xffffffffu : lim <= 0 ? 0u : (1u << lim) - 1u)) l[e][y] = NAN;
                     }
             }
-            bool move = false;
+            fit4 = __vminu4(fit4, ve4);
+            bool move = fit4 != ve4;
 #pragma unroll
             for (int e = 0; e < NR; ++e)
 #pragma unroll
                 for (int y = 0; y < 2; ++y)
-                    move |= fit[e][y] < ve[e][y] || top[e][y] > m[e][y] + (m[e][y] == -INFINITY ? 0.f : 8.f);
+                    move |= top[e][y] > m[e][y] + (m[e][y] == -INFINITY ? 0.f : 8.f);
             if (__any_sync(0xffffffffu, move)) {
 #pragma unroll
                 for (int e = 0; e < NR; ++e)
@@ -363,10 +366,9 @@ __global__ void __launch_bounds__(kFewWarps * 32, FewSmem<D, NR, NQ>::kCtas) chu
                         to = fmaxf(to, __shfl_xor_sync(0xffffffffu, to, 16));
                         const bool go = to > m[e][y] + (m[e][y] == -INFINITY ? 0.f : 8.f);
                         const float f = go ? (m[e][y] == -INFINITY ? 0.f : ex2_fast(m[e][y] - to)) : 1.f;
-                        const int fall = max(ve[e][y] - fit[e][y], 0);
+                        const int at = 8 * (2 * e + y), fall = static_cast<int>(ve4 >> at & 0xffu) - static_cast<int>(fit4 >> at & 0xffu);
                         const float fo = fall > 126 ? 0.f : f * pow2i(-fall);
                         if (go) m[e][y] = to;
-                        ve[e][y] -= fall;
                         l[e][y] *= f;
 #pragma unroll
                         for (int j = 0; j < D / 16; ++j) {
@@ -374,6 +376,7 @@ __global__ void __launch_bounds__(kFewWarps * 32, FewSmem<D, NR, NQ>::kCtas) chu
                             o[e][j][2 + y] *= fo;
                         }
                     }
+                ve4 = fit4;
             }
 #pragma unroll
             for (int mt = 0; mt < 2; ++mt) {
@@ -390,7 +393,7 @@ __global__ void __launch_bounds__(kFewWarps * 32, FewSmem<D, NR, NQ>::kCtas) chu
                             const float x = s[mt][e][2 * half + y];
                             const float pr = ex2_fast(x - (m[e][y] == -INFINITY ? 0.f : m[e][y]));
                             l[e][y] += pr;
-                            w[y] = pr * (vq * pow2i(ve[e][y]));
+                            w[y] = pr * (vq * scale_of(e, y));
                             if (masked && x == -INFINITY) w[y] = 0.f;  // a hidden token's scale may be anything
                         }
                         const uint32_t hi = pack_half(w[0], w[1]);
@@ -447,7 +450,7 @@ __global__ void __launch_bounds__(kFewWarps * 32, FewSmem<D, NR, NQ>::kCtas) chu
                 sum += __shfl_xor_sync(0xffffffffu, sum, 4);
                 sum += __shfl_xor_sync(0xffffffffu, sum, 8);
                 sum += __shfl_xor_sync(0xffffffffu, sum, 16);
-                const float back = pow2i(-ve[e][y]);
+                const float back = pow2i(127 - static_cast<int>(ve4 >> (8 * (2 * e + y)) & 0xffu));
                 float* row = merge + (warp * ROWS + 8 * e + 2 * c + y) * (D + 4);
 #pragma unroll
                 for (int j = 0; j < D / 16; ++j)
