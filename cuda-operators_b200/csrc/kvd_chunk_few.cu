@@ -19,11 +19,11 @@
 // fit beside each other.
 //
 // Bound: HBM where rows fill a unit, and behind it the widening of codes (64
-// single tokens of up to 8,192, 8 heads a KV head, 128 dims: DRAM 53 %, ALU 61 %;
-// 256 of them 648 us, 502 at the copy rate); short units by their chain of loads
-// (8 requests of 23 drafted tokens in all: 38 us, 8.4). 32-bit outputs: a product
-// cuts the sum that it adds to off, so each makes a sum of its own (98 us
-// instead of 89 for 16 fp32 rows of 8,192 tokens).
+// single tokens of up to 8,192, 8 heads a KV head, 128 dims: DRAM 52 %, ALU 61 %;
+// 256 of them 664 us, 502 at the copy rate); short units by their chain of loads
+// (8 requests of 23 drafted tokens in all: 44 us with the plan, 8.4). 32-bit outputs:
+// a product cuts the sum that it adds to off, so each makes a sum of its own (98 us
+// instead of 89 for 16 single fp32 tokens of up to 8,192 when it was tried, 93 now).
 #include "kvd_chunk.cuh"
 #include "kvd_decode.cuh"
 #include "kvd_tc.cuh"

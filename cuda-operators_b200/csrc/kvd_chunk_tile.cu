@@ -30,16 +30,21 @@
 //         looks its tiles' blocks up ahead: row offsets, scales.
 // Outputs in bf16 (FOLD) have the value scales in the values, one multiplication
 // where codes are widened instead of one for every row's weight: 4.33 ms instead
-// of 5.36 for 4,096 new tokens of 32,768 (64 heads, 8 KV heads, 128 dims); fp16
-// outputs keep 3 more bits than those products would have.
+// of 5.36 for 4,096 new tokens of 32,768 (64 heads, 8 KV heads, 128 dims) when it
+// was tried; fp16 outputs keep 3 more bits than those products would have. Tiles
+// in which hidden tokens have the largest value scales are without it: there
+// each row has an exponent of its own, from the tokens that it sees.
 //
-// Bound: the softmax's chain (scores out of tensor memory, scales, the largest,
-// exponentials, weights back): 3,700 of a step's 5,500 cycles a warpgroup, against
-// 1,024 of products; tensor pipe 40 %, exponentials' pipe 41 %. Measured: those
-// 4,096 tokens in 4.46 to 4.56 ms, 900 to 925 TFLOP/s; 512 of 8,192 in fp16
-// 233 us; 7,003 tokens of five fp32 prompts (32 heads) 583 us, 55 of them for
-// sums put aside. Tiles of 64 tokens with two score buffers took 8.0 ms, votes
-// per 32 columns 5.6, registers for a row's pieces over lanes 5.6.
+// Bound: latency. A step of 128 x 128 takes a warpgroup about 4,300 cycles, 2,600 to
+// 3,000 of them in the softmax's chain (scores out of tensor memory, scales, the
+// largest, exponentials, weights back; 3,900 where value scales multiply the
+// weights, 6,500 with two terms), against 1,024 of products. No pipe is full, tensor
+// 43 %, exponentials 43 %, issue slots 52 %: two softmax warps a scheduler do
+// not cover each other's waits. Measured: those 4,096 tokens in 4.2 to 4.3 ms, 970
+// TFLOP/s (4.7 in long runs, power cap); 512 of 8,192 in fp16 229 us; 7,003 tokens
+// of five fp32 prompts (32 heads) 571 to 600 us, about 55 of them for sums put
+// aside. When the 4,096 tokens took 5.4 ms: tiles of 64 tokens with two
+// score buffers 8.0, votes per 32 columns 5.6, a row's pieces over lanes 5.6.
 //
 // Every wait is bounded; on expiry the kernel records KVD_STATUS_WAIT_TIMEOUT
 // and unwinds.
